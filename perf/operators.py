@@ -272,8 +272,8 @@ def _wrap(x):
 
 
 def _paged_calls(s):
-    import gptc
     case, rt = s["case"], _rt()
+    import gptc
     cache = gptc.PagedCache(rt, 1, s["k"].shape[0], case["page"], case["KV"], case["D"],
                             gptc.F32 if case["dtype"] == "f32" else gptc.BF16,
                             k=[s["k"].data_ptr()], v=[s["v"].data_ptr()])
