@@ -1,0 +1,439 @@
+// Attention of a step's new tokens over keys and values in pages (include/paged.h).
+//
+// For query row (token i of its sequence, head h): with the sequence's keys and values j <= past + i,
+//   t_j = (q . k_j) log2(e)/sqrt(D),  y = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m),  m = max_j t_j,
+// in one pass over the keys with a running m, sum and weighted sum, rescaled when m grows.  The query heads
+// that share a kv head and the new tokens of a sequence are all rows of one product, 16 at a time, so a page is
+// read once for a whole group, and single tokens and prompts run the same way.
+//
+// A workgroup takes an item of the plan: up to 16 rows and a range of keys, which its four waves take in turns
+// of 16 (fp32 pages) or 32 (bf16) keys.  A wave's keys and values go from memory straight into the registers
+// that the matrix instructions read: nothing is shared between waves, so LDS would only add a trip.  All
+// products are transposed so that a lane holds one query (lane % 16):
+//   S^T (keys x rows) = K Q^T.  K is the A operand: lane (m, g) = (lane % 16, lane / 16) holds values of key m.
+//     The reduction may be taken in any order, so the lane reads 16 consecutive bytes of its key per load.
+//   The result leaves lane (n, g) with t of row n and keys 4g .. 4g+3: m and the sums of a row are the lane's
+//     own up to the four lanes n + 16 g, and p is, register for register, the B operand of the next product.
+//   O^T (D x rows) += V^T P^T.  V^T is the A operand with row m of tile c standing for value m DP/16 + c, so
+//     that lane m reads consecutive bytes of each value row (for bf16, where an operand register holds two
+//     keys, 16-bit halves of two rows are swapped into place).
+//
+// fp32 pages are multiplied by v_mfma_f32_16x16x4_f32.  bf16 pages by v_mfma_f32_16x16x32_bf16 with the query
+// and the weights as exact sums of three bf16 values (24 bits): three products at a sixteenth of the cost of an
+// fp32 one each.
+#include "attn_common.hpp"
+#include "hip_check.hpp"
+#include "paged_plan.hpp"
+
+namespace gptc {
+
+namespace {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+
+// What is known of the rows: D is the tile's width; every row starts at a multiple of 16 bytes and holds whole
+// vectors; or nothing.
+enum Rows { kFull, kVec, kAny };
+
+// N consecutive 32-bit words of T values from row + d; values at or past D are zeros (the load then takes the
+// row's first values instead, so that no branch parts the loads).
+template <typename T, int N, Rows R>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const T *row, int d, int D) {
+    if constexpr (R != kAny) {
+        static_assert(N == 2 || N == 4, "one vector load");
+        typedef uint32_t vec __attribute__((ext_vector_type(N)));
+        const bool in = R == kFull || d < D;
+        const vec x = *reinterpret_cast<const vec *>(row + (in ? d : 0));
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = in ? x[i] : 0;
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = d + i < D ? __builtin_bit_cast(uint32_t, row[d + i]) : 0u;
+    } else {
+        const uint16_t *r = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t lo = d + 2 * i < D ? r[d + 2 * i] : 0u, hi = d + 2 * i + 1 < D ? r[d + 2 * i + 1] : 0u;
+            w[i] = lo | hi << 16;
+        }
+    }
+}
+
+// x, y as sums of three bf16 values, packed in pairs.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const f32x2 v = {x, y};
+        p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+        x -= __builtin_bit_cast(float, p[i] << 16);
+        y -= __builtin_bit_cast(float, p[i] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma_bf16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
+    const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0,
+                                                   0);
+}
+
+// A matrix instruction's result may be read 11 cycles after it at the earliest.  The compiler counts them inside
+// a block; across a branch it was seen to read the last two registers at once (wrong sums at every second step of
+// bf16 pages).  So results are taken over in the block of the product, or after a wait of 16.
+__device__ __forceinline__ void settled(f32x4 &x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void finished(f32x4 &x) { asm volatile("s_nop 15" : "+a"(x)); }
+
+// A wave's operands: the query rows, and the keys and values of one turn.
+template <typename T, int DP, Rows R>
+struct Tile;
+
+template <int DP, Rows R>
+struct Tile<float, DP, R> {
+    static constexpr int kGroups = 1;  // of 16 keys
+    struct Q {
+        uint32_t w[DP / 16][4];  // d = 16c + 4g + e
+    };
+    uint32_t k[DP / 16][4], v[4][DP / 64][4];  // v[i][h][c]: key 4g + i, d = 64h + 4m + c
+
+    static __device__ __forceinline__ void load_q(Q &q, const float *row, int g, int D) {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            if (row != nullptr) {
+                load_words<float, 4, R>(q.w[c], row, 16 * c + 4 * g, D);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q.w[c][e] = 0;
+            }
+        }
+    }
+    // kp, vp: row 0 of each group of 16 keys.
+    __device__ __forceinline__ void load(const float *const (&kp)[1], const float *const (&vp)[1], int m, int g, int D) {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) load_words<float, 4, R>(k[c], kp[0] + m * D, 16 * c + 4 * g, D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h)
+                load_words<float, 4, R>(v[i][h], vp[0] + (4 * g + i) * D, 64 * h + 4 * m, D);
+    }
+    __device__ __forceinline__ void clear_values(int g, int left) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * g + i >= left)
+#pragma unroll
+                for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[i][h][c] = 0;
+    }
+    __device__ __forceinline__ void scores(const Q &q, f32x4 (&s)[1]) const {
+        s[0] = zero4();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                s[0] = mfma16(__builtin_bit_cast(float, k[c][e]), __builtin_bit_cast(float, q.w[c][e]), s[0]);
+    }
+    __device__ __forceinline__ void values(const f32x4 (&p)[1], f32x4 (&o)[DP / 16]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    o[4 * h + c] = mfma16(__builtin_bit_cast(float, v[i][h][c]), p[0][i], o[4 * h + c]);
+    }
+    // o[4 (j / 4) + c][r], c < 4, are d .. d+3 of this row.
+    static __device__ __forceinline__ int dim(int j, int g, int r) { return 16 * j + 16 * g + 4 * r; }
+};
+
+template <int DP, Rows R>
+struct Tile<__bf16, DP, R> {
+    static constexpr int kGroups = 2;
+    static constexpr int kWords = DP / 32;  // of a value row per lane
+    struct Q {
+        uint32_t w[3][DP / 32][4];  // d = 32c + 8g + 2e, + 1
+    };
+    uint32_t k[2][DP / 32][4], v[8][kWords];  // v[j]: key 4g + j of the first group, or 4g + j - 4 of the second
+
+    static __device__ __forceinline__ void load_q(Q &q, const float *row, int g, int D) {
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+            uint32_t x[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (row != nullptr) {
+                    load_words<float, 4, R>(x[h], row, 32 * c + 8 * g + 4 * h, D);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[h][e] = 0;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t p[3];
+                split3(__builtin_bit_cast(float, x[e / 2][2 * (e % 2)]), __builtin_bit_cast(float, x[e / 2][2 * (e % 2) + 1]), p);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) q.w[i][c][e] = p[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const __bf16 *const (&kp)[2], const __bf16 *const (&vp)[2], int m, int g, int D) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) load_words<__bf16, 4, R>(k[t][c], kp[t] + m * D, 32 * c + 8 * g, D);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            load_words<__bf16, kWords, R>(v[j], vp[j / 4] + (4 * g + j % 4) * D, 2 * kWords * m, D);
+    }
+    __device__ __forceinline__ void clear_values(int g, int left) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (16 * (j / 4) + 4 * g + j % 4 >= left)
+#pragma unroll
+                for (int c = 0; c < kWords; ++c) v[j][c] = 0;
+    }
+    __device__ __forceinline__ void scores(const Q &q, f32x4 (&s)[2]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = zero4();
+#pragma unroll
+            for (int i = 2; i >= 0; --i)  // the smallest parts first
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) s[t] = mfma_bf16(k[t][c], q.w[i][c], s[t]);
+        }
+    }
+    __device__ __forceinline__ void values(const f32x4 (&p)[2], f32x4 (&o)[DP / 16]) const {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t x[3];
+            split3(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], x);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) w[i][e] = x[i];
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            uint32_t a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                a[e] = __builtin_amdgcn_perm(v[2 * e + 1][c / 2], v[2 * e][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int i = 2; i >= 0; --i) o[c] = mfma_bf16(a, w[i], o[c]);
+        }
+    }
+    static __device__ __forceinline__ int dim(int j, int g, int r) { return DP / 4 * g + DP / 16 * r + j; }
+};
+
+template <typename T, int DP, Rows R>
+__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttnParams a) {
+    using Step = Tile<T, DP, R>;
+    constexpr int kKeys = 16 * Step::kGroups;
+    static_assert(kKeys * kWaves == paged_unit(sizeof(T) == 2 ? GPTC_BF16 : GPTC_F32), "the plan's rounds");
+    constexpr int kRow = DP + 4;  // floats of an LDS row: the four lanes of a row fall on other banks than its neighbours
+    __shared__ __attribute__((aligned(16))) float o_s[kWaves][kPagedRows][kRow];
+    __shared__ float m_s[kWaves][kPagedRows], l_s[kWaves][kPagedRows];
+
+    const int item = blockIdx.x / a.KV, kv = blockIdx.x - item * a.KV;
+    if (item >= a.head[1]) return;
+    const PagedItem it = a.items[item];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int total = it.past + it.rows / a.group;  // the sequence's tokens: slots past them hold anything
+
+    // The lane's query row, and the end of its keys.
+    const int row = it.row0 + n;
+    const int token = row / a.group;
+    const bool live = row < it.rows && it.tok0 + token < a.rows;
+    typename Step::Q q;
+    Step::load_q(q, live ? a.q + static_cast<int64_t>(it.tok0 + token) * a.q_stride + (kv * a.group + row - token * a.group) * a.D
+                         : nullptr, g, a.D);
+    const int end = it.past + token + 1;
+    const int first_end = it.past + it.row0 / a.group + 1;  // of the item's first row, which ends first
+
+    const T *kpool = static_cast<const T *>(a.k), *vpool = static_cast<const T *>(a.v);
+    const int *table = a.table + it.table;
+    const int mask = (1 << a.page_shift) - 1;
+    const int steps = (it.key1 - it.key0 - w * kKeys + kWaves * kKeys - 1) / (kWaves * kKeys);  // <= 0: none
+    int pages[Step::kGroups];  // lane i: the pages of the wave's step i, i + 64, ...
+    auto load_step = [&](Step &x, int i) {
+        if ((i & 63) == 0) {
+#pragma unroll
+            for (int t = 0; t < Step::kGroups; ++t) {
+                const int key = it.key0 + (w + kWaves * (i + lane)) * kKeys + 16 * t;
+                pages[t] = table[min(key, total - 1) >> a.page_shift];
+            }
+        }
+        const int key = it.key0 + (w + kWaves * i) * kKeys;
+        const T *kp[Step::kGroups], *vp[Step::kGroups];
+#pragma unroll
+        for (int t = 0; t < Step::kGroups; ++t) {
+            const int64_t page = __builtin_amdgcn_readlane(pages[t], i & 63);
+            const int64_t at = (((page * a.KV + kv) << a.page_shift) + ((key + 16 * t) & mask)) * a.D;
+            kp[t] = kpool + at;
+            vp[t] = vpool + at;
+        }
+        x.load(kp, vp, n, g, a.D);
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) o[c] = zero4();
+    auto step = [&](Step &x, int i) {
+        const int key = it.key0 + (w + kWaves * i) * kKeys;
+        if (key + kKeys > total) x.clear_values(g, total - key);
+        f32x4 s[Step::kGroups];
+        x.scores(q, s);
+#pragma unroll
+        for (int t = 0; t < Step::kGroups; ++t) settled(s[t]);
+#pragma unroll
+        for (int t = 0; t < Step::kGroups; ++t) s[t] *= a.scale_log2;
+        if (key + kKeys > first_end) {
+#pragma unroll
+            for (int t = 0; t < Step::kGroups; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (key + 16 * t + 4 * g + r >= end) s[t][r] = -INFINITY;
+        }
+        float mx = m;
+#pragma unroll
+        for (int t = 0; t < Step::kGroups; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
+        mx = max4_rows(mx);
+        const float base = mx == -INFINITY ? 0.0f : mx;  // no key of this row yet
+        if (__any(mx > m)) {
+            const float f = fast_exp2(m - base);
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) o[c] *= f;
+            m = mx;
+        }
+#pragma unroll
+        for (int t = 0; t < Step::kGroups; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[t][r] = fast_exp2(s[t][r] - base);
+                l += s[t][r];
+            }
+        x.values(s, o);
+    };
+    // Two steps in turn: the loads of one are in flight while the other is multiplied.
+    Step x, y;
+    if (steps > 0) load_step(x, 0);
+    for (int i = 0; i < steps; i += 2) {
+        if (i + 1 < steps) load_step(y, i + 1);
+        step(x, i);
+        if (i + 1 >= steps) break;
+        if (i + 2 < steps) load_step(x, i + 2);
+        step(y, i + 1);
+    }
+
+    // The waves' states joined: sums of o 2^(m_w - M).
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) finished(o[c]);
+    l = sum4_rows(l);
+    if (g == 0) {
+        m_s[w][n] = m;
+        l_s[w][n] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < DP / 16; j += 4)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<f32x4 *>(&o_s[w][n][Step::dim(j, g, r)]) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
+    __syncthreads();
+    const int r = tid >> 4;
+    float big = m_s[0][r];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) big = fmaxf(big, m_s[i][r]);
+    float f[kWaves], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        f[i] = m_s[i][r] == -INFINITY ? 0.0f : fast_exp2(m_s[i][r] - big);
+        sum = fmaf(l_s[i][r], f[i], sum);
+    }
+    const int out_row = it.row0 + r, out_token = it.tok0 + out_row / a.group;
+    if (out_row >= it.rows || out_token >= a.rows) return;
+    float *dst;
+    float scale = 1.0f;
+    if (it.part < 0) {
+        dst = a.out + (static_cast<int64_t>(out_token) * a.H + kv * a.group + out_row % a.group) * a.D;
+        scale = 1.0f / sum;
+    } else {
+        const int64_t slot = (static_cast<int64_t>(it.part) * a.KV + kv) * kPagedRows + r;
+        dst = a.part_o + slot * a.D;
+        if ((tid & 15) == 0) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * slot) = f32x2{big, sum};
+    }
+    for (int d = 4 * (tid & 15); d < a.D; d += 64) {
+        f32x4 y4 = zero4();
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) y4 += f[i] * *reinterpret_cast<const f32x4 *>(&o_s[i][r][d]);
+        store4<R != kAny>(dst, d, a.D, y4 * scale);
+    }
+}
+
+// Joins the parts of the rows whose keys were cut.
+template <bool VEC>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnParams a) {
+    const int i = blockIdx.x / a.KV, kv = blockIdx.x - i * a.KV;
+    if (i >= a.head[2]) return;
+    const PagedMerge mg = a.merges[i];
+    const int r = threadIdx.x >> 4, row = mg.row0 + r;
+    const int token = mg.tok0 + row / a.group;
+    if (row >= mg.rows || token >= a.rows) return;
+    const int64_t first = (static_cast<int64_t>(mg.part0) * a.KV + kv) * kPagedRows + r;
+    const int64_t next = static_cast<int64_t>(a.KV) * kPagedRows;
+    float big = -INFINITY;
+    for (int p = 0; p < mg.n; ++p) big = fmaxf(big, a.part_ml[2 * (first + p * next)]);
+    float *dst = a.out + (static_cast<int64_t>(token) * a.H + kv * a.group + row % a.group) * a.D;
+    for (int d = 4 * (threadIdx.x & 15); d < a.D; d += 64) {
+        f32x4 y = zero4();
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < mg.n; ++p) {
+            const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
+            const float f = ml[0] == -INFINITY ? 0.0f : fast_exp2(ml[0] - big);
+            sum = fmaf(ml[1], f, sum);
+            y += f * load4<VEC>(a.part_o + (first + p * next) * a.D, d, a.D);
+        }
+        store4<VEC>(dst, d, a.D, y / sum);
+    }
+}
+
+template <typename T, int DP>
+void launch(const PagedAttnParams &p, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(p.n_items) * p.KV);
+    if (p.vec && p.D == DP)
+        paged_attn_kernel<T, DP, kFull><<<grid, dim3(64 * kWaves), 0, s>>>(p);
+    else if (p.vec)
+        paged_attn_kernel<T, DP, kVec><<<grid, dim3(64 * kWaves), 0, s>>>(p);
+    else
+        paged_attn_kernel<T, DP, kAny><<<grid, dim3(64 * kWaves), 0, s>>>(p);
+    hipCheck(hipGetLastError());
+}
+
+}  // namespace
+
+void launch_paged_attention(const PagedAttnParams &p, hipStream_t s) {
+    if (p.bf16) {
+        if (p.D <= 64) launch<__bf16, 64>(p, s);
+        else launch<__bf16, 128>(p, s);
+    } else {
+        if (p.D <= 64) launch<float, 64>(p, s);
+        else launch<float, 128>(p, s);
+    }
+    if (p.n_merges == 0) return;
+    const dim3 grid(static_cast<unsigned>(p.n_merges) * p.KV);
+    if (p.vec) paged_merge_kernel<true><<<grid, dim3(256), 0, s>>>(p);
+    else paged_merge_kernel<false><<<grid, dim3(256), 0, s>>>(p);
+    hipCheck(hipGetLastError());
+}
+
+}  // namespace gptc

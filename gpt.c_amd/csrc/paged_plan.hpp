@@ -1,0 +1,60 @@
+// The plan of a paged step (include/paged.h) as the kernels and their launches see it (internal).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include "paged.h"
+
+namespace gptc {
+
+// One piece of attention work for one kv head: the query rows row0 .. of one sequence against the keys
+// [key0, key1).  Everything a workgroup needs is in its item, so that it waits for one load only.
+struct PagedItem {
+    int tok0;   // the sequence's first row of the step's tensors
+    int past;   // its tokens before the step
+    int rows;   // its query rows of one kv head: new tokens * group, row = token * group + head of the group
+    int row0;   // the item's first row
+    int key0, key1;
+    int part;   // -1: the item covers all keys of its rows; else its slot of the workspace
+    int table;  // where the sequence's page numbers start; on the host side of the list, its sequence
+};
+
+// The rows whose keys were cut into n items: their parts are part0 .. part0 + n - 1.
+struct PagedMerge {
+    int tok0, rows, row0, part0, n, pad0, pad1, pad2;
+};
+
+constexpr int kPagedRows = 16;  // query rows of an item
+
+// Keys that a round of the four waves of a workgroup takes: 16 or 32 each (csrc/paged_attn.hip).
+constexpr int paged_unit(int dtype) { return dtype == GPTC_BF16 ? 128 : 64; }
+
+// Items that the keys of one step are cut into at most, over all kv heads: see paged_schedule.
+constexpr int kPagedTarget = 1024;
+
+// Fills items (and merges) for a step; returns the number of items, or -1 when one of the lists does not fit.
+// items[i].table receives the sequence.
+int paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int dtype,
+                   PagedItem *items, int cap, PagedMerge *merges, int merge_cap, int *n_merges);
+
+// What the attention kernels take.
+struct PagedAttnParams {
+    const float *q;
+    float *out;
+    const void *k, *v;
+    const int *head;  // {tokens, items, merges} of the plan, read on the device: a captured launch covers the
+                      // plan's capacity and runs what the plan holds then
+    const PagedItem *items;
+    const PagedMerge *merges;
+    const int *table;
+    float *part_o, *part_ml;  // partial outputs [part][kv head][row][D], and their (max, sum) pairs
+    int q_stride, rows;       // floats of a q row; rows of q and out
+    int H, KV, group, D, page_shift;
+    float scale_log2;
+    int n_items, n_merges;  // of the launch
+    bool bf16, vec;         // vec: every row starts at a multiple of 16 bytes and holds whole vectors
+};
+
+void launch_paged_attention(const PagedAttnParams &p, hipStream_t s);
+
+}  // namespace gptc

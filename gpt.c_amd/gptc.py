@@ -17,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libgptc_amd.so")
 
 CPU, CUDA = 0, 1
+F32, BF16 = 0, 1  # page types (include/paged.h)
 
 
 class Tensor(ctypes.Structure):
@@ -215,6 +216,16 @@ SIGNATURES = {
     "gptc_kv_cache_free": (None, [_vp]),
     "gptc_gpt2_decode": (TensorP, [_vp, _vp, TensorP, _ci]),
     "gptc_gpt2_generate": (None, [_vp, _vp, TensorP, _ci, _ci]),
+    # paged.h
+    "gptc_paged_cache_create": (_vp, [_ci, _ci, _ci, _ci, _ci, _ci, ctypes.POINTER(_vp), ctypes.POINTER(_vp)]),
+    "gptc_paged_cache_free": (None, [_vp]),
+    "gptc_paged_plan_create": (_vp, [_vp, _ci, _ci, _ci, _ci]),
+    "gptc_paged_plan_set": (None, [_vp, _ci, _ip, _ip, _ip, _ci]),
+    "gptc_paged_plan_free": (None, [_vp]),
+    "gptc_rotary_table": (TensorP, [_ci, _ci, ctypes.c_double]),
+    "gptc_paged_append_cuda": (None, [_vp, _ci, TensorP, TensorP, _ci, TensorP]),
+    "gptc_paged_attention_cuda": (None, [_vp, _ci, TensorP, TensorP]),
+    "gptc_paged_schedule": (_ci, [_ci, _ip, _ip, _ci, _ci, _ci, _ip, _ci]),
     # tensor.h (BLAS front ends)
     "saxpy": (None, [_ci, _cf, TensorP, _ci, _ci, TensorP, _ci, _ci]),
     "sgemm": (None, [_ci, _ci, _ci, _ci, _ci, _cf, TensorP, _ci, _ci, TensorP, _ci, _ci, _cf, TensorP, _ci, _ci]),
@@ -588,3 +599,60 @@ class KVCache:
         if self.raw:
             self.rt.lib.gptc_kv_cache_free(self.raw)
             self.raw = None
+
+
+class PagedCacheT(ctypes.Structure):
+    """gptc_paged_cache_t (include/paged.h)."""
+    _fields_ = [("n_layers", _ci), ("n_pages", _ci), ("page", _ci), ("n_kv_heads", _ci), ("head_dim", _ci),
+                ("dtype", _ci), ("owned", _ci), ("k", ctypes.POINTER(_vp)), ("v", ctypes.POINTER(_vp))]
+
+
+class PagedCache:
+    """gptc_paged_cache_create: keys and values in pages.  k, v: device addresses of the layers' blocks, or None."""
+
+    def __init__(self, rt, n_layers, n_pages, page, n_kv_heads, head_dim, dtype=F32, k=None, v=None):
+        def addresses(x):
+            return None if x is None else (_vp * n_layers)(*x)
+        self.rt = rt
+        self.raw = ctypes.c_void_p(rt.lib.gptc_paged_cache_create(n_layers, n_pages, page, n_kv_heads, head_dim, dtype,
+                                                                  addresses(k), addresses(v)))
+        self.s = ctypes.cast(self.raw, ctypes.POINTER(PagedCacheT)).contents
+
+    def free(self):
+        if self.raw:
+            self.rt.lib.gptc_paged_cache_free(self.raw)
+            self.raw = None
+
+    def __del__(self):
+        self.free()
+
+
+class PagedPlan:
+    """gptc_paged_plan_create: what one step does, shared by its layers."""
+
+    def __init__(self, rt, cache, n_heads, max_seqs, max_tokens, max_len):
+        self.rt, self.cache = rt, cache
+        self.raw = ctypes.c_void_p(rt.lib.gptc_paged_plan_create(cache.raw, n_heads, max_seqs, max_tokens, max_len))
+
+    def set(self, past, fresh, table):
+        """past, fresh: tokens of each sequence before the step and new in it; table: (sequences, pages) page numbers."""
+        past, fresh = (np.ascontiguousarray(x, np.int32) for x in (past, fresh))
+        table = np.ascontiguousarray(table, np.int32)
+        if past.ndim != 1 or past.shape != fresh.shape or table.ndim != 2 or len(table) != len(past):
+            raise ValueError(f"expected (n,), (n,) and (n, pages), but got {past.shape}, {fresh.shape}, {table.shape}")
+        self.rt.lib.gptc_paged_plan_set(self.raw, len(past), past.ctypes.data_as(_ip), fresh.ctypes.data_as(_ip),
+                                        table.ctypes.data_as(_ip), table.shape[1])
+
+    def append(self, layer, qkv, rotary=None, interleaved=False, q_out=None):
+        self.rt.lib.gptc_paged_append_cuda(self.raw, layer, qkv, rotary, int(interleaved), q_out)
+
+    def attention(self, layer, q, output):
+        self.rt.lib.gptc_paged_attention_cuda(self.raw, layer, q, output)
+
+    def free(self):
+        if self.raw:
+            self.rt.lib.gptc_paged_plan_free(self.raw)
+            self.raw = None
+
+    def __del__(self):
+        self.free()

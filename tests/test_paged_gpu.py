@@ -1,0 +1,338 @@
+"""Appending to and attending over paged caches (include/paged.h) on the GPU, against the definitions in 64 bits.
+
+Tolerances.  A rounding is off by at most half a step: u = 2^-24 for fp32, 2^-8 for bf16 pages.
+  append: a rotated value x c - y s is two products and a sum: off by at most 3 u (|x c| + |y s|) <= 6 u max|x|,
+    (in bf16 pages half a step of the value on top); without rotation fp32 pages hold the values themselves and bf16
+    pages the nearest.
+  attention: y = sum p v / sum p.  A score of D products is off by at most (D + 2) u sum|q k| scale (any order, and
+    the scaling), which multiplies p by e^that; exp2 and the running sums of n weights add (log2 n + 8) u for sums in
+    trees and runs of a few dozen keys, taken here as 64 u.  The products of bf16 pages with three-part values are
+    exact to u.  So |dy| <= max|v| (2 max_j |dt_j| + 128 u), with |dt| <= (D + 2) u max_j sum_d |q k| / sqrt(D).
+"""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import gptc
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+class Pool:
+    """A cache whose pages are torch tensors, NaN wherever no token lies, and a plan over it."""
+
+    def __init__(self, rt, past, fresh, H, KV, D, page, dtype, seed=0, spare=3, layers=1, room=0, max_len=None):
+        self.rt, self.past, self.fresh = rt, list(past), list(fresh)
+        self.H, self.KV, self.D, self.page, self.layers = H, KV, D, page, layers
+        self.rng = np.random.default_rng(seed)
+        total = [p + f for p, f in zip(past, fresh)]
+        need = [-(-t // page) for t in total]
+        n_pages = sum(need) + spare
+        order = self.rng.permutation(n_pages)
+        self.table = np.zeros((len(total), max(need + [1])), np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = order[at:at + n]
+            at += n
+        self.tdtype = torch.bfloat16 if dtype == gptc.BF16 else torch.float32
+        self.k, self.v = ([torch.full((n_pages, KV, page, D), float("nan"), dtype=self.tdtype, device="cuda")
+                           for _ in range(layers)] for _ in range(2))
+        torch.cuda.synchronize()
+        self.cache = gptc.PagedCache(rt, layers, n_pages, page, KV, D, dtype, [x.data_ptr() for x in self.k],
+                                     [x.data_ptr() for x in self.v])
+        self.plan = gptc.PagedPlan(rt, self.cache, H, len(total) + room, max(1, sum(fresh)) + room,
+                                   max_len or max(total + [1]))
+
+    def set(self):
+        self.plan.set(self.past, self.fresh, self.table)
+
+    def normal(self, *shape):
+        return self.rng.standard_normal(shape).astype(np.float32)
+
+    def rows(self, s, lo, hi):
+        """Where tokens lo .. hi of sequence s lie: (pages, slots)."""
+        t = np.arange(lo, hi)
+        return torch.tensor(self.table[s, t // self.page], device="cuda").long(), torch.tensor(t % self.page, device="cuda")
+
+    def fill(self, upto, std=1.0, layer=0):
+        """Random tokens 0 .. upto[s] of each sequence, rounded to the pages' type; returned in 64 bits."""
+        kept = []
+        for s, n in enumerate(upto):
+            k, v = (torch.tensor(std * self.normal(n, self.KV, self.D)).to(self.tdtype) for _ in range(2))
+            at = self.rows(s, 0, n)
+            self.k[layer][at[0], :, at[1]] = k.cuda()
+            self.v[layer][at[0], :, at[1]] = v.cuda()
+            kept.append((k.double().numpy(), v.double().numpy()))
+        torch.cuda.synchronize()
+        return kept
+
+    def held(self, s, lo, hi, layer=0):
+        at = self.rows(s, lo, hi)
+        torch.cuda.synchronize()
+        return tuple(x[layer][at[0], :, at[1]].double().cpu().numpy() for x in (self.k, self.v))
+
+    def free(self):
+        self.rt.sync()
+        self.plan.free()
+        self.cache.free()
+
+
+def attention(q, kv, past, H, KV, D):
+    """One sequence in 64 bits: q (n, H, D), kv its keys and values (past + n, KV, D); y, and the bound on its error."""
+    k, v = kv
+    n = q.shape[0]
+    y, bound = np.zeros((n, H, D)), np.zeros((n, H, 1))
+    for i in range(n):
+        for h in range(H):
+            kk, vv = k[:past + i + 1, h * KV // H], v[:past + i + 1, h * KV // H]
+            t = kk @ q[i, h] / np.sqrt(D)
+            p = np.exp(t - t.max())
+            y[i, h] = p @ vv / p.sum()
+            dt = (D + 2) * U * (np.abs(kk) @ np.abs(q[i, h])).max() / np.sqrt(D)
+            bound[i, h] = np.abs(vv).max() * (2 * dt + 128 * U)
+    return y, bound
+
+
+def check_attention(pool, kept, q, got, width=None):
+    row = 0
+    for s, (p, f) in enumerate(zip(pool.past, pool.fresh)):
+        want, bound = attention(q[row:row + f].astype(np.float64), kept[s], p, pool.H, pool.KV, pool.D)
+        y = got[row:row + f].reshape(f, pool.H, pool.D)
+        err = np.abs(y - want)
+        assert (err <= bound).all(), (s, float((err / bound).max()))
+        row += f
+
+
+SHAPES = [
+    # past, fresh, H, KV, D, page
+    ([0], [1], 1, 1, 64, 16),                          # the very first token
+    ([299], [1], 12, 12, 64, 16),
+    ([0], [17], 2, 2, 64, 16),                         # one row past a tile
+    ([15, 16, 17, 31, 0], [1, 1, 1, 1, 1], 2, 1, 64, 16),  # around the page's end
+    ([63, 64, 65, 127, 128, 129], [1] * 6, 4, 2, 128, 64),
+    ([1000, 3, 0, 517], [1, 0, 33, 5], 6, 2, 64, 32),  # a sequence that waits, a prompt, chunks
+    ([5, 100], [70, 1], 25, 5, 80, 32),                # odd heads
+    ([40, 2], [3, 9], 3, 1, 33, 16),                   # rows that are no whole vectors
+    ([20], [4], 2, 2, 1, 16),
+    ([20], [4], 2, 2, 127, 16),
+    ([77, 0], [2, 18], 8, 1, 24, 128),
+    ([3000], [1], 2, 2, 128, 256),                     # keys cut into parts
+    ([2049, 700], [9, 20], 16, 1, 64, 64),             # cut, several tiles
+]
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_attention(rt, case, dtype):
+    past, fresh, H, KV, D, page = SHAPES[case]
+    pool = Pool(rt, past, fresh, H, KV, D, page, dtype, seed=case)
+    kept = pool.fill([p + f for p, f in zip(past, fresh)])
+    pool.set()
+    N = sum(fresh)
+    q = pool.normal(N, H, D)
+    tq, out = rt.from_numpy(q.reshape(N, -1)), rt.empty((N, H * D))
+    pool.plan.attention(0, tq, out)
+    got = rt.to_numpy(out)
+    pool.free()
+    check_attention(pool, kept, q, got)
+    rt.free(tq)
+    rt.free(out)
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+def test_attention_is_the_same_every_time_and_in_the_qkv_layout(rt, dtype):
+    pool = Pool(rt, [2500, 31], [3, 40], 6, 2, 64, 16, dtype, seed=5)
+    kept = pool.fill([2503, 71])
+    pool.set()
+    q = pool.normal(43, 6, 64)
+    wide = np.concatenate([q.reshape(43, -1), np.full((43, 2 * 2 * 64), np.nan, np.float32)], 1)
+    tq, tw, out = rt.from_numpy(q.reshape(43, -1)), rt.from_numpy(wide), rt.empty((43, 384))
+    got = []
+    for t in (tq, tw, tq):
+        pool.plan.attention(0, t, out)
+        got.append(rt.to_numpy(out))
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+    check_attention(pool, kept, q, got[0])
+    pool.free()
+    for t in (tq, tw, out):
+        rt.free(t)
+
+
+def rotate(x, table, rot, interleaved):
+    """x (n, heads, D) in 64 bits by rows of the table."""
+    x = x.copy()
+    cos, sin = table[:, None, :rot // 2], table[:, None, rot // 2:]
+    a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else (x[..., :rot // 2], x[..., rot // 2:rot])
+    one, two = a * cos - b * sin, b * cos + a * sin
+    if interleaved:
+        x[..., 0:rot:2], x[..., 1:rot:2] = one, two
+    else:
+        x[..., :rot // 2], x[..., rot // 2:rot] = one, two
+    return x
+
+
+APPENDS = [
+    # past, fresh, H, KV, D, page, rot, interleaved
+    ([0], [1], 1, 1, 64, 16, 0, False),
+    ([0, 15, 16, 500], [1, 1, 1, 1], 12, 12, 64, 16, 0, False),
+    ([7, 0, 40], [30, 0, 2], 4, 2, 128, 32, 128, False),
+    ([7, 0, 40], [30, 0, 2], 4, 2, 128, 32, 128, True),
+    ([3, 90], [50, 1], 5, 1, 80, 16, 32, True),
+    ([3, 90], [50, 1], 5, 1, 80, 16, 40, False),
+    ([1, 2], [3, 4], 2, 1, 66, 16, 4, False),   # rot 4: pairs of two halves of two
+    ([1, 2], [3, 4], 3, 3, 33, 16, 32, True),   # rows that are no whole vectors
+    ([1, 2], [3, 4], 3, 3, 33, 16, 30, False),
+    ([10], [5], 1, 1, 2, 16, 2, False),
+    ([10], [5], 2, 1, 1, 64, 0, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", range(len(APPENDS)))
+def test_append(rt, case, dtype):
+    past, fresh, H, KV, D, page, rot, interleaved = APPENDS[case]
+    pool = Pool(rt, past, fresh, H, KV, D, page, dtype, seed=case, max_len=600)
+    pool.set()
+    N, rows = sum(fresh), sum(fresh) + 2
+    x = pool.normal(rows, H + 2 * KV, D)
+    tx, rotary, q_out = rt.from_numpy(x.reshape(rows, -1)), None, None
+    if rot:
+        rotary = rt.lib.gptc_rotary_table(600, rot, 10000.0)
+        q_out = rt.from_numpy(np.full((rows, H * D), 7.5, np.float32))
+        table = rt.to_numpy(rotary).astype(np.float64)
+        angle = np.arange(600)[:, None] * 10000.0 ** (-np.arange(0, rot, 2) / rot)
+        # The nearest floats to the 64-bit values.
+        assert np.abs(table - np.concatenate([np.cos(angle), np.sin(angle)], 1)).max() <= U * (1 + 1e-6)
+    before = [pool.k[0].clone(), pool.v[0].clone()]
+    pool.plan.append(0, tx, rotary, interleaved, q_out)
+    rt.sync()
+    q = rt.to_numpy(q_out) if rot else None
+    row, written = 0, torch.zeros(pool.k[0].shape[0], page, dtype=torch.bool, device="cuda")
+    for s, (p, f) in enumerate(zip(past, fresh)):
+        if f == 0:
+            continue
+        mine = x[row:row + f].astype(np.float64)
+        k, v = pool.held(s, p, p + f)
+        want_k, want_v = mine[:, H:H + KV], mine[:, H + KV:]
+        tol_k = np.zeros(())
+        if rot:
+            want_q = rotate(mine[:, :H], table[p:p + f], rot, interleaved)
+            want_k = rotate(want_k, table[p:p + f], rot, interleaved)
+            tol = tol_k = 6 * U * np.abs(mine).max()
+            assert np.abs(q[row:row + f].reshape(f, H, D) - want_q).max() <= tol
+        if dtype == gptc.BF16:
+            tol_k = tol_k + 2.0 ** -8 * np.abs(want_k)
+            want_v = torch.tensor(x[row:row + f, H + KV:]).bfloat16().double().numpy()
+        assert (np.abs(k - want_k) <= tol_k).all()
+        assert np.array_equal(v, want_v)
+        at = pool.rows(s, p, p + f)
+        written[at[0], at[1]] = True
+        row += f
+    # Nothing else was touched: other slots hold what they held (NaN), and so do q_out's rows past the last token.
+    for now, was in zip((pool.k[0], pool.v[0]), before):
+        keep = ~written[:, None, :, None].expand_as(now)
+        assert torch.isnan(now[keep]).all() and torch.isnan(was).all()
+    if rot:
+        assert (q[N:] == 7.5).all()
+        rt.free(rotary)
+        rt.free(q_out)
+    rt.free(tx)
+    pool.free()
+
+
+def test_rows_past_the_last_token_are_left_as_they_were(rt):
+    pool = Pool(rt, [40, 9], [2, 1], 2, 2, 64, 16, gptc.F32)
+    kept = pool.fill([42, 10])
+    pool.set()
+    q = pool.normal(8, 2, 64)
+    tq, out = rt.from_numpy(q.reshape(8, -1)), rt.from_numpy(np.full((8, 128), 7.5, np.float32))
+    pool.plan.attention(0, tq, out)
+    got = rt.to_numpy(out)
+    assert (got[3:] == 7.5).all()
+    check_attention(pool, kept, q, got)
+    pool.free()
+
+
+def test_a_step_without_tokens_does_nothing(rt):
+    pool = Pool(rt, [40, 0], [0, 0], 2, 2, 64, 16, gptc.F32)
+    pool.set()
+    x, q, out = rt.from_numpy(pool.normal(1, 6 * 64)), rt.from_numpy(pool.normal(1, 128)), rt.from_numpy(np.full((1, 128), 7.5, np.float32))
+    pool.plan.append(0, x)
+    pool.plan.attention(0, q, out)
+    assert (rt.to_numpy(out) == 7.5).all()
+    assert torch.isnan(pool.k[0]).all()
+    pool.plan.set([], [], np.zeros((0, 1), np.int32))
+    pool.plan.attention(0, q, out)
+    assert (rt.to_numpy(out) == 7.5).all()
+    pool.free()
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+def test_large_scores_and_far_positions(rt, dtype):
+    """Scores of some hundreds: all weight on one key, others underflow to nothing; no infinities on the way."""
+    pool = Pool(rt, [700], [3], 2, 2, 64, 16, dtype, seed=9)
+    kept = pool.fill([703], std=6.0)
+    pool.set()
+    q = 6 * pool.normal(3, 2, 64)
+    tq, out = rt.from_numpy(q.reshape(3, -1)), rt.empty((3, 128))
+    pool.plan.attention(0, tq, out)
+    got = rt.to_numpy(out)
+    assert np.isfinite(got).all()
+    check_attention(pool, kept, q, got)
+    pool.free()
+
+
+def test_two_layers_and_shared_prefix(rt):
+    """Two sequences read the same first pages; each layer has its own."""
+    pool = Pool(rt, [64, 64], [1, 2], 4, 4, 64, 32, gptc.F32, layers=2, seed=4)
+    kept = [pool.fill([65, 66], layer=i) for i in range(2)]
+    pool.table[1, :2] = pool.table[0, :2]
+    pool.set()
+    q = pool.normal(3, 4, 64)
+    tq, out = rt.from_numpy(q.reshape(3, -1)), rt.empty((3, 256))
+    for i in range(2):
+        k, v = kept[i][1]
+        k0, v0 = kept[i][0]
+        kept[i][1] = np.concatenate([k0[:64], k[64:]]), np.concatenate([v0[:64], v[64:]])
+        pool.plan.attention(i, tq, out)
+        check_attention(pool, kept[i], q, rt.to_numpy(out))
+    pool.free()
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+def test_matches_the_frameworks_causal_forward(rt, dtype):
+    """A prompt in chunks and then single tokens: every row is that of the causal forward over the whole sequence."""
+    T, H, D = 130, 4, 64
+    C = H * D
+    pool = Pool(rt, [0], [T], H, H, D, 16, dtype, max_len=T)
+    x = pool.normal(T, 3 * C)
+    ref = x.copy()
+    if dtype == gptc.BF16:
+        ref[:, C:] = torch.tensor(x[:, C:]).bfloat16().float().numpy()
+    layer = gptc.AttentionLayer(rt, C, H, T)
+    layer.to(gptc.CUDA)
+    yt = layer.forward(rt.from_numpy(ref.reshape(1, T, 3 * C)))
+    want = rt.to_numpy(yt)[0]
+    rt.free(yt)
+    layer.free()
+    at, got = 0, []
+    for n in (1, 50, 16, 61, 1, 1):
+        pool.plan.set([at], [n], pool.table)
+        tx, out = rt.from_numpy(x[at:at + n]), rt.empty((n, C))
+        pool.plan.append(0, tx)
+        pool.plan.attention(0, tx, out)
+        got.append(rt.to_numpy(out))
+        rt.free(tx)
+        rt.free(out)
+        at += n
+    assert at == T
+    # Two fp32 evaluations of the same rows: 2 (2 dt + 128 u) max|v| with |t| terms of this size.
+    kv = ref[:, C:].reshape(T, 2, H, D).astype(np.float64)
+    _, bound = attention(x[:, :C].reshape(T, H, D).astype(np.float64), (kv[:, 0], kv[:, 1]), 0, H, H, D)
+    err = np.abs(np.concatenate(got) - want).reshape(T, H, D)
+    assert (err <= 2 * bound).all(), float((err / bound).max())
+    pool.free()
