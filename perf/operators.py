@@ -294,9 +294,10 @@ def _paged_calls(s):
 
 
 def _sample_calls(s):
+    lib = _rt().lib
     s["out"] = torch.empty(s["case"]["rows"], device="cuda"), torch.empty(s["case"]["rows"], device="cuda")
     args = [_wrap(x) for x in (s["logits"], s["params"], s["u"], *s["out"])]
-    s["call"] = _rt().lib.gptc_sample_cuda, args
+    s["call"] = lib.gptc_sample_cuda, args
 
 
 def prepare(case, seed):
