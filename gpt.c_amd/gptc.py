@@ -211,6 +211,7 @@ SIGNATURES = {
     "gptc_linear_rows_cuda": (None, [TensorP, TensorP, TensorP, TensorP, _ci, TensorP]),
     "gptc_embed_token_cuda": (None, [TensorP, TensorP, TensorP, _ci, TensorP]),
     "gptc_argmax_cuda": (None, [TensorP, TensorP]),
+    "gptc_sample_cuda": (None, [TensorP, TensorP, TensorP, TensorP, TensorP]),
     # generate.h
     "gptc_kv_cache_create": (_vp, [_vp, _ci, _ci]),
     "gptc_kv_cache_free": (None, [_vp]),

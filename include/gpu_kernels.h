@@ -365,12 +365,31 @@ long long gptc_decode_noalloc_scratch_floats(void);
  *   out (B, C) = wte[ids] + wpe[pos]; ids outside [0, V) give NaN rows.
  * gptc_argmax_cuda(logits, ids)
  *   ids[r] = first index of the maximum of logits row r (greedy decoding).
+ * gptc_sample_cuda(logits, params, u, ids, prob)
+ *   Draws a token of every row of logits (rows, V), V <= 2^24, from the random
+ *   number u[r] of [0, 1).  params (4), or (rows, 4) for settings per row:
+ *   temperature, top_k, top_p, min_p, whole numbers held in floats where they
+ *   count.  With the tokens ordered by logit, equal ones by index, and weights
+ *   exp((logit - maximum) / temperature): top_k keeps the first top_k tokens
+ *   (all when < 1 or >= V); top_p, of those, the shortest head with at least
+ *   top_p of their weight (all when >= 1, the first when <= 0); min_p, of
+ *   those, the weights of at least min_p (all when <= 0, the maximum's when
+ *   >= 1).  ids[r] is the first token, by index, at which the sum of the kept
+ *   weights passes u[r] of their total (u outside [0, 1) counts as its end);
+ *   prob[r], unless prob is NULL, that token's share of them.  A temperature
+ *   that is not above 0 takes the first maximum, prob 1.  Logits of -inf and
+ *   NaN are never drawn; a row of nothing else gives id -1 and prob 0.  Sums
+ *   are exact in integers, so the result depends on nothing but the row.
+ *   No counterpart on a device in the reference: infer_gpt.c draws on the host
+ *   from the softmax of one row (sample_mult).
  */
 void gptc_linear_rows_cuda(const tensor_t *W, const tensor_t *b, const tensor_t *x, const tensor_t *residual,
                            const int act, tensor_t *y);
 void gptc_embed_token_cuda(const tensor_t *wte, const tensor_t *wpe, const tensor_t *ids, const int pos,
                            tensor_t *out);
 void gptc_argmax_cuda(const tensor_t *logits, tensor_t *ids);
+void gptc_sample_cuda(const tensor_t *logits, const tensor_t *params, const tensor_t *u, tensor_t *ids,
+                      tensor_t *prob);
 
 void *gptc_stream(void);
 void gptc_set_kernel_events(void **events, int n);

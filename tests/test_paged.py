@@ -150,3 +150,33 @@ def test_long_contexts_are_cut_and_short_ones_are_not(lib):
     assert n > 50 and (items[:, 6] >= 0).all()
     sizes = items[:, 5] - items[:, 4]
     assert sizes.max() - sizes.min() <= 64
+
+
+SAMPLE_REFUSALS = {
+    "host logits": ("sample(host(2, 8), host(4), host(2), host(2))", "logits to be a tensor on the GPU"),
+    "null params": ("sample(gpu(2, 8), None, gpu(2), gpu(2))", "`params` (NULL)"),
+    "params of some rows": ("sample(gpu(3, 8), gpu(2, 4), gpu(3), gpu(3))", "4 for each of 3 rows"),
+    "random numbers": ("sample(gpu(3, 8), gpu(4), gpu(2), gpu(3))", "Expected 3 random numbers"),
+    "ids": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(4))", "Expected 3 ids"),
+    "shares": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3), gpu(2))", "Expected 3 probabilities"),
+    "vocabulary": ("sample(gpu(1, (1 << 24) + 1), gpu(4), gpu(1), gpu(1))", "up to 2^24 tokens"),
+    "without a runtime": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3))", "runtime_init"),
+}
+
+
+@pytest.mark.parametrize("name", sorted(SAMPLE_REFUSALS))
+def test_sampling_refused(name):
+    call, message = SAMPLE_REFUSALS[name]
+    r = run_c("""
+        def gpu(*shape):
+            t = gptc.Tensor()
+            t.t, t.ndims, t.length, t.device = ctypes.cast(4096, ctypes.POINTER(ctypes.c_float)), len(shape), int(np.prod(shape)), gptc.CUDA
+            for i, n in enumerate(shape):
+                t.shape[i] = n
+            return ctypes.pointer(t)
+
+        def sample(logits, params, u, ids, prob=None):
+            rt.lib.gptc_sample_cuda(logits, params, u, ids, prob)
+    """ + "\n        " + call)
+    assert r.returncode == 1 and "survived" not in r.stdout, r.stderr
+    assert message in r.stderr, r.stderr
