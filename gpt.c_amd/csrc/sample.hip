@@ -12,9 +12,14 @@
 // floats, and every sum of them is a 64-bit integer, the same in any order (atomics too).  shift leaves room for a
 // whole vocabulary (46 bits at 50257 tokens: a weight is off by at most 2^-47 of the largest).
 //
-// Nothing is sorted.  A bound is found in histograms: over 2048 steps of (M - l) / T first, then over the bits of
-// the logits in the one step where the bound lies, until it holds at most 1024 tokens, which are ranked by
-// counting, or equal logits only, whose order is that of the vocabulary.
+// A workgroup takes a row, and holds its first 57344 logits in registers, so that they are read once (the rest is
+// read again by each pass).  Nothing is sorted:
+//   top-k   the k-th largest of the threads' own maxima is a lower bound of the k-th logit, and few tokens lie
+//           above it: they are ranked by counting, and the rest of the work is theirs alone.
+//   else    a bound is found in histograms: over 8192 steps of (M - l) / T first, then over the bits of the logits
+//           in the one step where the bound lies, until it holds at most 1024 tokens, which are ranked, or equal
+//           logits only, whose order is that of the vocabulary.  The kept tokens are then gathered, and the draw
+//           finds the stretch of the vocabulary where the sum is passed, and the token in it.
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include "gpu_kernels.h"
@@ -27,8 +32,11 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kBins = 2048;
-constexpr int kList = 1024;  // tokens that are ranked by counting: one for each thread
+constexpr int kChunk = 8;            // logits of a thread that are handled together
+constexpr int kHeld = 56;            // logits of a thread that stay in registers
+constexpr int kBins = 8192;          // of a histogram; tokens that can be gathered
+constexpr int kList = kThreads;      // tokens that can be ranked
+constexpr int kTable = 256;
 
 struct SampleParams {
     const float *logits, *params, *u;
@@ -36,27 +44,37 @@ struct SampleParams {
     int V, param_rows, shift;
 };
 
-// Order-preserving bits of a float that is no NaN.
-__device__ __forceinline__ uint32_t key_of(float l) {
-    const uint32_t b = __float_as_uint(l);
-    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
-}
+struct Token {
+    float l;
+    int i;
+};
 
 struct Lds {
-    unsigned count[kBins];
-    u64 mass[kBins];
-    float list_l[kList];
-    int list_i[kList];
+    union {
+        u64 mass[kBins];
+        Token kept[kBins];
+    };
+    Token list[kList];
     u64 list_w[kList];
-    u64 wave_sum[kWaves];
+    u64 ahead[kList];
+    double table[kTable];  // 2^(-j / 256)
+    u64 wave_sum[2 * kWaves];
     float wave_max[kWaves];
     int wave_idx[kWaves];
     uint32_t key_lo, key_hi;
     int n, found;
-    float bound_l;
-    int bound_i;
     u64 before;
+    Token bound;
 };
+
+// Order-preserving bits of a float that is no NaN, and back.
+__device__ __forceinline__ uint32_t key_of(float l) {
+    const uint32_t b = __float_as_uint(l);
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+    return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
+}
 
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
 #pragma unroll
@@ -75,177 +93,298 @@ __device__ __forceinline__ u64 wave_scan64(u64 v) {
     return v;
 }
 
+// The sum over the workgroup (every thread gets it), and with `upto` the inclusive sums by thread.
+__device__ __forceinline__ u64 block_sum64(Lds &s, u64 v, u64 *upto = nullptr) {
+    const int w = threadIdx.x / kWave;
+    u64 in = upto != nullptr ? wave_scan64(v) : wave_sum64(v);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) s.wave_sum[w] = in;
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        const u64 x = s.wave_sum[i];
+        if (upto != nullptr && i < w) in += x;
+        total += x;
+    }
+    if (upto != nullptr) *upto = in;
+    return total;
+}
+
 struct Row {
     const float *logits;
     int V;
-    float M, inv_t_f;     // inv_t_f, limit_f: the histograms' steps, monotone in the logit whatever their rounding
-    double inv_t, limit;  // limit: where a weight rounds to nothing
-    float limit_f, bin_scale;
-    double one;  // 2^shift
-    float bound_l;
-    int bound_i;
+    int from, to, chunks;    // the wave's stretch of the held logits, and its chunks
+    int rest_from, rest_to, rest_chunks;  // and of the others
+    float M;
+    double per_256;  // log2(e) 256 / T: the weight is 2^(-(M - l) per_256 / 256)
+    double limit;    // of that exponent: from here on a weight rounds to nothing
+    int shift;
+    float inv_t, z_limit, bin_scale;  // the histogram's steps: monotone in the logit, whatever their rounding
+    Token bound;
     u64 min_w;
 
-    __device__ __forceinline__ float at(int i) const { return fmaxf(logits[i], -INFINITY) + 0.0f; }  // NaN: -inf; -0: 0
+    // NaN counts as -inf, and -0 as 0: equal logits have equal bits.
+    static __device__ __forceinline__ float plain(float l) { return fmaxf(l, -INFINITY) + 0.0f; }
 
-    __device__ __forceinline__ bool kept(float l, int i) const { return l > bound_l || (l == bound_l && i <= bound_i); }
+    __device__ __forceinline__ bool kept(float l, int i) const { return l > bound.l || (l == bound.l && i <= bound.i); }
 
-    __device__ __forceinline__ u64 weight(float l) const {
-        if (l == M) return static_cast<u64>(one);
-        const double z = (static_cast<double>(M) - static_cast<double>(l)) * inv_t;
-        if (!(z < limit)) return 0;
-        // Rounded to a whole number by the addition.
-        const double r = fma(exp(-z), one, 4503599627370496.0);
-        return static_cast<u64>(__double_as_longlong(r)) & ((1ull << 52) - 1);
+    // The exponent in steps of 1/256: a table's entry, and four terms of the exponential series for the rest (at
+    // most ln 2 / 512: the next term is below 2^-54).  The whole number comes out of the addition of 2^52.
+    __device__ __forceinline__ u64 weight(const Lds &s, float l) const {
+        if (l == M) return 1ull << shift;
+        const double t = (static_cast<double>(M) - static_cast<double>(l)) * per_256;
+        if (!(t < limit)) return 0;
+        const double n = rint(t), x = (n - t) * (0.6931471805599453 / 256);
+        const int e = static_cast<int>(n);
+        const double p = fma(x, fma(x, fma(x, fma(x, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * s.table[e & (kTable - 1)];
+        const double scale = __longlong_as_double(static_cast<long long>(1023 + shift - (e >> 8)) << 52);
+        return static_cast<u64>(__double_as_longlong(fma(p, scale, 4503599627370496.0))) & ((1ull << 52) - 1);
     }
 
     // The histogram's step, or -1 where the weight is nothing.
     __device__ __forceinline__ int bin(float l) const {
-        const float z = l == M ? 0.0f : (M - l) * inv_t_f;
-        return z < limit_f ? min(static_cast<int>(z * bin_scale), kBins - 1) : -1;
+        const float z = l == M ? 0.0f : (M - l) * inv_t;
+        return z < z_limit ? min(static_cast<int>(z * bin_scale), kBins - 1) : -1;
+    }
+
+    __device__ __forceinline__ void load_chunk(float (&l)[kChunk], int i0, int end) const {
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) l[e] = logits[min(i0 + e * kWave, V - 1)];  // all requested before one is used
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) l[e] = i0 + e * kWave < end ? plain(l[e]) : -INFINITY;
     }
 };
 
-// Tokens lo + lane, lo + lane + 64, ... below hi: f(logit, index), eight loads in flight.
+// A wave's share of n tokens: contiguous, in whole turns of its lanes.
+__device__ __forceinline__ int stretch(int n) { return (n + kThreads - 1) / kThreads * kWave; }
+
+typedef float Held[kHeld / kChunk][kChunk];
+
+// f(chunk, i) for each of the wave's chunks: chunk[e] is the logit of token i + 64 e, -inf past the stretch's end.
+// The loop stays a loop, and a switch copies a held chunk's registers: passes written out for every chunk are more
+// code than the instruction cache holds, and take registers.
 template <typename F>
-__device__ __forceinline__ void each(const Row &r, int lo, int hi, F f) {
-    constexpr int kAhead = 8;
-    for (int i0 = lo + (threadIdx.x & (kWave - 1)); i0 < hi; i0 += kAhead * kWave) {
-        float l[kAhead];
+__device__ __forceinline__ void each(const Row &r, const Held &h, F f) {
+    static_assert(kHeld / kChunk == 7, "the cases below");
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll 1
+    for (int c = 0; c < r.chunks + r.rest_chunks; ++c) {
+        float l[kChunk];
+        auto take = [&](const float (&x)[kChunk]) {
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e) l[e] = i0 + e * kWave < hi ? r.at(i0 + e * kWave) : -INFINITY;
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e)
-            if (i0 + e * kWave < hi) f(l[e], i0 + e * kWave);
+            for (int e = 0; e < kChunk; ++e) l[e] = x[e];
+        };
+        const bool rest = c >= r.chunks;
+        const int i = (rest ? r.rest_from + (c - r.chunks) * kChunk * kWave : r.from + c * kChunk * kWave) + lane;
+        switch (!rest ? c : 7) {
+            case 0: take(h[0]); break;
+            case 1: take(h[1]); break;
+            case 2: take(h[2]); break;
+            case 3: take(h[3]); break;
+            case 4: take(h[4]); break;
+            case 5: take(h[5]); break;
+            case 6: take(h[6]); break;
+            default: r.load_chunk(l, i, rest ? r.rest_to : r.to); break;
+        }
+        f(l, i);
     }
 }
 
-// Every token of the row: each wave takes a contiguous stretch.
-__device__ __forceinline__ int stretch(int n) { return (n + kWaves * kWave - 1) / (kWaves * kWave) * kWave; }
-
+// Gathers the tokens for which want(l, i); returns how many there are, of which the first `room` were written.
+// Their order is that of the waves' turns, so nothing may depend on it.
 template <typename F>
-__device__ __forceinline__ void all(const Row &r, F f) {
-    const int w = threadIdx.x / kWave, len = stretch(r.V);
-    each(r, min(w * len, r.V), min(w * len + len, r.V), f);
+__device__ __forceinline__ int gather(const Row &r, const Held &h, Lds &s, Token *to, int room, F want) {
+    const u64 below = (1ull << (threadIdx.x & (kWave - 1))) - 1;
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    each(r, h, [&](const float (&l)[kChunk], int i) {
+        u64 who[kChunk];
+        int count = 0;
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            who[e] = __ballot(want(l[e], i + e * kWave));
+            count += __popcll(who[e]);
+        }
+        if (count == 0) return;
+        int at = 0;
+        if (below == 0) at = atomicAdd(&s.n, count);
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            const int mine = at + __popcll(who[e] & below);
+            if ((who[e] & (below + 1)) != 0 && mine < room) to[mine] = Token{l[e], i + e * kWave};
+            at += __popcll(who[e]);
+        }
+    });
+    __syncthreads();
+    return s.n;
+}
+
+// ahead[i] = the sum over j < n of value(j) where before(j, i), for i < n <= kList: the pairs are shared out over
+// all threads.
+template <typename B, typename F>
+__device__ __forceinline__ void sum_ahead(Lds &s, int n, B before, F value) {
+    const int tid = threadIdx.x, parts = kThreads / n, i = tid % n, q = tid / n;
+    __syncthreads();
+    s.ahead[tid] = 0;
+    __syncthreads();
+    if (q < parts) {
+        const int from = n * q / parts, to = n * (q + 1) / parts;
+        u64 sum = 0;
+        for (int j = from; j < to; ++j)
+            if (before(j, i)) sum += value(j);
+        if (sum != 0) atomicAdd(&s.ahead[i], sum);
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ bool ahead_of(const Token &a, const Token &b) { return a.l > b.l || (a.l == b.l && a.i < b.i); }
+
+// Finds in the histogram the step where `target` (counted in what it holds) is reached: its number, and what lies
+// before it in `before`; -1 when the whole histogram holds less.  Each wave has a stretch of the steps.
+__device__ int locate(Lds &s, u64 target, u64 &before) {
+    constexpr int kPer = kBins / kThreads, kStretch = kPer * kWave;
+    const int w = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    u64 sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += s.mass[w * kStretch + e * kWave + lane];
+    block_sum64(s, sum);
+    u64 at = 0;
+    int q = 0;
+    while (q < kWaves && at + s.wave_sum[q] < target) at += s.wave_sum[q++];
+    if (q == kWaves) return -1;
+    if (w == q) {
+        u64 v[kPer];
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            v[e] = s.mass[w * kStretch + lane * kPer + e];
+            sum += v[e];
+        }
+        at += wave_scan64(sum) - sum;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            if (at < target && target <= at + v[e]) {
+                s.found = w * kStretch + lane * kPer + e;
+                s.before = at;
+            }
+            at += v[e];
+        }
+    }
+    __syncthreads();
+    before = s.before;
+    return s.found;
+}
+
+__device__ __forceinline__ void clear(Lds &s) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) s.mass[i * kThreads + threadIdx.x] = 0;
+    __syncthreads();
 }
 
 // The first token, in the order of the vocabulary, at which the sum of weigh(l, i) passes target(total); its
 // weight, and the total.  Stretches first, then stretches of the one it lies in, then its tokens.
 template <typename W, typename T>
-__device__ int pick(const Row &r, Lds &s, W weigh, T target, u64 &weight, u64 &total) {
+__device__ __forceinline__ int pick(const Row &r, const Held &h, Lds &s, W weigh, T target, u64 &weight, u64 &total) {
     const int w = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-    int lo = 0, hi = r.V;
-    u64 left = 0;
-    for (int level = 0; level < 2; ++level) {
-        const int len = stretch(hi - lo);
-        const int a = min(lo + w * len, hi), b = min(lo + w * len + len, hi);
+    auto sum_of = [&](int from, int to) {
         u64 sum = 0;
-        each(r, a, b, [&](float l, int i) { sum += weigh(l, i); });
-        sum = wave_sum64(sum);
+#pragma unroll 1
+        for (int i = from + lane; i < to + (kWave - 1); i += kChunk * kWave) {
+            float l[kChunk];
+            r.load_chunk(l, i, to);
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e) sum += weigh(l[e], i + e * kWave);
+        }
+        return wave_sum64(sum);
+    };
+    const int held = min(r.V, kHeld * kThreads);
+    u64 first = 0, second = 0;
+    each(r, h, [&](const float (&l)[kChunk], int i) {
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) sum += weigh(l[e], i + e * kWave);
+        (i - lane < held ? first : second) += sum;
+    });
+    first = wave_sum64(first);
+    second = wave_sum64(second);
+    __syncthreads();
+    if (lane == 0) {
+        s.wave_sum[w] = first;
+        s.wave_sum[kWaves + w] = second;
+    }
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < 2 * kWaves; ++i) total += s.wave_sum[i];
+    u64 left = target(total);
+    int q = 0;
+    while (q < 2 * kWaves - 1 && left >= s.wave_sum[q]) left -= s.wave_sum[q++];
+    const int from = q < kWaves ? 0 : held, upto = q < kWaves ? held : r.V;
+    int len = stretch(upto - from);
+    int lo = min(from + (q % kWaves) * len, upto), hi = min(lo + len, upto);
+    while (hi - lo > kChunk * kWave) {
+        len = stretch(hi - lo);
+        const int a = min(lo + w * len, hi);
+        const u64 sum = sum_of(a, min(a + len, hi));
         __syncthreads();
         if (lane == 0) s.wave_sum[w] = sum;
         __syncthreads();
-        if (level == 0) {
-            total = 0;
-            for (int i = 0; i < kWaves; ++i) total += s.wave_sum[i];
-            left = target(total);
-        }
-        int q = 0;
+        q = 0;
         while (q < kWaves - 1 && left >= s.wave_sum[q]) left -= s.wave_sum[q++];
-        const int from = min(lo + q * len, hi);
-        hi = min(from + len, hi);
-        lo = from;
+        lo = min(lo + q * len, hi);
+        hi = min(lo + len, hi);
     }
     // Every wave does the last part, so that all end with the token.
-    int last = lo;
-    weight = 0;
-    for (int i0 = lo; i0 < hi; i0 += kWave) {
-        const int i = i0 + lane;
-        const u64 mine = i < hi ? weigh(r.at(i), i) : 0;
-        const u64 upto = wave_scan64(mine);
-        const u64 over = __ballot(upto > left);
+    float l[kChunk];
+    r.load_chunk(l, lo + lane, hi);
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) {
+        const u64 mine = weigh(l[e], lo + e * kWave + lane), over_all = wave_scan64(mine);
+        const u64 over = __ballot(over_all > left);
         if (over != 0) {
             const int at = __ffsll(over) - 1;
             weight = __shfl(mine, at, kWave);
-            return i0 + at;
+            return lo + e * kWave + at;
         }
-        left -= __shfl(upto, kWave - 1, kWave);
-        last = min(i0 + kWave, hi) - 1;
+        left -= __shfl(over_all, kWave - 1, kWave);
     }
-    return last;  // not reached while target < total
-}
-
-// Finds in the histogram the step where `target` (counted in tokens, or in weight) is reached: its number, and what
-// lies before it in before; -1 when the whole histogram holds less.
-__device__ int locate(Lds &s, bool by_mass, u64 target, u64 &before) {
-    constexpr int kPer = kBins / kThreads;
-    const int tid = threadIdx.x, w = tid / kWave, lane = tid & (kWave - 1);
-    u64 v[kPer], sum = 0;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        v[e] = by_mass ? s.mass[tid * kPer + e] : s.count[tid * kPer + e];
-        sum += v[e];
-    }
-    const u64 upto = wave_scan64(sum);
-    if (lane == kWave - 1) s.wave_sum[w] = upto;
-    if (tid == 0) s.found = -1;
-    __syncthreads();
-    u64 at = upto - sum;
-    for (int i = 0; i < w; ++i) at += s.wave_sum[i];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        if (at < target && target <= at + v[e]) {
-            s.found = tid * kPer + e;
-            s.before = at;
-        }
-        at += v[e];
-    }
-    __syncthreads();
-    const int found = s.found;
-    before = s.before;
-    return found;
-}
-
-__device__ __forceinline__ void clear(Lds &s) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        s.count[i] = 0;
-        s.mass[i] = 0;
-    }
-    __syncthreads();
+    weight = 0;
+    return max(hi - 1, 0);  // not reached while target < total
 }
 
 // Moves the row's bound to the last token of the shortest head of the order (of the tokens kept so far) that holds
-// `target` tokens, or share of their weight.
-template <bool MASS>
-__device__ void bound_at(Row &r, Lds &s, u64 target, double share) {
+// `target` tokens, or `share` of their weight.
+__device__ __forceinline__ u64 head_of(double share, u64 total) {
+    const double want = ceil(share * static_cast<double>(total));
+    return want < 1.0 ? 1 : min(static_cast<u64>(want), total);
+}
+
+__device__ __forceinline__ void bound_at(Row &r, const Held &h, Lds &s, bool mass, u64 target, double share) {
     const int tid = threadIdx.x;
     clear(s);
-    all(r, [&](float l, int i) {
-        const int b = r.bin(l);
-        if (b < 0 || !r.kept(l, i)) return;
-        atomicAdd(&s.count[b], 1u);
-        if constexpr (MASS) atomicAdd(&s.mass[b], r.weight(l));
+    each(r, h, [&](const float (&l)[kChunk], int i) {
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            const int b = r.bin(l[e]);
+            if (b < 0 || !r.kept(l[e], i + e * kWave)) continue;
+            atomicAdd(&s.mass[b], mass ? r.weight(s, l[e]) : 1ull);
+        }
     });
     __syncthreads();
-    if constexpr (MASS) {
+    if (mass) {
         u64 sum = 0;
-        for (int i = tid; i < kBins; i += kThreads) sum += s.mass[i];
-        sum = wave_sum64(sum);
-        if ((tid & (kWave - 1)) == 0) s.wave_sum[tid / kWave] = sum;
-        __syncthreads();
-        sum = 0;
-        for (int i = 0; i < kWaves; ++i) sum += s.wave_sum[i];
-        const double want = ceil(share * static_cast<double>(sum));
-        target = want < 1.0 ? 1 : static_cast<u64>(want);
-        if (target > sum) target = sum;
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kBins / kThreads; ++i) sum += s.mass[i * kThreads + tid];
+        target = head_of(share, block_sum64(s, sum));
     }
     u64 before;
-    int b = locate(s, MASS, target, before);
+    int b = locate(s, target, before);
     if (b < 0) return;  // fewer tokens than that have any weight
     target -= before;
-    int n = s.count[b];
+    int n = gather(r, h, s, s.list, kList, [&](float l, int i) { return r.bin(l) == b && r.kept(l, i); });
     bool first = true;
     uint32_t lo = 0, hi = 0;
     auto in_group = [&](float l, int i) {
@@ -263,10 +402,13 @@ __device__ void bound_at(Row &r, Lds &s, u64 target, double share) {
         }
         __syncthreads();
         uint32_t k0 = 0xffffffffu, k1 = 0;
-        all(r, [&](float l, int i) {
-            if (!in_group(l, i)) return;
-            k0 = min(k0, key_of(l));
-            k1 = max(k1, key_of(l));
+        each(r, h, [&](const float (&l)[kChunk], int i) {
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e) {
+                if (!in_group(l[e], i + e * kWave)) continue;
+                k0 = min(k0, key_of(l[e]));
+                k1 = max(k1, key_of(l[e]));
+            }
         });
         atomicMin(&s.key_lo, k0);
         atomicMax(&s.key_hi, k1);
@@ -275,141 +417,238 @@ __device__ void bound_at(Row &r, Lds &s, u64 target, double share) {
         hi = s.key_hi;
         first = false;
         if (lo == hi) {
-            const float l = __uint_as_float(lo ^ (lo >> 31 ? 0x80000000u : 0xffffffffu));
-            if constexpr (MASS) {
-                const u64 w = r.weight(l);
+            const float l = of_key(lo);
+            if (mass) {
+                const u64 w = r.weight(s, l);
                 target = (target + w - 1) / w;
             }
             u64 weight, total;
-            const int i = pick(r, s, [&](float x, int j) { return static_cast<u64>(in_group(x, j)); },
+            const int i = pick(r, h, s, [&](float x, int j) { return static_cast<u64>(in_group(x, j)); },
                                [&](u64) { return target - 1; }, weight, total);
-            r.bound_l = l;
-            r.bound_i = i;
+            r.bound = Token{l, i};
             return;
         }
-        const int bits = 32 - __clz(hi - lo), down = bits > 11 ? bits - 11 : 0;
+        const int bits = 32 - __clz(hi - lo), down = bits > 13 ? bits - 13 : 0;
+        static_assert(kBins == 1 << 13, "steps of the logits' bits");
         clear(s);
-        all(r, [&](float l, int i) {
-            if (!in_group(l, i)) return;
-            const int at = static_cast<int>((hi - key_of(l)) >> down);
-            atomicAdd(&s.count[at], 1u);
-            if constexpr (MASS) atomicAdd(&s.mass[at], r.weight(l));
+        each(r, h, [&](const float (&l)[kChunk], int i) {
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e) {
+                if (!in_group(l[e], i + e * kWave)) continue;
+                atomicAdd(&s.mass[(hi - key_of(l[e])) >> down], mass ? r.weight(s, l[e]) : 1ull);
+            }
         });
         __syncthreads();
-        b = locate(s, MASS, target, before);
+        b = locate(s, target, before);
         target -= before;
-        n = s.count[b];
         hi -= static_cast<uint32_t>(b) << down;
         const uint32_t width = (1u << down) - 1;
         lo = hi - lo > width ? hi - width : lo;
+        n = gather(r, h, s, s.list, kList, in_group);
     }
+    if (tid < n) s.list_w[tid] = mass ? r.weight(s, s.list[tid].l) : 1;
+    sum_ahead(s, n, [&](int j, int i) { return ahead_of(s.list[j], s.list[i]); },
+              [&](int j) { return s.list_w[j]; });
+    if (tid < n && s.ahead[tid] < target && target <= s.ahead[tid] + s.list_w[tid]) s.bound = s.list[tid];
     __syncthreads();
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    all(r, [&](float l, int i) {
-        if (!in_group(l, i)) return;
-        const int at = atomicAdd(&s.n, 1);
-        s.list_l[at] = l;
-        s.list_i[at] = i;
-        if constexpr (MASS) s.list_w[at] = r.weight(l);
-    });
-    __syncthreads();
-    if (tid < n) {
-        const float l = s.list_l[tid];
-        const int i = s.list_i[tid];
-        u64 ahead = 0;
-        for (int j = 0; j < n; ++j)
-            if (s.list_l[j] > l || (s.list_l[j] == l && s.list_i[j] < i)) ahead += MASS ? s.list_w[j] : 1;
-        if (ahead < target && target <= ahead + (MASS ? s.list_w[tid] : 1)) {
-            s.bound_l = l;
-            s.bound_i = i;
-        }
-    }
-    __syncthreads();
-    r.bound_l = s.bound_l;
-    r.bound_i = s.bound_i;
+    r.bound = s.bound;
+}
+
+// The sum that the drawn token passes.
+__device__ __forceinline__ u64 draw_at(float u, u64 total) {
+    const double t = u > 0.0f ? static_cast<double>(u) * static_cast<double>(total) : 0.0;
+    return t < static_cast<double>(total) ? min(static_cast<u64>(t), total - 1) : total - 1;
 }
 
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) {
     __shared__ Lds s;
-    const int tid = threadIdx.x, w = tid / kWave, lane = tid & (kWave - 1);
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int row = blockIdx.x;
     Row r;
     r.logits = a.logits + static_cast<int64_t>(row) * a.V;
     r.V = a.V;
+    const int held = min(a.V, kHeld * kThreads);
+    int len = stretch(held);
+    r.from = min(w * len, held);
+    r.to = min(r.from + len, held);
+    r.chunks = (r.to - r.from + kChunk * kWave - 1) / (kChunk * kWave);
+    len = stretch(a.V - held);
+    r.rest_from = min(held + w * len, a.V);
+    r.rest_to = min(r.rest_from + len, a.V);
+    r.rest_chunks = (r.rest_to - r.rest_from + kChunk * kWave - 1) / (kChunk * kWave);
     const float *p = a.params + (a.param_rows > 1 ? 4 * row : 0);
-    float temperature = p[0];
-    const float top_k = p[1], top_p = p[2], min_p = p[3], u = a.u[row];
+    const float temperature = p[0], top_k = p[1], top_p = p[2], min_p = p[3], u = a.u[row];
+
+    Held h;
+#pragma unroll
+    for (int c = 0; c < kHeld / kChunk; ++c)
+        if (c < r.chunks)
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e) h[c][e] = r.logits[min(r.from + (c * kChunk + e) * kWave + lane, a.V - 1)];
+    if (tid < kTable) s.table[tid] = exp2(-tid / 256.0);
+#pragma unroll
+    for (int c = 0; c < kHeld / kChunk; ++c)
+        if (c < r.chunks)
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e)
+                h[c][e] = r.from + (c * kChunk + e) * kWave + lane < r.to ? Row::plain(h[c][e]) : -INFINITY;
 
     // The maximum and its first place.
-    float best = -INFINITY;
-    int where = a.V;
-    all(r, [&](float l, int i) {
-        if (l > best) {
-            best = l;
-            where = i;
-        }
+    Token best{-INFINITY, a.V};
+    each(r, h, [&](const float (&l)[kChunk], int i) {
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e)
+            if (l[e] > best.l) best = Token{l[e], i + e * kWave};
     });
+    const float own_max = best.l;
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) {
-        const float l = __shfl_xor(best, off, kWave);
-        const int i = __shfl_xor(where, off, kWave);
-        if (l > best || (l == best && i < where)) {
-            best = l;
-            where = i;
-        }
+        const Token o{__shfl_xor(best.l, off, kWave), __shfl_xor(best.i, off, kWave)};
+        if (ahead_of(o, best)) best = o;
     }
     if (lane == 0) {
-        s.wave_max[w] = best;
-        s.wave_idx[w] = where;
+        s.wave_max[w] = best.l;
+        s.wave_idx[w] = best.i;
     }
     __syncthreads();
-    best = s.wave_max[0];
-    where = s.wave_idx[0];
-    for (int i = 1; i < kWaves; ++i)  // stretches rise: an equal one later is further back
-        if (s.wave_max[i] > best) {
-            best = s.wave_max[i];
-            where = s.wave_idx[i];
-        }
-    if (best == -INFINITY || !(temperature > 0.0f)) {
-        if (tid == 0) {
-            const bool none = best == -INFINITY;
-            a.ids[row] = none ? -1.0f : static_cast<float>(where);
-            if (a.prob != nullptr) a.prob[row] = none ? 0.0f : 1.0f;
-        }
+    best = Token{s.wave_max[0], s.wave_idx[0]};
+    for (int i = 1; i < kWaves; ++i) {
+        const Token o{s.wave_max[i], s.wave_idx[i]};
+        if (ahead_of(o, best)) best = o;
+    }
+    auto answer = [&](int id, double prob) {
+        a.ids[row] = static_cast<float>(id);
+        if (a.prob != nullptr) a.prob[row] = static_cast<float>(prob);
+    };
+    if (best.l == -INFINITY || !(temperature > 0.0f)) {
+        if (tid == 0) answer(best.l == -INFINITY ? -1 : best.i, best.l == -INFINITY ? 0.0 : 1.0);
         return;
     }
-    r.M = best;
-    temperature = fminf(temperature, 1e30f);
-    r.inv_t = 1.0 / static_cast<double>(temperature);
-    r.limit = (a.shift + 2) * 0.6931471805599453;
-    r.limit_f = static_cast<float>(r.limit) * 1.001f;
-    r.inv_t_f = static_cast<float>(r.inv_t);
-    r.bin_scale = kBins / r.limit_f;
-    r.one = static_cast<double>(1ull << a.shift);
-    r.bound_l = -INFINITY;
-    r.bound_i = a.V;
-    r.min_w = min_p > 0.0f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * r.one)) : 1;
+    const double inv_t = 1.0 / static_cast<double>(fminf(temperature, 1e30f));
+    r.M = best.l;
+    r.shift = a.shift;
+    r.per_256 = inv_t * (256 * 1.4426950408889634);
+    r.limit = 256.0 * (a.shift + 2);
+    r.inv_t = static_cast<float>(inv_t);
+    r.z_limit = (a.shift + 2) * 0.6931471805599453f * 1.001f;
+    r.bin_scale = kBins / r.z_limit;
+    r.bound = Token{-INFINITY, -1};
+    const double one = static_cast<double>(1ull << a.shift);
+    r.min_w = min_p > 0.0f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * one)) : 1;
+    const bool by_k = top_k >= 1.0f && top_k < static_cast<float>(a.V), by_p = top_p < 1.0f;
+    const double share = fmax(static_cast<double>(top_p), 0.0);
 
-    if (top_k >= 1.0f && top_k < static_cast<float>(a.V)) bound_at<false>(r, s, static_cast<u64>(top_k), 0.0);
-    if (top_p < 1.0f) bound_at<true>(r, s, 0, fmax(static_cast<double>(top_p), 0.0));
-
-    u64 weight, total;
-    const int id = pick(r, s,
-                        [&](float l, int i) -> u64 {
-                            if (!r.kept(l, i) || r.bin(l) < 0) return 0;
-                            const u64 x = r.weight(l);
-                            return x >= r.min_w ? x : 0;
-                        },
-                        [&](u64 sum) {
-                            const double t = u > 0.0f ? static_cast<double>(u) * static_cast<double>(sum) : 0.0;
-                            return t < static_cast<double>(sum) ? min(static_cast<u64>(t), sum - 1) : sum - 1;
-                        },
-                        weight, total);
-    if (tid == 0) {
-        a.ids[row] = static_cast<float>(id);
-        if (a.prob != nullptr) a.prob[row] = static_cast<float>(static_cast<double>(weight) / static_cast<double>(total));
+    if (by_k) {
+        const u64 k = static_cast<u64>(top_k);
+        int n = kList + 1;
+        if (k <= kList) {
+            clear(s);
+            const int b = r.bin(own_max);
+            if (b >= 0) atomicAdd(&s.mass[b], 1ull);
+            __syncthreads();
+            u64 before;
+            const int last = locate(s, k, before);
+            if (last >= 0) {
+                // The smallest of the maxima that were counted.
+                const float least = -wave_max(b >= 0 && b <= last ? -own_max : -INFINITY);
+                if (lane == 0) s.wave_max[w] = least;
+                __syncthreads();
+                float bound = s.wave_max[0];
+                for (int i = 1; i < kWaves; ++i) bound = fminf(bound, s.wave_max[i]);
+                n = gather(r, h, s, s.list, kList, [&](float l, int) { return l >= bound; });
+            }
+        }
+        if (n <= kList) {
+            // All that counts is in the list: rank it, cut it, draw from it.
+            auto before = [&](int j, int i) { return ahead_of(s.list[j], s.list[i]); };
+            sum_ahead(s, n, before, [](int) { return 1ull; });
+            Token mine{};
+            int rank = kList;
+            if (tid < n) {
+                mine = s.list[tid];
+                rank = static_cast<int>(s.ahead[tid]);
+            }
+            __syncthreads();
+            if (rank < static_cast<int>(k)) s.list[rank] = mine;
+            __syncthreads();
+            n = static_cast<int>(k);
+            u64 weight = 0, upto;
+            if (tid < n) {
+                mine = s.list[tid];
+                weight = r.weight(s, mine.l);
+            }
+            const u64 all = block_sum64(s, weight, &upto);
+            if (by_p && upto - weight >= head_of(share, all)) weight = 0;
+            if (weight < r.min_w) weight = 0;
+            const u64 total = block_sum64(s, weight);
+            if (tid < n) s.list_w[tid] = weight;
+            sum_ahead(s, n, [&](int j, int i) { return s.list[j].i < s.list[i].i; }, [&](int j) { return s.list_w[j]; });
+            const u64 at = draw_at(u, total);
+            if (tid < n && weight != 0 && s.ahead[tid] <= at && at < s.ahead[tid] + weight)
+                answer(mine.i, static_cast<double>(weight) / static_cast<double>(total));
+            return;
+        }
     }
+#pragma unroll 1
+    for (int mass = by_k ? 0 : 1; mass < (by_p ? 2 : 1); ++mass)
+        bound_at(r, h, s, mass != 0, mass != 0 ? 0 : static_cast<u64>(top_k), share);
+
+    auto weigh = [&](float l, int i) -> u64 {
+        if (!r.kept(l, i) || r.bin(l) < 0) return 0;
+        const u64 x = r.weight(s, l);
+        return x >= r.min_w ? x : 0;
+    };
+    if (by_k || by_p || min_p > 0.0f) {
+        // The kept tokens, where they are few.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
+        const float z_most = min_p > 0.0f ? fmaxf(-logf(min_p), 0.0f) * 1.0001f + 1e-4f : INFINITY;
+        const int n = gather(r, h, s, s.kept, kBins, [&](float l, int) {
+            const float z = l == r.M ? 0.0f : (r.M - l) * r.inv_t;
+            return l >= r.bound.l && z < r.z_limit && z <= z_most;
+        });
+        if (n <= kBins) {
+            const int per = (a.V + kList - 1) / kList;
+            s.ahead[tid] = 0;
+            __syncthreads();
+            for (int j = tid; j < n; j += kThreads) {
+                const Token t = s.kept[j];
+                atomicAdd(&s.ahead[t.i / per], weigh(t.l, t.i));
+            }
+            __syncthreads();
+            const u64 weight = s.ahead[tid];
+            u64 upto;
+            const u64 total = block_sum64(s, weight, &upto), at = draw_at(u, total);
+            if (upto - weight <= at && at < upto) {
+                s.found = tid;
+                s.before = upto - weight;
+            }
+            if (tid == 0) s.n = 0;
+            __syncthreads();
+            const int found = s.found;
+            const u64 left = at - s.before;
+            for (int j = tid; j < n; j += kThreads) {
+                const Token t = s.kept[j];
+                if (t.i / per != found) continue;
+                const u64 x = weigh(t.l, t.i);
+                if (x == 0) continue;
+                const int m = atomicAdd(&s.n, 1);
+                if (m < kList) {
+                    s.list[m] = t;
+                    s.list_w[m] = x;
+                }
+            }
+            __syncthreads();
+            const int m = s.n;
+            if (m <= kList) {
+                sum_ahead(s, m, [&](int j, int i) { return s.list[j].i < s.list[i].i; }, [&](int j) { return s.list_w[j]; });
+                if (tid < m && s.ahead[tid] <= left && left < s.ahead[tid] + s.list_w[tid])
+                    answer(s.list[tid].i, static_cast<double>(s.list_w[tid]) / static_cast<double>(total));
+                return;
+            }
+        }
+    }
+    u64 weight, total;
+    const int id = pick(r, h, s, weigh, [&](u64 sum) { return draw_at(u, sum); }, weight, total);
+    if (tid == 0) answer(id, static_cast<double>(weight) / static_cast<double>(total));
 }
 
 }  // namespace
