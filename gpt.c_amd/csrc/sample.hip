@@ -12,12 +12,12 @@
 // floats, and every sum of them is a 64-bit integer, the same in any order (atomics too).  shift leaves room for a
 // whole vocabulary (46 bits at 50257 tokens: a weight is off by at most 2^-47 of the largest).
 //
-// A workgroup takes a row, and holds its first 57344 logits in registers, so that they are read once (the rest is
+// A workgroup takes a row, and holds its first 49152 logits in registers, so that they are read once (the rest is
 // read again by each pass).  Nothing is sorted:
 //   top-k   the k-th largest of the threads' own maxima is a lower bound of the k-th logit, and few tokens lie
 //           above it: they are ranked by counting, and the rest of the work is theirs alone.
 //   else    a bound is found in histograms: over 8192 steps of (M - l) / T first, then over the bits of the logits
-//           in the one step where the bound lies, until it holds at most 1024 tokens, which are ranked, or equal
+//           in the one step where the bound lies, until it holds at most 512 tokens, which are ranked, or equal
 //           logits only, whose order is that of the vocabulary.  The kept tokens are then gathered, and the draw
 //           finds the stretch of the vocabulary where the sum is passed, and the token in it.
 #include <hip/hip_runtime.h>
@@ -30,13 +30,14 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kChunk = 8;            // logits of a thread that are handled together
-constexpr int kHeld = 56;            // logits of a thread that stay in registers
+constexpr int kChunk = 8;            // logits of a thread whose weights are formed side by side
+constexpr int kMask = 24;            // logits of a thread that are looked through together
+constexpr int kHeld = 4 * kMask;     // logits of a thread that stay in registers
 constexpr int kBins = 8192;          // of a histogram; tokens that can be gathered
 constexpr int kList = kThreads;      // tokens that can be ranked
-constexpr int kTable = 256;
+constexpr int kTable = 2048;
 
 struct SampleParams {
     const float *logits, *params, *u;
@@ -57,7 +58,7 @@ struct Lds {
     Token list[kList];
     u64 list_w[kList];
     u64 ahead[kList];
-    double table[kTable];  // 2^(-j / 256)
+    double table[kTable];  // 2^(-j / 2048)
     u64 wave_sum[2 * kWaves];
     float wave_max[kWaves];
     int wave_idx[kWaves];
@@ -67,31 +68,40 @@ struct Lds {
     Token bound;
 };
 
-// Order-preserving bits of a float that is no NaN, and back.
+// Order-preserving bits of a float that is no NaN (-0 counts as 0), and back.
 __device__ __forceinline__ uint32_t key_of(float l) {
-    const uint32_t b = __float_as_uint(l);
+    const uint32_t b = __float_as_uint(l + 0.0f);
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-    return v;
+template <int kCtrl, int kRows>
+__device__ __forceinline__ u64 dpp64(u64 v) {  // 0 where the control has no lane to read, or the row is not written
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), kCtrl, kRows, 0xf, false);
+    return static_cast<u64>(hi) << 32 | lo;
 }
 
-// Inclusive sums over the lanes.
+// Inclusive sums over the lanes: within rows of 16 (shifts by 1, 2, 4 and 8), then the last lane of a row added to
+// the next row, and that of the lower half to the upper.
 __device__ __forceinline__ u64 wave_scan64(u64 v) {
-    const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const u64 o = __shfl_up(v, off, kWave);
-        if (lane >= off) v += o;
-    }
-    return v;
+    v += dpp64<0x111, 0xf>(v);
+    v += dpp64<0x112, 0xf>(v);
+    v += dpp64<0x114, 0xf>(v);
+    v += dpp64<0x118, 0xf>(v);
+    v += dpp64<0x142, 0xa>(v);
+    return v + dpp64<0x143, 0xc>(v);
 }
+
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+    return static_cast<u64>(hi) << 32 | lo;
+}
+
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return lane_of(wave_scan64(v), kWave - 1); }
 
 // The sum over the workgroup (every thread gets it), and with `upto` the inclusive sums by thread.
 __device__ __forceinline__ u64 block_sum64(Lds &s, u64 v, u64 *upto = nullptr) {
@@ -114,112 +124,128 @@ __device__ __forceinline__ u64 block_sum64(Lds &s, u64 v, u64 *upto = nullptr) {
 struct Row {
     const float *logits;
     int V;
-    int from, to, chunks;    // the wave's stretch of the held logits, and its chunks
-    int rest_from, rest_to, rest_chunks;  // and of the others
+    int from, to;            // the wave's stretch of the held logits
+    int rest_from, rest_to;  // and of the others
     float M;
-    double per_256;  // log2(e) 256 / T: the weight is 2^(-(M - l) per_256 / 256)
-    double limit;    // of that exponent: from here on a weight rounds to nothing
+    double per_entry;  // the weight is 2^(-(M - l) per_entry / kTable)
     int shift;
-    float inv_t, z_limit, bin_scale;  // the histogram's steps: monotone in the logit, whatever their rounding
+    float per_step;  // the histogram's steps by logit: monotone, whatever their rounding
     Token bound;
     u64 min_w;
 
-    // NaN counts as -inf, and -0 as 0: equal logits have equal bits.
-    static __device__ __forceinline__ float plain(float l) { return fmaxf(l, -INFINITY) + 0.0f; }
+    // NaN counts as -inf, and +inf as the largest number.
+    static __device__ __forceinline__ float plain(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f); }
 
-    __device__ __forceinline__ bool kept(float l, int i) const { return l > bound.l || (l == bound.l && i <= bound.i); }
+    // What follows has no branches: the chains of a chunk's logits run side by side.
+    __device__ __forceinline__ bool kept(float l, int i) const { return (l > bound.l) | ((l == bound.l) & (i <= bound.i)); }
 
-    // The exponent in steps of 1/256: a table's entry, and four terms of the exponential series for the rest (at
-    // most ln 2 / 512: the next term is below 2^-54).  The whole number comes out of the addition of 2^52.
+    // Where the logit lies in the histogram: kBins and more where the weight is nothing, 0 where the difference is 0
+    // and the scale infinite (a vanishing temperature).
+    __device__ __forceinline__ float step(float l) const { return fmaxf((M - l) * per_step, 0.0f); }
+
+    // Where step(l) < kBins.  The exponent in steps of 1/2048: a table's entry, and two terms of the exponential
+    // series for the rest (at most ln 2 / 4096: the next is below 2^-39 of the weight).  Whole numbers come out of
+    // additions of 2^52, or 1.5 times that.
     __device__ __forceinline__ u64 weight(const Lds &s, float l) const {
-        if (l == M) return 1ull << shift;
-        const double t = (static_cast<double>(M) - static_cast<double>(l)) * per_256;
-        if (!(t < limit)) return 0;
-        const double n = rint(t), x = (n - t) * (0.6931471805599453 / 256);
-        const int e = static_cast<int>(n);
-        const double p = fma(x, fma(x, fma(x, fma(x, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * s.table[e & (kTable - 1)];
-        const double scale = __longlong_as_double(static_cast<long long>(1023 + shift - (e >> 8)) << 52);
+        static_assert(kTable == 1 << 11, "the shift below");
+        constexpr double kWhole = 6755399441055744.0, kLn = 0.6931471805599453 / kTable;
+        const double t = (static_cast<double>(M) - static_cast<double>(l)) * per_entry;
+        const double n = t + kWhole, x = (n - kWhole) - t;
+        const int e = static_cast<int>(__double_as_longlong(n));
+        const double p = fma(x, fma(x, kLn * kLn / 2, kLn), 1.0) * s.table[e & (kTable - 1)];
+        const double scale = __hiloint2double((1023 + shift - (e >> 11)) << 20, 0);
         return static_cast<u64>(__double_as_longlong(fma(p, scale, 4503599627370496.0))) & ((1ull << 52) - 1);
     }
 
-    // The histogram's step, or -1 where the weight is nothing.
-    __device__ __forceinline__ int bin(float l) const {
-        const float z = l == M ? 0.0f : (M - l) * inv_t;
-        return z < z_limit ? min(static_cast<int>(z * bin_scale), kBins - 1) : -1;
-    }
-
-    __device__ __forceinline__ void load_chunk(float (&l)[kChunk], int i0, int end) const {
+    // Tokens i0 + lane + 64 e; -inf from `end` on.
+    template <int N>
+    __device__ __forceinline__ void load(float (&l)[N], int i0, int lane, int end) const {
+        if (i0 + N * kWave <= end) {
+            const float *at = logits + i0 + lane;
 #pragma unroll
-        for (int e = 0; e < kChunk; ++e) l[e] = logits[min(i0 + e * kWave, V - 1)];  // all requested before one is used
+            for (int e = 0; e < N; ++e) l[e] = at[e * kWave];
 #pragma unroll
-        for (int e = 0; e < kChunk; ++e) l[e] = i0 + e * kWave < end ? plain(l[e]) : -INFINITY;
+            for (int e = 0; e < N; ++e) l[e] = plain(l[e]);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) l[e] = logits[min(i0 + lane + e * kWave, V - 1)];
+#pragma unroll
+        for (int e = 0; e < N; ++e) l[e] = i0 + lane + e * kWave < end ? plain(l[e]) : -INFINITY;
     }
 };
 
 // A wave's share of n tokens: contiguous, in whole turns of its lanes.
 __device__ __forceinline__ int stretch(int n) { return (n + kThreads - 1) / kThreads * kWave; }
 
-typedef float Held[kHeld / kChunk][kChunk];
+typedef float Held[kHeld / kMask][kMask];
 
-// f(chunk, i) for each of the wave's chunks: chunk[e] is the logit of token i + 64 e, -inf past the stretch's end.
-// The loop stays a loop, and a switch copies a held chunk's registers: passes written out for every chunk are more
-// code than the instruction cache holds, and take registers.
+// f(l, i) over the wave's logits: l[e] is that of token i + 64 e, -inf past the stretch's end.  For what takes a few
+// instructions a logit: it is written out for every register.
 template <typename F>
-__device__ __forceinline__ void each(const Row &r, const Held &h, F f) {
-    static_assert(kHeld / kChunk == 7, "the cases below");
+__device__ __forceinline__ void each_held(const Row &r, const Held &h, F f) {
     const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll 1
-    for (int c = 0; c < r.chunks + r.rest_chunks; ++c) {
-        float l[kChunk];
-        auto take = [&](const float (&x)[kChunk]) {
 #pragma unroll
-            for (int e = 0; e < kChunk; ++e) l[e] = x[e];
-        };
-        const bool rest = c >= r.chunks;
-        const int i = (rest ? r.rest_from + (c - r.chunks) * kChunk * kWave : r.from + c * kChunk * kWave) + lane;
-        switch (!rest ? c : 7) {
-            case 0: take(h[0]); break;
-            case 1: take(h[1]); break;
-            case 2: take(h[2]); break;
-            case 3: take(h[3]); break;
-            case 4: take(h[4]); break;
-            case 5: take(h[5]); break;
-            case 6: take(h[6]); break;
-            default: r.load_chunk(l, i, rest ? r.rest_to : r.to); break;
-        }
-        f(l, i);
+    for (int c = 0; c < kHeld / kMask; ++c)
+        if (r.from + c * kMask * kWave < r.to) f(h[c], r.from + c * kMask * kWave + lane);
+#pragma unroll 1
+    for (int i = r.rest_from; i < r.rest_to; i += kMask * kWave) {
+        float l[kMask];
+        r.load(l, i, lane, r.rest_to);
+        f(l, i + lane);
     }
 }
 
-// Gathers the tokens for which want(l, i); returns how many there are, of which the first `room` were written.
-// Their order is that of the waves' turns, so nothing may depend on it.
+// The same in chunks that are read again, the next one while this one is worked on: for what takes many instructions
+// (written out for every register, the weights alone are more code than the instruction cache holds).
+template <typename F>
+__device__ __forceinline__ void each_again(const Row &r, int from, int to, F f) {
+    const int lane = threadIdx.x & (kWave - 1);
+    float l[kChunk], next[kChunk];
+    if (from < to) r.load(l, from, lane, to);
+#pragma unroll 1
+    for (int i = from; i < to; i += kChunk * kWave) {
+        r.load(next, i + kChunk * kWave, lane, to);
+        f(l, i + lane);
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) l[e] = next[e];
+    }
+}
+
+template <typename F>
+__device__ __forceinline__ void each_again(const Row &r, F f) {
+    for (int half = 0; half < 2; ++half) each_again(r, half ? r.rest_from : r.from, half ? r.rest_to : r.to, f);
+}
+
+// Gathers the tokens for which want(l); returns how many there are, of which the first `room` were written.  Their
+// order is that of the waves' turns, so nothing may depend on it.  A token that the bound leaves out by its index
+// alone is written as one of no weight.
 template <typename F>
 __device__ __forceinline__ int gather(const Row &r, const Held &h, Lds &s, Token *to, int room, F want) {
-    const u64 below = (1ull << (threadIdx.x & (kWave - 1))) - 1;
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    each(r, h, [&](const float (&l)[kChunk], int i) {
-        u64 who[kChunk];
-        int count = 0;
+    each_held(r, h, [&](const float (&l)[kMask], int i) {
+        uint32_t mask = 0;
 #pragma unroll
-        for (int e = 0; e < kChunk; ++e) {
-            who[e] = __ballot(want(l[e], i + e * kWave));
-            count += __popcll(who[e]);
-        }
-        if (count == 0) return;
-        int at = 0;
-        if (below == 0) at = atomicAdd(&s.n, count);
-        at = __builtin_amdgcn_readfirstlane(at);
-#pragma unroll
-        for (int e = 0; e < kChunk; ++e) {
-            const int mine = at + __popcll(who[e] & below);
-            if ((who[e] & (below + 1)) != 0 && mine < room) to[mine] = Token{l[e], i + e * kWave};
-            at += __popcll(who[e]);
+        for (int e = 0; e < kMask; ++e) mask |= want(l[e]) ? 1u << e : 0u;
+        if (mask == 0) return;
+        int at = atomicAdd(&s.n, __popc(mask));
+        while (mask != 0) {
+            if (at < room) to[at].i = i + (__ffs(mask) - 1) * kWave;
+            ++at;
+            mask &= mask - 1;
         }
     });
     __syncthreads();
-    return s.n;
+    const int n = s.n;
+    for (int j = threadIdx.x; j < min(n, room); j += kThreads) {  // the registers cannot be indexed: read again
+        const int i = to[j].i;
+        const float l = Row::plain(r.logits[i]);
+        to[j].l = r.kept(l, i) ? l : -INFINITY;
+    }
+    __syncthreads();
+    return n;
 }
 
 // ahead[i] = the sum over j < n of value(j) where before(j, i), for i < n <= kList: the pairs are shared out over
@@ -288,22 +314,19 @@ __device__ __forceinline__ void clear(Lds &s) {
 // The first token, in the order of the vocabulary, at which the sum of weigh(l, i) passes target(total); its
 // weight, and the total.  Stretches first, then stretches of the one it lies in, then its tokens.
 template <typename W, typename T>
-__device__ __forceinline__ int pick(const Row &r, const Held &h, Lds &s, W weigh, T target, u64 &weight, u64 &total) {
+__device__ __forceinline__ int pick(const Row &r, Lds &s, W weigh, T target, u64 &weight, u64 &total) {
     const int w = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
     auto sum_of = [&](int from, int to) {
         u64 sum = 0;
-#pragma unroll 1
-        for (int i = from + lane; i < to + (kWave - 1); i += kChunk * kWave) {
-            float l[kChunk];
-            r.load_chunk(l, i, to);
+        each_again(r, from, to, [&](const float (&l)[kChunk], int i) {
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) sum += weigh(l[e], i + e * kWave);
-        }
-        return wave_sum64(sum);
+        });
+        return sum;
     };
     const int held = min(r.V, kHeld * kThreads);
     u64 first = 0, second = 0;
-    each(r, h, [&](const float (&l)[kChunk], int i) {
+    each_again(r, [&](const float (&l)[kChunk], int i) {
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < kChunk; ++e) sum += weigh(l[e], i + e * kWave);
@@ -328,7 +351,7 @@ __device__ __forceinline__ int pick(const Row &r, const Held &h, Lds &s, W weigh
     while (hi - lo > kChunk * kWave) {
         len = stretch(hi - lo);
         const int a = min(lo + w * len, hi);
-        const u64 sum = sum_of(a, min(a + len, hi));
+        const u64 sum = wave_sum64(sum_of(a, min(a + len, hi)));
         __syncthreads();
         if (lane == 0) s.wave_sum[w] = sum;
         __syncthreads();
@@ -339,17 +362,17 @@ __device__ __forceinline__ int pick(const Row &r, const Held &h, Lds &s, W weigh
     }
     // Every wave does the last part, so that all end with the token.
     float l[kChunk];
-    r.load_chunk(l, lo + lane, hi);
+    r.load(l, lo, lane, hi);
 #pragma unroll
     for (int e = 0; e < kChunk; ++e) {
         const u64 mine = weigh(l[e], lo + e * kWave + lane), over_all = wave_scan64(mine);
         const u64 over = __ballot(over_all > left);
         if (over != 0) {
             const int at = __ffsll(over) - 1;
-            weight = __shfl(mine, at, kWave);
+            weight = lane_of(mine, at);
             return lo + e * kWave + at;
         }
-        left -= __shfl(over_all, kWave - 1, kWave);
+        left -= lane_of(over_all, kWave - 1);
     }
     weight = 0;
     return max(hi - 1, 0);  // not reached while target < total
@@ -362,15 +385,25 @@ __device__ __forceinline__ u64 head_of(double share, u64 total) {
     return want < 1.0 ? 1 : min(static_cast<u64>(want), total);
 }
 
-__device__ __forceinline__ void bound_at(Row &r, const Held &h, Lds &s, bool mass, u64 target, double share) {
+//
+// Returns how many tokens were gathered into s.kept on the way, all that are kept among them, or kBins + 1.
+__device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass, u64 target, double share) {
     const int tid = threadIdx.x;
     clear(s);
-    each(r, h, [&](const float (&l)[kChunk], int i) {
+    const bool all = r.bound.l == -INFINITY;
+    each_again(r, [&](const float (&l)[kChunk], int i) {
+        u64 w[kChunk];
+        if (mass) {
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e) w[e] = r.weight(s, l[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e) w[e] = 1;
+        }
 #pragma unroll
         for (int e = 0; e < kChunk; ++e) {
-            const int b = r.bin(l[e]);
-            if (b < 0 || !r.kept(l[e], i + e * kWave)) continue;
-            atomicAdd(&s.mass[b], mass ? r.weight(s, l[e]) : 1ull);
+            const float at = r.step(l[e]);
+            if (at < kBins && (all || r.kept(l[e], i + e * kWave))) atomicAdd(&s.mass[static_cast<int>(at)], w[e]);
         }
     });
     __syncthreads();
@@ -382,16 +415,30 @@ __device__ __forceinline__ void bound_at(Row &r, const Held &h, Lds &s, bool mas
     }
     u64 before;
     int b = locate(s, target, before);
-    if (b < 0) return;  // fewer tokens than that have any weight
+    if (b < 0) return kBins + 1;  // fewer tokens than that have any weight
     target -= before;
-    int n = gather(r, h, s, s.list, kList, [&](float l, int i) { return r.bin(l) == b && r.kept(l, i); });
-    bool first = true;
+    // The tokens up to that step, and in it.
+    const float from = static_cast<float>(b), upto = static_cast<float>(b + 1);
+    const int kept = gather(r, h, s, s.kept, kBins, [&](float l) { return (r.step(l) < upto) & (l >= r.bound.l); });
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    if (kept <= kBins)
+        for (int j = tid; j < kept; j += kThreads) {
+            const Token t = s.kept[j];
+            if (!(r.step(t.l) >= from)) continue;
+            const int m = atomicAdd(&s.n, 1);
+            if (m < kList) s.list[m] = t;
+        }
+    __syncthreads();
+    int n = kept <= kBins ? s.n : gather(r, h, s, s.list, kList, [&](float l) {
+        const float at = r.step(l);
+        return (at >= from) & (at < upto) & (l >= r.bound.l);
+    });
+    bool first = true;  // and s.kept still holds the tokens
     uint32_t lo = 0, hi = 0;
     auto in_group = [&](float l, int i) {
-        if (!r.kept(l, i)) return false;
-        if (first) return r.bin(l) == b;
         const uint32_t k = key_of(l);
-        return k >= lo && k <= hi;
+        return r.kept(l, i) && (first ? static_cast<int>(r.step(l)) == b : k >= lo && k <= hi);
     };
     while (n > kList) {
         // The logits that the step holds; then its steps of them.
@@ -402,7 +449,7 @@ __device__ __forceinline__ void bound_at(Row &r, const Held &h, Lds &s, bool mas
         }
         __syncthreads();
         uint32_t k0 = 0xffffffffu, k1 = 0;
-        each(r, h, [&](const float (&l)[kChunk], int i) {
+        each_again(r, [&](const float (&l)[kChunk], int i) {
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) {
                 if (!in_group(l[e], i + e * kWave)) continue;
@@ -423,15 +470,15 @@ __device__ __forceinline__ void bound_at(Row &r, const Held &h, Lds &s, bool mas
                 target = (target + w - 1) / w;
             }
             u64 weight, total;
-            const int i = pick(r, h, s, [&](float x, int j) { return static_cast<u64>(in_group(x, j)); },
+            const int i = pick(r, s, [&](float x, int j) { return static_cast<u64>(in_group(x, j)); },
                                [&](u64) { return target - 1; }, weight, total);
             r.bound = Token{l, i};
-            return;
+            return kBins + 1;  // the list made room for the histogram
         }
         const int bits = 32 - __clz(hi - lo), down = bits > 13 ? bits - 13 : 0;
         static_assert(kBins == 1 << 13, "steps of the logits' bits");
         clear(s);
-        each(r, h, [&](const float (&l)[kChunk], int i) {
+        each_again(r, [&](const float (&l)[kChunk], int i) {
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) {
                 if (!in_group(l[e], i + e * kWave)) continue;
@@ -444,14 +491,16 @@ __device__ __forceinline__ void bound_at(Row &r, const Held &h, Lds &s, bool mas
         hi -= static_cast<uint32_t>(b) << down;
         const uint32_t width = (1u << down) - 1;
         lo = hi - lo > width ? hi - width : lo;
-        n = gather(r, h, s, s.list, kList, in_group);
+        const float least = of_key(lo), most = of_key(hi);
+        n = gather(r, h, s, s.list, kList, [&](float l) { return (l >= least) & (l <= most) & (l >= r.bound.l); });
     }
-    if (tid < n) s.list_w[tid] = mass ? r.weight(s, s.list[tid].l) : 1;
+    if (tid < n) s.list_w[tid] = !mass ? 1 : r.step(s.list[tid].l) < kBins ? r.weight(s, s.list[tid].l) : 0;
     sum_ahead(s, n, [&](int j, int i) { return ahead_of(s.list[j], s.list[i]); },
               [&](int j) { return s.list_w[j]; });
     if (tid < n && s.ahead[tid] < target && target <= s.ahead[tid] + s.list_w[tid]) s.bound = s.list[tid];
     __syncthreads();
     r.bound = s.bound;
+    return first ? kept : kBins + 1;
 }
 
 // The sum that the drawn token passes.
@@ -471,41 +520,41 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
     int len = stretch(held);
     r.from = min(w * len, held);
     r.to = min(r.from + len, held);
-    r.chunks = (r.to - r.from + kChunk * kWave - 1) / (kChunk * kWave);
     len = stretch(a.V - held);
     r.rest_from = min(held + w * len, a.V);
     r.rest_to = min(r.rest_from + len, a.V);
-    r.rest_chunks = (r.rest_to - r.rest_from + kChunk * kWave - 1) / (kChunk * kWave);
     const float *p = a.params + (a.param_rows > 1 ? 4 * row : 0);
     const float temperature = p[0], top_k = p[1], top_p = p[2], min_p = p[3], u = a.u[row];
 
     Held h;
 #pragma unroll
-    for (int c = 0; c < kHeld / kChunk; ++c)
-        if (c < r.chunks)
+    for (int c = 0; c < kHeld / kMask; ++c)
+        if (r.from + c * kMask * kWave < r.to)
 #pragma unroll
-            for (int e = 0; e < kChunk; ++e) h[c][e] = r.logits[min(r.from + (c * kChunk + e) * kWave + lane, a.V - 1)];
-    if (tid < kTable) s.table[tid] = exp2(-tid / 256.0);
+            for (int e = 0; e < kMask; ++e) h[c][e] = r.logits[min(r.from + (c * kMask + e) * kWave + lane, a.V - 1)];
+    static_assert(kTable == 4 * kThreads, "the quarters below");
+    const double root = exp2(-tid / static_cast<double>(kTable));
+    s.table[tid] = root;
+    s.table[tid + kThreads] = root * 0.8408964152537145;      // 2^(-1/4)
+    s.table[tid + 2 * kThreads] = root * 0.7071067811865476;  // 2^(-1/2)
+    s.table[tid + 3 * kThreads] = root * 0.5946035575013605;  // 2^(-3/4)
 #pragma unroll
-    for (int c = 0; c < kHeld / kChunk; ++c)
-        if (c < r.chunks)
+    for (int c = 0; c < kHeld / kMask; ++c)
+        if (r.from + c * kMask * kWave < r.to)
 #pragma unroll
-            for (int e = 0; e < kChunk; ++e)
-                h[c][e] = r.from + (c * kChunk + e) * kWave + lane < r.to ? Row::plain(h[c][e]) : -INFINITY;
+            for (int e = 0; e < kMask; ++e)
+                h[c][e] = r.from + (c * kMask + e) * kWave + lane < r.to ? Row::plain(h[c][e]) : -INFINITY;
 
     // The maximum and its first place.
     Token best{-INFINITY, a.V};
-    each(r, h, [&](const float (&l)[kChunk], int i) {
+    each_held(r, h, [&](const float (&l)[kMask], int i) {
 #pragma unroll
-        for (int e = 0; e < kChunk; ++e)
+        for (int e = 0; e < kMask; ++e)
             if (l[e] > best.l) best = Token{l[e], i + e * kWave};
     });
     const float own_max = best.l;
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-        const Token o{__shfl_xor(best.l, off, kWave), __shfl_xor(best.i, off, kWave)};
-        if (ahead_of(o, best)) best = o;
-    }
+    const float top = wave_max(best.l);  // V <= 2^24: indices are floats too
+    best = Token{top, static_cast<int>(-wave_max(best.l == top ? -static_cast<float>(best.i) : -INFINITY))};
     if (lane == 0) {
         s.wave_max[w] = best.l;
         s.wave_idx[w] = best.i;
@@ -527,11 +576,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
     const double inv_t = 1.0 / static_cast<double>(fminf(temperature, 1e30f));
     r.M = best.l;
     r.shift = a.shift;
-    r.per_256 = inv_t * (256 * 1.4426950408889634);
-    r.limit = 256.0 * (a.shift + 2);
-    r.inv_t = static_cast<float>(inv_t);
-    r.z_limit = (a.shift + 2) * 0.6931471805599453f * 1.001f;
-    r.bin_scale = kBins / r.z_limit;
+    r.per_entry = inv_t * (kTable * 1.4426950408889634);
+    r.per_step = static_cast<float>(inv_t * (kBins / ((a.shift + 2) * 0.6931471805599453 * 1.001)));
     r.bound = Token{-INFINITY, -1};
     const double one = static_cast<double>(1ull << a.shift);
     r.min_w = min_p > 0.0f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * one)) : 1;
@@ -543,19 +589,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         int n = kList + 1;
         if (k <= kList) {
             clear(s);
-            const int b = r.bin(own_max);
-            if (b >= 0) atomicAdd(&s.mass[b], 1ull);
+            const float own = r.step(own_max);
+            if (own < kBins) atomicAdd(&s.mass[static_cast<int>(own)], 1ull);
             __syncthreads();
             u64 before;
             const int last = locate(s, k, before);
             if (last >= 0) {
                 // The smallest of the maxima that were counted.
-                const float least = -wave_max(b >= 0 && b <= last ? -own_max : -INFINITY);
+                const float least = -wave_max(own < static_cast<float>(last + 1) ? -own_max : -INFINITY);
                 if (lane == 0) s.wave_max[w] = least;
                 __syncthreads();
                 float bound = s.wave_max[0];
                 for (int i = 1; i < kWaves; ++i) bound = fminf(bound, s.wave_max[i]);
-                n = gather(r, h, s, s.list, kList, [&](float l, int) { return l >= bound; });
+                n = gather(r, h, s, s.list, kList, [&](float l) { return l >= bound; });
             }
         }
         if (n <= kList) {
@@ -575,7 +621,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
             u64 weight = 0, upto;
             if (tid < n) {
                 mine = s.list[tid];
-                weight = r.weight(s, mine.l);
+                weight = r.step(mine.l) < kBins ? r.weight(s, mine.l) : 0;
             }
             const u64 all = block_sum64(s, weight, &upto);
             if (by_p && upto - weight >= head_of(share, all)) weight = 0;
@@ -589,22 +635,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
             return;
         }
     }
+    int n = kBins + 1;
 #pragma unroll 1
     for (int mass = by_k ? 0 : 1; mass < (by_p ? 2 : 1); ++mass)
-        bound_at(r, h, s, mass != 0, mass != 0 ? 0 : static_cast<u64>(top_k), share);
+        n = bound_at(r, h, s, mass != 0, mass != 0 ? 0 : static_cast<u64>(top_k), share);
 
     auto weigh = [&](float l, int i) -> u64 {
-        if (!r.kept(l, i) || r.bin(l) < 0) return 0;
         const u64 x = r.weight(s, l);
-        return x >= r.min_w ? x : 0;
+        return r.kept(l, i) && r.step(l) < kBins && x >= r.min_w ? x : 0;
     };
     if (by_k || by_p || min_p > 0.0f) {
-        // The kept tokens, where they are few.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
-        const float z_most = min_p > 0.0f ? fmaxf(-logf(min_p), 0.0f) * 1.0001f + 1e-4f : INFINITY;
-        const int n = gather(r, h, s, s.kept, kBins, [&](float l, int) {
-            const float z = l == r.M ? 0.0f : (r.M - l) * r.inv_t;
-            return l >= r.bound.l && z < r.z_limit && z <= z_most;
-        });
+        // The kept tokens, where they are few and not gathered yet.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
+        const float most = min_p > 0.0f ? fminf((fmaxf(-logf(min_p), 0.0f) * 1.001f + 1e-3f) * (r.per_step * temperature), kBins) : kBins;
+        if (n > kBins)
+            n = gather(r, h, s, s.kept, kBins, [&](float l) { return (l >= r.bound.l) & (r.step(l) < most); });
         if (n <= kBins) {
             const int per = (a.V + kList - 1) / kList;
             s.ahead[tid] = 0;
@@ -646,8 +690,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
             }
         }
     }
+    auto target = [&](u64 sum) { return draw_at(u, sum); };
     u64 weight, total;
-    const int id = pick(r, h, s, weigh, [&](u64 sum) { return draw_at(u, sum); }, weight, total);
+    int id;
+    if (by_k || by_p || min_p > 0.0f)
+        id = pick(r, s, weigh, target, weight, total);
+    else
+        id = pick(r, s, [&](float l, int) { return r.step(l) < kBins ? r.weight(s, l) : 0; }, target, weight, total);
     if (tid == 0) answer(id, static_cast<double>(weight) / static_cast<double>(total));
 }
 
