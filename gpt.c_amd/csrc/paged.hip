@@ -6,6 +6,7 @@
 // into items of about equal size (paged_schedule), and every new token's slot and position are written out, so
 // that the kernels search nothing.  Its device memory is laid out for the plan's capacity and never moves.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <cstdlib>
@@ -19,17 +20,19 @@ using namespace gptc;
 struct gptc_paged_plan {
     const gptc_paged_cache_t *cache;
     int n_heads, group, max_seqs, max_tokens, max_len, max_pages;
-    int item_cap, merge_cap;
-    // Device memory (taken by the first set): ints [head 8 | items | merges | slot | pos | table], then the parts.
+    int item_cap, wide_cap, merge_cap, part_cap;
+    // Device memory (taken by the first set): ints [head 8 | items | wide items | merges | slot | pos | table], then
+    // the parts.
     int *dev;
     float *part_o, *part_ml;
-    size_t at_items, at_merges, at_slot, at_pos, at_table, ints;
+    size_t at_items, at_wide, at_merges, at_slot, at_pos, at_table, ints;
     // Two pinned copies of it, so that the host may prepare a step while the one before is still queued.
     int *host[2];
     hipEvent_t copied[2];
     int turn;
     bool is_set;
-    int n_tokens, n_items, n_merges;
+    int n_tokens, n_items, n_wide, n_merges;
+    int *table_at;  // where each sequence's page numbers start
     // Who writes each page in this step: checked without clearing the array between steps.
     long long *writer;  // step * max_seqs + sequence
     long long step;
@@ -40,57 +43,82 @@ namespace {
 constexpr int kMaxHeads = 4096;
 
 int64_t part_slots(const gptc_paged_plan *p) {
-    return static_cast<int64_t>(p->merge_cap) * p->cache->n_kv_heads;  // merge_cap bounds the parts (below)
+    return static_cast<int64_t>(p->part_cap) * p->cache->n_kv_heads;
+}
+
+// A sequence with this many query rows per kv head or more takes wide items.
+constexpr int kWideFrom = 64;
+
+// What a list of items is cut to: the total of its rounds over all kv heads makes about `target` items of at least
+// `least` rounds.
+struct Cutting {
+    int tile, unit, target;
+    int64_t total, per;
+};
+
+int tile_keys(int past, int rows, int row0, int tile, int group) {
+    const int end = row0 + tile < rows ? row0 + tile : rows;
+    return past + (end - 1) / group + 1;
 }
 
 }  // namespace
 
-int gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int dtype,
-                         PagedItem *items, int cap, PagedMerge *merges, int merge_cap, int *n_merges) {
-    // The work is counted in rounds of the workgroup's four waves.  A tile of rows whose keys take more rounds
-    // than `per` is cut evenly: `per` makes about kPagedTarget items in all (four workgroups per CU; fewer leave
-    // CUs idle in ragged steps, more cost merging) of at least kMinRounds rounds, below which joining the parts
-    // costs more than it saves.
+bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim,
+                          int dtype, PagedLists &lists) {
+    // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose
+    // keys take more rounds than `per` is cut evenly: `per` makes about four workgroups per CU (two wide ones) in
+    // all; fewer leave CUs idle in ragged steps, more cost merging.  Under kMinRounds rounds joining the parts costs
+    // more than it saves.
     constexpr int kMinRounds = 4;
-    const int unit = paged_unit(dtype);
-    int64_t total = 0;
+    Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 0, 0},
+                      {kPagedWide, paged_wide_keys(dtype, head_dim), kPagedWideTarget, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
-        for (int r = 0; r < rows; r += kPagedRows) {
-            const int end = r + kPagedRows < rows ? r + kPagedRows : rows;
-            total += (past[s] + (end - 1) / group + 1 + unit - 1) / unit;
-        }
+        Cutting &c = cut[rows >= kWideFrom];
+        for (int r = 0; r < rows; r += c.tile) c.total += (tile_keys(past[s], rows, r, c.tile, group) + c.unit - 1) / c.unit;
     }
-    int64_t per = (total * n_kv_heads + kPagedTarget - 1) / kPagedTarget;
-    if (per < kMinRounds) per = kMinRounds;
-    int n = 0, parts = 0, tok0 = 0, nm = 0;
+    for (Cutting &c : cut) {
+        c.per = (c.total * n_kv_heads + c.target - 1) / c.target;
+        if (c.per < kMinRounds) c.per = kMinRounds;
+    }
+    lists.n_items = lists.n_wide = lists.n_merges = 0;
+    int parts = 0, tok0 = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
-        for (int r = 0; r < rows; r += kPagedRows) {
-            const int end = r + kPagedRows < rows ? r + kPagedRows : rows;
-            const int keys = past[s] + (end - 1) / group + 1;
-            const int rounds = (keys + unit - 1) / unit;
-            const int cuts = static_cast<int>((rounds + per - 1) / per);
-            if (n + cuts > cap || (cuts > 1 && (nm >= merge_cap || parts + cuts > merge_cap))) return -1;
-            for (int c = 0; c < cuts; ++c) {
-                const int from = static_cast<int>(static_cast<int64_t>(rounds) * c / cuts);
-                const int to = static_cast<int>(static_cast<int64_t>(rounds) * (c + 1) / cuts);
-                const int key1 = to * static_cast<int64_t>(unit) < keys ? to * unit : keys;
-                items[n++] = PagedItem{tok0, past[s], rows, r, from * unit, key1, cuts > 1 ? parts + c : -1, s};
+        const bool wide = rows >= kWideFrom;
+        const Cutting &c = cut[wide];
+        const int slots = c.tile / kPagedRows;
+        for (int r = 0; r < rows; r += c.tile) {
+            const int keys = tile_keys(past[s], rows, r, c.tile, group);
+            const int rounds = (keys + c.unit - 1) / c.unit;
+            const int cuts = static_cast<int>((rounds + c.per - 1) / c.per);
+            int &n = wide ? lists.n_wide : lists.n_items;
+            if (n + cuts > (wide ? lists.wide_cap : lists.item_cap)) return false;
+            if (cuts > 1 && (parts + cuts * slots > lists.part_cap || lists.n_merges + slots > lists.merge_cap)) return false;
+            for (int i = 0; i < cuts; ++i) {
+                const int64_t from = static_cast<int64_t>(rounds) * i / cuts, to = static_cast<int64_t>(rounds) * (i + 1) / cuts;
+                const int key1 = to * c.unit < keys ? static_cast<int>(to * c.unit) : keys;
+                (wide ? lists.wide : lists.items)[n++] = PagedItem{
+                    tok0, past[s], rows, r, static_cast<int>(from * c.unit), key1, cuts > 1 ? parts + i * slots : -1, s};
             }
             if (cuts > 1) {
-                merges[nm++] = PagedMerge{tok0, rows, r, parts, cuts, 0, 0, 0};
-                parts += cuts;
+                for (int i = 0; i < slots && r + i * kPagedRows < rows; ++i)
+                    lists.merges[lists.n_merges++] = PagedMerge{tok0, rows, r + i * kPagedRows, parts + i, cuts, slots, 0, 0};
+                parts += cuts * slots;
             }
         }
         tok0 += fresh[s];
     }
-    *n_merges = nm;
-    return n;
+    // The longest first: workgroups start in this order, and what starts last should be short.
+    const auto longer = [](const PagedItem &x, const PagedItem &y) { return x.key1 - x.key0 > y.key1 - y.key0; };
+    std::sort(lists.items, lists.items + lists.n_items, longer);
+    std::sort(lists.wide, lists.wide + lists.n_wide, longer);
+    return true;
 }
 
 extern "C" int gptc_paged_schedule(const int n_seqs, const int *past, const int *fresh, const int n_heads,
-                                   const int n_kv_heads, const int dtype, int *items, const int cap) {
+                                   const int n_kv_heads, const int head_dim, const int dtype, int *items,
+                                   const int cap) {
     REQUIRE_ARG(past);
     REQUIRE_ARG(fresh);
     REQUIRE_ARG(items);
@@ -98,12 +126,25 @@ extern "C" int gptc_paged_schedule(const int n_seqs, const int *past, const int 
                 "Expected n_heads = %d to be a multiple of n_kv_heads = %d.", n_heads, n_kv_heads);
     CHECK_ERROR(dtype != GPTC_F32 && dtype != GPTC_BF16, "Unknown page type %d.", dtype);
     if (n_seqs <= 0 || cap <= 0) return n_seqs <= 0 ? 0 : -1;
-    auto *list = reinterpret_cast<PagedItem *>(items);
-    auto *merges = static_cast<PagedMerge *>(mallocCheck(sizeof(PagedMerge) * static_cast<size_t>(cap)));
-    int nm = 0;
-    const int n = paged_schedule(n_seqs, past, fresh, n_heads / n_kv_heads, n_kv_heads, dtype, list, cap, merges, cap, &nm);
-    free(merges);
-    for (int i = 0; i < n; ++i) list[i].table = 0;  // the item's kind: there is one
+    PagedLists l{};
+    l.items = reinterpret_cast<PagedItem *>(items);
+    l.item_cap = l.wide_cap = cap;
+    l.merge_cap = l.part_cap = INT32_MAX / 2;
+    l.merge_cap = 8 * cap;
+    l.wide = static_cast<PagedItem *>(mallocCheck(sizeof(PagedItem) * static_cast<size_t>(cap)));
+    l.merges = static_cast<PagedMerge *>(mallocCheck(sizeof(PagedMerge) * static_cast<size_t>(l.merge_cap)));
+    int n = -1;
+    if (paged_schedule(n_seqs, past, fresh, n_heads / n_kv_heads, n_kv_heads, head_dim, dtype, l) &&
+        l.n_items + l.n_wide <= cap) {
+        n = l.n_items + l.n_wide;
+        for (int i = 0; i < l.n_items; ++i) l.items[i].table = 0;  // the item's kind
+        for (int i = 0; i < l.n_wide; ++i) {
+            l.items[l.n_items + i] = l.wide[i];
+            l.items[l.n_items + i].table = 1;
+        }
+    }
+    free(l.wide);
+    free(l.merges);
     return n;
 }
 
@@ -175,14 +216,18 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     p->max_tokens = max_tokens;
     p->max_len = max_len;
     p->max_pages = (max_len + cache->page - 1) / cache->page;
-    // Every tile of rows is an item; cutting adds at most one item per `per` rounds, kPagedTarget / kv heads in
-    // all, and leaves at most as many cut tiles, so at most twice as many parts.
-    const int64_t tiles = static_cast<int64_t>(max_tokens) * group / kPagedRows + (max_seqs < max_tokens ? max_seqs : max_tokens);
-    const int64_t cut = kPagedTarget / cache->n_kv_heads + 1;
-    p->item_cap = static_cast<int>(tiles + cut);
-    p->merge_cap = static_cast<int>(2 * cut);
+    // Every tile of rows is an item; cutting adds at most one item per `per` rounds, target / kv heads in all, and
+    // cuts at most as many tiles, so it makes at most twice as many parts.
+    const int64_t work = static_cast<int64_t>(max_tokens) * group, active = max_seqs < max_tokens ? max_seqs : max_tokens;
+    const int cut = kPagedTarget / cache->n_kv_heads + 1, wide_cut = kPagedWideTarget / cache->n_kv_heads + 1;
+    constexpr int kSlots = kPagedWide / kPagedRows;
+    p->item_cap = static_cast<int>(work / kPagedRows + active) + cut;
+    p->wide_cap = static_cast<int>(work / kPagedWide + active) + wide_cut;
+    p->merge_cap = cut + kSlots * wide_cut;
+    p->part_cap = 2 * p->merge_cap;
     p->at_items = 8;
-    p->at_merges = p->at_items + 8 * static_cast<size_t>(p->item_cap);
+    p->at_wide = p->at_items + 8 * static_cast<size_t>(p->item_cap);
+    p->at_merges = p->at_wide + 8 * static_cast<size_t>(p->wide_cap);
     p->at_slot = p->at_merges + 8 * static_cast<size_t>(p->merge_cap);
     p->at_pos = p->at_slot + max_tokens;
     p->at_table = p->at_pos + max_tokens;
@@ -190,6 +235,7 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     const size_t n_pages = cache->n_pages;
     p->writer = static_cast<long long *>(mallocCheck(sizeof(long long) * n_pages));
     memset(p->writer, 0, sizeof(long long) * n_pages);
+    p->table_at = static_cast<int *>(mallocCheck(sizeof(int) * static_cast<size_t>(max_seqs)));
     return p;
 }
 
@@ -206,6 +252,7 @@ extern "C" void gptc_paged_plan_free(gptc_paged_plan_t *plan) {
         }
     }
     free(plan->writer);
+    free(plan->table_at);
     free(plan);
 }
 
@@ -269,12 +316,17 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     plan->turn ^= 1;
     hipCheck(hipEventSynchronize(plan->copied[plan->turn]));
     int *h = plan->host[plan->turn];
-    auto *items = reinterpret_cast<PagedItem *>(h + plan->at_items);
-    int nm = 0;
-    const int n = paged_schedule(n_seqs, past, fresh, plan->group, c->n_kv_heads, c->dtype, items, plan->item_cap,
-                                 reinterpret_cast<PagedMerge *>(h + plan->at_merges), plan->merge_cap, &nm);
-    CHECK_ERROR(n < 0, "The work of %d sequences does not fit the plan.", n_seqs);
-    int t = 0, at = 0, it = 0;
+    PagedLists lists{};
+    lists.items = reinterpret_cast<PagedItem *>(h + plan->at_items);
+    lists.wide = reinterpret_cast<PagedItem *>(h + plan->at_wide);
+    lists.merges = reinterpret_cast<PagedMerge *>(h + plan->at_merges);
+    lists.item_cap = plan->item_cap;
+    lists.wide_cap = plan->wide_cap;
+    lists.merge_cap = plan->merge_cap;
+    lists.part_cap = plan->part_cap;
+    const bool fits = paged_schedule(n_seqs, past, fresh, plan->group, c->n_kv_heads, c->head_dim, c->dtype, lists);
+    CHECK_ERROR(!fits, "The work of %d sequences does not fit the plan.", n_seqs);
+    int t = 0, at = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const int used = (past[s] + fresh[s] + c->page - 1) / c->page;
         const int *mine = table + static_cast<int64_t>(s) * stride;
@@ -284,26 +336,31 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
             h[plan->at_pos + t] = pos;
         }
         if (fresh[s] == 0) continue;  // nobody asks for its keys
-        for (; it < n && items[it].table == s; ++it) items[it].table = at;
+        plan->table_at[s] = at;
         memcpy(h + plan->at_table + at, mine, sizeof(int) * used);
         at += used;
     }
+    for (int i = 0; i < lists.n_items; ++i) lists.items[i].table = plan->table_at[lists.items[i].table];
+    for (int i = 0; i < lists.n_wide; ++i) lists.wide[i].table = plan->table_at[lists.wide[i].table];
     h[0] = t;
-    h[1] = n;
-    h[2] = nm;
+    h[1] = lists.n_items;
+    h[2] = lists.n_merges;
+    h[3] = lists.n_wide;
     auto send = [&](size_t from, size_t count) {
         if (count > 0)
             hipCheck(hipMemcpyAsync(plan->dev + from, h + from, sizeof(int) * count, hipMemcpyHostToDevice, stream));
     };
-    send(0, plan->at_items + 8 * static_cast<size_t>(n));
-    send(plan->at_merges, 8 * static_cast<size_t>(nm));
+    send(0, plan->at_items + 8 * static_cast<size_t>(lists.n_items));
+    send(plan->at_wide, 8 * static_cast<size_t>(lists.n_wide));
+    send(plan->at_merges, 8 * static_cast<size_t>(lists.n_merges));
     send(plan->at_slot, t);
     send(plan->at_pos, t);
     send(plan->at_table, at);
     hipCheck(hipEventRecord(plan->copied[plan->turn], stream));
     plan->n_tokens = t;
-    plan->n_items = n;
-    plan->n_merges = nm;
+    plan->n_items = lists.n_items;
+    plan->n_wide = lists.n_wide;
+    plan->n_merges = lists.n_merges;
     plan->is_set = true;
 }
 
@@ -525,6 +582,7 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.v = c->v[layer];
     a.head = plan->dev;
     a.items = reinterpret_cast<const PagedItem *>(plan->dev + plan->at_items);
+    a.wide = reinterpret_cast<const PagedItem *>(plan->dev + plan->at_wide);
     a.merges = reinterpret_cast<const PagedMerge *>(plan->dev + plan->at_merges);
     a.table = plan->dev + plan->at_table;
     a.part_o = plan->part_o;
@@ -538,9 +596,10 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.page_shift = log2_of(c->page);
     a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
     a.n_items = capturing ? plan->item_cap : plan->n_items;
+    a.n_wide = capturing ? plan->wide_cap : plan->n_wide;
     a.n_merges = capturing ? plan->merge_cap : plan->n_merges;
     a.bf16 = c->dtype == GPTC_BF16;
     a.vec = D % (a.bf16 ? 8 : 4) == 0 && aligned16(a.q) && aligned16(a.out);
-    if (a.n_items == 0) return;
+    if (a.n_items + a.n_wide == 0) return;
     launch_paged_attention(a, s);
 }

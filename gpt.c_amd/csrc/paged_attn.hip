@@ -21,72 +21,14 @@
 // fp32 pages are multiplied by v_mfma_f32_16x16x4_f32.  bf16 pages by v_mfma_f32_16x16x32_bf16 with the query
 // and the weights as exact sums of three bf16 values (24 bits): three products at a sixteenth of the cost of an
 // fp32 one each.
-#include "attn_common.hpp"
 #include "hip_check.hpp"
-#include "paged_plan.hpp"
+#include "paged_attn_common.hpp"
 
 namespace gptc {
 
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kWaves = 4;
-
-// What is known of the rows: D is the tile's width; every row starts at a multiple of 16 bytes and holds whole
-// vectors; or nothing.
-enum Rows { kFull, kVec, kAny };
-
-// N consecutive 32-bit words of T values from row + d; values at or past D are zeros (the load then takes the
-// row's first values instead, so that no branch parts the loads).
-template <typename T, int N, Rows R>
-__device__ __forceinline__ void load_words(uint32_t (&w)[N], const T *row, int d, int D) {
-    if constexpr (R != kAny) {
-        static_assert(N == 2 || N == 4, "one vector load");
-        typedef uint32_t vec __attribute__((ext_vector_type(N)));
-        const bool in = R == kFull || d < D;
-        const vec x = *reinterpret_cast<const vec *>(row + (in ? d : 0));
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = in ? x[i] : 0;
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = d + i < D ? __builtin_bit_cast(uint32_t, row[d + i]) : 0u;
-    } else {
-        const uint16_t *r = reinterpret_cast<const uint16_t *>(row);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t lo = d + 2 * i < D ? r[d + 2 * i] : 0u, hi = d + 2 * i + 1 < D ? r[d + 2 * i + 1] : 0u;
-            w[i] = lo | hi << 16;
-        }
-    }
-}
-
-// x, y as sums of three bf16 values, packed in pairs.
-__device__ __forceinline__ void split3(float x, float y, uint32_t (&p)[3]) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        const f32x2 v = {x, y};
-        p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-        x -= __builtin_bit_cast(float, p[i] << 16);
-        y -= __builtin_bit_cast(float, p[i] & 0xffff0000u);
-    }
-}
-
-__device__ __forceinline__ f32x4 mfma_bf16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
-    const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0,
-                                                   0);
-}
-
-// A matrix instruction's result may be read 11 cycles after it at the earliest.  The compiler counts them inside
-// a block; across a branch it was seen to read the last two registers at once (wrong sums at every second step of
-// bf16 pages).  So results are taken over in the block of the product, or after a wait of 16.
-__device__ __forceinline__ void settled(f32x4 &x) { asm volatile("" : "+v"(x)); }
-__device__ __forceinline__ void finished(f32x4 &x) { asm volatile("s_nop 15" : "+a"(x)); }
 
 // A wave's operands: the query rows, and the keys and values of one turn.
 template <typename T, int DP, Rows R>
@@ -389,7 +331,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnParams 
     const int token = mg.tok0 + row / a.group;
     if (row >= mg.rows || token >= a.rows) return;
     const int64_t first = (static_cast<int64_t>(mg.part0) * a.KV + kv) * kPagedRows + r;
-    const int64_t next = static_cast<int64_t>(a.KV) * kPagedRows;
+    const int64_t next = static_cast<int64_t>(mg.step) * a.KV * kPagedRows;
     float big = -INFINITY;
     for (int p = 0; p < mg.n; ++p) big = fmaxf(big, a.part_ml[2 * (first + p * next)]);
     float *dst = a.out + (static_cast<int64_t>(token) * a.H + kv * a.group + row % a.group) * a.D;
@@ -422,12 +364,15 @@ void launch(const PagedAttnParams &p, hipStream_t s) {
 }  // namespace
 
 void launch_paged_attention(const PagedAttnParams &p, hipStream_t s) {
-    if (p.bf16) {
-        if (p.D <= 64) launch<__bf16, 64>(p, s);
-        else launch<__bf16, 128>(p, s);
-    } else {
-        if (p.D <= 64) launch<float, 64>(p, s);
-        else launch<float, 128>(p, s);
+    if (p.n_wide > 0) launch_paged_wide(p, s);
+    if (p.n_items > 0) {
+        if (p.bf16) {
+            if (p.D <= 64) launch<__bf16, 64>(p, s);
+            else launch<__bf16, 128>(p, s);
+        } else {
+            if (p.D <= 64) launch<float, 64>(p, s);
+            else launch<float, 128>(p, s);
+        }
     }
     if (p.n_merges == 0) return;
     const dim3 grid(static_cast<unsigned>(p.n_merges) * p.KV);

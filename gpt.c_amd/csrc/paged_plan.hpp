@@ -19,42 +19,56 @@ struct PagedItem {
     int table;  // where the sequence's page numbers start; on the host side of the list, its sequence
 };
 
-// The rows whose keys were cut into n items: their parts are part0 .. part0 + n - 1.
+// Up to 16 rows whose keys were cut into n items: their parts are part0, part0 + step, ...
 struct PagedMerge {
-    int tok0, rows, row0, part0, n, pad0, pad1, pad2;
+    int tok0, rows, row0, part0, n, step, pad0, pad1;
 };
 
-constexpr int kPagedRows = 16;  // query rows of an item
+constexpr int kPagedRows = 16;   // query rows of an item, and of a slot of the workspace
+constexpr int kPagedWide = 128;  // query rows of a wide item (csrc/paged_attn_wide.hip): 8 slots
 
-// Keys that a round of the four waves of a workgroup takes: 16 or 32 each (csrc/paged_attn.hip).
+// Keys that an item's kernel takes at a time, which its range is made of: a round of the four waves of a workgroup,
+// 16 or 32 keys each (csrc/paged_attn.hip); an LDS tile of a wide item, 16 KB of keys.
 constexpr int paged_unit(int dtype) { return dtype == GPTC_BF16 ? 128 : 64; }
+constexpr int paged_wide_keys(int dtype, int head_dim) {
+    return (dtype == GPTC_BF16 ? 8192 : 4096) / (head_dim <= 64 ? 64 : 128);
+}
 
 // Items that the keys of one step are cut into at most, over all kv heads: see paged_schedule.
 constexpr int kPagedTarget = 1024;
+constexpr int kPagedWideTarget = 512;
 
-// Fills items (and merges) for a step; returns the number of items, or -1 when one of the lists does not fit.
-// items[i].table receives the sequence.
-int paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int dtype,
-                   PagedItem *items, int cap, PagedMerge *merges, int merge_cap, int *n_merges);
+// The lists of a step: items, wide items, and what is to be joined afterwards.
+struct PagedLists {
+    PagedItem *items, *wide;
+    PagedMerge *merges;
+    int item_cap, wide_cap, merge_cap, part_cap;
+    int n_items, n_wide, n_merges;
+};
+
+// Fills the lists for a step (an item's table receives its sequence); false when one of them does not fit.
+bool paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim, int dtype,
+                    PagedLists &lists);
 
 // What the attention kernels take.
 struct PagedAttnParams {
     const float *q;
     float *out;
     const void *k, *v;
-    const int *head;  // {tokens, items, merges} of the plan, read on the device: a captured launch covers the
+    const int *head;  // {tokens, items, merges, wide items} of the plan, read on the device: a captured launch covers the
                       // plan's capacity and runs what the plan holds then
-    const PagedItem *items;
+    const PagedItem *items, *wide;
     const PagedMerge *merges;
     const int *table;
     float *part_o, *part_ml;  // partial outputs [part][kv head][row][D], and their (max, sum) pairs
     int q_stride, rows;       // floats of a q row; rows of q and out
     int H, KV, group, D, page_shift;
     float scale_log2;
-    int n_items, n_merges;  // of the launch
+    int n_items, n_wide, n_merges;  // of the launch
     bool bf16, vec;         // vec: every row starts at a multiple of 16 bytes and holds whole vectors
 };
 
 void launch_paged_attention(const PagedAttnParams &p, hipStream_t s);
+void launch_paged_wide(const PagedAttnParams &p, hipStream_t s);
 
 }  // namespace gptc

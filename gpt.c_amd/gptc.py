@@ -226,7 +226,7 @@ SIGNATURES = {
     "gptc_rotary_table": (TensorP, [_ci, _ci, ctypes.c_double]),
     "gptc_paged_append_cuda": (None, [_vp, _ci, TensorP, TensorP, _ci, TensorP]),
     "gptc_paged_attention_cuda": (None, [_vp, _ci, TensorP, TensorP]),
-    "gptc_paged_schedule": (_ci, [_ci, _ip, _ip, _ci, _ci, _ci, _ip, _ci]),
+    "gptc_paged_schedule": (_ci, [_ci, _ip, _ip, _ci, _ci, _ci, _ci, _ip, _ci]),
     # tensor.h (BLAS front ends)
     "saxpy": (None, [_ci, _cf, TensorP, _ci, _ci, TensorP, _ci, _ci]),
     "sgemm": (None, [_ci, _ci, _ci, _ci, _ci, _cf, TensorP, _ci, _ci, TensorP, _ci, _ci, _cf, TensorP, _ci, _ci]),

@@ -116,17 +116,18 @@ void gptc_paged_append_cuda(gptc_paged_plan_t *plan, const int layer, const tens
 void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int layer, const tensor_t *q, tensor_t *output);
 
 /*
- * gptc_paged_schedule(n_seqs, past, fresh, n_heads, n_kv_heads, dtype, items, cap)
+ * gptc_paged_schedule(n_seqs, past, fresh, n_heads, n_kv_heads, head_dim, dtype, items, cap)
  *   The work list that gptc_paged_plan_set makes for such a step (host
  *   computation only, for tests and tuning): item i is items[8i .. 8i+7] =
  *   (first token row, past, query rows of the sequence, first query row, first
  *   key, end key, part, kind): query rows are token * group + head for the
- *   group = n_heads / n_kv_heads heads of one kv head; part -1 when the item
- *   covers all keys of its rows, else its place in the workspace.  Returns the
- *   number of items, or -1 when cap (in items) does not hold them.
+ *   group = n_heads / n_kv_heads heads of one kv head; kind 0: 16 rows, 1: 128
+ *   (wide); part -1 when the item covers all keys of its rows, else its place
+ *   in the workspace (the first of 8 for a wide one).  Returns the number of
+ *   items, or -1 when cap (in items) does not hold them.
  */
 int gptc_paged_schedule(const int n_seqs, const int *past, const int *fresh, const int n_heads, const int n_kv_heads,
-                        const int dtype, int *items, const int cap);
+                        const int head_dim, const int dtype, int *items, const int cap);
 
 #ifdef __cplusplus
 }

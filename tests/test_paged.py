@@ -94,27 +94,29 @@ def test_shared_pages_that_are_only_read_pass_the_checks():
     assert r.returncode == 1 and "runtime_init" in r.stderr, r.stderr
 
 
-def schedule(lib, past, fresh, heads, kv, dtype, cap):
+def schedule(lib, past, fresh, heads, kv, dtype, cap, dim=64):
     past, fresh = (np.ascontiguousarray(x, np.int32) for x in (past, fresh))
     items = np.zeros((cap, 8), np.int32)
     ip = ctypes.POINTER(ctypes.c_int)
-    n = lib.gptc_paged_schedule(len(past), past.ctypes.data_as(ip), fresh.ctypes.data_as(ip), heads, kv, dtype,
+    n = lib.gptc_paged_schedule(len(past), past.ctypes.data_as(ip), fresh.ctypes.data_as(ip), heads, kv, dim, dtype,
                                 items.ctypes.data_as(ip), cap)
     return n, items[:max(n, 0)]
 
 
-@settings(max_examples=150, deadline=None)
-@given(st.lists(st.tuples(st.integers(0, 3000), st.integers(0, 40)), min_size=1, max_size=9),
-       st.sampled_from([(1, 1), (12, 12), (32, 8), (25, 5), (8, 1)]), st.sampled_from([gptc.F32, gptc.BF16]))
-def test_work_list_covers_every_key_once(seqs, heads, dtype):
+@settings(max_examples=100, deadline=None)
+@given(st.lists(st.tuples(st.integers(0, 3000), st.integers(0, 300)), min_size=1, max_size=7),
+       st.sampled_from([(1, 1), (12, 12), (32, 8), (25, 5), (8, 1)]), st.sampled_from([gptc.F32, gptc.BF16]),
+       st.sampled_from([64, 80]))
+def test_work_list_covers_every_key_once(seqs, heads, dtype, dim):
     lib = gptc.load()
     past, fresh = zip(*seqs)
     H, KV = heads
     group = H // KV
-    n, items = schedule(lib, past, fresh, H, KV, dtype, 1 << 16)
+    n, items = schedule(lib, past, fresh, H, KV, dtype, 1 << 16, dim)
     assert n >= 0
-    parts = [i[6] for i in items if i[6] >= 0]
-    assert len(set(parts)) == len(parts) and (not parts or sorted(parts) == list(range(len(parts))))
+    # Every cut item has its place in the workspace: one for each 16 of its rows.
+    parts = [part + i for part, kind in items[:, 6:].tolist() if part >= 0 for i in range(8 if kind else 1)]
+    assert sorted(parts) == list(range(len(parts)))
     seen, token = {}, 0
     for s, (p, f) in enumerate(seqs):
         for row in range(f * group):
@@ -127,7 +129,7 @@ def test_work_list_covers_every_key_once(seqs, heads, dtype):
         token += f
     for tok0, p, rows, row0, key0, key1, part, kind in items.tolist():
         assert ends[tok0] == (p, rows // group) and kind in (0, 1) and key0 < key1
-        for row in range(row0, min(row0 + 16, rows)):
+        for row in range(row0, min(row0 + (128 if kind else 16), rows)):
             seen[(tok0, row)].append((key0, key1))
     for (tok0, row), spans in seen.items():
         need = ends[tok0][0] + row // group + 1

@@ -122,6 +122,17 @@ SHAPES = [
     ([77, 0], [2, 18], 8, 1, 24, 128),
     ([3000], [1], 2, 2, 128, 256),                     # keys cut into parts
     ([2049, 700], [9, 20], 16, 1, 64, 64),             # cut, several tiles
+    # From here on: many rows of a sequence, which share tiles of keys.
+    ([0], [64], 1, 1, 64, 16),
+    ([0], [130], 2, 2, 128, 16),
+    ([17, 300, 5], [127, 129, 2], 2, 2, 64, 16),
+    ([3001], [70], 2, 1, 128, 32),                     # cut
+    ([2000, 63], [66, 1], 3, 3, 64, 64),               # cut, with rows past the last tile's
+    ([7], [65], 3, 1, 33, 16),
+    ([90], [70], 2, 2, 127, 16),
+    ([20], [80], 1, 1, 1, 16),
+    ([33], [41], 10, 2, 72, 32),
+    ([0], [100], 4, 2, 24, 128),
 ]
 
 
