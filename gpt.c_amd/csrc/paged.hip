@@ -71,7 +71,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     // more than it saves.
     constexpr int kMinRounds = 4;
     Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 0, 0},
-                      {kPagedWide, paged_wide_keys(dtype, head_dim), kPagedWideTarget, 0, 0}};
+                      {paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
         Cutting &c = cut[rows >= kWideFrom];
@@ -220,10 +220,10 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     // cuts at most as many tiles, so it makes at most twice as many parts.
     const int64_t work = static_cast<int64_t>(max_tokens) * group, active = max_seqs < max_tokens ? max_seqs : max_tokens;
     const int cut = kPagedTarget / cache->n_kv_heads + 1, wide_cut = kPagedWideTarget / cache->n_kv_heads + 1;
-    constexpr int kSlots = kPagedWide / kPagedRows;
+    const int wide_rows = paged_wide_rows(cache->dtype), slots = wide_rows / kPagedRows;
     p->item_cap = static_cast<int>(work / kPagedRows + active) + cut;
-    p->wide_cap = static_cast<int>(work / kPagedWide + active) + wide_cut;
-    p->merge_cap = cut + kSlots * wide_cut;
+    p->wide_cap = static_cast<int>(work / wide_rows + active) + wide_cut;
+    p->merge_cap = cut + slots * wide_cut;
     p->part_cap = 2 * p->merge_cap;
     p->at_items = 8;
     p->at_wide = p->at_items + 8 * static_cast<size_t>(p->item_cap);

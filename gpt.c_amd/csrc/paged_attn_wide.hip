@@ -21,13 +21,15 @@ namespace gptc {
 
 namespace {
 
-constexpr int kWaves = kPagedWide / 16;
-constexpr int kThreads = 64 * kWaves;
+template <typename T>
+constexpr int kType = sizeof(T) == 4 ? GPTC_F32 : GPTC_BF16;
+template <typename T>
+constexpr int kThreadsOf = paged_wide_rows(kType<T>) / 16 * 64;
 
 template <typename T, int DP>
 struct Shape {
     static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
-    static constexpr int kKeys = paged_wide_keys(sizeof(T) == 4 ? GPTC_F32 : GPTC_BF16, DP);
+    static constexpr int kKeys = paged_wide_keys(kType<T>, DP);
     static constexpr int kKRow = DP + 8;      // bf16 values of an LDS row
     static constexpr int kVRow = kKeys + 8;
     static constexpr int kKPart = kKeys * kKRow, kVPart = DP * kVRow;
@@ -40,9 +42,9 @@ __device__ __forceinline__ void parts_of(uint32_t x0, uint32_t x1, uint32_t (&p)
 }
 
 template <typename T, int DP, Rows R>
-__global__ __launch_bounds__(kThreads) void paged_wide_kernel(const PagedAttnParams a) {
+__global__ __launch_bounds__(kThreadsOf<T>) void paged_wide_kernel(const PagedAttnParams a) {
     using S = Shape<T, DP>;
-    constexpr int kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
+    constexpr int kThreads = kThreadsOf<T>, kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
 
     const int item = blockIdx.x / a.KV, kv = blockIdx.x - item * a.KV;
@@ -280,7 +282,7 @@ void launch(const PagedAttnParams &p, hipStream_t s) {
                                          hipFuncAttributeMaxDynamicSharedMemorySize, kBytes));
         });
     }
-    paged_wide_kernel<T, DP, R><<<dim3(static_cast<unsigned>(p.n_wide) * p.KV), dim3(kThreads), kBytes, s>>>(p);
+    paged_wide_kernel<T, DP, R><<<dim3(static_cast<unsigned>(p.n_wide) * p.KV), dim3(kThreadsOf<T>), kBytes, s>>>(p);
     hipCheck(hipGetLastError());
 }
 

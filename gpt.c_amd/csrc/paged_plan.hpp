@@ -25,13 +25,14 @@ struct PagedMerge {
 };
 
 constexpr int kPagedRows = 16;   // query rows of an item, and of a slot of the workspace
-constexpr int kPagedWide = 128;  // query rows of a wide item (csrc/paged_attn_wide.hip): 8 slots
+// Query rows of a wide item (csrc/paged_attn_wide.hip).
+constexpr int paged_wide_rows(int dtype) { return dtype == GPTC_BF16 ? 64 : 128; }
 
 // Keys that an item's kernel takes at a time, which its range is made of: a round of the four waves of a workgroup,
-// 16 or 32 keys each (csrc/paged_attn.hip); an LDS tile of a wide item, 16 KB of keys.
+// 16 or 32 keys each (csrc/paged_attn.hip); an LDS tile of a wide item.
 constexpr int paged_unit(int dtype) { return dtype == GPTC_BF16 ? 128 : 64; }
 constexpr int paged_wide_keys(int dtype, int head_dim) {
-    return (dtype == GPTC_BF16 ? 8192 : 4096) / (head_dim <= 64 ? 64 : 128);
+    return dtype == GPTC_BF16 ? (head_dim <= 64 ? 128 : 64) : (head_dim <= 64 ? 64 : 32);
 }
 
 // Items that the keys of one step are cut into at most, over all kv heads: see paged_schedule.

@@ -121,10 +121,11 @@ void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int layer, const t
  *   computation only, for tests and tuning): item i is items[8i .. 8i+7] =
  *   (first token row, past, query rows of the sequence, first query row, first
  *   key, end key, part, kind): query rows are token * group + head for the
- *   group = n_heads / n_kv_heads heads of one kv head; kind 0: 16 rows, 1: 128
- *   (wide); part -1 when the item covers all keys of its rows, else its place
- *   in the workspace (the first of 8 for a wide one).  Returns the number of
- *   items, or -1 when cap (in items) does not hold them.
+ *   group = n_heads / n_kv_heads heads of one kv head; kind 0: 16 rows, 1:
+ *   64 of bf16 pages or 128 of fp32 ones; part -1 when the item covers all
+ *   keys of its rows, else its place in the workspace (the first of rows / 16
+ *   places).  Returns the number of items, or -1 when cap (in items) does not
+ *   hold them.
  */
 int gptc_paged_schedule(const int n_seqs, const int *past, const int *fresh, const int n_heads, const int n_kv_heads,
                         const int head_dim, const int dtype, int *items, const int cap);

@@ -115,7 +115,7 @@ def test_work_list_covers_every_key_once(seqs, heads, dtype, dim):
     n, items = schedule(lib, past, fresh, H, KV, dtype, 1 << 16, dim)
     assert n >= 0
     # Every cut item has its place in the workspace: one for each 16 of its rows.
-    parts = [part + i for part, kind in items[:, 6:].tolist() if part >= 0 for i in range(8 if kind else 1)]
+    parts = [part + i for part, kind in items[:, 6:].tolist() if part >= 0 for i in range((8 if dtype == gptc.F32 else 4) if kind else 1)]
     assert sorted(parts) == list(range(len(parts)))
     seen, token = {}, 0
     for s, (p, f) in enumerate(seqs):
@@ -129,7 +129,7 @@ def test_work_list_covers_every_key_once(seqs, heads, dtype, dim):
         token += f
     for tok0, p, rows, row0, key0, key1, part, kind in items.tolist():
         assert ends[tok0] == (p, rows // group) and kind in (0, 1) and key0 < key1
-        for row in range(row0, min(row0 + (128 if kind else 16), rows)):
+        for row in range(row0, min(row0 + ((128 if dtype == gptc.F32 else 64) if kind else 16), rows)):
             seen[(tok0, row)].append((key0, key1))
     for (tok0, row), spans in seen.items():
         need = ends[tok0][0] + row // group + 1
