@@ -31,7 +31,7 @@ struct gptc_paged_plan {
     hipEvent_t copied[2];
     int turn;
     bool is_set;
-    int n_tokens, n_items, n_wide, n_merges;
+    int n_tokens, n_items, n_wide, n_merges, max_parts, merge_rows;
     int *table_at;  // where each sequence's page numbers start
     // Who writes each page in this step: checked without clearing the array between steps.
     long long *writer;  // step * max_seqs + sequence
@@ -49,10 +49,9 @@ int64_t part_slots(const gptc_paged_plan *p) {
 // A sequence with this many query rows per kv head or more takes wide items.
 constexpr int kWideFrom = 64;
 
-// What a list of items is cut to: the total of its rounds over all kv heads makes about `target` items of at least
-// `least` rounds.
+// How a list's tiles of rows are cut.
 struct Cutting {
-    int tile, unit, target;
+    int tile, unit, target, whole;
     int64_t total, per;
 };
 
@@ -67,11 +66,12 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
                           int dtype, PagedLists &lists) {
     // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose
     // keys take more rounds than `per` is cut evenly: `per` makes about four workgroups per CU (two wide ones) in
-    // all; fewer leave CUs idle in ragged steps, more cost merging.  Under kMinRounds rounds joining the parts costs
-    // more than it saves.
-    constexpr int kMinRounds = 4;
-    Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 0, 0},
-                      {paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, 0, 0}};
+    // all; fewer leave CUs idle in ragged steps, more cost merging.  Parts have kLeast rounds at least, and what takes
+    // no more than `whole` stays whole: one token of 12 heads over 300 keys (5 rounds) takes 7.6 us whole and 9.5 us
+    // in two parts; a prompt of 1024 (16 tiles at most) 23.6 us in parts of 4 tiles and 27 us in parts of 8.
+    constexpr int kLeast = 4;
+    Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 8, 0, 0},
+                      {paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, 4, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
         Cutting &c = cut[rows >= kWideFrom];
@@ -79,9 +79,9 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     }
     for (Cutting &c : cut) {
         c.per = (c.total * n_kv_heads + c.target - 1) / c.target;
-        if (c.per < kMinRounds) c.per = kMinRounds;
+        if (c.per < kLeast) c.per = kLeast;
     }
-    lists.n_items = lists.n_wide = lists.n_merges = 0;
+    lists.n_items = lists.n_wide = lists.n_merges = lists.max_parts = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
@@ -91,7 +91,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
         for (int r = 0; r < rows; r += c.tile) {
             const int keys = tile_keys(past[s], rows, r, c.tile, group);
             const int rounds = (keys + c.unit - 1) / c.unit;
-            const int cuts = static_cast<int>((rounds + c.per - 1) / c.per);
+            const int cuts = rounds <= c.whole ? 1 : static_cast<int>((rounds + c.per - 1) / c.per);
             int &n = wide ? lists.n_wide : lists.n_items;
             if (n + cuts > (wide ? lists.wide_cap : lists.item_cap)) return false;
             if (cuts > 1 && (parts + cuts * slots > lists.part_cap || lists.n_merges + slots > lists.merge_cap)) return false;
@@ -105,6 +105,8 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
                 for (int i = 0; i < slots && r + i * kPagedRows < rows; ++i)
                     lists.merges[lists.n_merges++] = PagedMerge{tok0, rows, r + i * kPagedRows, parts + i, cuts, slots, 0, 0};
                 parts += cuts * slots;
+                lists.max_parts = std::max(lists.max_parts, cuts);
+                lists.merge_rows = std::max(lists.merge_rows, std::min(rows - r, kPagedRows));
             }
         }
         tok0 += fresh[s];
@@ -361,6 +363,8 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     plan->n_items = lists.n_items;
     plan->n_wide = lists.n_wide;
     plan->n_merges = lists.n_merges;
+    plan->max_parts = lists.max_parts;
+    plan->merge_rows = lists.merge_rows;
     plan->is_set = true;
 }
 
@@ -598,6 +602,8 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.n_items = capturing ? plan->item_cap : plan->n_items;
     a.n_wide = capturing ? plan->wide_cap : plan->n_wide;
     a.n_merges = capturing ? plan->merge_cap : plan->n_merges;
+    a.many_parts = capturing || plan->max_parts > 8;
+    a.merge_rows = capturing ? kPagedRows : plan->merge_rows;
     a.bf16 = c->dtype == GPTC_BF16;
     a.vec = D % (a.bf16 ? 8 : 4) == 0 && aligned16(a.q) && aligned16(a.out);
     if (a.n_items + a.n_wide == 0) return;

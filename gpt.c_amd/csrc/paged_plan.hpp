@@ -45,6 +45,7 @@ struct PagedLists {
     PagedMerge *merges;
     int item_cap, wide_cap, merge_cap, part_cap;
     int n_items, n_wide, n_merges;
+    int max_parts, merge_rows;  // of a tile: parts, and rows to be joined of 16
 };
 
 // Fills the lists for a step (an item's table receives its sequence); false when one of them does not fit.
@@ -66,6 +67,8 @@ struct PagedAttnParams {
     int H, KV, group, D, page_shift;
     float scale_log2;
     int n_items, n_wide, n_merges;  // of the launch
+    int merge_rows;         // rows of a merge, at most
+    bool many_parts;        // see launch_paged_attention
     bool bf16, vec;         // vec: every row starts at a multiple of 16 bytes and holds whole vectors
 };
 

@@ -37,7 +37,7 @@ constexpr int kMask = 24;            // logits of a thread that are looked throu
 constexpr int kHeld = 4 * kMask;     // logits of a thread that stay in registers
 constexpr int kBins = 8192;          // of a histogram; tokens that can be gathered
 constexpr int kList = kThreads;      // tokens that can be ranked
-constexpr int kTable = 2048;
+constexpr int kTable = 32;            // entries of 8 bytes: one for every two LDS banks, so lanes never collide
 
 struct SampleParams {
     const float *logits, *params, *u;
@@ -58,7 +58,7 @@ struct Lds {
     Token list[kList];
     u64 list_w[kList];
     u64 ahead[kList];
-    double table[kTable];  // 2^(-j / 2048)
+    double table[kTable];  // 2^(-j / 32)
     u64 wave_sum[2 * kWaves];
     float wave_max[kWaves];
     int wave_idx[kWaves];
@@ -137,23 +137,27 @@ struct Row {
     static __device__ __forceinline__ float plain(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f); }
 
     // What follows has no branches: the chains of a chunk's logits run side by side.
-    __device__ __forceinline__ bool kept(float l, int i) const { return (l > bound.l) | ((l == bound.l) & (i <= bound.i)); }
+    __device__ __forceinline__ bool kept(float l, int i) const { return static_cast<int>(l > bound.l) | (static_cast<int>(l == bound.l) & static_cast<int>(i <= bound.i)); }
 
     // Where the logit lies in the histogram: kBins and more where the weight is nothing, 0 where the difference is 0
     // and the scale infinite (a vanishing temperature).
     __device__ __forceinline__ float step(float l) const { return fmaxf((M - l) * per_step, 0.0f); }
 
-    // Where step(l) < kBins.  The exponent in steps of 1/2048: a table's entry, and two terms of the exponential
-    // series for the rest (at most ln 2 / 4096: the next is below 2^-39 of the weight).  Whole numbers come out of
-    // additions of 2^52, or 1.5 times that.
+    // Where step(l) < kBins.  The exponent in steps of 1/32: a table's entry, and five terms of the exponential series
+    // for the rest (at most ln 2 / 64: the next is below 2^-48 of the weight).  Whole numbers come out of additions of
+    // 2^52, or 1.5 times that.  A table of 2048 entries with two terms took 1.4 times as long: its reads collide.
     __device__ __forceinline__ u64 weight(const Lds &s, float l) const {
-        static_assert(kTable == 1 << 11, "the shift below");
+        static_assert(kTable == 1 << 5, "the shift below");
         constexpr double kWhole = 6755399441055744.0, kLn = 0.6931471805599453 / kTable;
         const double t = (static_cast<double>(M) - static_cast<double>(l)) * per_entry;
         const double n = t + kWhole, x = (n - kWhole) - t;
         const int e = static_cast<int>(__double_as_longlong(n));
-        const double p = fma(x, fma(x, kLn * kLn / 2, kLn), 1.0) * s.table[e & (kTable - 1)];
-        const double scale = __hiloint2double((1023 + shift - (e >> 11)) << 20, 0);
+        double p = fma(x, kLn * kLn * kLn * kLn * kLn / 120, kLn * kLn * kLn * kLn / 24);
+        p = fma(x, p, kLn * kLn * kLn / 6);
+        p = fma(x, p, kLn * kLn / 2);
+        p = fma(x, p, kLn);
+        p = fma(x, p, 1.0) * s.table[e & (kTable - 1)];
+        const double scale = __hiloint2double((1023 + shift - (e >> 5)) << 20, 0);
         return static_cast<u64>(__double_as_longlong(fma(p, scale, 4503599627370496.0))) & ((1ull << 52) - 1);
     }
 
@@ -419,7 +423,12 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
     target -= before;
     // The tokens up to that step, and in it.
     const float from = static_cast<float>(b), upto = static_cast<float>(b + 1);
-    const int kept = gather(r, h, s, s.kept, kBins, [&](float l) { return (r.step(l) < upto) & (l >= r.bound.l); });
+    // Gathered where they are few, going by the first held ones of each thread.
+    u64 some = 0;
+#pragma unroll
+    for (int e = 0; e < kMask; ++e) some += r.from < r.to && r.step(h[0][e]) < upto;
+    const bool few = static_cast<double>(block_sum64(s, some)) * r.V < static_cast<double>(kBins) * min(r.V, kMask * kThreads);
+    const int kept = few ? gather(r, h, s, s.kept, kBins, [&](float l) { return (r.step(l) < upto) & (l >= r.bound.l); }) : kBins + 1;
     if (tid == 0) s.n = 0;
     __syncthreads();
     if (kept <= kBins)
@@ -532,12 +541,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         if (r.from + c * kMask * kWave < r.to)
 #pragma unroll
             for (int e = 0; e < kMask; ++e) h[c][e] = r.logits[min(r.from + (c * kMask + e) * kWave + lane, a.V - 1)];
-    static_assert(kTable == 4 * kThreads, "the quarters below");
-    const double root = exp2(-tid / static_cast<double>(kTable));
-    s.table[tid] = root;
-    s.table[tid + kThreads] = root * 0.8408964152537145;      // 2^(-1/4)
-    s.table[tid + 2 * kThreads] = root * 0.7071067811865476;  // 2^(-1/2)
-    s.table[tid + 3 * kThreads] = root * 0.5946035575013605;  // 2^(-3/4)
+    if (tid < kTable) s.table[tid] = exp2(-tid / static_cast<double>(kTable));
 #pragma unroll
     for (int c = 0; c < kHeld / kMask; ++c)
         if (r.from + c * kMask * kWave < r.to)
@@ -642,12 +646,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
 
     auto weigh = [&](float l, int i) -> u64 {
         const u64 x = r.weight(s, l);
-        return r.kept(l, i) && r.step(l) < kBins && x >= r.min_w ? x : 0;
+        const int in = static_cast<int>(r.kept(l, i)) & static_cast<int>(r.step(l) < kBins) & static_cast<int>(x >= r.min_w);
+        return in ? x : 0;
     };
     if (by_k || by_p || min_p > 0.0f) {
-        // The kept tokens, where they are few and not gathered yet.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
+        // The kept tokens, where they are few and (top-p) were not found to be many.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
         const float most = min_p > 0.0f ? fminf((fmaxf(-logf(min_p), 0.0f) * 1.001f + 1e-3f) * (r.per_step * temperature), kBins) : kBins;
-        if (n > kBins)
+        if (n > kBins && !by_p)
             n = gather(r, h, s, s.kept, kBins, [&](float l) { return (l >= r.bound.l) & (r.step(l) < most); });
         if (n <= kBins) {
             const int per = (a.V + kList - 1) / kList;
@@ -696,7 +701,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
     if (by_k || by_p || min_p > 0.0f)
         id = pick(r, s, weigh, target, weight, total);
     else
-        id = pick(r, s, [&](float l, int) { return r.step(l) < kBins ? r.weight(s, l) : 0; }, target, weight, total);
+        id = pick(r, s, [&](float l, int) {
+            const u64 x = r.weight(s, l);
+            return r.step(l) < kBins ? x : 0;
+        }, target, weight, total);
     if (tid == 0) answer(id, static_cast<double>(weight) / static_cast<double>(total));
 }
 
