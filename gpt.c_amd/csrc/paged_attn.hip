@@ -72,6 +72,21 @@ struct Tile<float, DP, R> {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) v[i][h][c] = 0;
     }
+    // Takes out what is not finite; whether there was any.
+    __device__ __forceinline__ bool take_out() {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t w = finite_part<float>(v[i][h][c]);
+                    any |= w != v[i][h][c];
+                    v[i][h][c] = w;
+                }
+        return any;
+    }
     __device__ __forceinline__ void scores(const Q &q, f32x4 (&s)[1]) const {
         s[0] = zero4();
 #pragma unroll
@@ -140,6 +155,18 @@ struct Tile<__bf16, DP, R> {
 #pragma unroll
                 for (int c = 0; c < kWords; ++c) v[j][c] = 0;
     }
+    __device__ __forceinline__ bool take_out() {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < kWords; ++c) {
+                const uint32_t w = finite_part<__bf16>(v[j][c]);
+                any |= w != v[j][c];
+                v[j][c] = w;
+            }
+        return any;
+    }
     __device__ __forceinline__ void scores(const Q &q, f32x4 (&s)[2]) const {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -181,6 +208,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     constexpr int kRow = DP + 4;  // floats of an LDS row: the four lanes of a row fall on other banks than its neighbours
     __shared__ __attribute__((aligned(16))) float o_s[kWaves][kPagedRows][kRow];
     __shared__ float m_s[kWaves][kPagedRows], l_s[kWaves][kPagedRows];
+    __shared__ bool again_s[kWaves];
 
     const int item = blockIdx.x / a.KV, kv = blockIdx.x - item * a.KV;
     if (item >= a.head[1]) return;
@@ -224,6 +252,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
         x.load(kp, vp, n, g, a.D);
     };
 
+    bool again = false;  // see rows_by_key
     float m = -INFINITY, l = 0.0f;
     f32x4 o[DP / 16];
 #pragma unroll
@@ -231,6 +260,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     auto step = [&](Step &x, int i) {
         const int key = it.key0 + (w + kWaves * i) * kKeys;
         if (key + kKeys > total) x.clear_values(g, total - key);
+        if (key + kKeys > first_end) again |= x.take_out();
         f32x4 s[Step::kGroups];
         x.scores(q, s);
 #pragma unroll
@@ -286,12 +316,20 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
         m_s[w][n] = m;
         l_s[w][n] = l;
     }
+    again = __any(again);
+    if (lane == 0) again_s[w] = again;
 #pragma unroll
     for (int j = 0; j < DP / 16; j += 4)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             *reinterpret_cast<f32x4 *>(&o_s[w][n][Step::dim(j, g, r)]) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
     __syncthreads();
+    if (again_s[0] | again_s[1] | again_s[2] | again_s[3]) {
+        constexpr int kEach = kPagedRows / kWaves;
+        rows_by_key<T>(a, it, kv, it.row0 + kEach * w, kEach,
+                       (static_cast<int64_t>(it.part) * a.KV + kv) * kPagedRows + kEach * w);
+        return;
+    }
     const int r = tid >> 4;
     float big = m_s[0][r];
 #pragma unroll

@@ -69,4 +69,62 @@ __device__ __forceinline__ f32x4 mfma_bf16(const uint32_t (&a)[4], const uint32_
 __device__ __forceinline__ void settled(f32x4 &x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void finished(f32x4 &x) { asm volatile("s_nop 15" : "+a"(x)); }
 
+// ---- values that are no numbers, in the tokens that some rows of a tile must not see ----
+//
+// A hidden key's weight is 0, but 0 times NaN or infinity is not.  So in the tiles where keys are hidden from some
+// rows, values that are not finite are taken out of the products, and an item where there was one is done again, one
+// key after the other.
+
+// A 32-bit word of T values without those that are not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u ? 0 : w;
+    if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+    if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+    return w;
+}
+
+// Query rows row0 .. row0 + count - 1 of an item by one wave, whose lanes hold two values of a head each.  `slot`:
+// the workspace row of row0.
+template <typename T>
+__device__ __forceinline__ void rows_by_key(const PagedAttnParams &a, const PagedItem &it, int kv, int row0, int count,
+                                            int64_t slot) {
+    const int d0 = threadIdx.x & 63, d1 = d0 + 64;
+    const bool in0 = d0 < a.D, in1 = d1 < a.D;
+    const int *table = a.table + it.table;
+    for (int i = 0; i < count; ++i) {
+        const int row = row0 + i, token = row / a.group;
+        if (row >= it.rows || it.tok0 + token >= a.rows) return;
+        const int head = kv * a.group + row - token * a.group;
+        const float *q = a.q + static_cast<int64_t>(it.tok0 + token) * a.q_stride + static_cast<int64_t>(head) * a.D;
+        const float q0 = in0 ? q[d0] : 0.0f, q1 = in1 ? q[d1] : 0.0f;
+        float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        const int end = min(it.past + token + 1, it.key1);
+        for (int key = it.key0; key < end; ++key) {
+            const int64_t page = table[key >> a.page_shift];
+            const int64_t at = (((page * a.KV + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * a.D;
+            const T *k = static_cast<const T *>(a.k) + at, *v = static_cast<const T *>(a.v) + at;
+            float s = in0 ? q0 * static_cast<float>(k[d0]) : 0.0f;
+            if (in1) s = fmaf(q1, static_cast<float>(k[d1]), s);
+            s = wave_sum(s) * a.scale_log2;
+            const float top = fmaxf(m, s), base = top == -INFINITY ? 0.0f : top;
+            const float f = fast_exp2(m - base), p = fast_exp2(s - base);
+            l = fmaf(l, f, p);
+            if (in0) o0 = fmaf(o0, f, p * static_cast<float>(v[d0]));
+            if (in1) o1 = fmaf(o1, f, p * static_cast<float>(v[d1]));
+            m = top;
+        }
+        float *dst = a.part_o + (slot + i) * a.D, scale = 1.0f;
+        if (it.part < 0) {
+            dst = a.out + (static_cast<int64_t>(it.tok0 + token) * a.H + head) * a.D;
+            scale = 1.0f / l;
+        } else if (d0 == 0) {
+            a.part_ml[2 * (slot + i)] = m;
+            a.part_ml[2 * (slot + i) + 1] = l;
+        }
+        if (in0) dst[d0] = o0 * scale;
+        if (in1) dst[d1] = o1 * scale;
+    }
+}
+
 }  // namespace gptc

@@ -42,10 +42,11 @@ __device__ __forceinline__ void parts_of(uint32_t x0, uint32_t x1, uint32_t (&p)
 }
 
 template <typename T, int DP, Rows R>
-__global__ __launch_bounds__(kThreadsOf<T>) void paged_wide_kernel(const PagedAttnParams a) {
+__global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const PagedAttnParams a) {
     using S = Shape<T, DP>;
     constexpr int kThreads = kThreadsOf<T>, kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
+    __shared__ int again_s;  // see rows_by_key
 
     const int item = blockIdx.x / a.KV, kv = blockIdx.x - item * a.KV;
     if (item >= a.head[3]) return;
@@ -116,6 +117,7 @@ __global__ __launch_bounds__(kThreadsOf<T>) void paged_wide_kernel(const PagedAt
             load_words<T, kVWords, R>(vr[j], vpool + at * a.D, v_dim, a.D);
         }
     };
+    const int item_end = it.past + it.row0 / a.group + 1;  // of the item's first row
     auto store_tile = [&](uint16_t *buf, int key) {
         uint16_t *kb = buf, *vb = buf + kParts * S::kKPart;
 #pragma unroll
@@ -139,6 +141,18 @@ __global__ __launch_bounds__(kThreadsOf<T>) void paged_wide_kernel(const PagedAt
                 if (key + v_key + 16 * (j / 4) + j % 4 >= total)
 #pragma unroll
                     for (int i = 0; i < kVWords; ++i) vr[j][i] = 0;
+        }
+        if (key + kKeys > item_end) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < kVWords; ++i) {
+                    const uint32_t x = finite_part<T>(vr[j][i]);
+                    any |= x != vr[j][i];
+                    vr[j][i] = x;
+                }
+            if (any) again_s = 1;
         }
 #pragma unroll
         for (int i = 0; i < kVDims; ++i) {
@@ -243,6 +257,8 @@ __global__ __launch_bounds__(kThreadsOf<T>) void paged_wide_kernel(const PagedAt
     load_pages(it.key0);
     load_tile(it.key0);
     load_pages(it.key0 + kKeys);
+    if (tid == 0) again_s = 0;
+    __syncthreads();
     int turn = 0;
     for (int key = it.key0; key < it.key1; key += kKeys, turn ^= 1) {
         uint16_t *buf = lds + turn * S::kBuffer;
@@ -257,6 +273,10 @@ __global__ __launch_bounds__(kThreadsOf<T>) void paged_wide_kernel(const PagedAt
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) finished(o[c]);
     l = sum4_rows(l);
+    if (again_s != 0) {  // set before the last tile's barrier at the latest
+        rows_by_key<T>(a, it, kv, it.row0 + 16 * w, 16, (static_cast<int64_t>(it.part + w) * a.KV + kv) * kPagedRows);
+        return;
+    }
     if (!live) return;
     float *dst;
     float scale = 1.0f;

@@ -297,6 +297,42 @@ def test_large_scores_and_far_positions(rt, dtype):
     pool.free()
 
 
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("H, KV, D", [(1, 1, 64), (4, 2, 128), (3, 1, 40), (2, 2, 33)])
+@pytest.mark.parametrize("fresh", [20, 150])
+def test_a_later_tokens_values_stay_hidden(rt, dtype, fresh, H, KV, D):
+    """NaN and infinities in the keys and values of some new tokens: rows before them are what they are without, and
+    rows that see a value that is not finite are not finite in its place alone."""
+    pool = Pool(rt, [45], [fresh], H, KV, D, 16, dtype, seed=fresh)
+    kept = pool.fill([45 + fresh])
+    pool.set()
+    q = pool.normal(fresh, H, D)
+    tq, out = rt.from_numpy(q.reshape(fresh, -1)), rt.empty((fresh, H * D))
+    bad = [(fresh // 3, D - 1, float("nan")), (fresh // 2, 3, float("inf")), (fresh - 2, 0, float("-inf"))]
+    for i, d, x in bad:
+        page, slot = pool.rows(0, 45 + i, 46 + i)
+        pool.v[0][page[0], :, slot[0], d] = x
+    # A key that is no number: for its own row and the rows after it everything is lost.
+    page, slot = pool.rows(0, 45 + fresh - 1, 45 + fresh)
+    pool.k[0][page[0], :, slot[0], 0] = float("nan")
+    torch.cuda.synchronize()
+    pool.plan.attention(0, tq, out)
+    got = rt.to_numpy(out).reshape(fresh, H, D)
+    want, bound = attention(q.astype(np.float64), kept[0], 45, H, KV, D)
+    for i in range(fresh):
+        if i == fresh - 1:
+            assert np.isnan(got[i]).all()
+            continue
+        seen = {d for j, d, _ in bad if j <= i}
+        fine = [d for d in range(D) if d not in seen]
+        assert (np.abs(got[i][:, fine] - want[i][:, fine]) <= bound[i]).all(), i
+        for d in seen:
+            assert not np.isfinite(got[i][:, d]).any(), (i, d)
+    pool.free()
+    rt.free(tq)
+    rt.free(out)
+
+
 def test_two_layers_and_shared_prefix(rt):
     """Two sequences read the same first pages; each layer has its own."""
     pool = Pool(rt, [64, 64], [1, 2], 4, 4, 64, 32, gptc.F32, layers=2, seed=4)
