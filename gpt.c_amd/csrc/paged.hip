@@ -207,8 +207,11 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
                 "Expected room for sequences, tokens and lengths, but got %d, %d, %d.", max_seqs, max_tokens, max_len);
     CHECK_ERROR(max_len > (1 << 30), "Sequences of up to 2^30 tokens are supported, but got max_len = %d.", max_len);
     const int group = n_heads / cache->n_kv_heads;
-    CHECK_ERROR(static_cast<int64_t>(max_tokens) * group > (1 << 30),
-                "max_tokens = %d with %d heads per kv head is too large.", max_tokens, group);
+    // What the grids and the page lists can hold.
+    CHECK_ERROR(max_tokens > (1 << 22) || static_cast<int64_t>(max_tokens) * n_heads > (1 << 26),
+                "max_tokens = %d with %d heads is too large.", max_tokens, n_heads);
+    CHECK_ERROR(max_seqs > (1 << 20) || static_cast<int64_t>(max_seqs) * ((max_len + cache->page - 1) / cache->page) > (1 << 28),
+                "%d sequences of %d tokens have too many pages.", max_seqs, max_len);
     auto *p = static_cast<gptc_paged_plan_t *>(mallocCheck(sizeof(gptc_paged_plan_t)));
     memset(p, 0, sizeof(*p));
     p->cache = cache;
@@ -602,7 +605,7 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.n_items = capturing ? plan->item_cap : plan->n_items;
     a.n_wide = capturing ? plan->wide_cap : plan->n_wide;
     a.n_merges = capturing ? plan->merge_cap : plan->n_merges;
-    a.many_parts = capturing || plan->max_parts > 8;
+    a.many_parts = capturing || plan->max_parts > kPagedFewParts;
     a.merge_rows = capturing ? kPagedRows : plan->merge_rows;
     a.bf16 = c->dtype == GPTC_BF16;
     a.vec = D % (a.bf16 ? 8 : 4) == 0 && aligned16(a.q) && aligned16(a.out);

@@ -360,9 +360,11 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     }
 }
 
-// Joins the parts of rows whose keys were cut, few parts: 16 rows a workgroup, 16 threads a row.
+// Joins the parts of rows whose keys were cut, up to kPagedFewParts: 16 rows a workgroup, 16 threads a row.  Products and
+// sums are rounded one by one here and below, and in one order up to kPagedFewParts, so that both kernels give the same.
 template <bool VEC>
 __global__ __launch_bounds__(256) void paged_merge_few_kernel(const PagedAttnParams a) {
+#pragma clang fp contract(off)
     const int i = blockIdx.x / a.KV, kv = blockIdx.x - i * a.KV;
     if (i >= a.head[2]) return;
     const PagedMerge mg = a.merges[i];
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(256) void paged_merge_few_kernel(const PagedAttnPar
         for (int p = 0; p < mg.n; ++p) {
             const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
             const float f = ml[0] == -INFINITY ? 0.0f : fast_exp2(ml[0] - big);
-            sum = fmaf(ml[1], f, sum);
+            sum += ml[1] * f;
             y += f * load4<VEC>(a.part_o + (first + p * next) * a.D, d, a.D);
         }
         store4<VEC>(dst, d, a.D, y / sum);
@@ -396,7 +398,8 @@ constexpr int kMaxParts = kPagedTarget + 1;  // a tile is cut into at most targe
 
 template <bool VEC>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedAttnParams a) {
-    __shared__ float f_s[kMaxParts];
+#pragma clang fp contract(off)
+    __shared__ float f_s[kMaxParts], l_s[kPagedFewParts];
     __shared__ float red[2][kMergeThreads / 64];
     __shared__ __attribute__((aligned(16))) float y_s[kMergeThreads][4];
     const int i = blockIdx.x / (a.KV * a.merge_rows), left = blockIdx.x - i * a.KV * a.merge_rows;
@@ -419,13 +422,18 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
         const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
         const float f = ml[0] == -INFINITY ? 0.0f : fast_exp2(ml[0] - big);
         f_s[p] = f;
-        sum = fmaf(ml[1], f, sum);
+        if (p < kPagedFewParts) l_s[p] = ml[1] * f;
+        sum += ml[1] * f;
     }
     sum = wave_sum(sum);
     if ((tid & 63) == 0) red[1][w] = sum;
     __syncthreads();
     sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const int lanes = a.D <= 64 ? 16 : 32, groups = kMergeThreads / lanes;  // 4 values a thread
+    if (mg.n <= kPagedFewParts) {
+        sum = 0.0f;
+        for (int p = 0; p < mg.n; ++p) sum += l_s[p];
+    }
+    const int lanes = a.D <= 64 ? 16 : 32, groups = kMergeThreads / lanes;  // 4 values a thread; kPagedFewParts groups or more
     const int q = tid / lanes, d = tid % lanes * 4;
     f32x4 y = zero4();
     if (d < a.D) {

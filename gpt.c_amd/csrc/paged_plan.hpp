@@ -39,6 +39,8 @@ constexpr int paged_wide_keys(int dtype, int head_dim) {
 constexpr int kPagedTarget = 1024;
 constexpr int kPagedWideTarget = 512;
 
+constexpr int kPagedFewParts = 8;  // see launch_paged_attention
+
 // The lists of a step: items, wide items, and what is to be joined afterwards.
 struct PagedLists {
     PagedItem *items, *wide;

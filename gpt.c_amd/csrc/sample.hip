@@ -721,6 +721,7 @@ extern "C" void gptc_sample_cuda(const tensor_t *logits, const tensor_t *params,
     check_gpu(ids, "ids");
     const int V = last_dim(logits), rows = leading_rows(logits);
     CHECK_ERROR(logits->length > 0 && V > (1 << 24), "Vocabularies of up to 2^24 tokens are supported, but got %d.", V);
+    CHECK_ERROR(rows > (1 << 22), "Up to 2^22 rows are supported, but got %d.", rows);
     CHECK_ERROR(params->length != 4 && params->length != 4 * static_cast<int64_t>(rows),
                 "Expected 4 parameters, or 4 for each of %d rows, but got %d.", rows, params->length);
     CHECK_ERROR(u->length != rows, "Expected %d random numbers, but got %d.", rows, u->length);

@@ -366,8 +366,8 @@ long long gptc_decode_noalloc_scratch_floats(void);
  * gptc_argmax_cuda(logits, ids)
  *   ids[r] = first index of the maximum of logits row r (greedy decoding).
  * gptc_sample_cuda(logits, params, u, ids, prob)
- *   Draws a token of every row of logits (rows, V), V <= 2^24, from the random
- *   number u[r] of [0, 1).  params (4), or (rows, 4) for settings per row:
+ *   Draws a token of every row of logits (rows, V), rows <= 2^22, V <= 2^24, from
+ *   the random number u[r] of [0, 1).  params (4), or (rows, 4) for settings per row:
  *   temperature, top_k, top_p, min_p, whole numbers held in floats where they
  *   count.  With the tokens ordered by logit, equal ones by index, and weights
  *   exp((logit - maximum) / temperature): top_k keeps the first top_k tokens

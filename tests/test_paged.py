@@ -54,6 +54,9 @@ REFUSALS = {
     "unaligned pages": ("cache(k=[4100])", "16-byte aligned"),
     "pages without a runtime": ("gptc.PagedCache(rt, 1, 8, 16, 2, 4)", "runtime_init"),
     "heads no multiple": ("plan(heads=3)", "multiple of the cache's 2 kv heads"),
+    "too many tokens for the grid": ("plan(tokens=(1 << 22) + 1)", "is too large"),
+    "too many rows for the grid": ("plan(tokens=1 << 20, heads=128)", "is too large"),
+    "too many pages": ("plan(seqs=1 << 20, length=1 << 20)", "too many pages"),
     "no room": ("plan(seqs=0)", "Expected room"),
     "too many sequences": ("plan().set([0] * 4, [1] * 4, [[0], [1], [2], [3]])", "room for 3 sequences"),
     "negative past": ("plan().set([-1], [1], [[0]])", "-1 tokens"),
@@ -161,6 +164,7 @@ SAMPLE_REFUSALS = {
     "random numbers": ("sample(gpu(3, 8), gpu(4), gpu(2), gpu(3))", "Expected 3 random numbers"),
     "ids": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(4))", "Expected 3 ids"),
     "shares": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3), gpu(2))", "Expected 3 probabilities"),
+    "rows": ("sample(gpu((1 << 22) + 1, 1), gpu(4), gpu(1), gpu(1))", "Up to 2^22 rows"),
     "vocabulary": ("sample(gpu(1, (1 << 24) + 1), gpu(4), gpu(1), gpu(1))", "up to 2^24 tokens"),
     "without a runtime": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3))", "runtime_init"),
 }
