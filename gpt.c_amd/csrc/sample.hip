@@ -30,11 +30,9 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kChunk = 8;            // logits of a thread whose weights are formed side by side
-constexpr int kMask = 24;            // logits of a thread that are looked through together
-constexpr int kHeld = 4 * kMask;     // logits of a thread that stay in registers
+constexpr int kChunk = 8;            // logits of a thread that are worked on together, and that are on their way
 constexpr int kBins = 8192;          // of a histogram; tokens that can be gathered
 constexpr int kList = kThreads;      // tokens that can be ranked
 constexpr int kTable = 32;            // entries of 8 bytes: one for every two LDS banks, so lanes never collide
@@ -59,9 +57,8 @@ struct Lds {
     u64 list_w[kList];
     u64 ahead[kList];
     double table[kTable];  // 2^(-j / 32)
-    u64 wave_sum[2 * kWaves];
+    u64 wave_sum[kWaves];
     float wave_max[kWaves];
-    int wave_idx[kWaves];
     uint32_t key_lo, key_hi;
     int n, found;
     u64 before;
@@ -124,8 +121,7 @@ __device__ __forceinline__ u64 block_sum64(Lds &s, u64 v, u64 *upto = nullptr) {
 struct Row {
     const float *logits;
     int V;
-    int from, to;            // the wave's stretch of the held logits
-    int rest_from, rest_to;  // and of the others
+    int from, to;  // the wave's stretch of the vocabulary
     float M;
     double per_entry;  // the weight is 2^(-(M - l) per_entry / kTable)
     int shift;
@@ -162,48 +158,29 @@ struct Row {
     }
 
     // Tokens i0 + lane + 64 e; -inf from `end` on.
-    template <int N>
-    __device__ __forceinline__ void load(float (&l)[N], int i0, int lane, int end) const {
-        if (i0 + N * kWave <= end) {
+    __device__ __forceinline__ void load(float (&l)[kChunk], int i0, int lane, int end) const {
+        if (i0 + kChunk * kWave <= end) {
             const float *at = logits + i0 + lane;
 #pragma unroll
-            for (int e = 0; e < N; ++e) l[e] = at[e * kWave];
+            for (int e = 0; e < kChunk; ++e) l[e] = at[e * kWave];
 #pragma unroll
-            for (int e = 0; e < N; ++e) l[e] = plain(l[e]);
+            for (int e = 0; e < kChunk; ++e) l[e] = plain(l[e]);
             return;
         }
 #pragma unroll
-        for (int e = 0; e < N; ++e) l[e] = logits[min(i0 + lane + e * kWave, V - 1)];
+        for (int e = 0; e < kChunk; ++e) l[e] = logits[min(i0 + lane + e * kWave, V - 1)];
 #pragma unroll
-        for (int e = 0; e < N; ++e) l[e] = i0 + lane + e * kWave < end ? plain(l[e]) : -INFINITY;
+        for (int e = 0; e < kChunk; ++e) l[e] = i0 + lane + e * kWave < end ? plain(l[e]) : -INFINITY;
     }
 };
 
 // A wave's share of n tokens: contiguous, in whole turns of its lanes.
 __device__ __forceinline__ int stretch(int n) { return (n + kThreads - 1) / kThreads * kWave; }
 
-typedef float Held[kHeld / kMask][kMask];
-
-// f(l, i) over the wave's logits: l[e] is that of token i + 64 e, -inf past the stretch's end.  For what takes a few
-// instructions a logit: it is written out for every register.
+// f(l, i) over tokens from .. to of a wave in chunks: l[e] is the logit of token i + 64 e, -inf from `to` on.  The next
+// chunk is on its way while this one is worked on.
 template <typename F>
-__device__ __forceinline__ void each_held(const Row &r, const Held &h, F f) {
-    const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int c = 0; c < kHeld / kMask; ++c)
-        if (r.from + c * kMask * kWave < r.to) f(h[c], r.from + c * kMask * kWave + lane);
-#pragma unroll 1
-    for (int i = r.rest_from; i < r.rest_to; i += kMask * kWave) {
-        float l[kMask];
-        r.load(l, i, lane, r.rest_to);
-        f(l, i + lane);
-    }
-}
-
-// The same in chunks that are read again, the next one while this one is worked on: for what takes many instructions
-// (written out for every register, the weights alone are more code than the instruction cache holds).
-template <typename F>
-__device__ __forceinline__ void each_again(const Row &r, int from, int to, F f) {
+__device__ __forceinline__ void each(const Row &r, int from, int to, F f) {
     const int lane = threadIdx.x & (kWave - 1);
     float l[kChunk], next[kChunk];
     if (from < to) r.load(l, from, lane, to);
@@ -216,23 +193,18 @@ __device__ __forceinline__ void each_again(const Row &r, int from, int to, F f) 
     }
 }
 
-template <typename F>
-__device__ __forceinline__ void each_again(const Row &r, F f) {
-    for (int half = 0; half < 2; ++half) each_again(r, half ? r.rest_from : r.from, half ? r.rest_to : r.to, f);
-}
-
 // Gathers the tokens for which want(l); returns how many there are, of which the first `room` were written.  Their
 // order is that of the waves' turns, so nothing may depend on it.  A token that the bound leaves out by its index
 // alone is written as one of no weight.
 template <typename F>
-__device__ __forceinline__ int gather(const Row &r, const Held &h, Lds &s, Token *to, int room, F want) {
+__device__ __forceinline__ int gather(const Row &r, Lds &s, Token *to, int room, F want) {
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    each_held(r, h, [&](const float (&l)[kMask], int i) {
+    each(r, r.from, r.to, [&](const float (&l)[kChunk], int i) {
         uint32_t mask = 0;
 #pragma unroll
-        for (int e = 0; e < kMask; ++e) mask |= want(l[e]) ? 1u << e : 0u;
+        for (int e = 0; e < kChunk; ++e) mask |= want(l[e]) ? 1u << e : 0u;
         if (mask == 0) return;
         int at = atomicAdd(&s.n, __popc(mask));
         while (mask != 0) {
@@ -250,6 +222,35 @@ __device__ __forceinline__ int gather(const Row &r, const Held &h, Lds &s, Token
     }
     __syncthreads();
     return n;
+}
+
+// The same where few tokens are wanted: one comparison of wave masks for eight logits, most of which end there.
+template <typename F>
+__device__ __forceinline__ int gather_few(const Row &r, Lds &s, Token *to, int room, F want) {
+    const u64 below = (1ull << (threadIdx.x & (kWave - 1))) - 1;
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    each(r, r.from, r.to, [&](const float (&l)[kChunk], int i) {
+        u64 who[kChunk], any = 0;
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            who[e] = __ballot(want(l[e]));
+            any |= who[e];
+        }
+        if (any == 0) return;
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            if (who[e] == 0) continue;
+            int at = 0;
+            if (below == 0) at = atomicAdd(&s.n, __popcll(who[e]));
+            at = __builtin_amdgcn_readfirstlane(at) + __popcll(who[e] & below);
+            const int j = i + e * kWave;
+            if ((who[e] & (below + 1)) != 0 && at < room) to[at] = Token{r.kept(l[e], j) ? l[e] : -INFINITY, j};
+        }
+    });
+    __syncthreads();
+    return s.n;
 }
 
 // ahead[i] = the sum over j < n of value(j) where before(j, i), for i < n <= kList: the pairs are shared out over
@@ -316,50 +317,61 @@ __device__ __forceinline__ void clear(Lds &s) {
 }
 
 // The first token, in the order of the vocabulary, at which the sum of weigh(l, i) passes target(total); its
-// weight, and the total.  Stretches first, then stretches of the one it lies in, then its tokens.
+// weight, and the total.  Stretches first, then stretches of the one it lies in, then its tokens.  Where the total is
+// known (not 0), the stretches are summed from the nearer end only as far as they have to.
 template <typename W, typename T>
 __device__ __forceinline__ int pick(const Row &r, Lds &s, W weigh, T target, u64 &weight, u64 &total) {
     const int w = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
     auto sum_of = [&](int from, int to) {
         u64 sum = 0;
-        each_again(r, from, to, [&](const float (&l)[kChunk], int i) {
+        each(r, from, to, [&](const float (&l)[kChunk], int i) {
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) sum += weigh(l[e], i + e * kWave);
         });
         return sum;
     };
-    const int held = min(r.V, kHeld * kThreads);
-    u64 first = 0, second = 0;
-    each_again(r, [&](const float (&l)[kChunk], int i) {
-        u64 sum = 0;
-#pragma unroll
-        for (int e = 0; e < kChunk; ++e) sum += weigh(l[e], i + e * kWave);
-        (i - lane < held ? first : second) += sum;
-    });
-    first = wave_sum64(first);
-    second = wave_sum64(second);
-    __syncthreads();
-    if (lane == 0) {
-        s.wave_sum[w] = first;
-        s.wave_sum[kWaves + w] = second;
+    int lo, hi;
+    u64 left;
+    if (total != 0) {
+        constexpr int kSteps = 16;
+        left = target(total);
+        const bool back = left > total / 2;
+        if (back) left = total - 1 - left;
+        const int step = (r.V + kSteps - 1) / kSteps;
+        lo = back ? max(r.V - step, 0) : 0;
+        hi = back ? r.V : min(step, r.V);
+#pragma unroll 1
+        while (true) {
+            const int len = stretch(hi - lo), a = min(lo + w * len, hi);
+            const u64 sum = block_sum64(s, sum_of(a, min(a + len, hi)));
+            if (left < sum || (back ? lo == 0 : hi == r.V)) {
+                if (back) left = sum - 1 - min(left, sum - 1);
+                break;
+            }
+            left -= sum;
+            lo = back ? max(lo - step, 0) : hi;
+            hi = back ? lo + step : min(hi + step, r.V);
+        }
+    } else {
+        const u64 sum = wave_sum64(sum_of(r.from, r.to));
+        __syncthreads();
+        if (lane == 0) s.wave_sum[w] = sum;
+        __syncthreads();
+        for (int i = 0; i < kWaves; ++i) total += s.wave_sum[i];
+        left = target(total);
+        int q = 0;
+        while (q < kWaves - 1 && left >= s.wave_sum[q]) left -= s.wave_sum[q++];
+        const int len = stretch(r.V);
+        lo = min(q * len, r.V);
+        hi = min(lo + len, r.V);
     }
-    __syncthreads();
-    total = 0;
-    for (int i = 0; i < 2 * kWaves; ++i) total += s.wave_sum[i];
-    u64 left = target(total);
-    int q = 0;
-    while (q < 2 * kWaves - 1 && left >= s.wave_sum[q]) left -= s.wave_sum[q++];
-    const int from = q < kWaves ? 0 : held, upto = q < kWaves ? held : r.V;
-    int len = stretch(upto - from);
-    int lo = min(from + (q % kWaves) * len, upto), hi = min(lo + len, upto);
     while (hi - lo > kChunk * kWave) {
-        len = stretch(hi - lo);
-        const int a = min(lo + w * len, hi);
+        const int len = stretch(hi - lo), a = min(lo + w * len, hi);
         const u64 sum = wave_sum64(sum_of(a, min(a + len, hi)));
         __syncthreads();
         if (lane == 0) s.wave_sum[w] = sum;
         __syncthreads();
-        q = 0;
+        int q = 0;
         while (q < kWaves - 1 && left >= s.wave_sum[q]) left -= s.wave_sum[q++];
         lo = min(lo + q * len, hi);
         hi = min(lo + len, hi);
@@ -390,12 +402,13 @@ __device__ __forceinline__ u64 head_of(double share, u64 total) {
 }
 
 //
-// Returns how many tokens were gathered into s.kept on the way, all that are kept among them, or kBins + 1.
-__device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass, u64 target, double share) {
+// Returns how many tokens were gathered into s.kept on the way, all that are kept among them, or kBins + 1; and what
+// is kept, in what the target counts, in `kept_sum` (0: not known).
+__device__ __forceinline__ int bound_at(Row &r, Lds &s, bool mass, u64 target, double share, u64 &kept_sum) {
     const int tid = threadIdx.x;
     clear(s);
     const bool all = r.bound.l == -INFINITY;
-    each_again(r, [&](const float (&l)[kChunk], int i) {
+    each(r, r.from, r.to, [&](const float (&l)[kChunk], int i) {
         u64 w[kChunk];
         if (mass) {
 #pragma unroll
@@ -419,16 +432,21 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
     }
     u64 before;
     int b = locate(s, target, before);
+    kept_sum = 0;
     if (b < 0) return kBins + 1;  // fewer tokens than that have any weight
     target -= before;
+    u64 ahead = before;
     // The tokens up to that step, and in it.
     const float from = static_cast<float>(b), upto = static_cast<float>(b + 1);
-    // Gathered where they are few, going by the first held ones of each thread.
+    // Gathered where they are few, going by the first ones of each wave.
     u64 some = 0;
+    const int first_to = min(r.from + kChunk * kWave, r.to);
+    each(r, r.from, first_to, [&](const float (&l)[kChunk], int) {
 #pragma unroll
-    for (int e = 0; e < kMask; ++e) some += r.from < r.to && r.step(h[0][e]) < upto;
-    const bool few = static_cast<double>(block_sum64(s, some)) * r.V < static_cast<double>(kBins) * min(r.V, kMask * kThreads);
-    const int kept = few ? gather(r, h, s, s.kept, kBins, [&](float l) { return (r.step(l) < upto) & (l >= r.bound.l); }) : kBins + 1;
+        for (int e = 0; e < kChunk; ++e) some += r.step(l[e]) < upto;
+    });
+    const bool few = static_cast<double>(block_sum64(s, some)) * r.V < static_cast<double>(kBins) * min(r.V, kChunk * kThreads);
+    const int kept = few ? gather(r, s, s.kept, kBins, [&](float l) { return (r.step(l) < upto) & (l >= r.bound.l); }) : kBins + 1;
     if (tid == 0) s.n = 0;
     __syncthreads();
     if (kept <= kBins)
@@ -439,7 +457,7 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
             if (m < kList) s.list[m] = t;
         }
     __syncthreads();
-    int n = kept <= kBins ? s.n : gather(r, h, s, s.list, kList, [&](float l) {
+    int n = kept <= kBins ? s.n : gather(r, s, s.list, kList, [&](float l) {
         const float at = r.step(l);
         return (at >= from) & (at < upto) & (l >= r.bound.l);
     });
@@ -458,7 +476,7 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
         }
         __syncthreads();
         uint32_t k0 = 0xffffffffu, k1 = 0;
-        each_again(r, [&](const float (&l)[kChunk], int i) {
+        each(r, r.from, r.to, [&](const float (&l)[kChunk], int i) {
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) {
                 if (!in_group(l[e], i + e * kWave)) continue;
@@ -478,7 +496,7 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
                 const u64 w = r.weight(s, l);
                 target = (target + w - 1) / w;
             }
-            u64 weight, total;
+            u64 weight, total = 0;
             const int i = pick(r, s, [&](float x, int j) { return static_cast<u64>(in_group(x, j)); },
                                [&](u64) { return target - 1; }, weight, total);
             r.bound = Token{l, i};
@@ -487,7 +505,7 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
         const int bits = 32 - __clz(hi - lo), down = bits > 13 ? bits - 13 : 0;
         static_assert(kBins == 1 << 13, "steps of the logits' bits");
         clear(s);
-        each_again(r, [&](const float (&l)[kChunk], int i) {
+        each(r, r.from, r.to, [&](const float (&l)[kChunk], int i) {
 #pragma unroll
             for (int e = 0; e < kChunk; ++e) {
                 if (!in_group(l[e], i + e * kWave)) continue;
@@ -497,18 +515,23 @@ __device__ __forceinline__ int bound_at(Row &r, const Held &h, Lds &s, bool mass
         __syncthreads();
         b = locate(s, target, before);
         target -= before;
+        ahead += before;
         hi -= static_cast<uint32_t>(b) << down;
         const uint32_t width = (1u << down) - 1;
         lo = hi - lo > width ? hi - width : lo;
         const float least = of_key(lo), most = of_key(hi);
-        n = gather(r, h, s, s.list, kList, [&](float l) { return (l >= least) & (l <= most) & (l >= r.bound.l); });
+        n = gather(r, s, s.list, kList, [&](float l) { return (l >= least) & (l <= most) & (l >= r.bound.l); });
     }
     if (tid < n) s.list_w[tid] = !mass ? 1 : r.step(s.list[tid].l) < kBins ? r.weight(s, s.list[tid].l) : 0;
     sum_ahead(s, n, [&](int j, int i) { return ahead_of(s.list[j], s.list[i]); },
               [&](int j) { return s.list_w[j]; });
-    if (tid < n && s.ahead[tid] < target && target <= s.ahead[tid] + s.list_w[tid]) s.bound = s.list[tid];
+    if (tid < n && s.ahead[tid] < target && target <= s.ahead[tid] + s.list_w[tid]) {
+        s.bound = s.list[tid];
+        s.before = s.ahead[tid] + s.list_w[tid];
+    }
     __syncthreads();
     r.bound = s.bound;
+    kept_sum = ahead + s.before;
     return first ? kept : kBins + 1;
 }
 
@@ -525,60 +548,52 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
     Row r;
     r.logits = a.logits + static_cast<int64_t>(row) * a.V;
     r.V = a.V;
-    const int held = min(a.V, kHeld * kThreads);
-    int len = stretch(held);
-    r.from = min(w * len, held);
-    r.to = min(r.from + len, held);
-    len = stretch(a.V - held);
-    r.rest_from = min(held + w * len, a.V);
-    r.rest_to = min(r.rest_from + len, a.V);
+    r.from = min(w * stretch(a.V), a.V);
+    r.to = min(r.from + stretch(a.V), a.V);
     const float *p = a.params + (a.param_rows > 1 ? 4 * row : 0);
     const float temperature = p[0], top_k = p[1], top_p = p[2], min_p = p[3], u = a.u[row];
 
-    Held h;
-#pragma unroll
-    for (int c = 0; c < kHeld / kMask; ++c)
-        if (r.from + c * kMask * kWave < r.to)
-#pragma unroll
-            for (int e = 0; e < kMask; ++e) h[c][e] = r.logits[min(r.from + (c * kMask + e) * kWave + lane, a.V - 1)];
     if (tid < kTable) s.table[tid] = exp2(-tid / static_cast<double>(kTable));
-#pragma unroll
-    for (int c = 0; c < kHeld / kMask; ++c)
-        if (r.from + c * kMask * kWave < r.to)
-#pragma unroll
-            for (int e = 0; e < kMask; ++e)
-                h[c][e] = r.from + (c * kMask + e) * kWave + lane < r.to ? Row::plain(h[c][e]) : -INFINITY;
 
-    // The maximum and its first place.
-    Token best{-INFINITY, a.V};
-    each_held(r, h, [&](const float (&l)[kMask], int i) {
+    auto block_max = [&](float x) {
+        x = wave_max(x);
+        __syncthreads();
+        if (lane == 0) s.wave_max[w] = x;
+        __syncthreads();
+        x = s.wave_max[0];
 #pragma unroll
-        for (int e = 0; e < kMask; ++e)
-            if (l[e] > best.l) best = Token{l[e], i + e * kWave};
-    });
-    const float own_max = best.l;
-    const float top = wave_max(best.l);  // V <= 2^24: indices are floats too
-    best = Token{top, static_cast<int>(-wave_max(best.l == top ? -static_cast<float>(best.i) : -INFINITY))};
-    if (lane == 0) {
-        s.wave_max[w] = best.l;
-        s.wave_idx[w] = best.i;
-    }
-    __syncthreads();
-    best = Token{s.wave_max[0], s.wave_idx[0]};
-    for (int i = 1; i < kWaves; ++i) {
-        const Token o{s.wave_max[i], s.wave_idx[i]};
-        if (ahead_of(o, best)) best = o;
-    }
+        for (int i = 1; i < kWaves; ++i) x = fmaxf(x, s.wave_max[i]);
+        return x;
+    };
     auto answer = [&](int id, double prob) {
         a.ids[row] = static_cast<float>(id);
         if (a.prob != nullptr) a.prob[row] = static_cast<float>(prob);
     };
-    if (best.l == -INFINITY || !(temperature > 0.0f)) {
-        if (tid == 0) answer(best.l == -INFINITY ? -1 : best.i, best.l == -INFINITY ? 0.0 : 1.0);
+    if (!(temperature > 0.0f)) {
+        Token top{-INFINITY, -1};
+        each(r, r.from, r.to, [&](const float (&l)[kChunk], int i) {
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e)
+                if (l[e] > top.l) top = Token{l[e], i + e * kWave};
+        });
+        const float best = block_max(top.l);
+        // The first place, as a float (V <= 2^24); -1 where there is none.
+        const float first = block_max(top.l == best ? -static_cast<float>(top.i) : -INFINITY);
+        if (tid == 0) answer(static_cast<int>(-first), best == -INFINITY ? 0.0 : 1.0);
+        return;
+    }
+    float own_max = -INFINITY;
+    each(r, r.from, r.to, [&](const float (&l)[kChunk], int) {
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) own_max = fmaxf(own_max, l[e]);
+    });
+    const float best = block_max(own_max);
+    if (best == -INFINITY) {
+        if (tid == 0) answer(-1, 0.0);
         return;
     }
     const double inv_t = 1.0 / static_cast<double>(fminf(temperature, 1e30f));
-    r.M = best.l;
+    r.M = best;
     r.shift = a.shift;
     r.per_entry = inv_t * (kTable * 1.4426950408889634);
     r.per_step = static_cast<float>(inv_t * (kBins / ((a.shift + 2) * 0.6931471805599453 * 1.001)));
@@ -600,12 +615,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
             const int last = locate(s, k, before);
             if (last >= 0) {
                 // The smallest of the maxima that were counted.
-                const float least = -wave_max(own < static_cast<float>(last + 1) ? -own_max : -INFINITY);
-                if (lane == 0) s.wave_max[w] = least;
-                __syncthreads();
-                float bound = s.wave_max[0];
-                for (int i = 1; i < kWaves; ++i) bound = fminf(bound, s.wave_max[i]);
-                n = gather(r, h, s, s.list, kList, [&](float l) { return l >= bound; });
+                const float bound = -block_max(own < static_cast<float>(last + 1) ? -own_max : -INFINITY);
+                n = gather_few(r, s, s.list, kList, [&](float l) { return l >= bound; });
             }
         }
         if (n <= kList) {
@@ -640,9 +651,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         }
     }
     int n = kBins + 1;
+    u64 kept_sum = 0;
 #pragma unroll 1
     for (int mass = by_k ? 0 : 1; mass < (by_p ? 2 : 1); ++mass)
-        n = bound_at(r, h, s, mass != 0, mass != 0 ? 0 : static_cast<u64>(top_k), share);
+        n = bound_at(r, s, mass != 0, mass != 0 ? 0 : static_cast<u64>(top_k), share, kept_sum);
 
     auto weigh = [&](float l, int i) -> u64 {
         const u64 x = r.weight(s, l);
@@ -653,7 +665,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         // The kept tokens, where they are few and (top-p) were not found to be many.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
         const float most = min_p > 0.0f ? fminf((fmaxf(-logf(min_p), 0.0f) * 1.001f + 1e-3f) * (r.per_step * temperature), kBins) : kBins;
         if (n > kBins && !by_p)
-            n = gather(r, h, s, s.kept, kBins, [&](float l) { return (l >= r.bound.l) & (r.step(l) < most); });
+            n = gather(r, s, s.kept, kBins, [&](float l) { return (l >= r.bound.l) & (r.step(l) < most); });
         if (n <= kBins) {
             const int per = (a.V + kList - 1) / kList;
             s.ahead[tid] = 0;
@@ -696,7 +708,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         }
     }
     auto target = [&](u64 sum) { return draw_at(u, sum); };
-    u64 weight, total;
+    u64 weight, total = by_p && !(min_p > 0.0f) ? kept_sum : 0;
     int id;
     if (by_k || by_p || min_p > 0.0f)
         id = pick(r, s, weigh, target, weight, total);
