@@ -127,7 +127,8 @@ struct Row {
     int shift;
     float per_step;  // the histogram's steps by logit: monotone, whatever their rounding
     Token bound;
-    u64 min_w;
+    u64 min_w;                  // the least weight that min-p keeps,
+    float min_from, min_upto;   // and where it lies: before `from` every token is kept, from `upto` on none
 
     // NaN counts as -inf, and +inf as the largest number.
     static __device__ __forceinline__ float plain(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f); }
@@ -333,11 +334,12 @@ __device__ __forceinline__ int pick(const Row &r, Lds &s, W weigh, T target, u64
     int lo, hi;
     u64 left;
     if (total != 0) {
-        constexpr int kSteps = 16;
+        // Whole chunks of every thread: part of one takes as long.
+        constexpr int kTurn = kChunk * kThreads;
         left = target(total);
         const bool back = left > total / 2;
         if (back) left = total - 1 - left;
-        const int step = (r.V + kSteps - 1) / kSteps;
+        const int step = (r.V / 16 / kTurn + 1) * kTurn;
         lo = back ? max(r.V - step, 0) : 0;
         hi = back ? r.V : min(step, r.V);
 #pragma unroll 1
@@ -349,8 +351,13 @@ __device__ __forceinline__ int pick(const Row &r, Lds &s, W weigh, T target, u64
                 break;
             }
             left -= sum;
-            lo = back ? max(lo - step, 0) : hi;
-            hi = back ? lo + step : min(hi + step, r.V);
+            if (back) {
+                hi = lo;
+                lo = max(hi - step, 0);
+            } else {
+                lo = hi;
+                hi = min(lo + step, r.V);
+            }
         }
     } else {
         const u64 sum = wave_sum64(sum_of(r.from, r.to));
@@ -402,8 +409,8 @@ __device__ __forceinline__ u64 head_of(double share, u64 total) {
 }
 
 //
-// Returns how many tokens were gathered into s.kept on the way, all that are kept among them, or kBins + 1; and what
-// is kept, in what the target counts, in `kept_sum` (0: not known).
+// Returns how many tokens were gathered into s.kept on the way, all that are kept among them, or kBins + 1; and
+// what is kept after min-p, in what the target counts, in `kept_sum` (0: not known).
 __device__ __forceinline__ int bound_at(Row &r, Lds &s, bool mass, u64 target, double share, u64 &kept_sum) {
     const int tid = threadIdx.x;
     clear(s);
@@ -436,6 +443,7 @@ __device__ __forceinline__ int bound_at(Row &r, Lds &s, bool mass, u64 target, d
     if (b < 0) return kBins + 1;  // fewer tokens than that have any weight
     target -= before;
     u64 ahead = before;
+    if (mass && r.min_upto <= static_cast<float>(b)) return kBins + 1;  // min-p keeps less: the bound is its own
     // The tokens up to that step, and in it.
     const float from = static_cast<float>(b), upto = static_cast<float>(b + 1);
     // Gathered where they are few, going by the first ones of each wave.
@@ -531,7 +539,7 @@ __device__ __forceinline__ int bound_at(Row &r, Lds &s, bool mass, u64 target, d
     }
     __syncthreads();
     r.bound = s.bound;
-    kept_sum = ahead + s.before;
+    if (r.min_from >= upto) kept_sum = ahead + s.before;
     return first ? kept : kBins + 1;
 }
 
@@ -596,10 +604,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
     r.M = best;
     r.shift = a.shift;
     r.per_entry = inv_t * (kTable * 1.4426950408889634);
-    r.per_step = static_cast<float>(inv_t * (kBins / ((a.shift + 2) * 0.6931471805599453 * 1.001)));
+    const double z_most = (a.shift + 2) * 0.6931471805599453 * 1.001;  // (M - l) / T from which on a weight is nothing
+    r.per_step = static_cast<float>(inv_t * (kBins / z_most));
     r.bound = Token{-INFINITY, -1};
     const double one = static_cast<double>(1ull << a.shift);
-    r.min_w = min_p > 0.0f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * one)) : 1;
+    r.min_w = 1;
+    r.min_from = r.min_upto = kBins;
+    if (min_p > 0.0f) {  // (M - l) / T <= -log(min_p), with room for the roundings of both sides
+        r.min_w = static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * one));
+        const double z = fmax(-log(static_cast<double>(min_p)), 0.0), steps = kBins / z_most;
+        r.min_from = static_cast<float>(fmin((z * 0.999 - 1e-3) * steps, kBins));
+        r.min_upto = static_cast<float>(fmin((z * 1.001 + 1e-3) * steps, kBins));
+    }
     const bool by_k = top_k >= 1.0f && top_k < static_cast<float>(a.V), by_p = top_p < 1.0f;
     const double share = fmax(static_cast<double>(top_p), 0.0);
 
@@ -655,6 +671,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
 #pragma unroll 1
     for (int mass = by_k ? 0 : 1; mass < (by_p ? 2 : 1); ++mass)
         n = bound_at(r, s, mass != 0, mass != 0 ? 0 : static_cast<u64>(top_k), share, kept_sum);
+    if (!by_p) kept_sum = 0;  // it counts tokens
 
     auto weigh = [&](float l, int i) -> u64 {
         const u64 x = r.weight(s, l);
@@ -662,10 +679,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         return in ? x : 0;
     };
     if (by_k || by_p || min_p > 0.0f) {
-        // The kept tokens, where they are few and (top-p) were not found to be many.  min_p leaves (M - l) / T <= -log(min_p): a little more is gathered.
-        const float most = min_p > 0.0f ? fminf((fmaxf(-logf(min_p), 0.0f) * 1.001f + 1e-3f) * (r.per_step * temperature), kBins) : kBins;
-        if (n > kBins && !by_p)
-            n = gather(r, s, s.kept, kBins, [&](float l) { return (l >= r.bound.l) & (r.step(l) < most); });
+        // The kept tokens, where they are few: not yet gathered, and not found to be many.
+        if (n > kBins && r.bound.l == -INFINITY)
+            n = gather(r, s, s.kept, kBins, [&](float l) { return (l >= r.bound.l) & (r.step(l) < r.min_upto); });
         if (n <= kBins) {
             const int per = (a.V + kList - 1) / kList;
             s.ahead[tid] = 0;
@@ -708,7 +724,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams a) 
         }
     }
     auto target = [&](u64 sum) { return draw_at(u, sum); };
-    u64 weight, total = by_p && !(min_p > 0.0f) ? kept_sum : 0;
+    u64 weight, total = kept_sum;
     int id;
     if (by_k || by_p || min_p > 0.0f)
         id = pick(r, s, weigh, target, weight, total);

@@ -94,6 +94,11 @@ SETTINGS = {
     "min_p all": (1.0, 0, 1.0, 2.0),
     "all": (0.7, 50, 0.95, 0.02),
     "top_k and top_p": (1.1, 5000, 0.8, 0.0),
+    "top_p of many": (1.3, 0, 0.97, 0.0),
+    "top_p, then less by min_p": (0.9, 0, 0.95, 0.2),
+    "top_p, nothing by min_p": (1.2, 0, 0.9, 1e-5),
+    "top_p and min_p near": (1.0, 0, 0.8, 0.0015),
+    "all, many": (1.4, 4000, 0.9, 1e-4),
     "greedy": (0.0, 40, 0.9, 0.1),
 }
 
