@@ -51,7 +51,7 @@ constexpr int kWideFrom = 64;
 
 // How a list's tiles of rows are cut.
 struct Cutting {
-    int tile, unit, target, whole;
+    int tile, unit, target, least, whole;
     int64_t total, per;
 };
 
@@ -66,12 +66,12 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
                           int dtype, PagedLists &lists) {
     // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose
     // keys take more rounds than `per` is cut evenly: `per` makes about four workgroups per CU (two wide ones) in
-    // all; fewer leave CUs idle in ragged steps, more cost merging.  Parts have kLeast rounds at least, and what takes
-    // no more than `whole` stays whole: one token of 12 heads over 300 keys (5 rounds) takes 7.6 us whole and 9.5 us
-    // in two parts; a prompt of 1024 (16 tiles at most) 23.6 us in parts of 4 tiles and 27 us in parts of 8.
-    constexpr int kLeast = 4;
-    Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 8, 0, 0},
-                      {paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, 4, 0, 0}};
+    // all; fewer leave CUs idle in ragged steps, more cost merging.  Parts have `least` rounds at least (256 keys; wide
+    // ones of 128 or 512 keys take as long or longer), and what takes no more than `whole` stays whole: one token of
+    // 12 heads over 300 fp32 keys (5 rounds) takes 7.6 us whole and 9.5 us in two parts.
+    Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 4, 8, 0, 0},
+                      {paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget,
+                       256 / paged_wide_keys(dtype, head_dim), 256 / paged_wide_keys(dtype, head_dim), 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
         Cutting &c = cut[rows >= kWideFrom];
@@ -79,7 +79,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     }
     for (Cutting &c : cut) {
         c.per = (c.total * n_kv_heads + c.target - 1) / c.target;
-        if (c.per < kLeast) c.per = kLeast;
+        if (c.per < c.least) c.per = c.least;
     }
     lists.n_items = lists.n_wide = lists.n_merges = lists.max_parts = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;

@@ -330,7 +330,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
                        (static_cast<int64_t>(it.part) * a.KV + kv) * kPagedRows + kEach * w);
         return;
     }
-    const int r = tid >> 4;
+    constexpr int kPerRow = 4 * kWaves;  // threads
+    const int r = tid / kPerRow, place = tid % kPerRow;
     float big = m_s[0][r];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) big = fmaxf(big, m_s[i][r]);
@@ -350,9 +351,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     } else {
         const int64_t slot = (static_cast<int64_t>(it.part) * a.KV + kv) * kPagedRows + r;
         dst = a.part_o + slot * a.D;
-        if ((tid & 15) == 0) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * slot) = f32x2{big, sum};
+        if (place == 0) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * slot) = f32x2{big, sum};
     }
-    for (int d = 4 * (tid & 15); d < a.D; d += 64) {
+    for (int d = 4 * place; d < a.D; d += 4 * kPerRow) {
         f32x4 y4 = zero4();
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) y4 += f[i] * *reinterpret_cast<const f32x4 *>(&o_s[i][r][d]);

@@ -23,8 +23,9 @@ namespace {
 
 template <typename T>
 constexpr int kType = sizeof(T) == 4 ? GPTC_F32 : GPTC_BF16;
-template <typename T>
-constexpr int kThreadsOf = paged_wide_rows(kType<T>) / 16 * 64;
+// Groups of 16 rows that a wave takes: two read each operand from LDS once for both.
+template <typename T, int DP>
+constexpr int kGroupsOf = sizeof(T) == 4 && DP == 64 ? 2 : 1;
 
 template <typename T, int DP>
 struct Shape {
@@ -41,10 +42,10 @@ __device__ __forceinline__ void parts_of(uint32_t x0, uint32_t x1, uint32_t (&p)
     split3(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1), p);
 }
 
-template <typename T, int DP, Rows R>
-__global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const PagedAttnParams a) {
+template <typename T, int DP, Rows R, int THREADS>
+__global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnParams a) {
     using S = Shape<T, DP>;
-    constexpr int kThreads = kThreadsOf<T>, kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
+    constexpr int kThreads = THREADS, G = kGroupsOf<T, DP>, kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     __shared__ int again_s;  // see rows_by_key
 
@@ -55,18 +56,22 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int total = it.past + it.rows / a.group;
 
-    // The lane's query row, and the end of its keys.
-    const int row = it.row0 + 16 * w + n;
-    const int token = row / a.group;
-    const bool live = row < it.rows && it.tok0 + token < a.rows;
-    const int end = it.past + token + 1;
-    const int first_end = it.past + (it.row0 + 16 * w) / a.group + 1;  // of the wave's first row, which ends first
+    // The lane's query rows, one of each of the wave's groups, and the end of their keys.
+    const int row0 = it.row0 + 16 * G * w;  // the wave's first row, whose keys end first
+    const int first_end = it.past + row0 / a.group + 1;
     // Nothing of a tile that starts here or later is for this wave.
-    const int wave_end = it.row0 + 16 * w < it.rows ? min(it.past + min(it.row0 + 16 * w + 15, it.rows - 1) / a.group + 1, it.key1) : 0;
-    uint32_t q[3][DP / 32][4];  // [part][c][e]: d = 32c + 8g + 2e, + 1
-    {
-        const float *src = a.q + static_cast<int64_t>(it.tok0 + (live ? token : 0)) * a.q_stride +
-                           (kv * a.group + (live ? row - token * a.group : 0)) * a.D;
+    const int wave_end = row0 < it.rows ? min(it.past + min(row0 + 16 * G - 1, it.rows - 1) / a.group + 1, it.key1) : 0;
+    int row[G], token[G], end[G];
+    bool live[G];
+    uint32_t q[G][3][DP / 32][4];  // [group][part][c][e]: d = 32c + 8g + 2e, + 1
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        row[u] = row0 + 16 * u + n;
+        token[u] = row[u] / a.group;
+        live[u] = row[u] < it.rows && it.tok0 + token[u] < a.rows;
+        end[u] = it.past + token[u] + 1;
+        const float *src = a.q + static_cast<int64_t>(it.tok0 + (live[u] ? token[u] : 0)) * a.q_stride +
+                           (kv * a.group + (live[u] ? row[u] - token[u] * a.group : 0)) * a.D;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
             uint32_t x[2][4];
@@ -75,10 +80,10 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 uint32_t p[3];
-                split3(live ? __builtin_bit_cast(float, x[e / 2][2 * (e % 2)]) : 0.0f,
-                       live ? __builtin_bit_cast(float, x[e / 2][2 * (e % 2) + 1]) : 0.0f, p);
+                split3(live[u] ? __builtin_bit_cast(float, x[e / 2][2 * (e % 2)]) : 0.0f,
+                       live[u] ? __builtin_bit_cast(float, x[e / 2][2 * (e % 2) + 1]) : 0.0f, p);
 #pragma unroll
-                for (int i = 0; i < 3; ++i) q[i][c][e] = p[i];
+                for (int i = 0; i < 3; ++i) q[u][i][c][e] = p[i];
             }
         }
     }
@@ -178,10 +183,15 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
         }
     };
 
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o[DP / 16];
+    float m[G], l[G];
+    f32x4 o[G][DP / 16];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) o[c] = zero4();
+    for (int u = 0; u < G; ++u) {
+        m[u] = -INFINITY;
+        l[u] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) o[u][c] = zero4();
+    }
     auto read4 = [](uint32_t (&x)[4], const uint16_t *p) {
         const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
 #pragma unroll
@@ -189,10 +199,11 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
     };
     auto multiply = [&](const uint16_t *buf, int key) {
         const uint16_t *kb = buf + n * S::kKRow + 8 * g, *vb = buf + kParts * S::kKPart + n * S::kVRow + 8 * g;
-        f32x4 s[kTiles];
+        f32x4 s[G][kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-            s[t] = zero4();
+#pragma unroll
+            for (int u = 0; u < G; ++u) s[u][t] = zero4();
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) {
 #pragma unroll
@@ -200,48 +211,56 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
                     uint32_t k[4];
                     read4(k, kb + j * S::kKPart + 16 * t * S::kKRow + 32 * c);
 #pragma unroll
-                    for (int i = 2 - j; i >= 0; --i) s[t] = mfma_bf16(k, q[i][c], s[t]);
+                    for (int i = 2 - j; i >= 0; --i)
+#pragma unroll
+                        for (int u = 0; u < G; ++u) s[u][t] = mfma_bf16(k, q[u][i][c], s[u][t]);
                 }
             }
         }
+        float base[G];
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) settled(s[t]);
+        for (int u = 0; u < G; ++u) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) s[t] *= a.scale_log2;
-        if (key + kKeys > first_end) {
+            for (int t = 0; t < kTiles; ++t) settled(s[u][t]);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) s[u][t] *= a.scale_log2;
+            if (key + kKeys > first_end) {
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key + 16 * t + 4 * g + r >= end[u]) s[u][t][r] = -INFINITY;
+            }
+            float mx = m[u];
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (key + 16 * t + 4 * g + r >= end) s[t][r] = -INFINITY;
-        }
-        float mx = m;
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][t][r]);
+            mx = max4_rows(mx);
+            base[u] = mx == -INFINITY ? 0.0f : mx;
+            if (__any(mx > m[u])) {
+                const float f = fast_exp2(m[u] - base[u]);
+                l[u] *= f;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
-        mx = max4_rows(mx);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        if (__any(mx > m)) {
-            const float f = fast_exp2(m - base);
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) o[c] *= f;
-            m = mx;
+                for (int c = 0; c < DP / 16; ++c) o[u][c] *= f;
+                m[u] = mx;
+            }
         }
 #pragma unroll
         for (int b = 0; b < kTiles / 2; ++b) {
-            uint32_t p[3][4];
+            uint32_t p[G][3][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = 2 * b + e / 2, r = 2 * (e % 2);
-                const float p0 = fast_exp2(s[t][r] - base), p1 = fast_exp2(s[t][r + 1] - base);
-                l += p0 + p1;
-                uint32_t x[3];
-                split3(p0, p1, x);
+            for (int u = 0; u < G; ++u)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) p[i][e] = x[i];
-            }
+                for (int e = 0; e < 4; ++e) {
+                    const int t = 2 * b + e / 2, r = 2 * (e % 2);
+                    const float p0 = fast_exp2(s[u][t][r] - base[u]), p1 = fast_exp2(s[u][t][r + 1] - base[u]);
+                    l[u] += p0 + p1;
+                    uint32_t x[3];
+                    split3(p0, p1, x);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) p[u][i][e] = x[i];
+                }
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
@@ -249,7 +268,9 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
                     uint32_t v[4];
                     read4(v, vb + j * S::kVPart + 16 * c * S::kVRow + 32 * b);
 #pragma unroll
-                    for (int i = 2 - j; i >= 0; --i) o[c] = mfma_bf16(v, p[i], o[c]);
+                    for (int i = 2 - j; i >= 0; --i)
+#pragma unroll
+                        for (int u = 0; u < G; ++u) o[u][c] = mfma_bf16(v, p[u][i], o[u][c]);
                 }
         }
     };
@@ -270,39 +291,45 @@ __global__ __launch_bounds__(kThreadsOf<T>, 2) void paged_wide_kernel(const Page
         }
         if (key < wave_end) multiply(buf, key);
     }
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) finished(o[c]);
-    l = sum4_rows(l);
     if (again_s != 0) {  // set before the last tile's barrier at the latest
-        rows_by_key<T>(a, it, kv, it.row0 + 16 * w, 16, (static_cast<int64_t>(it.part + w) * a.KV + kv) * kPagedRows);
+        for (int u = 0; u < G; ++u)
+            rows_by_key<T>(a, it, kv, row0 + 16 * u, 16, (static_cast<int64_t>(it.part + G * w + u) * a.KV + kv) * kPagedRows);
         return;
     }
-    if (!live) return;
-    float *dst;
-    float scale = 1.0f;
-    if (it.part < 0) {
-        dst = a.out + (static_cast<int64_t>(it.tok0 + token) * a.H + kv * a.group + row - token * a.group) * a.D;
-        scale = 1.0f / l;
-    } else {
-        const int64_t slot = (static_cast<int64_t>(it.part + w) * a.KV + kv) * kPagedRows + n;
-        dst = a.part_o + slot * a.D;
-        if (g == 0) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * slot) = f32x2{m, l};
-    }
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) store4<R != kAny>(dst, 16 * c + 4 * g, a.D, o[c] * scale);
+    for (int u = 0; u < G; ++u) {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) finished(o[u][c]);
+        const float sum = sum4_rows(l[u]);
+        if (!live[u]) continue;
+        float *dst;
+        float scale = 1.0f;
+        if (it.part < 0) {
+            dst = a.out + (static_cast<int64_t>(it.tok0 + token[u]) * a.H + kv * a.group + row[u] - token[u] * a.group) * a.D;
+            scale = 1.0f / sum;
+        } else {
+            const int64_t slot = (static_cast<int64_t>(it.part + G * w + u) * a.KV + kv) * kPagedRows + n;
+            dst = a.part_o + slot * a.D;
+            if (g == 0) *reinterpret_cast<f32x2 *>(a.part_ml + 2 * slot) = f32x2{m[u], sum};
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) store4<R != kAny>(dst, 16 * c + 4 * g, a.D, o[u][c] * scale);
+    }
 }
 
 template <typename T, int DP, Rows R>
 void launch(const PagedAttnParams &p, hipStream_t s) {
     constexpr size_t kBytes = 2 * sizeof(uint16_t) * Shape<T, DP>::kBuffer;
+    constexpr int kThreads = paged_wide_rows(kType<T>) / (16 * kGroupsOf<T, DP>) * 64;
+    const auto kernel = paged_wide_kernel<T, DP, R, kThreads>;
     if constexpr (kBytes > 65536) {
         static std::once_flag once;
-        std::call_once(once, [] {
-            hipCheck(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_wide_kernel<T, DP, R>),
-                                         hipFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+        std::call_once(once, [&] {
+            hipCheck(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         kBytes));
         });
     }
-    paged_wide_kernel<T, DP, R><<<dim3(static_cast<unsigned>(p.n_wide) * p.KV), dim3(kThreadsOf<T>), kBytes, s>>>(p);
+    kernel<<<dim3(static_cast<unsigned>(p.n_wide) * p.KV), dim3(kThreads), kBytes, s>>>(p);
     hipCheck(hipGetLastError());
 }
 

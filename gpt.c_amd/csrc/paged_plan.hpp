@@ -32,7 +32,7 @@ constexpr int paged_wide_rows(int dtype) { return dtype == GPTC_BF16 ? 64 : 128;
 // 16 or 32 keys each (csrc/paged_attn.hip); an LDS tile of a wide item.
 constexpr int paged_unit(int dtype) { return dtype == GPTC_BF16 ? 128 : 64; }
 constexpr int paged_wide_keys(int dtype, int head_dim) {
-    return dtype == GPTC_BF16 ? (head_dim <= 64 ? 128 : 64) : (head_dim <= 64 ? 64 : 32);
+    return dtype == GPTC_BF16 ? (head_dim <= 64 ? 128 : 64) : 32;
 }
 
 // Items that the keys of one step are cut into at most, over all kv heads: see paged_schedule.
