@@ -23,10 +23,6 @@ namespace {
 
 template <typename T>
 constexpr int kType = sizeof(T) == 4 ? GPTC_F32 : GPTC_BF16;
-// Groups of 16 rows that a wave takes: two read each operand from LDS once for both.
-template <typename T, int DP>
-constexpr int kGroupsOf = sizeof(T) == 4 && DP == 64 ? 2 : 1;
-
 template <typename T, int DP>
 struct Shape {
     static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
@@ -42,10 +38,11 @@ __device__ __forceinline__ void parts_of(uint32_t x0, uint32_t x1, uint32_t (&p)
     split3(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1), p);
 }
 
-template <typename T, int DP, Rows R, int THREADS>
+// G: groups of 16 rows that a wave takes.  Two read each operand from LDS once for both.
+template <typename T, int DP, Rows R, int G, int THREADS>
 __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnParams a) {
     using S = Shape<T, DP>;
-    constexpr int kThreads = THREADS, G = kGroupsOf<T, DP>, kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
+    constexpr int kThreads = THREADS, kKeys = S::kKeys, kParts = S::kParts, kTiles = kKeys / 16;
     extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
     __shared__ int again_s;  // see rows_by_key
 
@@ -92,10 +89,11 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     // kVDims neighbouring values of the eight keys of a place 8g.
     constexpr int kPiece = 16 / sizeof(T), kPieces = DP / kPiece;
     constexpr int kKLoads = kKeys * kPieces / kThreads;
-    constexpr int kVDims = kKeys / 8 * DP / kThreads;
+    constexpr int kVShare = kKeys / 8 * DP / kThreads, kVDims = kVShare > 0 ? kVShare : 1;
     constexpr int kVWords = kVDims * sizeof(T) / 4;
     static_assert(kKLoads * kThreads == kKeys * kPieces && kVWords >= 1, "a tile is shared out evenly");
-    const int v_place = tid / (DP / kVDims), v_dim = tid % (DP / kVDims) * kVDims;
+    const bool brings_v = kVShare > 0 || tid < kKeys / 8 * DP;  // the others' loads are clamped into the tile
+    const int v_place = min(tid / (DP / kVDims), kKeys / 8 - 1), v_dim = tid % (DP / kVDims) * kVDims;
     const int v_key = v_place / 4 * 32 + v_place % 4 * 4;  // and the 3 after it, and 16 further
     const T *kpool = static_cast<const T *>(a.k), *vpool = static_cast<const T *>(a.v);
     const int *table = a.table + it.table;
@@ -139,6 +137,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
                 for (int t = 0; t < 3; ++t) *reinterpret_cast<u32x2 *>(dst + t * S::kKPart) = u32x2{p0[t], p1[t]};
             }
         }
+        if (!brings_v) return;
         // Slots past the sequence's end hold anything: their weights are 0, and 0 times NaN is not.
         if (key + kKeys > total) {
 #pragma unroll
@@ -317,11 +316,11 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     }
 }
 
-template <typename T, int DP, Rows R>
+template <typename T, int DP, Rows R, int G>
 void launch(const PagedAttnParams &p, hipStream_t s) {
     constexpr size_t kBytes = 2 * sizeof(uint16_t) * Shape<T, DP>::kBuffer;
-    constexpr int kThreads = paged_wide_rows(kType<T>) / (16 * kGroupsOf<T, DP>) * 64;
-    const auto kernel = paged_wide_kernel<T, DP, R, kThreads>;
+    constexpr int kThreads = paged_wide_rows(kType<T>) / (16 * G) * 64;
+    const auto kernel = paged_wide_kernel<T, DP, R, G, kThreads>;
     if constexpr (kBytes > 65536) {
         static std::once_flag once;
         std::call_once(once, [&] {
@@ -333,25 +332,32 @@ void launch(const PagedAttnParams &p, hipStream_t s) {
     hipCheck(hipGetLastError());
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int G>
 void launch(const PagedAttnParams &p, hipStream_t s) {
     if (p.vec && p.D == DP)
-        launch<T, DP, kFull>(p, s);
+        launch<T, DP, kFull, G>(p, s);
     else if (p.vec)
-        launch<T, DP, kVec>(p, s);
+        launch<T, DP, kVec, G>(p, s);
     else
-        launch<T, DP, kAny>(p, s);
+        launch<T, DP, kAny, G>(p, s);
 }
 
 }  // namespace
 
 void launch_paged_wide(const PagedAttnParams &p, hipStream_t s) {
+    // Rows of 16 to a wave.  With two groups a workgroup has half the waves, and two of them fit a CU: worth it from
+    // two workgroups per CU on (a prompt of 4096, 12 heads of 64, fp32: 239 us with one group and 219 with two; one
+    // of 1024, 288 workgroups: 24 and 29 us).  Both give the same sums.
+    constexpr int kTwoFrom = 2 * 256;
     if (p.bf16) {
-        if (p.D <= 64) launch<__bf16, 64>(p, s);
-        else launch<__bf16, 128>(p, s);
+        if (p.D <= 64) launch<__bf16, 64, 1>(p, s);
+        else launch<__bf16, 128, 1>(p, s);
+    } else if (p.D > 64) {
+        launch<float, 128, 1>(p, s);
+    } else if (static_cast<int64_t>(p.n_wide) * p.KV >= kTwoFrom) {
+        launch<float, 64, 2>(p, s);
     } else {
-        if (p.D <= 64) launch<float, 64>(p, s);
-        else launch<float, 128>(p, s);
+        launch<float, 64, 1>(p, s);
     }
 }
 
