@@ -309,8 +309,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     }
 
     // The waves' states joined: sums of o 2^(m_w - M).
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) finished(o[c]);
+    drain();
     l = sum4_rows(l);
     if (g == 0) {
         m_s[w][n] = m;

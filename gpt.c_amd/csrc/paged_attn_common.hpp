@@ -65,9 +65,14 @@ __device__ __forceinline__ f32x4 mfma_bf16(const uint32_t (&a)[4], const uint32_
 
 // A matrix instruction's result may be read 11 cycles after it at the earliest.  The compiler counts them inside
 // a block; across a branch it was seen to read the last two registers at once (wrong sums at every second step of
-// bf16 pages).  So results are taken over in the block of the product, or after a wait of 16.
+// bf16 pages).  So results are taken over in the block of the product (settled), or after a wait (drain) that nothing
+// is moved across.
 __device__ __forceinline__ void settled(f32x4 &x) { asm volatile("" : "+v"(x)); }
-__device__ __forceinline__ void finished(f32x4 &x) { asm volatile("s_nop 15" : "+a"(x)); }
+__device__ __forceinline__ void drain() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // ---- values that are no numbers, in the tokens that some rows of a tile must not see ----
 //

@@ -290,6 +290,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
         }
         if (key < wave_end) multiply(buf, key);
     }
+    drain();
     if (again_s != 0) {  // set before the last tile's barrier at the latest
         for (int u = 0; u < G; ++u)
             rows_by_key<T>(a, it, kv, row0 + 16 * u, 16, (static_cast<int64_t>(it.part + G * w + u) * a.KV + kv) * kPagedRows);
@@ -297,8 +298,6 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     }
 #pragma unroll
     for (int u = 0; u < G; ++u) {
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c) finished(o[u][c]);
         const float sum = sum4_rows(l[u]);
         if (!live[u]) continue;
         float *dst;

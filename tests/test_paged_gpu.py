@@ -268,6 +268,41 @@ def test_rows_past_the_last_token_are_left_as_they_were(rt):
     pool.free()
 
 
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+def test_tensors_off_16_bytes(rt, dtype):
+    """The step's tensors start anywhere a float can."""
+    H, KV, D, past, fresh = 4, 2, 64, 40, 90
+    pool = Pool(rt, [past], [fresh], H, KV, D, 16, dtype, seed=12, max_len=200)
+    kept = pool.fill([past])
+    pool.set()
+    x = pool.normal(fresh, H + 2 * KV, D)
+    table = rt.lib.gptc_rotary_table(200, 32, 10000.0)
+    turned = rotate(x[:, :H + KV].astype(np.float64), rt.to_numpy(table)[past:past + fresh].astype(np.float64), 32, False)
+
+    def off(a):
+        t = torch.zeros(a.size + 3, device="cuda")
+        t[3:] = torch.tensor(a.reshape(-1))
+        view = gptc.Tensor()
+        view.t = ctypes.cast(t.data_ptr() + 12, ctypes.POINTER(ctypes.c_float))
+        view.ndims, view.length, view.device = 2, a.size, gptc.CUDA
+        view.shape[0], view.shape[1] = len(a), a.size // len(a)
+        return t, ctypes.pointer(view)
+
+    (_, tx), (q, tq), (out, tout) = off(x), off(np.zeros((fresh, H * D), np.float32)), off(np.zeros((fresh, H * D), np.float32))
+    torch.cuda.synchronize()
+    pool.plan.append(0, tx, table, False, tq)
+    pool.plan.attention(0, tq, tout)
+    rt.sync()
+    got_q = q[3:].cpu().numpy().reshape(fresh, H, D)
+    assert np.abs(got_q - turned[:, :H]).max() <= 6 * U * np.abs(x).max()
+    held = pool.held(0, past, past + fresh)
+    kv = [(np.concatenate([kept[0][0], held[0]]), np.concatenate([kept[0][1], held[1]]))]
+    check_attention(pool, kv, got_q.reshape(fresh, H, D), out[3:].cpu().numpy().reshape(fresh, H * D))
+    assert np.abs(held[0] - turned[:, H:]).max() <= 6 * U * np.abs(x).max() + (2.0 ** -8 * np.abs(turned).max() if dtype else 0)
+    pool.free()
+    rt.free(table)
+
+
 def test_a_step_without_tokens_does_nothing(rt):
     pool = Pool(rt, [40, 0], [0, 0], 2, 2, 64, 16, gptc.F32)
     pool.set()

@@ -208,3 +208,11 @@ def test_rows_of_three_dimensions_and_none(rt):
     t = [rt.from_numpy(a) for a in (x.reshape(4, 1, 100), p, u)] + [rt.empty((4, 1)), None]
     rt.lib.gptc_sample_cuda(*t)
     assert np.array_equal(rt.to_numpy(t[3])[:, 0], flat)
+
+
+def test_the_largest_vocabulary(rt):
+    """2^24 tokens: sums of 2^24 weights, stretches longer than a list, indices that are floats just so."""
+    rng = np.random.default_rng(17)
+    x = rng.standard_normal((3, 1 << 24)).astype(np.float32)
+    x[:, -1] = x.max() + 1
+    check(rt, x, [SETTINGS["top_k"], SETTINGS["top_p"], SETTINGS["plain"]], [0.3, 0.97, 1 - 2.0 ** -24])
