@@ -31,6 +31,9 @@ struct Shape {
     static constexpr int kVRow = kKeys + 8;
     static constexpr int kKPart = kKeys * kKRow, kVPart = DP * kVRow;
     static constexpr int kBuffer = kParts * (kKPart + kVPart);
+    // Two of fp32 pages with heads past 64 would take 114 KB and leave a CU to one workgroup: one is 1.04 times as fast
+    // there at a second barrier, and 1.07 to 1.15 times once two workgroups share the CU.
+    static constexpr int kBuffers = sizeof(T) == 4 && DP == 128 ? 1 : 2;
 };
 
 // Two floats as three bf16 values each, packed in pairs.
@@ -281,7 +284,8 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     __syncthreads();
     int turn = 0;
     for (int key = it.key0; key < it.key1; key += kKeys, turn ^= 1) {
-        uint16_t *buf = lds + turn * S::kBuffer;
+        uint16_t *buf = lds + (S::kBuffers == 2 ? turn * S::kBuffer : 0);
+        if (S::kBuffers == 1) __syncthreads();
         store_tile(buf, key);
         __syncthreads();
         if (key + kKeys < it.key1) {
@@ -317,7 +321,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
 
 template <typename T, int DP, Rows R, int G>
 void launch(const PagedAttnParams &p, hipStream_t s) {
-    constexpr size_t kBytes = 2 * sizeof(uint16_t) * Shape<T, DP>::kBuffer;
+    constexpr size_t kBytes = Shape<T, DP>::kBuffers * sizeof(uint16_t) * Shape<T, DP>::kBuffer;
     constexpr int kThreads = paged_wide_rows(kType<T>) / (16 * G) * 64;
     const auto kernel = paged_wide_kernel<T, DP, R, G, kThreads>;
     if constexpr (kBytes > 65536) {
@@ -344,19 +348,20 @@ void launch(const PagedAttnParams &p, hipStream_t s) {
 }  // namespace
 
 void launch_paged_wide(const PagedAttnParams &p, hipStream_t s) {
-    // Rows of 16 to a wave.  With two groups a workgroup has half the waves, and two of them fit a CU: worth it from
-    // two workgroups per CU on (a prompt of 4096, 12 heads of 64, fp32: 239 us with one group and 219 with two; one
-    // of 1024, 288 workgroups: 24 and 29 us).  Both give the same sums.
-    constexpr int kTwoFrom = 2 * 256;
+    // Groups of 16 rows to a wave, fp32 pages.  With two a workgroup has half the waves, and two of them fit a CU: worth
+    // it from one and a half per CU on.  12 heads of 64, a prompt of 4096: 239 us with one group and 219 with two; of
+    // 1024 (240 workgroups): 24 and 29 us.  Heads of 128, 64 tokens each of 8 sequences over 2000: 82 and 76 us; a
+    // prompt of 1024 with 12 heads: 42 and 52 us.  Both give the same sums.
+    const bool two = static_cast<int64_t>(p.n_wide) * p.KV >= 384;
     if (p.bf16) {
         if (p.D <= 64) launch<__bf16, 64, 1>(p, s);
         else launch<__bf16, 128, 1>(p, s);
-    } else if (p.D > 64) {
-        launch<float, 128, 1>(p, s);
-    } else if (static_cast<int64_t>(p.n_wide) * p.KV >= kTwoFrom) {
-        launch<float, 64, 2>(p, s);
+    } else if (p.D <= 64) {
+        if (two) launch<float, 64, 2>(p, s);
+        else launch<float, 64, 1>(p, s);
     } else {
-        launch<float, 64, 1>(p, s);
+        if (two) launch<float, 128, 2>(p, s);
+        else launch<float, 128, 1>(p, s);
     }
 }
 
