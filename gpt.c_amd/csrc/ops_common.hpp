@@ -42,6 +42,11 @@ inline int blocks_for(int64_t work, int64_t per_block) {
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+inline bool overlap(const tensor_t *a, const tensor_t *b) {
+    const auto x = reinterpret_cast<uintptr_t>(a->t), y = reinterpret_cast<uintptr_t>(b->t);
+    return x < y + 4 * static_cast<uintptr_t>(b->length) && y < x + 4 * static_cast<uintptr_t>(a->length);
+}
+
 inline void check_gpu(const tensor_t *t, const char *name) {
     CHECK_ERROR(t == NULL, "missing tensor argument `%s` (NULL).", name);
     CHECK_ERROR(t->device != CUDA, "Expected %s to be a tensor on the GPU.", name);

@@ -127,12 +127,19 @@ extern "C" int gptc_paged_schedule(const int n_seqs, const int *past, const int 
     CHECK_ERROR(n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads != 0,
                 "Expected n_heads = %d to be a multiple of n_kv_heads = %d.", n_heads, n_kv_heads);
     CHECK_ERROR(dtype != GPTC_F32 && dtype != GPTC_BF16, "Unknown page type %d.", dtype);
+    CHECK_ERROR(head_dim < 1 || head_dim > 128, "Head size %d is not supported in pages (1 <= head_dim <= 128).",
+                head_dim);
+    CHECK_ERROR(cap > 1 << 24, "Expected room for up to 2^24 items, but got %d.", cap);
+    for (int s = 0; s < n_seqs; ++s)
+        CHECK_ERROR(past[s] < 0 || fresh[s] < 0 || static_cast<int64_t>(past[s]) + fresh[s] > (1 << 30) ||
+                        static_cast<int64_t>(fresh[s]) * n_heads > (1 << 26),
+                    "Sequence %d has %d tokens and %d new ones.", s, past[s], fresh[s]);
     if (n_seqs <= 0 || cap <= 0) return n_seqs <= 0 ? 0 : -1;
     PagedLists l{};
     l.items = reinterpret_cast<PagedItem *>(items);
     l.item_cap = l.wide_cap = cap;
-    l.merge_cap = l.part_cap = INT32_MAX / 2;
-    l.merge_cap = 8 * cap;
+    l.part_cap = INT32_MAX / 2;
+    l.merge_cap = 8 * cap;  // a cut tile has at least two items, and at most one merge for each 16 of its 128 rows
     l.wide = static_cast<PagedItem *>(mallocCheck(sizeof(PagedItem) * static_cast<size_t>(cap)));
     l.merges = static_cast<PagedMerge *>(mallocCheck(sizeof(PagedMerge) * static_cast<size_t>(l.merge_cap)));
     int n = -1;
@@ -230,6 +237,9 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     p->wide_cap = static_cast<int>(work / wide_rows + active) + wide_cut;
     p->merge_cap = cut + slots * wide_cut;
     p->part_cap = 2 * p->merge_cap;
+    // A launch has fewer than 2^32 threads: 256 for each item and kv head, up to 512 for wide ones.
+    CHECK_ERROR(static_cast<int64_t>(std::max(p->item_cap, 2 * p->wide_cap)) * cache->n_kv_heads >= 1 << 24,
+                "The work of %d sequences and %d tokens with %d heads is too large.", max_seqs, max_tokens, n_heads);
     p->at_items = 8;
     p->at_wide = p->at_items + 8 * static_cast<size_t>(p->item_cap);
     p->at_merges = p->at_wide + 8 * static_cast<size_t>(p->wide_cap);
@@ -247,6 +257,7 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
 extern "C" void gptc_paged_plan_free(gptc_paged_plan_t *plan) {
     if (plan == NULL) return;
     if (plan->dev != nullptr) {
+        CHECK_ERROR(gptc_stream_capturing(), "A plan cannot be freed while the stream is being captured.");
         free_cuda(plan->dev);
         free_cuda(plan->part_o);
         free_cuda(plan->part_ml);
@@ -472,11 +483,6 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams a) {
     T *dst = static_cast<T *>(is_k ? a.k : a.v) +
              (((page * a.KV + (is_k ? kv : kv - a.KV)) << a.page_shift) + in) * a.D + d;
     store_vec<W>(dst, x);
-}
-
-bool overlap(const tensor_t *a, const tensor_t *b) {
-    const auto x = reinterpret_cast<uintptr_t>(a->t), y = reinterpret_cast<uintptr_t>(b->t);
-    return x < y + 4 * static_cast<uintptr_t>(b->length) && y < x + 4 * static_cast<uintptr_t>(a->length);
 }
 
 int log2_of(int page) { return __builtin_ctz(static_cast<unsigned>(page)); }

@@ -366,7 +366,7 @@ long long gptc_decode_noalloc_scratch_floats(void);
  * gptc_argmax_cuda(logits, ids)
  *   ids[r] = first index of the maximum of logits row r (greedy decoding).
  * gptc_sample_cuda(logits, params, u, ids, prob)
- *   Draws a token of every row of logits (rows, V), rows <= 2^22, V <= 2^24, from
+ *   Draws a token of every row of logits (rows, V), rows < 2^22, V <= 2^24, from
  *   the random number u[r] of [0, 1).  params (4), or (rows, 4) for settings per row:
  *   temperature, top_k, top_p, min_p, whole numbers held in floats where they
  *   count.  With the tokens ordered by logit, equal ones by index, and weights
@@ -377,9 +377,12 @@ long long gptc_decode_noalloc_scratch_floats(void);
  *   >= 1).  ids[r] is the first token, by index, at which the sum of the kept
  *   weights passes u[r] of their total (u outside [0, 1) counts as its end);
  *   prob[r], unless prob is NULL, that token's share of them.  A temperature
- *   that is not above 0 takes the first maximum, prob 1.  Logits of -inf and
- *   NaN are never drawn; a row of nothing else gives id -1 and prob 0.  Sums
- *   are exact in integers, so the result depends on nothing but the row.
+ *   that is not above 0 takes the first maximum, prob 1; one above 1e30 counts
+ *   as 1e30.  Logits of -inf and NaN are never drawn, +inf counts as the largest
+ *   float; a row of nothing but the former gives id -1 and prob 0.  Weights are
+ *   whole multiples of 2^-46 of the largest (of 2^-38 for 2^24 tokens), and sums
+ *   of them exact, so the result depends on nothing but the row.  Neither ids
+ *   nor prob may overlap another tensor of the call.
  *   No counterpart on a device in the reference: infer_gpt.c draws on the host
  *   from the softmax of one row (sample_mult).
  */

@@ -62,7 +62,8 @@ void gptc_paged_cache_free(gptc_paged_cache_t *cache);
  *   all, each sequence at most max_len tokens long with them.  n_heads is a
  *   multiple of the cache's n_kv_heads: query head h reads kv head
  *   h / (n_heads / n_kv_heads).  Its device memory is taken by the first
- *   gptc_paged_plan_set and never moves.
+ *   gptc_paged_plan_set and never moves; the cache has to outlive the plan, and
+ *   the plan the graphs captured with it.
  * gptc_paged_plan_set(plan, n_seqs, past, fresh, table, stride)
  *   All arrays are host memory, read before the call returns.  Sequence s has
  *   past[s] >= 0 tokens in its pages and brings fresh[s] >= 0 new ones; its
@@ -108,7 +109,12 @@ void gptc_paged_plan_free(gptc_paged_plan_t *plan);
  *   attends, scaled by 1/sqrt(head_dim), to that sequence's tokens
  *   0 .. past[s] + i, which have to be in their pages.  output rows past the
  *   last token are left as they were; output may not overlap q.
- *   Deterministic; no allocation.
+ *   Deterministic; no allocation.  Sums are fp32.  Keys and values of later
+ *   tokens, and what unused slots hold, have no influence, finite or not.  Those
+ *   of the tokens attended to are taken to be finite: infinities and NaN make
+ *   the results that use them NaN or infinite.  Where a sequence brings 64 query
+ *   rows per kv head or more, products are sums of bf16 parts: fp32 values below
+ *   2^-110 count with fewer than 24 bits there.
  */
 tensor_t *gptc_rotary_table(const int rows, const int rot, const double theta);
 void gptc_paged_append_cuda(gptc_paged_plan_t *plan, const int layer, const tensor_t *qkv, const tensor_t *rotary,

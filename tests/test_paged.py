@@ -33,6 +33,10 @@ def run_c(body):
         def plan(heads=4, seqs=3, tokens=40, length=64, **kw):
             return gptc.PagedPlan(rt, cache(**kw), heads, seqs, tokens, length)
 
+        def sched(past, fresh, dim=64, cap=4):
+            a, b, items = (np.array(x, np.int32).ctypes.data_as(ctypes.POINTER(ctypes.c_int)) for x in (past, fresh, [0] * 32))
+            rt.lib.gptc_paged_schedule(len(past), a, b, 4, 2, dim, gptc.F32, items, cap)
+
         def host(*shape):
             return rt.from_numpy(np.zeros(shape, np.float32), gptc.CPU)
     """) + textwrap.dedent(body) + "\nprint('survived')\n"
@@ -56,6 +60,11 @@ REFUSALS = {
     "heads no multiple": ("plan(heads=3)", "multiple of the cache's 2 kv heads"),
     "too many tokens for the grid": ("plan(tokens=(1 << 22) + 1)", "is too large"),
     "too many rows for the grid": ("plan(tokens=1 << 20, heads=128)", "is too large"),
+    "too many items for the grid": ("gptc.PagedPlan(rt, cache(heads=64), 64, 1 << 20, 1 << 20, 64)", "is too large"),
+    "schedule past": ("sched([-1], [1])", "-1 tokens"),
+    "schedule rows": ("sched([0], [1 << 25])", "new ones"),
+    "schedule head size": ("sched([0], [1], dim=129)", "Head size 129"),
+    "schedule room": ("sched([0], [1], cap=(1 << 24) + 1)", "2^24 items"),
     "too many pages": ("plan(seqs=1 << 20, length=1 << 20)", "too many pages"),
     "no room": ("plan(seqs=0)", "Expected room"),
     "too many sequences": ("plan().set([0] * 4, [1] * 4, [[0], [1], [2], [3]])", "room for 3 sequences"),
@@ -164,8 +173,13 @@ SAMPLE_REFUSALS = {
     "random numbers": ("sample(gpu(3, 8), gpu(4), gpu(2), gpu(3))", "Expected 3 random numbers"),
     "ids": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(4))", "Expected 3 ids"),
     "shares": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3), gpu(2))", "Expected 3 probabilities"),
-    "rows": ("sample(gpu((1 << 22) + 1, 1), gpu(4), gpu(1), gpu(1))", "Up to 2^22 rows"),
+    "rows": ("sample(gpu((1 << 22) + 1, 1), gpu(4), gpu(1), gpu(1))", "Fewer than 2^22 rows"),
+    "rows of 2^32 threads": ("sample(gpu(1 << 22, 1), gpu(4), gpu(1), gpu(1))", "Fewer than 2^22 rows"),
     "vocabulary": ("sample(gpu(1, (1 << 24) + 1), gpu(4), gpu(1), gpu(1))", "up to 2^24 tokens"),
+    "ids over the random numbers": ("sample(gpu(3, 8), gpu(4), gpu(3, at=8192), gpu(3, at=8200))", "may not overlap"),
+    "ids over the logits": ("sample(gpu(3, 8, at=8192), gpu(4), gpu(3), gpu(3, at=8284))", "may not overlap"),
+    "shares over the parameters": ("sample(gpu(3, 8), gpu(4, at=8192), gpu(3), gpu(3), gpu(3, at=8192))", "may not overlap"),
+    "ids over the shares": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3, at=8192), gpu(3, at=8192))", "ids and prob may not overlap"),
     "without a runtime": ("sample(gpu(3, 8), gpu(4), gpu(3), gpu(3))", "runtime_init"),
 }
 
@@ -174,9 +188,13 @@ SAMPLE_REFUSALS = {
 def test_sampling_refused(name):
     call, message = SAMPLE_REFUSALS[name]
     r = run_c("""
-        def gpu(*shape):
+        free = [4096]
+
+        def gpu(*shape, at=None):
             t = gptc.Tensor()
-            t.t, t.ndims, t.length, t.device = ctypes.cast(4096, ctypes.POINTER(ctypes.c_float)), len(shape), int(np.prod(shape)), gptc.CUDA
+            at = free[0] if at is None else at
+            free[0] = max(free[0], at + 4 * int(np.prod(shape)))
+            t.t, t.ndims, t.length, t.device = ctypes.cast(at, ctypes.POINTER(ctypes.c_float)), len(shape), int(np.prod(shape)), gptc.CUDA
             for i, n in enumerate(shape):
                 t.shape[i] = n
             return ctypes.pointer(t)
