@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     float f[kWaves], sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-        f[i] = m_s[i][r] == -INFINITY ? 0.0f : fast_exp2(m_s[i][r] - big);
+        f[i] = m_s[i][r] == -INFINITY ? l_s[i][r] : fast_exp2(m_s[i][r] - big);  // 0; NaN where a key's score was
         sum = fmaf(l_s[i][r], f[i], sum);
     }
     const int out_row = it.row0 + r, out_token = it.tok0 + out_row / a.group;
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256) void paged_merge_few_kernel(const PagedAttnPar
 #pragma unroll 4
         for (int p = 0; p < mg.n; ++p) {
             const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
-            const float f = ml[0] == -INFINITY ? 0.0f : fast_exp2(ml[0] - big);
+            const float f = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - big);
             sum += ml[1] * f;
             y += f * load4<VEC>(a.part_o + (first + p * next) * a.D, d, a.D);
         }
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
     float sum = 0.0f;
     for (int p = tid; p < mg.n; p += kMergeThreads) {
         const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
-        const float f = ml[0] == -INFINITY ? 0.0f : fast_exp2(ml[0] - big);
+        const float f = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - big);
         f_s[p] = f;
         if (p < kPagedFewParts) l_s[p] = ml[1] * f;
         sum += ml[1] * f;

@@ -113,8 +113,9 @@ void gptc_paged_plan_free(gptc_paged_plan_t *plan);
  *   tokens, and what unused slots hold, have no influence, finite or not.  Those
  *   of the tokens attended to are taken to be finite: infinities and NaN make
  *   the results that use them NaN or infinite.  Where a sequence brings 64 query
- *   rows per kv head or more, products are sums of bf16 parts: fp32 values below
- *   2^-110 count with fewer than 24 bits there.
+ *   rows per kv head or more, products are sums of bf16 parts: there fp32 values
+ *   below 2^-110 count with fewer than 24 bits, and those past the largest bf16
+ *   value as infinite.  So do queries with bf16 pages.
  */
 tensor_t *gptc_rotary_table(const int rows, const int rot, const double theta);
 void gptc_paged_append_cuda(gptc_paged_plan_t *plan, const int layer, const tensor_t *qkv, const tensor_t *rotary,

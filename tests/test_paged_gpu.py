@@ -368,6 +368,25 @@ def test_a_later_tokens_values_stay_hidden(rt, dtype, fresh, H, KV, D):
     rt.free(out)
 
 
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16])
+@pytest.mark.parametrize("past, fresh, bad", [(300, 1, (64, 96)), (6000, 1, (1024, 2048)), (400, 70, (32, 64)),
+                                              (200, 130, (200, 210)), (40000, 3, (20000, 20600))])
+def test_keys_that_are_nan_are_not_lost(rt, dtype, past, fresh, bad):
+    """Whole rounds, waves and parts whose keys' scores are NaN: every row that attends to them is NaN."""
+    pool = Pool(rt, [past], [fresh], 2, 2, 32, 32, dtype, seed=4)
+    pool.fill([past + fresh])
+    page, slot = pool.rows(0, *bad)
+    pool.k[0][page, :, slot] = float("nan")
+    torch.cuda.synchronize()
+    pool.set()
+    out = rt.empty((fresh, 64))
+    pool.plan.attention(0, rt.from_numpy(pool.normal(fresh, 64)), out)
+    got = rt.to_numpy(out)
+    sees = past + np.arange(fresh) >= bad[0]
+    assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
+    pool.free()
+
+
 def test_two_layers_and_shared_prefix(rt):
     """Two sequences read the same first pages; each layer has its own."""
     pool = Pool(rt, [64, 64], [1, 2], 4, 4, 64, 32, gptc.F32, layers=2, seed=4)
