@@ -33,7 +33,7 @@ struct Shape {
     static constexpr int kBuffer = kParts * (kKPart + kVPart);
     // Two of fp32 pages with heads past 64 would take 114 KB and leave a CU to one workgroup: one is 1.04 times as fast
     // there at a second barrier, and 1.07 to 1.15 times once two workgroups share the CU.
-    static constexpr int kBuffers = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+    static constexpr int kBuffers = sizeof(T) == 4 && DP > 64 ? 1 : 2;
 };
 
 // Two floats as three bf16 values each, packed in pairs.
@@ -91,11 +91,12 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     // What this thread brings of a tile.  Keys: kKLoads pieces of 16 bytes, piece i being row i / per row.  Values:
     // kVDims neighbouring values of the eight keys of a place 8g.
     constexpr int kPiece = 16 / sizeof(T), kPieces = DP / kPiece;
-    constexpr int kKLoads = kKeys * kPieces / kThreads;
-    constexpr int kVShare = kKeys / 8 * DP / kThreads, kVDims = kVShare > 0 ? kVShare : 1;
+    // Where that does not come out even, some threads bring nothing: their loads are clamped into the tile.
+    constexpr int kKAll = kKeys * kPieces, kKLoads = (kKAll + kThreads - 1) / kThreads;
+    constexpr int kVAll = kKeys / 8 * DP, kVDims = kVAll > 2 * kThreads ? 4 : kVAll > kThreads || sizeof(T) == 2 ? 2 : 1;
     constexpr int kVWords = kVDims * sizeof(T) / 4;
-    static_assert(kKLoads * kThreads == kKeys * kPieces && kVWords >= 1, "a tile is shared out evenly");
-    const bool brings_v = kVShare > 0 || tid < kKeys / 8 * DP;  // the others' loads are clamped into the tile
+    static_assert(kVAll <= kVDims * kThreads && DP % kVDims == 0, "the values of a tile are brought at once");
+    const bool brings_v = kVAll == kVDims * kThreads || tid < kVAll / kVDims;
     const int v_place = min(tid / (DP / kVDims), kKeys / 8 - 1), v_dim = tid % (DP / kVDims) * kVDims;
     const int v_key = v_place / 4 * 32 + v_place % 4 * 4;  // and the 3 after it, and 16 further
     const T *kpool = static_cast<const T *>(a.k), *vpool = static_cast<const T *>(a.v);
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     int k_page[kKLoads], v_page[2];
     auto load_pages = [&](int key) {
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i) k_page[i] = table[min(key + (tid + i * kThreads) / kPieces, total - 1) >> a.page_shift];
+        for (int i = 0; i < kKLoads; ++i) k_page[i] = table[min(key + min(tid + i * kThreads, kKAll - 1) / kPieces, total - 1) >> a.page_shift];
 #pragma unroll
         for (int h = 0; h < 2; ++h) v_page[h] = table[min(key + v_key + 16 * h, total - 1) >> a.page_shift];
     };
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
     auto load_tile = [&](int key) {
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i) {
-            const int p = tid + i * kThreads, r = p / kPieces;
+            const int p = min(tid + i * kThreads, kKAll - 1), r = p / kPieces;
             const int64_t at = ((static_cast<int64_t>(k_page[i]) * a.KV + kv) << a.page_shift) + ((key + r) & mask);
             load_words<T, 4, R>(kr[i], kpool + at * a.D, p % kPieces * kPiece, a.D);
         }
@@ -129,6 +130,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i) {
             const int p = tid + i * kThreads;
+            if (kKAll % kThreads != 0 && p >= kKAll) break;
             uint16_t *dst = kb + p / kPieces * S::kKRow + p % kPieces * kPiece;
             if constexpr (kParts == 1) {
                 *reinterpret_cast<u32x4 *>(dst) = u32x4{kr[i][0], kr[i][1], kr[i][2], kr[i][3]};
@@ -353,12 +355,18 @@ void launch_paged_wide(const PagedAttnParams &p, hipStream_t s) {
     // 1024 (240 workgroups): 24 and 29 us.  Heads of 128, 64 tokens each of 8 sequences over 2000: 82 and 76 us; a
     // prompt of 1024 with 12 heads: 42 and 52 us.  Both give the same sums.
     const bool two = static_cast<int64_t>(p.n_wide) * p.KV >= 384;
+    // Tiles of 64, 96 and 128 values of a head: what pads a head is multiplied too.  Heads of 80 as 128, fp32 and bf16
+    // pages: a prompt of 4096 with 12 heads 383 and 217 us, as 96 294 and 191 us.
     if (p.bf16) {
         if (p.D <= 64) launch<__bf16, 64, 1>(p, s);
+        else if (p.D <= 96) launch<__bf16, 96, 1>(p, s);
         else launch<__bf16, 128, 1>(p, s);
     } else if (p.D <= 64) {
         if (two) launch<float, 64, 2>(p, s);
         else launch<float, 64, 1>(p, s);
+    } else if (p.D <= 96) {
+        if (two) launch<float, 96, 2>(p, s);
+        else launch<float, 96, 1>(p, s);
     } else {
         if (two) launch<float, 128, 2>(p, s);
         else launch<float, 128, 1>(p, s);

@@ -133,6 +133,11 @@ SHAPES = [
     ([20], [80], 1, 1, 1, 16),
     ([33], [41], 10, 2, 72, 32),
     ([0], [100], 4, 2, 24, 128),
+    ([70, 2100], [150, 66], 2, 2, 96, 32),             # and heads of 65 .. 96, cut
+    ([11], [97], 6, 2, 65, 16),
+    ([260], [70], 5, 5, 95, 64),
+    ([0, 500], [64, 90], 4, 1, 88, 16),
+    ([500], [64], 2, 2, 97, 16),
 ]
 
 
