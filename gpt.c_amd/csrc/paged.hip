@@ -31,7 +31,7 @@ struct gptc_paged_plan {
     hipEvent_t copied[2];
     int turn;
     bool is_set;
-    int n_tokens, n_items, n_wide, n_merges, max_parts, merge_rows;
+    int n_tokens, n_items, n_wide, n_many, n_few, merge_rows;
     int *table_at;  // where each sequence's page numbers start
     // Who writes each page in this step: checked without clearing the array between steps.
     long long *writer;  // step * max_seqs + sequence
@@ -81,7 +81,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
         c.per = (c.total * n_kv_heads + c.target - 1) / c.target;
         if (c.per < c.least) c.per = c.least;
     }
-    lists.n_items = lists.n_wide = lists.n_merges = lists.max_parts = lists.merge_rows = 0;
+    lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
@@ -105,8 +105,6 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
                 for (int i = 0; i < slots && r + i * kPagedRows < rows; ++i)
                     lists.merges[lists.n_merges++] = PagedMerge{tok0, rows, r + i * kPagedRows, parts + i, cuts, slots, 0, 0};
                 parts += cuts * slots;
-                lists.max_parts = std::max(lists.max_parts, cuts);
-                lists.merge_rows = std::max(lists.merge_rows, std::min(rows - r, kPagedRows));
             }
         }
         tok0 += fresh[s];
@@ -115,6 +113,11 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     const auto longer = [](const PagedItem &x, const PagedItem &y) { return x.key1 - x.key0 > y.key1 - y.key0; };
     std::sort(lists.items, lists.items + lists.n_items, longer);
     std::sort(lists.wide, lists.wide + lists.n_wide, longer);
+    const auto rows_of = [](const PagedMerge &x) { return std::min(x.rows - x.row0, kPagedRows); };
+    lists.n_many = static_cast<int>(std::partition(lists.merges, lists.merges + lists.n_merges,
+                                                   [&](const PagedMerge &x) { return paged_many(x.n, rows_of(x)); }) -
+                                    lists.merges);
+    for (int i = 0; i < lists.n_many; ++i) lists.merge_rows = std::max(lists.merge_rows, rows_of(lists.merges[i]));
     return true;
 }
 
@@ -362,6 +365,7 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     h[1] = lists.n_items;
     h[2] = lists.n_merges;
     h[3] = lists.n_wide;
+    h[4] = lists.n_many;
     auto send = [&](size_t from, size_t count) {
         if (count > 0)
             hipCheck(hipMemcpyAsync(plan->dev + from, h + from, sizeof(int) * count, hipMemcpyHostToDevice, stream));
@@ -376,8 +380,8 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     plan->n_tokens = t;
     plan->n_items = lists.n_items;
     plan->n_wide = lists.n_wide;
-    plan->n_merges = lists.n_merges;
-    plan->max_parts = lists.max_parts;
+    plan->n_many = lists.n_many;
+    plan->n_few = lists.n_merges - lists.n_many;
     plan->merge_rows = lists.merge_rows;
     plan->is_set = true;
 }
@@ -610,8 +614,8 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
     a.n_items = capturing ? plan->item_cap : plan->n_items;
     a.n_wide = capturing ? plan->wide_cap : plan->n_wide;
-    a.n_merges = capturing ? plan->merge_cap : plan->n_merges;
-    a.many_parts = capturing || plan->max_parts > kPagedFewParts;
+    a.n_many = capturing ? plan->part_cap / (kPagedFewParts + 1) : plan->n_many;  // each has more parts than that
+    a.n_few = capturing ? plan->merge_cap : plan->n_few;
     a.merge_rows = capturing ? kPagedRows : plan->merge_rows;
     a.bf16 = c->dtype == GPTC_BF16;
     a.vec = D % (a.bf16 ? 8 : 4) == 0 && aligned16(a.q) && aligned16(a.out);

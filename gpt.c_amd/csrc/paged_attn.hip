@@ -360,14 +360,10 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     }
 }
 
-// Joins the parts of rows whose keys were cut, up to kPagedFewParts: 16 rows a workgroup, 16 threads a row.  Products and
-// sums are rounded one by one here and below, and in one order up to kPagedFewParts, so that both kernels give the same.
+// The parts of rows whose keys were cut are joined by one launch, in two ways (paged_many).  Few parts: 16 rows a
+// workgroup, 16 threads a row.
 template <bool VEC>
-__global__ __launch_bounds__(256) void paged_merge_few_kernel(const PagedAttnParams a) {
-#pragma clang fp contract(off)
-    const int i = blockIdx.x / a.KV, kv = blockIdx.x - i * a.KV;
-    if (i >= a.head[2]) return;
-    const PagedMerge mg = a.merges[i];
+__device__ __forceinline__ void merge_few(const PagedAttnParams &a, const PagedMerge &mg, int kv) {
     const int r = threadIdx.x >> 4, row = mg.row0 + r;
     const int token = mg.tok0 + row / a.group;
     if (row >= mg.rows || token >= a.rows) return;
@@ -384,28 +380,23 @@ __global__ __launch_bounds__(256) void paged_merge_few_kernel(const PagedAttnPar
         for (int p = 0; p < mg.n; ++p) {
             const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
             const float f = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - big);
-            sum += ml[1] * f;
+            sum = fmaf(ml[1], f, sum);
             y += f * load4<VEC>(a.part_o + (first + p * next) * a.D, d, a.D);
         }
         store4<VEC>(dst, d, a.D, y / sum);
     }
 }
 
-// The same for many parts.  A workgroup takes one row: its threads weigh a part each, then sum the parts in groups of
-// threads that hold four values each, and the groups' sums are added in order.
+// Many parts: a workgroup takes one row.  Its threads weigh a part each, then sum the parts in groups of threads that
+// hold four values each, and the groups' sums are added in order.
 constexpr int kMergeThreads = 256;
 constexpr int kMaxParts = kPagedTarget + 1;  // a tile is cut into at most target / kv heads + 1 items
 
 template <bool VEC>
-__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedAttnParams a) {
-#pragma clang fp contract(off)
-    __shared__ float f_s[kMaxParts], l_s[kPagedFewParts];
+__device__ __forceinline__ void merge_many(const PagedAttnParams &a, const PagedMerge &mg, int kv, int r) {
+    __shared__ float f_s[kMaxParts];
     __shared__ float red[2][kMergeThreads / 64];
     __shared__ __attribute__((aligned(16))) float y_s[kMergeThreads][4];
-    const int i = blockIdx.x / (a.KV * a.merge_rows), left = blockIdx.x - i * a.KV * a.merge_rows;
-    if (i >= a.head[2]) return;
-    const int kv = left / a.merge_rows, r = left - kv * a.merge_rows;
-    const PagedMerge mg = a.merges[i];
     const int row = mg.row0 + r, token = mg.tok0 + row / a.group;
     if (row >= mg.rows || token >= a.rows) return;
     const int64_t first = (static_cast<int64_t>(mg.part0) * a.KV + kv) * kPagedRows + r;
@@ -422,18 +413,13 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
         const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (first + p * next));
         const float f = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - big);
         f_s[p] = f;
-        if (p < kPagedFewParts) l_s[p] = ml[1] * f;
-        sum += ml[1] * f;
+        sum = fmaf(ml[1], f, sum);
     }
     sum = wave_sum(sum);
     if ((tid & 63) == 0) red[1][w] = sum;
     __syncthreads();
     sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    if (mg.n <= kPagedFewParts) {
-        sum = 0.0f;
-        for (int p = 0; p < mg.n; ++p) sum += l_s[p];
-    }
-    const int lanes = a.D <= 64 ? 16 : 32, groups = kMergeThreads / lanes;  // 4 values a thread; kPagedFewParts groups or more
+    const int lanes = a.D <= 64 ? 16 : 32, groups = kMergeThreads / lanes;  // 4 values a thread
     const int q = tid / lanes, d = tid % lanes * 4;
     f32x4 y = zero4();
     if (d < a.D) {
@@ -445,6 +431,23 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
     if (q > 0 || d >= a.D) return;
     for (int k = 1; k < groups; ++k) y += *reinterpret_cast<const f32x4 *>(y_s[k * lanes + tid]);
     store4<VEC>(a.out + (static_cast<int64_t>(token) * a.H + kv * a.group + row % a.group) * a.D, d, a.D, y / sum);
+}
+
+// 16 contexts of 15000 on average (14 parts each, 4 rows): 17 us by few, 5 us by many; a prompt of 1024 (up to 4 parts
+// of all rows): 5 us by few, 14 us by many.
+template <bool VEC>
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedAttnParams a) {
+    const int many = a.n_many * a.KV * a.merge_rows;  // workgroups; they come first
+    if (static_cast<int>(blockIdx.x) < many) {
+        const int i = blockIdx.x / (a.KV * a.merge_rows), left = blockIdx.x - i * a.KV * a.merge_rows;
+        if (i >= a.head[4]) return;
+        const int kv = left / a.merge_rows;
+        merge_many<VEC>(a, a.merges[i], kv, left - kv * a.merge_rows);
+    } else {
+        const int at = blockIdx.x - many, i = at / a.KV;
+        if (a.head[4] + i >= a.head[2]) return;
+        merge_few<VEC>(a, a.merges[a.head[4] + i], at - i * a.KV);
+    }
 }
 
 template <typename T, int DP>
@@ -472,18 +475,10 @@ void launch_paged_attention(const PagedAttnParams &p, hipStream_t s) {
             else launch<float, 128>(p, s);
         }
     }
-    if (p.n_merges == 0) return;
-    // 16 contexts of 15000 on average (14 parts each, 4 rows): 17 us by the first kernel, 5 us by the second; a prompt
-    // of 1024 (up to 4 parts of all rows): 5 us by the first, 14 us by the second.
-    const unsigned n = static_cast<unsigned>(p.n_merges) * p.KV;
-    if (p.many_parts) {
-        const dim3 grid(n * p.merge_rows);
-        if (p.vec) paged_merge_kernel<true><<<grid, dim3(kMergeThreads), 0, s>>>(p);
-        else paged_merge_kernel<false><<<grid, dim3(kMergeThreads), 0, s>>>(p);
-    } else {
-        if (p.vec) paged_merge_few_kernel<true><<<dim3(n), dim3(256), 0, s>>>(p);
-        else paged_merge_few_kernel<false><<<dim3(n), dim3(256), 0, s>>>(p);
-    }
+    const unsigned n = static_cast<unsigned>(p.n_many * p.merge_rows + p.n_few) * p.KV;
+    if (n == 0) return;
+    if (p.vec) paged_merge_kernel<true><<<dim3(n), dim3(kMergeThreads), 0, s>>>(p);
+    else paged_merge_kernel<false><<<dim3(n), dim3(kMergeThreads), 0, s>>>(p);
     hipCheck(hipGetLastError());
 }
 

@@ -39,7 +39,9 @@ constexpr int paged_wide_keys(int dtype, int head_dim) {
 constexpr int kPagedTarget = 1024;
 constexpr int kPagedWideTarget = 512;
 
-constexpr int kPagedFewParts = 8;  // see launch_paged_attention
+// Which merges take a workgroup for each row, see paged_merge_kernel.
+constexpr int kPagedFewParts = 8;
+constexpr bool paged_many(int parts, int rows) { return parts > (rows > 8 ? 4 : 1) * kPagedFewParts; }
 
 // The lists of a step: items, wide items, and what is to be joined afterwards.
 struct PagedLists {
@@ -47,7 +49,8 @@ struct PagedLists {
     PagedMerge *merges;
     int item_cap, wide_cap, merge_cap, part_cap;
     int n_items, n_wide, n_merges;
-    int max_parts, merge_rows;  // of a tile: parts, and rows to be joined of 16
+    int n_many;      // merges of many parts, which come first
+    int merge_rows;  // the rows of one of them, at most
 };
 
 // Fills the lists for a step (an item's table receives its sequence); false when one of them does not fit.
@@ -59,7 +62,7 @@ struct PagedAttnParams {
     const float *q;
     float *out;
     const void *k, *v;
-    const int *head;  // {tokens, items, merges, wide items} of the plan, read on the device: a captured launch covers the
+    const int *head;  // {tokens, items, merges, wide items, merges of many parts} of the plan, read on the device: a captured launch covers the
                       // plan's capacity and runs what the plan holds then
     const PagedItem *items, *wide;
     const PagedMerge *merges;
@@ -68,9 +71,8 @@ struct PagedAttnParams {
     int q_stride, rows;       // floats of a q row; rows of q and out
     int H, KV, group, D, page_shift;
     float scale_log2;
-    int n_items, n_wide, n_merges;  // of the launch
-    int merge_rows;         // rows of a merge, at most
-    bool many_parts;        // see launch_paged_attention
+    int n_items, n_wide, n_many, n_few;  // of the launch
+    int merge_rows;         // rows of a merge of many parts, at most
     bool bf16, vec;         // vec: every row starts at a multiple of 16 bytes and holds whole vectors
 };
 
