@@ -50,15 +50,29 @@ int64_t part_slots(const gptc_paged_plan *p) {
 constexpr int kWideFrom = 64;
 
 // How a list's tiles of rows are cut.
-struct Cutting {
-    int tile, unit, target, least, whole;
-    int64_t total, per;
-};
-
 int tile_keys(int past, int rows, int row0, int tile, int group) {
     const int end = row0 + tile < rows ? row0 + tile : rows;
     return past + (end - 1) / group + 1;
 }
+
+struct Cutting {
+    bool wide;
+    int tile, unit, target, least, whole;
+    int64_t tiles, total, per;
+
+    int rounds(int keys) const { return (keys + unit - 1) / unit; }
+    int cuts(int rounds) const { return rounds <= whole ? 1 : static_cast<int>((rounds + per - 1) / per); }
+    bool takes(int rows) const { return (rows >= kWideFrom) == wide; }
+    int64_t items(int n_seqs, const int *past, const int *fresh, int group) const {
+        int64_t n = 0;
+        for (int s = 0; s < n_seqs; ++s) {
+            const int rows = fresh[s] * group;
+            if (!takes(rows)) continue;
+            for (int r = 0; r < rows; r += tile) n += cuts(rounds(tile_keys(past[s], rows, r, tile, group)));
+        }
+        return n;
+    }
+};
 
 }  // namespace
 
@@ -69,17 +83,22 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     // all; fewer leave CUs idle in ragged steps, more cost merging.  Parts have `least` rounds at least (256 keys; wide
     // ones of 128 or 512 keys take as long or longer), and what takes no more than `whole` stays whole: one token of
     // 12 heads over 300 fp32 keys (5 rounds) takes 7.6 us whole and 9.5 us in two parts.
-    Cutting cut[2] = {{kPagedRows, paged_unit(dtype), kPagedTarget, 4, 8, 0, 0},
-                      {paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget,
-                       256 / paged_wide_keys(dtype, head_dim), 256 / paged_wide_keys(dtype, head_dim), 0, 0}};
+    Cutting cut[2] = {{false, kPagedRows, paged_unit(dtype), kPagedTarget, 4, 8, 0, 0, 0},
+                      {true, paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget,
+                       256 / paged_wide_keys(dtype, head_dim), 256 / paged_wide_keys(dtype, head_dim), 0, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
         Cutting &c = cut[rows >= kWideFrom];
-        for (int r = 0; r < rows; r += c.tile) c.total += (tile_keys(past[s], rows, r, c.tile, group) + c.unit - 1) / c.unit;
+        for (int r = 0; r < rows; r += c.tile) c.total += c.rounds(tile_keys(past[s], rows, r, c.tile, group));
+        c.tiles += (rows + c.tile - 1) / c.tile;
     }
     for (Cutting &c : cut) {
         c.per = (c.total * n_kv_heads + c.target - 1) / c.target;
         if (c.per < c.least) c.per = c.least;
+        // Not a few more than run at once: 16 contexts of 8 kv heads took 165 us in 1048 workgroups, and take 158 us in
+        // fewer than 1024.  Wide ones differ too much in length for that (a prompt of 4096: 220 us became 244).
+        if (c.wide || c.tiles * n_kv_heads >= c.target) continue;
+        while (c.items(n_seqs, past, fresh, group) * n_kv_heads > c.target) c.per += (c.per + 15) / 16;
     }
     lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
@@ -90,8 +109,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
         const int slots = c.tile / kPagedRows;
         for (int r = 0; r < rows; r += c.tile) {
             const int keys = tile_keys(past[s], rows, r, c.tile, group);
-            const int rounds = (keys + c.unit - 1) / c.unit;
-            const int cuts = rounds <= c.whole ? 1 : static_cast<int>((rounds + c.per - 1) / c.per);
+            const int rounds = c.rounds(keys), cuts = c.cuts(rounds);
             int &n = wide ? lists.n_wide : lists.n_items;
             if (n + cuts > (wide ? lists.wide_cap : lists.item_cap)) return false;
             if (cuts > 1 && (parts + cuts * slots > lists.part_cap || lists.n_merges + slots > lists.merge_cap)) return false;
