@@ -21,6 +21,7 @@
 // fp32 pages are multiplied by v_mfma_f32_16x16x4_f32.  bf16 pages by v_mfma_f32_16x16x32_bf16 with the query
 // and the weights as exact sums of three bf16 values (24 bits): three products at a sixteenth of the cost of an
 // fp32 one each.
+#include <type_traits>
 #include "hip_check.hpp"
 #include "paged_attn_common.hpp"
 
@@ -46,7 +47,7 @@ struct Tile<float, DP, R> {
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
             if (row != nullptr) {
-                load_words<float, 4, R>(q.w[c], row, 16 * c + 4 * g, D);
+                load_words<float, 4, R, true>(q.w[c], row, 16 * c + 4 * g, D);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) q.w[c][e] = 0;
@@ -56,12 +57,12 @@ struct Tile<float, DP, R> {
     // kp, vp: row 0 of each group of 16 keys.
     __device__ __forceinline__ void load(const float *const (&kp)[1], const float *const (&vp)[1], int m, int g, int D) {
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) load_words<float, 4, R>(k[c], kp[0] + m * D, 16 * c + 4 * g, D);
+        for (int c = 0; c < DP / 16; ++c) load_words<float, 4, R, false>(k[c], kp[0] + m * D, 16 * c + 4 * g, D);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int h = 0; h < DP / 64; ++h)
-                load_words<float, 4, R>(v[i][h], vp[0] + (4 * g + i) * D, 64 * h + 4 * m, D);
+                load_words<float, 4, R, false>(v[i][h], vp[0] + (4 * g + i) * D, 64 * h + 4 * m, D);
     }
     __device__ __forceinline__ void clear_values(int g, int left) {
 #pragma unroll
@@ -124,7 +125,7 @@ struct Tile<__bf16, DP, R> {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (row != nullptr) {
-                    load_words<float, 4, R>(x[h], row, 32 * c + 8 * g + 4 * h, D);
+                    load_words<float, 4, R, true>(x[h], row, 32 * c + 8 * g + 4 * h, D);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[h][e] = 0;
@@ -143,10 +144,10 @@ struct Tile<__bf16, DP, R> {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int c = 0; c < DP / 32; ++c) load_words<__bf16, 4, R>(k[t][c], kp[t] + m * D, 32 * c + 8 * g, D);
+            for (int c = 0; c < DP / 32; ++c) load_words<__bf16, 4, R, false>(k[t][c], kp[t] + m * D, 32 * c + 8 * g, D);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            load_words<__bf16, kWords, R>(v[j], vp[j / 4] + (4 * g + j % 4) * D, 2 * kWords * m, D);
+            load_words<__bf16, kWords, R, false>(v[j], vp[j / 4] + (4 * g + j % 4) * D, 2 * kWords * m, D);
     }
     __device__ __forceinline__ void clear_values(int g, int left) {
 #pragma unroll
@@ -199,6 +200,91 @@ struct Tile<__bf16, DP, R> {
     static __device__ __forceinline__ int dim(int j, int g, int r) { return DP / 4 * g + DP / 16 * r + j; }
 };
 
+// One or two query rows over fp32 pages: a wave's products as multiplications and additions, sixteen lanes to a key.  Keys
+// come in the layout of the values (lane (m, g) holds values 64h + 4m + c of key 4g + i), so that after the sums over m
+// every lane has the weights that its values need.  The running maximum and sum are those of the lane's own g; they are
+// joined after the last key.
+template <int DP, Rows R, int NR>
+struct Dots {
+    static constexpr int kH = DP / 64;
+    uint32_t q[NR][kH][4];
+    float m[NR], l[NR];
+    f32x4 o[NR][kH];
+
+    __device__ __forceinline__ void init(const float *const (&rows)[NR], int lane, int D) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < kH; ++h) {
+                o[r][h] = zero4();
+                load_words<float, 4, R, true>(q[r][h], rows[r], 64 * h + 4 * (lane & 15), D);
+            }
+        }
+    }
+    static __device__ __forceinline__ void load(Tile<float, DP, R> &x, const float *kp, const float *vp, int m, int g, int D) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < kH; ++h) load_words<float, 4, R, false>(x.k[i * kH + h], kp + (4 * g + i) * D, 64 * h + 4 * m, D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < kH; ++h) load_words<float, 4, R, false>(x.v[i][h], vp + (4 * g + i) * D, 64 * h + 4 * m, D);
+    }
+    // key: of the lane's first; hides: some of the keys are past an end.
+    __device__ __forceinline__ void step(const Tile<float, DP, R> &x, int key, const int (&end)[NR], bool hides, float scale_log2) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            float s[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[i] = 0.0f;
+#pragma unroll
+                for (int h = 0; h < kH; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        s[i] = fmaf(__builtin_bit_cast(float, x.k[i * kH + h][c]), __builtin_bit_cast(float, q[r][h][c]), s[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = row16_sum(s[i]) * scale_log2;
+            if (hides) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key + i >= end[r]) s[i] = -INFINITY;
+            }
+            const float mx = fmaxf(fmaxf(m[r], fmaxf(s[0], s[1])), fmaxf(s[2], s[3]));
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            const float f = fast_exp2(m[r] - base);
+            l[r] *= f;
+#pragma unroll
+            for (int h = 0; h < kH; ++h) o[r][h] *= f;
+            m[r] = mx;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = fast_exp2(s[i] - base);
+                l[r] += p;
+#pragma unroll
+                for (int h = 0; h < kH; ++h)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[r][h][c] = fmaf(p, __builtin_bit_cast(float, x.v[i][h][c]), o[r][h][c]);
+            }
+        }
+    }
+    // The wave's state of row r in all its lanes.
+    __device__ __forceinline__ void join(int r) {
+        const float big = max4_rows(m[r]);
+        const float f = m[r] == -INFINITY ? l[r] : fast_exp2(m[r] - big);  // 0; NaN where a key's score was
+        m[r] = big;
+        l[r] = sum4_rows(l[r] * f);
+#pragma unroll
+        for (int h = 0; h < kH; ++h)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[r][h][c] = sum4_rows(o[r][h][c] * f);
+    }
+};
+
 template <typename T, int DP, Rows R>
 __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttnParams a) {
     using Step = Tile<T, DP, R>;
@@ -217,22 +303,22 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int total = it.past + it.rows / a.group;  // the sequence's tokens: slots past them hold anything
 
-    // The lane's query row, and the end of its keys.
-    const int row = it.row0 + n;
-    const int token = row / a.group;
-    const bool live = row < it.rows && it.tok0 + token < a.rows;
-    typename Step::Q q;
-    Step::load_q(q, live ? a.q + static_cast<int64_t>(it.tok0 + token) * a.q_stride + (kv * a.group + row - token * a.group) * a.D
-                         : nullptr, g, a.D);
-    const int end = it.past + token + 1;
-    const int first_end = it.past + it.row0 / a.group + 1;  // of the item's first row, which ends first
+    const int first_end = it.past + it.row0 / a.group + 1;  // the end of the first row's keys, which is the first
+    // Row i of the item: its end, and its query, or NULL for rows that are not there.
+    auto end_of = [&](int i) { return it.past + (it.row0 + i) / a.group + 1; };
+    auto query_of = [&](int i) {
+        const int row = it.row0 + i, token = row / a.group;
+        const bool live = row < it.rows && it.tok0 + token < a.rows;
+        return live ? a.q + static_cast<int64_t>(it.tok0 + token) * a.q_stride + (kv * a.group + row - token * a.group) * a.D
+                    : nullptr;
+    };
 
     const T *kpool = static_cast<const T *>(a.k), *vpool = static_cast<const T *>(a.v);
     const int *table = a.table + it.table;
     const int mask = (1 << a.page_shift) - 1;
     const int steps = (it.key1 - it.key0 - w * kKeys + kWaves * kKeys - 1) / (kWaves * kKeys);  // <= 0: none
     int pages[Step::kGroups];  // lane i: the pages of the wave's step i, i + 64, ...
-    auto load_step = [&](Step &x, int i) {
+    auto rows_of = [&](int i, const T *(&kp)[Step::kGroups], const T *(&vp)[Step::kGroups]) {
         if ((i & 63) == 0) {
 #pragma unroll
             for (int t = 0; t < Step::kGroups; ++t) {
@@ -241,7 +327,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
             }
         }
         const int key = it.key0 + (w + kWaves * i) * kKeys;
-        const T *kp[Step::kGroups], *vp[Step::kGroups];
 #pragma unroll
         for (int t = 0; t < Step::kGroups; ++t) {
             const int64_t page = __builtin_amdgcn_readlane(pages[t], i & 63);
@@ -249,79 +334,146 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
             kp[t] = kpool + at;
             vp[t] = vpool + at;
         }
-        x.load(kp, vp, n, g, a.D);
     };
-
     bool again = false;  // see rows_by_key
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o[DP / 16];
+
+    // All rows, on the matrix units.
+    auto products = [&] {
+        typename Step::Q q;
+        Step::load_q(q, query_of(n), g, a.D);
+        const int end = end_of(n);
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o[DP / 16];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) o[c] = zero4();
-    auto step = [&](Step &x, int i) {
-        const int key = it.key0 + (w + kWaves * i) * kKeys;
-        if (key + kKeys > total) x.clear_values(g, total - key);
-        if (key + kKeys > first_end) again |= x.take_out();
-        f32x4 s[Step::kGroups];
-        x.scores(q, s);
+        for (int c = 0; c < DP / 16; ++c) o[c] = zero4();
+        auto step = [&](Step &x, int i) {
+            const int key = it.key0 + (w + kWaves * i) * kKeys;
+            if (key + kKeys > total) x.clear_values(g, total - key);
+            if (key + kKeys > first_end) again |= x.take_out();
+            f32x4 s[Step::kGroups];
+            x.scores(q, s);
 #pragma unroll
-        for (int t = 0; t < Step::kGroups; ++t) settled(s[t]);
+            for (int t = 0; t < Step::kGroups; ++t) settled(s[t]);
 #pragma unroll
-        for (int t = 0; t < Step::kGroups; ++t) s[t] *= a.scale_log2;
-        if (key + kKeys > first_end) {
+            for (int t = 0; t < Step::kGroups; ++t) s[t] *= a.scale_log2;
+            if (key + kKeys > first_end) {
+#pragma unroll
+                for (int t = 0; t < Step::kGroups; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key + 16 * t + 4 * g + r >= end) s[t][r] = -INFINITY;
+            }
+            float mx = m;
 #pragma unroll
             for (int t = 0; t < Step::kGroups; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (key + 16 * t + 4 * g + r >= end) s[t][r] = -INFINITY;
-        }
-        float mx = m;
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
+            mx = max4_rows(mx);
+            const float base = mx == -INFINITY ? 0.0f : mx;  // no key of this row yet
+            if (__any(mx > m)) {
+                const float f = fast_exp2(m - base);
+                l *= f;
 #pragma unroll
-        for (int t = 0; t < Step::kGroups; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
-        mx = max4_rows(mx);
-        const float base = mx == -INFINITY ? 0.0f : mx;  // no key of this row yet
-        if (__any(mx > m)) {
-            const float f = fast_exp2(m - base);
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) o[c] *= f;
-            m = mx;
-        }
-#pragma unroll
-        for (int t = 0; t < Step::kGroups; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[t][r] = fast_exp2(s[t][r] - base);
-                l += s[t][r];
+                for (int c = 0; c < DP / 16; ++c) o[c] *= f;
+                m = mx;
             }
-        x.values(s, o);
+#pragma unroll
+            for (int t = 0; t < Step::kGroups; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[t][r] = fast_exp2(s[t][r] - base);
+                    l += s[t][r];
+                }
+            x.values(s, o);
+        };
+        // Two steps in turn: the loads of one are in flight while the other is multiplied.
+        auto load_step = [&](Step &x, int i) {
+            const T *kp[Step::kGroups], *vp[Step::kGroups];
+            rows_of(i, kp, vp);
+            x.load(kp, vp, n, g, a.D);
+        };
+        Step x, y;
+        if (steps > 0) load_step(x, 0);
+        for (int i = 0; i < steps; i += 2) {
+            if (i + 1 < steps) load_step(y, i + 1);
+            step(x, i);
+            if (i + 1 >= steps) break;
+            if (i + 2 < steps) load_step(x, i + 2);
+            step(y, i + 1);
+        }
+
+        drain();
+        l = sum4_rows(l);
+        if (g == 0) {
+            m_s[w][n] = m;
+            l_s[w][n] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < DP / 16; j += 4)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<f32x4 *>(&o_s[w][n][Step::dim(j, g, r)]) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
     };
-    // Two steps in turn: the loads of one are in flight while the other is multiplied.
-    Step x, y;
-    if (steps > 0) load_step(x, 0);
-    for (int i = 0; i < steps; i += 2) {
-        if (i + 1 < steps) load_step(y, i + 1);
-        step(x, i);
-        if (i + 1 >= steps) break;
-        if (i + 2 < steps) load_step(x, i + 2);
-        step(y, i + 1);
+    // One or two, fp32 pages.
+    auto dots = [&](auto count) {
+        constexpr int NR = decltype(count)::value, kAhead = 4;  // steps on their way
+        Dots<DP, R, NR> dots;
+        const float *src[NR];
+        int end[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            src[r] = query_of(r);
+            if (src[r] == nullptr) src[r] = a.q;  // its result is not stored
+            end[r] = end_of(r);
+        }
+        dots.init(src, lane, a.D);
+        Step x[kAhead];
+        auto load_step = [&](Step &x, int i) {
+            const T *kp[Step::kGroups], *vp[Step::kGroups];
+            rows_of(i, kp, vp);
+            dots.load(x, kp[0], vp[0], n, g, a.D);
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (i < steps) load_step(x[i], i);
+        for (int i0 = 0; i0 < steps; i0 += kAhead) {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int i = i0 + j;
+                if (i >= steps) break;
+                const int key = it.key0 + (w + kWaves * i) * kKeys;
+                if (key + kKeys > total) x[j].clear_values(g, total - key);
+                const bool hides = key + kKeys > first_end;
+                if (hides) again |= x[j].take_out();
+                dots.step(x[j], key + 4 * g, end, hides, a.scale_log2);
+                if (i + kAhead < steps) load_step(x[j], i + kAhead);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            dots.join(r);
+            if (g != 0) continue;
+            m_s[w][r] = dots.m[r];
+            l_s[w][r] = dots.l[r];
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h) *reinterpret_cast<f32x4 *>(&o_s[w][r][64 * h + 4 * n]) = dots.o[r][h];
+        }
+    };
+    const int n_rows = it.rows - it.row0;
+    if constexpr (sizeof(T) == 4) {
+        if (n_rows == 1)
+            dots(std::integral_constant<int, 1>());
+        else if (n_rows == 2)
+            dots(std::integral_constant<int, 2>());
+        else
+            products();
+    } else {
+        products();
     }
 
     // The waves' states joined: sums of o 2^(m_w - M).
-    drain();
-    l = sum4_rows(l);
-    if (g == 0) {
-        m_s[w][n] = m;
-        l_s[w][n] = l;
-    }
     again = __any(again);
     if (lane == 0) again_s[w] = again;
-#pragma unroll
-    for (int j = 0; j < DP / 16; j += 4)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<f32x4 *>(&o_s[w][n][Step::dim(j, g, r)]) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
     __syncthreads();
     if (again_s[0] | again_s[1] | again_s[2] | again_s[3]) {
         constexpr int kEach = kPagedRows / kWaves;

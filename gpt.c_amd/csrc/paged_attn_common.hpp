@@ -16,33 +16,37 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // vectors; or nothing.
 enum Rows { kFull, kVec, kAny };
 
-// N consecutive 32-bit words of T values from row + d; values at or past D are zeros (the load then takes the
-// row's first values instead, so that no branch parts the loads).
-template <typename T, int N, Rows R>
+// N consecutive 32-bit words of T values from row + d.  Values at or past D come from the row itself, so that no branch
+// parts the loads; with kZero (queries) they are zeros.  Keys and values go without: the query is 0 there and results
+// past D are not stored, and a selection between load and use would have to wait for the load.
+template <typename T, int N, Rows R, bool kZero>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const T *row, int d, int D) {
     if constexpr (R != kAny) {
         static_assert(N == 1 || N == 2 || N == 4, "one load");
         const bool in = R == kFull || d < D;
         const T *from = row + (in ? d : 0);
         if constexpr (N == 1) {
-            const uint32_t x = *reinterpret_cast<const uint32_t *>(from);
-            w[0] = in ? x : 0;
+            w[0] = *reinterpret_cast<const uint32_t *>(from);
         } else {
             typedef uint32_t vec __attribute__((ext_vector_type(N)));
             const vec x = *reinterpret_cast<const vec *>(from);
 #pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = in ? x[i] : 0;
+            for (int i = 0; i < N; ++i) w[i] = x[i];
         }
+        if (kZero && !in)
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = 0;
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = d + i < D ? __builtin_bit_cast(uint32_t, row[d + i]) : 0u;
+        for (int i = 0; i < N; ++i) {
+            w[i] = __builtin_bit_cast(uint32_t, row[min(d + i, D - 1)]);
+            if (kZero && d + i >= D) w[i] = 0;
+        }
     } else {
+        static_assert(!kZero, "queries are floats");
         const uint16_t *r = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t lo = d + 2 * i < D ? r[d + 2 * i] : 0u, hi = d + 2 * i + 1 < D ? r[d + 2 * i + 1] : 0u;
-            w[i] = lo | hi << 16;
-        }
+        for (int i = 0; i < N; ++i) w[i] = r[min(d + 2 * i, D - 1)] | static_cast<uint32_t>(r[min(d + 2 * i + 1, D - 1)]) << 16;
     }
 }
 

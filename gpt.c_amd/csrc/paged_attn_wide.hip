@@ -75,8 +75,8 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
             uint32_t x[2][4];
-            load_words<float, 4, R>(x[0], src, 32 * c + 8 * g, a.D);
-            load_words<float, 4, R>(x[1], src, 32 * c + 8 * g + 4, a.D);
+            load_words<float, 4, R, true>(x[0], src, 32 * c + 8 * g, a.D);
+            load_words<float, 4, R, true>(x[1], src, 32 * c + 8 * g + 4, a.D);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 uint32_t p[3];
@@ -115,13 +115,13 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
         for (int i = 0; i < kKLoads; ++i) {
             const int p = min(tid + i * kThreads, kKAll - 1), r = p / kPieces;
             const int64_t at = ((static_cast<int64_t>(k_page[i]) * a.KV + kv) << a.page_shift) + ((key + r) & mask);
-            load_words<T, 4, R>(kr[i], kpool + at * a.D, p % kPieces * kPiece, a.D);
+            load_words<T, 4, R, false>(kr[i], kpool + at * a.D, p % kPieces * kPiece, a.D);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int r = v_key + 16 * (j / 4) + j % 4;
             const int64_t at = ((static_cast<int64_t>(v_page[j / 4]) * a.KV + kv) << a.page_shift) + ((key + r) & mask);
-            load_words<T, kVWords, R>(vr[j], vpool + at * a.D, v_dim, a.D);
+            load_words<T, kVWords, R, false>(vr[j], vpool + at * a.D, v_dim, a.D);
         }
     };
     const int item_end = it.past + it.row0 / a.group + 1;  // of the item's first row
