@@ -78,26 +78,36 @@ struct Cutting {
 
 bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim,
                           int dtype, PagedLists &lists) {
-    // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose
-    // keys take more rounds than `per` is cut evenly: `per` makes about four workgroups per CU (two wide ones) in
-    // all; fewer leave CUs idle in ragged steps, more cost merging.  Parts have `least` rounds at least (256 keys; wide
-    // ones of 128 or 512 keys take as long or longer), and what takes no more than `whole` stays whole: one token of
-    // 12 heads over 300 fp32 keys (5 rounds) takes 7.6 us whole and 9.5 us in two parts.
-    Cutting cut[2] = {{false, kPagedRows, paged_unit(dtype), kPagedTarget, 4, 8, 0, 0, 0},
-                      {true, paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget,
-                       256 / paged_wide_keys(dtype, head_dim), 256 / paged_wide_keys(dtype, head_dim), 0, 0, 0}};
+    // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose keys take
+    // more than `per` rounds is cut evenly, into parts of `least` rounds at least; what takes no more than `whole` stays
+    // whole.  Joining costs 3 to 4 us, a round 0.5 us up to heads of 64 and 1.4 us above: one token of 32 heads of 128
+    // over 900 bf16 keys (8 rounds) takes 14.5 us whole and 11.3 us in four parts, of 12 heads of 64 over 364 fp32 keys
+    // (6 rounds) 6.2 us and 7.9 us.  Wide ones have 256 keys at least (parts of 128 or 512 take as long or longer).
+    const bool small = head_dim <= 64;
+    const int tile_256 = 256 / paged_wide_keys(dtype, head_dim);
+    Cutting cut[2] = {{false, kPagedRows, paged_unit(dtype), kPagedTarget, small ? 4 : 2, small ? 8 : 4, 0, 0, 0},
+                      {true, paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, tile_256, tile_256,
+                       0, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
         Cutting &c = cut[rows >= kWideFrom];
         for (int r = 0; r < rows; r += c.tile) c.total += c.rounds(tile_keys(past[s], rows, r, c.tile, group));
         c.tiles += (rows + c.tile - 1) / c.tile;
     }
-    for (Cutting &c : cut) {
-        c.per = (c.total * n_kv_heads + c.target - 1) / c.target;
-        if (c.per < c.least) c.per = c.least;
-        // Not a few more than run at once: 16 contexts of 8 kv heads took 165 us in 1048 workgroups, and take 158 us in
-        // fewer than 1024.  Wide ones differ too much in length for that (a prompt of 4096: 220 us became 244).
-        if (c.wide || c.tiles * n_kv_heads >= c.target) continue;
+    for (Cutting &c : cut) c.per = std::max<int64_t>(c.least, (c.total * n_kv_heads + c.target - 1) / c.target);
+    // Single tokens, or few.  `slots` workgroups run at once, two on a CU up to heads of 64 (224 registers) and one above;
+    // the work is done soonest when all of them get the same, and a few too many would run alone.  So there are as many
+    // as that where the tiles can be cut in three, twice as many where they cannot, and where there are more tiles than
+    // that, only the longest are cut.  Heads of 128, fp32: 8 contexts of 3200 of 8 kv heads 45 us in 256 and 48 in 512
+    // workgroups (59 us in 1024), 32 of 1700 107 and 92 us, 64 of 900 90 us whole, 104 us where every one was cut in two.
+    // Wide items differ too much in length for that (a prompt of 4096: 220 us became 244).
+    Cutting &c = cut[0];
+    const int64_t slots = small ? 512 : 256, tiles = c.tiles * n_kv_heads;
+    if (tiles >= 2 * slots) {
+        c.per = std::max(c.per, (2 * c.total + c.tiles - 1) / c.tiles);
+    } else {
+        c.target = static_cast<int>(3 * tiles <= slots ? slots : 2 * slots);
+        c.per = std::max(c.per, (c.total * n_kv_heads + c.target - 1) / c.target);
         while (c.items(n_seqs, past, fresh, group) * n_kv_heads > c.target) c.per += (c.per + 15) / 16;
     }
     lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;

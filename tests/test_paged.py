@@ -161,7 +161,7 @@ def test_long_contexts_are_cut_and_short_ones_are_not(lib):
     n, items = schedule(lib, [100], [1], 12, 12, gptc.F32, 4096)
     assert n == 1 and items[0][6] == -1
     n, items = schedule(lib, [100000], [1], 12, 12, gptc.F32, 4096)
-    assert n > 50 and (items[:, 6] >= 0).all()
+    assert n > 30 and (items[:, 6] >= 0).all()
     sizes = items[:, 5] - items[:, 4]
     assert sizes.max() - sizes.min() <= 64
 
