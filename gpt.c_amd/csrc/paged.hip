@@ -101,14 +101,14 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     // that, only the longest are cut.  Heads of 128, fp32: 8 contexts of 3200 of 8 kv heads 45 us in 256 and 48 in 512
     // workgroups (59 us in 1024), 32 of 1700 107 and 92 us, 64 of 900 90 us whole, 104 us where every one was cut in two.
     // Wide items differ too much in length for that (a prompt of 4096: 220 us became 244).
-    Cutting &c = cut[0];
-    const int64_t slots = small ? 512 : 256, tiles = c.tiles * n_kv_heads;
+    Cutting &few = cut[0];
+    const int64_t slots = small ? 512 : 256, tiles = few.tiles * n_kv_heads;
     if (tiles >= 2 * slots) {
-        c.per = std::max(c.per, (2 * c.total + c.tiles - 1) / c.tiles);
+        few.per = std::max(few.per, (2 * few.total + few.tiles - 1) / few.tiles);
     } else {
-        c.target = static_cast<int>(3 * tiles <= slots ? slots : 2 * slots);
-        c.per = std::max(c.per, (c.total * n_kv_heads + c.target - 1) / c.target);
-        while (c.items(n_seqs, past, fresh, group) * n_kv_heads > c.target) c.per += (c.per + 15) / 16;
+        few.target = static_cast<int>(3 * tiles <= slots ? slots : 2 * slots);
+        few.per = std::max(few.per, (few.total * n_kv_heads + few.target - 1) / few.target);
+        while (few.items(n_seqs, past, fresh, group) * n_kv_heads > few.target) few.per += (few.per + 15) / 16;
     }
     lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
