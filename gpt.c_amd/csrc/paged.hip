@@ -82,12 +82,12 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     // more than `per` rounds is cut evenly, into parts of `least` rounds at least; what takes no more than `whole` stays
     // whole.  Joining costs 3 to 4 us, a round 0.5 us up to heads of 64 and 1.4 us above: one token of 32 heads of 128
     // over 900 bf16 keys (8 rounds) takes 14.5 us whole and 11.3 us in four parts, of 12 heads of 64 over 364 fp32 keys
-    // (6 rounds) 6.2 us and 7.9 us.  Wide ones have 256 keys at least (parts of 128 or 512 take as long or longer).
+    // (6 rounds) 6.2 us and 7.9 us.
     const bool small = head_dim <= 64;
-    const int tile_256 = 256 / paged_wide_keys(dtype, head_dim);
+    const int wide_least = std::max(1, 64 / paged_wide_keys(dtype, head_dim));
     Cutting cut[2] = {{false, kPagedRows, paged_unit(dtype), kPagedTarget, small ? 4 : 2, small ? 8 : 4, 0, 0, 0},
-                      {true, paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, tile_256, tile_256,
-                       0, 0, 0}};
+                      {true, paged_wide_rows(dtype), paged_wide_keys(dtype, head_dim), kPagedWideTarget, wide_least,
+                       wide_least, 0, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
         Cutting &c = cut[rows >= kWideFrom];
@@ -100,7 +100,6 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     // as that where the tiles can be cut in three, twice as many where they cannot, and where there are more tiles than
     // that, only the longest are cut.  Heads of 128, fp32: 8 contexts of 3200 of 8 kv heads 45 us in 256 and 48 in 512
     // workgroups (59 us in 1024), 32 of 1700 107 and 92 us, 64 of 900 90 us whole, 104 us where every one was cut in two.
-    // Wide items differ too much in length for that (a prompt of 4096: 220 us became 244).
     Cutting &few = cut[0];
     const int64_t slots = small ? 512 : 256, tiles = few.tiles * n_kv_heads;
     if (tiles >= 2 * slots) {
@@ -110,6 +109,11 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
         few.per = std::max(few.per, (few.total * n_kv_heads + few.target - 1) / few.target);
         while (few.items(n_seqs, past, fresh, group) * n_kv_heads > few.target) few.per += (few.per + 15) / 16;
     }
+    // Wide ones differ too much in length for that (a prompt of 4096: 220 us became 244), but parts of less than 256 keys
+    // pay only as long as every workgroup has a CU of its own: a prompt of 512 with 12 heads of 64 takes 22 us in parts of
+    // 256 fp32 keys and 14 us in 240 workgroups of 64, one of 1024 26 us in 240 of 256 and 28 us in 432 of 128.
+    const int wide_most = 256 / paged_wide_keys(dtype, head_dim);
+    while (cut[1].per < wide_most && cut[1].items(n_seqs, past, fresh, group) * n_kv_heads > 256) ++cut[1].per;
     lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
     for (int s = 0; s < n_seqs; ++s) {
