@@ -24,8 +24,9 @@
 // The weights bind it, eleven 64-bit operations each, and then the adds to the histogram.  Logits held in registers
 // between the passes (49152 of a row at 512 threads) spilled and came out 1.1 to 1.3 times as slow.
 //
-// MI355X: a row of 50257 logits takes 15.5 us with top-k 40, 64 rows of them with top-p and ordinary settings 50 us,
-// 256 rows of 131072 (134 MB) 138 us, 0.97 TB/s.
+// MI355X, rows of 50257 logits: greedy 6 us, top-k 40 15 us, min-p 14 us, no filter 23 us, top-p 37 to 50 us, for one row
+// as for 64.  256 rows of 131072 (134 MB): greedy 26 us (5.2 TB/s), top-k 54 us, top-p 97 to 142 us (three to four
+// passes of 23 us or more).
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include "gpu_kernels.h"
@@ -96,6 +97,15 @@ __device__ __forceinline__ u64 wave_scan64(u64 v) {
     v += dpp64<0x118, 0xf>(v);
     v += dpp64<0x142, 0xa>(v);
     return v + dpp64<0x143, 0xc>(v);
+}
+
+__device__ __forceinline__ int wave_scan32(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
 __device__ __forceinline__ u64 lane_of(u64 v, int lane) {
@@ -212,8 +222,12 @@ __device__ __forceinline__ int gather(const Row &r, Lds &s, Token *to, int room,
         uint32_t mask = 0;
 #pragma unroll
         for (int e = 0; e < kChunk; ++e) mask |= want(l[e]) ? 1u << e : 0u;
-        if (mask == 0) return;
-        int at = atomicAdd(&s.n, __popc(mask));
+        const int count = __popc(mask), upto = wave_scan32(count), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+        if (all == 0) return;
+        int at = 0;
+        // One for the wave: its lanes' would queue (top-k 3000 of 50257 tokens: 38 us with an add a lane, 31 us so).
+        if ((threadIdx.x & (kWave - 1)) == 0) at = atomicAdd(&s.n, all);
+        at = __builtin_amdgcn_readfirstlane(at) + upto - count;
         while (mask != 0) {
             if (at < room) to[at].i = i + (__ffs(mask) - 1) * kWave;
             ++at;
