@@ -239,6 +239,21 @@ extern "C" void gptc_paged_cache_free(gptc_paged_cache_t *cache) {
 
 // ---- the plan ----
 
+namespace {
+
+// What a step uses of the plan's memory, from the pinned copy to the device, at the same places.
+constexpr int kSegments = 6;
+struct Segments {
+    size_t from[kSegments], count[kSegments];
+};
+
+__global__ __launch_bounds__(256) void send_plan_kernel(const Segments s, const int *src, int *dst) {
+    const size_t from = s.from[blockIdx.y], count = s.count[blockIdx.y];
+    for (size_t i = blockIdx.x * 256 + threadIdx.x; i < count; i += 256 * gridDim.x) dst[from + i] = src[from + i];
+}
+
+}  // namespace
+
 extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *cache, const int n_heads,
                                                      const int max_seqs, const int max_tokens, const int max_len) {
     REQUIRE_ARG(cache);
@@ -398,16 +413,15 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     h[2] = lists.n_merges;
     h[3] = lists.n_wide;
     h[4] = lists.n_many;
-    auto send = [&](size_t from, size_t count) {
-        if (count > 0)
-            hipCheck(hipMemcpyAsync(plan->dev + from, h + from, sizeof(int) * count, hipMemcpyHostToDevice, stream));
-    };
-    send(0, plan->at_items + 8 * static_cast<size_t>(lists.n_items));
-    send(plan->at_wide, 8 * static_cast<size_t>(lists.n_wide));
-    send(plan->at_merges, 8 * static_cast<size_t>(lists.n_merges));
-    send(plan->at_slot, t);
-    send(plan->at_pos, t);
-    send(plan->at_table, at);
+    // One kernel that reads the host's memory: with a copy command for each piece the call took 10 us longer.
+    const Segments segments = {{0, plan->at_wide, plan->at_merges, plan->at_slot, plan->at_pos, plan->at_table},
+                               {plan->at_items + 8 * static_cast<size_t>(lists.n_items), 8 * static_cast<size_t>(lists.n_wide),
+                                8 * static_cast<size_t>(lists.n_merges), static_cast<size_t>(t), static_cast<size_t>(t),
+                                static_cast<size_t>(at)}};
+    const size_t most = *std::max_element(segments.count, segments.count + kSegments);
+    send_plan_kernel<<<dim3(static_cast<unsigned>(std::min<size_t>((most + 255) / 256, 512)), kSegments), dim3(256), 0, stream>>>(
+        segments, h, plan->dev);
+    hipCheck(hipGetLastError());
     hipCheck(hipEventRecord(plan->copied[plan->turn], stream));
     plan->n_tokens = t;
     plan->n_items = lists.n_items;
@@ -474,7 +488,9 @@ __device__ __forceinline__ void store_vec(__bf16 *p, const Vec<W> &x) {
 
 // One thread per W consecutive values of a head of a token.  A pass over the data and nothing else: each value is
 // read once (a rotated one's partner comes from the same cache lines) and written once, so HBM bounds it for
-// prompts and the launch for single tokens.  Without rotation the queries stay where they are.
+// prompts and the launch for single tokens.  Without rotation the queries stay where they are.  MI355X: 5740 tokens of
+// prompts, 32 and 8 heads of 128 into bf16 pages (262 MB) 51 us, 5.1 TB/s (a copy of that size reaches 5.1); 8 single
+// tokens 3.4 us.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void append_kernel(const AppendParams a) {
     const int per_head = a.D / W;

@@ -20,7 +20,11 @@
 //
 // fp32 pages are multiplied by v_mfma_f32_16x16x4_f32.  bf16 pages by v_mfma_f32_16x16x32_bf16 with the query
 // and the weights as exact sums of three bf16 values (24 bits): three products at a sixteenth of the cost of an
-// fp32 one each.
+// fp32 one each.  One or two rows over fp32 pages go without either (Dots).
+//
+// HBM bounds many or long contexts, each page being read once; round trips bound few and short ones.  MI355X: 64 tokens
+// over up to 4000 keys, 12 heads of 64, fp32 (889 MB) 158 us, 5.6 TB/s; 16 over up to 30000, 32 heads on 8 of 128, bf16
+// (836 MB) 154 us, 5.4 TB/s; one token over 300 keys 5.6 us.
 #include <type_traits>
 #include "hip_check.hpp"
 #include "paged_attn_common.hpp"
@@ -204,6 +208,9 @@ struct Tile<__bf16, DP, R> {
 // come in the layout of the values (lane (m, g) holds values 64h + 4m + c of key 4g + i), so that after the sums over m
 // every lane has the weights that its values need.  The running maximum and sum are those of the lane's own g; they are
 // joined after the last key.
+// The matrix instruction takes 16 rows for the price of one: 12 heads of 64, one token over 300 keys 8.1 us by it, 5.6 us
+// so; 8 heads of 128, 8 over 400 keys 18.7 and 9.8 us.  Four rows take as long or longer (32 heads on 8 of 128, 8 over
+// 3500 keys: 43 us by the matrix instruction, 46 us so).
 template <int DP, Rows R, int NR>
 struct Dots {
     static constexpr int kH = DP / 64;
@@ -386,7 +393,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
                 }
             x.values(s, o);
         };
-        // Two steps in turn: the loads of one are in flight while the other is multiplied.
+        // Two steps in turn: the loads of one are in flight while the other is multiplied.  Four, as below, were slower
+        // here (16 heads of 128 on bf16 pages: 8 to 20 %), the matrix instructions of a step covering its loads.
         auto load_step = [&](Step &x, int i) {
             const T *kp[Step::kGroups], *vp[Step::kGroups];
             rows_of(i, kp, vp);
@@ -416,7 +424,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttn
     };
     // One or two, fp32 pages.
     auto dots = [&](auto count) {
-        constexpr int NR = decltype(count)::value, kAhead = 4;  // steps on their way
+        constexpr int NR = decltype(count)::value, kAhead = 4;  // steps on their way: the work of one is short
         Dots<DP, R, NR> dots;
         const float *src[NR];
         int end[NR];
