@@ -667,6 +667,6 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.merge_rows = capturing ? kPagedRows : plan->merge_rows;
     a.bf16 = c->dtype == GPTC_BF16;
     a.vec = D % (a.bf16 ? 8 : 4) == 0 && aligned16(a.q) && aligned16(a.out);
-    if (a.n_items + a.n_wide == 0) return;
+    if (a.n_items + a.n_wide == 0 || rows == 0) return;
     launch_paged_attention(a, s);
 }

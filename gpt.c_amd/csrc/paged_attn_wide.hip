@@ -75,8 +75,9 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
         token[u] = row[u] / a.group;
         live[u] = row[u] < it.rows && it.tok0 + token[u] < a.rows;
         end[u] = it.past + token[u] + 1;
-        const float *src = a.q + static_cast<int64_t>(it.tok0 + (live[u] ? token[u] : 0)) * a.q_stride +
-                           (kv * a.group + (live[u] ? row[u] - token[u] * a.group : 0)) * a.D;
+        const float *src = a.q;  // a captured launch may hold items of tokens that its tensors have no rows for
+        if (live[u])
+            src += static_cast<int64_t>(it.tok0 + token[u]) * a.q_stride + (kv * a.group + row[u] - token[u] * a.group) * a.D;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
             uint32_t x[2][4];

@@ -215,6 +215,38 @@ def test_a_captured_step_follows_the_plan(rt, dtype):
     rt.free(table)
 
 
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 30, 130])
+def test_a_captured_step_with_more_tokens_than_rows(rt, dtype, rows):
+    """A graph whose tensors have fewer rows than a later step has tokens serves the first of them, reads no others (they
+    would be NaN) and writes nothing behind its own rows."""
+    H, KV, D, page = 2, 2, 64, 16
+    past, fresh = [500, 20, 3], [100, 2, 150]
+    pool = Pool(rt, past, fresh, H, KV, D, page, dtype, seed=3)
+    pool.fill([p + f for p, f in zip(past, fresh)])
+    n = sum(fresh)
+    q = torch.full((n, H * D), float("nan"), device="cuda")
+    q[:rows] = torch.tensor(pool.normal(rows, H * D))
+    out = torch.full((n, H * D), 7.5, device="cuda")
+    whole, want = torch.nan_to_num(q), torch.empty(n, H * D, device="cuda")
+    torch.cuda.synchronize()
+    tq, tout = as_tensor(rt, q[:rows]), as_tensor(rt, out[:rows])
+    pool.plan.set(past, [1, 0, 0], pool.table)
+    pool.plan.attention(0, tq, tout)
+    graph = Graph(rt, lambda: pool.plan.attention(0, tq, tout))
+    out.fill_(7.5)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        pool.plan.set(past, fresh, pool.table)
+        graph.replay()
+        rt.sync()
+        pool.plan.attention(0, as_tensor(rt, whole), as_tensor(rt, want))
+        rt.sync()
+        assert torch.equal(out[:rows], want[:rows]) and (out[rows:] == 7.5).all()
+    graph.free()
+    pool.free()
+
+
 def test_captured_sampling(rt):
     rng = np.random.default_rng(4)
     rows, V = 6, 5003
