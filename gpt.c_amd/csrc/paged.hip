@@ -20,7 +20,7 @@ using namespace gptc;
 struct gptc_paged_plan {
     const gptc_paged_cache_t *cache;
     int n_heads, group, max_seqs, max_tokens, max_len, max_pages;
-    int item_cap, wide_cap, merge_cap, part_cap;
+    int item_cap, wide_cap, merge_cap, part_cap;  // wide_cap 0: no wide items
     // Device memory (taken by the first set): ints [head 8 | items | wide items | merges | slot | pos | table], then
     // the parts.
     int *dev;
@@ -62,12 +62,11 @@ struct Cutting {
 
     int rounds(int keys) const { return (keys + unit - 1) / unit; }
     int cuts(int rounds) const { return rounds <= whole ? 1 : static_cast<int>((rounds + per - 1) / per); }
-    bool takes(int rows) const { return (rows >= kWideFrom) == wide; }
-    int64_t items(int n_seqs, const int *past, const int *fresh, int group) const {
+    int64_t items(int n_seqs, const int *past, const int *fresh, int group, int wide_from) const {
         int64_t n = 0;
         for (int s = 0; s < n_seqs; ++s) {
             const int rows = fresh[s] * group;
-            if (!takes(rows)) continue;
+            if ((rows >= wide_from) != wide) continue;
             for (int r = 0; r < rows; r += tile) n += cuts(rounds(tile_keys(past[s], rows, r, tile, group)));
         }
         return n;
@@ -77,7 +76,8 @@ struct Cutting {
 }  // namespace
 
 bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim,
-                          int dtype, PagedLists &lists) {
+                          int dtype, bool wide, PagedLists &lists) {
+    const int wide_from = wide ? kWideFrom : INT32_MAX;
     // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose keys take
     // more than `per` rounds is cut evenly, into parts of `least` rounds at least; what takes no more than `whole` stays
     // whole.  Joining costs 3 to 4 us, a round 0.5 us up to heads of 64 and 1.4 us above: one token of 32 heads of 128
@@ -90,7 +90,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
                        wide_least, 0, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
-        Cutting &c = cut[rows >= kWideFrom];
+        Cutting &c = cut[rows >= wide_from];
         for (int r = 0; r < rows; r += c.tile) c.total += c.rounds(tile_keys(past[s], rows, r, c.tile, group));
         c.tiles += (rows + c.tile - 1) / c.tile;
     }
@@ -107,18 +107,18 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     } else {
         few.target = static_cast<int>(3 * tiles <= slots ? slots : 2 * slots);
         few.per = std::max(few.per, (few.total * n_kv_heads + few.target - 1) / few.target);
-        while (few.items(n_seqs, past, fresh, group) * n_kv_heads > few.target) few.per += (few.per + 15) / 16;
+        while (few.items(n_seqs, past, fresh, group, wide_from) * n_kv_heads > few.target) few.per += (few.per + 15) / 16;
     }
     // Wide ones differ too much in length for that (a prompt of 4096: 220 us became 244), but parts of less than 256 keys
     // pay only as long as every workgroup has a CU of its own: a prompt of 512 with 12 heads of 64 takes 22 us in parts of
     // 256 fp32 keys and 14 us in 240 workgroups of 64, one of 1024 26 us in 240 of 256 and 28 us in 432 of 128.
     const int wide_most = 256 / paged_wide_keys(dtype, head_dim);
-    while (cut[1].per < wide_most && cut[1].items(n_seqs, past, fresh, group) * n_kv_heads > 256) ++cut[1].per;
+    while (cut[1].per < wide_most && cut[1].items(n_seqs, past, fresh, group, wide_from) * n_kv_heads > 256) ++cut[1].per;
     lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
-        const bool wide = rows >= kWideFrom;
+        const bool wide = rows >= wide_from;
         const Cutting &c = cut[wide];
         const int slots = c.tile / kPagedRows;
         for (int r = 0; r < rows; r += c.tile) {
@@ -178,7 +178,7 @@ extern "C" int gptc_paged_schedule(const int n_seqs, const int *past, const int 
     l.wide = static_cast<PagedItem *>(mallocCheck(sizeof(PagedItem) * static_cast<size_t>(cap)));
     l.merges = static_cast<PagedMerge *>(mallocCheck(sizeof(PagedMerge) * static_cast<size_t>(l.merge_cap)));
     int n = -1;
-    if (paged_schedule(n_seqs, past, fresh, n_heads / n_kv_heads, n_kv_heads, head_dim, dtype, l) &&
+    if (paged_schedule(n_seqs, past, fresh, n_heads / n_kv_heads, n_kv_heads, head_dim, dtype, true, l) &&
         l.n_items + l.n_wide <= cap) {
         n = l.n_items + l.n_wide;
         for (int i = 0; i < l.n_items; ++i) l.items[i].table = 0;  // the item's kind
@@ -284,7 +284,9 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     const int cut = kPagedTarget / cache->n_kv_heads + 1, wide_cut = kPagedWideTarget / cache->n_kv_heads + 1;
     const int wide_rows = paged_wide_rows(cache->dtype), slots = wide_rows / kPagedRows;
     p->item_cap = static_cast<int>(work / kPagedRows + active) + cut;
-    p->wide_cap = static_cast<int>(work / wide_rows + active) + wide_cut;
+    // Plans of single tokens have no wide items, so that a graph captured with them has no launch for those.
+    const bool wide = group >= kWideFrom || (max_tokens > max_seqs && work >= kWideFrom);
+    p->wide_cap = wide ? static_cast<int>(work / wide_rows + active) + wide_cut : 0;
     p->merge_cap = cut + slots * wide_cut;
     p->part_cap = 2 * p->merge_cap;
     // A launch has fewer than 2^32 threads: 256 for each item and kv head, up to 512 for wide ones.
@@ -390,7 +392,7 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     lists.wide_cap = plan->wide_cap;
     lists.merge_cap = plan->merge_cap;
     lists.part_cap = plan->part_cap;
-    const bool fits = paged_schedule(n_seqs, past, fresh, plan->group, c->n_kv_heads, c->head_dim, c->dtype, lists);
+    const bool fits = paged_schedule(n_seqs, past, fresh, plan->group, c->n_kv_heads, c->head_dim, c->dtype, plan->wide_cap > 0, lists);
     CHECK_ERROR(!fits, "The work of %d sequences does not fit the plan.", n_seqs);
     int t = 0, at = 0;
     for (int s = 0; s < n_seqs; ++s) {
@@ -662,9 +664,12 @@ extern "C" void gptc_paged_attention_cuda(gptc_paged_plan_t *plan, const int lay
     a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
     a.n_items = capturing ? plan->item_cap : plan->n_items;
     a.n_wide = capturing ? plan->wide_cap : plan->n_wide;
-    a.n_many = capturing ? plan->part_cap / (kPagedFewParts + 1) : plan->n_many;  // each has more parts than that
-    a.n_few = capturing ? plan->merge_cap : plan->n_few;
-    a.merge_rows = capturing ? kPagedRows : plan->merge_rows;
+    a.merge_rows = plan->merge_rows;
+    a.merge_groups = (plan->n_many * plan->merge_rows + plan->n_few) * KV;
+    if (capturing) {
+        a.merge_rows = kPagedRows;
+        a.merge_groups = std::min(KV * plan->merge_cap, 1024);
+    }
     a.bf16 = c->dtype == GPTC_BF16;
     a.vec = D % (a.bf16 ? 8 : 4) == 0 && aligned16(a.q) && aligned16(a.out);
     if (a.n_items + a.n_wide == 0 || rows == 0) return;

@@ -562,6 +562,7 @@ __device__ __forceinline__ void merge_many(const PagedAttnParams &a, const Paged
     const int64_t first = (static_cast<int64_t>(mg.part0) * a.KV + kv) * kPagedRows + r;
     const int64_t next = static_cast<int64_t>(mg.step) * a.KV * kPagedRows;
     const int tid = threadIdx.x, w = tid >> 6;
+    __syncthreads();  // the workgroup's row before has been read
     float big = -INFINITY;
     for (int p = tid; p < mg.n; p += kMergeThreads) big = fmaxf(big, a.part_ml[2 * (first + p * next)]);
     big = wave_max(big);
@@ -595,18 +596,20 @@ __device__ __forceinline__ void merge_many(const PagedAttnParams &a, const Paged
 
 // 16 contexts of 15000 on average (14 parts each, 4 rows): 17 us by few, 5 us by many; a prompt of 1024 (up to 4 parts
 // of all rows): 5 us by few, 14 us by many.
+//
+// A workgroup takes what lies `gridDim.x` apart: a captured launch has no more of them than run at once, whatever the
+// plan can hold.
 template <bool VEC>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedAttnParams a) {
-    const int many = a.n_many * a.KV * a.merge_rows;  // workgroups; they come first
-    if (static_cast<int>(blockIdx.x) < many) {
-        const int i = blockIdx.x / (a.KV * a.merge_rows), left = blockIdx.x - i * a.KV * a.merge_rows;
-        if (i >= a.head[4]) return;
-        const int kv = left / a.merge_rows;
-        merge_many<VEC>(a, a.merges[i], kv, left - kv * a.merge_rows);
-    } else {
-        const int at = blockIdx.x - many, i = at / a.KV;
-        if (a.head[4] + i >= a.head[2]) return;
-        merge_few<VEC>(a, a.merges[a.head[4] + i], at - i * a.KV);
+    const int n_many = a.head[4], many = n_many * a.KV * a.merge_rows, all = many + (a.head[2] - n_many) * a.KV;
+    for (int at = blockIdx.x; at < all; at += gridDim.x) {
+        if (at < many) {
+            const int i = at / (a.KV * a.merge_rows), left = at - i * a.KV * a.merge_rows, kv = left / a.merge_rows;
+            merge_many<VEC>(a, a.merges[i], kv, left - kv * a.merge_rows);
+        } else {
+            const int few = at - many, i = few / a.KV;
+            merge_few<VEC>(a, a.merges[n_many + i], few - i * a.KV);
+        }
     }
 }
 
@@ -635,7 +638,7 @@ void launch_paged_attention(const PagedAttnParams &p, hipStream_t s) {
             else launch<float, 128>(p, s);
         }
     }
-    const unsigned n = static_cast<unsigned>(p.n_many * p.merge_rows + p.n_few) * p.KV;
+    const unsigned n = p.merge_groups;
     if (n == 0) return;
     if (p.vec) paged_merge_kernel<true><<<dim3(n), dim3(kMergeThreads), 0, s>>>(p);
     else paged_merge_kernel<false><<<dim3(n), dim3(kMergeThreads), 0, s>>>(p);

@@ -54,8 +54,9 @@ struct PagedLists {
 };
 
 // Fills the lists for a step (an item's table receives its sequence); false when one of them does not fit.
+// `wide` is false where wide items are not to be used.
 bool paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim, int dtype,
-                    PagedLists &lists);
+                    bool wide, PagedLists &lists);
 
 // What the attention kernels take.
 struct PagedAttnParams {
@@ -71,7 +72,7 @@ struct PagedAttnParams {
     int q_stride, rows;       // floats of a q row; rows of q and out
     int H, KV, group, D, page_shift;
     float scale_log2;
-    int n_items, n_wide, n_many, n_few;  // of the launch
+    int n_items, n_wide, merge_groups;  // of the launch
     int merge_rows;         // rows of a merge of many parts, at most
     bool bf16, vec;         // vec: every row starts at a multiple of 16 bytes and holds whole vectors
 };

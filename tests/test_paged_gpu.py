@@ -160,6 +160,21 @@ def test_attention(rt, case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("past, fresh", [([40, 3], [90, 9]), ([2000, 0], [70, 30])])
+def test_prompts_under_a_plan_of_single_tokens(rt, dtype, past, fresh):
+    pool = Pool(rt, past, fresh, 3, 3, 64, 32, dtype, seed=9)
+    kept = pool.fill([p + f for p, f in zip(past, fresh)])
+    plan = gptc.PagedPlan(rt, pool.cache, 3, 100, 100, 2100)
+    plan.set(past, fresh, pool.table)
+    q = pool.normal(sum(fresh), 3, 64)
+    tq, out = rt.from_numpy(q.reshape(sum(fresh), -1)), rt.empty((sum(fresh), 192))
+    plan.attention(0, tq, out)
+    check_attention(pool, kept, q, rt.to_numpy(out))
+    plan.free()
+    pool.free()
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
 def test_attention_is_the_same_every_time_and_in_the_qkv_layout(rt, dtype):
     pool = Pool(rt, [2500, 31], [3, 40], 6, 2, 64, 16, dtype, seed=5)
     kept = pool.fill([2503, 71])
