@@ -281,11 +281,11 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     // Every tile of rows is an item; cutting adds at most one item per `per` rounds, target / kv heads in all, and
     // cuts at most as many tiles, so it makes at most twice as many parts.
     const int64_t work = static_cast<int64_t>(max_tokens) * group, active = max_seqs < max_tokens ? max_seqs : max_tokens;
-    const int cut = kPagedTarget / cache->n_kv_heads + 1, wide_cut = kPagedWideTarget / cache->n_kv_heads + 1;
-    const int wide_rows = paged_wide_rows(cache->dtype), slots = wide_rows / kPagedRows;
-    p->item_cap = static_cast<int>(work / kPagedRows + active) + cut;
     // Plans of single tokens have no wide items, so that a graph captured with them has no launch for those.
     const bool wide = group >= kWideFrom || (max_tokens > max_seqs && work >= kWideFrom);
+    const int cut = kPagedTarget / cache->n_kv_heads + 1, wide_cut = wide ? kPagedWideTarget / cache->n_kv_heads + 1 : 0;
+    const int wide_rows = paged_wide_rows(cache->dtype), slots = wide_rows / kPagedRows;
+    p->item_cap = static_cast<int>(work / kPagedRows + active) + cut;
     p->wide_cap = wide ? static_cast<int>(work / wide_rows + active) + wide_cut : 0;
     p->merge_cap = cut + slots * wide_cut;
     p->part_cap = 2 * p->merge_cap;
