@@ -40,8 +40,7 @@ constexpr int kPagedTarget = 1024;
 constexpr int kPagedWideTarget = 512;
 
 // Which merges take a workgroup for each row, see paged_merge_kernel.
-constexpr int kPagedFewParts = 8;
-constexpr bool paged_many(int parts, int rows) { return parts > (rows > 8 ? 4 : 1) * kPagedFewParts; }
+constexpr bool paged_many(int parts, int rows) { return parts > (rows > 8 ? 32 : 4); }
 
 // The lists of a step: items, wide items, and what is to be joined afterwards.
 struct PagedLists {
