@@ -84,10 +84,11 @@ __device__ __forceinline__ void drain() {
 // rows, values that are not finite are taken out of the products, and an item where there was one is done again, one
 // key after the other.
 
-// A 32-bit word of T values without those that are not finite.
-template <typename T>
+// A 32-bit word of T values without those that are not finite; with kSplit also without the floats that split3 rounds to
+// infinity, from half a step past the largest bf16 value on.
+template <typename T, bool kSplit = false>
 __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
-    if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u ? 0 : w;
+    if constexpr (sizeof(T) == 4) return (w & 0x7fffffffu) >= (kSplit ? 0x7f7f8000u : 0x7f800000u) ? 0 : w;
     if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
     return w;

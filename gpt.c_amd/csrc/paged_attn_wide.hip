@@ -163,7 +163,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_wide_kernel(const PagedAttnP
             for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int i = 0; i < kVWords; ++i) {
-                    const uint32_t x = finite_part<T>(vr[j][i]);
+                    const uint32_t x = finite_part<T, true>(vr[j][i]);
                     any |= x != vr[j][i];
                     vr[j][i] = x;
                 }

@@ -457,3 +457,35 @@ def test_matches_the_frameworks_causal_forward(rt, dtype):
     err = np.abs(np.concatenate(got) - want).reshape(T, H, D)
     assert (err <= 2 * bound).all(), float((err / bound).max())
     pool.free()
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("H, KV, D", [(1, 1, 64), (4, 2, 128), (3, 1, 40), (2, 2, 33), (2, 2, 80)])
+@pytest.mark.parametrize("fresh", [20, 150])
+def test_a_later_tokens_largest_values_stay_hidden(rt, dtype, fresh, H, KV, D):
+    """Values at the end of the pages' range (of fp32 also the least that is rounded to infinity as bf16, and the one
+    before it), and keys of that size: rows before them are what they are without."""
+    pool = Pool(rt, [45], [fresh], H, KV, D, 16, dtype, seed=fresh + D)
+    kept = pool.fill([45 + fresh])
+    pool.set()
+    q = pool.normal(fresh, H, D)
+    tq, out = rt.from_numpy(q.reshape(fresh, -1)), rt.empty((fresh, H * D))
+    most = float(torch.finfo(pool.tdtype).max)
+    over, under = (float(np.array([b], np.uint32).view(np.float32)[0]) for b in (0x7f7f8000, 0x7f7f7fff))
+    bad = [(fresh // 3, D - 1, most), (fresh // 2, 3, -most), (fresh // 2 + 1, 4, -over), (fresh - 2, 5, over),
+           (fresh - 1, 0, under)]
+    for i, d, x in bad:
+        page, slot = pool.rows(0, 45 + i, 46 + i)
+        pool.v[0][page[0], :, slot[0], d] = x if dtype == gptc.F32 else np.copysign(most, x)
+    page, slot = pool.rows(0, 45 + fresh - 1, 45 + fresh)
+    pool.k[0][page[0], :, slot[0], 1] = most
+    torch.cuda.synchronize()
+    pool.plan.attention(0, tq, out)
+    got = rt.to_numpy(out).reshape(fresh, H, D)
+    want, bound = attention(q.astype(np.float64), kept[0], 45, H, KV, D)
+    for i in range(fresh - 1):
+        fine = [d for d in range(D) if d not in {d for j, d, _ in bad if j <= i}]
+        assert (np.abs(got[i][:, fine] - want[i][:, fine]) <= bound[i]).all(), i
+    pool.free()
+    rt.free(tq)
+    rt.free(out)
