@@ -20,7 +20,8 @@ using namespace gptc;
 struct gptc_paged_plan {
     const gptc_paged_cache_t *cache;
     int n_heads, group, max_seqs, max_tokens, max_len, max_pages;
-    int item_cap, wide_cap, merge_cap, part_cap;  // wide_cap 0: no wide items
+    int max_fresh;  // new tokens of a sequence
+    int item_cap, wide_cap, merge_cap, part_cap;  // wide_cap 0: no sequence can have wide items
     // Device memory (taken by the first set): ints [head 8 | items | wide items | merges | slot | pos | table], then
     // the parts.
     int *dev;
@@ -62,11 +63,11 @@ struct Cutting {
 
     int rounds(int keys) const { return (keys + unit - 1) / unit; }
     int cuts(int rounds) const { return rounds <= whole ? 1 : static_cast<int>((rounds + per - 1) / per); }
-    int64_t items(int n_seqs, const int *past, const int *fresh, int group, int wide_from) const {
+    int64_t items(int n_seqs, const int *past, const int *fresh, int group) const {
         int64_t n = 0;
         for (int s = 0; s < n_seqs; ++s) {
             const int rows = fresh[s] * group;
-            if ((rows >= wide_from) != wide) continue;
+            if ((rows >= kWideFrom) != wide) continue;
             for (int r = 0; r < rows; r += tile) n += cuts(rounds(tile_keys(past[s], rows, r, tile, group)));
         }
         return n;
@@ -76,8 +77,7 @@ struct Cutting {
 }  // namespace
 
 bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim,
-                          int dtype, bool wide, PagedLists &lists) {
-    const int wide_from = wide ? kWideFrom : INT32_MAX;
+                          int dtype, PagedLists &lists) {
     // The work is counted in rounds: of a workgroup's four waves, or tiles of a wide item.  A tile of rows whose keys take
     // more than `per` rounds is cut evenly, into parts of `least` rounds at least; what takes no more than `whole` stays
     // whole.  Joining costs 3 to 4 us, a round 0.5 us up to heads of 64 and 1.4 us above: one token of 32 heads of 128
@@ -90,7 +90,7 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
                        wide_least, 0, 0, 0}};
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
-        Cutting &c = cut[rows >= wide_from];
+        Cutting &c = cut[rows >= kWideFrom];
         for (int r = 0; r < rows; r += c.tile) c.total += c.rounds(tile_keys(past[s], rows, r, c.tile, group));
         c.tiles += (rows + c.tile - 1) / c.tile;
     }
@@ -107,18 +107,18 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
     } else {
         few.target = static_cast<int>(3 * tiles <= slots ? slots : 2 * slots);
         few.per = std::max(few.per, (few.total * n_kv_heads + few.target - 1) / few.target);
-        while (few.items(n_seqs, past, fresh, group, wide_from) * n_kv_heads > few.target) few.per += (few.per + 15) / 16;
+        while (few.items(n_seqs, past, fresh, group) * n_kv_heads > few.target) few.per += (few.per + 15) / 16;
     }
     // Wide ones differ too much in length for that (a prompt of 4096: 220 us became 244), but parts of less than 256 keys
     // pay only as long as every workgroup has a CU of its own: a prompt of 512 with 12 heads of 64 takes 22 us in parts of
     // 256 fp32 keys and 14 us in 240 workgroups of 64, one of 1024 26 us in 240 of 256 and 28 us in 432 of 128.
     const int wide_most = 256 / paged_wide_keys(dtype, head_dim);
-    while (cut[1].per < wide_most && cut[1].items(n_seqs, past, fresh, group, wide_from) * n_kv_heads > 256) ++cut[1].per;
+    while (cut[1].per < wide_most && cut[1].items(n_seqs, past, fresh, group) * n_kv_heads > 256) ++cut[1].per;
     lists.n_items = lists.n_wide = lists.n_merges = lists.merge_rows = 0;
     int parts = 0, tok0 = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const int rows = fresh[s] * group;
-        const bool wide = rows >= wide_from;
+        const bool wide = rows >= kWideFrom;
         const Cutting &c = cut[wide];
         const int slots = c.tile / kPagedRows;
         for (int r = 0; r < rows; r += c.tile) {
@@ -178,7 +178,7 @@ extern "C" int gptc_paged_schedule(const int n_seqs, const int *past, const int 
     l.wide = static_cast<PagedItem *>(mallocCheck(sizeof(PagedItem) * static_cast<size_t>(cap)));
     l.merges = static_cast<PagedMerge *>(mallocCheck(sizeof(PagedMerge) * static_cast<size_t>(l.merge_cap)));
     int n = -1;
-    if (paged_schedule(n_seqs, past, fresh, n_heads / n_kv_heads, n_kv_heads, head_dim, dtype, true, l) &&
+    if (paged_schedule(n_seqs, past, fresh, n_heads / n_kv_heads, n_kv_heads, head_dim, dtype, l) &&
         l.n_items + l.n_wide <= cap) {
         n = l.n_items + l.n_wide;
         for (int i = 0; i < l.n_items; ++i) l.items[i].table = 0;  // the item's kind
@@ -254,9 +254,8 @@ __global__ __launch_bounds__(256) void send_plan_kernel(const Segments s, const 
 
 }  // namespace
 
-extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *cache, const int n_heads,
-                                                     const int max_seqs, const int max_tokens, const int max_len) {
-    REQUIRE_ARG(cache);
+static gptc_paged_plan_t *make_plan(const gptc_paged_cache_t *cache, int n_heads, int max_seqs, int max_tokens, int max_len,
+                                    int max_fresh) {
     CHECK_ERROR(n_heads < 1 || n_heads > kMaxHeads || n_heads % cache->n_kv_heads != 0,
                 "Expected n_heads = %d to be a multiple of the cache's %d kv heads, up to %d.", n_heads,
                 cache->n_kv_heads, kMaxHeads);
@@ -277,16 +276,17 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     p->max_seqs = max_seqs;
     p->max_tokens = max_tokens;
     p->max_len = max_len;
+    p->max_fresh = max_fresh;
     p->max_pages = (max_len + cache->page - 1) / cache->page;
     // Every tile of rows is an item; cutting adds at most one item per `per` rounds, target / kv heads in all, and
     // cuts at most as many tiles, so it makes at most twice as many parts.
     const int64_t work = static_cast<int64_t>(max_tokens) * group, active = max_seqs < max_tokens ? max_seqs : max_tokens;
-    // Plans of single tokens have no wide items, so that a graph captured with them has no launch for those.
-    const bool wide = group >= kWideFrom || (max_tokens > max_seqs && work >= kWideFrom);
+    // Where no sequence can have the rows for wide items, a graph captured with the plan has no launch for them.
+    const bool wide = static_cast<int64_t>(max_fresh) * group >= kWideFrom;
     const int cut = kPagedTarget / cache->n_kv_heads + 1, wide_cut = wide ? kPagedWideTarget / cache->n_kv_heads + 1 : 0;
     const int wide_rows = paged_wide_rows(cache->dtype), slots = wide_rows / kPagedRows;
     p->item_cap = static_cast<int>(work / kPagedRows + active) + cut;
-    p->wide_cap = wide ? static_cast<int>(work / wide_rows + active) + wide_cut : 0;
+    p->wide_cap = wide ? static_cast<int>(work / wide_rows + std::min(active, work / kWideFrom)) + wide_cut : 0;
     p->merge_cap = cut + slots * wide_cut;
     p->part_cap = 2 * p->merge_cap;
     // A launch has fewer than 2^32 threads: 256 for each item and kv head, up to 512 for wide ones.
@@ -304,6 +304,18 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *c
     memset(p->writer, 0, sizeof(long long) * n_pages);
     p->table_at = static_cast<int *>(mallocCheck(sizeof(int) * static_cast<size_t>(max_seqs)));
     return p;
+}
+
+extern "C" gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *cache, const int n_heads,
+                                                     const int max_seqs, const int max_tokens, const int max_len) {
+    REQUIRE_ARG(cache);
+    return make_plan(cache, n_heads, max_seqs, max_tokens, max_len, std::min(max_tokens, max_len));
+}
+
+extern "C" gptc_paged_plan_t *gptc_paged_plan_create_single(const gptc_paged_cache_t *cache, const int n_heads,
+                                                            const int max_seqs, const int max_len) {
+    REQUIRE_ARG(cache);
+    return make_plan(cache, n_heads, max_seqs, max_seqs, max_len, 1);
 }
 
 extern "C" void gptc_paged_plan_free(gptc_paged_plan_t *plan) {
@@ -343,6 +355,8 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
                     static_cast<long long>(len), plan->max_len);
         CHECK_ERROR((len + c->page - 1) / c->page > stride, "Sequence %d needs %lld pages, but the table has %d.", s,
                     static_cast<long long>((len + c->page - 1) / c->page), stride);
+        CHECK_ERROR(fresh[s] > plan->max_fresh, "Sequence %d has %d new tokens: the plan was made for %d.", s, fresh[s],
+                    plan->max_fresh);
         tokens += fresh[s];
     }
     CHECK_ERROR(tokens > plan->max_tokens, "The plan has room for %d new tokens, but got %lld.", plan->max_tokens,
@@ -392,7 +406,7 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
     lists.wide_cap = plan->wide_cap;
     lists.merge_cap = plan->merge_cap;
     lists.part_cap = plan->part_cap;
-    const bool fits = paged_schedule(n_seqs, past, fresh, plan->group, c->n_kv_heads, c->head_dim, c->dtype, plan->wide_cap > 0, lists);
+    const bool fits = paged_schedule(n_seqs, past, fresh, plan->group, c->n_kv_heads, c->head_dim, c->dtype, lists);
     CHECK_ERROR(!fits, "The work of %d sequences does not fit the plan.", n_seqs);
     int t = 0, at = 0;
     for (int s = 0; s < n_seqs; ++s) {

@@ -53,9 +53,8 @@ struct PagedLists {
 };
 
 // Fills the lists for a step (an item's table receives its sequence); false when one of them does not fit.
-// `wide` is false where wide items are not to be used.
 bool paged_schedule(int n_seqs, const int *past, const int *fresh, int group, int n_kv_heads, int head_dim, int dtype,
-                    bool wide, PagedLists &lists);
+                    PagedLists &lists);
 
 // What the attention kernels take.
 struct PagedAttnParams {

@@ -221,6 +221,7 @@ SIGNATURES = {
     "gptc_paged_cache_create": (_vp, [_ci, _ci, _ci, _ci, _ci, _ci, ctypes.POINTER(_vp), ctypes.POINTER(_vp)]),
     "gptc_paged_cache_free": (None, [_vp]),
     "gptc_paged_plan_create": (_vp, [_vp, _ci, _ci, _ci, _ci]),
+    "gptc_paged_plan_create_single": (_vp, [_vp, _ci, _ci, _ci]),
     "gptc_paged_plan_set": (None, [_vp, _ci, _ip, _ip, _ip, _ci]),
     "gptc_paged_plan_free": (None, [_vp]),
     "gptc_rotary_table": (TensorP, [_ci, _ci, ctypes.c_double]),
@@ -634,6 +635,14 @@ class PagedPlan:
     def __init__(self, rt, cache, n_heads, max_seqs, max_tokens, max_len):
         self.rt, self.cache = rt, cache
         self.raw = ctypes.c_void_p(rt.lib.gptc_paged_plan_create(cache.raw, n_heads, max_seqs, max_tokens, max_len))
+
+    @classmethod
+    def single(cls, rt, cache, n_heads, max_seqs, max_len):
+        """gptc_paged_plan_create_single: for steps of single tokens only."""
+        plan = cls.__new__(cls)
+        plan.rt, plan.cache = rt, cache
+        plan.raw = ctypes.c_void_p(rt.lib.gptc_paged_plan_create_single(cache.raw, n_heads, max_seqs, max_len))
+        return plan
 
     def set(self, past, fresh, table):
         """past, fresh: tokens of each sequence before the step and new in it; table: (sequences, pages) page numbers."""

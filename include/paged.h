@@ -64,6 +64,11 @@ void gptc_paged_cache_free(gptc_paged_cache_t *cache);
  *   h / (n_heads / n_kv_heads).  Its device memory is taken by the first
  *   gptc_paged_plan_set and never moves; the cache has to outlive the plan, and
  *   the plan the graphs captured with it.
+ * gptc_paged_plan_create_single(cache, n_heads, max_seqs, max_len)
+ *   For steps in which no sequence brings more than one token (others are
+ *   refused).  Captured launches cover what a plan can hold: up to 63 query heads
+ *   per kv head this one has no workspace for prompts, and graphs captured with it
+ *   no launch for them.  A step's results are the same under every plan.
  * gptc_paged_plan_set(plan, n_seqs, past, fresh, table, stride)
  *   All arrays are host memory, read before the call returns.  Sequence s has
  *   past[s] >= 0 tokens in its pages and brings fresh[s] >= 0 new ones; its
@@ -83,6 +88,8 @@ typedef struct gptc_paged_plan gptc_paged_plan_t;
 
 gptc_paged_plan_t *gptc_paged_plan_create(const gptc_paged_cache_t *cache, const int n_heads, const int max_seqs,
                                           const int max_tokens, const int max_len);
+gptc_paged_plan_t *gptc_paged_plan_create_single(const gptc_paged_cache_t *cache, const int n_heads, const int max_seqs,
+                                                 const int max_len);
 void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, const int *past, const int *fresh,
                          const int *table, const int stride);
 void gptc_paged_plan_free(gptc_paged_plan_t *plan);

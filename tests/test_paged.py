@@ -204,3 +204,26 @@ def test_sampling_refused(name):
     """ + "\n        " + call)
     assert r.returncode == 1 and "survived" not in r.stdout, r.stderr
     assert message in r.stderr, r.stderr
+
+
+SINGLE_REFUSALS = {
+    "two tokens of one": ("single().set([0, 4], [1, 2], [[0], [1]])", "Sequence 1 has 2 new tokens: the plan was made for 1"),
+    "heads no multiple": ("single(heads=3)", "multiple of the cache's 2 kv heads"),
+    "too many sequences": ("single().set([0] * 4, [1] * 4, [[0], [1], [2], [3]])", "room for 3 sequences"),
+    "too long": ("single().set([64], [1], [[0, 1, 2, 3, 4]])", "grows to 65 tokens"),
+    "single tokens pass, set without a runtime": ("single().set([0, 63, 5], [1, 1, 0], [[0, 0, 0, 0], [1, 2, 3, 4], [5, 0, 0, 0]])",
+                                                  "runtime_init"),
+    "a general plan of as many tokens as sequences takes prompts": (
+        "plan(seqs=40, tokens=40).set([0, 4], [33, 2], [[0, 1, 2], [3, 0, 0]])", "runtime_init"),
+}
+
+
+@pytest.mark.parametrize("name", sorted(SINGLE_REFUSALS))
+def test_plans_of_single_tokens_refuse_others(name):
+    call, message = SINGLE_REFUSALS[name]
+    r = run_c("""
+        def single(heads=4, seqs=3, length=64):
+            return gptc.PagedPlan.single(rt, cache(), heads, seqs, length)
+    """ + "\n        " + call)
+    assert r.returncode == 1 and "survived" not in r.stdout, r.stderr
+    assert message in r.stderr, r.stderr

@@ -345,3 +345,72 @@ def test_pool_past_32_bits(rt, dtype, page):
     rt.free(out)
     plan.free()
     cache.free()
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("past, fresh, seqs, tokens", [([40, 3], [90, 9], 100, 100), ([2000, 0], [70, 30], 128, 100),
+                                                       ([0], [64], 64, 64), ([700, 5, 90], [1, 1, 1], 3, 3)])
+def test_every_plan_gives_a_step_the_same_results(rt, dtype, past, fresh, seqs, tokens):
+    """A prompt is cut the same way under a plan of no more tokens than sequences as under one with room for more."""
+    H, KV, D = 6, 3, 64
+    pool = Pool(rt, past, fresh, H, KV, D, 32, dtype, seed=9, max_len=2100)
+    pool.fill([p + f for p, f in zip(past, fresh)])
+    N = sum(fresh)
+    tq, got = rt.from_numpy(pool.normal(N, H * D)), []
+    plans = [gptc.PagedPlan(rt, pool.cache, H, seqs, n, 2100) for n in (tokens, 4096)]
+    if max(fresh) == 1:
+        plans.append(gptc.PagedPlan.single(rt, pool.cache, H, seqs, 2100))
+    for plan in plans:
+        out = rt.empty((N, H * D))
+        plan.set(past, fresh, pool.table)
+        plan.attention(0, tq, out)
+        got.append(rt.to_numpy(out))
+        rt.free(out)
+        plan.free()
+    for y in got[1:]:
+        assert np.array_equal(y, got[0])
+    pool.free()
+    rt.free(tq)
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("H, KV", [(4, 2), (64, 1)], ids=["group2", "group64"])
+def test_captured_single_tokens_follow_their_plan(rt, dtype, H, KV):
+    """A graph under a plan of single tokens: sequences that come, go, wait and grow, cut and uncut; 64 heads on one kv
+    head are rows of a wide item each.  Each replay is the eager call of a general plan bit for bit."""
+    D, page, n = 64, 16, 4
+    pool = Pool(rt, [3000, 700, 40, 17], [1] * n, H, KV, D, page, dtype, seed=5, max_len=3200)
+    pool.fill([3001, 701, 41, 18])
+    plan = gptc.PagedPlan.single(rt, pool.cache, H, n, 3200)
+    x = torch.tensor(pool.normal(n, (H + 2 * KV) * D)).cuda()
+    table = rt.lib.gptc_rotary_table(3200, D, 10000.0)
+    q, out = (torch.zeros(n, H * D, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    tx, tq, tout = (as_tensor(rt, v) for v in (x, q, out))
+
+    def step(p):
+        p.append(0, tx, table, False, tq)
+        p.attention(0, tq, tout)
+
+    plan.set([5, 0, 0, 0], [1, 0, 0, 0], pool.table)
+    step(plan)
+    graph = Graph(rt, lambda: step(plan))
+    steps = [([3000, 700, 40, 17], [1, 1, 1, 1]), ([0, 0, 0, 0], [1, 1, 0, 1]), ([2999, 16, 15, 0], [0, 1, 1, 1]),
+             ([0, 0, 0, 0], [0, 0, 0, 0]), ([3000, 1, 1, 1], [1, 0, 0, 0])]
+    for past, fresh in steps * 2:
+        rows = sum(fresh)
+        got = []
+        for p, run in ((plan, graph.replay), (pool.plan, lambda: step(pool.plan))):
+            q.fill_(7.5)
+            out.fill_(7.5)
+            torch.cuda.synchronize()
+            p.set(past, fresh, pool.table)
+            run()
+            rt.sync()
+            got.append((q.clone(), out.clone()))
+        for a, b in zip(*got):
+            assert torch.equal(a, b) and (a[rows:] == 7.5).all() and (rows == 0 or not (a[:rows] == 7.5).any())
+    graph.free()
+    plan.free()
+    pool.free()
+    rt.free(table)
