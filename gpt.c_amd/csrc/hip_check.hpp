@@ -20,6 +20,9 @@ inline void hip_check(hipError_t err, const char *file, int line) {
 // (fatal if runtime_init_cuda() has not run).
 hipStream_t gptc_stream_checked();
 
+// Whether there is one: device memory that is still held when the runtime is destroyed is not given back.
+bool gptc_runtime_up();
+
 // Whether that stream is being captured into a graph.  A graph's replays use the pool's blocks
 // that its launches took for scratch after those have gone to someone else: entry points that
 // can do without scratch do so under capture.

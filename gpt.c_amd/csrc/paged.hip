@@ -11,6 +11,8 @@
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
+#include <mutex>
+#include <utility>
 #include "gpu_kernels.h"
 #include "ops_common.hpp"
 #include "paged_plan.hpp"
@@ -37,6 +39,7 @@ struct gptc_paged_plan {
     // Who writes each page in this step: checked without clearing the array between steps.
     long long *writer;  // step * max_seqs + sequence
     long long step;
+    gptc_paged_plan *next_freed;
 };
 
 namespace {
@@ -228,7 +231,7 @@ extern "C" gptc_paged_cache_t *gptc_paged_cache_create(const int n_layers, const
 
 extern "C" void gptc_paged_cache_free(gptc_paged_cache_t *cache) {
     if (cache == NULL) return;
-    for (int l = 0; cache->owned && l < cache->n_layers; ++l) {
+    for (int l = 0; cache->owned && gptc_runtime_up() && l < cache->n_layers; ++l) {
         free_cuda(cache->k[l]);
         free_cuda(cache->v[l]);
     }
@@ -254,8 +257,46 @@ __global__ __launch_bounds__(256) void send_plan_kernel(const Segments s, const 
 
 }  // namespace
 
+// Plans that were freed while the stream was being captured.  They go with the next call that makes, sets or frees a
+// plan when it is not.
+static std::mutex g_freed_mu;
+static gptc_paged_plan_t *g_freed = nullptr;
+
+static void release_plan(gptc_paged_plan_t *plan) {
+    if (plan->dev != nullptr) {
+        if (gptc_runtime_up()) {
+            free_cuda(plan->dev);
+            free_cuda(plan->part_o);
+            free_cuda(plan->part_ml);
+        }
+        for (int i = 0; i < 2; ++i) {
+            hipCheck(hipEventSynchronize(plan->copied[i]));  // its last copy may still read the host memory
+            hipCheck(hipEventDestroy(plan->copied[i]));
+            hipCheck(hipHostFree(plan->host[i]));
+        }
+    }
+    free(plan->writer);
+    free(plan->table_at);
+    free(plan);
+}
+
+static void release_freed() {
+    gptc_paged_plan_t *plan = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(g_freed_mu);
+        if (g_freed == nullptr || (gptc_runtime_up() && gptc_stream_capturing())) return;
+        std::swap(plan, g_freed);
+    }
+    while (plan != nullptr) {
+        gptc_paged_plan_t *next = plan->next_freed;
+        release_plan(plan);
+        plan = next;
+    }
+}
+
 static gptc_paged_plan_t *make_plan(const gptc_paged_cache_t *cache, int n_heads, int max_seqs, int max_tokens, int max_len,
                                     int max_fresh) {
+    release_freed();
     CHECK_ERROR(n_heads < 1 || n_heads > kMaxHeads || n_heads % cache->n_kv_heads != 0,
                 "Expected n_heads = %d to be a multiple of the cache's %d kv heads, up to %d.", n_heads,
                 cache->n_kv_heads, kMaxHeads);
@@ -320,20 +361,14 @@ extern "C" gptc_paged_plan_t *gptc_paged_plan_create_single(const gptc_paged_cac
 
 extern "C" void gptc_paged_plan_free(gptc_paged_plan_t *plan) {
     if (plan == NULL) return;
-    if (plan->dev != nullptr) {
-        CHECK_ERROR(gptc_stream_capturing(), "A plan cannot be freed while the stream is being captured.");
-        free_cuda(plan->dev);
-        free_cuda(plan->part_o);
-        free_cuda(plan->part_ml);
-        for (int i = 0; i < 2; ++i) {
-            hipCheck(hipEventSynchronize(plan->copied[i]));  // its last copy may still read the host memory
-            hipCheck(hipEventDestroy(plan->copied[i]));
-            hipCheck(hipHostFree(plan->host[i]));
-        }
+    if (plan->dev != nullptr && gptc_runtime_up() && gptc_stream_capturing()) {
+        std::lock_guard<std::mutex> lock(g_freed_mu);
+        plan->next_freed = g_freed;
+        g_freed = plan;
+        return;
     }
-    free(plan->writer);
-    free(plan->table_at);
-    free(plan);
+    release_plan(plan);
+    release_freed();
 }
 
 extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, const int *past, const int *fresh,
@@ -385,6 +420,7 @@ extern "C" void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, c
 
     hipStream_t stream = gptc_stream_checked();
     CHECK_ERROR(gptc_stream_capturing(), "A plan cannot be set while the stream is being captured.");
+    release_freed();
     if (plan->dev == nullptr) {
         plan->dev = static_cast<int *>(alloc_cuda(sizeof(int) * plan->ints));
         plan->part_o = static_cast<float *>(alloc_cuda(sizeof(float) * part_slots(plan) * kPagedRows * c->head_dim));

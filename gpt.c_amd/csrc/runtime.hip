@@ -78,6 +78,8 @@ hipStream_t gptc_stream_checked() {
     return g_stream;
 }
 
+bool gptc_runtime_up() { return g_ready; }
+
 bool gptc_stream_capturing() {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     hipCheck(hipStreamIsCapturing(gptc_stream_checked(), &st));

@@ -10,6 +10,7 @@ loudly when the library has not been built.
 import ctypes
 import os
 import subprocess
+import sys
 
 import numpy as np
 
@@ -612,6 +613,8 @@ class PagedCacheT(ctypes.Structure):
 class PagedCache:
     """gptc_paged_cache_create: keys and values in pages.  k, v: device addresses of the layers' blocks, or None."""
 
+    raw = None
+
     def __init__(self, rt, n_layers, n_pages, page, n_kv_heads, head_dim, dtype=F32, k=None, v=None):
         def addresses(x):
             return None if x is None else (_vp * n_layers)(*x)
@@ -626,11 +629,15 @@ class PagedCache:
             self.raw = None
 
     def __del__(self):
-        self.free()
+        if not sys.is_finalizing():  # then the memory goes with the process
+            self.free()
 
 
 class PagedPlan:
-    """gptc_paged_plan_create: what one step does, shared by its layers."""
+    """gptc_paged_plan_create: what one step does, shared by its layers.  It has to be kept as long as graphs captured
+    with it are launched."""
+
+    raw = None
 
     def __init__(self, rt, cache, n_heads, max_seqs, max_tokens, max_len):
         self.rt, self.cache = rt, cache
@@ -665,4 +672,5 @@ class PagedPlan:
             self.raw = None
 
     def __del__(self):
-        self.free()
+        if not sys.is_finalizing():  # then the memory goes with the process
+            self.free()

@@ -92,7 +92,7 @@ gptc_paged_plan_t *gptc_paged_plan_create_single(const gptc_paged_cache_t *cache
                                                  const int max_len);
 void gptc_paged_plan_set(gptc_paged_plan_t *plan, const int n_seqs, const int *past, const int *fresh,
                          const int *table, const int stride);
-void gptc_paged_plan_free(gptc_paged_plan_t *plan);
+void gptc_paged_plan_free(gptc_paged_plan_t *plan);  // during a capture: done by the first plan call after it
 
 /*
  * gptc_rotary_table(rows, rot, theta)

@@ -227,3 +227,18 @@ def test_plans_of_single_tokens_refuse_others(name):
     """ + "\n        " + call)
     assert r.returncode == 1 and "survived" not in r.stdout, r.stderr
     assert message in r.stderr, r.stderr
+
+
+def test_a_cache_that_could_not_be_made_ends_quietly():
+    r = run_c("""
+        try:
+            gptc.PagedCache(rt, 1, 8, 16, 2, 4, gptc.F32, [4096, 8192], [4096, 8192])
+        except IndexError:
+            pass
+        try:
+            gptc.PagedPlan(rt, None, 2, 1, 1, 16)
+        except AttributeError:
+            pass
+        plan(), cache()
+    """)
+    assert r.returncode == 0 and "survived" in r.stdout and r.stderr == "", r.stderr

@@ -2,6 +2,10 @@
 generate side by side; steps in captured graphs; several plans over one pool; a pool past 32 bits of offsets.
 """
 import ctypes
+import os
+import subprocess
+import sys
+import textwrap
 
 import numpy as np
 import pytest
@@ -15,6 +19,8 @@ from test_paged_gpu import Pool, attention, check_attention
 from test_sample_gpu import SETTINGS, draw, language
 
 pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 class Server:
@@ -414,3 +420,58 @@ def test_captured_single_tokens_follow_their_plan(rt, dtype, H, KV):
     plan.free()
     pool.free()
     rt.free(table)
+
+
+def test_plans_dropped_during_a_capture(rt):
+    """Their memory goes back to the library once the capture is over; the graph and other plans are as they were."""
+    pool = Pool(rt, [500], [3], 8, 8, 128, 64, gptc.F32, seed=1)
+    kept = pool.fill([503])
+    q = pool.normal(3, 8, 128)
+    tq, out = rt.from_numpy(q.reshape(3, -1)), rt.empty((3, 1024))
+    pool.set()
+    pool.plan.attention(0, tq, out)
+    free = None
+    for i in range(20):
+        held = [gptc.PagedPlan(rt, pool.cache, 8, 64, 4096, 1024) for _ in range(2)]  # 85 MB each
+        for plan in held:
+            plan.set(pool.past, pool.fresh, pool.table)
+            plan.attention(0, tq, out)
+
+        def call():
+            held.pop().free()
+            held.clear()  # the finalizer
+            pool.plan.attention(0, tq, out)
+
+        graph = Graph(rt, call)
+        for _ in range(2):
+            rt.lib.fill_tensor_data_cuda(out, ctypes.c_float(7.0))
+            graph.replay()
+            check_attention(pool, kept, q, rt.to_numpy(out))
+            pool.set()
+        graph.free()
+        rt.sync()
+        if i == 1:
+            free = torch.cuda.mem_get_info()[0]
+    assert free - torch.cuda.mem_get_info()[0] < 2 ** 28
+    pool.free()
+    rt.free(tq)
+    rt.free(out)
+
+
+def test_plans_and_caches_that_outlive_the_runtime(rt):
+    code = textwrap.dedent(f"""
+        import sys
+        sys.path.insert(0, {os.path.join(ROOT, 'gpt.c_amd')!r})
+        import gptc
+        rt = gptc.Runtime(gptc.load())
+        rt.init()
+        left = [gptc.PagedCache(rt, 1, 8, 16, 2, 64) for _ in range(2)]
+        left += [gptc.PagedPlan(rt, c, 2, 1, 40, 64) for c in left]
+        for plan in left[2:]:
+            plan.set([0], [1], [[3]])
+        rt.lib.runtime_destroy(gptc.CUDA)
+        left[0] = left[2] = None
+        print("survived")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "survived" in r.stdout and "ERROR" not in r.stderr, r.stderr
