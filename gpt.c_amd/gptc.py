@@ -633,6 +633,16 @@ class PagedCache:
             self.free()
 
 
+def _int32(x, name):
+    """A C-contiguous int32 array of x, whose values have to fit."""
+    x = np.asarray(x)
+    with np.errstate(invalid="ignore"):
+        y = np.ascontiguousarray(x, np.int32)
+    if x.dtype != np.int32 and not np.array_equal(x, y):
+        raise ValueError(f"expected {name} to hold 32-bit whole numbers")
+    return y
+
+
 class PagedPlan:
     """gptc_paged_plan_create: what one step does, shared by its layers.  It has to be kept as long as graphs captured
     with it are launched."""
@@ -653,8 +663,7 @@ class PagedPlan:
 
     def set(self, past, fresh, table):
         """past, fresh: tokens of each sequence before the step and new in it; table: (sequences, pages) page numbers."""
-        past, fresh = (np.ascontiguousarray(x, np.int32) for x in (past, fresh))
-        table = np.ascontiguousarray(table, np.int32)
+        past, fresh, table = _int32(past, "past"), _int32(fresh, "fresh"), _int32(table, "table")
         if past.ndim != 1 or past.shape != fresh.shape or table.ndim != 2 or len(table) != len(past):
             raise ValueError(f"expected (n,), (n,) and (n, pages), but got {past.shape}, {fresh.shape}, {table.shape}")
         self.rt.lib.gptc_paged_plan_set(self.raw, len(past), past.ctypes.data_as(_ip), fresh.ctypes.data_as(_ip),

@@ -242,3 +242,25 @@ def test_a_cache_that_could_not_be_made_ends_quietly():
         plan(), cache()
     """)
     assert r.returncode == 0 and "survived" in r.stdout and r.stderr == "", r.stderr
+
+
+@pytest.mark.parametrize("call", [
+    "set(np.array([2**32 + 5]), [1], [[0]])", "set([5], np.array([1 - 2**32]), [[0]])", "set([0], [1], np.array([[2**32]]))",
+    "set([0], [1], np.array([[2**63]], np.uint64))", "set([0.5], [1], [[0]])", "set([0], [1], [[float('nan')]])",
+    "set([[0]], [1], [[0]])", "set([0], [1], [[0], [1]])"])
+def test_plans_take_32_bit_whole_numbers(call):
+    """Nothing is cut to 32 bits on its way to the checks of the library."""
+    r = run_c(f"""
+        try:
+            plan().{call}
+        except ValueError as e:
+            print("refused", e)
+    """)
+    assert r.returncode == 0 and "refused" in r.stdout, r.stderr
+
+
+def test_plans_take_whole_numbers_of_other_types():
+    r = run_c("plan().set(np.array([5, 0], np.int64), np.array([1.0, 2.0]), np.array([[5, 0], [6, 0]], np.uint8))")
+    assert r.returncode == 1 and "runtime_init" in r.stderr, r.stderr
+    r = run_c("plan().set([], [], np.zeros((0, 1)))")
+    assert r.returncode == 1 and "runtime_init" in r.stderr, r.stderr
