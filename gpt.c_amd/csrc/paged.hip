@@ -98,11 +98,12 @@ bool gptc::paged_schedule(int n_seqs, const int *past, const int *fresh, int gro
         c.tiles += (rows + c.tile - 1) / c.tile;
     }
     for (Cutting &c : cut) c.per = std::max<int64_t>(c.least, (c.total * n_kv_heads + c.target - 1) / c.target);
-    // Single tokens, or few.  `slots` workgroups run at once, two on a CU up to heads of 64 (224 registers) and one above;
-    // the work is done soonest when all of them get the same, and a few too many would run alone.  So there are as many
-    // as that where the tiles can be cut in three, twice as many where they cannot, and where there are more tiles than
-    // that, only the longest are cut.  Heads of 128, fp32: 8 contexts of 3200 of 8 kv heads 45 us in 256 and 48 in 512
-    // workgroups (59 us in 1024), 32 of 1700 107 and 92 us, 64 of 900 90 us whole, 104 us where every one was cut in two.
+    // Single tokens, or few.  `slots` workgroups run at once, two on a CU up to heads of 64 (the kernel's launch bounds
+    // see to it) and one above; the work is done soonest when all of them get the same, and a few too many would run
+    // alone.  So there are as many as that where the tiles can be cut in three, twice as many where they cannot, and where
+    // there are more tiles than that, only the longest are cut.  Heads of 128, fp32: 8 contexts of 3200 of 8 kv heads 45 us
+    // in 256 and 48 in 512 workgroups (59 us in 1024), 32 of 1700 107 and 92 us, 64 of 900 90 us whole, 104 us where every
+    // one was cut in two.
     Cutting &few = cut[0];
     const int64_t slots = small ? 512 : 256, tiles = few.tiles * n_kv_heads;
     if (tiles >= 2 * slots) {

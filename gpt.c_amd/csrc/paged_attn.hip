@@ -292,8 +292,10 @@ struct Dots {
     }
 };
 
+// Up to heads of 64 two workgroups share a CU, which the plan counts on: without the bound the kernel for bf16 rows that are
+// no whole vectors took 260 registers and ran alone (12 heads of 60, 64 contexts of 2000: 163 us, with it 149 us).
 template <typename T, int DP, Rows R>
-__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedAttnParams a) {
+__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void paged_attn_kernel(const PagedAttnParams a) {
     using Step = Tile<T, DP, R>;
     constexpr int kKeys = 16 * Step::kGroups;
     static_assert(kPagedWideTarget <= kPagedTarget, "kMaxParts");

@@ -67,10 +67,11 @@ __device__ __forceinline__ f32x4 mfma_bf16(const uint32_t (&a)[4], const uint32_
                                                    0);
 }
 
-// A matrix instruction's result may be read 11 cycles after it at the earliest.  The compiler counts them inside
-// a block; across a branch it was seen to read the last two registers at once (wrong sums at every second step of
-// bf16 pages).  So results are taken over in the block of the product (settled), or after a wait (drain) that nothing
-// is moved across.
+// A matrix instruction's result may be touched 8 instruction slots after it at the earliest (16x16x32 bf16), or 10
+// (16x16x4 fp32), and the hardware does not wait.  The compiler counts them inside a block; across a branch it was seen
+// to read the last two registers at once (wrong sums at every second step of bf16 pages), and a slot too soon where a
+// branch was turned round after the count.  So results are taken over in the block of the product (settled), or after
+// a wait (drain) that nothing is moved across; tests/test_kernel_code.py looks at every path of the built kernels.
 __device__ __forceinline__ void settled(f32x4 &x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void drain() {
     __builtin_amdgcn_sched_barrier(0);
