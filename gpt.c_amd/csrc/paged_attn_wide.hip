@@ -359,7 +359,8 @@ void launch_paged_wide(const PagedAttnParams &p, hipStream_t s) {
     // Groups of 16 rows to a wave, fp32 pages.  With two a workgroup has half the waves, and two of them fit a CU: worth
     // it from one and a half per CU on.  12 heads of 64, a prompt of 4096: 239 us with one group and 219 with two; of
     // 1024 (240 workgroups): 24 and 29 us.  Heads of 128, 64 tokens each of 8 sequences over 2000: 82 and 76 us; a
-    // prompt of 1024 with 12 heads: 42 and 52 us.  Both give the same sums.
+    // prompt of 1024 with 12 heads: 42 and 52 us.  Both give the same sums.  With two, heads past 96 spill 8 registers a
+    // lane (21 where rows are no whole vectors), which these figures include.
     const bool two = static_cast<int64_t>(p.n_wide) * p.KV >= 384;
     // Tiles of 64, 96 and 128 values of a head: what pads a head is multiplied too.  Heads of 80 as 128, fp32 and bf16
     // pages: a prompt of 4096 with 12 heads 383 and 217 us, as 96 294 and 191 us.

@@ -22,7 +22,8 @@
 //           logits only, whose order is that of the vocabulary.  The kept tokens are gathered where they are few, and
 //           the draw finds the stretch of the vocabulary where the sum is passed, and the token in it.
 // The weights bind it, eleven 64-bit operations each, and then the adds to the histogram.  Logits held in registers
-// between the passes (49152 of a row at 512 threads) spilled and came out 1.1 to 1.3 times as slow.
+// between the passes (49152 of a row at 512 threads) spilled more and came out 1.1 to 1.3 times as slow; as it is the
+// kernel fills the 128 registers that 1024 threads leave each, and spills 11 (44 bytes a lane) outside its inner loops.
 //
 // MI355X, rows of 50257 logits: greedy 6 us, top-k 40 15 us, min-p 14 us, no filter 23 us, top-p 37 to 50 us, for one row
 // as for 64.  256 rows of 131072 (134 MB): greedy 26 us (5.2 TB/s), top-k 54 us, top-p 97 to 142 us (three to four

@@ -83,6 +83,10 @@ void gptc_paged_cache_free(gptc_paged_cache_t *cache);
  * launched on streams of the caller's) need a plan each.  A captured graph
  * reads the plan as it is when the graph runs: after another plan_set the same
  * graph serves the new step, as long as its tensors have the rows for it.
+ * plan_set returns when its arrays have been read; the plan's device memory is
+ * written by work queued on gptc_stream().  A graph launched on another stream
+ * has to wait for an event recorded on gptc_stream() after plan_set, and
+ * gptc_stream() for one recorded behind the graph before the next plan_set.
  */
 typedef struct gptc_paged_plan gptc_paged_plan_t;
 

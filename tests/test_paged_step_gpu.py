@@ -475,3 +475,43 @@ def test_plans_and_caches_that_outlive_the_runtime(rt):
     """)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "survived" in r.stdout and "ERROR" not in r.stderr, r.stderr
+
+
+@pytest.mark.parametrize("dtype", [gptc.F32, gptc.BF16], ids=["f32", "bf16"])
+def test_a_graph_on_another_stream(rt, dtype):
+    """Events order it behind its plan_set, and the next plan_set behind it: several steps without waiting on the host."""
+    H, KV, D = 4, 2, 64
+    pool = Pool(rt, [900, 500, 30], [1, 70, 1], H, KV, D, 32, dtype, seed=6, max_len=1000, room=40)
+    kept = pool.fill([901, 570, 31])
+    q = pool.normal(72, H, D)
+    tq = rt.from_numpy(q.reshape(72, -1))
+    steps = [([900, 500, 30], [1, 70, 1]), ([3, 0, 2], [1, 0, 1]), ([880, 520, 0], [20, 50, 2]), ([0, 0, 7], [0, 0, 1])]
+    outs, graphs = [torch.full((72, H * D), 7.5, device="cuda") for _ in steps], []
+    torch.cuda.synchronize()
+    pool.set()
+    for out in outs:
+        call = lambda: pool.plan.attention(0, tq, as_tensor(rt, out))  # noqa: E731
+        call()
+        graphs.append(Graph(rt, call))
+        rt.sync()
+    mine, other = torch.cuda.ExternalStream(rt.stream()), torch.cuda.Stream()
+    for out in outs:
+        out.fill_(7.5)
+    torch.cuda.synchronize()
+    for (past, fresh), graph in zip(steps, graphs):
+        pool.plan.set(past, fresh, pool.table)
+        other.wait_event(mine.record_event())
+        assert graph.hip.hipGraphLaunch(graph.exec, ctypes.c_void_p(other.cuda_stream)) == 0
+        mine.wait_event(other.record_event())
+    torch.cuda.synchronize()
+    for (past, fresh), out, graph in zip(steps, outs, graphs):
+        got, row = out.cpu().numpy(), 0
+        for s, (p, f) in enumerate(zip(past, fresh)):
+            kv = tuple(x[:p + f] for x in kept[s])
+            want, bound = attention(q[row:row + f].astype(np.float64), kv, p, H, KV, D)
+            assert (np.abs(got[row:row + f].reshape(f, H, D) - want) <= bound).all()
+            row += f
+        assert (got[row:] == 7.5).all()
+        graph.free()
+    pool.free()
+    rt.free(tq)
