@@ -628,8 +628,8 @@ class PagedCache:
             self.rt.lib.gptc_paged_cache_free(self.raw)
             self.raw = None
 
-    def __del__(self):
-        if not sys.is_finalizing():  # then the memory goes with the process
+    def __del__(self, ending=sys.is_finalizing):
+        if not ending():  # then the memory goes with the process
             self.free()
 
 
@@ -680,6 +680,6 @@ class PagedPlan:
             self.rt.lib.gptc_paged_plan_free(self.raw)
             self.raw = None
 
-    def __del__(self):
-        if not sys.is_finalizing():  # then the memory goes with the process
+    def __del__(self, ending=sys.is_finalizing):
+        if not ending():  # then the memory goes with the process
             self.free()

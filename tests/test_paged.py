@@ -264,3 +264,14 @@ def test_plans_take_whole_numbers_of_other_types():
     assert r.returncode == 1 and "runtime_init" in r.stderr, r.stderr
     r = run_c("plan().set([], [], np.zeros((0, 1)))")
     assert r.returncode == 1 and "runtime_init" in r.stderr, r.stderr
+
+
+@pytest.mark.parametrize("main_stays", [False, True])
+def test_plans_left_to_the_interpreter_end_quietly(main_stays):
+    """Also where the names of the gptc module go before them, as where an extension holds on to the main module."""
+    r = run_c(f"""
+        kept = plan(), cache()
+        if {main_stays}:
+            ctypes.pythonapi.Py_IncRef(ctypes.py_object(sys.modules["__main__"]))
+    """)
+    assert r.returncode == 0 and "survived" in r.stdout and r.stderr == "", r.stderr
