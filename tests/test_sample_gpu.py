@@ -216,3 +216,29 @@ def test_the_largest_vocabulary(rt):
     x = rng.standard_normal((3, 1 << 24)).astype(np.float32)
     x[:, -1] = x.max() + 1
     check(rt, x, [SETTINGS["top_k"], SETTINGS["top_p"], SETTINGS["plain"]], [0.3, 0.97, 1 - 2.0 ** -24])
+
+
+def test_sampled_generation_over_a_contiguous_cache(rt):
+    """gptc_gpt2_decode's logits go to the draw as they are, and the drawn ids to the next step, without a copy between."""
+    from test_generate_gpu import c3_params, make_model
+    V, block, L, H, C, B, steps = 523, 64, 2, 4, 64, 3, 24
+    model = make_model(rt, c3_params(V, block, L, C, 5, std=0.2, jitter=0.05), V, block, L, H, C)
+    cache, rng = gptc.KVCache(rt, model, B, block), np.random.default_rng(5)
+    settings = np.array([SETTINGS[n] for n in ("top_k", "top_p", "all")], np.float32)
+    coins = rng.random((steps, B)).astype(np.float32)
+    params, u = rt.from_numpy(settings), [rt.from_numpy(c) for c in coins]
+    ids = rt.from_numpy(rng.integers(0, V, (B, 1)).astype(np.float32))
+    kept = []
+    for pos in range(steps):
+        logits, drawn = cache.decode(ids, pos), rt.empty((B, 1))
+        rt.lib.gptc_sample_cuda(logits, params, u[pos], ids, None)
+        rt.lib.tensor_copy(drawn, ids)
+        kept.append((logits, drawn))
+    for (logits, drawn), coin in zip(kept, coins):
+        want, _ = draw(rt.to_numpy(logits)[:, 0], settings.astype(np.float64), coin.astype(np.float64))
+        assert np.array_equal(rt.to_numpy(drawn)[:, 0], want)
+    assert len({tuple(rt.to_numpy(d)[:, 0]) for _, d in kept}) > steps // 2
+    for t in [params, ids, *u, *(t for pair in kept for t in pair)]:
+        rt.free(t)
+    cache.free()
+    model.free()
