@@ -14,8 +14,8 @@
 //     order in which the scores' product leaves them with the lanes: place 8 g + j holds key 16 (j / 4) + 4 g + j % 4,
 //     so a lane reads its eight keys as 16 bytes.
 //
-// The matrix cores bound long chunks: 2048 tokens on 8192 bf16 keys, 32 heads on 8 of 128, take 895 us, 346 TFLOP/s or
-// 1037 in bf16 products (MI355X; a library product of 8192 reaches 1254).  A prompt of 1024, 12 heads of 64, fp32, has one
+// The matrix cores bound long chunks: 2048 tokens on 8192 bf16 keys, 32 heads on 8 of 128, take 900 us, 344 TFLOP/s or
+// 1031 in bf16 products (MI355X; a library product of 8192 reaches 1254).  A prompt of 1024, 12 heads of 64, fp32, has one
 // workgroup a CU, whose waves do their loads, splits, products and exponentials in step: 21 us and 5 to join, where the
 // products alone would take 8.
 #include <mutex>
