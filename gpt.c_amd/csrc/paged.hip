@@ -270,11 +270,15 @@ static void release_plan(gptc_paged_plan_t *plan) {
             free_cuda(plan->part_o);
             free_cuda(plan->part_ml);
         }
+        // None of this touches a stream that somebody may be capturing in the mode that forbids such calls.
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        hipCheck(hipThreadExchangeStreamCaptureMode(&mode));
         for (int i = 0; i < 2; ++i) {
             hipCheck(hipEventSynchronize(plan->copied[i]));  // its last copy may still read the host memory
             hipCheck(hipEventDestroy(plan->copied[i]));
             hipCheck(hipHostFree(plan->host[i]));
         }
+        hipCheck(hipThreadExchangeStreamCaptureMode(&mode));
     }
     free(plan->writer);
     free(plan->table_at);

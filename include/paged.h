@@ -126,7 +126,7 @@ void gptc_paged_plan_free(gptc_paged_plan_t *plan);  // during a capture: done b
  *   the results that use them NaN or infinite.  Where a sequence brings 64 query
  *   rows per kv head or more, products are sums of bf16 parts: there fp32 values
  *   below 2^-110 count with fewer than 24 bits, and those past the largest bf16
- *   value as infinite.  So do queries with bf16 pages.
+ *   value may count as infinite.  So do queries with bf16 pages.
  */
 tensor_t *gptc_rotary_table(const int rows, const int rot, const double theta);
 void gptc_paged_append_cuda(gptc_paged_plan_t *plan, const int layer, const tensor_t *qkv, const tensor_t *rotary,

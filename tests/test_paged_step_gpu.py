@@ -515,3 +515,33 @@ def test_a_graph_on_another_stream(rt, dtype):
         graph.free()
     pool.free()
     rt.free(tq)
+
+
+def test_a_plan_freed_while_another_stream_is_captured(rt):
+    """In the mode in which a capture forbids waits and frees of the process: it ends as if nothing had been."""
+    pool = Pool(rt, [500], [3], 4, 2, 64, 64, gptc.F32, seed=2)
+    kept = pool.fill([503])
+    q = pool.normal(3, 4, 64)
+    tq, out = rt.from_numpy(q.reshape(3, -1)), rt.empty((3, 256))
+    plan = gptc.PagedPlan(rt, pool.cache, 4, 2, 100, 600)
+    plan.set(pool.past, pool.fresh, pool.table)
+    plan.attention(0, tq, out)
+    x = torch.arange(1000.0, device="cuda")
+    y = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="global"):
+        y.add_(x)
+        plan.free()
+        y.mul_(2.0)
+    for _ in range(3):
+        y.fill_(1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, 2 * (x + 1))
+    pool.set()
+    pool.plan.attention(0, tq, out)
+    check_attention(pool, kept, q, rt.to_numpy(out))
+    pool.free()
+    rt.free(tq)
+    rt.free(out)
