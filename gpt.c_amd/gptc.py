@@ -207,6 +207,9 @@ SIGNATURES = {
     "embedding_backward_cuda_kernel": (None, [TensorP, TensorP, TensorP]),
     "cross_entropy_forward_cuda_kernel": (None, [TensorP, TensorP, ctypes.POINTER(TensorP), TensorP]),
     "cross_entropy_backward_cuda_kernel": (None, [TensorP, ctypes.POINTER(TensorP), TensorP]),
+    "gptc_linear_cross_entropy_cuda": (None, [TensorP] * 8 + [_ci]),
+    "gptc_embedding_forward_scaled_cuda": (None, [TensorP, TensorP, TensorP, _cf, TensorP]),
+    "gptc_embedding_backward_sorted_cuda": (None, [TensorP, TensorP, _cf, TensorP, TensorP, _ci]),
     "step_adamW_cuda_kernel": (None, [ctypes.POINTER(TensorP)] * 4 + [_ci, _cf, _cf, _cf, _cf, _cf, _ci]),
     "zero_grad_adamW_cuda_kernel": (None, [ctypes.POINTER(TensorP), _ci]),
     "gptc_linear_rows_cuda": (None, [TensorP, TensorP, TensorP, TensorP, _ci, TensorP]),
@@ -245,6 +248,8 @@ SIGNATURES = {
     "SelfAttention": (_vp, [_ci, _ci, _ci, _ci]),
     "Block": (_vp, [_ci, _ci, _ci, _ci]),
     "GPT2": (_vp, [_vp]),
+    "gptc_gpt2_loss": (TensorP, [_vp, TensorP, TensorP, TensorP]),
+    "gptc_gpt2_loss_backward": (TensorP, [_vp, TensorP, TensorP, TensorP]),
     # rand.h
     "manual_seed": (None, [_vp, ctypes.c_uint]),
     "randint32": (ctypes.c_uint, [_vp]),
@@ -539,6 +544,14 @@ class GPT2Model(_Layer):
             else:
                 out.append(self.rt.normal(shp, seed_base + i, 0.0, std))
         return out
+
+    def loss(self, ids, targets, weights=None):
+        """gptc_gpt2_loss: the mean loss on device tensors, without the logits."""
+        return self.rt.lib.gptc_gpt2_loss(self.raw, ids, targets, weights)
+
+    def loss_backward(self, ids, targets, weights=None):
+        """gptc_gpt2_loss_backward: the same, adding to every parameter's gradient."""
+        return self.rt.lib.gptc_gpt2_loss_backward(self.raw, ids, targets, weights)
 
     def fast_load(self, arrays):
         """fast_load_state_dict from numpy arrays in parameters() order."""

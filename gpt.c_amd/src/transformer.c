@@ -49,6 +49,63 @@ static tensor_t *backward_transformer(gpt2_t *gpt, tensor_t *global_grad) {
     return d_tok_emb;
 }
 
+/* ln_f's output for ids x: the embeddings in one lookup, then the blocks. */
+static tensor_t *forward_hidden(gpt2_t *gpt, const tensor_t *x) {
+    const int T = x->shape[1];
+    int shape[3] = {x->shape[0], T, gpt->n_embd};
+    CHECK_ERROR(T > gpt->block_size, "Cannot forward a sequence of length %d, block size is %d.", T, gpt->block_size);
+    tensor_t *out = create_tensor(shape, 3, CUDA);
+    gptc_embedding_forward_scaled_cuda(gpt->wte->W, gpt->wpe->W, x, 1.0f, out);
+    for (int i = 0; i < gpt->n_layers; i++) out = gpt->layers[i]->forward(gpt->layers[i], out);
+    return gpt->ln_f->forward(gpt->ln_f, out);
+}
+
+static void check_loss_args(const gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights) {
+    CHECK_ERROR(x->ndims != 2, "Expected ids of shape (B, T), but got %d dims.", x->ndims);
+    CHECK_ERROR(x->device != CUDA || targets->device != CUDA || gpt->wte->W->device != CUDA ||
+                    (weights != NULL && weights->device != CUDA),
+                "The loss without logits runs on the GPU: move the model, ids, targets and weights there.");
+    CHECK_ERROR(x->length < 1 || targets->length != x->length, "Expected as many targets as ids, but got %d and %d.",
+                targets->length, x->length);
+    CHECK_ERROR(weights != NULL && weights->length != x->length, "Expected as many weights as ids, but got %d and %d.",
+                weights != NULL ? weights->length : 0, x->length);
+}
+
+tensor_t *gptc_gpt2_loss(gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights) {
+    REQUIRE_ARG(gpt);
+    REQUIRE_ARG(x);
+    REQUIRE_ARG(targets);
+    check_loss_args(gpt, x, targets, weights);
+    int one[1] = {1};
+    tensor_t *loss = create_tensor(one, 1, CUDA);
+    tensor_t *out = forward_hidden(gpt, x);
+    gptc_linear_cross_entropy_cuda(out, gpt->wte->W, targets, weights, loss, NULL, NULL, NULL, 0);
+    free_tensor(out);
+    gpt->free_cache(gpt);
+    return loss;
+}
+
+tensor_t *gptc_gpt2_loss_backward(gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights) {
+    REQUIRE_ARG(gpt);
+    REQUIRE_ARG(x);
+    REQUIRE_ARG(targets);
+    check_loss_args(gpt, x, targets, weights);
+    embedding_t *wte = gpt->wte, *wpe = gpt->wpe;
+    if (!wte->dW) wte->dW = zeros(wte->W->shape, wte->W->ndims, CUDA);
+    if (!wpe->dW) wpe->dW = zeros(wpe->W->shape, wpe->W->ndims, CUDA);
+    int one[1] = {1};
+    tensor_t *loss = create_tensor(one, 1, CUDA);
+    tensor_t *hidden = forward_hidden(gpt, x);
+    tensor_t *out = create_tensor(hidden->shape, hidden->ndims, CUDA);
+    gptc_linear_cross_entropy_cuda(hidden, wte->W, targets, weights, loss, NULL, out, wte->dW, 1);
+    free_tensor(hidden);
+    out = gpt->ln_f->backward(gpt->ln_f, out);
+    for (int i = gpt->n_layers - 1; i >= 0; i--) out = gpt->layers[i]->backward(gpt->layers[i], out);
+    gptc_embedding_backward_sorted_cuda(out, x, 1.0f, wte->dW, wpe->dW, 1);
+    free_tensor(out);
+    return loss;
+}
+
 static void description_transformer(const gpt2_t *gpt) {
     printf("GPT-2 model: %d layers, %d heads, width %d, context %d, vocabulary %d; %d parameters\n",
            gpt->n_layers, gpt->n_heads, gpt->n_embd, gpt->block_size, gpt->vocab_size, gpt->num_parameters(gpt));

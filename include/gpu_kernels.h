@@ -243,6 +243,45 @@ void cross_entropy_forward_cuda_kernel(
 );
 void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tensor_t **cache, tensor_t *dout);
 
+/*
+ * ---- the two ends of a GPT in training: no counterpart in the reference ----
+ * gptc_linear_cross_entropy_cuda(x, W, targets, weights, output, row_losses, dx, dW, accumulate)
+ *   Linear without bias and cross-entropy in one, without keeping the logits
+ *   (three (rows, V) tensors in gpt.c): with l = x W^T, x (..., C), W (V, C),
+ *   and loss[r] = log(sum_j exp l[r, j]) - l[r, targets[r]],
+ *   output[0]   = sum_r weights[r] loss[r] / rows;
+ *   row_losses  (rows), or NULL: loss[r];
+ *   dx          like x, or NULL: output's gradient of x, overwritten;
+ *   dW          like W, or NULL: output's gradient of W, overwritten, or added
+ *               to dW when `accumulate`.
+ *   dx and dW both NULL: the loss alone, at a third of the products.  weights
+ *   (rows) or NULL for ones.  A row of weight 0 takes no part, whatever its x
+ *   and target hold (padding): loss 0, dx 0.  With other weights a target
+ *   outside [0, V) gives a NaN loss and the softmax part of the gradients, as
+ *   cross_entropy_*_cuda_kernel.  V < 2^22.  Results may not overlap another
+ *   tensor of the call.  Deterministic.  Takes scratch: not under graph capture.
+ *
+ * gptc_embedding_forward_scaled_cuda(W, pos, ids, scale, output)
+ *   output (ids..., C) = scale W[ids] (+ pos[i], i the id's place in ids' last
+ *   dimension; pos (positions, C) or NULL).  Ids are floats truncated to int;
+ *   those outside [0, V) give NaN rows.
+ * gptc_embedding_backward_sorted_cuda(global_grad, ids, scale, dW, dpos, accumulate)
+ *   Its gradients: dW (V, C) = scale sum of global_grad over the places of each
+ *   id, dpos (positions, C), or NULL, = sum of global_grad over each place of
+ *   ids' last dimension; overwritten (zeros where nothing falls), or added to
+ *   when `accumulate`.  Ids outside [0, V) count for dpos alone.
+ *   Rows are sorted by id and added in their order, long runs in parts of fixed
+ *   lengths: deterministic, but not embedding_backward_cuda_kernel's one chain.
+ *   Takes scratch: not under graph capture.
+ */
+void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t *W, const tensor_t *targets,
+                                    const tensor_t *weights, tensor_t *output, tensor_t *row_losses, tensor_t *dx,
+                                    tensor_t *dW, const int accumulate);
+void gptc_embedding_forward_scaled_cuda(const tensor_t *W, const tensor_t *pos, const tensor_t *ids, const float scale,
+                                        tensor_t *output);
+void gptc_embedding_backward_sorted_cuda(const tensor_t *global_grad, const tensor_t *ids, const float scale,
+                                         tensor_t *dW, tensor_t *dpos, const int accumulate);
+
 /* AdamW, replaces kernels/src/cuda/AdamW.h:9-24 (cpu/AdamW.c:5-58).
  * One launch per 36 tensors of the list. */
 void step_adamW_cuda_kernel(

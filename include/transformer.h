@@ -56,6 +56,24 @@ typedef struct {
 
 gpt2_t *GPT2(GPT2Config_t *config);
 
+/*
+ * A step without the logits: no counterpart in the reference, whose loop keeps
+ * them, their log-softmax and their gradient (train_gpt.c:481-521).  On the GPU.
+ *
+ * gptc_gpt2_loss(gpt, x, targets, weights)
+ *   The mean cross entropy of the model's predictions for ids x (B, T) against
+ *   targets (B, T), a 1-element tensor: CrossEntropyLoss over forward(x).
+ *   weights (B, T), or NULL for ones: the sum of weights times losses over B T;
+ *   what a position of weight 0 is given as a target does not matter (the loss of
+ *   gptc_linear_cross_entropy_cuda, gpu_kernels.h).  Leaves no caches behind.
+ * gptc_gpt2_loss_backward(gpt, x, targets, weights)
+ *   The same, and every parameter's gradient is added to: forward, loss, and the
+ *   two backwards of gpt.c's loop for an upstream gradient of ones.
+ * Both read x, targets and weights, which stay the caller's.
+ */
+tensor_t *gptc_gpt2_loss(gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights);
+tensor_t *gptc_gpt2_loss_backward(gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights);
+
 #ifdef __cplusplus
 }
 #endif
