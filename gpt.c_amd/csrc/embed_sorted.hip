@@ -165,13 +165,6 @@ __global__ __launch_bounds__(kScanThreads) void digit_scan_kernel(int *hist, int
     }
 }
 
-// A wave's own LDS accesses are done in order; this keeps the compiler's order.
-__device__ __forceinline__ void wave_lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 __global__ __launch_bounds__(kSortThreads) void digit_move_kernel(const SortArgs a) {
     constexpr int kW = kSortThreads / kWave;
     __shared__ int at[kW][kDigits];  // where a wave's next row of a digit goes

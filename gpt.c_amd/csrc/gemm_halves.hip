@@ -1,0 +1,483 @@
+// Products of operands laid out as two fp16 parts (gemm_halves.hpp), fp32 results.
+//
+// A float times a power of two is the sum of two fp16 values to 2^-24 of it (11 +
+// 11 bits and the low part's sign), as close as fp32 itself.  Of the four products
+// of two such sums three are formed, low high, high low and high high; the fourth
+// is at most 2^-24 of the product.  A product of fp16 values is exact in fp32, so
+// three v_mfma_f32_32x32x16_f16 do what takes six bf16 instructions from three-part
+// sums (gemm_split.hip), whose parts need no common scale.
+//
+// Sums.  As there: the matrix core drops bits below its accumulator towards minus
+// infinity, so each step of 32 terms is summed in a fresh accumulator, smallest
+// products first, and taken into the tile by a rounded fp32 add; every other step
+// is formed negated and subtracted, which cancels what shift is left.
+//
+// A workgroup forms 128 x 128 outputs, its four waves 64 x 64 each.  The operands lie
+// in memory as the instruction takes them, so a step's 32 KB go to LDS by 32 loads
+// of 1 KB that pass no register, and every LDS access is 1 KB in a row.  Two buffers:
+// a step's fragments are read to registers at once, and the loads of the step after
+// next go out into the same buffer as soon as all waves have read it.
+#include <algorithm>
+#include "gemm_halves.hpp"
+#include "gpu_kernels.h"
+#include "ops_common.hpp"
+
+namespace gptc {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kStageBytes = 32768;
+
+__device__ __forceinline__ hf32x16 mfma(hu32x4 a, hu32x4 b, hf32x16 c) {
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// ---- operands ----
+
+// One block of 32 rows a workgroup; the four waves take terms in turns.
+__global__ __launch_bounds__(kThreads) void halves_rows_kernel(const float *__restrict__ x, int ld,
+                                                              const float *__restrict__ weights, Halves h, bool negate,
+                                                              bool vec) {
+    __shared__ int shift[32];
+    const int rb = blockIdx.x, tid = threadIdx.x;
+    const int lane = tid & 63, w = tid >> 6;
+    {  // eight threads a row find its largest value
+        const int row = rb * 32 + (tid >> 3);
+        const bool live = row < h.rows && (weights == nullptr || weights[row] != 0.0f);
+        const float *p = x + static_cast<int64_t>(row) * ld;
+        float m = 0.0f;
+        if (live) {
+            if (vec) {
+                for (int k = 4 * (tid & 7); k < h.terms; k += 32) {
+                    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p + k);
+                    m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                }
+            } else {
+                for (int k = tid & 7; k < h.terms; k += 8) m = fmaxf(m, fabsf(p[k]));
+            }
+        }
+        m = fmaxf(m, __shfl_xor(m, 1, 64));
+        m = fmaxf(m, __shfl_xor(m, 2, 64));
+        m = fmaxf(m, __shfl_xor(m, 4, 64));
+        if ((tid & 7) == 0) {
+            shift[tid >> 3] = halves_shift(m);
+            h.shift[row] = halves_shift(m);
+        }
+    }
+    __syncthreads();
+    const int row = rb * 32 + (lane & 31), hf = lane >> 5, kbs = h.term_blocks();
+    const bool live = row < h.rows && (weights == nullptr || weights[row] != 0.0f);
+    const float *p = x + static_cast<int64_t>(live ? row : 0) * ld;
+    const int up = shift[lane & 31];
+    hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs * 2) * 64 + lane;
+    for (int kb = w; kb < kbs; kb += 4) {
+        const int k0 = kb * 16 + 4 * hf;
+        float v[8];
+        if (vec && k0 + 12 <= h.terms) {
+            const f32x4_t a = *reinterpret_cast<const f32x4_t *>(p + k0), b = *reinterpret_cast<const f32x4_t *>(p + k0 + 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = a[e];
+                v[4 + e] = b[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = k0 + (e & 3) + 8 * (e >> 2);
+                v[e] = k < h.terms ? p[k] : 0.0f;
+            }
+        }
+        const bool minus = negate && halves_negated(kb * 16);
+        hu32x4 high, low;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a = live ? __builtin_amdgcn_ldexpf(v[2 * e], up) : 0.0f;
+            float b = live ? __builtin_amdgcn_ldexpf(v[2 * e + 1], up) : 0.0f;
+            uint32_t hi, lo;
+            halves_split(minus ? -a : a, minus ? -b : b, hi, lo);
+            high[e] = hi;
+            low[e] = lo;
+        }
+        out[(kb * 2) * 64] = high;
+        out[(kb * 2 + 1) * 64] = low;
+    }
+}
+
+// The factor of term k of an operand that is read across its rows.
+__device__ __forceinline__ float term_factor(const float *weights, float divisor, int k) {
+    return weights != nullptr ? weights[k] / divisor : 1.0f / divisor;
+}
+
+constexpr int kColumnTerms = 128;  // terms a workgroup
+
+// largest[c] = bits of the largest magnitude of column c so far (whole numbers: in any order the same).
+__global__ __launch_bounds__(kThreads) void column_largest_kernel(const float *__restrict__ x, int ld,
+                                                                 const float *__restrict__ weights, float divisor,
+                                                                 int terms, int cols, uint32_t *largest) {
+    const int c = blockIdx.x * kThreads + threadIdx.x;
+    if (c >= cols) return;
+    const int k0 = blockIdx.y * kColumnTerms, k1 = min(terms, k0 + kColumnTerms);
+    float m = 0.0f;
+#pragma unroll 8
+    for (int k = k0; k < k1; ++k) {
+        const float f = term_factor(weights, divisor, k);
+        if (f != 0.0f) m = fmaxf(m, fabsf(f * x[static_cast<int64_t>(k) * ld + c]));
+    }
+    atomicMax(largest + c, __float_as_uint(m));
+}
+
+// A wave: 32 columns, kColumnTerms / 4 terms.
+__global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *__restrict__ x, int ld,
+                                                                 const float *__restrict__ weights, float divisor,
+                                                                 Halves h, const uint32_t *__restrict__ largest) {
+    const int lane = threadIdx.x & 63, hf = lane >> 5, w = threadIdx.x >> 6;
+    const int rb = blockIdx.x, c = rb * 32 + (lane & 31), kbs = h.term_blocks();
+    const int up = c < h.rows ? halves_shift(__uint_as_float(largest[c])) : 0;
+    if (blockIdx.y == 0 && w == 0 && hf == 0) h.shift[c] = up;
+    hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs * 2) * 64 + lane;
+    const int first = blockIdx.y * (kColumnTerms / 16) + w * (kColumnTerms / 64);
+#pragma unroll
+    for (int i = 0; i < kColumnTerms / 64; ++i) {
+        const int kb = first + i;
+        if (kb >= kbs) return;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = kb * 16 + 4 * hf + (e & 3) + 8 * (e >> 2);
+            v[e] = 0.0f;
+            if (k < h.terms && c < h.rows) {
+                const float f = term_factor(weights, divisor, k);
+                if (f != 0.0f) v[e] = __builtin_amdgcn_ldexpf(f * x[static_cast<int64_t>(k) * ld + c], up);
+            }
+        }
+        hu32x4 high, low;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t hi, lo;
+            halves_split(v[2 * e], v[2 * e + 1], hi, lo);
+            high[e] = hi;
+            low[e] = lo;
+        }
+        out[(kb * 2) * 64] = high;
+        out[(kb * 2 + 1) * 64] = low;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void zero_words_kernel(uint32_t *p, int n) {
+    const int i = blockIdx.x * kThreads + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+
+// ---- the product's loop ----
+
+struct Tile {
+    const hu32x4 *A, *B;
+    const int *shift_a, *shift_b;
+    int all_a, all_b;  // where shift_a or shift_b is null
+    int tiles_m, tiles_n, kbs, stages, slice;  // stages of 32 terms in all, and of a slice
+};
+
+__device__ __forceinline__ int shift_of(const int *shift, int all, int row) { return shift != nullptr ? shift[row] : all; }
+
+// The tile of this workgroup: 8 contiguous ranges of tiles, one per XCD (workgroup i runs on XCD
+// i % 8); in a range, columns of 8 row tiles, so that the tiles that run together share rows
+// and columns.
+__device__ __forceinline__ void tile_of(const Tile &t, int &tm, int &tn) {
+    const int n = t.tiles_m * t.tiles_n;
+    int i = blockIdx.x;
+    const int x = i & 7, q = n >> 3, r = n & 7;
+    i = (i >> 3) + x * q + min(x, r);
+    const int G = 8, per = G * t.tiles_n;
+    const int g = i / per, first = g * G, h = min(G, t.tiles_m - first);
+    const int in = i - g * per;
+    tm = first + in % h;
+    tn = in / h;
+}
+
+__device__ __forceinline__ void load_stage(const hu32x4 *a, const hu32x4 *b, hu32x4 *lds, int w, int lane) {
+    using Global = const __attribute__((address_space(1))) void *;
+    using Shared = __attribute__((address_space(3))) void *;
+    const Global ga = (Global)(a + lane), gb = (Global)(b + lane);
+    const Shared la = (Shared)(lds + w * 256), lb = (Shared)(lds + 1024 + w * 256);
+    __builtin_amdgcn_global_load_lds(ga, la, 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(ga, la, 16, 1024, 0);
+    __builtin_amdgcn_global_load_lds(ga, la, 16, 2048, 0);
+    __builtin_amdgcn_global_load_lds(ga, la, 16, 3072, 0);
+    __builtin_amdgcn_global_load_lds(gb, lb, 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(gb, lb, 16, 1024, 0);
+    __builtin_amdgcn_global_load_lds(gb, lb, 16, 2048, 0);
+    __builtin_amdgcn_global_load_lds(gb, lb, 16, 3072, 0);
+}
+
+// A wave's fragments of a step: of either operand two blocks of 32 rows, two of 16 terms, two parts.
+struct Fragments {
+    hu32x4 a[2][2][2], b[2][2][2];
+};
+
+// The reads and their wait are one block, so no register is used before its data is there.
+__device__ __forceinline__ void read_stage(uint32_t at_a, uint32_t at_b, Fragments &f) {
+    asm volatile(
+        "ds_read_b128 %0, %16\n\t"
+        "ds_read_b128 %1, %16 offset:1024\n\t"
+        "ds_read_b128 %2, %16 offset:2048\n\t"
+        "ds_read_b128 %3, %16 offset:3072\n\t"
+        "ds_read_b128 %8, %17\n\t"
+        "ds_read_b128 %9, %17 offset:1024\n\t"
+        "ds_read_b128 %10, %17 offset:2048\n\t"
+        "ds_read_b128 %11, %17 offset:3072\n\t"
+        "ds_read_b128 %4, %16 offset:4096\n\t"
+        "ds_read_b128 %5, %16 offset:5120\n\t"
+        "ds_read_b128 %6, %16 offset:6144\n\t"
+        "ds_read_b128 %7, %16 offset:7168\n\t"
+        "ds_read_b128 %12, %17 offset:4096\n\t"
+        "ds_read_b128 %13, %17 offset:5120\n\t"
+        "ds_read_b128 %14, %17 offset:6144\n\t"
+        "ds_read_b128 %15, %17 offset:7168\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(f.a[0][0][0]), "=&v"(f.a[0][0][1]), "=&v"(f.a[0][1][0]), "=&v"(f.a[0][1][1]), "=&v"(f.a[1][0][0]),
+          "=&v"(f.a[1][0][1]), "=&v"(f.a[1][1][0]), "=&v"(f.a[1][1][1]), "=&v"(f.b[0][0][0]), "=&v"(f.b[0][0][1]),
+          "=&v"(f.b[0][1][0]), "=&v"(f.b[0][1][1]), "=&v"(f.b[1][0][0]), "=&v"(f.b[1][0][1]), "=&v"(f.b[1][1][0]),
+          "=&v"(f.b[1][1][1])
+        : "v"(at_a), "v"(at_b)
+        : "memory");
+}
+
+// acc = the wave's 64 x 64 outputs of tile (tm, tn) over this slice's terms, without the shifts.
+__device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int s0, int s1, hu32x4 *lds,
+                                             hf32x16 (&acc)[2][2]) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Wave w loads the w-th block of rows of either operand: 4 KB each a step.
+    const hu32x4 *a = t.A + (static_cast<int64_t>(tm * 4 + w) * t.kbs + 2 * s0) * 128;
+    const hu32x4 *b = t.B + (static_cast<int64_t>(tn * 4 + w) * t.kbs + 2 * s0) * 128;
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) void *)lds));
+    const uint32_t at_a = base + (w >> 1) * 8192 + lane * 16, at_b = base + 16384 + (w & 1) * 8192 + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    load_stage(a, b, lds, w, lane);
+    if (s0 + 1 < s1) load_stage(a + 256, b + 256, lds + 2048, w, lane);
+    float sign = s0 & 1 ? -1.0f : 1.0f;
+    for (int s = s0; s < s1; ++s) {
+        const uint32_t off = (s - s0) & 1 ? kStageBytes : 0;
+        // This wave's loads of step s have landed (those of the next may be on their way), then all waves'.
+        if (s + 1 < s1)
+            asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        Fragments f;
+        read_stage(at_a + off, at_b + off, f);
+        asm volatile("s_barrier" ::: "memory");  // all waves have read this buffer
+        if (s + 2 < s1) load_stage(a + (s + 2 - s0) * 256, b + (s + 2 - s0) * 256, lds + (off >> 4), w, lane);
+        hf32x16 p[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[i][j][r] = 0.0f;
+        constexpr int kProd[3][2] = {{1, 0}, {0, 1}, {0, 0}};
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) p[i][j] = mfma(f.a[i][k][kProd[q][0]], f.b[j][k][kProd[q][1]], p[i][j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(sign, p[i][j][r], acc[i][j][r]);
+        sign = -sign;
+    }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void logits_kernel(const Tile t,
+                                                                                                   const LogitsArgs l) {
+    __shared__ hu32x4 lds[2 * kStageBytes / 16];
+    int tm, tn;
+    tile_of(t, tm, tn);
+    hf32x16 acc[2][2];
+    tile_product(t, tm, tn, 0, t.stages, lds, acc);
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int token0 = tm * 128 + (w >> 1) * 64, row0 = tn * 128 + (w & 1) * 64;
+    const int jbs = t.tiles_m * 4, rows = t.tiles_n * 128;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int row = row0 + 32 * j + l32;
+        const int up = shift_of(t.shift_b, t.all_b, row);
+        const int target = l.targets[row];
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int token = token0 + 32 * i + 8 * q + 4 * hf;
+                const int4 back = *reinterpret_cast<const int4 *>(t.shift_a + token);
+                const int shift[4] = {back.x, back.y, back.z, back.w};
+                f32x4_t v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + e], -up - shift[e]);
+                    if (token + e >= l.vocabulary) x = -INFINITY;
+                    if (token + e == target) l.target_logits[row] = x;
+                    acc[i][j][4 * q + e] = v[e] = x;
+                    m = fmaxf(m, x);
+                }
+                if (l.logits != nullptr) {
+                    const int64_t block = static_cast<int64_t>((row0 >> 5) + j) * jbs + (token0 >> 5) + i;
+                    reinterpret_cast<f32x4_t *>(l.logits)[(block * 4 + q) * 64 + lane] = v;
+                }
+            }
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        float s = 0.0f;
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
+        s += __shfl_xor(s, 32, 64);
+        if (hf == 0) l.stats[static_cast<int64_t>(token0 >> 6) * rows + row] = make_float2(m, s);
+    }
+}
+
+struct ProductArgs {
+    HalvesProduct p;
+    int M, N;
+    float *part;  // the slices' sums, (M, N) each, or null
+};
+
+__device__ __forceinline__ float times_row_factor(const HalvesProduct &p, int row, float v) {
+    const float f = p.row_factor != nullptr ? p.row_factor[row] : 1.0f;
+    return f != 0.0f ? v * (f / p.divisor) : 0.0f;
+}
+
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
+    const Tile t, const ProductArgs a) {
+    __shared__ hu32x4 lds[2 * kStageBytes / 16];
+    int tm, tn;
+    tile_of(t, tm, tn);
+    hf32x16 acc[2][2];
+    const int s0 = blockIdx.y * t.slice;
+    tile_product(t, tm, tn, s0, min(t.stages, s0 + t.slice), lds, acc);
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m0 = tm * 128 + (w >> 1) * 64, n0 = tn * 128 + (w & 1) * 64;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int n = n0 + 32 * j + l32;
+        if (n >= a.N) continue;
+        const int up = shift_of(t.shift_b, t.all_b, n);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float old[16];
+            if (a.part == nullptr && a.p.add)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int m = min(m0 + 32 * i + 8 * (r >> 2) + 4 * hf + (r & 3), a.M - 1);
+                    old[r] = a.p.C[static_cast<int64_t>(m) * a.p.ldc + n];
+                }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = m0 + 32 * i + 8 * (r >> 2) + 4 * hf + (r & 3);
+                if (m >= a.M) continue;
+                float v = __builtin_amdgcn_ldexpf(acc[i][j][r], -up - shift_of(t.shift_a, t.all_a, m));
+                if (a.part != nullptr) {
+                    a.part[(static_cast<int64_t>(blockIdx.y) * a.M + m) * a.N + n] = v;
+                } else {
+                    v = times_row_factor(a.p, m, v);
+                    a.p.C[static_cast<int64_t>(m) * a.p.ldc + n] = a.p.add ? old[r] + v : v;
+                }
+            }
+        }
+    }
+}
+
+// C = the slices' sums in their order, times the row's factor (+ C).
+__global__ __launch_bounds__(kThreads) void join_slices_kernel(const ProductArgs a, int slices) {
+    const int64_t n = static_cast<int64_t>(a.M) * a.N, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n; i += stride) {
+        float v = a.part[i];
+        for (int s = 1; s < slices; ++s) v += a.part[s * n + i];
+        const int m = static_cast<int>(i / a.N);
+        float *c = a.p.C + static_cast<int64_t>(m) * a.p.ldc + (i - static_cast<int64_t>(m) * a.N);
+        v = times_row_factor(a.p, m, v);
+        *c = a.p.add ? *c + v : v;
+    }
+}
+
+Tile tile_args(const Halves &A, const Halves &B) {
+    CHECK_ERROR(A.terms != B.terms, "Operands of %d and %d terms.", A.terms, B.terms);
+    const int stages = A.term_blocks() / 2;
+    return {A.data, B.data, A.shift, B.shift, A.shift_all, B.shift_all, A.row_blocks() / 4, B.row_blocks() / 4,
+            A.term_blocks(), stages, stages};
+}
+
+}  // namespace
+
+void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s) {
+    const bool vec = ld % 4 == 0 && h.terms % 4 == 0 && aligned16(x);
+    halves_rows_kernel<<<dim3(h.row_blocks()), dim3(kThreads), 0, s>>>(x, ld, weights, h, negate, vec);
+    hipCheck(hipGetLastError());
+}
+
+void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
+                           uint32_t *scratch, hipStream_t s) {
+    zero_words_kernel<<<dim3((h.rows + kThreads - 1) / kThreads), dim3(kThreads), 0, s>>>(scratch, h.rows);
+    hipCheck(hipGetLastError());
+    const int chunks = (h.term_blocks() * 16 + kColumnTerms - 1) / kColumnTerms;
+    column_largest_kernel<<<dim3((h.rows + kThreads - 1) / kThreads, chunks), dim3(kThreads), 0, s>>>(
+        x, ld, weights, divisor, h.terms, h.rows, scratch);
+    hipCheck(hipGetLastError());
+    halves_columns_kernel<<<dim3(h.row_blocks(), chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor, h, scratch);
+    hipCheck(hipGetLastError());
+}
+
+void launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s) {
+    const Tile t = tile_args(A, B);
+    logits_kernel<<<dim3(t.tiles_m * t.tiles_n), dim3(kThreads), 0, s>>>(t, l);
+    hipCheck(hipGetLastError());
+}
+
+void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
+    Tile t = tile_args(A, B);
+    const int tiles = t.tiles_m * t.tiles_n;
+    // Slices of the reduction so that the last round of 512 workgroups (two a CU) is full.  In steps of
+    // 32 terms: a workgroup's start and end cost about 8, a slice's sums go out and come back.
+    int best = 1;
+    double best_cost = 1e30;
+    for (int S = 1; S <= 32 && S <= t.stages; ++S) {
+        const int mine = (t.stages + S - 1) / S;
+        const int rounds = (tiles * S + 511) / 512;
+        const double cost = rounds * (mine + 8.0) + (S > 1 ? 8.0 + S * 0.02 * tiles : 0.0);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = S;
+        }
+    }
+    t.slice = (t.stages + best - 1) / best;
+    const int slices = (t.stages + t.slice - 1) / t.slice;
+    ProductArgs a{p, A.rows, B.rows, nullptr};
+    if (slices > 1) a.part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(A.rows) * B.rows * slices));
+    product_kernel<<<dim3(tiles, slices), dim3(kThreads), 0, s>>>(t, a);
+    hipCheck(hipGetLastError());
+    if (slices == 1) return;
+    join_slices_kernel<<<dim3(blocks_for(static_cast<int64_t>(A.rows) * B.rows, kThreads)), dim3(kThreads), 0, s>>>(a,
+                                                                                                                  slices);
+    hipCheck(hipGetLastError());
+    free_cuda(a.part);
+}
+
+}  // namespace gptc

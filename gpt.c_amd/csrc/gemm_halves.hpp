@@ -1,0 +1,83 @@
+// Products of fp32 operands that are laid out beforehand as sums of two fp16
+// values, three matrix instructions a product (gemm_halves.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+namespace gptc {
+
+typedef float hf32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t hu32x4 __attribute__((ext_vector_type(4)));
+
+// An operand of `rows` (of the product's M or N) by `terms` (of its reduction),
+// padded with zeros to rows of 128 and terms of 32.  Row r's values are held
+// times 2^shift[r], which puts the largest below 2^15: value = high + low to
+// 2^-24 of it, or to 2^-40 of the row's largest for values below its 2^-17th.
+// Blocks of 32 rows x 16 terms, block (r / 32, k / 16) after block, high part
+// (1 KB) then low part: lane l of a wave holds row l % 32 and the terms
+// 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11}, as the 32x32x16 instruction takes them
+// (in an order of terms that suits fp32 results as the next product's operand).
+struct Halves {
+    hu32x4 *data;
+    int *shift;  // (padded rows), or null: every row's is `shift_all`
+    int shift_all;
+    int rows, terms;
+    __host__ __device__ int row_blocks() const { return (rows + 127) / 128 * 4; }
+    __host__ __device__ int term_blocks() const { return (terms + 31) / 32 * 2; }
+    __host__ __device__ int64_t bytes() const { return static_cast<int64_t>(row_blocks()) * term_blocks() * 2048; }
+};
+
+constexpr int kHalvesTop = 14;  // the largest value of a row is held below 2^(kHalvesTop + 1)
+
+// The shift of a row whose largest magnitude is m (0, infinities and NaN: as they are).
+__device__ __forceinline__ int halves_shift(float m) {
+    const int e = static_cast<int>((__float_as_uint(m) >> 23) & 0xff);
+    if (e == 0xff || m == 0.0f) return 0;
+    return kHalvesTop - (e == 0 ? -127 : e - 127);  // subnormal values end up to 2^23 lower, still exact
+}
+
+// Two values as high parts and low parts (packed): each part the nearest fp16 of what is left.
+__device__ __forceinline__ void halves_split(float x, float y, uint32_t &high, uint32_t &low) {
+    const _Float16 hx = static_cast<_Float16>(x), hy = static_cast<_Float16>(y);
+    const _Float16 lx = static_cast<_Float16>(x - static_cast<float>(hx));
+    const _Float16 ly = static_cast<_Float16>(y - static_cast<float>(hy));
+    high = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, hx)) |
+           static_cast<uint32_t>(__builtin_bit_cast(uint16_t, hy)) << 16;
+    low = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, lx)) |
+          static_cast<uint32_t>(__builtin_bit_cast(uint16_t, ly)) << 16;
+}
+
+// Negating every other step of 32 terms of one of a product's operands (the first) keeps the
+// matrix core's truncation from adding up: the kernels subtract those steps.
+__device__ __forceinline__ bool halves_negated(int term) { return ((term >> 5) & 1) != 0; }
+
+// x (rows x terms, rows of ld floats; with weights, rows of weight 0 as zeros) into h.data and
+// h.shift; negate: as a product's first operand.
+void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s);
+// x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
+// as a second operand.  scratch: h.rows words.
+void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
+                           uint32_t *scratch, hipStream_t s);
+
+// The logits of a piece: A = W (vocabulary x features), B = x (rows x features).
+struct LogitsArgs {
+    float *logits;         // blocks of 32 rows x 32 tokens in the order of the accumulators, or null
+    float2 *stats;         // (tokens / 64, rows): largest logit and the sum of exp of the distances from it
+    const int *targets;    // (rows)
+    float *target_logits;  // (rows), written where the target is
+    int vocabulary;
+};
+void launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s);
+
+// C (A.rows x B.rows, rows of ldc) = A B^T times row_factor[m] / divisor (+ C); rows of factor 0 are 0.
+struct HalvesProduct {
+    float *C;
+    int ldc;
+    const float *row_factor;  // or null for ones
+    float divisor;
+    bool add;
+};
+void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
+
+}  // namespace gptc

@@ -6,6 +6,7 @@
 // The rows go through in pieces, so that a piece's logits fit the scratch: its
 // logits are formed once, turned into d, and used for both gradients.
 #include <algorithm>
+#include "gemm_halves.hpp"
 #include "gemm_split.hpp"
 #include "gpu_kernels.h"
 #include "ops_common.hpp"
@@ -18,10 +19,16 @@ constexpr int kThreads = 256;
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int64_t kPieceFloats = 1ll << 27;  // logits of a piece
+constexpr int kHalvesRows = 128;             // from here on the operands are laid out first
 constexpr int kMaxVocabulary = 1 << 22;      // a product's tile offsets fit 32 bits
 
 __device__ __forceinline__ float weight_of(const float *weights, int row) {
     return weights != nullptr ? weights[row] : 1.0f;
+}
+
+// A target held in a float, truncated; -1 for what is not in [0, V).
+__device__ __forceinline__ int target_of(float f, int V) {
+    return f > -1.0f && f < static_cast<float>(V) ? static_cast<int>(f) : -1;
 }
 
 // One row a workgroup: its loss, and with `grad` its logits become d.
@@ -62,8 +69,7 @@ __global__ __launch_bounds__(kRowThreads) void loss_row_kernel(float *__restrict
 #pragma unroll
     for (int i = 1; i < kRowWaves; ++i) online_merge(m, s, sm[i], ss[i]);
     const float logsum = logf(s);
-    const float f = targets[row];
-    const int t = f > -1.0f && f < static_cast<float>(V) ? static_cast<int>(f) : -1;
+    const int t = target_of(targets[row], V);
     if (threadIdx.x == 0) losses[row] = t >= 0 ? logsum - (x[t] - m) : NAN;
     if (!grad) return;
     __syncthreads();  // the target's logit has been read
@@ -104,6 +110,216 @@ struct HeadLoss {
     int rows, V, C;
     bool add;
 };
+
+// ---- many rows: products of operands laid out as two fp16 parts ----
+
+// Targets as whole numbers, -1 where there is none; rows past the last one have none.
+__global__ __launch_bounds__(kThreads) void whole_targets_kernel(const float *__restrict__ targets,
+                                                                const float *__restrict__ weights,
+                                                                int *__restrict__ out, int rows, int padded, int V) {
+    const int r = blockIdx.x * kThreads + threadIdx.x;
+    if (r >= padded) return;
+    int t = -1;
+    if (r < rows && weight_of(weights, r) != 0.0f) t = target_of(targets[r], V);
+    out[r] = t;
+}
+
+// A row's loss and lse from the parts of its tokens: 32 rows a workgroup, whose 32
+// slices of the parts are joined in order.  Rows that take no part: lse is
+// infinite, which makes their shares 0.
+constexpr int kJoinThreads = 1024;
+__global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const float2 *__restrict__ stats, int parts,
+                                                                 const int *__restrict__ targets,
+                                                                 const float *__restrict__ target_logits,
+                                                                 const float *__restrict__ weights,
+                                                                 float *__restrict__ lse, float *__restrict__ losses,
+                                                                 int rows, int padded) {
+    __shared__ float2 red[32][33];
+    const int r = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + r;
+    const int per = (parts + 31) / 32, end = min(parts, (slice + 1) * per);
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll 4
+    for (int p = slice * per; p < end; ++p) {
+        const float2 v = stats[static_cast<int64_t>(p) * padded + row];
+        online_merge(m, s, v.x, v.y);
+    }
+    red[slice][r] = make_float2(m, s);
+    __syncthreads();
+    if (slice != 0) return;
+    for (int i = 1; i < 32; ++i) online_merge(m, s, red[i][r].x, red[i][r].y);
+    const bool live = row < rows && weight_of(weights, row) != 0.0f;
+    const float logsum = logf(s);
+    lse[row] = live ? m + logsum : INFINITY;
+    if (row < rows) losses[row] = !live ? 0.0f : targets[row] >= 0 ? logsum - (target_logits[row] - m) : NAN;
+}
+
+struct ShareArgs {
+    const float *logits, *lse;
+    const int *targets;
+    hu32x4 *d, *dt;  // as first operands of d W and d^T x; either may be null
+    int row_blocks, token_blocks;  // of the logits
+    int rows_used, tokens_used;    // blocks that the products' reductions reach
+};
+
+constexpr int kShareShift = 15;  // shares are held times 2^15
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr int kShareStride = 36;  // words of LDS a token: 16-byte rows, no two in the same banks
+constexpr int kShareTokens = 4;   // blocks of 32 tokens a wave
+
+// d' = exp(l - lse) - [target] of a block of 32 rows x 32 tokens, in two fp16 parts, as the
+// operand of either product.  The logits come in the order of the accumulators: a lane holds row
+// l % 32 and tokens 8 q + 4 (l / 32) + {0 .. 3}, which is also its share of d's block; d^T's goes
+// through LDS.  Memory bound: 4 bytes in, 8 out.
+__global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
+    __shared__ uint32_t lds[4][32 * kShareStride];
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rb = blockIdx.y;
+    const int first = (blockIdx.x * 4 + w) * kShareTokens;
+    const int row = rb * 32 + l32;
+    const float lse = a.lse[row];
+    const int target = a.targets[row];
+    uint32_t *mine = lds[w];
+    for (int jb = first; jb < min(first + kShareTokens, a.token_blocks); ++jb) {
+        const f32x4_t *x = reinterpret_cast<const f32x4_t *>(a.logits) +
+                           (static_cast<int64_t>(rb) * a.token_blocks + jb) * 256 + lane;
+        f32x4_t v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = x[q * 64];
+        uint32_t high[4][2], low[4][2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f((v[q][e] - lse) * kLog2eF);
+                d[e] = (p - (jb * 32 + 8 * q + 4 * hf + e == target ? 1.0f : 0.0f)) *
+                       static_cast<float>(1 << kShareShift);
+            }
+            halves_split(d[0], d[1], high[q][0], low[q][0]);
+            halves_split(d[2], d[3], high[q][1], low[q][1]);
+        }
+        if (a.d != nullptr && jb < a.tokens_used) {
+            const uint32_t flip = jb & 1 ? 0x80008000u : 0;  // halves_negated
+            hu32x4 *out = a.d + (static_cast<int64_t>(rb) * a.tokens_used + jb) * 256 + lane;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                out[(2 * k) * 64] = hu32x4{high[2 * k][0], high[2 * k][1], high[2 * k + 1][0], high[2 * k + 1][1]} ^ flip;
+                out[(2 * k + 1) * 64] = hu32x4{low[2 * k][0], low[2 * k][1], low[2 * k + 1][0], low[2 * k + 1][1]} ^ flip;
+            }
+        }
+        if (a.dt == nullptr || rb >= a.rows_used) continue;
+        const uint32_t flip = rb & 1 ? 0x80008000u : 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t *at = mine + (8 * q + 4 * hf + 2 * e) * kShareStride + l32;
+                at[0] = ((high[q][e] & 0xffffu) | (low[q][e] << 16)) ^ flip;
+                at[kShareStride] = ((high[q][e] >> 16) | (low[q][e] & 0xffff0000u)) ^ flip;
+            }
+        wave_lds_order();
+        hu32x4 *out = a.dt + (static_cast<int64_t>(jb) * a.rows_used + rb) * 256 + lane;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const hu32x4 *at = reinterpret_cast<const hu32x4 *>(mine + l32 * kShareStride + 16 * k + 4 * hf);
+            const hu32x4 one = at[0], two = at[2];
+            const uint32_t word[8] = {one[0], one[1], one[2], one[3], two[0], two[1], two[2], two[3]};
+            hu32x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi[e] = (word[2 * e] & 0xffffu) | (word[2 * e + 1] << 16);
+                lo[e] = (word[2 * e] >> 16) | (word[2 * e + 1] & 0xffff0000u);
+            }
+            out[(2 * k) * 64] = hi;
+            out[(2 * k + 1) * 64] = lo;
+        }
+        wave_lds_order();
+    }
+}
+
+// Blocks of the pool for the length of a call.
+struct Scratch {
+    static constexpr int kMax = 24;
+    void *blocks[kMax];
+    int n = 0;
+    template <typename T>
+    T *take(int64_t count) {
+        CHECK_ERROR(n == kMax, "Too many blocks of scratch.");
+        blocks[n] = alloc_cuda(static_cast<size_t>(std::max<int64_t>(count, 1)) * sizeof(T));
+        return static_cast<T *>(blocks[n++]);
+    }
+    Halves halves(int rows, int terms) {
+        Halves h{nullptr, nullptr, 0, rows, terms};
+        h.data = take<hu32x4>(h.bytes() / 16);
+        h.shift = take<int>(h.row_blocks() * 32);
+        return h;
+    }
+    void release() {
+        while (n > 0) free_cuda(blocks[--n]);
+    }
+};
+
+constexpr int64_t kPieceBytes = 5ll << 28;  // logits, d and d^T of a piece
+constexpr int kLossPiece = 16384;           // rows of a piece whose logits are not written
+
+void run_halves(const HeadLoss &h, hipStream_t s) {
+    const bool grad = h.dx != nullptr || h.dW != nullptr;
+    const int tokens = (h.V + 127) / 128 * 128;
+    const int64_t fit = std::max<int64_t>(1, kPieceBytes / (12ll * tokens) / 128) * 128;
+    const int piece = static_cast<int>(std::min<int64_t>(h.rows, grad ? fit : kLossPiece));
+    const int padded = (piece + 127) / 128 * 128;
+    Scratch scratch;
+    const Halves W = scratch.halves(h.V, h.C);
+    launch_halves_rows(h.W, h.C, nullptr, W, true, s);
+    uint32_t *largest = scratch.take<uint32_t>(h.C);
+    Halves Wt{};
+    if (h.dx != nullptr) {
+        Wt = scratch.halves(h.C, h.V);
+        launch_halves_columns(h.W, h.C, nullptr, 1.0f, Wt, largest, s);
+    }
+    Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V},
+           dt{nullptr, nullptr, kShareShift, h.V, piece};
+    if (h.dW != nullptr) {
+        xt = scratch.halves(h.C, piece);
+        dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
+    }
+    if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / 16);
+    float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
+    float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 64));
+    int *targets = scratch.take<int>(padded);
+    float *target_logits = scratch.take<float>(padded), *lse = scratch.take<float>(padded);
+    for (int r = 0; r < h.rows; r += piece) {
+        const int n = std::min(piece, h.rows - r), n_padded = (n + 127) / 128 * 128;
+        const float *xr = h.x + static_cast<int64_t>(r) * h.C;
+        const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
+        x.rows = d.rows = xt.terms = dt.terms = n;
+        launch_halves_rows(xr, h.C, weights, x, false, s);
+        whole_targets_kernel<<<dim3((n_padded + kThreads - 1) / kThreads), dim3(kThreads), 0, s>>>(
+            h.targets + r, weights, targets, n, n_padded, h.V);
+        hipCheck(hipGetLastError());
+        launch_logits(W, x, {logits, stats, targets, target_logits, h.V}, s);
+        join_stats_kernel<<<dim3(n_padded / 32), dim3(kJoinThreads), 0, s>>>(
+            stats, tokens / 64, targets, target_logits, weights, lse, h.losses + r, n, n_padded);
+        hipCheck(hipGetLastError());
+        if (!grad) continue;
+        const ShareArgs a{logits, lse, targets, d.data, dt.data, n_padded / 32, tokens / 32, (n + 31) / 32, (h.V + 31) / 32};
+        shares_kernel<<<dim3((a.token_blocks + 4 * kShareTokens - 1) / (4 * kShareTokens), a.row_blocks),
+                        dim3(kThreads), 0, s>>>(a);
+        hipCheck(hipGetLastError());
+        if (h.dx != nullptr)
+            launch_halves_product(d, Wt, {h.dx + static_cast<int64_t>(r) * h.C, h.C, weights,
+                                          static_cast<float>(h.rows), false},
+                                  s);
+        if (h.dW != nullptr) {
+            launch_halves_columns(xr, h.C, weights, static_cast<float>(h.rows), xt, largest, s);
+            launch_halves_product(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
+        }
+    }
+    scratch.release();
+}
+
+// ---- few rows: products that split the floats as they come ----
 
 void run_pieces(const HeadLoss &h, hipStream_t s) {
     const bool grad = h.dx != nullptr || h.dW != nullptr;
@@ -189,9 +405,12 @@ extern "C" void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t
     CHECK_ERROR(gptc_stream_capturing(), "gptc_linear_cross_entropy_cuda takes scratch: not under graph capture.");
     hipStream_t s = gptc_stream_checked();
     float *losses = row_losses != NULL ? row_losses->t : static_cast<float *>(alloc_cuda(sizeof(float) * rows));
-    run_pieces({x->t, W->t, targets->t, weights != NULL ? weights->t : nullptr, losses, dx != NULL ? dx->t : nullptr,
-                dW != NULL ? dW->t : nullptr, rows, V, C, accumulate != 0},
-               s);
+    const HeadLoss h{x->t, W->t, targets->t, weights != NULL ? weights->t : nullptr, losses, dx != NULL ? dx->t : nullptr,
+                     dW != NULL ? dW->t : nullptr, rows, V, C, accumulate != 0};
+    if (rows >= kHalvesRows)
+        run_halves(h, s);
+    else
+        run_pieces(h, s);
     mean_loss_kernel<<<dim3(1), dim3(kThreads), 0, s>>>(losses, weights != NULL ? weights->t : nullptr, output->t, rows);
     hipCheck(hipGetLastError());
     if (row_losses == NULL) free_cuda(losses);

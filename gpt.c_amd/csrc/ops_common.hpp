@@ -32,6 +32,13 @@ __device__ __forceinline__ void wave_online(float &m, float &s) {
     }
 }
 
+// A wave's own LDS accesses are done in order; this keeps the compiler's order.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Workgroups for a grid-stride loop over `work` items of `per_block` each,
 // capped at 8 workgroups per CU of a 256-CU MI355X.
 inline int blocks_for(int64_t work, int64_t per_block) {
