@@ -11,6 +11,7 @@
 // kernel adds these in the order of their places.  So sums depend on the ids
 // alone (no float atomics), and a token that fills the batch is shared by all
 // waves.
+#include <algorithm>
 #include "gpu_kernels.h"
 #include "ops_common.hpp"
 
@@ -67,39 +68,75 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const T *__restrict__ 
 }
 
 // ---- sorting ----
+// The sort's launches are short and mostly wait; where dW is to be overwritten, further workgroups of
+// the same launches clear it meanwhile (8192 rows of 768 on 50257: 25 us beside the ranking's 13).
+struct Clear {
+    f32x4_t *at;  // n of them from here on, by the workgroups after the first `blocks` of a launch
+    int64_t n;
+    int blocks;
+};
+
+__device__ __forceinline__ void clear_part(const Clear &c) {
+    const int64_t stride = static_cast<int64_t>(gridDim.x - c.blocks) * blockDim.x;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - c.blocks) * blockDim.x + threadIdx.x; i < c.n; i += stride)
+        c.at[i] = splat<f32x4_t>(0.0f);
+}
+
+// Workgroups for a part: eight waves a CU.
+int clear_blocks(const Clear &c, int threads) {
+    return static_cast<int>(std::min<int64_t>((c.n + threads - 1) / threads, 256 * 512 / threads));
+}
+
 // order[r] = (key, row) of the r-th row by (key, row); key: the id, V for rows
 // without one.
 
 // Up to kRankRows rows: a row's place is the number of rows before it, counted
-// by comparing it with all of them.  One launch; 8192 rows are 67 million
-// comparisons, 4 us of the chip, about what one of the six launches of the
-// digit passes below takes.
+// by comparing it with all of them, in one launch.
 constexpr int kRankRows = 12288;
 constexpr int kRankThreads = 512;
 constexpr int kRankPer = 32;  // rows a workgroup
 constexpr int kRankSlices = kRankThreads / kRankPer;
 
 __global__ __launch_bounds__(kRankThreads) void rank_kernel(const float *__restrict__ ids, int n, int V,
-                                                           int2 *__restrict__ order) {
+                                                           int2 *__restrict__ order, Clear clear) {
+    if (static_cast<int>(blockIdx.x) >= clear.blocks) {
+        clear_part(clear);
+        return;
+    }
     extern __shared__ uint32_t keys[];  // all rows, padded to slices of whole 16 bytes with keys past all others
     __shared__ int count[kRankPer];
     const int per = ((n + kRankSlices - 1) / kRankSlices + 3) & ~3;  // rows a slice
-    for (int j = threadIdx.x; j < per * kRankSlices; j += kRankThreads) {
-        const int id = j < n ? id_of(ids[j], V) : 0;
-        keys[j] = j >= n ? 0xffffffffu : id < 0 ? static_cast<uint32_t>(V) : static_cast<uint32_t>(id);
+    for (int j0 = threadIdx.x; j0 < per * kRankSlices; j0 += 8 * kRankThreads) {
+        float id[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) id[k] = ids[min(j0 + k * kRankThreads, n - 1)];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int j = j0 + k * kRankThreads;
+            if (j >= per * kRankSlices) break;
+            const int key = id_of(id[k], V);
+            keys[j] = j >= n ? 0xffffffffu : key < 0 ? static_cast<uint32_t>(V) : static_cast<uint32_t>(key);
+        }
     }
     if (threadIdx.x < kRankPer) count[threadIdx.x] = 0;
     __syncthreads();
-    const int i = blockIdx.x * kRankPer + static_cast<int>(threadIdx.x % kRankPer);
+    const int i0 = blockIdx.x * kRankPer, i = i0 + static_cast<int>(threadIdx.x % kRankPer);
     const int first = (threadIdx.x / kRankPer) * per;
     if (i < n) {
         const uint32_t key = keys[i];
         int before = 0;
-        // Rows of this key count up to row i: key + 1 is the bound there, key after it.
-        for (int j = first; j < first + per; j += 4) {
+        // Rows of this key count up to row i.  Before the workgroup's rows all of them do, behind them none.
+        const int upto = max(first, min(first + per, i0 & ~3)), from = max(first, min(first + per, i0 + kRankPer));
+#pragma unroll 4
+        for (int j = first; j < upto; j += 4) {
             const uint4 k = *reinterpret_cast<const uint4 *>(keys + j);
-            before += (k.x < key + (j < i)) + (k.y < key + (j + 1 < i)) + (k.z < key + (j + 2 < i)) +
-                      (k.w < key + (j + 3 < i));
+            before += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+        }
+        for (int j = upto; j < from; ++j) before += keys[j] < key + (j < i);
+#pragma unroll 4
+        for (int j = from; j < first + per; j += 4) {
+            const uint4 k = *reinterpret_cast<const uint4 *>(keys + j);
+            before += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
         }
         atomicAdd(&count[threadIdx.x % kRankPer], before);  // whole numbers: in any order the same
     }
@@ -121,6 +158,7 @@ struct SortArgs {
     int2 *out;
     int *hist;  // digit-major: (kDigits, blocks)
     int n, V, shift, blocks;
+    Clear clear;
 };
 
 __device__ __forceinline__ int2 sort_item(const SortArgs &a, int i) {
@@ -130,24 +168,37 @@ __device__ __forceinline__ int2 sort_item(const SortArgs &a, int i) {
 }
 
 __global__ __launch_bounds__(kSortThreads) void digit_count_kernel(const SortArgs a) {
+    if (static_cast<int>(blockIdx.x) >= a.blocks) {
+        clear_part(a.clear);
+        return;
+    }
     __shared__ int count[kDigits];
     count[threadIdx.x] = 0;
     __syncthreads();
-    for (int t = 0; t < kSortItems; ++t) {
-        const int i = blockIdx.x * kSortBlock + t * kSortThreads + threadIdx.x;
-        if (i < a.n) atomicAdd(&count[(sort_item(a, i).x >> a.shift) & (kDigits - 1)], 1);
-    }
+    int key[kSortItems];
+#pragma unroll
+    for (int t = 0; t < kSortItems; ++t)
+        key[t] = sort_item(a, min(blockIdx.x * kSortBlock + t * kSortThreads + static_cast<int>(threadIdx.x), a.n - 1)).x;
+#pragma unroll
+    for (int t = 0; t < kSortItems; ++t)
+        if (static_cast<int>(blockIdx.x * kSortBlock + t * kSortThreads + threadIdx.x) < a.n)
+            atomicAdd(&count[(key[t] >> a.shift) & (kDigits - 1)], 1);
     __syncthreads();
     a.hist[threadIdx.x * a.blocks + blockIdx.x] = count[threadIdx.x];
 }
 
 // hist := its running sums, the entry itself left out; one workgroup.
 constexpr int kScanThreads = 1024;
-__global__ __launch_bounds__(kScanThreads) void digit_scan_kernel(int *hist, int n) {
+__global__ __launch_bounds__(kScanThreads) void digit_scan_kernel(int *hist, int n, Clear clear) {
+    if (blockIdx.x > 0) {
+        clear_part(clear);
+        return;
+    }
     __shared__ int part[kScanThreads];
     const int per = (n + kScanThreads - 1) / kScanThreads;
     const int lo = min(n, static_cast<int>(threadIdx.x) * per), hi = min(n, lo + per);
     int sum = 0;
+#pragma unroll 8
     for (int i = lo; i < hi; ++i) sum += hist[i];
     part[threadIdx.x] = sum;
     __syncthreads();
@@ -166,6 +217,10 @@ __global__ __launch_bounds__(kScanThreads) void digit_scan_kernel(int *hist, int
 }
 
 __global__ __launch_bounds__(kSortThreads) void digit_move_kernel(const SortArgs a) {
+    if (static_cast<int>(blockIdx.x) >= a.blocks) {
+        clear_part(a.clear);
+        return;
+    }
     constexpr int kW = kSortThreads / kWave;
     __shared__ int at[kW][kDigits];  // where a wave's next row of a digit goes
     const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
@@ -225,12 +280,47 @@ struct GatherArgs {
     float scale;
     int n, V, C, chunk, blocks;  // blocks: of columns
     bool add;
+    float *dP;  // or null
+    int seqs, seq, positions;
 };
+
+// dP[t] (+)= the sequences' rows t, in their order; rows past the sequences' length: 0.  By the workgroups
+// after the first `before` of a launch.
+template <typename T>
+__device__ __forceinline__ void position_sums(const GatherArgs &a, int before) {
+    const int cols = a.C / (sizeof(T) / sizeof(float));
+    const int64_t n = static_cast<int64_t>(a.seq) * cols, total = static_cast<int64_t>(a.positions) * cols;
+    const int64_t stride = static_cast<int64_t>(gridDim.x - before) * kThreads;
+    const T *g = reinterpret_cast<const T *>(a.g);
+    T *dP = reinterpret_cast<T *>(a.dP);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - before) * kThreads + threadIdx.x; i < total; i += stride) {
+        T sum = splat<T>(0.0f);
+        if (i < n) {
+            int b = 0;
+            for (; b + 8 <= a.seqs; b += 8) {
+                T v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = g[(b + k) * n + i];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += v[k];
+            }
+            for (; b < a.seqs; ++b) sum += g[b * n + i];
+        } else if (a.add) {
+            return;
+        }
+        dP[i] = a.add ? dP[i] + sum : sum;
+    }
+}
 
 // One wave: `chunk` sorted places x 64 columns in units of T.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void gather_kernel(const GatherArgs a, int items) {
     constexpr int kAhead = 8;  // rows whose loads are on their way together
+    const int gather_blocks = (items + kWaves - 1) / kWaves;
+    if (static_cast<int>(blockIdx.x) >= gather_blocks) {
+        position_sums<T>(a, gather_blocks);
+        return;
+    }
     const int lane = threadIdx.x & (kWave - 1);
     const int item = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (item >= items) return;
@@ -299,16 +389,20 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const GatherArgs a) {
     const int last = min(p0 + a.chunk, a.n) - 1;
     // Goes on behind this chunk: a later workgroup's.
     if (a.order[last].x == key && last + 1 < a.n && a.order[last + 1].x == key) return;
-    int lo = 0, hi = p0 - 1;  // the run's first place
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.order[mid].x < key)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    const int first = lo / a.chunk, count = chunk - first, per = (count + kWaves - 1) / kWaves;
     const int lane = threadIdx.x & (kWave - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    int first = chunk - 1;  // the run's first chunk: back from here while chunks start with this key, 64 at a time
+    for (;;) {
+        const int c = first - lane;
+        const bool same = c > 0 && a.order[c * static_cast<int64_t>(a.chunk)].x == key &&
+                          a.order[c * static_cast<int64_t>(a.chunk) - 1].x == key;
+        const uint64_t others = __ballot(!same);
+        if (others != 0) {
+            first -= __builtin_ctzll(others);
+            break;
+        }
+        first -= kWave;
+    }
+    const int count = chunk - first, per = (count + kWaves - 1) / kWaves;
     const int cols = a.C / (sizeof(T) / sizeof(float)), col = blockIdx.y * kWave + lane;
     const bool on = col < cols;
     const T *part = reinterpret_cast<const T *>(a.part);
@@ -335,43 +429,19 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const GatherArgs a) {
     *at = a.add ? fma_of(a.scale, sum, *at) : a.scale * sum;
 }
 
-// dP[t] (+)= the sequences' rows t, in their order; rows past the sequences' length: 0.  n: seq * cols.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void position_kernel(const T *__restrict__ g, T *dP, int seqs, int64_t n,
-                                                           int64_t total, bool add) {
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total; i += stride) {
-        T sum = splat<T>(0.0f);
-        if (i < n) {
-            int b = 0;
-            for (; b + 8 <= seqs; b += 8) {
-                T v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = g[(b + k) * n + i];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum += v[k];
-            }
-            for (; b < seqs; ++b) sum += g[b * n + i];
-        } else if (add) {
-            return;
-        }
-        dP[i] = add ? dP[i] + sum : sum;
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void clear_kernel(T *p, int64_t n) {
+__global__ __launch_bounds__(kThreads) void clear_kernel(float *p, int64_t n) {
     const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
     for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n; i += stride)
-        p[i] = splat<T>(0.0f);
+        p[i] = 0.0f;
 }
 
-// The rows sorted by (id, row); scratch is taken from the pool and returned by the caller.
-void launch_sort(const float *ids, int n, int V, int2 *order, hipStream_t s) {
+// The rows sorted by (id, row); `clear`, if it has any, is zeroed on the way.
+void launch_sort(const float *ids, int n, int V, int2 *order, Clear clear, hipStream_t s) {
     if (n <= kRankRows) {
         const int per = ((n + kRankSlices - 1) / kRankSlices + 3) & ~3;
-        rank_kernel<<<dim3((n + kRankPer - 1) / kRankPer), dim3(kRankThreads),
-                      static_cast<size_t>(per) * kRankSlices * sizeof(uint32_t), s>>>(ids, n, V, order);
+        clear.blocks = (n + kRankPer - 1) / kRankPer;
+        rank_kernel<<<dim3(clear.blocks + clear_blocks(clear, kRankThreads)), dim3(kRankThreads),
+                      static_cast<size_t>(per) * kRankSlices * sizeof(uint32_t), s>>>(ids, n, V, order, clear);
         hipCheck(hipGetLastError());
         return;
     }
@@ -380,13 +450,23 @@ void launch_sort(const float *ids, int n, int V, int2 *order, hipStream_t s) {
     const int blocks = (n + kSortBlock - 1) / kSortBlock;
     int2 *other = static_cast<int2 *>(alloc_cuda(sizeof(int2) * static_cast<size_t>(n)));
     int *hist = static_cast<int *>(alloc_cuda(sizeof(int) * kDigits * static_cast<size_t>(blocks)));
-    SortArgs a{ids, nullptr, passes & 1 ? order : other, hist, n, V, 0, blocks};
+    const int64_t share = (clear.n + 3 * passes - 1) / (3 * passes);  // an equal part with every launch
+    int64_t left = clear.n;
+    auto part = [&](int before) {
+        const Clear c{clear.at + (clear.n - left), std::min(left, share), before};
+        left -= c.n;
+        return c;
+    };
+    SortArgs a{ids, nullptr, passes & 1 ? order : other, hist, n, V, 0, blocks, {}};
     for (int p = 0; p < passes; ++p) {
-        digit_count_kernel<<<dim3(blocks), dim3(kSortThreads), 0, s>>>(a);
+        a.clear = part(blocks);
+        digit_count_kernel<<<dim3(blocks + clear_blocks(a.clear, kSortThreads)), dim3(kSortThreads), 0, s>>>(a);
         hipCheck(hipGetLastError());
-        digit_scan_kernel<<<dim3(1), dim3(kScanThreads), 0, s>>>(hist, kDigits * blocks);
+        const Clear c = part(1);
+        digit_scan_kernel<<<dim3(1 + clear_blocks(c, kScanThreads)), dim3(kScanThreads), 0, s>>>(hist, kDigits * blocks, c);
         hipCheck(hipGetLastError());
-        digit_move_kernel<<<dim3(blocks), dim3(kSortThreads), 0, s>>>(a);
+        a.clear = part(blocks);
+        digit_move_kernel<<<dim3(blocks + clear_blocks(a.clear, kSortThreads)), dim3(kSortThreads), 0, s>>>(a);
         hipCheck(hipGetLastError());
         a.ids = nullptr;
         a.in = a.out;
@@ -398,7 +478,7 @@ void launch_sort(const float *ids, int n, int V, int2 *order, hipStream_t s) {
 }
 
 template <typename T>
-void launch_gather(const float *ids, GatherArgs a, float *dP, int seqs, int64_t seq, int64_t positions, hipStream_t s) {
+void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
     constexpr int kW = sizeof(T) / sizeof(float);
     const int cols = a.C / kW;
     a.blocks = (cols + kWave - 1) / kWave;
@@ -407,27 +487,27 @@ void launch_gather(const float *ids, GatherArgs a, float *dP, int seqs, int64_t 
     while (a.chunk > 8 && static_cast<int64_t>(a.n) * a.blocks < 2048ll * a.chunk) a.chunk /= 2;
     const int chunks = (a.n + a.chunk - 1) / a.chunk;
     const int64_t items = static_cast<int64_t>(chunks) * a.blocks;
-    CHECK_ERROR(items > INT32_MAX - kWaves, "Too many rows and columns for one call: %d x %d.", a.n, a.C);
+    CHECK_ERROR(items > INT32_MAX / 2, "Too many rows and columns for one call: %d x %d.", a.n, a.C);
     int2 *order = static_cast<int2 *>(alloc_cuda(sizeof(int2) * static_cast<size_t>(a.n)));
     a.part = static_cast<float *>(alloc_cuda(sizeof(float) * 2 * static_cast<size_t>(chunks) * a.C));
     a.order = order;
+    Clear clear{nullptr, 0, 0};
     if (!a.add) {
-        const int64_t n = static_cast<int64_t>(a.V) * cols;
-        clear_kernel<T><<<dim3(blocks_for(n, kThreads)), dim3(kThreads), 0, s>>>(reinterpret_cast<T *>(a.dW), n);
-        hipCheck(hipGetLastError());
+        const int64_t n = static_cast<int64_t>(a.V) * a.C;
+        if (aligned16(a.dW)) clear = {reinterpret_cast<f32x4_t *>(a.dW), n / 4, 0};
+        const int64_t rest = n - 4 * clear.n;
+        if (rest > 0) {
+            clear_kernel<<<dim3(blocks_for(rest, kThreads)), dim3(kThreads), 0, s>>>(a.dW + 4 * clear.n, rest);
+            hipCheck(hipGetLastError());
+        }
     }
-    launch_sort(ids, a.n, a.V, order, s);
-    gather_kernel<T><<<dim3(static_cast<unsigned>((items + kWaves - 1) / kWaves)), dim3(kThreads), 0, s>>>(
-        a, static_cast<int>(items));
+    launch_sort(ids, a.n, a.V, order, clear, s);
+    const int gather_blocks = static_cast<int>((items + kWaves - 1) / kWaves);
+    const int extra = a.dP != nullptr ? blocks_for(static_cast<int64_t>(a.positions) * cols, kThreads) : 0;
+    gather_kernel<T><<<dim3(gather_blocks + extra), dim3(kThreads), 0, s>>>(a, static_cast<int>(items));
     hipCheck(hipGetLastError());
     if (chunks > 1) {
         join_kernel<T><<<dim3(chunks - 1, a.blocks), dim3(kThreads), 0, s>>>(a);
-        hipCheck(hipGetLastError());
-    }
-    if (dP != nullptr) {
-        const int64_t n = seq * cols, total = positions * cols;
-        position_kernel<T><<<dim3(blocks_for(total, kThreads)), dim3(kThreads), 0, s>>>(
-            reinterpret_cast<const T *>(a.g), reinterpret_cast<T *>(dP), seqs, n, total, a.add);
         hipCheck(hipGetLastError());
     }
     free_cuda(a.part);
@@ -491,20 +571,20 @@ extern "C" void gptc_embedding_backward_sorted_cuda(const tensor_t *global_grad,
     const int V = dW->shape[0], C = dW->shape[1];
     if (n == 0) {
         if (accumulate) return;
-        clear_kernel<float><<<dim3(blocks_for(dW->length, kThreads)), dim3(kThreads), 0, s>>>(dW->t, dW->length);
+        clear_kernel<<<dim3(blocks_for(dW->length, kThreads)), dim3(kThreads), 0, s>>>(dW->t, dW->length);
         hipCheck(hipGetLastError());
         if (dpos != NULL && dpos->length > 0) {
-            clear_kernel<float><<<dim3(blocks_for(dpos->length, kThreads)), dim3(kThreads), 0, s>>>(dpos->t,
+            clear_kernel<<<dim3(blocks_for(dpos->length, kThreads)), dim3(kThreads), 0, s>>>(dpos->t,
                                                                                                   dpos->length);
             hipCheck(hipGetLastError());
         }
         return;
     }
-    const GatherArgs a{global_grad->t, nullptr, dW->t, nullptr, scale, n, V, C, 0, 0, accumulate != 0};
-    const int seq = last_dim(ids), positions = dpos != NULL ? dpos->shape[0] : 0;
-    float *dP = dpos != NULL ? dpos->t : nullptr;
-    if (C % 4 == 0 && aligned16(global_grad->t) && aligned16(dW->t) && (dP == nullptr || aligned16(dP)))
-        launch_gather<f32x4_t>(ids->t, a, dP, n / seq, seq, positions, s);
+    const int seq = last_dim(ids);
+    const GatherArgs a{global_grad->t, nullptr, dW->t, nullptr, scale, n, V, C, 0, 0, accumulate != 0,
+                       dpos != NULL ? dpos->t : nullptr, n / seq, seq, dpos != NULL ? dpos->shape[0] : 0};
+    if (C % 4 == 0 && aligned16(a.g) && aligned16(a.dW) && aligned16(a.dP))
+        launch_gather<f32x4_t>(ids->t, a, s);
     else
-        launch_gather<float>(ids->t, a, dP, n / seq, seq, positions, s);
+        launch_gather<float>(ids->t, a, s);
 }

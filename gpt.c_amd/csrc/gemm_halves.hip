@@ -50,11 +50,13 @@ __global__ __launch_bounds__(kThreads) void halves_rows_kernel(const float *__re
         float m = 0.0f;
         if (live) {
             if (vec) {
+#pragma unroll 8
                 for (int k = 4 * (tid & 7); k < h.terms; k += 32) {
                     const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p + k);
                     m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
                 }
             } else {
+#pragma unroll 8
                 for (int k = tid & 7; k < h.terms; k += 8) m = fmaxf(m, fabsf(p[k]));
             }
         }
@@ -72,6 +74,7 @@ __global__ __launch_bounds__(kThreads) void halves_rows_kernel(const float *__re
     const float *p = x + static_cast<int64_t>(live ? row : 0) * ld;
     const int up = shift[lane & 31];
     hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs * 2) * 64 + lane;
+#pragma unroll 4
     for (int kb = w; kb < kbs; kb += 4) {
         const int k0 = kb * 16 + 4 * hf;
         float v[8];
@@ -110,23 +113,44 @@ __device__ __forceinline__ float term_factor(const float *weights, float divisor
     return weights != nullptr ? weights[k] / divisor : 1.0f / divisor;
 }
 
-constexpr int kColumnTerms = 128;  // terms a workgroup
+constexpr int kLargestTerms = 64;  // terms a workgroup
 
 // largest[c] = bits of the largest magnitude of column c so far (whole numbers: in any order the same).
+// A workgroup: 64 columns in units of T, its waves take the terms in turns.
+template <typename T>
 __global__ __launch_bounds__(kThreads) void column_largest_kernel(const float *__restrict__ x, int ld,
                                                                  const float *__restrict__ weights, float divisor,
                                                                  int terms, int cols, uint32_t *largest) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
-    const int k0 = blockIdx.y * kColumnTerms, k1 = min(terms, k0 + kColumnTerms);
-    float m = 0.0f;
+    constexpr int kW = sizeof(T) / sizeof(float);
+    __shared__ uint32_t red[64 * kW];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int c = (blockIdx.x * 64 + lane) * kW;
+    for (int i = threadIdx.x; i < 64 * kW; i += kThreads) red[i] = 0;
+    __syncthreads();
+    if (c < cols) {
+        float m[kW];
+#pragma unroll
+        for (int e = 0; e < kW; ++e) m[e] = 0.0f;
+        const int k1 = min(terms, static_cast<int>(blockIdx.y + 1) * kLargestTerms);
 #pragma unroll 8
-    for (int k = k0; k < k1; ++k) {
-        const float f = term_factor(weights, divisor, k);
-        if (f != 0.0f) m = fmaxf(m, fabsf(f * x[static_cast<int64_t>(k) * ld + c]));
+        for (int k = blockIdx.y * kLargestTerms + w; k < k1; k += 4) {
+            const T v = *reinterpret_cast<const T *>(x + static_cast<int64_t>(k) * ld + c);
+            const float f = term_factor(weights, divisor, k);
+#pragma unroll
+            for (int e = 0; e < kW; ++e)
+                if (f != 0.0f) m[e] = fmaxf(m[e], fabsf(f * reinterpret_cast<const float *>(&v)[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < kW; ++e) atomicMax(&red[lane * kW + e], __float_as_uint(m[e]));
     }
-    atomicMax(largest + c, __float_as_uint(m));
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * kW; i += kThreads) {
+        const int at = blockIdx.x * 64 * kW + i;
+        if (at < cols && red[i] != 0) atomicMax(largest + at, red[i]);
+    }
 }
+
+constexpr int kColumnTerms = 128;  // terms a workgroup
 
 // A wave: 32 columns, kColumnTerms / 4 terms.
 __global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *__restrict__ x, int ld,
@@ -318,7 +342,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     for (int j = 0; j < 2; ++j) {
         const int row = row0 + 32 * j + l32;
         const int up = shift_of(t.shift_b, t.all_b, row);
-        const int target = l.targets[row];
+        const int target = row < l.rows ? token_of(l.targets[row], l.vocabulary) : -1;
         float m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -433,15 +457,27 @@ void launch_halves_rows(const float *x, int ld, const float *weights, const Halv
     hipCheck(hipGetLastError());
 }
 
+void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,
+                           uint32_t *largest, hipStream_t s) {
+    const int chunks = (terms + kLargestTerms - 1) / kLargestTerms;
+    if (ld % 4 == 0 && cols % 4 == 0 && aligned16(x))
+        column_largest_kernel<f32x4_t><<<dim3((cols + 255) / 256, chunks), dim3(kThreads), 0, s>>>(
+            x, ld, weights, divisor, terms, cols, largest);
+    else
+        column_largest_kernel<float><<<dim3((cols + 63) / 64, chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor,
+                                                                                              terms, cols, largest);
+    hipCheck(hipGetLastError());
+}
+
+void launch_zero_words(uint32_t *p, int n, hipStream_t s) {
+    zero_words_kernel<<<dim3((n + kThreads - 1) / kThreads), dim3(kThreads), 0, s>>>(p, n);
+    hipCheck(hipGetLastError());
+}
+
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
-                           uint32_t *scratch, hipStream_t s) {
-    zero_words_kernel<<<dim3((h.rows + kThreads - 1) / kThreads), dim3(kThreads), 0, s>>>(scratch, h.rows);
-    hipCheck(hipGetLastError());
+                           const uint32_t *largest, hipStream_t s) {
     const int chunks = (h.term_blocks() * 16 + kColumnTerms - 1) / kColumnTerms;
-    column_largest_kernel<<<dim3((h.rows + kThreads - 1) / kThreads, chunks), dim3(kThreads), 0, s>>>(
-        x, ld, weights, divisor, h.terms, h.rows, scratch);
-    hipCheck(hipGetLastError());
-    halves_columns_kernel<<<dim3(h.row_blocks(), chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor, h, scratch);
+    halves_columns_kernel<<<dim3(h.row_blocks(), chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor, h, largest);
     hipCheck(hipGetLastError());
 }
 

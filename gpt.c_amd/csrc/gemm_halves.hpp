@@ -56,17 +56,26 @@ __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 5) &
 // h.shift; negate: as a product's first operand.
 void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
-// as a second operand.  scratch: h.rows words.
+// as a second operand.  largest: the bits of each column's largest magnitude, which the first call raises
+// from what it holds (launch_zero_words) and which may count further terms too.
+void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,
+                           uint32_t *largest, hipStream_t s);
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
-                           uint32_t *scratch, hipStream_t s);
+                           const uint32_t *largest, hipStream_t s);
+void launch_zero_words(uint32_t *p, int n, hipStream_t s);
+
+// A token held in a float, truncated; -1 for what is not in [0, V).
+__device__ __forceinline__ int token_of(float f, int V) {
+    return f > -1.0f && f < static_cast<float>(V) ? static_cast<int>(f) : -1;
+}
 
 // The logits of a piece: A = W (vocabulary x features), B = x (rows x features).
 struct LogitsArgs {
     float *logits;         // blocks of 32 rows x 32 tokens in the order of the accumulators, or null
     float2 *stats;         // (tokens / 64, rows): largest logit and the sum of exp of the distances from it
-    const int *targets;    // (rows)
+    const float *targets;  // (rows)
     float *target_logits;  // (rows), written where the target is
-    int vocabulary;
+    int vocabulary, rows;
 };
 void launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s);
 

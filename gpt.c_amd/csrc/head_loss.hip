@@ -26,11 +26,6 @@ __device__ __forceinline__ float weight_of(const float *weights, int row) {
     return weights != nullptr ? weights[row] : 1.0f;
 }
 
-// A target held in a float, truncated; -1 for what is not in [0, V).
-__device__ __forceinline__ int target_of(float f, int V) {
-    return f > -1.0f && f < static_cast<float>(V) ? static_cast<int>(f) : -1;
-}
-
 // One row a workgroup: its loss, and with `grad` its logits become d.
 __global__ __launch_bounds__(kRowThreads) void loss_row_kernel(float *__restrict__ logits,
                                                               const float *__restrict__ targets,
@@ -69,7 +64,7 @@ __global__ __launch_bounds__(kRowThreads) void loss_row_kernel(float *__restrict
 #pragma unroll
     for (int i = 1; i < kRowWaves; ++i) online_merge(m, s, sm[i], ss[i]);
     const float logsum = logf(s);
-    const int t = target_of(targets[row], V);
+    const int t = token_of(targets[row], V);
     if (threadIdx.x == 0) losses[row] = t >= 0 ? logsum - (x[t] - m) : NAN;
     if (!grad) return;
     __syncthreads();  // the target's logit has been read
@@ -78,20 +73,22 @@ __global__ __launch_bounds__(kRowThreads) void loss_row_kernel(float *__restrict
 }
 
 // out[0] = sum of w[r] loss[r] / rows in a fixed order, in 64 bits.
-__global__ __launch_bounds__(kThreads) void mean_loss_kernel(const float *__restrict__ losses,
-                                                            const float *__restrict__ weights, float *__restrict__ out,
-                                                            int rows) {
-    __shared__ double part[kThreads];
+constexpr int kMeanThreads = 1024;
+__global__ __launch_bounds__(kMeanThreads) void mean_loss_kernel(const float *__restrict__ losses,
+                                                                const float *__restrict__ weights,
+                                                                float *__restrict__ out, int rows) {
+    __shared__ double part[kMeanThreads / kWave];
     double t = 0.0;
-    for (int r = threadIdx.x; r < rows; r += kThreads)
+#pragma unroll 8
+    for (int r = threadIdx.x; r < rows; r += kMeanThreads)
         t += static_cast<double>(losses[r]) * weight_of(weights, r);  // rows of weight 0: 0 * 0
-    part[threadIdx.x] = t;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) t += __shfl_xor(t, off, kWave);
+    if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = t;
     __syncthreads();
-    for (int off = kThreads / 2; off > 0; off >>= 1) {
-        if (static_cast<int>(threadIdx.x) < off) part[threadIdx.x] += part[threadIdx.x + off];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) out[0] = static_cast<float>(part[0] / rows);
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < kMeanThreads / kWave; ++i) t += part[i];
+    out[0] = static_cast<float>(t / rows);
 }
 
 // y = x with rows of weight 0 as zeros.
@@ -113,44 +110,48 @@ struct HeadLoss {
 
 // ---- many rows: products of operands laid out as two fp16 parts ----
 
-// Targets as whole numbers, -1 where there is none; rows past the last one have none.
-__global__ __launch_bounds__(kThreads) void whole_targets_kernel(const float *__restrict__ targets,
-                                                                const float *__restrict__ weights,
-                                                                int *__restrict__ out, int rows, int padded, int V) {
-    const int r = blockIdx.x * kThreads + threadIdx.x;
-    if (r >= padded) return;
-    int t = -1;
-    if (r < rows && weight_of(weights, r) != 0.0f) t = target_of(targets[r], V);
-    out[r] = t;
-}
-
-// A row's loss and lse from the parts of its tokens: 32 rows a workgroup, whose 32
-// slices of the parts are joined in order.  Rows that take no part: lse is
-// infinite, which makes their shares 0.
+// A row's loss, lse and target from the parts of its tokens: 32 rows a workgroup, whose
+// 32 slices of the parts are joined in order.  Rows that take no part, those past the
+// last one among them: lse is infinite, which makes their shares 0, and the target -1.
 constexpr int kJoinThreads = 1024;
 __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const float2 *__restrict__ stats, int parts,
-                                                                 const int *__restrict__ targets,
+                                                                 const float *__restrict__ targets,
                                                                  const float *__restrict__ target_logits,
                                                                  const float *__restrict__ weights,
-                                                                 float *__restrict__ lse, float *__restrict__ losses,
-                                                                 int rows, int padded) {
+                                                                 float *__restrict__ lse, int *__restrict__ whole,
+                                                                 float *__restrict__ losses, int rows, int padded,
+                                                                 int V) {
+    constexpr int kAhead = 8;
     __shared__ float2 red[32][33];
     const int r = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + r;
     const int per = (parts + 31) / 32, end = min(parts, (slice + 1) * per);
     float m = -INFINITY, s = 0.0f;
-#pragma unroll 4
-    for (int p = slice * per; p < end; ++p) {
-        const float2 v = stats[static_cast<int64_t>(p) * padded + row];
-        online_merge(m, s, v.x, v.y);
+    for (int p0 = slice * per; p0 < end; p0 += kAhead) {
+        float2 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            v[k] = stats[static_cast<int64_t>(min(p0 + k, end - 1)) * padded + row];
+            if (p0 + k >= end) v[k] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) top = fmaxf(top, v[k].x);
+        if (top == -INFINITY) continue;  // nothing but parts without a logit
+        s *= expf(m - top);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) s += v[k].y * expf(v[k].x - top);
+        m = top;
     }
     red[slice][r] = make_float2(m, s);
     __syncthreads();
     if (slice != 0) return;
     for (int i = 1; i < 32; ++i) online_merge(m, s, red[i][r].x, red[i][r].y);
     const bool live = row < rows && weight_of(weights, row) != 0.0f;
+    const int target = live ? token_of(targets[row], V) : -1;
     const float logsum = logf(s);
     lse[row] = live ? m + logsum : INFINITY;
-    if (row < rows) losses[row] = !live ? 0.0f : targets[row] >= 0 ? logsum - (target_logits[row] - m) : NAN;
+    whole[row] = target;
+    if (row < rows) losses[row] = !live ? 0.0f : target >= 0 ? logsum - (target_logits[row] - m) : NAN;
 }
 
 struct ShareArgs {
@@ -272,10 +273,13 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     Scratch scratch;
     const Halves W = scratch.halves(h.V, h.C);
     launch_halves_rows(h.W, h.C, nullptr, W, true, s);
-    uint32_t *largest = scratch.take<uint32_t>(h.C);
+    // The largest magnitudes of the columns of W and x.
+    uint32_t *largest = scratch.take<uint32_t>(2 * h.C), *largest_x = largest + h.C;
+    if (grad) launch_zero_words(largest, 2 * h.C, s);
     Halves Wt{};
     if (h.dx != nullptr) {
         Wt = scratch.halves(h.C, h.V);
+        launch_column_largest(h.W, h.C, nullptr, 1.0f, h.V, h.C, largest, s);
         launch_halves_columns(h.W, h.C, nullptr, 1.0f, Wt, largest, s);
     }
     Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V},
@@ -283,6 +287,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     if (h.dW != nullptr) {
         xt = scratch.halves(h.C, piece);
         dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
+        launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest_x, s);
     }
     if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / 16);
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
@@ -295,12 +300,9 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
         x.rows = d.rows = xt.terms = dt.terms = n;
         launch_halves_rows(xr, h.C, weights, x, false, s);
-        whole_targets_kernel<<<dim3((n_padded + kThreads - 1) / kThreads), dim3(kThreads), 0, s>>>(
-            h.targets + r, weights, targets, n, n_padded, h.V);
-        hipCheck(hipGetLastError());
-        launch_logits(W, x, {logits, stats, targets, target_logits, h.V}, s);
+        launch_logits(W, x, {logits, stats, h.targets + r, target_logits, h.V, n}, s);
         join_stats_kernel<<<dim3(n_padded / 32), dim3(kJoinThreads), 0, s>>>(
-            stats, tokens / 64, targets, target_logits, weights, lse, h.losses + r, n, n_padded);
+            stats, tokens / 64, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n, n_padded, h.V);
         hipCheck(hipGetLastError());
         if (!grad) continue;
         const ShareArgs a{logits, lse, targets, d.data, dt.data, n_padded / 32, tokens / 32, (n + 31) / 32, (h.V + 31) / 32};
@@ -312,7 +314,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
                                           static_cast<float>(h.rows), false},
                                   s);
         if (h.dW != nullptr) {
-            launch_halves_columns(xr, h.C, weights, static_cast<float>(h.rows), xt, largest, s);
+            launch_halves_columns(xr, h.C, weights, static_cast<float>(h.rows), xt, largest_x, s);
             launch_halves_product(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
         }
     }
@@ -411,7 +413,7 @@ extern "C" void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t
         run_halves(h, s);
     else
         run_pieces(h, s);
-    mean_loss_kernel<<<dim3(1), dim3(kThreads), 0, s>>>(losses, weights != NULL ? weights->t : nullptr, output->t, rows);
+    mean_loss_kernel<<<dim3(1), dim3(kMeanThreads), 0, s>>>(losses, weights != NULL ? weights->t : nullptr, output->t, rows);
     hipCheck(hipGetLastError());
     if (row_losses == NULL) free_cuda(losses);
 }
