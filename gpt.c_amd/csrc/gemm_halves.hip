@@ -27,7 +27,6 @@ namespace gptc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kStageBytes = 32768;
 
 __device__ __forceinline__ hf32x16 mfma(hu32x4 a, hu32x4 b, hf32x16 c) {
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -220,124 +219,133 @@ __device__ __forceinline__ void tile_of(const Tile &t, int &tm, int &tn) {
     tn = in / h;
 }
 
-__device__ __forceinline__ void load_stage(const hu32x4 *a, const hu32x4 *b, hu32x4 *lds, int w, int lane) {
-    using Global = const __attribute__((address_space(1))) void *;
-    using Shared = __attribute__((address_space(3))) void *;
-    const Global ga = (Global)(a + lane), gb = (Global)(b + lane);
-    const Shared la = (Shared)(lds + w * 256), lb = (Shared)(lds + 1024 + w * 256);
-    __builtin_amdgcn_global_load_lds(ga, la, 16, 0, 0);
-    __builtin_amdgcn_global_load_lds(ga, la, 16, 1024, 0);
-    __builtin_amdgcn_global_load_lds(ga, la, 16, 2048, 0);
-    __builtin_amdgcn_global_load_lds(ga, la, 16, 3072, 0);
-    __builtin_amdgcn_global_load_lds(gb, lb, 16, 0, 0);
-    __builtin_amdgcn_global_load_lds(gb, lb, 16, 1024, 0);
-    __builtin_amdgcn_global_load_lds(gb, lb, 16, 2048, 0);
-    __builtin_amdgcn_global_load_lds(gb, lb, 16, 3072, 0);
-}
-
-// A wave's fragments of a step: of either operand two blocks of 32 rows, two of 16 terms, two parts.
-struct Fragments {
-    hu32x4 a[2][2][2], b[2][2][2];
+// The workgroup's shapes: waves WM x WN, each forming 32 NI x 64 outputs.
+template <int WM_, int WN_, int NI_>
+struct Shape {
+    static constexpr int WM = WM_, WN = WN_, NI = NI_;
+    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+    static constexpr int BM = WM * NI * 32, BN = WN * 64;
+    static constexpr int kBlocks = (BM + BN) / 32;             // blocks of 32 rows of either operand, 4 KB a step each
+    static constexpr int kLoads = kBlocks / kWaves;            // of a wave
+    static constexpr int kStage = kBlocks * 4096;              // bytes
 };
 
-// The reads and their wait are one block, so no register is used before its data is there.
-__device__ __forceinline__ void read_stage(uint32_t at_a, uint32_t at_b, Fragments &f) {
+// Loads of 1 KB from `base` (and behind) to LDS at `to` (and behind).  They write no register; the
+// compiler does not count them, so its own waits wait for more than they need.
+__device__ __forceinline__ void load_block(const hu32x4 *base, uint32_t to, uint32_t lane16) {
     asm volatile(
-        "ds_read_b128 %0, %16\n\t"
-        "ds_read_b128 %1, %16 offset:1024\n\t"
-        "ds_read_b128 %2, %16 offset:2048\n\t"
-        "ds_read_b128 %3, %16 offset:3072\n\t"
-        "ds_read_b128 %8, %17\n\t"
-        "ds_read_b128 %9, %17 offset:1024\n\t"
-        "ds_read_b128 %10, %17 offset:2048\n\t"
-        "ds_read_b128 %11, %17 offset:3072\n\t"
-        "ds_read_b128 %4, %16 offset:4096\n\t"
-        "ds_read_b128 %5, %16 offset:5120\n\t"
-        "ds_read_b128 %6, %16 offset:6144\n\t"
-        "ds_read_b128 %7, %16 offset:7168\n\t"
-        "ds_read_b128 %12, %17 offset:4096\n\t"
-        "ds_read_b128 %13, %17 offset:5120\n\t"
-        "ds_read_b128 %14, %17 offset:6144\n\t"
-        "ds_read_b128 %15, %17 offset:7168\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(f.a[0][0][0]), "=&v"(f.a[0][0][1]), "=&v"(f.a[0][1][0]), "=&v"(f.a[0][1][1]), "=&v"(f.a[1][0][0]),
-          "=&v"(f.a[1][0][1]), "=&v"(f.a[1][1][0]), "=&v"(f.a[1][1][1]), "=&v"(f.b[0][0][0]), "=&v"(f.b[0][0][1]),
-          "=&v"(f.b[0][1][0]), "=&v"(f.b[0][1][1]), "=&v"(f.b[1][0][0]), "=&v"(f.b[1][0][1]), "=&v"(f.b[1][1][0]),
-          "=&v"(f.b[1][1][1])
-        : "v"(at_a), "v"(at_b)
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %1\n\t"
+        "global_load_lds_dwordx4 %0, %1 offset:1024\n\t"
+        "global_load_lds_dwordx4 %0, %1 offset:2048\n\t"
+        "global_load_lds_dwordx4 %0, %1 offset:3072"
+        :
+        : "v"(lane16), "s"(base), "s"(to)
         : "memory");
 }
 
-// acc = the wave's 64 x 64 outputs of tile (tm, tn) over this slice's terms, without the shifts.
+// acc = the wave's outputs of tile (tm, tn) over steps [s0, s1), without the shifts.
+template <class S>
 __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int s0, int s1, hu32x4 *lds,
-                                             hf32x16 (&acc)[2][2]) {
+                                             hf32x16 (&acc)[S::NI][2]) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Wave w loads the w-th block of rows of either operand: 4 KB each a step.
-    const hu32x4 *a = t.A + (static_cast<int64_t>(tm * 4 + w) * t.kbs + 2 * s0) * 128;
-    const hu32x4 *b = t.B + (static_cast<int64_t>(tn * 4 + w) * t.kbs + 2 * s0) * 128;
+    constexpr int kA = S::BM / 32, kB = S::BN / 32;
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) void *)lds));
-    const uint32_t at_a = base + (w >> 1) * 8192 + lane * 16, at_b = base + 16384 + (w & 1) * 8192 + lane * 16;
+    const uint32_t lane16 = lane * 16;
+    // Wave w loads blocks w kLoads .. of A's and B's rows.
+    const hu32x4 *from[S::kLoads];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < S::kLoads; ++i) {
+        const int block = w + i * S::kWaves;
+        const hu32x4 *p = block < kA ? t.A + static_cast<int64_t>(tm * kA + block) * t.kbs * 128
+                                     : t.B + static_cast<int64_t>(tn * kB + block - kA) * t.kbs * 128;
+        from[i] = p + s0 * 256;
+    }
+    // Past the last step the last one is loaded again, into a buffer that nobody reads any more: the
+    // loop needs no branch then, and its waits are the same in every step.
+    int next = s0;
+    auto load_stage = [&](uint32_t off) {
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i)
+            load_block(from[i], base + off + (w + i * S::kWaves) * 4096, lane16);
+        if (++next < s1) {
+#pragma unroll
+            for (int i = 0; i < S::kLoads; ++i) from[i] += 256;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < S::NI; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    load_stage(a, b, lds, w, lane);
-    if (s0 + 1 < s1) load_stage(a + 256, b + 256, lds + 2048, w, lane);
-    float sign = s0 & 1 ? -1.0f : 1.0f;
-    for (int s = s0; s < s1; ++s) {
-        const uint32_t off = (s - s0) & 1 ? kStageBytes : 0;
-        // This wave's loads of step s have landed (those of the next may be on their way), then all waves'.
-        if (s + 1 < s1)
-            asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        Fragments f;
-        read_stage(at_a + off, at_b + off, f);
-        asm volatile("s_barrier" ::: "memory");  // all waves have read this buffer
-        if (s + 2 < s1) load_stage(a + (s + 2 - s0) * 256, b + (s + 2 - s0) * 256, lds + (off >> 4), w, lane);
-        hf32x16 p[2][2];
+    load_stage(0);
+    load_stage(S::kStage);
+    const hu32x4 *at_a = lds + (w / S::WN) * S::NI * 256 + lane;
+    const hu32x4 *at_b = lds + (kA + (w % S::WN) * 2) * 256 + lane;
+    float sign = s0 & 2 ? -1.0f : 1.0f;
+    for (int s = s0; s < s1; s += 2) {
+        hf32x16 p[S::NI][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::NI; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p[i][j][r] = 0.0f;
-        constexpr int kProd[3][2] = {{1, 0}, {0, 1}, {0, 0}};
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
+        for (int half = 0; half < 2; ++half) {
+            const int off = half * (S::kStage / 16);
+            // This wave's loads of the step have landed (those of the next are on their way), then all waves'.
+            static_assert(S::kLoads == 2, "4 kLoads loads a step");
+            asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+            hu32x4 fb[2][2][2], fa[S::NI][2][2];  // blocks of 32 rows, of 16 terms, parts
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int i = 0; i < 8; ++i) fb[i >> 2][(i >> 1) & 1][i & 1] = at_b[off + i * 64];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 4 * S::NI; ++i) fa[i >> 2][(i >> 1) & 1][i & 1] = at_a[off + i * 64];
+            // All waves have read this buffer: the step after next goes there.
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            load_stage(half * S::kStage);
+            constexpr int kProd[3][2] = {{1, 0}, {0, 1}, {0, 0}};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) p[i][j] = mfma(f.a[i][k][kProd[q][0]], f.b[j][k][kProd[q][1]], p[i][j]);
+            for (int q = 0; q < 3; ++q)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < S::NI; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            p[i][j] = mfma(fa[i][k][kProd[q][0]], fb[j][k][kProd[q][1]], p[i][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < S::NI; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(sign, p[i][j][r], acc[i][j][r]);
         sign = -sign;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void logits_kernel(const Tile t,
-                                                                                                   const LogitsArgs l) {
-    __shared__ hu32x4 lds[2 * kStageBytes / 16];
+template <class S>
+__global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void logits_kernel(
+    const Tile t, const LogitsArgs l) {
+    __shared__ hu32x4 lds[2 * S::kStage / 16];
     int tm, tn;
     tile_of(t, tm, tn);
-    hf32x16 acc[2][2];
-    tile_product(t, tm, tn, 0, t.stages, lds, acc);
+    hf32x16 acc[S::NI][2];
+    tile_product<S>(t, tm, tn, 0, t.stages, lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int token0 = tm * 128 + (w >> 1) * 64, row0 = tn * 128 + (w & 1) * 64;
-    const int jbs = t.tiles_m * 4, rows = t.tiles_n * 128;
+    const int token0 = tm * S::BM + (w / S::WN) * (S::NI * 32), row0 = tn * S::BN + (w % S::WN) * 64;
+    const int jbs = l.token_blocks, rows = l.row_stride;
+    if (token0 >= jbs * 32) return;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int row = row0 + 32 * j + l32;
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         const int target = row < l.rows ? token_of(l.targets[row], l.vocabulary) : -1;
         float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::NI; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int token = token0 + 32 * i + 8 * q + 4 * hf;
@@ -369,11 +377,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         float s = 0.0f;
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::NI; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
         s += __shfl_xor(s, 32, 64);
-        if (hf == 0) l.stats[static_cast<int64_t>(token0 >> 6) * rows + row] = make_float2(m, s);
+        if (hf == 0) l.stats[static_cast<int64_t>(token0 / (S::NI * 32)) * rows + row] = make_float2(m, s);
     }
 }
 
@@ -388,42 +396,59 @@ __device__ __forceinline__ float times_row_factor(const HalvesProduct &p, int ro
     return f != 0.0f ? v * (f / p.divisor) : 0.0f;
 }
 
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
+template <class S>
+__global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
     const Tile t, const ProductArgs a) {
-    __shared__ hu32x4 lds[2 * kStageBytes / 16];
+    __shared__ hu32x4 lds[2 * S::kStage / 16];
     int tm, tn;
     tile_of(t, tm, tn);
-    hf32x16 acc[2][2];
+    hf32x16 acc[S::NI][2];
     const int s0 = blockIdx.y * t.slice;
-    tile_product(t, tm, tn, s0, min(t.stages, s0 + t.slice), lds, acc);
+    tile_product<S>(t, tm, tn, s0, min(t.stages, s0 + t.slice), lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int m0 = tm * 128 + (w >> 1) * 64, n0 = tn * 128 + (w & 1) * 64;
+    const int m0 = tm * S::BM + (w / S::WN) * (S::NI * 32), n0 = tn * S::BN + (w % S::WN) * 64;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int n = n0 + 32 * j + l32;
         if (n >= a.N) continue;
         const int up = shift_of(t.shift_b, t.all_b, n);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float old[16];
-            if (a.part == nullptr && a.p.add)
+        for (int i = 0; i < S::NI; ++i) {
+            const int m1 = m0 + 32 * i + 4 * hf;  // and + 8 (r / 4) + r % 4
+            if (m0 + 32 * i >= a.M) continue;
+            float v[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int m = min(m0 + 32 * i + 8 * (r >> 2) + 4 * hf + (r & 3), a.M - 1);
-                    old[r] = a.p.C[static_cast<int64_t>(m) * a.p.ldc + n];
+            for (int q = 0; q < 4; ++q) {
+                int4 back = make_int4(t.all_a, t.all_a, t.all_a, t.all_a);
+                if (t.shift_a != nullptr) back = *reinterpret_cast<const int4 *>(t.shift_a + m1 + 8 * q);
+                v[4 * q] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q], -up - back.x);
+                v[4 * q + 1] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + 1], -up - back.y);
+                v[4 * q + 2] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + 2], -up - back.z);
+                v[4 * q + 3] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + 3], -up - back.w);
+            }
+            float *C = a.p.C + n;
+            int64_t ld = a.p.ldc;
+            if (a.part != nullptr) {
+                C = a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.N + n;
+                ld = a.N;
+            } else {
+                if (a.p.row_factor != nullptr || a.p.divisor != 1.0f)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        v[r] = times_row_factor(a.p, min(m1 + 8 * (r >> 2) + (r & 3), a.M - 1), v[r]);
+                if (a.p.add) {
+                    float old[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) old[r] = C[min(m1 + 8 * (r >> 2) + (r & 3), a.M - 1) * ld];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) v[r] = old[r] + v[r];
                 }
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = m0 + 32 * i + 8 * (r >> 2) + 4 * hf + (r & 3);
-                if (m >= a.M) continue;
-                float v = __builtin_amdgcn_ldexpf(acc[i][j][r], -up - shift_of(t.shift_a, t.all_a, m));
-                if (a.part != nullptr) {
-                    a.part[(static_cast<int64_t>(blockIdx.y) * a.M + m) * a.N + n] = v;
-                } else {
-                    v = times_row_factor(a.p, m, v);
-                    a.p.C[static_cast<int64_t>(m) * a.p.ldc + n] = a.p.add ? old[r] + v : v;
-                }
+                const int m = m1 + 8 * (r >> 2) + (r & 3);
+                if (m < a.M) C[m * ld] = v[r];
             }
         }
     }
@@ -442,11 +467,54 @@ __global__ __launch_bounds__(kThreads) void join_slices_kernel(const ProductArgs
     }
 }
 
+template <class S>
 Tile tile_args(const Halves &A, const Halves &B) {
     CHECK_ERROR(A.terms != B.terms, "Operands of %d and %d terms.", A.terms, B.terms);
     const int stages = A.term_blocks() / 2;
-    return {A.data, B.data, A.shift, B.shift, A.shift_all, B.shift_all, A.row_blocks() / 4, B.row_blocks() / 4,
-            A.term_blocks(), stages, stages};
+    return {A.data, B.data, A.shift, B.shift, A.shift_all, B.shift_all, (A.rows + S::BM - 1) / S::BM,
+            (B.rows + S::BN - 1) / S::BN, A.term_blocks(), stages, stages};
+}
+
+using Small = Shape<2, 2, 2>;  // 128 x 128
+
+template <class S>
+void run_logits(const Halves &A, const Halves &B, LogitsArgs l, hipStream_t s) {
+    Tile t = tile_args<S>(A, B);
+    t.tiles_m = A.row_blocks() * 32 / S::BM;  // the padding too: its parts are joined
+    t.tiles_n = B.row_blocks() * 32 / S::BN;
+    logits_kernel<S><<<dim3(t.tiles_m * t.tiles_n), dim3(S::kThreads), 0, s>>>(t, l);
+    hipCheck(hipGetLastError());
+}
+
+// Slices of the reduction so that the last round of workgroups (kSlots at once) is full.  In steps of
+// 32 terms: a workgroup's start and end cost about 8, a slice's sums go out and come back.
+template <class S>
+void run_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
+    constexpr int kSlots = 256 * (8 / S::kWaves);
+    Tile t = tile_args<S>(A, B);
+    const int tiles = t.tiles_m * t.tiles_n;
+    int best = 1;
+    double best_cost = 1e30;
+    for (int n = 1; n <= 32 && n <= t.stages; ++n) {
+        const int mine = (t.stages + n - 1) / n;
+        const int rounds = (tiles * n + kSlots - 1) / kSlots;
+        const double cost = rounds * (mine + 8.0) + (n > 1 ? 8.0 + n * 0.02 * tiles * (S::BM / 128) : 0.0);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = n;
+        }
+    }
+    t.slice = ((t.stages + best - 1) / best + 1) & ~1;
+    const int slices = (t.stages + t.slice - 1) / t.slice;
+    ProductArgs a{p, A.rows, B.rows, nullptr};
+    if (slices > 1) a.part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(A.rows) * B.rows * slices));
+    product_kernel<S><<<dim3(tiles, slices), dim3(S::kThreads), 0, s>>>(t, a);
+    hipCheck(hipGetLastError());
+    if (slices == 1) return;
+    join_slices_kernel<<<dim3(blocks_for(static_cast<int64_t>(A.rows) * B.rows, kThreads)), dim3(kThreads), 0, s>>>(a,
+                                                                                                                  slices);
+    hipCheck(hipGetLastError());
+    free_cuda(a.part);
 }
 
 }  // namespace
@@ -481,39 +549,13 @@ void launch_halves_columns(const float *x, int ld, const float *weights, float d
     hipCheck(hipGetLastError());
 }
 
-void launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s) {
-    const Tile t = tile_args(A, B);
-    logits_kernel<<<dim3(t.tiles_m * t.tiles_n), dim3(kThreads), 0, s>>>(t, l);
-    hipCheck(hipGetLastError());
+int launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s) {
+    run_logits<Small>(A, B, l, s);
+    return 64;
 }
 
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
-    Tile t = tile_args(A, B);
-    const int tiles = t.tiles_m * t.tiles_n;
-    // Slices of the reduction so that the last round of 512 workgroups (two a CU) is full.  In steps of
-    // 32 terms: a workgroup's start and end cost about 8, a slice's sums go out and come back.
-    int best = 1;
-    double best_cost = 1e30;
-    for (int S = 1; S <= 32 && S <= t.stages; ++S) {
-        const int mine = (t.stages + S - 1) / S;
-        const int rounds = (tiles * S + 511) / 512;
-        const double cost = rounds * (mine + 8.0) + (S > 1 ? 8.0 + S * 0.02 * tiles : 0.0);
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = S;
-        }
-    }
-    t.slice = (t.stages + best - 1) / best;
-    const int slices = (t.stages + t.slice - 1) / t.slice;
-    ProductArgs a{p, A.rows, B.rows, nullptr};
-    if (slices > 1) a.part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(A.rows) * B.rows * slices));
-    product_kernel<<<dim3(tiles, slices), dim3(kThreads), 0, s>>>(t, a);
-    hipCheck(hipGetLastError());
-    if (slices == 1) return;
-    join_slices_kernel<<<dim3(blocks_for(static_cast<int64_t>(A.rows) * B.rows, kThreads)), dim3(kThreads), 0, s>>>(a,
-                                                                                                                  slices);
-    hipCheck(hipGetLastError());
-    free_cuda(a.part);
+    run_product<Small>(A, B, p, s);
 }
 
 }  // namespace gptc

@@ -11,7 +11,7 @@ typedef float hf32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t hu32x4 __attribute__((ext_vector_type(4)));
 
 // An operand of `rows` (of the product's M or N) by `terms` (of its reduction),
-// padded with zeros to rows of 128 and terms of 32.  Row r's values are held
+// padded with zeros to rows of 256 and terms of 32.  Row r's values are held
 // times 2^shift[r], which puts the largest below 2^15: value = high + low to
 // 2^-24 of it, or to 2^-40 of the row's largest for values below its 2^-17th.
 // Blocks of 32 rows x 16 terms, block (r / 32, k / 16) after block, high part
@@ -24,7 +24,7 @@ struct Halves {
     int shift_all;
     int rows, terms;
     __host__ __device__ int row_blocks() const { return (rows + 127) / 128 * 4; }
-    __host__ __device__ int term_blocks() const { return (terms + 31) / 32 * 2; }
+    __host__ __device__ int term_blocks() const { return (terms + 63) / 64 * 4; }
     __host__ __device__ int64_t bytes() const { return static_cast<int64_t>(row_blocks()) * term_blocks() * 2048; }
 };
 
@@ -50,7 +50,7 @@ __device__ __forceinline__ void halves_split(float x, float y, uint32_t &high, u
 
 // Negating every other step of 32 terms of one of a product's operands (the first) keeps the
 // matrix core's truncation from adding up: the kernels subtract those steps.
-__device__ __forceinline__ bool halves_negated(int term) { return ((term >> 5) & 1) != 0; }
+__device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) & 1) != 0; }
 
 // x (rows x terms, rows of ld floats; with weights, rows of weight 0 as zeros) into h.data and
 // h.shift; negate: as a product's first operand.
@@ -72,12 +72,14 @@ __device__ __forceinline__ int token_of(float f, int V) {
 // The logits of a piece: A = W (vocabulary x features), B = x (rows x features).
 struct LogitsArgs {
     float *logits;         // blocks of 32 rows x 32 tokens in the order of the accumulators, or null
-    float2 *stats;         // (tokens / 64, rows): largest logit and the sum of exp of the distances from it
+    float2 *stats;         // (parts of the tokens, rows): largest logit and the sum of exp of the distances from it
     const float *targets;  // (rows)
     float *target_logits;  // (rows), written where the target is
     int vocabulary, rows;
+    int token_blocks, row_stride;  // blocks of 32 tokens of `logits`, rows of `stats`
 };
-void launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s);
+// Returns the tokens of each of the stats' parts.
+int launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s);
 
 // C (A.rows x B.rows, rows of ldc) = A B^T times row_factor[m] / divisor (+ C); rows of factor 0 are 0.
 struct HalvesProduct {

@@ -201,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
             halves_split(d[2], d[3], high[q][1], low[q][1]);
         }
         if (a.d != nullptr && jb < a.tokens_used) {
-            const uint32_t flip = jb & 1 ? 0x80008000u : 0;  // halves_negated
+            const uint32_t flip = halves_negated(jb * 32) ? 0x80008000u : 0;
             hu32x4 *out = a.d + (static_cast<int64_t>(rb) * a.tokens_used + jb) * 256 + lane;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
             }
         }
         if (a.dt == nullptr || rb >= a.rows_used) continue;
-        const uint32_t flip = rb & 1 ? 0x80008000u : 0;
+        const uint32_t flip = halves_negated(rb * 32) ? 0x80008000u : 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -300,12 +300,13 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
         x.rows = d.rows = xt.terms = dt.terms = n;
         launch_halves_rows(xr, h.C, weights, x, false, s);
-        launch_logits(W, x, {logits, stats, h.targets + r, target_logits, h.V, n}, s);
+        const int part = launch_logits(
+            W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
         join_stats_kernel<<<dim3(n_padded / 32), dim3(kJoinThreads), 0, s>>>(
-            stats, tokens / 64, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n, n_padded, h.V);
+            stats, tokens / part, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n, n_padded, h.V);
         hipCheck(hipGetLastError());
         if (!grad) continue;
-        const ShareArgs a{logits, lse, targets, d.data, dt.data, n_padded / 32, tokens / 32, (n + 31) / 32, (h.V + 31) / 32};
+        const ShareArgs a{logits, lse, targets, d.data, dt.data, n_padded / 32, tokens / 32, (n + 63) / 64 * 2, (h.V + 63) / 64 * 2};
         shares_kernel<<<dim3((a.token_blocks + 4 * kShareTokens - 1) / (4 * kShareTokens), a.row_blocks),
                         dim3(kThreads), 0, s>>>(a);
         hipCheck(hipGetLastError());
