@@ -69,14 +69,32 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const T *__restrict__ 
 
 // ---- sorting ----
 // The sort's launches are short and mostly wait; where dW is to be overwritten, further workgroups of
-// the same launches clear it meanwhile (8192 rows of 768 on 50257: 25 us beside the ranking's 13).
+// the same launches clear it meanwhile (8192 rows of 768 on 50257: 30 us for both, 13 for the ranking alone).
 struct Clear {
     f32x4_t *at;  // n of them from here on, by the workgroups after the first `blocks` of a launch
     int64_t n;
     int blocks;
+    const uint32_t *hit;  // or null; else n counts rows of `units`, of which those that are hit stay
+    int units;
 };
 
 __device__ __forceinline__ void clear_part(const Clear &c) {
+    if (c.hit != nullptr) {
+        // A wave a row, 64 rows' flags at a time.
+        const int lane = threadIdx.x & (kWave - 1), per = blockDim.x / kWave;
+        const int64_t waves = static_cast<int64_t>(gridDim.x - c.blocks) * per;
+        const int64_t first = static_cast<int64_t>(blockIdx.x - c.blocks) * per +
+                              __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        for (int64_t r0 = first; r0 < c.n; r0 += kWave * waves) {
+            const int64_t mine = r0 + lane * waves;
+            uint64_t left = __ballot(mine < c.n && c.hit[min(mine, c.n - 1)] == 0);
+            for (; left != 0; left &= left - 1) {
+                f32x4_t *row = c.at + (r0 + __builtin_ctzll(left) * waves) * c.units;
+                for (int j = lane; j < c.units; j += kWave) row[j] = splat<f32x4_t>(0.0f);
+            }
+        }
+        return;
+    }
     const int64_t stride = static_cast<int64_t>(gridDim.x - c.blocks) * blockDim.x;
     for (int64_t i = static_cast<int64_t>(blockIdx.x - c.blocks) * blockDim.x + threadIdx.x; i < c.n; i += stride)
         c.at[i] = splat<f32x4_t>(0.0f);
@@ -84,7 +102,8 @@ __device__ __forceinline__ void clear_part(const Clear &c) {
 
 // Workgroups for a part: eight waves a CU.
 int clear_blocks(const Clear &c, int threads) {
-    return static_cast<int>(std::min<int64_t>((c.n + threads - 1) / threads, 256 * 512 / threads));
+    const int64_t units = c.hit != nullptr ? c.n * kWave : c.n;
+    return static_cast<int>(std::min<int64_t>((units + threads - 1) / threads, 256 * 512 / threads));
 }
 
 // order[r] = (key, row) of the r-th row by (key, row); key: the id, V for rows
@@ -149,8 +168,9 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const float *__restr
 // counts up, move every row to its place.
 constexpr int kDigits = 256;
 constexpr int kSortThreads = 256;
-constexpr int kSortItems = 16;  // 64 rows at a time of a wave
-constexpr int kSortBlock = kSortThreads * kSortItems;
+// Rows a thread: few rows in many workgroups of short chains (65536 rows of 1600 on 50257: the sort 52 us with 4,
+// 72 with 16), until the counts of all workgroups cost their one summing workgroup more.
+constexpr int kSortFew = 4, kSortMany = 16, kSortFewRows = 1 << 17;
 
 struct SortArgs {
     const float *ids;  // the first pass reads the ids, the others `in`
@@ -158,6 +178,7 @@ struct SortArgs {
     int2 *out;
     int *hist;  // digit-major: (kDigits, blocks)
     int n, V, shift, blocks;
+    uint32_t *hit;  // or null: set where an id occurs, by the first count
     Clear clear;
 };
 
@@ -167,6 +188,7 @@ __device__ __forceinline__ int2 sort_item(const SortArgs &a, int i) {
     return make_int2(id < 0 ? a.V : id, i);
 }
 
+template <int kItems>
 __global__ __launch_bounds__(kSortThreads) void digit_count_kernel(const SortArgs a) {
     if (static_cast<int>(blockIdx.x) >= a.blocks) {
         clear_part(a.clear);
@@ -175,47 +197,79 @@ __global__ __launch_bounds__(kSortThreads) void digit_count_kernel(const SortArg
     __shared__ int count[kDigits];
     count[threadIdx.x] = 0;
     __syncthreads();
-    int key[kSortItems];
+    const int first = blockIdx.x * (kSortThreads * kItems) + threadIdx.x;
+    int key[kItems];
 #pragma unroll
-    for (int t = 0; t < kSortItems; ++t)
-        key[t] = sort_item(a, min(blockIdx.x * kSortBlock + t * kSortThreads + static_cast<int>(threadIdx.x), a.n - 1)).x;
+    for (int t = 0; t < kItems; ++t)
+        key[t] = sort_item(a, min(first + t * kSortThreads, a.n - 1)).x;
 #pragma unroll
-    for (int t = 0; t < kSortItems; ++t)
-        if (static_cast<int>(blockIdx.x * kSortBlock + t * kSortThreads + threadIdx.x) < a.n)
+    for (int t = 0; t < kItems; ++t)
+        if (first + t * kSortThreads < a.n) {
             atomicAdd(&count[(key[t] >> a.shift) & (kDigits - 1)], 1);
+            if (a.hit != nullptr && key[t] < a.V) a.hit[key[t]] = 1;  // all that write here write the same
+        }
     __syncthreads();
     a.hist[threadIdx.x * a.blocks + blockIdx.x] = count[threadIdx.x];
 }
 
-// hist := its running sums, the entry itself left out; one workgroup.
+// hist (n entries, n a multiple of 4) := its running sums, the entry itself left out; one workgroup,
+// 16384 entries at a time in one exchange between its waves.
 constexpr int kScanThreads = 1024;
+constexpr int kScanParts = 4;
 __global__ __launch_bounds__(kScanThreads) void digit_scan_kernel(int *hist, int n, Clear clear) {
     if (blockIdx.x > 0) {
         clear_part(clear);
         return;
     }
-    __shared__ int part[kScanThreads];
-    const int per = (n + kScanThreads - 1) / kScanThreads;
-    const int lo = min(n, static_cast<int>(threadIdx.x) * per), hi = min(n, lo + per);
-    int sum = 0;
-#pragma unroll 8
-    for (int i = lo; i < hi; ++i) sum += hist[i];
-    part[threadIdx.x] = sum;
-    __syncthreads();
-    for (int off = 1; off < kScanThreads; off <<= 1) {
-        const int add = static_cast<int>(threadIdx.x) >= off ? part[threadIdx.x - off] : 0;
+    constexpr int kW = kScanThreads / kWave;
+    __shared__ int total[kScanParts * kW];
+    const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave, units = n / 4;
+    int4 *at = reinterpret_cast<int4 *>(hist);
+    int before = 0;
+    for (int u0 = 0; u0 < units; u0 += kScanParts * kScanThreads) {
+        int4 v[kScanParts];
+        int up[kScanParts];  // this lane's entries and those of the lanes before it
+#pragma unroll
+        for (int k = 0; k < kScanParts; ++k) {
+            const int u = u0 + k * kScanThreads + static_cast<int>(threadIdx.x);
+            v[k] = u < units ? at[u] : make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kScanParts; ++k) {
+            up[k] = v[k].x + v[k].y + v[k].z + v[k].w;
+#pragma unroll
+            for (int off = 1; off < kWave; off <<= 1) {
+                const int other = __shfl_up(up[k], off, kWave);
+                up[k] += lane >= off ? other : 0;
+            }
+            if (lane == kWave - 1) total[k * kW + w] = up[k];
+        }
         __syncthreads();
-        part[threadIdx.x] += add;
+        // Every wave sums up all waves' totals for itself.
+        static_assert(kScanParts * kW == kWave, "a total a lane");
+        const int own = total[lane];
+        int sum = own;
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const int other = __shfl_up(sum, off, kWave);
+            sum += lane >= off ? other : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < kScanParts; ++k) {
+            const int u = u0 + k * kScanThreads + static_cast<int>(threadIdx.x);
+            int4 out;
+            out.x = before + __shfl(sum - own, k * kW + w, kWave) + up[k] - (v[k].x + v[k].y + v[k].z + v[k].w);
+            out.y = out.x + v[k].x;
+            out.z = out.y + v[k].y;
+            out.w = out.z + v[k].z;
+            if (u < units) at[u] = out;
+        }
+        before += __shfl(sum, kWave - 1, kWave);
         __syncthreads();
-    }
-    int at = part[threadIdx.x] - sum;
-    for (int i = lo; i < hi; ++i) {
-        const int v = hist[i];
-        hist[i] = at;
-        at += v;
     }
 }
 
+template <int kItems>
 __global__ __launch_bounds__(kSortThreads) void digit_move_kernel(const SortArgs a) {
     if (static_cast<int>(blockIdx.x) >= a.blocks) {
         clear_part(a.clear);
@@ -228,15 +282,15 @@ __global__ __launch_bounds__(kSortThreads) void digit_move_kernel(const SortArgs
     for (int k = 0; k < kW; ++k) at[k][threadIdx.x] = 0;
     __syncthreads();
     // Wave w takes the w-th quarter of the block, 64 rows at a time.
-    const int first = blockIdx.x * kSortBlock + w * (kSortItems * kWave) + lane;
-    int2 item[kSortItems];
+    const int first = blockIdx.x * (kSortThreads * kItems) + w * (kItems * kWave) + lane;
+    int2 item[kItems];
 #pragma unroll
-    for (int t = 0; t < kSortItems; ++t) {
+    for (int t = 0; t < kItems; ++t) {
         const int i = first + t * kWave;
         item[t] = i < a.n ? sort_item(a, i) : make_int2(0, -1);
     }
 #pragma unroll
-    for (int t = 0; t < kSortItems; ++t)
+    for (int t = 0; t < kItems; ++t)
         if (item[t].y >= 0) atomicAdd(&at[w][(item[t].x >> a.shift) & (kDigits - 1)], 1);
     __syncthreads();
     {
@@ -250,7 +304,7 @@ __global__ __launch_bounds__(kSortThreads) void digit_move_kernel(const SortArgs
     }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < kSortItems; ++t) {
+    for (int t = 0; t < kItems; ++t) {
         const bool live = item[t].y >= 0;
         const int digit = (item[t].x >> a.shift) & (kDigits - 1);
         uint64_t same = __ballot(live);  // the lanes of this digit
@@ -284,47 +338,45 @@ struct GatherArgs {
     int seqs, seq, positions;
 };
 
-// dP[t] (+)= the sequences' rows t, in their order; rows past the sequences' length: 0.  By the workgroups
-// after the first `before` of a launch.
+// dP[t] (+)= the sequences' rows t, in their order; rows past the sequences' length: 0.
 template <typename T>
-__device__ __forceinline__ void position_sums(const GatherArgs &a, int before) {
+__device__ __forceinline__ void position_sum(const GatherArgs &a, int t, int col) {
     const int cols = a.C / (sizeof(T) / sizeof(float));
-    const int64_t n = static_cast<int64_t>(a.seq) * cols, total = static_cast<int64_t>(a.positions) * cols;
-    const int64_t stride = static_cast<int64_t>(gridDim.x - before) * kThreads;
-    const T *g = reinterpret_cast<const T *>(a.g);
-    T *dP = reinterpret_cast<T *>(a.dP);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x - before) * kThreads + threadIdx.x; i < total; i += stride) {
-        T sum = splat<T>(0.0f);
-        if (i < n) {
-            int b = 0;
-            for (; b + 8 <= a.seqs; b += 8) {
-                T v[8];
+    if (col >= cols || (a.add && t >= a.seq)) return;
+    const int64_t n = static_cast<int64_t>(a.seq) * cols, i = static_cast<int64_t>(t) * cols + col;
+    const T *g = reinterpret_cast<const T *>(a.g) + i;
+    T *dP = reinterpret_cast<T *>(a.dP) + i;
+    T sum = splat<T>(0.0f);
+    if (t < a.seq) {
+        int b = 0;
+        for (; b + 8 <= a.seqs; b += 8) {
+            T v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = g[(b + k) * n + i];
+            for (int k = 0; k < 8; ++k) v[k] = g[(b + k) * n];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum += v[k];
-            }
-            for (; b < a.seqs; ++b) sum += g[b * n + i];
-        } else if (a.add) {
-            return;
+            for (int k = 0; k < 8; ++k) sum += v[k];
         }
-        dP[i] = a.add ? dP[i] + sum : sum;
+        for (; b < a.seqs; ++b) sum += g[b * n];
     }
+    *dP = a.add ? *dP + sum : sum;
 }
 
-// One wave: `chunk` sorted places x 64 columns in units of T.
+// One wave: `chunk` sorted places x 64 columns in units of T, or such columns of a position.  Workgroups go
+// through one block of columns after the other, so that the rows are still near when they are read for the
+// second time (64 x 1024 rows of 1600, with the positions: 160 us; one chunk after the other 212).
 template <typename T>
-__global__ __launch_bounds__(kThreads) void gather_kernel(const GatherArgs a, int items) {
+__global__ __launch_bounds__(kThreads) void gather_kernel(const GatherArgs a, int chunks) {
     constexpr int kAhead = 8;  // rows whose loads are on their way together
-    const int gather_blocks = (items + kWaves - 1) / kWaves;
-    if (static_cast<int>(blockIdx.x) >= gather_blocks) {
-        position_sums<T>(a, gather_blocks);
+    const int lane = threadIdx.x & (kWave - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int position_blocks = a.dP != nullptr ? (a.positions + kWaves - 1) / kWaves : 0;
+    const int per = position_blocks + (chunks + kWaves - 1) / kWaves;
+    const int block = blockIdx.x / per, at = blockIdx.x - block * per, col = block * kWave + lane;
+    if (at < position_blocks) {
+        if (at * kWaves + w < a.positions) position_sum<T>(a, at * kWaves + w, col);
         return;
     }
-    const int lane = threadIdx.x & (kWave - 1);
-    const int item = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    if (item >= items) return;
-    const int chunk = item / a.blocks, col = (item - chunk * a.blocks) * kWave + lane;
+    const int chunk = (at - position_blocks) * kWaves + w;
+    if (chunk >= chunks) return;
     const int cols = a.C / (sizeof(T) / sizeof(float));
     const int p0 = chunk * a.chunk, left = min(a.chunk, a.n - p0);
     const int2 mine = lane < left ? a.order[p0 + lane] : make_int2(a.V, 0);
@@ -435,6 +487,9 @@ __global__ __launch_bounds__(kThreads) void clear_kernel(float *p, int64_t n) {
         p[i] = 0.0f;
 }
 
+// Rows times units that are worth flags: 34 MB are 7 us of writing at the rate of a copy, the flags' launch 4.6.
+constexpr int64_t kHitUnits = 1 << 21;
+
 // The rows sorted by (id, row); `clear`, if it has any, is zeroed on the way.
 void launch_sort(const float *ids, int n, int V, int2 *order, Clear clear, hipStream_t s) {
     if (n <= kRankRows) {
@@ -447,32 +502,47 @@ void launch_sort(const float *ids, int n, int V, int2 *order, Clear clear, hipSt
     }
     int passes = 1;  // over the digits of V, the largest key
     while (passes < 4 && (V >> (8 * passes)) != 0) ++passes;
-    const int blocks = (n + kSortBlock - 1) / kSortBlock;
+    const bool few = n <= kSortFewRows;
+    const int per = kSortThreads * (few ? kSortFew : kSortMany), blocks = (n + per - 1) / per;
+    auto count_kernel = few ? digit_count_kernel<kSortFew> : digit_count_kernel<kSortMany>;
+    auto move_kernel = few ? digit_move_kernel<kSortFew> : digit_move_kernel<kSortMany>;
     int2 *other = static_cast<int2 *>(alloc_cuda(sizeof(int2) * static_cast<size_t>(n)));
     int *hist = static_cast<int *>(alloc_cuda(sizeof(int) * kDigits * static_cast<size_t>(blocks)));
-    const int64_t share = (clear.n + 3 * passes - 1) / (3 * passes);  // an equal part with every launch
-    int64_t left = clear.n;
+    // Rows of ids that occur are not cleared, where this spares more than the flags cost.
+    uint32_t *hit = nullptr;
+    if (clear.units > 0 && static_cast<int64_t>(std::min(n, V)) * clear.units >= kHitUnits) {
+        hit = static_cast<uint32_t *>(alloc_cuda(sizeof(uint32_t) * static_cast<size_t>(V)));
+        clear_kernel<<<dim3(blocks_for(V, kThreads)), dim3(kThreads), 0, s>>>(reinterpret_cast<float *>(hit), V);
+        hipCheck(hipGetLastError());
+    }
+    // An equal part with every launch, but for the one that sets the flags.
+    const int64_t unit = hit != nullptr ? clear.units : 1, count = clear.n / unit;
+    const int shares = 3 * passes - (hit != nullptr);
+    int64_t done = 0;
     auto part = [&](int before) {
-        const Clear c{clear.at + (clear.n - left), std::min(left, share), before};
-        left -= c.n;
+        const int64_t n = std::min(count - done, (count + shares - 1) / shares);
+        const Clear c{clear.at + done * unit, n, before, hit != nullptr ? hit + done : nullptr, clear.units};
+        done += n;
         return c;
     };
-    SortArgs a{ids, nullptr, passes & 1 ? order : other, hist, n, V, 0, blocks, {}};
+    SortArgs a{ids, nullptr, passes & 1 ? order : other, hist, n, V, 0, blocks, hit, {}};
     for (int p = 0; p < passes; ++p) {
-        a.clear = part(blocks);
-        digit_count_kernel<<<dim3(blocks + clear_blocks(a.clear, kSortThreads)), dim3(kSortThreads), 0, s>>>(a);
+        a.clear = p == 0 && hit != nullptr ? Clear{} : part(blocks);
+        count_kernel<<<dim3(blocks + clear_blocks(a.clear, kSortThreads)), dim3(kSortThreads), 0, s>>>(a);
         hipCheck(hipGetLastError());
         const Clear c = part(1);
         digit_scan_kernel<<<dim3(1 + clear_blocks(c, kScanThreads)), dim3(kScanThreads), 0, s>>>(hist, kDigits * blocks, c);
         hipCheck(hipGetLastError());
         a.clear = part(blocks);
-        digit_move_kernel<<<dim3(blocks + clear_blocks(a.clear, kSortThreads)), dim3(kSortThreads), 0, s>>>(a);
+        move_kernel<<<dim3(blocks + clear_blocks(a.clear, kSortThreads)), dim3(kSortThreads), 0, s>>>(a);
         hipCheck(hipGetLastError());
         a.ids = nullptr;
+        a.hit = nullptr;
         a.in = a.out;
         a.out = a.out == order ? other : order;
         a.shift += 8;
     }
+    if (hit != nullptr) free_cuda(hit);
     free_cuda(hist);
     free_cuda(other);
 }
@@ -486,15 +556,15 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
     a.chunk = 32;
     while (a.chunk > 8 && static_cast<int64_t>(a.n) * a.blocks < 2048ll * a.chunk) a.chunk /= 2;
     const int chunks = (a.n + a.chunk - 1) / a.chunk;
-    const int64_t items = static_cast<int64_t>(chunks) * a.blocks;
+    const int64_t items = (static_cast<int64_t>(chunks) + (a.dP != nullptr ? a.positions : 0) + 2 * kWaves) * a.blocks;
     CHECK_ERROR(items > INT32_MAX / 2, "Too many rows and columns for one call: %d x %d.", a.n, a.C);
     int2 *order = static_cast<int2 *>(alloc_cuda(sizeof(int2) * static_cast<size_t>(a.n)));
     a.part = static_cast<float *>(alloc_cuda(sizeof(float) * 2 * static_cast<size_t>(chunks) * a.C));
     a.order = order;
-    Clear clear{nullptr, 0, 0};
+    Clear clear{};
     if (!a.add) {
         const int64_t n = static_cast<int64_t>(a.V) * a.C;
-        if (aligned16(a.dW)) clear = {reinterpret_cast<f32x4_t *>(a.dW), n / 4, 0};
+        if (aligned16(a.dW)) clear = {reinterpret_cast<f32x4_t *>(a.dW), n / 4, 0, nullptr, a.C % 4 == 0 ? a.C / 4 : 0};
         const int64_t rest = n - 4 * clear.n;
         if (rest > 0) {
             clear_kernel<<<dim3(blocks_for(rest, kThreads)), dim3(kThreads), 0, s>>>(a.dW + 4 * clear.n, rest);
@@ -502,9 +572,9 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
         }
     }
     launch_sort(ids, a.n, a.V, order, clear, s);
-    const int gather_blocks = static_cast<int>((items + kWaves - 1) / kWaves);
-    const int extra = a.dP != nullptr ? blocks_for(static_cast<int64_t>(a.positions) * cols, kThreads) : 0;
-    gather_kernel<T><<<dim3(gather_blocks + extra), dim3(kThreads), 0, s>>>(a, static_cast<int>(items));
+    const int position_blocks = a.dP != nullptr ? (a.positions + kWaves - 1) / kWaves : 0;
+    const int per = position_blocks + (chunks + kWaves - 1) / kWaves;
+    gather_kernel<T><<<dim3(per * a.blocks), dim3(kThreads), 0, s>>>(a, chunks);
     hipCheck(hipGetLastError());
     if (chunks > 1) {
         join_kernel<T><<<dim3(chunks - 1, a.blocks), dim3(kThreads), 0, s>>>(a);

@@ -18,8 +18,8 @@
 // a step's fragments are read to registers at once, and the loads of the step after
 // next go out into the same buffer as soon as all waves have read it.
 #include <algorithm>
-#include "gemm_halves.hpp"
 #include "gpu_kernels.h"
+#include "head_loss.hpp"
 #include "ops_common.hpp"
 
 namespace gptc {
@@ -149,37 +149,48 @@ __global__ __launch_bounds__(kThreads) void column_largest_kernel(const float *_
     }
 }
 
-constexpr int kColumnTerms = 128;  // terms a workgroup
-
-// A wave: 32 columns, kColumnTerms / 4 terms.
+// A workgroup: 32 columns, kColumnTerms terms; with `largest` null these are all terms.
 __global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *__restrict__ x, int ld,
                                                                  const float *__restrict__ weights, float divisor,
                                                                  Halves h, const uint32_t *__restrict__ largest) {
     const int lane = threadIdx.x & 63, hf = lane >> 5, w = threadIdx.x >> 6;
     const int rb = blockIdx.x, c = rb * 32 + (lane & 31), kbs = h.term_blocks();
-    const int up = c < h.rows ? halves_shift(__uint_as_float(largest[c])) : 0;
+    const int first = blockIdx.y * (kColumnTerms / 16) + w * (kColumnTerms / 64);
+    float v[kColumnTerms / 64][8];
+#pragma unroll
+    for (int i = 0; i < kColumnTerms / 64; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = (first + i) * 16 + 4 * hf + (e & 3) + 8 * (e >> 2), at = min(k, h.terms - 1);
+            const float f = term_factor(weights, divisor, at);
+            const float y = x[static_cast<int64_t>(at) * ld + min(c, h.rows - 1)];
+            v[i][e] = f != 0.0f && k < h.terms && c < h.rows ? f * y : 0.0f;
+        }
+    float top = largest != nullptr && c < h.rows ? __uint_as_float(largest[c]) : 0.0f;
+    if (largest == nullptr) {
+        __shared__ float red[kThreads / 64][32];
+#pragma unroll
+        for (int i = 0; i < kColumnTerms / 64; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[i][e]));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (hf == 0) red[w][lane] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kThreads / 64; ++i) top = fmaxf(top, red[i][lane & 31]);
+    }
+    const int up = halves_shift(top);
     if (blockIdx.y == 0 && w == 0 && hf == 0) h.shift[c] = up;
     hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs * 2) * 64 + lane;
-    const int first = blockIdx.y * (kColumnTerms / 16) + w * (kColumnTerms / 64);
 #pragma unroll
     for (int i = 0; i < kColumnTerms / 64; ++i) {
         const int kb = first + i;
         if (kb >= kbs) return;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int k = kb * 16 + 4 * hf + (e & 3) + 8 * (e >> 2);
-            v[e] = 0.0f;
-            if (k < h.terms && c < h.rows) {
-                const float f = term_factor(weights, divisor, k);
-                if (f != 0.0f) v[e] = __builtin_amdgcn_ldexpf(f * x[static_cast<int64_t>(k) * ld + c], up);
-            }
-        }
         hu32x4 high, low;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             uint32_t hi, lo;
-            halves_split(v[2 * e], v[2 * e + 1], hi, lo);
+            halves_split(__builtin_amdgcn_ldexpf(v[i][2 * e], up), __builtin_amdgcn_ldexpf(v[i][2 * e + 1], up), hi, lo);
             high[e] = hi;
             low[e] = lo;
         }
@@ -239,9 +250,9 @@ __device__ __forceinline__ void load_block(const hu32x4 *base, uint32_t to, uint
         "global_load_lds_dwordx4 %0, %1\n\t"
         "global_load_lds_dwordx4 %0, %1 offset:1024\n\t"
         "global_load_lds_dwordx4 %0, %1 offset:2048\n\t"
-        "global_load_lds_dwordx4 %0, %1 offset:3072"
+        "global_load_lds_dwordx4 %0, %1 offset:%3"
         :
-        : "v"(lane16), "s"(base), "s"(to)
+        : "v"(lane16), "s"(base), "s"(to), "n"(3 << 10)
         : "memory");
 }
 
@@ -331,8 +342,6 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 template <class S>
 __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void logits_kernel(
     const Tile t, const LogitsArgs l) {
@@ -344,44 +353,25 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int token0 = tm * S::BM + (w / S::WN) * (S::NI * 32), row0 = tn * S::BN + (w % S::WN) * 64;
-    const int jbs = l.token_blocks, rows = l.row_stride;
-    if (token0 >= jbs * 32) return;
-#pragma unroll
+    // In a loop, as its code is fetched by every workgroup.
+#pragma unroll 1
     for (int j = 0; j < 2; ++j) {
-        const int row = row0 + 32 * j + l32;
-        const int up = shift_of(t.shift_b, t.all_b, row);
-        const int target = row < l.rows ? token_of(l.targets[row], l.vocabulary) : -1;
-        float m = -INFINITY;
+        const int up = shift_of(t.shift_b, t.all_b, row0 + 32 * j + l32);
+        hf32x16 x[S::NI];
 #pragma unroll
-        for (int i = 0; i < S::NI; ++i)
+        for (int i = 0; i < S::NI; ++i) {
+            x[i] = acc[i][0];
+            acc[i][0] = acc[i][1];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int token = token0 + 32 * i + 8 * q + 4 * hf;
-                const int4 back = *reinterpret_cast<const int4 *>(t.shift_a + token);
+                const int4 back = *reinterpret_cast<const int4 *>(t.shift_a + token0 + 32 * i + 8 * q + 4 * hf);
                 const int shift[4] = {back.x, back.y, back.z, back.w};
-                f32x4_t v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + e], -up - shift[e]);
-                    if (token + e >= l.vocabulary) x = -INFINITY;
-                    if (token + e == target) l.target_logits[row] = x;
-                    acc[i][j][4 * q + e] = v[e] = x;
-                    m = fmaxf(m, x);
-                }
-                if (l.logits != nullptr) {
-                    const int64_t block = static_cast<int64_t>((row0 >> 5) + j) * jbs + (token0 >> 5) + i;
-                    reinterpret_cast<f32x4_t *>(l.logits)[(block * 4 + q) * 64 + lane] = v;
-                }
+                for (int e = 0; e < 4; ++e) x[i][4 * q + e] = __builtin_amdgcn_ldexpf(x[i][4 * q + e], -up - shift[e]);
             }
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        float s = 0.0f;
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
-        s += __shfl_xor(s, 32, 64);
-        if (hf == 0) l.stats[static_cast<int64_t>(token0 / (S::NI * 32)) * rows + row] = make_float2(m, s);
+        }
+        const float2 stat = put_logits<S::NI>(l, x, token0, (row0 >> 5) + j);
+        if (hf == 0) l.stats[static_cast<int64_t>(token0 / (S::NI * 32)) * l.row_stride + row0 + 32 * j + l32] = stat;
     }
 }
 
@@ -408,68 +398,75 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m0 = tm * S::BM + (w / S::WN) * (S::NI * 32), n0 = tn * S::BN + (w % S::WN) * 64;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int n = n0 + 32 * j + l32;
-        if (n >= a.N) continue;
-        const int up = shift_of(t.shift_b, t.all_b, n);
+    // One block of 32 x 32 after the other, in a loop: its code is fetched by every workgroup.
+#pragma unroll 1
+    for (int block = 0; block < 2 * S::NI; ++block) {
+        hf32x16 v = acc[0][0];
 #pragma unroll
         for (int i = 0; i < S::NI; ++i) {
-            const int m1 = m0 + 32 * i + 4 * hf;  // and + 8 (r / 4) + r % 4
-            if (m0 + 32 * i >= a.M) continue;
-            float v[16];
+            acc[i][0] = acc[i][1];
+            if (i + 1 < S::NI) acc[i][1] = acc[i + 1][0];
+        }
+        const int n = n0 + 32 * (block & 1) + l32, first = m0 + 32 * (block >> 1), m = first + 4 * hf;
+        if (first >= a.M) break;
+        const int up = shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                int4 back = make_int4(t.all_a, t.all_a, t.all_a, t.all_a);
-                if (t.shift_a != nullptr) back = *reinterpret_cast<const int4 *>(t.shift_a + m1 + 8 * q);
-                v[4 * q] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q], -up - back.x);
-                v[4 * q + 1] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + 1], -up - back.y);
-                v[4 * q + 2] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + 2], -up - back.z);
-                v[4 * q + 3] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + 3], -up - back.w);
+        for (int q = 0; q < 4; ++q) {
+            int4 back = make_int4(t.all_a, t.all_a, t.all_a, t.all_a);
+            if (t.shift_a != nullptr) back = *reinterpret_cast<const int4 *>(t.shift_a + m + 8 * q);
+            v[4 * q] = __builtin_amdgcn_ldexpf(v[4 * q], -up - back.x);
+            v[4 * q + 1] = __builtin_amdgcn_ldexpf(v[4 * q + 1], -up - back.y);
+            v[4 * q + 2] = __builtin_amdgcn_ldexpf(v[4 * q + 2], -up - back.z);
+            v[4 * q + 3] = __builtin_amdgcn_ldexpf(v[4 * q + 3], -up - back.w);
+        }
+        // The block's rows of C or of the slice's part; what lies past the last row or column is neither read nor written.
+        const int ld = a.part != nullptr ? a.N : a.p.ldc;
+        float *C = a.part != nullptr ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.N : a.p.C;
+        const int bytes = 4 * min(32, a.M - first) * ld;
+        const __amdgpu_buffer_rsrc_t rows =
+            __builtin_amdgcn_make_buffer_rsrc(C + static_cast<int64_t>(first) * ld, 0, bytes, 0x00020000);
+        const uint32_t mine = n < a.N ? 4 * (static_cast<uint32_t>(4 * hf) * ld + n) : 0x80000000u;
+        auto row_at = [&](int r) { return min(4 * (8 * (r >> 2) + (r & 3)) * ld, bytes); };
+        if (a.part == nullptr) {
+            if (a.p.row_factor != nullptr || a.p.divisor != 1.0f) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    v[r] = times_row_factor(a.p, min(m + 8 * (r >> 2) + (r & 3), a.M - 1), v[r]);
             }
-            float *C = a.p.C + n;
-            int64_t ld = a.p.ldc;
-            if (a.part != nullptr) {
-                C = a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.N + n;
-                ld = a.N;
-            } else {
-                if (a.p.row_factor != nullptr || a.p.divisor != 1.0f)
+            if (a.p.add) {
+                float old[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        v[r] = times_row_factor(a.p, min(m1 + 8 * (r >> 2) + (r & 3), a.M - 1), v[r]);
-                if (a.p.add) {
-                    float old[16];
+                for (int r = 0; r < 16; ++r)
+                    old[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, mine, row_at(r), 0));
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) old[r] = C[min(m1 + 8 * (r >> 2) + (r & 3), a.M - 1) * ld];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) v[r] = old[r] + v[r];
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = m1 + 8 * (r >> 2) + (r & 3);
-                if (m < a.M) C[m * ld] = v[r];
+                for (int r = 0; r < 16; ++r) v[r] = old[r] + v[r];
             }
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[r]), rows, mine, row_at(r), 0);
     }
 }
 
 // C = the slices' sums in their order, times the row's factor (+ C).
-__global__ __launch_bounds__(kThreads) void join_slices_kernel(const ProductArgs a, int slices) {
-    const int64_t n = static_cast<int64_t>(a.M) * a.N, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+__global__ __launch_bounds__(kThreads) void join_slices_kernel(const float *__restrict__ part, int M, int N, int slices,
+                                                              const HalvesProduct p) {
+    const int64_t n = static_cast<int64_t>(M) * N, stride = static_cast<int64_t>(gridDim.x) * kThreads;
     for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n; i += stride) {
-        float v = a.part[i];
-        for (int s = 1; s < slices; ++s) v += a.part[s * n + i];
-        const int m = static_cast<int>(i / a.N);
-        float *c = a.p.C + static_cast<int64_t>(m) * a.p.ldc + (i - static_cast<int64_t>(m) * a.N);
-        v = times_row_factor(a.p, m, v);
-        *c = a.p.add ? *c + v : v;
+        float v = part[i];
+#pragma unroll 8
+        for (int s = 1; s < slices; ++s) v += part[s * n + i];
+        const int m = static_cast<int>(i / N);
+        float *c = p.C + static_cast<int64_t>(m) * p.ldc + (i - static_cast<int64_t>(m) * N);
+        v = times_row_factor(p, m, v);
+        *c = p.add ? *c + v : v;
     }
 }
 
 template <class S>
 Tile tile_args(const Halves &A, const Halves &B) {
-    CHECK_ERROR(A.terms != B.terms, "Operands of %d and %d terms.", A.terms, B.terms);
+    CHECK_ERROR(A.terms != B.terms || B.rows >= 1 << 22, "Operands of %d and %d terms, %d columns.", A.terms, B.terms,
+                B.rows);
     const int stages = A.term_blocks() / 2;
     return {A.data, B.data, A.shift, B.shift, A.shift_all, B.shift_all, (A.rows + S::BM - 1) / S::BM,
             (B.rows + S::BN - 1) / S::BN, A.term_blocks(), stages, stages};
@@ -511,13 +508,17 @@ void run_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipSt
     product_kernel<S><<<dim3(tiles, slices), dim3(S::kThreads), 0, s>>>(t, a);
     hipCheck(hipGetLastError());
     if (slices == 1) return;
-    join_slices_kernel<<<dim3(blocks_for(static_cast<int64_t>(A.rows) * B.rows, kThreads)), dim3(kThreads), 0, s>>>(a,
-                                                                                                                  slices);
-    hipCheck(hipGetLastError());
+    launch_join_slices(a.part, A.rows, B.rows, slices, p, s);
     free_cuda(a.part);
 }
 
 }  // namespace
+
+void launch_join_slices(const float *part, int M, int N, int slices, const HalvesProduct &p, hipStream_t s) {
+    join_slices_kernel<<<dim3(blocks_for(static_cast<int64_t>(M) * N, kThreads)), dim3(kThreads), 0, s>>>(part, M, N,
+                                                                                                        slices, p);
+    hipCheck(hipGetLastError());
+}
 
 void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s) {
     const bool vec = ld % 4 == 0 && h.terms % 4 == 0 && aligned16(x);

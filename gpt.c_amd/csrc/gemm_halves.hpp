@@ -57,29 +57,14 @@ __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) &
 void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
 // as a second operand.  largest: the bits of each column's largest magnitude, which the first call raises
-// from what it holds (launch_zero_words) and which may count further terms too.
+// from what it holds (launch_zero_words) and which may count further terms too; null with up to
+// kColumnTerms terms, whose largest the second call finds by itself.
+constexpr int kColumnTerms = 128;
 void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,
                            uint32_t *largest, hipStream_t s);
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
                            const uint32_t *largest, hipStream_t s);
 void launch_zero_words(uint32_t *p, int n, hipStream_t s);
-
-// A token held in a float, truncated; -1 for what is not in [0, V).
-__device__ __forceinline__ int token_of(float f, int V) {
-    return f > -1.0f && f < static_cast<float>(V) ? static_cast<int>(f) : -1;
-}
-
-// The logits of a piece: A = W (vocabulary x features), B = x (rows x features).
-struct LogitsArgs {
-    float *logits;         // blocks of 32 rows x 32 tokens in the order of the accumulators, or null
-    float2 *stats;         // (parts of the tokens, rows): largest logit and the sum of exp of the distances from it
-    const float *targets;  // (rows)
-    float *target_logits;  // (rows), written where the target is
-    int vocabulary, rows;
-    int token_blocks, row_stride;  // blocks of 32 tokens of `logits`, rows of `stats`
-};
-// Returns the tokens of each of the stats' parts.
-int launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s);
 
 // C (A.rows x B.rows, rows of ldc) = A B^T times row_factor[m] / divisor (+ C); rows of factor 0 are 0.
 struct HalvesProduct {
@@ -90,5 +75,7 @@ struct HalvesProduct {
     bool add;
 };
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
+// The same from the sums of `slices` parts of the reduction, (M, N) each, in their order.
+void launch_join_slices(const float *part, int M, int N, int slices, const HalvesProduct &p, hipStream_t s);
 
 }  // namespace gptc

@@ -6,70 +6,19 @@
 // The rows go through in pieces, so that a piece's logits fit the scratch: its
 // logits are formed once, turned into d, and used for both gradients.
 #include <algorithm>
-#include "gemm_halves.hpp"
-#include "gemm_split.hpp"
 #include "gpu_kernels.h"
-#include "ops_common.hpp"
+#include "head_loss.hpp"
 
 namespace gptc {
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowThreads = 512;
-constexpr int kRowWaves = kRowThreads / kWave;
-constexpr int64_t kPieceFloats = 1ll << 27;  // logits of a piece
-constexpr int kHalvesRows = 128;             // from here on the operands are laid out first
+constexpr float kLog2eF = 1.4426950408889634f;
 constexpr int kMaxVocabulary = 1 << 22;      // a product's tile offsets fit 32 bits
 
 __device__ __forceinline__ float weight_of(const float *weights, int row) {
     return weights != nullptr ? weights[row] : 1.0f;
-}
-
-// One row a workgroup: its loss, and with `grad` its logits become d.
-__global__ __launch_bounds__(kRowThreads) void loss_row_kernel(float *__restrict__ logits,
-                                                              const float *__restrict__ targets,
-                                                              const float *__restrict__ weights,
-                                                              float *__restrict__ losses, int V, float rows,
-                                                              bool grad) {
-    __shared__ float sm[kRowWaves], ss[kRowWaves];
-    const int row = blockIdx.x;
-    float *x = logits + static_cast<int64_t>(row) * V;
-    const float weight = weight_of(weights, row);
-    if (weight == 0.0f) {
-        if (threadIdx.x == 0) losses[row] = 0.0f;
-        if (grad)
-            for (int j = threadIdx.x; j < V; j += kRowThreads) x[j] = 0.0f;
-        return;
-    }
-    float m = -INFINITY, s = 0.0f;
-    for (int j = threadIdx.x; j < V; j += kRowThreads) {
-        const float v = x[j];
-        if (v > m) {
-            s = s * expf(m - v) + 1.0f;
-            m = v;
-        } else if (v != -INFINITY) {
-            s += expf(v - m);
-        }
-    }
-    wave_online(m, s);
-    const int w = threadIdx.x / kWave;
-    if ((threadIdx.x & (kWave - 1)) == 0) {
-        sm[w] = m;
-        ss[w] = s;
-    }
-    __syncthreads();
-    m = sm[0];
-    s = ss[0];
-#pragma unroll
-    for (int i = 1; i < kRowWaves; ++i) online_merge(m, s, sm[i], ss[i]);
-    const float logsum = logf(s);
-    const int t = token_of(targets[row], V);
-    if (threadIdx.x == 0) losses[row] = t >= 0 ? logsum - (x[t] - m) : NAN;
-    if (!grad) return;
-    __syncthreads();  // the target's logit has been read
-    const float factor = weight / rows;
-    for (int j = threadIdx.x; j < V; j += kRowThreads) x[j] = factor * (expf(x[j] - m - logsum) - (j == t ? 1.0f : 0.0f));
 }
 
 // out[0] = sum of w[r] loss[r] / rows in a fixed order, in 64 bits.
@@ -91,81 +40,117 @@ __global__ __launch_bounds__(kMeanThreads) void mean_loss_kernel(const float *__
     out[0] = static_cast<float>(t / rows);
 }
 
-// y = x with rows of weight 0 as zeros.
-__global__ __launch_bounds__(kThreads) void live_rows_kernel(const float *__restrict__ x,
-                                                            const float *__restrict__ weights, float *__restrict__ y,
-                                                            int C) {
-    const int row = blockIdx.x;
-    const int64_t base = static_cast<int64_t>(row) * C;
-    const bool live = weights[row] != 0.0f;
-    for (int c = threadIdx.x; c < C; c += kThreads) y[base + c] = live ? x[base + c] : 0.0f;
-}
+constexpr int kMeanRows = 32;  // up to here, the kernel that forms the rows' losses forms their mean
 
 struct HeadLoss {
     const float *x, *W, *targets, *weights;
-    float *losses, *dx, *dW;
+    float *losses, *mean, *dx, *dW;
     int rows, V, C;
     bool add;
 };
 
+void launch_mean(const HeadLoss &h, hipStream_t s) {
+    mean_loss_kernel<<<dim3(1), dim3(kMeanThreads), 0, s>>>(h.losses, h.weights, h.mean, h.rows);
+    hipCheck(hipGetLastError());
+}
+
 // ---- many rows: products of operands laid out as two fp16 parts ----
 
-// A row's loss, lse and target from the parts of its tokens: 32 rows a workgroup, whose
-// 32 slices of the parts are joined in order.  Rows that take no part, those past the
-// last one among them: lse is infinite, which makes their shares 0, and the target -1.
+struct JoinArgs {
+    const float2 *stats;
+    int parts;
+    const float *targets, *target_logits, *weights;
+    float *lse;
+    int *whole;  // the targets, -1 for none
+    float *losses;
+    int rows, padded, V;
+    float *mean;  // MEAN: of all rows, which are one workgroup's
+};
+
+// A row's loss, lse and target from the parts of its tokens: ROWS rows a workgroup, whose slices of
+// the parts are joined in a fixed order.  Rows that take no part, those past the last one among them:
+// lse is infinite, which makes their shares 0, and the target -1.  Latency bound.
 constexpr int kJoinThreads = 1024;
-__global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const float2 *__restrict__ stats, int parts,
-                                                                 const float *__restrict__ targets,
-                                                                 const float *__restrict__ target_logits,
-                                                                 const float *__restrict__ weights,
-                                                                 float *__restrict__ lse, int *__restrict__ whole,
-                                                                 float *__restrict__ losses, int rows, int padded,
-                                                                 int V) {
-    constexpr int kAhead = 8;
-    __shared__ float2 red[32][33];
-    const int r = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + r;
-    const int per = (parts + 31) / 32, end = min(parts, (slice + 1) * per);
+template <int ROWS, bool MEAN>
+__global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs a) {
+    constexpr int kAhead = 16, kWaves = kJoinThreads / kWave, kSlices = kJoinThreads / ROWS;
+    __shared__ float2 red[kWaves][ROWS];
+    const int r = threadIdx.x % ROWS, slice = threadIdx.x / ROWS, row = blockIdx.x * ROWS + r;
     float m = -INFINITY, s = 0.0f;
-    for (int p0 = slice * per; p0 < end; p0 += kAhead) {
+    for (int p0 = slice; p0 < a.parts; p0 += kAhead * kSlices) {
         float2 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            v[k] = stats[static_cast<int64_t>(min(p0 + k, end - 1)) * padded + row];
-            if (p0 + k >= end) v[k] = make_float2(-INFINITY, 0.0f);
+            const int p = p0 + k * kSlices;
+            v[k] = a.stats[static_cast<int64_t>(min(p, a.parts - 1)) * a.padded + row];
+            if (p >= a.parts) v[k] = make_float2(-INFINITY, 0.0f);
         }
         float top = m;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) top = fmaxf(top, v[k].x);
         if (top == -INFINITY) continue;  // nothing but parts without a logit
-        s *= expf(m - top);
+        s *= __builtin_amdgcn_exp2f((m - top) * kLog2eF);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) s += v[k].y * expf(v[k].x - top);
+        for (int k = 0; k < kAhead; ++k) s += v[k].y * __builtin_amdgcn_exp2f((v[k].x - top) * kLog2eF);
         m = top;
     }
-    red[slice][r] = make_float2(m, s);
+#pragma unroll
+    for (int off = ROWS; off < kWave; off <<= 1) {
+        const float m2 = __shfl_xor(m, off, kWave), s2 = __shfl_xor(s, off, kWave);
+        online_merge(m, s, m2, s2);
+    }
+    if ((threadIdx.x & (kWave - 1)) < ROWS) red[threadIdx.x / kWave][r] = make_float2(m, s);
     __syncthreads();
-    if (slice != 0) return;
-    for (int i = 1; i < 32; ++i) online_merge(m, s, red[i][r].x, red[i][r].y);
-    const bool live = row < rows && weight_of(weights, row) != 0.0f;
-    const int target = live ? token_of(targets[row], V) : -1;
+    if (threadIdx.x >= kWave) return;
+    constexpr int kGroups = kWave / ROWS;  // of the first wave, each with an equal part of the waves' sums
+    m = red[slice][r].x;
+    s = red[slice][r].y;
+#pragma unroll
+    for (int k = kGroups; k < kWaves; k += kGroups) {
+        const float2 b = red[slice + k][r];
+        online_merge(m, s, b.x, b.y);
+    }
+#pragma unroll
+    for (int off = ROWS; off < kWave; off <<= 1) {
+        const float m2 = __shfl_xor(m, off, kWave), s2 = __shfl_xor(s, off, kWave);
+        online_merge(m, s, m2, s2);
+    }
+    if (threadIdx.x >= ROWS) return;
+    const float weight = row < a.rows ? weight_of(a.weights, row) : 0.0f;
+    const bool live = weight != 0.0f;
+    const int target = live ? token_of(a.targets[row], a.V) : -1;
     const float logsum = logf(s);
-    lse[row] = live ? m + logsum : INFINITY;
-    whole[row] = target;
-    if (row < rows) losses[row] = !live ? 0.0f : target >= 0 ? logsum - (target_logits[row] - m) : NAN;
+    const float loss = !live ? 0.0f : target >= 0 ? logsum - (a.target_logits[row] - m) : NAN;
+    a.lse[row] = live ? m + logsum : INFINITY;
+    a.whole[row] = target;
+    if (row < a.rows) a.losses[row] = loss;
+    if (!MEAN) return;
+    double t = static_cast<double>(loss) * weight;
+#pragma unroll
+    for (int off = 1; off < ROWS; off <<= 1) t += __shfl_xor(t, off, ROWS);
+    if (threadIdx.x == 0) a.mean[0] = static_cast<float>(t / a.rows);
+}
+
+void launch_join_stats(const JoinArgs &a, hipStream_t s) {
+    if (a.mean != nullptr)
+        join_stats_kernel<kMeanRows, true><<<dim3(1), dim3(kJoinThreads), 0, s>>>(a);
+    else
+        join_stats_kernel<8, false><<<dim3(a.padded / 8), dim3(kJoinThreads), 0, s>>>(a);
+    hipCheck(hipGetLastError());
 }
 
 struct ShareArgs {
     const float *logits, *lse;
     const int *targets;
     hu32x4 *d, *dt;  // as first operands of d W and d^T x; either may be null
+    hu32x4 *thirds;  // or d in three bf16 parts, for few rows
     int row_blocks, token_blocks;  // of the logits
     int rows_used, tokens_used;    // blocks that the products' reductions reach
+    int per_wave;                  // blocks of tokens a wave
 };
 
 constexpr int kShareShift = 15;  // shares are held times 2^15
-constexpr float kLog2eF = 1.4426950408889634f;
 constexpr int kShareStride = 36;  // words of LDS a token: 16-byte rows, no two in the same banks
-constexpr int kShareTokens = 4;   // blocks of 32 tokens a wave
 
 // d' = exp(l - lse) - [target] of a block of 32 rows x 32 tokens, in two fp16 parts, as the
 // operand of either product.  The logits come in the order of the accumulators: a lane holds row
@@ -176,29 +161,47 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rb = blockIdx.y;
-    const int first = (blockIdx.x * 4 + w) * kShareTokens;
+    const int first = (blockIdx.x * 4 + w) * a.per_wave;
     const int row = rb * 32 + l32;
     const float lse = a.lse[row];
     const int target = a.targets[row];
     uint32_t *mine = lds[w];
-    for (int jb = first; jb < min(first + kShareTokens, a.token_blocks); ++jb) {
+    for (int jb = first; jb < min(first + a.per_wave, a.token_blocks); ++jb) {
         const f32x4_t *x = reinterpret_cast<const f32x4_t *>(a.logits) +
                            (static_cast<int64_t>(rb) * a.token_blocks + jb) * 256 + lane;
         f32x4_t v[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = x[q * 64];
-        uint32_t high[4][2], low[4][2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float d[4];
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float p = __builtin_amdgcn_exp2f((v[q][e] - lse) * kLog2eF);
-                d[e] = (p - (jb * 32 + 8 * q + 4 * hf + e == target ? 1.0f : 0.0f)) *
-                       static_cast<float>(1 << kShareShift);
+                v[q][e] = p - (jb * 32 + 8 * q + 4 * hf + e == target ? 1.0f : 0.0f);
             }
-            halves_split(d[0], d[1], high[q][0], low[q][0]);
-            halves_split(d[2], d[3], high[q][1], low[q][1]);
+        if (a.thirds != nullptr) {
+            const float scale = jb & 1 ? -1.0f : 1.0f;
+            hu32x4 *out = a.thirds + (static_cast<int64_t>(rb) * a.token_blocks + jb) * 384 + lane;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                hu32x4 f[3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t p[3];
+                    thirds_split(scale * v[2 * k + (e >> 1)][2 * (e & 1)], scale * v[2 * k + (e >> 1)][2 * (e & 1) + 1], p);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) f[i][e] = p[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 3; ++i) out[(3 * k + i) * 64] = f[i];
+            }
+        }
+        uint32_t high[4][2], low[4][2];
+        constexpr float kUp = static_cast<float>(1 << kShareShift);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            halves_split(v[q][0] * kUp, v[q][1] * kUp, high[q][0], low[q][0]);
+            halves_split(v[q][2] * kUp, v[q][3] * kUp, high[q][1], low[q][1]);
         }
         if (a.d != nullptr && jb < a.tokens_used) {
             const uint32_t flip = halves_negated(jb * 32) ? 0x80008000u : 0;
@@ -237,6 +240,14 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
         }
         wave_lds_order();
     }
+}
+
+void launch_shares(ShareArgs a, hipStream_t s) {
+    // Four blocks a wave, fewer where that leaves less than eight waves a CU.
+    a.per_wave = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, static_cast<int64_t>(a.row_blocks) * a.token_blocks / 2048)));
+    const int per = 4 * a.per_wave;
+    shares_kernel<<<dim3((a.token_blocks + per - 1) / per, a.row_blocks), dim3(kThreads), 0, s>>>(a);
+    hipCheck(hipGetLastError());
 }
 
 // Blocks of the pool for the length of a call.
@@ -302,14 +313,12 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         launch_halves_rows(xr, h.C, weights, x, false, s);
         const int part = launch_logits(
             W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
-        join_stats_kernel<<<dim3(n_padded / 32), dim3(kJoinThreads), 0, s>>>(
-            stats, tokens / part, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n, n_padded, h.V);
-        hipCheck(hipGetLastError());
+        launch_join_stats({stats, tokens / part, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n,
+                           n_padded, h.V, nullptr},
+                          s);
         if (!grad) continue;
-        const ShareArgs a{logits, lse, targets, d.data, dt.data, n_padded / 32, tokens / 32, (n + 63) / 64 * 2, (h.V + 63) / 64 * 2};
-        shares_kernel<<<dim3((a.token_blocks + 4 * kShareTokens - 1) / (4 * kShareTokens), a.row_blocks),
-                        dim3(kThreads), 0, s>>>(a);
-        hipCheck(hipGetLastError());
+        const ShareArgs a{logits, lse, targets, d.data, dt.data, nullptr, n_padded / 32, tokens / 32, (n + 63) / 64 * 2, (h.V + 63) / 64 * 2, 0};
+        launch_shares(a, s);
         if (h.dx != nullptr)
             launch_halves_product(d, Wt, {h.dx + static_cast<int64_t>(r) * h.C, h.C, weights,
                                           static_cast<float>(h.rows), false},
@@ -319,43 +328,72 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
             launch_halves_product(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
         }
     }
+    launch_mean(h, s);
     scratch.release();
 }
 
-// ---- few rows: products that split the floats as they come ----
+// ---- few rows: W as it comes (head_few.hip) ----
 
-void run_pieces(const HeadLoss &h, hipStream_t s) {
+void run_few(const HeadLoss &h, hipStream_t s) {
     const bool grad = h.dx != nullptr || h.dW != nullptr;
-    const int64_t fit = std::max<int64_t>(1, kPieceFloats / h.V);
-    const int piece = static_cast<int>(std::min<int64_t>(h.rows, fit));
-    float *logits = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(piece) * h.V));
-    const float *x = h.x;
-    float *live = nullptr;
-    if (h.weights != nullptr) {
-        live = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(h.rows) * h.C));
-        live_rows_kernel<<<dim3(h.rows), dim3(kThreads), 0, s>>>(h.x, h.weights, live, h.C);
-        hipCheck(hipGetLastError());
-        x = live;
-    }
-    for (int r = 0; r < h.rows; r += piece) {
-        const int n = std::min(piece, h.rows - r);
-        const float *xr = x + static_cast<int64_t>(r) * h.C;
-        launch_split_gemm({xr, h.W, logits, nullptr, nullptr, n, h.V, h.C, h.C, h.C, h.V, false, true}, s);
-        loss_row_kernel<<<dim3(n), dim3(kRowThreads), 0, s>>>(
-            logits, h.targets + r, h.weights != nullptr ? h.weights + r : nullptr, h.losses + r, h.V,
-            static_cast<float>(h.rows), grad);
-        hipCheck(hipGetLastError());
+    const int tokens = (h.V + 127) / 128 * 128;
+    // dt's terms are whole pairs of blocks.
+    const int blocks = std::max(few_row_blocks(h.rows), h.dW != nullptr ? 2 : 1), padded = blocks * 32;
+    Scratch scratch;
+    const Thirds x{nullptr, blocks, h.C}, d{nullptr, blocks, tokens};
+    Thirds xs = x, ds = d;
+    xs.data = scratch.take<hu32x4>(x.bytes() / 16);
+    launch_thirds_rows(h.x, h.weights, h.rows, xs, s);
+    float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
+    float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 32));
+    int *targets = scratch.take<int>(padded);
+    float *target_logits = scratch.take<float>(padded), *lse = scratch.take<float>(padded);
+    const int part = launch_few_logits(
+        h.W, h.V, h.C, xs, {logits, stats, h.targets, target_logits, h.V, h.rows, tokens / 32, padded}, s);
+    const bool mean = h.rows <= kMeanRows && padded == kMeanRows;
+    launch_join_stats({stats, tokens / part, h.targets, target_logits, h.weights, lse, targets, h.losses, h.rows, padded,
+                       h.V, mean ? h.mean : nullptr},
+                      s);
+    if (!mean) launch_mean(h, s);
+    if (grad) {
+        Halves dt{nullptr, nullptr, kShareShift, h.V, h.rows}, xt{};
+        if (h.dx != nullptr) ds.data = scratch.take<hu32x4>(d.bytes() / 16);
+        if (h.dW != nullptr) dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
+        launch_shares({logits, lse, targets, nullptr, dt.data, ds.data, blocks, tokens / 32, dt.term_blocks() / 2,
+                       tokens / 32, 0},
+                      s);
         if (h.dx != nullptr)
-            launch_split_gemm({logits, h.W, h.dx + static_cast<int64_t>(r) * h.C, nullptr, nullptr, n, h.C, h.V, h.V, h.C,
-                               h.C, false, false},
-                              s);
-        if (h.dW != nullptr)
-            launch_split_gemm({logits, xr, h.dW, nullptr, h.add || r > 0 ? h.dW : nullptr, h.V, h.C, n, h.V, h.C, h.C,
-                               true, false},
-                              s);
+            launch_few_dx(ds, h.W, h.V, h.C, h.rows,
+                          {h.dx, h.C, h.weights, static_cast<float>(h.rows), false}, s);
+        if (h.dW != nullptr) {
+            xt = scratch.halves(h.C, h.rows);
+            if (h.rows <= kColumnTerms) {
+                launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, nullptr, s);
+            } else {
+                uint32_t *largest = scratch.take<uint32_t>(h.C);
+                launch_zero_words(largest, h.C, s);
+                launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest, s);
+                launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, largest, s);
+            }
+            if (h.rows <= kFewDwTerms)
+                launch_few_dw(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add}, s);
+            else
+                launch_halves_product(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add}, s);
+        }
     }
-    free_cuda(live);
-    free_cuda(logits);
+    scratch.release();
+}
+
+// Whether W is read as it comes.  A row costs that path about twice as much, but W is not laid out, which is
+// worth 360 rows and the time of 5e8 products of those.  Rows, vocabulary x features: us as it comes / laid out,
+// with both gradients, then the loss alone:
+//   100, 50257 x 768: 238 / 369, 78 / 143      384, 50257 x 768: 606 / 557, 188 / 193
+//   384, 50257 x 64: 183 / 203, 39 / 41        1024, 50257 x 64: 383 / 359, 70 / 67
+//   384, 5003 x 1600: 210 / 192, 83 / 83       1024, 5003 x 1600: 456 / 298, 136 / 108
+//   768, 5003 x 100: 77 / 83, 23 / 25          4096, 5003 x 100: 213 / 187, 55 / 46
+bool few_rows(int rows, int V, int C) {
+    const int64_t weights = static_cast<int64_t>(V) * C;
+    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 && (rows - 360) * weights < 500000000;
 }
 
 }  // namespace
@@ -408,13 +446,11 @@ extern "C" void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t
     CHECK_ERROR(gptc_stream_capturing(), "gptc_linear_cross_entropy_cuda takes scratch: not under graph capture.");
     hipStream_t s = gptc_stream_checked();
     float *losses = row_losses != NULL ? row_losses->t : static_cast<float *>(alloc_cuda(sizeof(float) * rows));
-    const HeadLoss h{x->t, W->t, targets->t, weights != NULL ? weights->t : nullptr, losses, dx != NULL ? dx->t : nullptr,
-                     dW != NULL ? dW->t : nullptr, rows, V, C, accumulate != 0};
-    if (rows >= kHalvesRows)
-        run_halves(h, s);
+    const HeadLoss h{x->t, W->t, targets->t, weights != NULL ? weights->t : nullptr, losses, output->t,
+                     dx != NULL ? dx->t : nullptr, dW != NULL ? dW->t : nullptr, rows, V, C, accumulate != 0};
+    if (few_rows(rows, V, C))
+        run_few(h, s);
     else
-        run_pieces(h, s);
-    mean_loss_kernel<<<dim3(1), dim3(kMeanThreads), 0, s>>>(losses, weights != NULL ? weights->t : nullptr, output->t, rows);
-    hipCheck(hipGetLastError());
+        run_halves(h, s);
     if (row_losses == NULL) free_cuda(losses);
 }

@@ -1,0 +1,95 @@
+"""The cross entropy without logits and the sorted gradient at sizes on either side of where their kernels change, with
+the references, inputs and tolerances of test_head_loss_gpu.py and test_embed_sorted_gpu.py.
+
+W is read as it comes for up to 4096 rows while (rows - 360) V C < 5e8, else it is laid out first; there are kernels for
+32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  The sort ranks up to 12288 rows, then
+goes by digits, with more rows a workgroup from 131073 on; rows that are to be overwritten are not cleared where
+min(n, V) C >= 2^23.
+"""
+import numpy as np
+import pytest
+
+import test_embed_sorted_gpu as sorted_gpu
+import test_head_loss_gpu as head
+
+pytestmark = pytest.mark.gpu
+
+MANY = 4225  # rows past 4096: W is laid out
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("R,V,C", [
+    (4096, 130, 36), (4097, 1, 1), (4097, 2, 3), (4100, 129, 33), (4225, 257, 100), (4351, 127, 65), (5000, 700, 64),
+    (8193, 300, 31), (900, 3001, 336), (16384, 140, 16)])
+def test_many_rows(rt, R, V, C, weights):
+    a = head.inputs(R, V, C, weights=weights)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("V,C", [(127, 31), (257, 32), (300, 33), (129, 96), (1000, 130)])
+@pytest.mark.parametrize("R", [31, 32, 33, 64, 65, 96, 127, 128, 129, 255, 385])
+def test_few_rows(rt, R, V, C):
+    a = head.inputs(R, V, C, seed=1, weights=R % 2 == 1)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R", [857, 858])
+def test_where_w_is_laid_out(rt, R):
+    a = head.inputs(R, 50257, 20, weights=True)
+    head.agree(head.Call(rt, *a), head.Exact(*a))
+
+
+def test_many_rows_alike(rt):
+    """The cases that may go wrong at any number of rows, at one of many."""
+    head.test_parts_of_the_results(rt, MANY, 300, 40)
+    head.test_padding_rows_take_no_part(rt, MANY, 200, 64)
+    head.test_all_rows_padding(rt, MANY)
+    head.test_targets_outside_the_vocabulary(rt, MANY)
+    head.test_confident_and_far_logits(rt, MANY)
+    head.test_zeros(rt, MANY)
+    head.test_tensors_off_16_bytes(rt, MANY, 257, 33)
+    head.test_tensors_off_16_bytes(rt, MANY, 128, 64)
+    head.test_the_same_every_time(rt, MANY, 500, 80)
+
+
+@pytest.mark.parametrize("shift", [-60, -30, 30, 50])
+def test_many_rows_far_from_one(rt, shift):
+    head.test_values_far_from_one(rt, MANY, shift)
+
+
+def test_many_rows_of_other_sizes(rt):
+    head.test_rows_and_columns_of_other_sizes(rt, MANY)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_many_rows_not_finite(rt, bad):
+    head.test_values_that_are_not_finite(rt, MANY, bad)
+
+
+def test_many_rows_against_differences(rt):
+    head.test_gradients_against_differences(rt, MANY)
+
+
+@pytest.mark.parametrize("R", [32, 64, 128, 129])
+def test_few_rows_alike(rt, R):
+    head.test_parts_of_the_results(rt, R, 300, 40)
+    head.test_padding_rows_take_no_part(rt, R, 200, 64)
+    head.test_all_rows_padding(rt, R)
+    head.test_targets_outside_the_vocabulary(rt, R)
+    head.test_confident_and_far_logits(rt, R)
+    head.test_zeros(rt, R)
+    head.test_tensors_off_16_bytes(rt, R, 257, 33)
+    head.test_values_that_are_not_finite(rt, R, np.nan)
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("shape,V,C,kind", [
+    ((16, 1024), 9000, 936, "text"), ((13, 1000), 8200, 1028, "one"), ((13, 1000), 8200, 1027, "uniform"),
+    ((13, 1000), 8193, 1024, "outside"), ((130, 1024), 300, 8, "text"), ((128, 1024), 300, 8, "text"),
+    ((1, 131073), 70000, 4, "uniform"), ((20, 10000), 200000, 44, "outside"), ((300, 1000), 5, 3, "two")])
+def test_sorted_gradient(rt, shape, V, C, kind, accumulate):
+    sorted_gpu.test_gradient(rt, shape, V, C, kind, accumulate)
