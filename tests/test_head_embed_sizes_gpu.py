@@ -2,8 +2,8 @@
 the references, inputs and tolerances of test_head_loss_gpu.py and test_embed_sorted_gpu.py.
 
 W is read as it comes for up to 4096 rows while (rows - 360) V C < 5e8, else it is laid out first; there are kernels for
-32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  The sort ranks up to 12288 rows, then
-goes by digits, with more rows a workgroup from 131073 on; rows that are to be overwritten are not cleared where
+32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
+other; the sort ranks up to 12288 rows, then goes by digits, with more rows a workgroup from 131073 on; rows that are to be overwritten are not cleared where
 min(n, V) C >= 2^23.
 """
 import numpy as np
@@ -93,3 +93,17 @@ def test_few_rows_alike(rt, R):
     ((1, 131073), 70000, 4, "uniform"), ((20, 10000), 200000, 44, "outside"), ((300, 1000), 5, 3, "two")])
 def test_sorted_gradient(rt, shape, V, C, kind, accumulate):
     sorted_gpu.test_gradient(rt, shape, V, C, kind, accumulate)
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("shape,V,C,kind", [
+    ((63,), 9, 3, "two"), ((1, 64), 5, 4, "one"), ((5, 13), 8193, 5, "outside"), ((255, 1), 16385, 33, "text"),
+    ((2, 128), 33, 257, "uniform"), ((257, 1), 100, 260, "one"), ((4, 256), 3, 520, "two"), ((2, 512), 5000, 36, "text"),
+    ((1023, 1), 1, 7, "one"), ((32, 32), 4000000, 1, "outside"), ((1, 1025), 64, 12, "text"), ((25, 41), 2, 5, "two")])
+def test_gradient_of_few_rows(rt, shape, V, C, kind, accumulate):
+    sorted_gpu.test_gradient(rt, shape, V, C, kind, accumulate)
+
+
+def test_few_rows_are_added_in_their_order(rt):
+    sorted_gpu.test_the_same_every_time(rt, (4, 250), 90, 64, "text")
+    sorted_gpu.test_the_same_every_time(rt, (1, 1024), 3, 300, "two")
