@@ -152,7 +152,8 @@ __global__ __launch_bounds__(kThreads) void column_largest_kernel(const float *_
 // A workgroup: 32 columns, kColumnTerms terms; with `largest` null these are all terms.
 __global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *__restrict__ x, int ld,
                                                                  const float *__restrict__ weights, float divisor,
-                                                                 Halves h, const uint32_t *__restrict__ largest) {
+                                                                 Halves h, bool negate,
+                                                                 const uint32_t *__restrict__ largest) {
     const int lane = threadIdx.x & 63, hf = lane >> 5, w = threadIdx.x >> 6;
     const int rb = blockIdx.x, c = rb * 32 + (lane & 31), kbs = h.term_blocks();
     const int first = blockIdx.y * (kColumnTerms / 16) + w * (kColumnTerms / 64);
@@ -186,13 +187,14 @@ __global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *_
     for (int i = 0; i < kColumnTerms / 64; ++i) {
         const int kb = first + i;
         if (kb >= kbs) return;
+        const uint32_t flip = negate && halves_negated(kb * 16) ? 0x80008000u : 0;
         hu32x4 high, low;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             uint32_t hi, lo;
             halves_split(__builtin_amdgcn_ldexpf(v[i][2 * e], up), __builtin_amdgcn_ldexpf(v[i][2 * e + 1], up), hi, lo);
-            high[e] = hi;
-            low[e] = lo;
+            high[e] = hi ^ flip;
+            low[e] = lo ^ flip;
         }
         out[(kb * 2) * 64] = high;
         out[(kb * 2 + 1) * 64] = low;
@@ -211,6 +213,7 @@ struct Tile {
     const int *shift_a, *shift_b;
     int all_a, all_b;  // where shift_a or shift_b is null
     int tiles_m, tiles_n, kbs, stages, slice;  // stages of 32 terms in all, and of a slice
+    int kbs_across;  // blocks of 16 of what are A's rows here
 };
 
 __device__ __forceinline__ int shift_of(const int *shift, int all, int row) { return shift != nullptr ? shift[row] : all; }
@@ -241,23 +244,35 @@ struct Shape {
     static constexpr int kStage = kBlocks * 4096;              // bytes
 };
 
-// Loads of 1 KB from `base` (and behind) to LDS at `to` (and behind).  They write no register; the
-// compiler does not count them, so its own waits wait for more than they need.
-__device__ __forceinline__ void load_block(const hu32x4 *base, uint32_t to, uint32_t lane16) {
+// Loads of 4 KB from `base` on to LDS at `to` and behind, lane l's 16 bytes of a kilobyte from `first` there, of the last
+// two from `last`.  They write no register; the compiler does not count them, so its own waits wait for more than they
+// need.
+__device__ __forceinline__ void load_block(const hu32x4 *base, uint32_t to, uint32_t first, uint32_t last) {
     asm volatile(
-        "s_mov_b32 m0, %2\n\t"
+        "s_mov_b32 m0, %3\n\t"
         "s_nop 0\n\t"
-        "global_load_lds_dwordx4 %0, %1\n\t"
-        "global_load_lds_dwordx4 %0, %1 offset:1024\n\t"
-        "global_load_lds_dwordx4 %0, %1 offset:2048\n\t"
-        "global_load_lds_dwordx4 %0, %1 offset:%3"
+        "global_load_lds_dwordx4 %0, %2\n\t"
+        "global_load_lds_dwordx4 %0, %2 offset:1024\n\t"
+        "global_load_lds_dwordx4 %1, %2 offset:2048\n\t"
+        "global_load_lds_dwordx4 %1, %2 offset:%4"
         :
-        : "v"(lane16), "s"(base), "s"(to), "n"(3 << 10)
+        : "v"(first), "v"(last), "s"(base), "s"(to), "n"(3 << 10)
         : "memory");
 }
 
+// Four fp16 values, 16 lanes transposed: lane j receives value j % 4 of lanes j / 4 + {0, 4, 8, 12} of its 16.
+__device__ __forceinline__ uint2 read_across(uint32_t at) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<__attribute__((address_space(3))) s16x4 *>(static_cast<uintptr_t>(at))));
+}
+
 // acc = the wave's outputs of tile (tm, tn) over steps [s0, s1), without the shifts.
-template <class S>
+// ACROSS: A comes as the operand of the other product, its rows as terms and its terms as rows: four consecutive terms
+// of a row are 8 bytes in LDS, which a transposing read gives to four lanes.  There 16-byte chunk c of a kilobyte lies
+// at c ^ 4 (c / 32), and ^ 8 in every other block of 16 terms, so that no two of a read's lanes meet in a bank.  The
+// sign of every other 64 terms is a sign of rows here, and B holds that of the reduction.
+template <class S, bool ACROSS>
 __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int s0, int s1, hu32x4 *lds,
                                              hf32x16 (&acc)[S::NI][2]) {
     const int tid = threadIdx.x, lane = tid & 63;
@@ -265,26 +280,31 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     constexpr int kA = S::BM / 32, kB = S::BN / 32;
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) void *)lds));
-    const uint32_t lane16 = lane * 16;
-    // Wave w loads blocks w kLoads .. of A's and B's rows.
+    const uint32_t lane16 = lane * 16, hf = lane >> 5;
+    static_assert(!ACROSS || (kA == S::kWaves && S::kLoads == 2), "a wave loads one block of A, then one of B");
+    // Wave w loads blocks w, w + kWaves .. of A's and B's rows.
     const hu32x4 *from[S::kLoads];
+    int64_t step[S::kLoads];
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
         const int block = w + i * S::kWaves;
-        const hu32x4 *p = block < kA ? t.A + static_cast<int64_t>(tm * kA + block) * t.kbs * 128
+        const hu32x4 *p = block < kA ? t.A + static_cast<int64_t>(tm * kA + block) * (ACROSS ? 2 : t.kbs) * 128
                                      : t.B + static_cast<int64_t>(tn * kB + block - kA) * t.kbs * 128;
-        from[i] = p + s0 * 256;
+        step[i] = ACROSS && block < kA ? static_cast<int64_t>(t.kbs_across) * 128 : 256;
+        from[i] = p + s0 * step[i];
     }
+    const uint32_t lane_first = ACROSS ? lane16 ^ (64 * hf) : lane16, lane_last = ACROSS ? lane_first ^ 128 : lane16;
     // Past the last step the last one is loaded again, into a buffer that nobody reads any more: the
     // loop needs no branch then, and its waits are the same in every step.
     int next = s0;
     auto load_stage = [&](uint32_t off) {
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i)
-            load_block(from[i], base + off + (w + i * S::kWaves) * 4096, lane16);
+            load_block(from[i], base + off + (w + i * S::kWaves) * 4096, i == 0 ? lane_first : lane16,
+                       i == 0 ? lane_last : lane16);
         if (++next < s1) {
 #pragma unroll
-            for (int i = 0; i < S::kLoads; ++i) from[i] += 256;
+            for (int i = 0; i < S::kLoads; ++i) from[i] += step[i];
         }
     };
 #pragma unroll
@@ -297,7 +317,13 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     load_stage(S::kStage);
     const hu32x4 *at_a = lds + (w / S::WN) * S::NI * 256 + lane;
     const hu32x4 *at_b = lds + (kA + (w % S::WN) * 2) * 256 + lane;
-    float sign = s0 & 2 ? -1.0f : 1.0f;
+    // Lane l reads, of terms (rows of the block) 4 (l / 32) + l / 4 % 4 and 8 behind, rows (terms) 16 (l / 16 % 2) + 4 (l % 4) ..
+    const uint32_t in16 = lane & 15, half16 = (lane >> 4) & 1;
+    const uint32_t across = (w / S::WN) * (S::NI * 4096) + half16 * 2048 + (in16 & 1) * 512 + half16 * 128 +
+                            (hf ^ (in16 & 1)) * 64 + (in16 >> 2) * 16 + ((in16 >> 1) & 1) * 8;
+    const uint32_t across_first = base + across, across_last = base + (across ^ 128);
+    float sign = ((s0 & 2) != 0) != (ACROSS && ((w / S::WN * S::NI) & 2) != 0) ? -1.0f : 1.0f;
+    static_assert(!ACROSS || (S::NI == 2 && S::BM % 128 == 0), "a wave's rows are 64 of one sign");
     for (int s = s0; s < s1; s += 2) {
         hf32x16 p[S::NI][2];
 #pragma unroll
@@ -316,7 +342,16 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
 #pragma unroll
             for (int i = 0; i < 8; ++i) fb[i >> 2][(i >> 1) & 1][i & 1] = at_b[off + i * 64];
 #pragma unroll
-            for (int i = 0; i < 4 * S::NI; ++i) fa[i >> 2][(i >> 1) & 1][i & 1] = at_a[off + i * 64];
+            for (int i = 0; i < 4 * S::NI; ++i) {
+                hu32x4 &f = fa[i >> 2][(i >> 1) & 1][i & 1];
+                if constexpr (ACROSS) {
+                    const uint32_t at = half * S::kStage + (i >> 2) * 4096 + ((i >> 1) & 1) * 256 + (i & 1) * 1024;
+                    const uint2 one = read_across(across_first + at), two = read_across(across_last + at);
+                    f = hu32x4{one.x, one.y, two.x, two.y};
+                } else {
+                    f = at_a[off + i * 64];
+                }
+            }
             // All waves have read this buffer: the step after next goes there.
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             load_stage(half * S::kStage);
@@ -349,7 +384,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
     int tm, tn;
     tile_of(t, tm, tn);
     hf32x16 acc[S::NI][2];
-    tile_product<S>(t, tm, tn, 0, t.stages, lds, acc);
+    tile_product<S, false>(t, tm, tn, 0, t.stages, lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int token0 = tm * S::BM + (w / S::WN) * (S::NI * 32), row0 = tn * S::BN + (w % S::WN) * 64;
@@ -386,7 +421,7 @@ __device__ __forceinline__ float times_row_factor(const HalvesProduct &p, int ro
     return f != 0.0f ? v * (f / p.divisor) : 0.0f;
 }
 
-template <class S>
+template <class S, bool ACROSS>
 __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
     const Tile t, const ProductArgs a) {
     __shared__ hu32x4 lds[2 * S::kStage / 16];
@@ -394,7 +429,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
     tile_of(t, tm, tn);
     hf32x16 acc[S::NI][2];
     const int s0 = blockIdx.y * t.slice;
-    tile_product<S>(t, tm, tn, s0, min(t.stages, s0 + t.slice), lds, acc);
+    tile_product<S, ACROSS>(t, tm, tn, s0, min(t.stages, s0 + t.slice), lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m0 = tm * S::BM + (w / S::WN) * (S::NI * 32), n0 = tn * S::BN + (w % S::WN) * 64;
@@ -469,7 +504,7 @@ Tile tile_args(const Halves &A, const Halves &B) {
                 B.rows);
     const int stages = A.term_blocks() / 2;
     return {A.data, B.data, A.shift, B.shift, A.shift_all, B.shift_all, (A.rows + S::BM - 1) / S::BM,
-            (B.rows + S::BN - 1) / S::BN, A.term_blocks(), stages, stages};
+            (B.rows + S::BN - 1) / S::BN, A.term_blocks(), stages, stages, 0};
 }
 
 using Small = Shape<2, 2, 2>;  // 128 x 128
@@ -485,10 +520,11 @@ void run_logits(const Halves &A, const Halves &B, LogitsArgs l, hipStream_t s) {
 
 // Slices of the reduction so that the last round of workgroups (kSlots at once) is full.  In steps of
 // 32 terms: a workgroup's start and end cost about 8, a slice's sums go out and come back.
-template <class S>
-void run_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
+template <class S, bool ACROSS>
+void run_product(const Halves &A, const Halves &B, int kbs_across, const HalvesProduct &p, hipStream_t s) {
     constexpr int kSlots = 256 * (8 / S::kWaves);
     Tile t = tile_args<S>(A, B);
+    t.kbs_across = kbs_across;
     const int tiles = t.tiles_m * t.tiles_n;
     int best = 1;
     double best_cost = 1e30;
@@ -505,7 +541,7 @@ void run_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipSt
     const int slices = (t.stages + t.slice - 1) / t.slice;
     ProductArgs a{p, A.rows, B.rows, nullptr};
     if (slices > 1) a.part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(A.rows) * B.rows * slices));
-    product_kernel<S><<<dim3(tiles, slices), dim3(S::kThreads), 0, s>>>(t, a);
+    product_kernel<S, ACROSS><<<dim3(tiles, slices), dim3(S::kThreads), 0, s>>>(t, a);
     hipCheck(hipGetLastError());
     if (slices == 1) return;
     launch_join_slices(a.part, A.rows, B.rows, slices, p, s);
@@ -544,9 +580,9 @@ void launch_zero_words(uint32_t *p, int n, hipStream_t s) {
 }
 
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
-                           const uint32_t *largest, hipStream_t s) {
+                           bool negate, const uint32_t *largest, hipStream_t s) {
     const int chunks = (h.term_blocks() * 16 + kColumnTerms - 1) / kColumnTerms;
-    halves_columns_kernel<<<dim3(h.row_blocks(), chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor, h, largest);
+    halves_columns_kernel<<<dim3(h.row_blocks(), chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor, h, negate, largest);
     hipCheck(hipGetLastError());
 }
 
@@ -556,7 +592,14 @@ int launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStre
 }
 
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
-    run_product<Small>(A, B, p, s);
+    run_product<Small, false>(A, B, 0, p, s);
+}
+
+void launch_halves_product_across(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
+    CHECK_ERROR(A.rows != B.terms || A.shift != nullptr, "Operands of %d and %d terms, or shifts by term.", A.rows, B.terms);
+    // As an operand of A.terms rows; only its size counts from here on.
+    const Halves across{A.data, nullptr, A.shift_all, A.terms, A.rows};
+    run_product<Small, true>(across, B, A.term_blocks(), p, s);
 }
 
 }  // namespace gptc

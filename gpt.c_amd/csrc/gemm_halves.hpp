@@ -56,14 +56,14 @@ __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) &
 // h.shift; negate: as a product's first operand.
 void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
-// as a second operand.  largest: the bits of each column's largest magnitude, which the first call raises
+// as a second operand, or as the one that is negated.  largest: the bits of each column's largest magnitude, which the first call raises
 // from what it holds (launch_zero_words) and which may count further terms too; null with up to
 // kColumnTerms terms, whose largest the second call finds by itself.
 constexpr int kColumnTerms = 128;
 void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,
                            uint32_t *largest, hipStream_t s);
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
-                           const uint32_t *largest, hipStream_t s);
+                           bool negate, const uint32_t *largest, hipStream_t s);
 void launch_zero_words(uint32_t *p, int n, hipStream_t s);
 
 // C (A.rows x B.rows, rows of ldc) = A B^T times row_factor[m] / divisor (+ C); rows of factor 0 are 0.
@@ -75,7 +75,10 @@ struct HalvesProduct {
     bool add;
 };
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
-// The same from the sums of `slices` parts of the reduction, (M, N) each, in their order.
+// C (A.terms x B.rows) = A^T B^T for A as in another product, where it was the first operand; its shifts are one, and
+// B is negated.  A's data are readable up to 8 KB past their end.
+void launch_halves_product_across(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
+// C from the sums of `slices` parts of the reduction, (M, N) each, in their order.
 void launch_join_slices(const float *part, int M, int N, int slices, const HalvesProduct &p, hipStream_t s);
 
 }  // namespace gptc

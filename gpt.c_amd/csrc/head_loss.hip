@@ -272,13 +272,13 @@ struct Scratch {
     }
 };
 
-constexpr int64_t kPieceBytes = 5ll << 28;  // logits, d and d^T of a piece
+constexpr int64_t kPieceBytes = 5ll << 28;  // logits and d of a piece
 constexpr int kLossPiece = 16384;           // rows of a piece whose logits are not written
 
 void run_halves(const HeadLoss &h, hipStream_t s) {
     const bool grad = h.dx != nullptr || h.dW != nullptr;
     const int tokens = (h.V + 127) / 128 * 128;
-    const int64_t fit = std::max<int64_t>(1, kPieceBytes / (12ll * tokens) / 128) * 128;
+    const int64_t fit = std::max<int64_t>(1, kPieceBytes / (8ll * tokens) / 128) * 128;
     const int piece = static_cast<int>(std::min<int64_t>(h.rows, grad ? fit : kLossPiece));
     const int padded = (piece + 127) / 128 * 128;
     Scratch scratch;
@@ -291,16 +291,14 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     if (h.dx != nullptr) {
         Wt = scratch.halves(h.C, h.V);
         launch_column_largest(h.W, h.C, nullptr, 1.0f, h.V, h.C, largest, s);
-        launch_halves_columns(h.W, h.C, nullptr, 1.0f, Wt, largest, s);
+        launch_halves_columns(h.W, h.C, nullptr, 1.0f, Wt, false, largest, s);
     }
-    Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V},
-           dt{nullptr, nullptr, kShareShift, h.V, piece};
+    Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
     if (h.dW != nullptr) {
         xt = scratch.halves(h.C, piece);
-        dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
         launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest_x, s);
     }
-    if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / 16);
+    if (grad) d.data = scratch.take<hu32x4>((d.bytes() + 8192) / 16);
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
     float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 64));
     int *targets = scratch.take<int>(padded);
@@ -309,7 +307,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         const int n = std::min(piece, h.rows - r), n_padded = (n + 127) / 128 * 128;
         const float *xr = h.x + static_cast<int64_t>(r) * h.C;
         const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
-        x.rows = d.rows = xt.terms = dt.terms = n;
+        x.rows = d.rows = xt.terms = n;
         launch_halves_rows(xr, h.C, weights, x, false, s);
         const int part = launch_logits(
             W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
@@ -317,15 +315,16 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
                            n_padded, h.V, nullptr},
                           s);
         if (!grad) continue;
-        const ShareArgs a{logits, lse, targets, d.data, dt.data, nullptr, n_padded / 32, tokens / 32, (n + 63) / 64 * 2, (h.V + 63) / 64 * 2, 0};
+        const ShareArgs a{logits, lse, targets, d.data, nullptr, nullptr, n_padded / 32, tokens / 32, 0,
+                          (h.V + 63) / 64 * 2, 0};
         launch_shares(a, s);
         if (h.dx != nullptr)
             launch_halves_product(d, Wt, {h.dx + static_cast<int64_t>(r) * h.C, h.C, weights,
                                           static_cast<float>(h.rows), false},
                                   s);
         if (h.dW != nullptr) {
-            launch_halves_columns(xr, h.C, weights, static_cast<float>(h.rows), xt, largest_x, s);
-            launch_halves_product(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
+            launch_halves_columns(xr, h.C, weights, static_cast<float>(h.rows), xt, true, largest_x, s);
+            launch_halves_product_across(d, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
         }
     }
     launch_mean(h, s);
@@ -368,12 +367,12 @@ void run_few(const HeadLoss &h, hipStream_t s) {
         if (h.dW != nullptr) {
             xt = scratch.halves(h.C, h.rows);
             if (h.rows <= kColumnTerms) {
-                launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, nullptr, s);
+                launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, false, nullptr, s);
             } else {
                 uint32_t *largest = scratch.take<uint32_t>(h.C);
                 launch_zero_words(largest, h.C, s);
                 launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest, s);
-                launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, largest, s);
+                launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, false, largest, s);
             }
             if (h.rows <= kFewDwTerms)
                 launch_few_dw(dt, xt, {h.dW, h.C, nullptr, 1.0f, h.add}, s);
