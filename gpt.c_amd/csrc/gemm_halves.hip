@@ -107,6 +107,71 @@ __global__ __launch_bounds__(kThreads) void halves_rows_kernel(const float *__re
     }
 }
 
+// largest[0] = bits of the largest magnitude of n values so far.
+__global__ __launch_bounds__(kThreads) void largest_kernel(const float *__restrict__ x, int64_t n, bool vec,
+                                                          uint32_t *largest) {
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    const int64_t first = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x, whole = vec ? n / 4 : 0;
+    float m = 0.0f;
+#pragma unroll 8
+    for (int64_t i = first; i < whole; i += stride) {
+        const f32x4_t v = reinterpret_cast<const f32x4_t *>(x)[i];
+        m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    }
+    for (int64_t i = 4 * whole + first; i < n; i += stride) m = fmaxf(m, fabsf(x[i]));
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    __shared__ float red[kThreads / 64];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; ++i) m = fmaxf(m, red[i]);
+    atomicMax(largest, __float_as_uint(m));
+}
+
+// Rows by one shift, in one pass: a workgroup 32 rows x 128 terms, whose lines are read whole and written whole, through
+// LDS.
+__global__ __launch_bounds__(kThreads) void halves_table_kernel(const float *__restrict__ x, int ld, Halves h, bool vec,
+                                                               const uint32_t *__restrict__ largest) {
+    __shared__ hu32x4 lds[8 * 128];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, kbs = h.term_blocks(), rb = blockIdx.x, kb0 = blockIdx.y * 8;
+    const int up = halves_shift(__uint_as_float(*largest));
+    if (blockIdx.y == 0 && threadIdx.x < 32) h.shift[rb * 32 + threadIdx.x] = up;
+    float v[4][4];
+    // Piece i of a wave: rows 8 w .. + 7, terms 32 i .. + 31 of the workgroup's.
+    const int in = w * 8 + (lane >> 3), row = rb * 32 + in;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = kb0 * 16 + 32 * i + 4 * (lane & 7);
+        const float *p = x + static_cast<int64_t>(row) * ld + k;
+        if (vec && row < h.rows && k < h.terms) {
+            const f32x4_t y = *reinterpret_cast<const f32x4_t *>(p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = row < h.rows && k + e < h.terms ? p[e] : 0.0f;
+        }
+    }
+    uint2 *to = reinterpret_cast<uint2 *>(lds);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = 8 * i + (lane & 7), q = c & 3;  // four terms of block c / 4
+        const uint32_t flip = halves_negated((kb0 + (c >> 2)) * 16) ? 0x80008000u : 0;
+        uint2 high, low;
+        halves_split(__builtin_amdgcn_ldexpf(v[i][0], up), __builtin_amdgcn_ldexpf(v[i][1], up), high.x, low.x);
+        halves_split(__builtin_amdgcn_ldexpf(v[i][2], up), __builtin_amdgcn_ldexpf(v[i][3], up), high.y, low.y);
+        const int at = (c >> 2) * 256 + ((q & 1) * 32 + in) * 2 + (q >> 1);
+        to[at] = make_uint2(high.x ^ flip, high.y ^ flip);
+        to[at + 128] = make_uint2(low.x ^ flip, low.y ^ flip);
+    }
+    __syncthreads();
+    const int blocks = min(8, kbs - kb0);
+    hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs + kb0) * 128;
+    for (int i = threadIdx.x; i < blocks * 128; i += kThreads) out[i] = lds[i];
+}
+
 // The factor of term k of an operand that is read across its rows.
 __device__ __forceinline__ float term_factor(const float *weights, float divisor, int k) {
     return weights != nullptr ? weights[k] / divisor : 1.0f / divisor;
@@ -213,7 +278,7 @@ struct Tile {
     const int *shift_a, *shift_b;
     int all_a, all_b;  // where shift_a or shift_b is null
     int tiles_m, tiles_n, kbs, stages, slice;  // stages of 32 terms in all, and of a slice
-    int kbs_across;  // blocks of 16 of what are A's rows here
+    int kbs_across;  // blocks of 16 of what are rows here of the operand that is read across
 };
 
 __device__ __forceinline__ int shift_of(const int *shift, int all, int row) { return shift != nullptr ? shift[row] : all; }
@@ -268,11 +333,14 @@ __device__ __forceinline__ uint2 read_across(uint32_t at) {
 }
 
 // acc = the wave's outputs of tile (tm, tn) over steps [s0, s1), without the shifts.
-// ACROSS: A comes as the operand of the other product, its rows as terms and its terms as rows: four consecutive terms
-// of a row are 8 bytes in LDS, which a transposing read gives to four lanes.  There 16-byte chunk c of a kilobyte lies
-// at c ^ 4 (c / 32), and ^ 8 in every other block of 16 terms, so that no two of a read's lanes meet in a bank.  The
-// sign of every other 64 terms is a sign of rows here, and B holds that of the reduction.
-template <class S, bool ACROSS>
+// The operand that is read `Across` comes as the first one of another product, its rows as terms and its terms as
+// rows: four consecutive terms of a row are 8 bytes in LDS, which a transposing read gives to four lanes.  There 16-byte
+// chunk c of a kilobyte lies at c ^ 4 (c / 32), and ^ 8 in every other block of 16 terms, so that no two of a read's
+// lanes meet in a bank.  The sign of every other 64 terms is a sign of the outputs' rows or columns here, and the other
+// operand holds that of the reduction.
+enum class Across { kNone, kA, kB };
+
+template <class S, Across ACROSS>
 __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int s0, int s1, hu32x4 *lds,
                                              hf32x16 (&acc)[S::NI][2]) {
     const int tid = threadIdx.x, lane = tid & 63;
@@ -281,27 +349,29 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) void *)lds));
     const uint32_t lane16 = lane * 16, hf = lane >> 5;
-    static_assert(!ACROSS || (kA == S::kWaves && S::kLoads == 2), "a wave loads one block of A, then one of B");
+    constexpr int kAt = ACROSS == Across::kA ? 0 : ACROSS == Across::kB ? 1 : -1;  // which of a wave's blocks it is
+    static_assert(kAt < 0 || (kA == S::kWaves && S::kLoads == 2), "a wave loads one block of A, then one of B");
     // Wave w loads blocks w, w + kWaves .. of A's and B's rows.
     const hu32x4 *from[S::kLoads];
     int64_t step[S::kLoads];
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
         const int block = w + i * S::kWaves;
-        const hu32x4 *p = block < kA ? t.A + static_cast<int64_t>(tm * kA + block) * (ACROSS ? 2 : t.kbs) * 128
-                                     : t.B + static_cast<int64_t>(tn * kB + block - kA) * t.kbs * 128;
-        step[i] = ACROSS && block < kA ? static_cast<int64_t>(t.kbs_across) * 128 : 256;
+        const int kbs = i == kAt ? 2 : t.kbs;
+        const hu32x4 *p = block < kA ? t.A + static_cast<int64_t>(tm * kA + block) * kbs * 128
+                                     : t.B + static_cast<int64_t>(tn * kB + block - kA) * kbs * 128;
+        step[i] = i == kAt ? static_cast<int64_t>(t.kbs_across) * 128 : 256;
         from[i] = p + s0 * step[i];
     }
-    const uint32_t lane_first = ACROSS ? lane16 ^ (64 * hf) : lane16, lane_last = ACROSS ? lane_first ^ 128 : lane16;
+    const uint32_t lane_first = lane16 ^ (64 * hf), lane_last = lane_first ^ 128;
     // Past the last step the last one is loaded again, into a buffer that nobody reads any more: the
     // loop needs no branch then, and its waits are the same in every step.
     int next = s0;
     auto load_stage = [&](uint32_t off) {
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i)
-            load_block(from[i], base + off + (w + i * S::kWaves) * 4096, i == 0 ? lane_first : lane16,
-                       i == 0 ? lane_last : lane16);
+            load_block(from[i], base + off + (w + i * S::kWaves) * 4096, i == kAt ? lane_first : lane16,
+                       i == kAt ? lane_last : lane16);
         if (++next < s1) {
 #pragma unroll
             for (int i = 0; i < S::kLoads; ++i) from[i] += step[i];
@@ -319,11 +389,19 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     const hu32x4 *at_b = lds + (kA + (w % S::WN) * 2) * 256 + lane;
     // Lane l reads, of terms (rows of the block) 4 (l / 32) + l / 4 % 4 and 8 behind, rows (terms) 16 (l / 16 % 2) + 4 (l % 4) ..
     const uint32_t in16 = lane & 15, half16 = (lane >> 4) & 1;
-    const uint32_t across = (w / S::WN) * (S::NI * 4096) + half16 * 2048 + (in16 & 1) * 512 + half16 * 128 +
+    const uint32_t block_across = ACROSS == Across::kA ? (w / S::WN) * S::NI : kA + (w % S::WN) * 2;
+    const uint32_t across = block_across * 4096 + half16 * 2048 + (in16 & 1) * 512 + half16 * 128 +
                             (hf ^ (in16 & 1)) * 64 + (in16 >> 2) * 16 + ((in16 >> 1) & 1) * 8;
     const uint32_t across_first = base + across, across_last = base + (across ^ 128);
-    float sign = ((s0 & 2) != 0) != (ACROSS && ((w / S::WN * S::NI) & 2) != 0) ? -1.0f : 1.0f;
-    static_assert(!ACROSS || (S::NI == 2 && S::BM % 128 == 0), "a wave's rows are 64 of one sign");
+    auto fragment_across = [&](int half, int i) {
+        const uint32_t at = half * S::kStage + (i >> 2) * 4096 + ((i >> 1) & 1) * 256 + (i & 1) * 1024;
+        const uint2 one = read_across(across_first + at), two = read_across(across_last + at);
+        return hu32x4{one.x, one.y, two.x, two.y};
+    };
+    // A wave's 64 rows and 64 columns are of one sign each.
+    static_assert(S::NI == 2 && S::BM % 128 == 0 && S::BN % 128 == 0, "");
+    const bool minus = ACROSS == Across::kA ? ((w / S::WN) & 1) != 0 : ACROSS == Across::kB ? ((w % S::WN) & 1) != 0 : false;
+    float sign = ((s0 & 2) != 0) != minus ? -1.0f : 1.0f;
     for (int s = s0; s < s1; s += 2) {
         hf32x16 p[S::NI][2];
 #pragma unroll
@@ -340,18 +418,11 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
             asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
             hu32x4 fb[2][2][2], fa[S::NI][2][2];  // blocks of 32 rows, of 16 terms, parts
 #pragma unroll
-            for (int i = 0; i < 8; ++i) fb[i >> 2][(i >> 1) & 1][i & 1] = at_b[off + i * 64];
+            for (int i = 0; i < 8; ++i)
+                fb[i >> 2][(i >> 1) & 1][i & 1] = ACROSS == Across::kB ? fragment_across(half, i) : at_b[off + i * 64];
 #pragma unroll
-            for (int i = 0; i < 4 * S::NI; ++i) {
-                hu32x4 &f = fa[i >> 2][(i >> 1) & 1][i & 1];
-                if constexpr (ACROSS) {
-                    const uint32_t at = half * S::kStage + (i >> 2) * 4096 + ((i >> 1) & 1) * 256 + (i & 1) * 1024;
-                    const uint2 one = read_across(across_first + at), two = read_across(across_last + at);
-                    f = hu32x4{one.x, one.y, two.x, two.y};
-                } else {
-                    f = at_a[off + i * 64];
-                }
-            }
+            for (int i = 0; i < 4 * S::NI; ++i)
+                fa[i >> 2][(i >> 1) & 1][i & 1] = ACROSS == Across::kA ? fragment_across(half, i) : at_a[off + i * 64];
             // All waves have read this buffer: the step after next goes there.
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             load_stage(half * S::kStage);
@@ -384,7 +455,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
     int tm, tn;
     tile_of(t, tm, tn);
     hf32x16 acc[S::NI][2];
-    tile_product<S, false>(t, tm, tn, 0, t.stages, lds, acc);
+    tile_product<S, Across::kNone>(t, tm, tn, 0, t.stages, lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int token0 = tm * S::BM + (w / S::WN) * (S::NI * 32), row0 = tn * S::BN + (w % S::WN) * 64;
@@ -421,7 +492,7 @@ __device__ __forceinline__ float times_row_factor(const HalvesProduct &p, int ro
     return f != 0.0f ? v * (f / p.divisor) : 0.0f;
 }
 
-template <class S, bool ACROSS>
+template <class S, Across ACROSS>
 __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
     const Tile t, const ProductArgs a) {
     __shared__ hu32x4 lds[2 * S::kStage / 16];
@@ -444,7 +515,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
         }
         const int n = n0 + 32 * (block & 1) + l32, first = m0 + 32 * (block >> 1), m = first + 4 * hf;
         if (first >= a.M) break;
-        const int up = shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
+        const int up = ACROSS == Across::kB ? t.shift_b[0] : shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             int4 back = make_int4(t.all_a, t.all_a, t.all_a, t.all_a);
@@ -520,7 +591,7 @@ void run_logits(const Halves &A, const Halves &B, LogitsArgs l, hipStream_t s) {
 
 // Slices of the reduction so that the last round of workgroups (kSlots at once) is full.  In steps of
 // 32 terms: a workgroup's start and end cost about 8, a slice's sums go out and come back.
-template <class S, bool ACROSS>
+template <class S, Across ACROSS>
 void run_product(const Halves &A, const Halves &B, int kbs_across, const HalvesProduct &p, hipStream_t s) {
     constexpr int kSlots = 256 * (8 / S::kWaves);
     Tile t = tile_args<S>(A, B);
@@ -562,6 +633,15 @@ void launch_halves_rows(const float *x, int ld, const float *weights, const Halv
     hipCheck(hipGetLastError());
 }
 
+void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s) {
+    const int64_t n = static_cast<int64_t>(h.rows) * h.terms;
+    largest_kernel<<<dim3(blocks_for(n, 16 * kThreads)), dim3(kThreads), 0, s>>>(x, n, aligned16(x), largest);
+    hipCheck(hipGetLastError());
+    halves_table_kernel<<<dim3(h.row_blocks(), (h.term_blocks() + 7) / 8), dim3(kThreads), 0, s>>>(
+        x, h.terms, h, h.terms % 4 == 0 && aligned16(x), largest);
+    hipCheck(hipGetLastError());
+}
+
 void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,
                            uint32_t *largest, hipStream_t s) {
     const int chunks = (terms + kLargestTerms - 1) / kLargestTerms;
@@ -592,14 +672,18 @@ int launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStre
 }
 
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
-    run_product<Small, false>(A, B, 0, p, s);
+    run_product<Small, Across::kNone>(A, B, 0, p, s);
 }
 
-void launch_halves_product_across(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
+// Of the operand that is read across only its size counts from here on, as it is in this product.
+void launch_product_across_a(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
     CHECK_ERROR(A.rows != B.terms || A.shift != nullptr, "Operands of %d and %d terms, or shifts by term.", A.rows, B.terms);
-    // As an operand of A.terms rows; only its size counts from here on.
-    const Halves across{A.data, nullptr, A.shift_all, A.terms, A.rows};
-    run_product<Small, true>(across, B, A.term_blocks(), p, s);
+    run_product<Small, Across::kA>({A.data, nullptr, A.shift_all, A.terms, A.rows}, B, A.term_blocks(), p, s);
+}
+
+void launch_product_across_b(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
+    CHECK_ERROR(A.terms != B.rows, "Operands of %d and %d terms.", A.terms, B.rows);
+    run_product<Small, Across::kB>(A, {B.data, B.shift, 0, B.terms, B.rows}, B.term_blocks(), p, s);
 }
 
 }  // namespace gptc

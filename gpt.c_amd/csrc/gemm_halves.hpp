@@ -55,6 +55,9 @@ __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) &
 // x (rows x terms, rows of ld floats; with weights, rows of weight 0 as zeros) into h.data and
 // h.shift; negate: as a product's first operand.
 void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s);
+// x (rows x terms without gaps) as a first operand, all rows by the shift of its largest magnitude, whose bits *largest
+// receives (0 before).
+void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
 // as a second operand, or as the one that is negated.  largest: the bits of each column's largest magnitude, which the first call raises
 // from what it holds (launch_zero_words) and which may count further terms too; null with up to
@@ -75,9 +78,11 @@ struct HalvesProduct {
     bool add;
 };
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
-// C (A.terms x B.rows) = A^T B^T for A as in another product, where it was the first operand; its shifts are one, and
-// B is negated.  A's data are readable up to 8 KB past their end.
-void launch_halves_product_across(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
+// C (A.terms x B.rows) = A^T B^T for A as in another product, where it was the first operand, with one shift; B is
+// negated.  C (A.rows x B.terms) = A B for such a B (of one shift, shift[0]).  What is read across is readable up to
+// 8 KB past its end.
+void launch_product_across_a(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
+void launch_product_across_b(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
 // C from the sums of `slices` parts of the reduction, (M, N) each, in their order.
 void launch_join_slices(const float *part, int M, int N, int slices, const HalvesProduct &p, hipStream_t s);
 

@@ -250,6 +250,8 @@ void launch_shares(ShareArgs a, hipStream_t s) {
     hipCheck(hipGetLastError());
 }
 
+constexpr int kPastEnd = 8192;  // bytes behind an operand that products across may read
+
 // Blocks of the pool for the length of a call.
 struct Scratch {
     static constexpr int kMax = 24;
@@ -263,7 +265,7 @@ struct Scratch {
     }
     Halves halves(int rows, int terms) {
         Halves h{nullptr, nullptr, 0, rows, terms};
-        h.data = take<hu32x4>(h.bytes() / 16);
+        h.data = take<hu32x4>((h.bytes() + kPastEnd) / 16);
         h.shift = take<int>(h.row_blocks() * 32);
         return h;
     }
@@ -282,23 +284,23 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     const int piece = static_cast<int>(std::min<int64_t>(h.rows, grad ? fit : kLossPiece));
     const int padded = (piece + 127) / 128 * 128;
     Scratch scratch;
+    // The largest magnitudes of the columns of x, and of W.
+    uint32_t *largest_x = scratch.take<uint32_t>(h.C + 1), *largest = largest_x + h.C;
+    if (grad) launch_zero_words(largest_x, h.C + 1, s);
+    // For dx, whose terms are its rows, W is held by one shift: to 2^-40 of its largest value where it is below the
+    // 2^-17th of that, which counts for features of dx that small.  Laid out a second time by columns it would be held to
+    // 2^-40 of each column's largest, and cost 171 us instead of XX (768 x 50257) and XX instead of XX (1600 x 50257).
     const Halves W = scratch.halves(h.V, h.C);
-    launch_halves_rows(h.W, h.C, nullptr, W, true, s);
-    // The largest magnitudes of the columns of W and x.
-    uint32_t *largest = scratch.take<uint32_t>(2 * h.C), *largest_x = largest + h.C;
-    if (grad) launch_zero_words(largest, 2 * h.C, s);
-    Halves Wt{};
-    if (h.dx != nullptr) {
-        Wt = scratch.halves(h.C, h.V);
-        launch_column_largest(h.W, h.C, nullptr, 1.0f, h.V, h.C, largest, s);
-        launch_halves_columns(h.W, h.C, nullptr, 1.0f, Wt, false, largest, s);
-    }
+    if (h.dx != nullptr)
+        launch_halves_table(h.W, W, largest, s);
+    else
+        launch_halves_rows(h.W, h.C, nullptr, W, true, s);
     Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
     if (h.dW != nullptr) {
         xt = scratch.halves(h.C, piece);
         launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest_x, s);
     }
-    if (grad) d.data = scratch.take<hu32x4>((d.bytes() + 8192) / 16);
+    if (grad) d.data = scratch.take<hu32x4>((d.bytes() + kPastEnd) / 16);
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
     float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 64));
     int *targets = scratch.take<int>(padded);
@@ -319,12 +321,12 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
                           (h.V + 63) / 64 * 2, 0};
         launch_shares(a, s);
         if (h.dx != nullptr)
-            launch_halves_product(d, Wt, {h.dx + static_cast<int64_t>(r) * h.C, h.C, weights,
+            launch_product_across_b(d, W, {h.dx + static_cast<int64_t>(r) * h.C, h.C, weights,
                                           static_cast<float>(h.rows), false},
                                   s);
         if (h.dW != nullptr) {
             launch_halves_columns(xr, h.C, weights, static_cast<float>(h.rows), xt, true, largest_x, s);
-            launch_halves_product_across(d, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
+            launch_product_across_a(d, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
         }
     }
     launch_mean(h, s);
