@@ -289,7 +289,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     if (grad) launch_zero_words(largest_x, h.C + 1, s);
     // For dx, whose terms are its rows, W is held by one shift: to 2^-40 of its largest value where it is below the
     // 2^-17th of that, which counts for features of dx that small.  Laid out a second time by columns it would be held to
-    // 2^-40 of each column's largest, and cost 171 us instead of XX (768 x 50257) and XX instead of XX (1600 x 50257).
+    // 2^-40 of each column's largest, and cost 171 us instead of 94 (50257 x 768) and 371 instead of 174 (50257 x 1600).
     const Halves W = scratch.halves(h.V, h.C);
     if (h.dx != nullptr)
         launch_halves_table(h.W, W, largest, s);
@@ -385,16 +385,22 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     scratch.release();
 }
 
-// Whether W is read as it comes.  A row costs that path about twice as much, but W is not laid out, which is
-// worth 360 rows and the time of 5e8 products of those.  Rows, vocabulary x features: us as it comes / laid out,
-// with both gradients, then the loss alone:
-//   100, 50257 x 768: 238 / 369, 78 / 143      384, 50257 x 768: 606 / 557, 188 / 193
-//   384, 50257 x 64: 183 / 203, 39 / 41        1024, 50257 x 64: 383 / 359, 70 / 67
-//   384, 5003 x 1600: 210 / 192, 83 / 83       1024, 5003 x 1600: 456 / 298, 136 / 108
-//   768, 5003 x 100: 77 / 83, 23 / 25          4096, 5003 x 100: 213 / 187, 55 / 46
-bool few_rows(int rows, int V, int C) {
+// Whether W is read as it comes.  A row costs that path about twice as much, but W is not laid out, which is worth
+// some rows and the time of some products.  Rows, vocabulary x features: us as it comes / laid out.
+// With both gradients:
+//   128, 50257 x 768: 248 / 281       384, 50257 x 768: 584 / 462
+//   192, 50257 x 64: 130 / 135        320, 50257 x 64: 169 / 151
+//   256, 5003 x 1600: 162 / 167       320, 5003 x 1600: 201 / 177
+//   512, 5003 x 100: 69 / 71          1024, 5003 x 100: 91 / 84
+// The loss alone:
+//   100, 50257 x 768: 78 / 143        512, 50257 x 768: 250 / 225
+//   384, 50257 x 64: 39 / 41          1024, 50257 x 64: 70 / 67
+//   512, 5003 x 1600: 85 / 83         1024, 5003 x 1600: 136 / 108
+//   768, 5003 x 100: 23 / 25          2048, 5003 x 100: 36 / 34
+bool few_rows(int rows, int V, int C, bool grad) {
     const int64_t weights = static_cast<int64_t>(V) * C;
-    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 && (rows - 360) * weights < 500000000;
+    const int64_t past = rows - (grad ? 190 : 360);
+    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 && past * weights < (grad ? 250000000 : 500000000);
 }
 
 }  // namespace
@@ -449,7 +455,7 @@ extern "C" void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t
     float *losses = row_losses != NULL ? row_losses->t : static_cast<float *>(alloc_cuda(sizeof(float) * rows));
     const HeadLoss h{x->t, W->t, targets->t, weights != NULL ? weights->t : nullptr, losses, output->t,
                      dx != NULL ? dx->t : nullptr, dW != NULL ? dW->t : nullptr, rows, V, C, accumulate != 0};
-    if (few_rows(rows, V, C))
+    if (few_rows(rows, V, C, dx != NULL || dW != NULL))
         run_few(h, s);
     else
         run_halves(h, s);

@@ -1,8 +1,8 @@
 """The cross entropy without logits and the sorted gradient at sizes on either side of where their kernels change, with
 the references, inputs and tolerances of test_head_loss_gpu.py and test_embed_sorted_gpu.py.
 
-W is read as it comes for up to 4096 rows while (rows - 360) V C < 5e8, else it is laid out first; there are kernels for
-32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
+W is read as it comes for up to 4096 rows while (rows - 190) V C < 2.5e8, or (rows - 360) V C < 5e8 for the loss alone,
+else it is laid out first; there are kernels for 32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
 other; the sort ranks up to 12288 rows, then goes by digits, with more rows a workgroup from 131073 on; rows that are to be overwritten are not cleared where
 min(n, V) C >= 2^23.
 """
@@ -107,3 +107,47 @@ def test_gradient_of_few_rows(rt, shape, V, C, kind, accumulate):
 def test_few_rows_are_added_in_their_order(rt):
     sorted_gpu.test_the_same_every_time(rt, (4, 250), 90, 64, "text")
     sorted_gpu.test_the_same_every_time(rt, (1, 1024), 3, 300, "two")
+
+
+@pytest.mark.parametrize("R", [438, 439, 857, 858])
+def test_where_w_is_laid_out_for_gradients(rt, R):
+    a = head.inputs(R, 50257, 20, seed=2, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False), ref)
+    head.agree(head.Call(rt, *a, dW=False), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R,V,C", [(4129, 129, 65), (5120, 384, 1), (4097, 20, 700), (4300, 1000, 129), (12345, 64, 64)])
+def test_many_rows_by_their_parts(rt, R, V, C):
+    """Each gradient alone: W is laid out by one shift for dx, by a row's for dW."""
+    a = head.inputs(R, V, C, seed=3, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a, dx=False), ref)
+    head.agree(head.Call(rt, *a, dW=False), ref)
+
+
+@pytest.mark.parametrize("R", [40, MANY])
+def test_quiet_rows_and_features_of_w(rt, R):
+    """Rows and features of W of many sizes.  For dx, W's values are held to 2^-40 of the largest of all: each share's
+    product with one is off by that, and so is each logit's."""
+    x, W, t, w = head.inputs(R, 500, 70, weights=True)
+    rng = np.random.default_rng(11)
+    W = (W * np.ldexp(1.0, rng.integers(-14, 1, (500, 1))) * np.ldexp(1.0, rng.integers(-14, 1, 70))).astype(np.float32)
+    W[7] = 0
+    W[:, 5] = 0
+    ref, got = head.Exact(x, W, t, w), head.Call(rt, x, W, t, w)
+    live = head.dev(np.where(w != 0, 1.0, 0.0))[:, None]
+    ad, f = ref.d.abs().sum(1)[:, None], (head.dev(w) / R).abs()[:, None]
+    top = float(np.abs(W).max())
+    # A logit is off by 2^-39 of `top` times its row's magnitudes more, a share by its value times twice that.
+    logit = head.END * top * head.dev(np.abs(x)).sum(1)
+    assert 4 * logit.max().item() < 1e-6
+    ref.losses_tol = ref.losses_tol + 2 * logit * live[:, 0]
+    ref.loss_tol = ref.loss_tol + (2 * logit * head.dev(np.abs(w))).sum() / R
+    share = 4 * logit[:, None] * f * live
+    ref.dx_tol = ref.dx_tol + head.END * top * ad + share * head.dev(np.abs(W)).amax(0)
+    ref.dW_tol = ref.dW_tol + (share * head.dev(np.abs(x))).amax(0)
+    head.agree(got, ref)
+    assert not got.dx[:, 5].any()
