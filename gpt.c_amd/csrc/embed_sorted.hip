@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const T *__restrict__ 
 
 // ---- sorting ----
 // The sort's launches are short and mostly wait; where dW is to be overwritten, further workgroups of
-// the same launches clear it meanwhile (8192 rows of 768 on 50257: 30 us for both, 13 for the ranking alone).
+// the same launches clear it meanwhile (8192 rows of 768 on 50257: 31 us for both, 23 for the ranking alone).
 struct Clear {
     f32x4_t *at;  // n of them from here on, by the workgroups after the first `blocks` of a launch
     int64_t n;
@@ -100,10 +100,11 @@ __device__ __forceinline__ void clear_part(const Clear &c) {
         c.at[i] = splat<f32x4_t>(0.0f);
 }
 
-// Workgroups for a part: eight waves a CU.
-int clear_blocks(const Clear &c, int threads) {
+// Workgroups for a part, up to `waves` waves in all.
+constexpr int kClearWaves = 2048;
+int clear_blocks(const Clear &c, int threads, int waves = kClearWaves) {
     const int64_t units = c.hit != nullptr ? c.n * kWave : c.n;
-    return static_cast<int>(std::min<int64_t>((units + threads - 1) / threads, 256 * 512 / threads));
+    return static_cast<int>(std::min<int64_t>((units + threads - 1) / threads, waves * kWave / threads));
 }
 
 // order[r] = (key, row) of the r-th row by (key, row); key: the id, V for rows
@@ -115,6 +116,9 @@ constexpr int kRankRows = 12288;
 constexpr int kRankThreads = 512;
 constexpr int kRankPer = 32;  // rows a workgroup
 constexpr int kRankSlices = kRankThreads / kRankPer;
+// Enough to clear while the others rank; more only fill the queues that the ids have to pass (8192 rows beside 154 MB:
+// 31 us with 512 or 768 waves, 42 with 256, 41 with 2048).
+constexpr int kRankClearWaves = 640;
 
 __global__ __launch_bounds__(kRankThreads) void rank_kernel(const float *__restrict__ ids, int n, int V,
                                                            int2 *__restrict__ order, Clear clear) {
@@ -600,7 +604,7 @@ void launch_sort(const float *ids, int n, int V, int2 *order, Clear clear, hipSt
     if (n <= kRankRows) {
         const int per = ((n + kRankSlices - 1) / kRankSlices + 3) & ~3;
         clear.blocks = (n + kRankPer - 1) / kRankPer;
-        rank_kernel<<<dim3(clear.blocks + clear_blocks(clear, kRankThreads)), dim3(kRankThreads),
+        rank_kernel<<<dim3(clear.blocks + clear_blocks(clear, kRankThreads, kRankClearWaves)), dim3(kRankThreads),
                       static_cast<size_t>(per) * kRankSlices * sizeof(uint32_t), s>>>(ids, n, V, order, clear);
         hipCheck(hipGetLastError());
         return;

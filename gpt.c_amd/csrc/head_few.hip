@@ -290,11 +290,13 @@ void run_few(const FewArgs &a, int across, hipStream_t s) {
 // (Halves).  A workgroup keeps its 128 columns of x in LDS and its waves stream blocks of 32 tokens.
 template <int KB>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void few_dw_kernel(
-    const Halves dt, const Halves xt, const HalvesProduct p) {
+    const Halves dt, const Halves xt, const HalvesProduct p, int columns) {
     __shared__ hu32x4 lds[4 * KB * 128];
     const int lane = threadIdx.x & 63, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const hu32x4 *from = xt.data + static_cast<int64_t>(blockIdx.x) * (4 * KB * 128);
+    // The workgroups that read the same blocks of d^T and write the same rows go to one XCD (workgroup i runs on XCD i % 8).
+    const int turn = blockIdx.x >> 3, column = turn % columns, group = turn / columns * 8 + static_cast<int>(blockIdx.x & 7);
+    const hu32x4 *from = xt.data + static_cast<int64_t>(column) * (4 * KB * 128);
     {
         constexpr int kPer = 4 * KB * 128 / kThreads;
         hu32x4 v[kPer];
@@ -303,8 +305,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int i = 0; i < kPer; ++i) lds[threadIdx.x + i * kThreads] = v[i];
     }
-    const int blocks = (dt.rows + 31) / 32, stride = gridDim.y * kFewWaves;
-    int m = blockIdx.y * kFewWaves + w;
+    const int blocks = (dt.rows + 31) / 32, stride = static_cast<int>(gridDim.x) / columns * kFewWaves;
+    int m = group * kFewWaves + w;
     hu32x4 a[KB][2];
     auto load = [&](int block) {
         const hu32x4 *at = dt.data + static_cast<int64_t>(min(block, blocks - 1)) * (KB * 128) + lane;
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             const __amdgpu_buffer_rsrc_t C = __builtin_amdgcn_make_buffer_rsrc(
                 p.C + static_cast<int64_t>(m) * 32 * p.ldc, 0, bytes, 0x00020000);
             auto row_at = [&](int r) { return min(4 * (8 * (r >> 2) + (r & 3)) * p.ldc, bytes); };
-            const int c = blockIdx.x * 128 + 32 * j + (lane & 31);
+            const int c = column * 128 + 32 * j + (lane & 31);
             const int up = -dt.shift_all - xt.shift[c];
             const uint32_t mine = c < xt.rows ? 4 * (static_cast<uint32_t>(4 * hf) * p.ldc + c) : 0x80000000u;
             float old[16];
@@ -406,10 +408,10 @@ void launch_few_dw(const Halves &dt, const Halves &xt, const HalvesProduct &p, h
     CHECK_ERROR(dt.terms != xt.terms || dt.terms > kFewDwTerms || p.ldc >= 1 << 22, "few_dw: %d and %d terms, rows of %d.",
                 dt.terms, xt.terms, p.ldc);
     const int columns = (xt.rows + 127) / 128, blocks = (dt.rows + 31) / 32;
-    // Two workgroups a CU.
-    const int rows = std::max(1, std::min((blocks + kFewWaves - 1) / kFewWaves, 512 / columns));
+    // Two workgroups a CU, the same number for each XCD.
+    const int groups = std::max(1, std::min((blocks + 8 * kFewWaves - 1) / (8 * kFewWaves), 64 / columns)) * 8;
     auto kernel = dt.term_blocks() == 4 ? few_dw_kernel<4> : few_dw_kernel<8>;
-    kernel<<<dim3(columns, rows), dim3(kThreads), 0, s>>>(dt, xt, p);
+    kernel<<<dim3(columns * groups), dim3(kThreads), 0, s>>>(dt, xt, p, columns);
     hipCheck(hipGetLastError());
 }
 
