@@ -11,7 +11,7 @@ typedef float hf32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t hu32x4 __attribute__((ext_vector_type(4)));
 
 // An operand of `rows` (of the product's M or N) by `terms` (of its reduction),
-// padded with zeros to rows of 256 and terms of 32.  Row r's values are held
+// padded with zeros to 128 rows and 64 terms.  Row r's values are held
 // times 2^shift[r], which puts the largest below 2^15: value = high + low to
 // 2^-24 of it, or to 2^-40 of the row's largest for values below its 2^-17th.
 // Blocks of 32 rows x 16 terms, block (r / 32, k / 16) after block, high part
@@ -48,8 +48,8 @@ __device__ __forceinline__ void halves_split(float x, float y, uint32_t &high, u
           static_cast<uint32_t>(__builtin_bit_cast(uint16_t, ly)) << 16;
 }
 
-// Negating every other step of 32 terms of one of a product's operands (the first) keeps the
-// matrix core's truncation from adding up: the kernels subtract those steps.
+// Negating every other 64 terms of one of a product's operands keeps the matrix core's truncation
+// from adding up: the kernels subtract those sums.
 __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) & 1) != 0; }
 
 // x (rows x terms, rows of ld floats; with weights, rows of weight 0 as zeros) into h.data and
@@ -59,8 +59,8 @@ void launch_halves_rows(const float *x, int ld, const float *weights, const Halv
 // receives (0 before).
 void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
-// as a second operand, or as the one that is negated.  largest: the bits of each column's largest magnitude, which the first call raises
-// from what it holds (launch_zero_words) and which may count further terms too; null with up to
+// as a second operand, or as the one that is negated.  largest: the bits of each column's largest magnitude, which the
+// first call raises from what it holds (launch_zero_words) and which may count further terms too; null with up to
 // kColumnTerms terms, whose largest the second call finds by itself.
 constexpr int kColumnTerms = 128;
 void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,

@@ -258,8 +258,14 @@ void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tenso
  *   (rows) or NULL for ones.  A row of weight 0 takes no part, whatever its x
  *   and target hold (padding): loss 0, dx 0.  With other weights a target
  *   outside [0, V) gives a NaN loss and the softmax part of the gradients, as
- *   cross_entropy_*_cuda_kernel.  V < 2^22.  Results may not overlap another
- *   tensor of the call.  Deterministic.  Takes scratch: not under graph capture.
+ *   cross_entropy_*_cuda_kernel.  Values of x and W are held to 24 bits where
+ *   they are not far smaller than the largest of their row of x, row of W (of
+ *   all of W where dx is asked for and rows are many) or column of x, else to
+ *   2^-40 of that largest one.  W is taken to be finite: a value that is not
+ *   makes the loss NaN.  A row of x that is not finite spoils its own loss and
+ *   dx, output and dW.  V < 2^22.  Results may not overlap another tensor of
+ *   the call.  Deterministic.  Takes scratch (the logits of up to 3328 rows of
+ *   50257 at a time, and W's copy): not under graph capture.
  *
  * gptc_embedding_forward_scaled_cuda(W, pos, ids, scale, output)
  *   output (ids..., C) = scale W[ids] (+ pos[i], i the id's place in ids' last
@@ -270,8 +276,8 @@ void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tenso
  *   id, dpos (positions, C), or NULL, = sum of global_grad over each place of
  *   ids' last dimension; overwritten (zeros where nothing falls), or added to
  *   when `accumulate`.  Ids outside [0, V) count for dpos alone.
- *   Rows are sorted by id and added in their order, long runs in parts of fixed
- *   lengths: deterministic, but not embedding_backward_cuda_kernel's one chain.
+ *   An id's rows are added in their order, long runs in parts of fixed lengths:
+ *   deterministic, but not embedding_backward_cuda_kernel's one chain.
  *   Takes scratch: not under graph capture.
  */
 void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t *W, const tensor_t *targets,
