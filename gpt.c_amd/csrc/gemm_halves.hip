@@ -290,15 +290,22 @@ struct Tile {
 
 __device__ __forceinline__ int shift_of(const int *shift, int all, int row) { return shift != nullptr ? shift[row] : all; }
 
-// The tile of this workgroup: 8 contiguous ranges of tiles, one per XCD (workgroup i runs on XCD
-// i % 8); in a range, columns of 8 row tiles, so that the tiles that run together share rows
-// and columns.
-__device__ __forceinline__ void tile_of(const Tile &t, int &tm, int &tn) {
-    const int n = t.tiles_m * t.tiles_n;
+// The tile and slice of this workgroup (grid: tiles by slices, or slices of few tiles one after the other).  Workgroup i
+// runs on XCD i % 8: 8 contiguous ranges of a slice's tiles, or of all slices' where those are few (so that a slice's
+// operands go to one L2 or two), one per XCD.  In a range, columns of G row tiles, so that the tiles that run together
+// share rows and columns.  Few columns come one after the other (G = 1): the workgroups of a row start one by one as
+// others end, and what lies between them has to stay in the L2.
+__device__ __forceinline__ void tile_of(const Tile &t, int &tm, int &tn, int &slice) {
+    const int tiles = t.tiles_m * t.tiles_n, n = gridDim.x;
     int i = blockIdx.x;
     const int x = i & 7, q = n >> 3, r = n & 7;
     i = (i >> 3) + x * q + min(x, r);
-    const int G = 8, per = G * t.tiles_n;
+    slice = blockIdx.y;
+    if (n > tiles) {
+        slice = i / tiles;
+        i -= slice * tiles;
+    }
+    const int G = t.tiles_n <= 8 ? 1 : 8, per = G * t.tiles_n;
     const int g = i / per, first = g * G, h = min(G, t.tiles_m - first);
     const int in = i - g * per;
     tm = first + in % h;
@@ -459,8 +466,8 @@ template <class S>
 __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void logits_kernel(
     const Tile t, const LogitsArgs l) {
     __shared__ hu32x4 lds[2 * S::kStage / 16];
-    int tm, tn;
-    tile_of(t, tm, tn);
+    int tm, tn, slice;
+    tile_of(t, tm, tn, slice);
     hf32x16 acc[S::NI][2];
     tile_product<S, Across::kNone>(t, tm, tn, 0, t.stages, lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
@@ -503,10 +510,10 @@ template <class S, Across ACROSS>
 __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
     const Tile t, const ProductArgs a) {
     __shared__ hu32x4 lds[2 * S::kStage / 16];
-    int tm, tn;
-    tile_of(t, tm, tn);
+    int tm, tn, slice;
+    tile_of(t, tm, tn, slice);
     hf32x16 acc[S::NI][2];
-    const int s0 = blockIdx.y * t.slice;
+    const int s0 = slice * t.slice;
     tile_product<S, ACROSS>(t, tm, tn, s0, min(t.stages, s0 + t.slice), lds, acc);
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -534,7 +541,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
         }
         // The block's rows of C or of the slice's part; what lies past the last row or column is neither read nor written.
         const int ld = a.part != nullptr ? a.N : a.p.ldc;
-        float *C = a.part != nullptr ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.N : a.p.C;
+        float *C = a.part != nullptr ? a.part + static_cast<int64_t>(slice) * a.M * a.N : a.p.C;
         const int bytes = 4 * min(32, a.M - first) * ld;
         const __amdgpu_buffer_rsrc_t rows =
             __builtin_amdgcn_make_buffer_rsrc(C + static_cast<int64_t>(first) * ld, 0, bytes, 0x00020000);
@@ -619,7 +626,10 @@ void run_product(const Halves &A, const Halves &B, int kbs_across, const HalvesP
     const int slices = (t.stages + t.slice - 1) / t.slice;
     ProductArgs a{p, A.rows, B.rows, nullptr};
     if (slices > 1) a.part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(A.rows) * B.rows * slices));
-    product_kernel<S, ACROSS><<<dim3(tiles, slices), dim3(S::kThreads), 0, s>>>(t, a);
+    // dx with its slices one after the other / side by side: 1024 rows of 768 (48 tiles) 252 / 265 us, 3328 rows (156
+    // tiles) 638 / 643, 2000 rows of 1600 (208 tiles) 975 / 943.
+    const bool in_turn = tiles <= 3 * kSlots / 8;
+    product_kernel<S, ACROSS><<<in_turn ? dim3(tiles * slices) : dim3(tiles, slices), dim3(S::kThreads), 0, s>>>(t, a);
     hipCheck(hipGetLastError());
     if (slices == 1) return;
     launch_join_slices(a.part, A.rows, B.rows, slices, p, s);
