@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kMaxGroups = 1 << 24;  // a launch's threads are counted in 32 bits
 
 // An id held in a float, truncated; -1 for what is not in [0, V).
 __device__ __forceinline__ int id_of(float f, int V) {
@@ -670,7 +671,7 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
             f.clears = static_cast<int>(std::max<int64_t>((a.V + kClearRows - 1) / kClearRows,
                                                           std::min<int64_t>(512, (bytes + 16383) / 16384)));
         const int64_t grid = static_cast<int64_t>(f.position_blocks + a.n) * a.blocks + f.clears;
-        CHECK_ERROR(grid > INT32_MAX / 2, "Too many rows and columns for one call: %d x %d.", a.n, a.C);
+        CHECK_ERROR(grid >= kMaxGroups, "Too many positions for one call: %d x %d.", a.positions, a.C);
         gather_few_kernel<T><<<dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s>>>(f);
         hipCheck(hipGetLastError());
         return;
@@ -679,8 +680,10 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
     a.chunk = 32;
     while (a.chunk > 8 && static_cast<int64_t>(a.n) * a.blocks < 2048ll * a.chunk) a.chunk /= 2;
     const int chunks = (a.n + a.chunk - 1) / a.chunk;
-    const int64_t items = (static_cast<int64_t>(chunks) + (a.dP != nullptr ? a.positions : 0) + 2 * kWaves) * a.blocks;
-    CHECK_ERROR(items > INT32_MAX / 2, "Too many rows and columns for one call: %d x %d.", a.n, a.C);
+    const int position_blocks = a.dP != nullptr ? (a.positions + kWaves - 1) / kWaves : 0;
+    const int per = position_blocks + (chunks + kWaves - 1) / kWaves;
+    CHECK_ERROR(static_cast<int64_t>(std::max(per, chunks)) * a.blocks >= kMaxGroups,
+                "Too many rows or positions for one call: %d, %d x %d.", a.n, a.positions, a.C);
     int2 *order = static_cast<int2 *>(alloc_cuda(sizeof(int2) * static_cast<size_t>(a.n)));
     a.part = static_cast<float *>(alloc_cuda(sizeof(float) * 2 * static_cast<size_t>(chunks) * a.C));
     a.order = order;
@@ -695,8 +698,6 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
         }
     }
     launch_sort(ids, a.n, a.V, order, clear, s);
-    const int position_blocks = a.dP != nullptr ? (a.positions + kWaves - 1) / kWaves : 0;
-    const int per = position_blocks + (chunks + kWaves - 1) / kWaves;
     gather_kernel<T><<<dim3(per * a.blocks), dim3(kThreads), 0, s>>>(a, chunks);
     hipCheck(hipGetLastError());
     if (chunks > 1) {

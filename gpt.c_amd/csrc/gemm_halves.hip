@@ -195,16 +195,16 @@ __global__ __launch_bounds__(kThreads) void column_largest_kernel(const float *_
     constexpr int kW = sizeof(T) / sizeof(float);
     __shared__ uint32_t red[64 * kW];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int c = (blockIdx.x * 64 + lane) * kW;
+    const int c = (blockIdx.y * 64 + lane) * kW;
     for (int i = threadIdx.x; i < 64 * kW; i += kThreads) red[i] = 0;
     __syncthreads();
     if (c < cols) {
         float m[kW];
 #pragma unroll
         for (int e = 0; e < kW; ++e) m[e] = 0.0f;
-        const int k1 = min(terms, static_cast<int>(blockIdx.y + 1) * kLargestTerms);
+        const int k1 = min(terms, static_cast<int>(blockIdx.x + 1) * kLargestTerms);
 #pragma unroll 8
-        for (int k = blockIdx.y * kLargestTerms + w; k < k1; k += 4) {
+        for (int k = blockIdx.x * kLargestTerms + w; k < k1; k += 4) {
             const T v = *reinterpret_cast<const T *>(x + static_cast<int64_t>(k) * ld + c);
             const float f = term_factor(weights, divisor, k);
 #pragma unroll
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void column_largest_kernel(const float *_
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * kW; i += kThreads) {
-        const int at = blockIdx.x * 64 * kW + i;
+        const int at = blockIdx.y * 64 * kW + i;
         if (at < cols && red[i] != 0) atomicMax(largest + at, red[i]);
     }
 }
@@ -663,10 +663,10 @@ void launch_column_largest(const float *x, int ld, const float *weights, float d
                            uint32_t *largest, hipStream_t s) {
     const int chunks = (terms + kLargestTerms - 1) / kLargestTerms;
     if (ld % 4 == 0 && cols % 4 == 0 && aligned16(x))
-        column_largest_kernel<f32x4_t><<<dim3((cols + 255) / 256, chunks), dim3(kThreads), 0, s>>>(
+        column_largest_kernel<f32x4_t><<<dim3(chunks, (cols + 255) / 256), dim3(kThreads), 0, s>>>(
             x, ld, weights, divisor, terms, cols, largest);
     else
-        column_largest_kernel<float><<<dim3((cols + 63) / 64, chunks), dim3(kThreads), 0, s>>>(x, ld, weights, divisor,
+        column_largest_kernel<float><<<dim3(chunks, (cols + 63) / 64), dim3(kThreads), 0, s>>>(x, ld, weights, divisor,
                                                                                               terms, cols, largest);
     hipCheck(hipGetLastError());
 }

@@ -151,3 +151,26 @@ def test_quiet_rows_and_features_of_w(rt, R):
     ref.dW_tol = ref.dW_tol + (share * head.dev(np.abs(x))).amax(0)
     head.agree(got, ref)
     assert not got.dx[:, 5].any()
+
+
+def test_millions_of_rows(rt):
+    """Launches whose workgroups pass 65535 in one direction, and four pieces of rows."""
+    a = head.inputs(4200000, 3, 2, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_more_positions_than_the_ids_have(rt, n, accumulate):
+    """A table of positions far longer than the sequences: the rest is zero, or left as it was."""
+    rng = np.random.default_rng(6)
+    g = rng.standard_normal((2, n, 3)).astype(np.float32)
+    ids = sorted_gpu.ids_of("uniform", (2, n), 50)
+    before = rng.standard_normal((300000, 3)).astype(np.float32)
+    _, dP = sorted_gpu.gather(rt, g, ids, 1.0, np.zeros((50, 3), np.float32), before, accumulate)
+    want = g.astype(np.float64).sum(0) + (before[:n] if accumulate else 0)
+    tol = 3 * sorted_gpu.U * (np.abs(g).sum(0) + np.abs(before[:n]))
+    sorted_gpu.close("dP", dP[:n], want, tol)
+    assert np.array_equal(dP[n:], before[n:] if accumulate else np.zeros_like(before[n:]))
