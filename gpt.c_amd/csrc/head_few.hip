@@ -2,14 +2,14 @@
 //
 // Reading W is the time there (154 MB for GPT-2 small's, 29 us at the rate of a large
 // copy), so W is read as it comes and each of its floats split once for up to 128
-// rows: into three bf16 parts, which need no common scale, and six products of parts
-// (the terms of order 2^-16 and larger; sums as in gemm_split.hip; what lies below
-// 2^-133 is lost).  The other operand is small; its parts are formed once, in the order
-// of the fragments.
+// rows.  The parts are those of gemm_halves.hpp, two fp16 values by a common scale; W's
+// is the largest value of a row (logits) or column (d W) within a step of 32 terms,
+// whose products are summed apart and come into the sum times that scale.  The other
+// operand is small; its parts are formed once, in the order of the fragments.
 //
-// 768 features, 50257 tokens: 16 rows' logits 28 us (5.5 TB/s), where W comes from HBM 35;
-// 100 rows' 66 to 72, d W 58 to 62: there the six products of 128 rows take 50 at the rate
-// of the library's bf16 product.
+// 768 features, 50257 tokens: 16 rows' logits 28 us (5.5 TB/s), where W comes from HBM 35
+// to 37; 100 rows' 58, d W 47.  With three bf16 parts, which need no scale but six products
+// instead of three, those took 70 and 60.
 #include <algorithm>
 #include "gpu_kernels.h"
 #include "head_loss.hpp"
@@ -20,78 +20,69 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kFewWaves = 4;
-constexpr int kProd[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-
-__device__ __forceinline__ hf32x16 mfma_bf16(hu32x4 a, hu32x4 b, hf32x16 c) {
-    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                   0, 0);
-}
-
 __device__ __forceinline__ hf32x16 mfma_f16(hu32x4 a, hu32x4 b, hf32x16 c) {
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Eight floats as a fragment's three parts.
-__device__ __forceinline__ void split8(const float (&v)[8], hu32x4 (&f)[3]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        uint32_t p[3];
-        thirds_split(v[2 * e], v[2 * e + 1], p);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) f[q][e] = p[q];
-    }
-}
-
 // The terms that lane l holds of block kb of x and W's rows, hf = l / 32: a step's two blocks are 64 consecutive
-// bytes of a row for either half of the lanes, so that a step's loads take whole lines of 128 bytes at once.
-// (In the order of Halves each line was asked for four times, and left the L1 cache in between.)
-__device__ __forceinline__ int x_term_of(int kb, int hf, int e) { return (kb >> 1) * 32 + 16 * hf + 8 * (kb & 1) + e; }
-
-// A wave a block of 32 rows x 16 terms.
-__global__ __launch_bounds__(kThreads) void thirds_rows_kernel(const float *__restrict__ x,
-                                                              const float *__restrict__ weights, int rows, Thirds t) {
-    const int lane = threadIdx.x & 63, hf = lane >> 5, kbs = t.term_blocks();
-    const int kb = blockIdx.x * kFewWaves + static_cast<int>(threadIdx.x >> 6), rb = blockIdx.y;
-    if (kb >= kbs) return;
-    const int row = rb * 32 + (lane & 31);
+// bytes of a row for either half of the lanes,
+//   k = 32 (kb / 2) + 16 hf + 8 (kb % 2) + {0 .. 7}.
+// A wave a row; its first kRowsKeep * 256 terms stay in registers, the others are read again for their parts.
+constexpr int kRowsKeep = 4;
+__global__ __launch_bounds__(kThreads) void few_rows_kernel(const float *__restrict__ x,
+                                                           const float *__restrict__ weights, int rows, bool vec,
+                                                           FewRows t) {
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x * kFewWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool live = row < rows && (weights == nullptr || weights[row] != 0.0f);
-    float v[8];
+    const float *p = x + static_cast<int64_t>(row) * t.terms;
+    auto four = [&](int k) {
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vec) {
+            if (live && k < t.terms) v = *reinterpret_cast<const f32x4_t *>(p + k);
+        } else if (live) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int k = x_term_of(kb, hf, e);
-        const float y = live && k < t.terms ? x[static_cast<int64_t>(row) * t.terms + k] : 0.0f;
-        v[e] = (kb >> 1) & 1 ? -y : y;
-    }
-    hu32x4 f[3];
-    split8(v, f);
-    hu32x4 *out = t.data + (static_cast<int64_t>(rb) * kbs + kb) * 192 + lane;
+            for (int e = 0; e < 4; ++e) v[e] = k + e < t.terms ? p[k + e] : 0.0f;
+        }
+        return v;
+    };
+    f32x4_t own[kRowsKeep];
+    float top = 0.0f;
+    auto larger = [&](f32x4_t v) {
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    };
 #pragma unroll
-    for (int q = 0; q < 3; ++q) out[q * 64] = f[q];
+    for (int i = 0; i < kRowsKeep; ++i) own[i] = four(256 * i + 4 * lane);
+#pragma unroll 4
+    for (int k = 256 * kRowsKeep + 4 * lane; k < t.terms; k += 256) larger(four(k));
+#pragma unroll
+    for (int i = 0; i < kRowsKeep; ++i) larger(own[i]);
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const int up = halves_shift(top), kbs = t.term_blocks();
+    if (lane == 0) t.shift[row] = up;
+    uint2 *out = reinterpret_cast<uint2 *>(t.data + static_cast<int64_t>(row >> 5) * kbs * 128 + (row & 31));
+    auto put = [&](int k, f32x4_t v) {
+        if (k >= 16 * kbs) return;
+        const uint32_t flip = halves_negated(k) ? 0x80008000u : 0;
+        uint2 high, low;
+        halves_split(__builtin_amdgcn_ldexpf(v[0], up), __builtin_amdgcn_ldexpf(v[1], up), high.x, low.x);
+        halves_split(__builtin_amdgcn_ldexpf(v[2], up), __builtin_amdgcn_ldexpf(v[3], up), high.y, low.y);
+        const int kb = 2 * (k >> 5) + ((k >> 3) & 1), hf = (k >> 4) & 1;
+        uint2 *at = out + 2 * (kb * 128 + 32 * hf) + ((k >> 2) & 1);
+        at[0] = make_uint2(high.x ^ flip, high.y ^ flip);
+        at[2 * 64] = make_uint2(low.x ^ flip, low.y ^ flip);
+    };
+#pragma unroll
+    for (int i = 0; i < kRowsKeep; ++i) put(256 * i + 4 * lane, own[i]);
+    for (int k = 256 * kRowsKeep + 4 * lane; k < 16 * kbs; k += 256) put(k, four(k));
 }
 
-// acc[i] += sign a[i] b (or b a[i]) over a step of 32 terms (two blocks), each a fresh sum, smallest products first.
-template <int N, bool A_FIRST>
-__device__ __forceinline__ void add_products(const hu32x4 (&a)[2][N][3], const hu32x4 (&b)[2][3], float sign,
-                                             hf32x16 (&acc)[N]) {
-    hf32x16 t[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) t[i][r] = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 6; ++q)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                t[i] = A_FIRST ? mfma_bf16(a[k][i][kProd[q][0]], b[k][kProd[q][1]], t[i])
-                               : mfma_bf16(b[k][kProd[q][0]], a[k][i][kProd[q][1]], t[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] = fmaf(sign, t[i][r], acc[i][r]);
+// The larger one of lanes l and l ^ 32.
+__device__ __forceinline__ float across_halves(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
 }
 
 // A kilobyte to LDS at `to` by loads that write no register (the compiler does not count them, so that its own
@@ -130,7 +121,7 @@ struct RowsOfW {
 struct FewArgs {
     const float *W;
     int V, C;
-    Thirds small;  // x or d
+    FewRows small;  // x or d
     LogitsArgs l;
     int rows, slice, columns;  // of the gradient: blocks of 16 tokens a workgroup, workgroups side by side
     float *part;
@@ -139,15 +130,15 @@ struct FewArgs {
 // 128 tokens (logits) or 128 columns (the gradient, DX) by 32 NB rows a workgroup, 32 by up to 64 a wave.  Both
 // operands go to LDS, kDepth - 1 steps of 32 terms ahead: the waves share the small one, and W's rows come in
 // whole lines (a lane a row, as the fragments want them, costs a cycle of the address path for every lane: the
-// logits of 16 rows of 768 on 50257 tokens took 39 us so and take 28).  Up to four waves a SIMD: a wave alone
-// on its SIMD needs 4060 cycles for a step whose matrix instructions take 1536.
+// logits of 16 rows of 768 on 50257 tokens took 39 us so and take 28).  Up to four waves a SIMD, which hide
+// each other's chain of loads, largest value, split and products.
 template <int NB>
 struct FewShape {
     static constexpr int kBlocks = NB < 2 ? NB : 2;                     // of 32 rows a wave
     static constexpr int kWaves = 4 * NB / kBlocks;
-    static constexpr int kSmall = NB * 384, kStage = kSmall + 4 * 256;  // 16-byte chunks
-    static constexpr int kDepth = NB == 1 ? 3 : 2;                      // two workgroups a CU in 160 KB
-    static constexpr int kLoadsSmall = (NB * 6 + kWaves - 1) / kWaves, kLoadsW = 16 / kWaves;  // kilobytes of a wave
+    static constexpr int kSmall = NB * 256, kStage = kSmall + 4 * 256;  // 16-byte chunks
+    static constexpr int kDepth = NB == 1 ? 4 : NB == 2 ? 3 : 2;                    // two workgroups a CU in 160 KB
+    static constexpr int kLoadsSmall = NB * 4 / kWaves, kLoadsW = 16 / kWaves;  // kilobytes of a wave
 };
 
 template <int NB, bool DX>
@@ -172,7 +163,7 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
     const int steps = count / 2;
     const RowsOfW rows(a.W, a.V, a.C, DX ? first * 16 : at128 * 128);
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
-    const hu32x4 *small = a.small.data + (static_cast<int64_t>(rb) * kbs + first) * 192;
+    const hu32x4 *small = a.small.data + (static_cast<int64_t>(rb) * kbs + first) * 128;
 
     // Kilobyte q of W's 16 of a step.  Logits: eight rows' 128 bytes, whose 16-byte chunk c lies at c ^ (row / 2 % 8).
     // Gradient: two rows' 512 bytes, whose columns change places with the next 32 in every other four rows.  So a
@@ -188,8 +179,8 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
         const uint32_t to = base + buffer * (S::kStage * 16);
 #pragma unroll
         for (int i = 0; i < S::kLoadsSmall; ++i) {
-            const int c = min(w + i * S::kWaves, NB * 6 - 1);  // a kilobyte of block c / 6
-            load_kilobyte(small + (static_cast<int64_t>(c / 6) * kbs + 2 * step) * 192 + (c % 6) * 64, lane * 16,
+            const int c = w + i * S::kWaves;  // a kilobyte of block c / 4
+            load_kilobyte(small + (static_cast<int64_t>(c / 4) * kbs + 2 * step) * 128 + (c % 4) * 64, lane * 16,
                           to + c * 1024);
         }
 #pragma unroll
@@ -206,54 +197,106 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
 #pragma unroll
     for (int d = 0; d + 1 < S::kDepth; ++d) load_stage(min(d, steps - 1), d);
-    float sign = 1.0f;
     int buffer = 0, free_buffer = S::kDepth - 1;
     for (int step = 0; step < steps; ++step) {
         // This step's loads have landed, all waves', and the buffer of the step before has been read.
-        static_assert(S::kDepth == 2 || (S::kDepth == 3 && S::kLoadsSmall + S::kLoadsW == 6), "the waits");
-        if constexpr (S::kDepth == 3)
+        constexpr int kLoads = S::kLoadsSmall + S::kLoadsW;
+        constexpr int kAhead = (S::kDepth - 2) * kLoads;
+        static_assert(kAhead == 0 || kAhead == 6 || kAhead == 10, "the waits");
+        if constexpr (kAhead == 0)
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else if constexpr (kAhead == 6)
             asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         load_stage(min(step + S::kDepth - 1, steps - 1), free_buffer);
         const hu32x4 *at = lds + buffer * S::kStage;
-        hu32x4 f[2][3], g[2][S::kBlocks][3];
+        float v[2][8];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            float v[8];
             if (DX) {
                 const float *p = reinterpret_cast<const float *>(at + S::kSmall) + 4 * hf * 128 + (mine ^ hf) * 32 + l32;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = p[(16 * k + (e & 3) + 8 * (e >> 2)) * 128];
+                for (int e = 0; e < 8; ++e) v[k][e] = p[(16 * k + (e & 3) + 8 * (e >> 2)) * 128];
             } else {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const hu32x4 c = at[S::kSmall + mine * 256 + l32 * 8 + ((4 * hf + 2 * k + e) ^ (l32 >> 1 & 7))];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[4 * e + i] = __uint_as_float(c[i]);
+                    for (int i = 0; i < 4; ++i) v[k][4 * e + i] = __uint_as_float(c[i]);
                 }
             }
-            split8(v, f[k]);
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
+        top = across_halves(top);
+        const int up = min(halves_shift(top), 126);
+        hf32x16 t[S::kBlocks];
+#pragma unroll
+        for (int i = 0; i < S::kBlocks; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[i][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            hu32x4 f[2], g[S::kBlocks][2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t hi, lo;
+                halves_split(__builtin_amdgcn_ldexpf(v[k][2 * e], up), __builtin_amdgcn_ldexpf(v[k][2 * e + 1], up), hi, lo);
+                f[0][e] = hi;
+                f[1][e] = lo;
+            }
 #pragma unroll
             for (int i = 0; i < S::kBlocks; ++i)
 #pragma unroll
-                for (int q = 0; q < 3; ++q)
-                    g[k][i][q] = at[((w >> 2) * S::kBlocks + i) * 384 + k * 192 + q * 64 + lane];
+                for (int q = 0; q < 2; ++q)
+                    g[i][q] = at[((w >> 2) * S::kBlocks + i) * 256 + k * 128 + q * 64 + lane];
+            constexpr int kParts[3][2] = {{1, 0}, {0, 1}, {0, 0}};  // smallest products first
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+#pragma unroll
+                for (int i = 0; i < S::kBlocks; ++i) t[i] = mfma_f16(g[i][kParts[q][0]], f[kParts[q][1]], t[i]);
         }
-        add_products<S::kBlocks, DX>(g, f, sign, acc);
-        sign = -sign;
+        const float down = __builtin_amdgcn_ldexpf(step & 2 ? -1.0f : 1.0f, -up);  // 64 terms of a sign
+#pragma unroll
+        for (int i = 0; i < S::kBlocks; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][r] = fmaf(down, t[i][r], acc[i][r]);
         free_buffer = buffer;
         buffer = buffer + 1 == S::kDepth ? 0 : buffer + 1;
     }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");  // from here on `lds` is free
     const int block = rb + (w >> 2) * S::kBlocks;
+    // A lane holds a token (or column) and 16 rows.  The logits are put with a row a lane, and change over in LDS.
+    constexpr int kStride = 36;  // words of a row
     float2 *stats = reinterpret_cast<float2 *>(lds);  // (blocks of 32 rows, the four waves' tokens, rows)
+    float *across = reinterpret_cast<float *>(stats + NB * 128) + w * (32 * kStride);
+    static_assert(DX || NB * 1024 + S::kWaves * 32 * kStride * 4 <= S::kDepth * S::kStage * 16, "room");
     // In a loop over the blocks, whose sums move up: code that runs once a wave is paid by its fetch.
 #pragma unroll 1
     for (int i = 0; i < S::kBlocks; ++i) {
         hf32x16 v[1] = {acc[0]};
         if (S::kBlocks == 2) acc[0] = acc[S::kBlocks - 1];
         if (!DX) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int4 back = *reinterpret_cast<const int4 *>(a.small.shift + (block + i) * 32 + 8 * q + 4 * hf);
+                const int shift[4] = {back.x, back.y, back.z, back.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    across[(8 * q + 4 * hf + e) * kStride + l32] = __builtin_amdgcn_ldexpf(v[0][4 * q + e], -shift[e]);
+            }
+            wave_lds_order();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4_t x = *reinterpret_cast<const f32x4_t *>(across + l32 * kStride + 8 * q + 4 * hf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[0][4 * q + e] = x[e];
+            }
+            wave_lds_order();
             const float2 stat = put_logits<1>(a.l, v, at128 * 128 + mine * 32, block + i);
             if (hf == 0) stats[((w >> 2) * S::kBlocks + i) * 128 + mine * 32 + l32] = stat;
             continue;
@@ -265,8 +308,9 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
         const uint32_t lane_out = c < a.C ? 4 * (static_cast<uint32_t>((block + i) * 32 + 4 * hf) * a.C + c) : 0x80000000u;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0][r]), out, lane_out,
-                                                  min(4 * (8 * (r >> 2) + (r & 3)) * a.C, bytes), 0);
+            __builtin_amdgcn_raw_buffer_store_b32(
+                __float_as_uint(__builtin_amdgcn_ldexpf(v[0][r], -a.small.shift_all)), out, lane_out,
+                min(4 * (8 * (r >> 2) + (r & 3)) * a.C, bytes), 0);
     }
     if (DX) return;
     __syncthreads();
@@ -382,18 +426,18 @@ int few_row_blocks(int rows) {
     return blocks <= 2 ? blocks : (blocks + 3) / 4 * 4;
 }
 
-void launch_thirds_rows(const float *x, const float *weights, int rows, const Thirds &t, hipStream_t s) {
-    thirds_rows_kernel<<<dim3((t.term_blocks() + kFewWaves - 1) / kFewWaves, t.row_blocks), dim3(kThreads), 0, s>>>(
-        x, weights, rows, t);
+void launch_few_rows(const float *x, const float *weights, int rows, const FewRows &t, hipStream_t s) {
+    few_rows_kernel<<<dim3(t.row_blocks * 32 / kFewWaves), dim3(kThreads), 0, s>>>(
+        x, weights, rows, t.terms % 4 == 0 && aligned16(x), t);
     hipCheck(hipGetLastError());
 }
 
-int launch_few_logits(const float *W, int V, int C, const Thirds &x, const LogitsArgs &l, hipStream_t s) {
+int launch_few_logits(const float *W, int V, int C, const FewRows &x, const LogitsArgs &l, hipStream_t s) {
     run_few<false>({W, V, C, x, l, 0, 0, 0, nullptr}, l.token_blocks / 4, s);
     return 128;
 }
 
-void launch_few_dx(const Thirds &d, const float *W, int V, int C, int rows, const HalvesProduct &p, hipStream_t s) {
+void launch_few_dx(const FewRows &d, const float *W, int V, int C, int rows, const HalvesProduct &p, hipStream_t s) {
     CHECK_ERROR(static_cast<int64_t>(rows) * C >= 1 << 29, "few_dx: %d x %d results.", rows, C);
     const int groups = d.row_blocks <= 2 ? 1 : d.row_blocks / 4, columns = (C + 127) / 128, kbs = d.term_blocks();
     // About two workgroups a CU, at least 128 terms each; a slice's offsets stay within 32 bits.

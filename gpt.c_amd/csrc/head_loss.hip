@@ -143,7 +143,6 @@ struct ShareArgs {
     const float *logits, *lse;
     const int *targets;
     hu32x4 *d, *dt;  // as first operands of d W and d^T x; either may be null
-    hu32x4 *thirds;  // or d in three bf16 parts, for few rows
     int row_blocks, token_blocks;  // of the logits
     int rows_used, tokens_used;    // blocks that the products' reductions reach
     int per_wave;                  // blocks of tokens a wave
@@ -179,23 +178,6 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
                 const float p = __builtin_amdgcn_exp2f((v[q][e] - lse) * kLog2eF);
                 v[q][e] = p - (jb * 32 + 8 * q + 4 * hf + e == target ? 1.0f : 0.0f);
             }
-        if (a.thirds != nullptr) {
-            const float scale = jb & 1 ? -1.0f : 1.0f;
-            hu32x4 *out = a.thirds + (static_cast<int64_t>(rb) * a.token_blocks + jb) * 384 + lane;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                hu32x4 f[3];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t p[3];
-                    thirds_split(scale * v[2 * k + (e >> 1)][2 * (e & 1)], scale * v[2 * k + (e >> 1)][2 * (e & 1) + 1], p);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) f[i][e] = p[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 3; ++i) out[(3 * k + i) * 64] = f[i];
-            }
-        }
         uint32_t high[4][2], low[4][2];
         constexpr float kUp = static_cast<float>(1 << kShareShift);
 #pragma unroll
@@ -317,7 +299,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
                            n_padded, h.V, nullptr},
                           s);
         if (!grad) continue;
-        const ShareArgs a{logits, lse, targets, d.data, nullptr, nullptr, n_padded / 32, tokens / 32, 0,
+        const ShareArgs a{logits, lse, targets, d.data, nullptr, n_padded / 32, tokens / 32, 0,
                           (h.V + 63) / 64 * 2, 0};
         launch_shares(a, s);
         if (h.dx != nullptr)
@@ -341,16 +323,15 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     // dt's terms are whole pairs of blocks.
     const int blocks = std::max(few_row_blocks(h.rows), h.dW != nullptr ? 2 : 1), padded = blocks * 32;
     Scratch scratch;
-    const Thirds x{nullptr, blocks, h.C}, d{nullptr, blocks, tokens};
-    Thirds xs = x, ds = d;
-    xs.data = scratch.take<hu32x4>(x.bytes() / 16);
-    launch_thirds_rows(h.x, h.weights, h.rows, xs, s);
+    FewRows x{nullptr, scratch.take<int>(padded), 0, blocks, h.C}, d{nullptr, nullptr, kShareShift, blocks, tokens};
+    x.data = scratch.take<hu32x4>(x.bytes() / 16);
+    launch_few_rows(h.x, h.weights, h.rows, x, s);
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
     float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 32));
     int *targets = scratch.take<int>(padded);
     float *target_logits = scratch.take<float>(padded), *lse = scratch.take<float>(padded);
     const int part = launch_few_logits(
-        h.W, h.V, h.C, xs, {logits, stats, h.targets, target_logits, h.V, h.rows, tokens / 32, padded}, s);
+        h.W, h.V, h.C, x, {logits, stats, h.targets, target_logits, h.V, h.rows, tokens / 32, padded}, s);
     const bool mean = h.rows <= kMeanRows && padded == kMeanRows;
     launch_join_stats({stats, tokens / part, h.targets, target_logits, h.weights, lse, targets, h.losses, h.rows, padded,
                        h.V, mean ? h.mean : nullptr},
@@ -358,13 +339,13 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     if (!mean) launch_mean(h, s);
     if (grad) {
         Halves dt{nullptr, nullptr, kShareShift, h.V, h.rows}, xt{};
-        if (h.dx != nullptr) ds.data = scratch.take<hu32x4>(d.bytes() / 16);
+        if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / 16);
         if (h.dW != nullptr) dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
-        launch_shares({logits, lse, targets, nullptr, dt.data, ds.data, blocks, tokens / 32, dt.term_blocks() / 2,
+        launch_shares({logits, lse, targets, d.data, dt.data, blocks, tokens / 32, dt.term_blocks() / 2,
                        tokens / 32, 0},
                       s);
         if (h.dx != nullptr)
-            launch_few_dx(ds, h.W, h.V, h.C, h.rows,
+            launch_few_dx(d, h.W, h.V, h.C, h.rows,
                           {h.dx, h.C, h.weights, static_cast<float>(h.rows), false}, s);
         if (h.dW != nullptr) {
             xt = scratch.halves(h.C, h.rows);
@@ -385,22 +366,24 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     scratch.release();
 }
 
-// Whether W is read as it comes.  A row costs that path about twice as much, but W is not laid out, which is worth
-// some rows and the time of some products.  Rows, vocabulary x features: us as it comes / laid out.
+// Whether W is read as it comes, again for every 128 rows and with a split of each float, instead of laid out first.
+// Rows, vocabulary x features: us as it comes / laid out.
 // With both gradients:
-//   128, 50257 x 768: 248 / 281       384, 50257 x 768: 584 / 462
-//   192, 50257 x 64: 130 / 135        320, 50257 x 64: 169 / 151
-//   256, 5003 x 1600: 162 / 167       320, 5003 x 1600: 201 / 177
-//   512, 5003 x 100: 69 / 71          1024, 5003 x 100: 91 / 84
+//   256, 50257 x 768: 330 / 367       384, 50257 x 768: 475 / 452
+//   384, 50257 x 256: 215 / 246       512, 50257 x 256: 286 / 280
+//   384, 50257 x 64: 144 / 155        768, 50257 x 64: 254 / 222
+//   512, 5003 x 1600: 171 / 191       768, 5003 x 1600: 236 / 228
+//   1024, 1000 x 768: 97 / 101        1536, 1000 x 768: 112 / 102
+//   1024, 5003 x 100: 82 / 81         4095, 5003 x 100: 173 / 154
 // The loss alone:
-//   100, 50257 x 768: 78 / 143        512, 50257 x 768: 250 / 225
-//   384, 50257 x 64: 39 / 41          1024, 50257 x 64: 70 / 67
-//   512, 5003 x 1600: 85 / 83         1024, 5003 x 1600: 136 / 108
-//   768, 5003 x 100: 23 / 25          2048, 5003 x 100: 36 / 34
+//   100, 50257 x 768: 62 / 140        768, 50257 x 768: 270 / 279       1024, 50257 x 768: 349 / 335
+//   512, 50257 x 64: 41 / 44          1024, 50257 x 64: 63 / 61
+//   768, 5003 x 1600: 74 / 89         1536, 5003 x 1600: 121 / 121
+//   2048, 5003 x 100: 32 / 34         4095, 5003 x 100: 45 / 46
 bool few_rows(int rows, int V, int C, bool grad) {
-    const int64_t weights = static_cast<int64_t>(V) * C;
-    const int64_t past = rows - (grad ? 190 : 360);
-    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 && past * weights < (grad ? 250000000 : 500000000);
+    const int64_t read = (rows + 127) / 128 * 128, room = 2400000000 / (V * (C + 100ll));
+    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 &&
+           read <= (grad ? 256 + std::min<int64_t>(900, room) : 768 + room);
 }
 
 }  // namespace

@@ -70,40 +70,25 @@ __device__ __forceinline__ float2 put_logits(const LogitsArgs &l, hf32x16 (&x)[N
 // A = W (vocabulary x features), B = x (rows x features).  Returns the tokens of each of the stats' parts.
 int launch_logits(const Halves &A, const Halves &B, const LogitsArgs &l, hipStream_t s);
 
-// An operand of few rows as three bf16 parts a float (every other step of 32 terms negated),
-// padded with zeros to 32 terms: blocks of 32 rows x 16 terms, a kilobyte for each part.  d's terms lie as
-// in Halves, x's as head_few.hip reads W's rows.
-struct Thirds {
+// An operand of few rows in two fp16 parts, as Halves, but padded to row_blocks of 32 rows and 32 terms.  d's terms lie as
+// there, x's as head_few.hip reads W's rows.
+struct FewRows {
     hu32x4 *data;
+    int *shift;  // (padded rows), or null: every row's is `shift_all`
+    int shift_all;
     int row_blocks, terms;
     __host__ __device__ int term_blocks() const { return (terms + 31) / 32 * 2; }
-    __host__ __device__ int64_t bytes() const { return static_cast<int64_t>(row_blocks) * term_blocks() * (3 << 10); }
+    __host__ __device__ int64_t bytes() const { return static_cast<int64_t>(row_blocks) * term_blocks() * 2048; }
 };
-
-typedef float thirds_f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 thirds_bf16x2 __attribute__((ext_vector_type(2)));
-
-// x and y as the sums of their three bf16 parts (packed): each the nearest of what is left.
-__device__ __forceinline__ void thirds_split(float x, float y, uint32_t (&p)[3]) {
-    auto pack = [](float a, float b) {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(thirds_f32x2{a, b}, thirds_bf16x2));
-    };
-    auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
-    auto high = [](uint32_t v) { return __uint_as_float(v & 0xffff0000u); };
-    p[0] = pack(x, y);
-    const float x1 = x - low(p[0]), y1 = y - high(p[0]);
-    p[1] = pack(x1, y1);
-    p[2] = pack(x1 - low(p[1]), y1 - high(p[1]));
-}
 
 // Blocks of 32 rows that launch_few_logits and launch_few_dx take for this many rows.
 int few_row_blocks(int rows);
-// x (rows x terms without gaps) into t; rows of weight 0 as zeros.
-void launch_thirds_rows(const float *x, const float *weights, int rows, const Thirds &t, hipStream_t s);
+// x (rows x terms without gaps) into t, rows of weight 0 as zeros.
+void launch_few_rows(const float *x, const float *weights, int rows, const FewRows &t, hipStream_t s);
 // The logits of x (V x C floats W as they come).  Returns the tokens of each of the stats' parts.
-int launch_few_logits(const float *W, int V, int C, const Thirds &x, const LogitsArgs &l, hipStream_t s);
+int launch_few_logits(const float *W, int V, int C, const FewRows &x, const LogitsArgs &l, hipStream_t s);
 // p.C (rows x C) = d W by the rows' factors.
-void launch_few_dx(const Thirds &d, const float *W, int V, int C, int rows, const HalvesProduct &p, hipStream_t s);
+void launch_few_dx(const FewRows &d, const float *W, int V, int C, int rows, const HalvesProduct &p, hipStream_t s);
 
 // p.C (dt.rows x xt.rows) = d^T x (+ p.C) for up to kFewDwTerms rows; p without factors.
 constexpr int kFewDwTerms = 128;

@@ -1,8 +1,8 @@
 """The cross entropy without logits and the sorted gradient at sizes on either side of where their kernels change, with
 the references, inputs and tolerances of test_head_loss_gpu.py and test_embed_sorted_gpu.py.
 
-W is read as it comes for up to 4096 rows while (rows - 190) V C < 2.5e8, or (rows - 360) V C < 5e8 for the loss alone,
-else it is laid out first; there are kernels for 32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
+W is read as it comes for few rows, up to 4096: as a multiple of 128, up to 256 + min(900, 2.4e9 / (V (C + 100))), or
+768 + 2.4e9 / (V (C + 100)) for the loss alone; else it is laid out first; there are kernels for 32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
 other; the sort ranks up to 12288 rows, then goes by digits, with more rows a workgroup from 131073 on; rows that are to be overwritten are not cleared where
 min(n, V) C >= 2^23.
 """
@@ -174,3 +174,32 @@ def test_more_positions_than_the_ids_have(rt, n, accumulate):
     tol = 3 * sorted_gpu.U * (np.abs(g).sum(0) + np.abs(before[:n]))
     sorted_gpu.close("dP", dP[:n], want, tol)
     assert np.array_equal(dP[n:], before[n:] if accumulate else np.zeros_like(before[n:]))
+
+
+@pytest.mark.parametrize("R", [640, 641, 1152, 1153])
+def test_where_w_is_laid_out_by_128_rows(rt, R):
+    a = head.inputs(R, 50257, 20, seed=4, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R,V,C", [(3, 300, 1024), (5, 200, 1028), (33, 130, 2052), (65, 257, 1027), (130, 500, 1300)])
+def test_few_rows_of_many_features(rt, R, V, C):
+    """Rows of x that do not fit a wave's registers."""
+    a = head.inputs(R, V, C, seed=5, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R", [7, 90])
+def test_few_rows_where_w_changes_size(rt, R):
+    """Steps of 32 tokens, and of 32 features, whose largest values are far apart: each has a scale of its own."""
+    x, W, t, w = head.inputs(R, 900, 200, weights=True)
+    rng = np.random.default_rng(12)
+    W = (W * np.ldexp(1.0, rng.integers(-20, 1, (29, 1))).repeat(32, 0)[:900]).astype(np.float32)
+    W[64:96] = 0
+    W[200:232, 32:64] = 1e-38
+    a = x, W, t, w
+    head.agree(head.Call(rt, *a), head.Exact(*a))
