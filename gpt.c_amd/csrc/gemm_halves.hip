@@ -41,77 +41,59 @@ __device__ __forceinline__ hf32x16 mfma(hu32x4 a, hu32x4 b, hf32x16 c) {
 
 // ---- operands ----
 
-// One block of 32 rows a workgroup; the four waves take terms in turns.  Reads x twice, the second time from the
-// caches (768 x 50257: 90 us, 309 MB in and out once).
-__global__ __launch_bounds__(kThreads) void halves_rows_kernel(const float *__restrict__ x, int ld,
-                                                              const float *__restrict__ weights, Halves h, bool negate,
-                                                              bool vec) {
-    __shared__ int shift[32];
-    const int rb = blockIdx.x, tid = threadIdx.x;
-    const int lane = tid & 63, w = tid >> 6;
-    {  // eight threads a row find its largest value
-        const int row = rb * 32 + (tid >> 3);
-        const bool live = row < h.rows && (weights == nullptr || weights[row] != 0.0f);
-        const float *p = x + static_cast<int64_t>(row) * ld;
-        float m = 0.0f;
-        if (live) {
-            if (vec) {
-#pragma unroll 8
-                for (int k = 4 * (tid & 7); k < h.terms; k += 32) {
-                    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p + k);
-                    m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
-                }
-            } else {
-#pragma unroll 8
-                for (int k = tid & 7; k < h.terms; k += 8) m = fmaxf(m, fabsf(p[k]));
-            }
+// A wave a row, which is read once: its first kRowsKeep * 256 terms stay in registers (the others are read again for their
+// parts).  A workgroup's eight rows fill lines of 128 bytes.  8192 rows of 768 in three pieces: 24 us.
+constexpr int kRowsWaves = 8;
+constexpr int kRowsKeep = 4;
+__global__ __launch_bounds__(64 * kRowsWaves) void halves_rows_kernel(const float *__restrict__ x,
+                                                                     const float *__restrict__ weights, int rows,
+                                                                     int terms, bool vec, HalvesRows t) {
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x * kRowsWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool live = row < rows && (weights == nullptr || weights[row] != 0.0f);
+    const float *p = x + static_cast<int64_t>(row) * terms;
+    auto four = [&](int k) {
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vec) {
+            if (live && k < terms) v = *reinterpret_cast<const f32x4_t *>(p + k);
+        } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = k + e < terms ? p[k + e] : 0.0f;
         }
-        m = fmaxf(m, __shfl_xor(m, 1, 64));
-        m = fmaxf(m, __shfl_xor(m, 2, 64));
-        m = fmaxf(m, __shfl_xor(m, 4, 64));
-        if ((tid & 7) == 0) {
-            shift[tid >> 3] = halves_shift(m);
-            h.shift[row] = halves_shift(m);
-        }
-    }
-    __syncthreads();
-    const int row = rb * 32 + (lane & 31), hf = lane >> 5, kbs = h.term_blocks();
-    const bool live = row < h.rows && (weights == nullptr || weights[row] != 0.0f);
-    const float *p = x + static_cast<int64_t>(live ? row : 0) * ld;
-    const int up = shift[lane & 31];
-    hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs * 2) * 64 + lane;
+        return v;
+    };
+    f32x4_t own[kRowsKeep];
+    float top = 0.0f;
+    auto larger = [&](f32x4_t v) {
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    };
+#pragma unroll
+    for (int i = 0; i < kRowsKeep; ++i) own[i] = four(256 * i + 4 * lane);
 #pragma unroll 4
-    for (int kb = w; kb < kbs; kb += 4) {
-        const int k0 = kb * 16 + 4 * hf;
-        float v[8];
-        if (vec && k0 + 12 <= h.terms) {
-            const f32x4_t a = *reinterpret_cast<const f32x4_t *>(p + k0), b = *reinterpret_cast<const f32x4_t *>(p + k0 + 8);
+    for (int k = 256 * kRowsKeep + 4 * lane; k < terms; k += 256) larger(four(k));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = a[e];
-                v[4 + e] = b[e];
-            }
-        } else {
+    for (int i = 0; i < kRowsKeep; ++i) larger(own[i]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int k = k0 + (e & 3) + 8 * (e >> 2);
-                v[e] = k < h.terms ? p[k] : 0.0f;
-            }
-        }
-        const bool minus = negate && halves_negated(kb * 16);
-        hu32x4 high, low;
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const int up = halves_shift(top);
+    if (lane == 0) t.shift[row] = up;
+    uint2 *out = reinterpret_cast<uint2 *>(t.data + static_cast<int64_t>(row >> 5) * t.term_blocks * 128 + (row & 31));
+    auto put = [&](int k, f32x4_t v) {
+        if (k >= 16 * t.term_blocks) return;
+        const uint32_t flip = t.negate && halves_negated(k) ? 0x80008000u : 0;
+        uint2 high, low;
+        halves_split(__builtin_amdgcn_ldexpf(v[0], up), __builtin_amdgcn_ldexpf(v[1], up), high.x, low.x);
+        halves_split(__builtin_amdgcn_ldexpf(v[2], up), __builtin_amdgcn_ldexpf(v[3], up), high.y, low.y);
+        // Block, lanes' half and place in 16 bytes of term k = 32 j + 16 a + 8 b + 4 c.
+        const int j = k >> 5, a = (k >> 4) & 1, b = (k >> 3) & 1, c = (k >> 2) & 1;
+        const int kb = 2 * j + (t.in_lines ? b : a), hf = t.in_lines ? a : c, half = t.in_lines ? c : b;
+        uint2 *at = out + 2 * (kb * 128 + 32 * hf) + half;
+        at[0] = make_uint2(high.x ^ flip, high.y ^ flip);
+        at[2 * 64] = make_uint2(low.x ^ flip, low.y ^ flip);
+    };
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float a = live ? __builtin_amdgcn_ldexpf(v[2 * e], up) : 0.0f;
-            float b = live ? __builtin_amdgcn_ldexpf(v[2 * e + 1], up) : 0.0f;
-            uint32_t hi, lo;
-            halves_split(minus ? -a : a, minus ? -b : b, hi, lo);
-            high[e] = hi;
-            low[e] = lo;
-        }
-        out[(kb * 2) * 64] = high;
-        out[(kb * 2 + 1) * 64] = low;
-    }
+    for (int i = 0; i < kRowsKeep; ++i) put(256 * i + 4 * lane, own[i]);
+    for (int k = 256 * kRowsKeep + 4 * lane; k < 16 * t.term_blocks; k += 256) put(k, four(k));
 }
 
 // largest[0] = bits of the largest magnitude of n values so far (768 x 50257: 42 us, 3.7 TB/s of reads alone).
@@ -644,10 +626,14 @@ void launch_join_slices(const float *part, int M, int N, int slices, const Halve
     hipCheck(hipGetLastError());
 }
 
-void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s) {
-    const bool vec = ld % 4 == 0 && h.terms % 4 == 0 && aligned16(x);
-    halves_rows_kernel<<<dim3(h.row_blocks()), dim3(kThreads), 0, s>>>(x, ld, weights, h, negate, vec);
+void launch_rows(const float *x, const float *weights, int rows, int terms, const HalvesRows &t, hipStream_t s) {
+    halves_rows_kernel<<<dim3(t.row_blocks * 32 / kRowsWaves), dim3(64 * kRowsWaves), 0, s>>>(
+        x, weights, rows, terms, terms % 4 == 0 && aligned16(x), t);
     hipCheck(hipGetLastError());
+}
+
+void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, hipStream_t s) {
+    launch_rows(x, weights, h.rows, h.terms, {h.data, h.shift, h.row_blocks(), h.term_blocks(), negate, false}, s);
 }
 
 void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s) {

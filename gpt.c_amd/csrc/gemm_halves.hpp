@@ -52,9 +52,18 @@ __device__ __forceinline__ void halves_split(float x, float y, uint32_t &high, u
 // from adding up: the kernels subtract those sums.
 __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) & 1) != 0; }
 
-// x (rows x terms, rows of ld floats; with weights, rows of weight 0 as zeros) into h.data and
-// h.shift; negate: as a product's first operand.
-void launch_halves_rows(const float *x, int ld, const float *weights, const Halves &h, bool negate, hipStream_t s);
+// x (rows x terms without gaps; with weights, rows of weight 0 as zeros) into h.data and h.shift; negate: as a product's
+// first operand.
+void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, hipStream_t s);
+// The same for other paddings, and (in_lines) another order of a block's terms: lane l of blocks 2 j and 2 j + 1 holds
+// 32 j + 16 (l / 32) + {0 .. 7} and {8 .. 15}, a step's 64 consecutive bytes for either half of the lanes.
+struct HalvesRows {
+    hu32x4 *data;
+    int *shift;
+    int row_blocks, term_blocks;  // of 32 and of 16
+    bool negate, in_lines;
+};
+void launch_rows(const float *x, const float *weights, int rows, int terms, const HalvesRows &t, hipStream_t s);
 // x (rows x terms without gaps) as a first operand, all rows by the shift of its largest magnitude, whose bits *largest
 // receives (0 before).
 void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s);

@@ -25,60 +25,6 @@ __device__ __forceinline__ hf32x16 mfma_f16(hu32x4 a, hu32x4 b, hf32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// The terms that lane l holds of block kb of x and W's rows, hf = l / 32: a step's two blocks are 64 consecutive
-// bytes of a row for either half of the lanes,
-//   k = 32 (kb / 2) + 16 hf + 8 (kb % 2) + {0 .. 7}.
-// A wave a row; its first kRowsKeep * 256 terms stay in registers, the others are read again for their parts.
-constexpr int kRowsKeep = 4;
-__global__ __launch_bounds__(kThreads) void few_rows_kernel(const float *__restrict__ x,
-                                                           const float *__restrict__ weights, int rows, bool vec,
-                                                           FewRows t) {
-    const int lane = threadIdx.x & 63;
-    const int row = blockIdx.x * kFewWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool live = row < rows && (weights == nullptr || weights[row] != 0.0f);
-    const float *p = x + static_cast<int64_t>(row) * t.terms;
-    auto four = [&](int k) {
-        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (vec) {
-            if (live && k < t.terms) v = *reinterpret_cast<const f32x4_t *>(p + k);
-        } else if (live) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = k + e < t.terms ? p[k + e] : 0.0f;
-        }
-        return v;
-    };
-    f32x4_t own[kRowsKeep];
-    float top = 0.0f;
-    auto larger = [&](f32x4_t v) {
-        top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    };
-#pragma unroll
-    for (int i = 0; i < kRowsKeep; ++i) own[i] = four(256 * i + 4 * lane);
-#pragma unroll 4
-    for (int k = 256 * kRowsKeep + 4 * lane; k < t.terms; k += 256) larger(four(k));
-#pragma unroll
-    for (int i = 0; i < kRowsKeep; ++i) larger(own[i]);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    const int up = halves_shift(top), kbs = t.term_blocks();
-    if (lane == 0) t.shift[row] = up;
-    uint2 *out = reinterpret_cast<uint2 *>(t.data + static_cast<int64_t>(row >> 5) * kbs * 128 + (row & 31));
-    auto put = [&](int k, f32x4_t v) {
-        if (k >= 16 * kbs) return;
-        const uint32_t flip = halves_negated(k) ? 0x80008000u : 0;
-        uint2 high, low;
-        halves_split(__builtin_amdgcn_ldexpf(v[0], up), __builtin_amdgcn_ldexpf(v[1], up), high.x, low.x);
-        halves_split(__builtin_amdgcn_ldexpf(v[2], up), __builtin_amdgcn_ldexpf(v[3], up), high.y, low.y);
-        const int kb = 2 * (k >> 5) + ((k >> 3) & 1), hf = (k >> 4) & 1;
-        uint2 *at = out + 2 * (kb * 128 + 32 * hf) + ((k >> 2) & 1);
-        at[0] = make_uint2(high.x ^ flip, high.y ^ flip);
-        at[2 * 64] = make_uint2(low.x ^ flip, low.y ^ flip);
-    };
-#pragma unroll
-    for (int i = 0; i < kRowsKeep; ++i) put(256 * i + 4 * lane, own[i]);
-    for (int k = 256 * kRowsKeep + 4 * lane; k < 16 * kbs; k += 256) put(k, four(k));
-}
-
 // The larger one of lanes l and l ^ 32.
 __device__ __forceinline__ float across_halves(float x) {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -427,9 +373,7 @@ int few_row_blocks(int rows) {
 }
 
 void launch_few_rows(const float *x, const float *weights, int rows, const FewRows &t, hipStream_t s) {
-    few_rows_kernel<<<dim3(t.row_blocks * 32 / kFewWaves), dim3(kThreads), 0, s>>>(
-        x, weights, rows, t.terms % 4 == 0 && aligned16(x), t);
-    hipCheck(hipGetLastError());
+    launch_rows(x, weights, rows, t.terms, {t.data, t.shift, t.row_blocks, t.term_blocks(), true, true}, s);
 }
 
 int launch_few_logits(const float *W, int V, int C, const FewRows &x, const LogitsArgs &l, hipStream_t s) {

@@ -268,15 +268,13 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     Scratch scratch;
     // The largest magnitudes of the columns of x, and of W.
     uint32_t *largest_x = scratch.take<uint32_t>(h.C + 1), *largest = largest_x + h.C;
-    if (grad) launch_zero_words(largest_x, h.C + 1, s);
-    // For dx, whose terms are its rows, W is held by one shift: to 2^-40 of its largest value where it is below the
-    // 2^-17th of that, which counts for features of dx that small.  Laid out a second time by columns it would be held to
-    // 2^-40 of each column's largest, and cost 171 us instead of 94 (50257 x 768) and 371 instead of 174 (50257 x 1600).
+    launch_zero_words(largest_x, h.C + 1, s);
+    // W is held by one shift, as its rows are the terms of dx: to 2^-40 of its largest value where it is below the 2^-17th
+    // of that, which counts for features of dx that small.  Laid out by rows and, for dx, a second time by columns it would
+    // be held to 2^-40 of each row's and column's largest, and cost 171 us instead of 90 (50257 x 768) and 371 instead of
+    // 169 (50257 x 1600).
     const Halves W = scratch.halves(h.V, h.C);
-    if (h.dx != nullptr)
-        launch_halves_table(h.W, W, largest, s);
-    else
-        launch_halves_rows(h.W, h.C, nullptr, W, true, s);
+    launch_halves_table(h.W, W, largest, s);
     Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
     if (h.dW != nullptr) {
         xt = scratch.halves(h.C, piece);
@@ -292,7 +290,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         const float *xr = h.x + static_cast<int64_t>(r) * h.C;
         const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
         x.rows = d.rows = xt.terms = n;
-        launch_halves_rows(xr, h.C, weights, x, false, s);
+        launch_halves_rows(xr, weights, x, false, s);
         const int part = launch_logits(
             W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
         launch_join_stats({stats, tokens / part, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n,

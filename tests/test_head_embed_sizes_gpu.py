@@ -121,7 +121,7 @@ def test_where_w_is_laid_out_for_gradients(rt, R):
 
 @pytest.mark.parametrize("R,V,C", [(4129, 129, 65), (5120, 384, 1), (4097, 20, 700), (4300, 1000, 129), (12345, 64, 64)])
 def test_many_rows_by_their_parts(rt, R, V, C):
-    """Each gradient alone: W is laid out by one shift for dx, by a row's for dW."""
+    """Each gradient alone."""
     a = head.inputs(R, V, C, seed=3, weights=True)
     ref = head.Exact(*a)
     head.agree(head.Call(rt, *a, dx=False), ref)
