@@ -71,7 +71,9 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const T *__restrict__ 
 
 // ---- sorting ----
 // The sort's launches are short and mostly wait; where dW is to be overwritten, further workgroups of
-// the same launches clear it meanwhile (8192 rows of 768 on 50257: 31 us for both, 23 for the ranking alone).
+// the same launches clear it meanwhile (8192 rows of 768 on 50257: 23 us for the ranking alone).  What is written of dW is
+// marked as not to be read again soon, here and in the sums: the caches keep the rows that are read twice (the call 53 us
+// without the marks, 40 with them; 65536 rows of 1600: 224, 208).
 struct Clear {
     f32x4_t *at;  // n of them from here on, by the workgroups after the first `blocks` of a launch
     int64_t n;
@@ -92,17 +94,17 @@ __device__ __forceinline__ void clear_part(const Clear &c) {
             uint64_t left = __ballot(mine < c.n && c.hit[min(mine, c.n - 1)] == 0);
             for (; left != 0; left &= left - 1) {
                 f32x4_t *row = c.at + (r0 + __builtin_ctzll(left) * waves) * c.units;
-                for (int j = lane; j < c.units; j += kWave) row[j] = splat<f32x4_t>(0.0f);
+                for (int j = lane; j < c.units; j += kWave) __builtin_nontemporal_store(splat<f32x4_t>(0.0f), row + j);
             }
         }
         return;
     }
     const int64_t stride = static_cast<int64_t>(gridDim.x - c.blocks) * blockDim.x;
     for (int64_t i = static_cast<int64_t>(blockIdx.x - c.blocks) * blockDim.x + threadIdx.x; i < c.n; i += stride)
-        c.at[i] = splat<f32x4_t>(0.0f);
+        __builtin_nontemporal_store(splat<f32x4_t>(0.0f), c.at + i);
 }
 
-// Workgroups for a part, up to `waves` waves in all.
+// Workgroups for a part, up to `waves` waves in all (65536 rows of 1600: 208 us with 2048, 220 with 512).
 constexpr int kClearWaves = 2048;
 int clear_blocks(const Clear &c, int threads, int waves = kClearWaves) {
     const int64_t units = c.hit != nullptr ? c.n * kWave : c.n;
@@ -118,9 +120,9 @@ constexpr int kRankRows = 12288;
 constexpr int kRankThreads = 512;
 constexpr int kRankPer = 32;  // rows a workgroup
 constexpr int kRankSlices = kRankThreads / kRankPer;
-// Enough to clear while the others rank; more only fill the queues that the ids have to pass (8192 rows beside 154 MB:
-// 31 us with 512 or 768 waves, 42 with 256, 41 with 2048).
-constexpr int kRankClearWaves = 640;
+// Enough to clear while the others rank; more only fill the queues that the ids have to pass (8192 rows of 768 on 50257:
+// the call 40 us with 512 waves, 47 with 384, 42 with 640, 51 with 2048).
+constexpr int kRankClearWaves = 512;
 
 __global__ __launch_bounds__(kRankThreads) void rank_kernel(const float *__restrict__ ids, int n, int V,
                                                            int2 *__restrict__ order, Clear clear) {
@@ -425,7 +427,8 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(const GatherArgs a, in
                     if (open)
                         part[cols + col] = sum;
                     else
-                        dW[id * cols + col] = a.add ? fma_of(a.scale, sum, old[k]) : a.scale * sum;
+                        __builtin_nontemporal_store(a.add ? fma_of(a.scale, sum, old[k]) : a.scale * sum,
+                                                    dW + id * cols + col);
                 }
                 open = false;
                 sum = splat<T>(0.0f);
@@ -532,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void gather_few_kernel(const FewArgs f) {
         for (int v = w; v < count; v += kWaves) {
             if ((named[v / 32] >> (v % 32)) & 1) continue;
             T *row = dW + static_cast<int64_t>(first + v) * cols;
-            for (int j = lane; j < cols; j += kWave) row[j] = splat<T>(0.0f);
+            for (int j = lane; j < cols; j += kWave) __builtin_nontemporal_store(splat<T>(0.0f), row + j);
         }
         return;
     }

@@ -472,7 +472,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 for (int e = 0; e < 4; ++e) x[i][4 * q + e] = __builtin_amdgcn_ldexpf(x[i][4 * q + e], -up - shift[e]);
             }
         }
-        const float2 stat = put_logits<S::NI>(l, x, token0, (row0 >> 5) + j);
+        const float2 stat = put_logits<S::NI, true>(l, x, token0, (row0 >> 5) + j);
         if (hf == 0) l.stats[static_cast<int64_t>(token0 / (S::NI * 32)) * l.row_stride + row0 + 32 * j + l32] = stat;
     }
 }
@@ -546,7 +546,8 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[r]), rows, mine, row_at(r), 0);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[r]), rows, mine, row_at(r),
+                                                  ACROSS == Across::kA ? kStreamed : 0);
     }
 }
 

@@ -28,6 +28,10 @@ struct Halves {
     __host__ __device__ int64_t bytes() const { return static_cast<int64_t>(row_blocks()) * term_blocks() * 2048; }
 };
 
+// The cache hint of stores whose values are not read again soon: dW's, beside which W stays in the caches (100 rows of 768
+// on 50257: 183 us without it, 174 with it; 1024 rows: 872, 868).
+constexpr int kStreamed = 2;
+
 constexpr int kHalvesTop = 14;  // the largest value of a row is held below 2^(kHalvesTop + 1)
 
 // The shift of a row whose largest magnitude is m (0, infinities and NaN: as they are).

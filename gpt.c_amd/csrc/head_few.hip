@@ -243,7 +243,7 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
                 for (int e = 0; e < 4; ++e) v[0][4 * q + e] = x[e];
             }
             wave_lds_order();
-            const float2 stat = put_logits<1>(a.l, v, at128 * 128 + mine * 32, block + i);
+            const float2 stat = put_logits<1, false>(a.l, v, at128 * 128 + mine * 32, block + i);
             if (hf == 0) stats[((w >> 2) * S::kBlocks + i) * 128 + mine * 32 + l32] = stat;
             continue;
         }
@@ -280,8 +280,8 @@ void run_few(const FewArgs &a, int across, hipStream_t s) {
     hipCheck(hipGetLastError());
 }
 
-// dW = d^T x for up to 16 KB terms (rows): writing dW is the time (100 rows of 768 on 50257: 49 us for 154 MB out and
-// 26 in; 55 without the order by XCD).  Both operands come as two fp16 parts (Halves).  A workgroup keeps its 128 columns of x in LDS and its waves stream blocks of 32 tokens.
+// dW = d^T x for up to 16 KB terms (rows): writing dW is the time (100 rows of 768 on 50257: 40 us for 154 MB out and
+// 26 in; 7 more without the order by XCD, 8 more without the stores' hint).  Both operands come as two fp16 parts (Halves).  A workgroup keeps its 128 columns of x in LDS and its waves stream blocks of 32 tokens.
 template <int KB>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void few_dw_kernel(
     const Halves dt, const Halves xt, const HalvesProduct p, int columns) {
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                 if (KB == 8) v -= t[KB / 4 - 1][r];
                 v = __builtin_amdgcn_ldexpf(v, up);
                 if (p.add) v = old[r] + v;
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), C, mine, row_at(r), 0);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), C, mine, row_at(r), kStreamed);
             }
         }
     }
