@@ -501,6 +501,24 @@ constexpr int kFewRows = 1024;
 constexpr int kFewItems = kFewRows / kThreads;  // ids a thread
 constexpr int kClearRows = 1 << 13;             // of a workgroup, at most
 
+// A wave: `cols` values from `row` on to zero, in whole 16 bytes where they may be and there are many (176 rows of 346 on
+// 50257: 16.7 us, by floats 21.3; 256 of 17: 16.0, by floats 10.5).
+__device__ __forceinline__ void clear_row(f32x4_t *row, int cols) {
+    for (int j = threadIdx.x & (kWave - 1); j < cols; j += kWave) __builtin_nontemporal_store(splat<f32x4_t>(0.0f), row + j);
+}
+__device__ __forceinline__ void clear_row(float *row, int cols) {
+    const int lane = threadIdx.x & (kWave - 1);
+    if (cols <= 2 * kWave) {
+        for (int j = lane; j < cols; j += kWave) row[j] = 0.0f;
+        return;
+    }
+    const int before = min(cols, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) / 4 & 3));
+    const int units = (cols - before) / 4, behind = before + 4 * units;
+    if (lane < before) row[lane] = 0.0f;
+    if (lane < cols - behind) row[behind + lane] = 0.0f;
+    clear_row(reinterpret_cast<f32x4_t *>(row + before), units);
+}
+
 struct FewArgs {
     GatherArgs a;
     const float *ids;
@@ -534,8 +552,7 @@ __global__ __launch_bounds__(kThreads) void gather_few_kernel(const FewArgs f) {
         __syncthreads();
         for (int v = w; v < count; v += kWaves) {
             if ((named[v / 32] >> (v % 32)) & 1) continue;
-            T *row = dW + static_cast<int64_t>(first + v) * cols;
-            for (int j = lane; j < cols; j += kWave) __builtin_nontemporal_store(splat<T>(0.0f), row + j);
+            clear_row(dW + static_cast<int64_t>(first + v) * cols, cols);
         }
         return;
     }

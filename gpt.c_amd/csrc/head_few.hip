@@ -273,7 +273,10 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
 
 template <bool DX>
 void run_few(const FewArgs &a, int across, hipStream_t s) {
-    const int n = a.small.row_blocks <= 2 ? a.small.row_blocks : 4;
+    int n = a.small.row_blocks <= 2 ? a.small.row_blocks : 4;
+    // Rather W again than CUs without work: 450 rows of 1820 on 2029 tokens 77 us in 64 workgroups, 57 in 128, 49 in 256;
+    // 64 of 768 on 20000 33 in 157, 40 in 314; 200 of 768 on 5003 40 in 80, 32 in 160, 34 in 320.
+    while (!DX && n > 1 && across * (a.small.row_blocks / n) < 144) n /= 2;
     auto kernel = n == 1 ? few_kernel<1, DX> : n == 2 ? few_kernel<2, DX> : few_kernel<4, DX>;
     const int waves = n == 1 ? FewShape<1>::kWaves : n == 2 ? FewShape<2>::kWaves : FewShape<4>::kWaves;
     kernel<<<dim3(across, a.small.row_blocks / n), dim3(64 * waves), 0, s>>>(a);

@@ -203,3 +203,20 @@ def test_few_rows_where_w_changes_size(rt, R):
     W[200:232, 32:64] = 1e-38
     a = x, W, t, w
     head.agree(head.Call(rt, *a), head.Exact(*a))
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("shape,V,C,kind", [
+    ((5, 8), 700, 127, "uniform"), ((5, 8), 700, 129, "uniform"), ((3, 50), 900, 130, "text"), ((1, 9), 400, 131, "two"),
+    ((2, 88), 5000, 346, "outside"), ((8, 8), 300, 1601, "uniform")])
+def test_rows_cleared_by_16_bytes(rt, shape, V, C, kind, accumulate):
+    sorted_gpu.test_gradient(rt, shape, V, C, kind, accumulate)
+
+
+@pytest.mark.parametrize("R,V,C", [(65, 129, 40), (128, 3000, 40), (300, 4700, 33), (450, 2029, 182), (512, 900, 64)])
+def test_few_workgroups(rt, R, V, C):
+    """Where there are few tokens, fewer rows share a reading of W."""
+    a = head.inputs(R, V, C, seed=6, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
