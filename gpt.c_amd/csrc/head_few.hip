@@ -80,10 +80,10 @@ struct FewArgs {
 // each other's chain of loads, largest value, split and products.
 template <int NB>
 struct FewShape {
-    static constexpr int kBlocks = NB < 2 ? NB : 2;                     // of 32 rows a wave
+    static constexpr int kBlocks = NB < 2 ? NB : 2;                      // of 32 rows a wave
     static constexpr int kWaves = 4 * NB / kBlocks;
     static constexpr int kSmall = NB * 256, kStage = kSmall + 4 * 256;  // 16-byte chunks
-    static constexpr int kDepth = NB == 1 ? 4 : NB == 2 ? 3 : 2;                    // two workgroups a CU in 160 KB
+    static constexpr int kDepth = NB == 1 ? 4 : NB == 2 ? 3 : 2;         // two workgroups a CU in 160 KB
     static constexpr int kLoadsSmall = NB * 4 / kWaves, kLoadsW = 16 / kWaves;  // kilobytes of a wave
 };
 
@@ -268,15 +268,12 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
     constexpr float kLog2e = 1.4426950408889634f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) s += p[32 * k].y * __builtin_amdgcn_exp2f((p[32 * k].x - m) * kLog2e);
+    if (m == -INFINITY) s = 0.0f;  // no logit but minus infinity
     a.l.stats[static_cast<int64_t>(at128) * a.l.row_stride + rb * 32 + threadIdx.x] = make_float2(m, s);
 }
 
 template <bool DX>
-void run_few(const FewArgs &a, int across, hipStream_t s) {
-    int n = a.small.row_blocks <= 2 ? a.small.row_blocks : 4;
-    // Rather W again than CUs without work: 450 rows of 1820 on 2029 tokens 77 us in 64 workgroups, 57 in 128, 49 in 256;
-    // 64 of 768 on 20000 33 in 157, 40 in 314; 200 of 768 on 5003 40 in 80, 32 in 160, 34 in 320.
-    while (!DX && n > 1 && across * (a.small.row_blocks / n) < 144) n /= 2;
+void run_few(const FewArgs &a, int n, int across, hipStream_t s) {
     auto kernel = n == 1 ? few_kernel<1, DX> : n == 2 ? few_kernel<2, DX> : few_kernel<4, DX>;
     const int waves = n == 1 ? FewShape<1>::kWaves : n == 2 ? FewShape<2>::kWaves : FewShape<4>::kWaves;
     kernel<<<dim3(across, a.small.row_blocks / n), dim3(64 * waves), 0, s>>>(a);
@@ -380,7 +377,12 @@ void launch_few_rows(const float *x, const float *weights, int rows, const FewRo
 }
 
 int launch_few_logits(const float *W, int V, int C, const FewRows &x, const LogitsArgs &l, hipStream_t s) {
-    run_few<false>({W, V, C, x, l, 0, 0, 0, nullptr}, l.token_blocks / 4, s);
+    const int across = l.token_blocks / 4;
+    int n = std::min(x.row_blocks, 4);
+    // Rather W again than CUs without work: 450 rows of 1820 on 2029 tokens 77 us in 64 workgroups, 57 in 128, 49 in 256;
+    // 64 of 768 on 20000 33 in 157, 40 in 314; 200 of 768 on 5003 40 in 80, 32 in 160, 34 in 320.
+    while (n > 1 && across * (x.row_blocks / n) < 144) n /= 2;
+    run_few<false>({W, V, C, x, l, 0, 0, 0, nullptr}, n, across, s);
     return 128;
 }
 
@@ -394,7 +396,8 @@ void launch_few_dx(const FewRows &d, const float *W, int V, int C, int rows, con
     const int slice = ((kbs + slices - 1) / slices + 7) / 8 * 8;  // whole steps, whose signs alternate
     slices = (kbs + slice - 1) / slice;
     float *part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(rows) * C * slices));
-    run_few<true>({W, V, C, d, {}, rows, slice, columns, part}, columns * ((slices + 7) / 8 * 8), s);
+    run_few<true>({W, V, C, d, {}, rows, slice, columns, part}, std::min(d.row_blocks, 4),
+                  columns * ((slices + 7) / 8 * 8), s);
     launch_join_slices(part, rows, C, slices, p, s);
     free_cuda(part);
 }

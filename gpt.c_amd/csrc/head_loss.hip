@@ -64,7 +64,7 @@ struct JoinArgs {
     int *whole;  // the targets, -1 for none
     float *losses;
     int rows, padded, V;
-    float *mean;  // MEAN: of all rows, which are one workgroup's
+    float *mean;  // MEAN: of all rows, which are the first workgroup's
 };
 
 // A row's loss, lse and target from the parts of its tokens: ROWS rows a workgroup, whose slices of
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs
     a.lse[row] = live ? m + logsum : INFINITY;
     a.whole[row] = target;
     if (row < a.rows) a.losses[row] = loss;
-    if (!MEAN) return;
+    if (!MEAN || blockIdx.x > 0) return;
     double t = static_cast<double>(loss) * weight;
 #pragma unroll
     for (int off = 1; off < ROWS; off <<= 1) t += __shfl_xor(t, off, ROWS);
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs
 
 void launch_join_stats(const JoinArgs &a, hipStream_t s) {
     if (a.mean != nullptr)
-        join_stats_kernel<kMeanRows, true><<<dim3(1), dim3(kJoinThreads), 0, s>>>(a);
+        join_stats_kernel<kMeanRows, true><<<dim3(a.padded / kMeanRows), dim3(kJoinThreads), 0, s>>>(a);
     else
         join_stats_kernel<8, false><<<dim3(a.padded / 8), dim3(kJoinThreads), 0, s>>>(a);
     hipCheck(hipGetLastError());
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
     const int row = rb * 32 + l32;
     const float lse = a.lse[row];
     const int target = a.targets[row];
+    const bool live = lse != INFINITY;  // else there may be no logits
     uint32_t *mine = lds[w];
     for (int jb = first; jb < min(first + a.per_wave, a.token_blocks); ++jb) {
         const f32x4_t *x = reinterpret_cast<const f32x4_t *>(a.logits) +
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
         for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f((v[q][e] - lse) * kLog2eF);
+                const float p = live ? __builtin_amdgcn_exp2f((v[q][e] - lse) * kLog2eF) : 0.0f;
                 v[q][e] = p - (jb * 32 + 8 * q + 4 * hf + e == target ? 1.0f : 0.0f);
             }
         uint32_t high[4][2], low[4][2];
@@ -318,10 +319,10 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
 void run_few(const HeadLoss &h, hipStream_t s) {
     const bool grad = h.dx != nullptr || h.dW != nullptr;
     const int tokens = (h.V + 127) / 128 * 128;
-    // dt's terms are whole pairs of blocks.
-    const int blocks = std::max(few_row_blocks(h.rows), h.dW != nullptr ? 2 : 1), padded = blocks * 32;
+    // Blocks of 32 rows; dt's terms are whole pairs of them, whose second one may hold no row and have no logits.
+    const int own = few_row_blocks(h.rows), blocks = std::max(own, h.dW != nullptr ? 2 : 1), padded = blocks * 32;
     Scratch scratch;
-    FewRows x{nullptr, scratch.take<int>(padded), 0, blocks, h.C}, d{nullptr, nullptr, kShareShift, blocks, tokens};
+    FewRows x{nullptr, scratch.take<int>(padded), 0, own, h.C}, d{nullptr, nullptr, kShareShift, own, tokens};
     x.data = scratch.take<hu32x4>(x.bytes() / 16);
     launch_few_rows(h.x, h.weights, h.rows, x, s);
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
@@ -330,14 +331,14 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     float *target_logits = scratch.take<float>(padded), *lse = scratch.take<float>(padded);
     const int part = launch_few_logits(
         h.W, h.V, h.C, x, {logits, stats, h.targets, target_logits, h.V, h.rows, tokens / 32, padded}, s);
-    const bool mean = h.rows <= kMeanRows && padded == kMeanRows;
+    const bool mean = h.rows <= kMeanRows;
     launch_join_stats({stats, tokens / part, h.targets, target_logits, h.weights, lse, targets, h.losses, h.rows, padded,
                        h.V, mean ? h.mean : nullptr},
                       s);
     if (!mean) launch_mean(h, s);
     if (grad) {
         Halves dt{nullptr, nullptr, kShareShift, h.V, h.rows}, xt{};
-        if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / 16);
+        if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / own * blocks / 16);
         if (h.dW != nullptr) dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
         launch_shares({logits, lse, targets, d.data, dt.data, blocks, tokens / 32, dt.term_blocks() / 2,
                        tokens / 32, 0},
