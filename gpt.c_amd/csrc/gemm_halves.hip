@@ -13,9 +13,9 @@
 // negated and subtracted, which cancels what shift is left.
 //
 // What bounds them: the matrix cores' power.  8192 rows of 768 against 50257 tokens,
-// 1.9e15 fp16 operations for each of the three products, take 1.86 to 2.03 ms for the
-// logits and 1.84 to 2.02 for a gradient: 930 to 1020 TFLOP/s, 81 to 89 % of the
-// library's fp16 product of 8192^3 on such values (1145; 1594 on zeros, as the clock
+// 1.9e12 fp16 operations for each of the three products, take 1.73 to 1.9 ms for the
+// logits and 1.7 to 1.9 for a gradient, from box to box: 1000 to 1130 TFLOP/s beside the
+// library's fp16 product of 8192^3 on such values, 1145 (1594 on zeros, as the clock
 // falls with what toggles).  Tiles of 256 x 256 were no quicker.
 //
 // A workgroup forms 128 x 128 outputs, its four waves 64 x 64 each.  The operands lie
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void halves_rows_kernel(const floa
     for (int k = 256 * kRowsKeep + 4 * lane; k < 16 * t.term_blocks; k += 256) put(k, four(k));
 }
 
-// largest[0] = bits of the largest magnitude of n values so far (768 x 50257: 42 us, 3.7 TB/s of reads alone).
+// largest[0] = bits of the largest magnitude of n values so far (768 x 50257: 39 us, 4.0 TB/s of reads alone).
 __global__ __launch_bounds__(kThreads) void largest_kernel(const float *__restrict__ x, int64_t n, bool vec,
                                                           uint32_t *largest) {
     const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;

@@ -154,7 +154,7 @@ constexpr int kShareStride = 36;  // words of LDS a token: 16-byte rows, no two 
 // d' = exp(l - lse) - [target] of a block of 32 rows x 32 tokens, in two fp16 parts, as the
 // operand of either product.  The logits come in the order of the accumulators: a lane holds row
 // l % 32 and tokens 8 q + 4 (l / 32) + {0 .. 3}, which is also its share of d's block; d^T's goes
-// through LDS.  Memory bound: 4 bytes in, 4 out for each operand (8192 rows, 50257 tokens, d alone: 587 us, 5.6 TB/s).
+// through LDS.  Memory bound: 4 bytes in, 4 out for each operand (8192 rows, 50257 tokens, d alone: 575 us, 5.7 TB/s).
 __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
     __shared__ uint32_t lds[4][32 * kShareStride];
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
