@@ -8,8 +8,8 @@
 // operand is small; its parts are formed once, in the order of the fragments.
 //
 // 768 features, 50257 tokens: 16 rows' logits 28 us (5.5 TB/s), where W comes from HBM 35
-// to 37; 100 rows' 53 to 58, d W 45 to 47.  With three bf16 parts, which need no scale but six products
-// instead of three, those took 70 and 60.
+// to 37; 100 rows' 53 to 58, d W 45 to 47.  With three bf16 parts, which need no scale but
+// six products instead of three, those took 70 and 60.
 #include <algorithm>
 #include "gpu_kernels.h"
 #include "head_loss.hpp"
@@ -266,9 +266,9 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_wa
 #pragma unroll
     for (int k = 1; k < 4; ++k) m = fmaxf(m, p[32 * k].x);
     constexpr float kLog2e = 1.4426950408889634f;
+    const float ref = m == -INFINITY ? 0.0f : m;  // no logit but minus infinity or NaN, which stays in the sum
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s += p[32 * k].y * __builtin_amdgcn_exp2f((p[32 * k].x - m) * kLog2e);
-    if (m == -INFINITY) s = 0.0f;  // no logit but minus infinity
+    for (int k = 0; k < 4; ++k) s += p[32 * k].y * __builtin_amdgcn_exp2f((p[32 * k].x - ref) * kLog2e);
     a.l.stats[static_cast<int64_t>(at128) * a.l.row_stride + rb * 32 + threadIdx.x] = make_float2(m, s);
 }
 
@@ -281,7 +281,8 @@ void run_few(const FewArgs &a, int n, int across, hipStream_t s) {
 }
 
 // dW = d^T x for up to 16 KB terms (rows): writing dW is the time (100 rows of 768 on 50257: 40 us for 154 MB out and
-// 26 in; 7 more without the order by XCD, 8 more without the stores' hint).  Both operands come as two fp16 parts (Halves).  A workgroup keeps its 128 columns of x in LDS and its waves stream blocks of 32 tokens.
+// 26 in; 7 more without the order by XCD, 8 more without the stores' hint).  Both operands come as two fp16 parts
+// (Halves).  A workgroup keeps its 128 columns of x in LDS and its waves stream blocks of 32 tokens.
 template <int KB>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void few_dw_kernel(
     const Halves dt, const Halves xt, const HalvesProduct p, int columns) {

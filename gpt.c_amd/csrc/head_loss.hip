@@ -71,6 +71,16 @@ struct JoinArgs {
 // the parts are joined in a fixed order.  Rows that take no part, those past the last one among them:
 // lse is infinite, which makes their shares 0, and the target -1.  Latency bound (100 rows: 8.8 us).
 constexpr int kJoinThreads = 1024;
+
+// What sums are taken relative to: without a logit but minus infinity they are 0, or NaN where there is one.
+__device__ __forceinline__ float reference(float largest) { return largest == -INFINITY ? 0.0f : largest; }
+
+__device__ __forceinline__ void join_sums(float &m, float &s, float m2, float s2) {
+    const float top = fmaxf(m, m2), ref = reference(top);
+    s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2eF) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * kLog2eF);
+    m = top;
+}
+
 template <int ROWS, bool MEAN>
 __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs a) {
     constexpr int kAhead = 16, kWaves = kJoinThreads / kWave, kSlices = kJoinThreads / ROWS;
@@ -88,16 +98,16 @@ __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs
         float top = m;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) top = fmaxf(top, v[k].x);
-        if (top == -INFINITY) continue;  // nothing but parts without a logit
-        s *= __builtin_amdgcn_exp2f((m - top) * kLog2eF);
+        const float ref = reference(top);
+        s *= __builtin_amdgcn_exp2f((m - ref) * kLog2eF);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) s += v[k].y * __builtin_amdgcn_exp2f((v[k].x - top) * kLog2eF);
+        for (int k = 0; k < kAhead; ++k) s += v[k].y * __builtin_amdgcn_exp2f((v[k].x - ref) * kLog2eF);
         m = top;
     }
 #pragma unroll
     for (int off = ROWS; off < kWave; off <<= 1) {
         const float m2 = __shfl_xor(m, off, kWave), s2 = __shfl_xor(s, off, kWave);
-        online_merge(m, s, m2, s2);
+        join_sums(m, s, m2, s2);
     }
     if ((threadIdx.x & (kWave - 1)) < ROWS) red[threadIdx.x / kWave][r] = make_float2(m, s);
     __syncthreads();
@@ -108,12 +118,12 @@ __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs
 #pragma unroll
     for (int k = kGroups; k < kWaves; k += kGroups) {
         const float2 b = red[slice + k][r];
-        online_merge(m, s, b.x, b.y);
+        join_sums(m, s, b.x, b.y);
     }
 #pragma unroll
     for (int off = ROWS; off < kWave; off <<= 1) {
         const float m2 = __shfl_xor(m, off, kWave), s2 = __shfl_xor(s, off, kWave);
-        online_merge(m, s, m2, s2);
+        join_sums(m, s, m2, s2);
     }
     if (threadIdx.x >= ROWS) return;
     const float weight = row < a.rows ? weight_of(a.weights, row) : 0.0f;

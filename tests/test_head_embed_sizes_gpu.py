@@ -220,3 +220,23 @@ def test_few_workgroups(rt, R, V, C):
     ref = head.Exact(*a)
     head.agree(head.Call(rt, *a), ref)
     head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R", [3, 40, 100, MANY])
+@pytest.mark.parametrize("first,last", [(0, 300), (128, 256), (256, 300), (295, 296)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_w_that_is_not_finite(rt, R, first, last, bad):
+    """Any such value makes the loss NaN, whole parts of them too."""
+    x, W, t, _ = head.inputs(R, 300, 40, seed=7)
+    W[first:last] = bad
+    for kw in ({}, {"dx": False, "dW": False}):
+        got = head.Call(rt, x, W, t, **kw)
+        assert np.isnan(got.loss[0]) and np.isnan(got.losses).all()
+
+
+@pytest.mark.parametrize("R,V,C", [(1, 4194303, 1), (130, 1000003, 5), (400, 600001, 3)])
+def test_large_vocabularies(rt, R, V, C):
+    a = head.inputs(R, V, C, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
