@@ -50,6 +50,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void halves_rows_kernel(const floa
                                                                      int terms, bool vec, HalvesRows t) {
     const int lane = threadIdx.x & 63;
     const int row = blockIdx.x * kRowsWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int i = blockIdx.x * (64 * kRowsWaves) + threadIdx.x; i < t.zeros; i += gridDim.x * (64 * kRowsWaves)) t.zero[i] = 0;
     const bool live = row < rows && (weights == nullptr || weights[row] != 0.0f);
     const float *p = x + static_cast<int64_t>(row) * terms;
     auto four = [&](int k) {
@@ -253,11 +254,6 @@ __global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *_
         out[(kb * 2) * 64] = high;
         out[(kb * 2 + 1) * 64] = low;
     }
-}
-
-__global__ __launch_bounds__(kThreads) void zero_words_kernel(uint32_t *p, int n) {
-    const int i = blockIdx.x * kThreads + threadIdx.x;
-    if (i < n) p[i] = 0;
 }
 
 // ---- the product's loop ----
@@ -633,8 +629,10 @@ void launch_rows(const float *x, const float *weights, int rows, int terms, cons
     hipCheck(hipGetLastError());
 }
 
-void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, hipStream_t s) {
-    launch_rows(x, weights, h.rows, h.terms, {h.data, h.shift, h.row_blocks(), h.term_blocks(), negate, false}, s);
+void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, uint32_t *zero, int zeros,
+                        hipStream_t s) {
+    launch_rows(x, weights, h.rows, h.terms,
+                {h.data, h.shift, h.row_blocks(), h.term_blocks(), negate, false, zero, zeros}, s);
 }
 
 void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s) {
@@ -655,11 +653,6 @@ void launch_column_largest(const float *x, int ld, const float *weights, float d
     else
         column_largest_kernel<float><<<dim3(chunks, (cols + 63) / 64), dim3(kThreads), 0, s>>>(x, ld, weights, divisor,
                                                                                               terms, cols, largest);
-    hipCheck(hipGetLastError());
-}
-
-void launch_zero_words(uint32_t *p, int n, hipStream_t s) {
-    zero_words_kernel<<<dim3((n + kThreads - 1) / kThreads), dim3(kThreads), 0, s>>>(p, n);
     hipCheck(hipGetLastError());
 }
 

@@ -57,8 +57,9 @@ __device__ __forceinline__ void halves_split(float x, float y, uint32_t &high, u
 __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) & 1) != 0; }
 
 // x (rows x terms without gaps; with weights, rows of weight 0 as zeros) into h.data and h.shift; negate: as a product's
-// first operand.
-void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, hipStream_t s);
+// first operand; `zeros` words at `zero` to 0.
+void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, uint32_t *zero, int zeros,
+                        hipStream_t s);
 // The same for other paddings, and (in_lines) another order of a block's terms: lane l of blocks 2 j and 2 j + 1 holds
 // 32 j + 16 (l / 32) + {0 .. 7} and {8 .. 15}, a step's 64 consecutive bytes for either half of the lanes.
 struct HalvesRows {
@@ -66,6 +67,8 @@ struct HalvesRows {
     int *shift;
     int row_blocks, term_blocks;  // of 32 and of 16
     bool negate, in_lines;
+    uint32_t *zero;  // the same launch sets `zeros` words here to 0
+    int zeros;
 };
 void launch_rows(const float *x, const float *weights, int rows, int terms, const HalvesRows &t, hipStream_t s);
 // x (rows x terms without gaps) as a first operand, all rows by the shift of its largest magnitude, whose bits *largest
@@ -73,14 +76,13 @@ void launch_rows(const float *x, const float *weights, int rows, int terms, cons
 void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
 // as a second operand, or as the one that is negated.  largest: the bits of each column's largest magnitude, which the
-// first call raises from what it holds (launch_zero_words) and which may count further terms too; null with up to
+// first call raises from what it holds and which may count further terms too; null with up to
 // kColumnTerms terms, whose largest the second call finds by itself.
 constexpr int kColumnTerms = 128;
 void launch_column_largest(const float *x, int ld, const float *weights, float divisor, int terms, int cols,
                            uint32_t *largest, hipStream_t s);
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
                            bool negate, const uint32_t *largest, hipStream_t s);
-void launch_zero_words(uint32_t *p, int n, hipStream_t s);
 
 // C (A.rows x B.rows, rows of ldc) = A B^T times row_factor[m] / divisor (+ C); rows of factor 0 are 0.
 struct HalvesProduct {

@@ -21,26 +21,33 @@ __device__ __forceinline__ float weight_of(const float *weights, int row) {
     return weights != nullptr ? weights[row] : 1.0f;
 }
 
-// out[0] = sum of w[r] loss[r] / rows in a fixed order, in 64 bits.
-constexpr int kMeanThreads = 1024;
-__global__ __launch_bounds__(kMeanThreads) void mean_loss_kernel(const float *__restrict__ losses,
-                                                                const float *__restrict__ weights,
-                                                                float *__restrict__ out, int rows) {
-    __shared__ double part[kMeanThreads / kWave];
+struct MeanArgs {
+    const float *losses, *weights;
+    float *out;
+    int rows;
+};
+
+// out[0] = sum of w[r] loss[r] / rows in a fixed order, in 64 bits; one workgroup.
+template <int THREADS>
+__device__ __forceinline__ void mean_loss(const MeanArgs &a) {
+    __shared__ double part[THREADS / kWave];
     double t = 0.0;
 #pragma unroll 8
-    for (int r = threadIdx.x; r < rows; r += kMeanThreads)
-        t += static_cast<double>(losses[r]) * weight_of(weights, r);  // rows of weight 0: 0 * 0
+    for (int r = threadIdx.x; r < a.rows; r += THREADS)
+        t += static_cast<double>(a.losses[r]) * weight_of(a.weights, r);  // rows of weight 0: 0 * 0
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) t += __shfl_xor(t, off, kWave);
     if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = t;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    for (int i = 1; i < kMeanThreads / kWave; ++i) t += part[i];
-    out[0] = static_cast<float>(t / rows);
+    for (int i = 1; i < THREADS / kWave; ++i) t += part[i];
+    a.out[0] = static_cast<float>(t / a.rows);
 }
 
-constexpr int kMeanRows = 32;  // up to here, the kernel that forms the rows' losses forms their mean
+constexpr int kMeanThreads = 1024;
+__global__ __launch_bounds__(kMeanThreads) void mean_loss_kernel(const MeanArgs a) { mean_loss<kMeanThreads>(a); }
+
+constexpr int kMeanRows = 32;  // up to here, the kernel that forms the rows' losses forms their mean; else the shares' does
 
 struct HeadLoss {
     const float *x, *W, *targets, *weights;
@@ -50,7 +57,7 @@ struct HeadLoss {
 };
 
 void launch_mean(const HeadLoss &h, hipStream_t s) {
-    mean_loss_kernel<<<dim3(1), dim3(kMeanThreads), 0, s>>>(h.losses, h.weights, h.mean, h.rows);
+    mean_loss_kernel<<<dim3(1), dim3(kMeanThreads), 0, s>>>({h.losses, h.weights, h.mean, h.rows});
     hipCheck(hipGetLastError());
 }
 
@@ -156,6 +163,7 @@ struct ShareArgs {
     int row_blocks, token_blocks;  // of the logits
     int rows_used, tokens_used;    // blocks that the products' reductions reach
     int per_wave;                  // blocks of tokens a wave
+    MeanArgs mean;                 // by one more workgroup, unless `out` is null
 };
 
 constexpr int kShareShift = 15;  // shares are held times 2^15
@@ -166,6 +174,10 @@ constexpr int kShareStride = 36;  // words of LDS a token: 16-byte rows, no two 
 // l % 32 and tokens 8 q + 4 (l / 32) + {0 .. 3}, which is also its share of d's block; d^T's goes
 // through LDS.  Memory bound: 4 bytes in, 4 out for each operand (8192 rows, 50257 tokens, d alone: 575 us, 5.7 TB/s).
 __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
+    if (a.mean.out != nullptr && blockIdx.x == gridDim.x - 1) {
+        if (blockIdx.y == 0) mean_loss<kThreads>(a.mean);
+        return;
+    }
     __shared__ uint32_t lds[4][32 * kShareStride];
     const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -239,7 +251,7 @@ void launch_shares(ShareArgs a, hipStream_t s) {
     // Four blocks a wave, fewer where that leaves less than eight waves a CU.
     a.per_wave = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, static_cast<int64_t>(a.row_blocks) * a.token_blocks / 2048)));
     const int per = 4 * a.per_wave;
-    shares_kernel<<<dim3((a.token_blocks + per - 1) / per, a.row_blocks), dim3(kThreads), 0, s>>>(a);
+    shares_kernel<<<dim3((a.token_blocks + per - 1) / per + (a.mean.out != nullptr), a.row_blocks), dim3(kThreads), 0, s>>>(a);
     hipCheck(hipGetLastError());
 }
 
@@ -277,16 +289,16 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     const int piece = static_cast<int>(std::min<int64_t>(h.rows, grad ? fit : kLossPiece));
     const int padded = (piece + 127) / 128 * 128;
     Scratch scratch;
+    Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
     // The largest magnitudes of the columns of x, and of W.
     uint32_t *largest_x = scratch.take<uint32_t>(h.C + 1), *largest = largest_x + h.C;
-    launch_zero_words(largest_x, h.C + 1, s);
+    launch_halves_rows(h.x, h.weights, x, false, largest_x, h.C + 1, s);
     // W is held by one shift, as its rows are the terms of dx: to 2^-40 of its largest value where it is below the 2^-17th
     // of that, which counts for features of dx that small.  Laid out by rows and, for dx, a second time by columns it would
-    // be held to 2^-40 of each row's and column's largest, and cost 171 us instead of 90 (50257 x 768) and 371 instead of
-    // 169 (50257 x 1600).
+    // be held to 2^-40 of each row's and column's largest, and cost 171 us instead of 88 (50257 x 768) and 371 instead of
+    // 164 (50257 x 1600).
     const Halves W = scratch.halves(h.V, h.C);
     launch_halves_table(h.W, W, largest, s);
-    Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
     if (h.dW != nullptr) {
         xt = scratch.halves(h.C, piece);
         launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest_x, s);
@@ -301,7 +313,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         const float *xr = h.x + static_cast<int64_t>(r) * h.C;
         const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
         x.rows = d.rows = xt.terms = n;
-        launch_halves_rows(xr, weights, x, false, s);
+        if (r > 0) launch_halves_rows(xr, weights, x, false, nullptr, 0, s);
         const int part = launch_logits(
             W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
         launch_join_stats({stats, tokens / part, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n,
@@ -309,7 +321,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
                           s);
         if (!grad) continue;
         const ShareArgs a{logits, lse, targets, d.data, nullptr, n_padded / 32, tokens / 32, 0,
-                          (h.V + 63) / 64 * 2, 0};
+                          (h.V + 63) / 64 * 2, 0, {h.losses, h.weights, r + piece >= h.rows ? h.mean : nullptr, h.rows}};
         launch_shares(a, s);
         if (h.dx != nullptr)
             launch_product_across_b(d, W, {h.dx + static_cast<int64_t>(r) * h.C, h.C, weights,
@@ -320,7 +332,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
             launch_product_across_a(d, xt, {h.dW, h.C, nullptr, 1.0f, h.add || r > 0}, s);
         }
     }
-    launch_mean(h, s);
+    if (!grad) launch_mean(h, s);
     scratch.release();
 }
 
@@ -334,7 +346,8 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     Scratch scratch;
     FewRows x{nullptr, scratch.take<int>(padded), 0, own, h.C}, d{nullptr, nullptr, kShareShift, own, tokens};
     x.data = scratch.take<hu32x4>(x.bytes() / 16);
-    launch_few_rows(h.x, h.weights, h.rows, x, s);
+    uint32_t *largest = scratch.take<uint32_t>(h.C);  // of x's columns
+    launch_few_rows(h.x, h.weights, h.rows, x, largest, h.C, s);
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
     float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 32));
     int *targets = scratch.take<int>(padded);
@@ -345,13 +358,13 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     launch_join_stats({stats, tokens / part, h.targets, target_logits, h.weights, lse, targets, h.losses, h.rows, padded,
                        h.V, mean ? h.mean : nullptr},
                       s);
-    if (!mean) launch_mean(h, s);
+    if (!grad && !mean) launch_mean(h, s);
     if (grad) {
         Halves dt{nullptr, nullptr, kShareShift, h.V, h.rows}, xt{};
         if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / own * blocks / 16);
         if (h.dW != nullptr) dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
         launch_shares({logits, lse, targets, d.data, dt.data, blocks, tokens / 32, dt.term_blocks() / 2,
-                       tokens / 32, 0},
+                       tokens / 32, 0, {h.losses, h.weights, mean ? nullptr : h.mean, h.rows}},
                       s);
         if (h.dx != nullptr)
             launch_few_dx(d, h.W, h.V, h.C, h.rows,
@@ -361,8 +374,6 @@ void run_few(const HeadLoss &h, hipStream_t s) {
             if (h.rows <= kColumnTerms) {
                 launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, false, nullptr, s);
             } else {
-                uint32_t *largest = scratch.take<uint32_t>(h.C);
-                launch_zero_words(largest, h.C, s);
                 launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest, s);
                 launch_halves_columns(h.x, h.C, h.weights, static_cast<float>(h.rows), xt, false, largest, s);
             }

@@ -90,8 +90,9 @@ struct FewRows {
 
 // Blocks of 32 rows that launch_few_logits and launch_few_dx take for this many rows.
 int few_row_blocks(int rows);
-// x (rows x terms without gaps) into t, rows of weight 0 as zeros.
-void launch_few_rows(const float *x, const float *weights, int rows, const FewRows &t, hipStream_t s);
+// x (rows x terms without gaps) into t, rows of weight 0 as zeros; `zeros` words at `zero` to 0.
+void launch_few_rows(const float *x, const float *weights, int rows, const FewRows &t, uint32_t *zero, int zeros,
+                     hipStream_t s);
 // The logits of x (V x C floats W as they come).  Returns the tokens of each of the stats' parts.
 int launch_few_logits(const float *W, int V, int C, const FewRows &x, const LogitsArgs &l, hipStream_t s);
 // p.C (rows x C) = d W by the rows' factors.
