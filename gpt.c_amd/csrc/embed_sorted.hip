@@ -494,29 +494,54 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const GatherArgs a) {
 
 // Up to kFewRows rows, in one launch: a workgroup a row and 64 columns in units of T compares the row's id with all
 // others, and if it is the first of its id adds their rows, a quarter of them a wave.  The first a.clears workgroups
-// clear the rows that no id names, an equal range of them each.  3 x 333 rows of 100 on 5003: 6.0 us, sorted 13.2;
-// 1024 of 768 on 50257: 25.3, sorted 29.6; of 1600: 66.8, sorted 63.5.  With room for more ids it is behind: 2048 rows
-// of 768 on 50257 50.5, sorted 30.9.
+// clear the rows that no id names.  3 x 333 rows of 100 on 5003: 5.6 us, sorted 13.2; 1000 of 768 on 50257: 26.2, sorted
+// 29.6; of 1600: 56, sorted 63.  With room for more ids it is behind: 2048 rows of 768 on 50257 50.5, sorted 30.9.
 constexpr int kFewRows = 1024;
 constexpr int kFewItems = kFewRows / kThreads;  // ids a thread
-constexpr int kClearRows = 1 << 13;             // of a workgroup, at most
+constexpr int kClearRows = 1 << 16;             // whose ids are marked at a time
 
-// A wave: `cols` values from `row` on to zero, in whole 16 bytes where they may be and there are many (176 rows of 346 on
-// 50257: 16.7 us, by floats 21.3; 256 of 17: 16.0, by floats 10.5).
-__device__ __forceinline__ void clear_row(f32x4_t *row, int cols) {
-    for (int j = threadIdx.x & (kWave - 1); j < cols; j += kWave) __builtin_nontemporal_store(splat<f32x4_t>(0.0f), row + j);
-}
-__device__ __forceinline__ void clear_row(float *row, int cols) {
-    const int lane = threadIdx.x & (kWave - 1);
-    if (cols <= 2 * kWave) {
-        for (int j = lane; j < cols; j += kWave) row[j] = 0.0f;
-        return;
+// `count` rows of C floats from `base` on to zero, but for those whose bit in `named` (LDS) is set, by `groups` workgroups
+// together: 16 bytes at a time, whatever rows they belong to, so that what is written at a time is one stretch.
+template <typename T>
+__device__ __forceinline__ void clear_unnamed(float *base, int C, int count, const uint32_t *named, int groups) {
+    auto stays = [&](int row) { return ((named[row / 32] >> (row % 32)) & 1) != 0; };
+    auto clear = [](float *to) {
+        __builtin_nontemporal_store(splat<f32x4_t>(0.0f), reinterpret_cast<f32x4_t *>(to));
+    };
+    const int total = count * C, step = 4 * kThreads * groups, rows = step / C, rest = step - rows * C;
+    const int first = blockIdx.x * kThreads + threadIdx.x;
+    int before = 0;  // the first whole 16 bytes
+    if constexpr (sizeof(T) == sizeof(float)) {
+        before = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) / 4 & 3);
+        if (first < min(before, total) && !stays(first / C)) base[first] = 0.0f;
     }
-    const int before = min(cols, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) / 4 & 3));
-    const int units = (cols - before) / 4, behind = before + 4 * units;
-    if (lane < before) row[lane] = 0.0f;
-    if (lane < cols - behind) row[behind + lane] = 0.0f;
-    clear_row(reinterpret_cast<f32x4_t *>(row + before), units);
+    int64_t at = before + 4ll * first;
+    int row = static_cast<int>(at / C), in = static_cast<int>(at - static_cast<int64_t>(row) * C);
+    for (; at < total; at += step) {
+        if constexpr (sizeof(T) == sizeof(f32x4_t)) {
+            if (!stays(row)) clear(base + at);
+        } else {
+            const bool one = in + 3 < C;  // of one row, else of two or more
+            if (!stays(row) && (one || (C >= 4 && at + 3 < total && !stays(row + 1)))) {
+                clear(base + at);
+            } else if (!one) {
+                int r = row, i = in;
+                for (int e = 0; e < 4; ++e, ++i) {
+                    if (i >= C) {
+                        i = 0;
+                        ++r;
+                    }
+                    if (at + e < total && !stays(r)) base[at + e] = 0.0f;
+                }
+            }
+        }
+        row += rows;
+        in += rest;
+        if (in >= C) {
+            in -= C;
+            ++row;
+        }
+    }
 }
 
 struct FewArgs {
@@ -540,19 +565,18 @@ __global__ __launch_bounds__(kThreads) void gather_few_kernel(const FewArgs f) {
     }
     if (static_cast<int>(blockIdx.x) < f.clears) {
         __shared__ uint32_t named[kClearRows / 32];
-        const int first = static_cast<int>(static_cast<int64_t>(a.V) * blockIdx.x / f.clears);
-        const int count = static_cast<int>(static_cast<int64_t>(a.V) * (blockIdx.x + 1) / f.clears) - first;
-        for (int i = threadIdx.x; i < (count + 31) / 32; i += kThreads) named[i] = 0;
-        __syncthreads();
+        for (int first = 0; first < a.V; first += kClearRows) {
+            const int count = min(kClearRows, a.V - first);
+            __syncthreads();
+            for (int i = threadIdx.x; i < (count + 31) / 32; i += kThreads) named[i] = 0;
+            __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kFewItems; ++k) {
-            const int v = key[k] - first;
-            if (key[k] >= 0 && v >= 0 && v < count) atomicOr(&named[v / 32], 1u << (v % 32));
-        }
-        __syncthreads();
-        for (int v = w; v < count; v += kWaves) {
-            if ((named[v / 32] >> (v % 32)) & 1) continue;
-            clear_row(dW + static_cast<int64_t>(first + v) * cols, cols);
+            for (int k = 0; k < kFewItems; ++k) {
+                const int v = key[k] - first;
+                if (key[k] >= 0 && v >= 0 && v < count) atomicOr(&named[v / 32], 1u << (v % 32));
+            }
+            __syncthreads();
+            clear_unnamed<T>(a.dW + static_cast<int64_t>(first) * a.C, a.C, count, named, f.clears);
         }
         return;
     }
@@ -684,12 +708,12 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
     const int cols = a.C / kW;
     a.blocks = (cols + kWave - 1) / kWave;
     if (a.n <= kFewRows) {
-        // Clearing: two workgroups a CU, fewer where they would write less than 16 KB each.
+        // Clearing: a workgroup a CU (26 rows of 1600 on 50257: 56 us; 272 workgroups 70, 512 61, as many as 16 KB each 58;
+        // 1000 rows 56, 70, 64, 65), a few more where rows share 16 bytes (64 rows of 1601: 51 us with 320, 58 with 256, 64
+        // with 384).
         const int64_t bytes = static_cast<int64_t>(a.V) * a.C * sizeof(float);
         FewArgs f{a, ids, 0, a.dP != nullptr ? (a.positions + kWaves - 1) / kWaves : 0};
-        if (!a.add)
-            f.clears = static_cast<int>(std::max<int64_t>((a.V + kClearRows - 1) / kClearRows,
-                                                          std::min<int64_t>(512, (bytes + 16383) / 16384)));
+        if (!a.add) f.clears = static_cast<int>(std::min<int64_t>(kW == 4 ? 256 : 320, (bytes + 16383) / 16384));
         const int64_t grid = static_cast<int64_t>(f.position_blocks + a.n) * a.blocks + f.clears;
         CHECK_ERROR(grid >= kMaxGroups, "Too many positions for one call: %d x %d.", a.positions, a.C);
         gather_few_kernel<T><<<dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s>>>(f);

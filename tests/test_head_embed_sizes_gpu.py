@@ -240,3 +240,12 @@ def test_large_vocabularies(rt, R, V, C):
     ref = head.Exact(*a)
     head.agree(head.Call(rt, *a), ref)
     head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("shape,V,C,kind", [
+    ((7, 9), 65536, 4, "uniform"), ((7, 9), 65537, 4, "uniform"), ((1, 40), 140001, 5, "outside"), ((64,), 70000, 2, "text"),
+    ((3, 5), 66000, 17, "two"), ((1, 1000), 131073, 8, "text")])
+def test_rows_cleared_of_long_tables(rt, shape, V, C, kind, accumulate):
+    """Ids are marked for 65536 rows at a time."""
+    sorted_gpu.test_gradient(rt, shape, V, C, kind, accumulate)
