@@ -76,7 +76,7 @@ struct JoinArgs {
 
 // A row's loss, lse and target from the parts of its tokens: ROWS rows a workgroup, whose slices of
 // the parts are joined in a fixed order.  Rows that take no part, those past the last one among them:
-// lse is infinite, which makes their shares 0, and the target -1.  Latency bound (100 rows: 8.8 us).
+// lse is infinite, which makes their shares 0, and the target -1.  Latency bound (100 rows: 5.6 us).
 constexpr int kJoinThreads = 1024;
 
 // What sums are taken relative to: without a logit but minus infinity they are 0, or NaN where there is one.
