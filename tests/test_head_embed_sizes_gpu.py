@@ -249,3 +249,14 @@ def test_large_vocabularies(rt, R, V, C):
 def test_rows_cleared_of_long_tables(rt, shape, V, C, kind, accumulate):
     """Ids are marked for 65536 rows at a time."""
     sorted_gpu.test_gradient(rt, shape, V, C, kind, accumulate)
+
+
+@pytest.mark.parametrize("R,V,C", [(2, 50257, 45), (1, 4096, 1), (5, 4100, 129), (31, 12000, 64), (70, 9000, 200)])
+def test_many_slices(rt, R, V, C):
+    """The gradient of x of few rows comes in up to 512 parts."""
+    a = head.inputs(R, V, C, seed=8, weights=True)
+    ref = head.Exact(*a)
+    one = head.Call(rt, *a)
+    head.agree(one, ref)
+    two = head.Call(rt, *a)
+    assert np.array_equal(one.dx, two.dx)
