@@ -379,7 +379,8 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     load_stage(S::kStage);
     const hu32x4 *at_a = lds + (w / S::WN) * S::NI * 256 + lane;
     const hu32x4 *at_b = lds + (kA + (w % S::WN) * 2) * 256 + lane;
-    // Lane l reads, of terms (rows of the block) 4 (l / 32) + l / 4 % 4 and 8 behind, rows (terms) 16 (l / 16 % 2) + 4 (l % 4) ..
+    // Lane l reads, of terms (rows of the block) 4 (l / 32) + l / 4 % 4 and 8 behind, rows (terms) 16 (l / 16 % 2) +
+    // 4 (l % 4) and the next three.
     const uint32_t in16 = lane & 15, half16 = (lane >> 4) & 1;
     const uint32_t block_across = ACROSS == Across::kA ? (w / S::WN) * S::NI : kA + (w % S::WN) * 2;
     const uint32_t across = block_across * 4096 + half16 * 2048 + (in16 & 1) * 512 + half16 * 128 +

@@ -88,8 +88,8 @@ struct FewShape {
 };
 
 template <int NB, bool DX>
-__global__ __launch_bounds__(64 * FewShape<NB>::kWaves) __attribute__((amdgpu_waves_per_eu(FewShape<NB>::kWaves / 2))) void few_kernel(
-    const FewArgs a) {
+__global__ __launch_bounds__(64 * FewShape<NB>::kWaves)
+    __attribute__((amdgpu_waves_per_eu(FewShape<NB>::kWaves / 2))) void few_kernel(const FewArgs a) {
     using S = FewShape<NB>;
     __shared__ hu32x4 lds[S::kDepth * S::kStage];
     const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;

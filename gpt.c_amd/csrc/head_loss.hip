@@ -249,9 +249,11 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
 
 void launch_shares(ShareArgs a, hipStream_t s) {
     // Four blocks a wave, fewer where that leaves less than eight waves a CU.
-    a.per_wave = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, static_cast<int64_t>(a.row_blocks) * a.token_blocks / 2048)));
+    const int64_t blocks = static_cast<int64_t>(a.row_blocks) * a.token_blocks;
+    a.per_wave = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, blocks / 2048)));
     const int per = 4 * a.per_wave;
-    shares_kernel<<<dim3((a.token_blocks + per - 1) / per + (a.mean.out != nullptr), a.row_blocks), dim3(kThreads), 0, s>>>(a);
+    const int across = (a.token_blocks + per - 1) / per + (a.mean.out != nullptr);
+    shares_kernel<<<dim3(across, a.row_blocks), dim3(kThreads), 0, s>>>(a);
     hipCheck(hipGetLastError());
 }
 
