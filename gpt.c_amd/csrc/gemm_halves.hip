@@ -97,69 +97,82 @@ __global__ __launch_bounds__(64 * kRowsWaves) void halves_rows_kernel(const floa
     for (int k = 256 * kRowsKeep + 4 * lane; k < 16 * t.term_blocks; k += 256) put(k, four(k));
 }
 
-// largest[0] = bits of the largest magnitude of n values so far (768 x 50257: 39 us, 4.0 TB/s of reads alone).
-__global__ __launch_bounds__(kThreads) void largest_kernel(const float *__restrict__ x, int64_t n, bool vec,
-                                                          uint32_t *largest) {
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
-    const int64_t first = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x, whole = vec ? n / 4 : 0;
-    float m = 0.0f;
-#pragma unroll 8
-    for (int64_t i = first; i < whole; i += stride) {
-        const f32x4_t v = reinterpret_cast<const f32x4_t *>(x)[i];
-        m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    }
-    for (int64_t i = 4 * whole + first; i < n; i += stride) m = fmaxf(m, fabsf(x[i]));
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    __shared__ float red[kThreads / 64];
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-#pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i) m = fmaxf(m, red[i]);
-    atomicMax(largest, __float_as_uint(m));
-}
+constexpr int kTableThreads = 512;
 
-// Rows by one shift, in one pass: a workgroup 32 rows x 128 terms, whose lines are read whole and written whole, through
-// LDS (768 x 50257: 50 us, 6.1 TB/s).
-__global__ __launch_bounds__(kThreads) void halves_table_kernel(const float *__restrict__ x, int ld, Halves h, bool vec,
-                                                               const uint32_t *__restrict__ largest) {
-    __shared__ hu32x4 lds[8 * 128];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, kbs = h.term_blocks(), rb = blockIdx.x, kb0 = blockIdx.y * 8;
-    const int up = halves_shift(__uint_as_float(*largest));
-    if (blockIdx.y == 0 && threadIdx.x < 32) h.shift[rb * 32 + threadIdx.x] = up;
-    float v[4][4];
-    // Piece i of a wave: rows 8 w .. + 7, terms 32 i .. + 31 of the workgroup's.
-    const int in = w * 8 + (lane >> 3), row = rb * 32 + in;
+// 64 rows by one shift, in one pass: a workgroup's values stay in registers until the largest is known, its lines are read
+// whole and written whole, through LDS.  PIECES of 32 terms stay, up to 24 with two workgroups a CU (768 x 50257: 69 us,
+// 4.5 TB/s; a pass for the largest value and one for the parts 88), else 52 with one (1600 x 50257: 166 us; with 24, and
+// the others read again, 206); MORE: there are more, which are read again.
+template <int PIECES, bool MORE>
+__global__ __launch_bounds__(kTableThreads) __attribute__((amdgpu_waves_per_eu(PIECES > 24 ? 2 : 4))) void halves_table_kernel(
+    const float *__restrict__ x, Halves h, bool vec) {
+    __shared__ hu32x4 lds[2][8 * 128];  // of each block of 32 rows, 128 terms
+    __shared__ float red[kTableThreads / 64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, kbs = h.term_blocks(), pieces = kbs / 2;
+    // Piece i of a wave: rows 8 w .. + 7, terms 32 i .. + 31.
+    const int in = w * 8 + (lane >> 3), row = blockIdx.x * 64 + in;
+    const float *p = x + static_cast<int64_t>(row) * h.terms;
+    auto four = [&](int i) {
+        const int k = 32 * i + 4 * (lane & 7);
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vec) {
+            if (row < h.rows && k < h.terms) v = *reinterpret_cast<const f32x4_t *>(p + k);
+        } else if (row < h.rows) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = kb0 * 16 + 32 * i + 4 * (lane & 7);
-        const float *p = x + static_cast<int64_t>(row) * ld + k;
-        if (vec && row < h.rows && k < h.terms) {
-            const f32x4_t y = *reinterpret_cast<const f32x4_t *>(p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = y[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = row < h.rows && k + e < h.terms ? p[e] : 0.0f;
+            for (int e = 0; e < 4; ++e) v[e] = k + e < h.terms ? p[k + e] : 0.0f;
         }
-    }
-    uint2 *to = reinterpret_cast<uint2 *>(lds);
+        return v;
+    };
+    float top = 0.0f;
+    auto larger = [&](f32x4_t v) {
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    };
+    f32x4_t own[PIECES];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = 8 * i + (lane & 7), q = c & 3;  // four terms of block c / 4
-        const uint32_t flip = halves_negated((kb0 + (c >> 2)) * 16) ? 0x80008000u : 0;
-        uint2 high, low;
-        halves_split(__builtin_amdgcn_ldexpf(v[i][0], up), __builtin_amdgcn_ldexpf(v[i][1], up), high.x, low.x);
-        halves_split(__builtin_amdgcn_ldexpf(v[i][2], up), __builtin_amdgcn_ldexpf(v[i][3], up), high.y, low.y);
-        const int at = (c >> 2) * 256 + ((q & 1) * 32 + in) * 2 + (q >> 1);
-        to[at] = make_uint2(high.x ^ flip, high.y ^ flip);
-        to[at + 128] = make_uint2(low.x ^ flip, low.y ^ flip);
-    }
+    for (int i = 0; i < PIECES; ++i) own[i] = four(i);
+    if (MORE)
+#pragma unroll 4
+        for (int i = PIECES; i < pieces; ++i) larger(four(i));
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) larger(own[i]);
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    if (lane == 0) red[w] = top;
     __syncthreads();
-    const int blocks = min(8, kbs - kb0);
-    hu32x4 *out = h.data + (static_cast<int64_t>(rb) * kbs + kb0) * 128;
-    for (int i = threadIdx.x; i < blocks * 128; i += kThreads) out[i] = lds[i];
+#pragma unroll
+    for (int i = 0; i < kTableThreads / 64; ++i) top = fmaxf(top, red[i]);
+    const int up = min(halves_shift(top), 126);
+    if ((lane & 7) == 0) h.shift[row] = up;
+    uint2 *to = reinterpret_cast<uint2 *>(lds[in >> 5]);
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += 4) {
+        f32x4_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = !MORE || p0 < PIECES ? own[i] : four(p0 + i);
+#pragma unroll
+        for (int i = 0; i + 4 < PIECES; ++i) own[i] = own[i + 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = 8 * i + (lane & 7), q = c & 3;  // four terms of block c / 4
+            const uint32_t flip = halves_negated((2 * p0 + (c >> 2)) * 16) ? 0x80008000u : 0;
+            uint2 high, low;
+            halves_split(__builtin_amdgcn_ldexpf(v[i][0], up), __builtin_amdgcn_ldexpf(v[i][1], up), high.x, low.x);
+            halves_split(__builtin_amdgcn_ldexpf(v[i][2], up), __builtin_amdgcn_ldexpf(v[i][3], up), high.y, low.y);
+            const int at = (c >> 2) * 256 + ((q & 1) * 32 + (in & 31)) * 2 + (q >> 1);
+            to[at] = make_uint2(high.x ^ flip, high.y ^ flip);
+            to[at + 128] = make_uint2(low.x ^ flip, low.y ^ flip);
+        }
+        __syncthreads();
+        const int chunks = min(8, kbs - 2 * p0) * 128;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            hu32x4 *out = h.data + (static_cast<int64_t>(blockIdx.x * 2 + b) * kbs + 2 * p0) * 128;
+#pragma unroll
+            for (int i = 0; i < 8 * 128; i += kTableThreads)
+                if (i + static_cast<int>(threadIdx.x) < chunks) out[i + threadIdx.x] = lds[b][i + threadIdx.x];
+        }
+        __syncthreads();
+    }
 }
 
 // The factor of term k of an operand that is read across its rows.
@@ -395,7 +408,13 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     static_assert(S::NI == 2 && S::BM % 128 == 0 && S::BN % 128 == 0, "");
     const bool minus = ACROSS == Across::kA ? ((w / S::WN) & 1) != 0 : ACROSS == Across::kB ? ((w % S::WN) & 1) != 0 : false;
     float sign = ((s0 & 2) != 0) != minus ? -1.0f : 1.0f;
+    int shifts = 0;  // of B read across: lane l holds that of the 64 terms after 64 l others
     for (int s = s0; s < s1; s += 2) {
+        float times = sign;
+        if constexpr (ACROSS == Across::kB) {
+            if (((s - s0) & 127) == 0) shifts = t.shift_b[32 * min(s + 2 * lane, t.stages - 1)];
+            times = __builtin_amdgcn_ldexpf(sign, -__builtin_amdgcn_readlane(shifts, ((s - s0) & 127) >> 1));
+        }
         hf32x16 p[S::NI][2];
 #pragma unroll
         for (int i = 0; i < S::NI; ++i)
@@ -435,7 +454,7 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(sign, p[i][j][r], acc[i][j][r]);
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(times, p[i][j][r], acc[i][j][r]);
         sign = -sign;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -508,7 +527,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
         }
         const int n = n0 + 32 * (block & 1) + l32, first = m0 + 32 * (block >> 1), m = first + 4 * hf;
         if (first >= a.M) break;
-        const int up = ACROSS == Across::kB ? t.shift_b[0] : shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
+        const int up = ACROSS == Across::kB ? 0 : shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             int4 back = make_int4(t.all_a, t.all_a, t.all_a, t.all_a);
@@ -659,12 +678,11 @@ void launch_halves_rows(const float *x, const float *weights, const Halves &h, b
                 {h.data, h.shift, h.row_blocks(), h.term_blocks(), negate, false, zero, zeros}, s);
 }
 
-void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s) {
-    const int64_t n = static_cast<int64_t>(h.rows) * h.terms;
-    largest_kernel<<<dim3(blocks_for(n, 16 * kThreads)), dim3(kThreads), 0, s>>>(x, n, aligned16(x), largest);
-    hipCheck(hipGetLastError());
-    halves_table_kernel<<<dim3(h.row_blocks(), (h.term_blocks() + 7) / 8), dim3(kThreads), 0, s>>>(
-        x, h.terms, h, h.terms % 4 == 0 && aligned16(x), largest);
+void launch_halves_table(const float *x, const Halves &h, hipStream_t s) {
+    auto kernel = h.terms <= 32 * 24   ? halves_table_kernel<24, false>
+                  : h.terms <= 32 * 52 ? halves_table_kernel<52, false>
+                                       : halves_table_kernel<52, true>;
+    kernel<<<dim3(h.row_blocks() / 2), dim3(kTableThreads), 0, s>>>(x, h, h.terms % 4 == 0 && aligned16(x));
     hipCheck(hipGetLastError());
 }
 

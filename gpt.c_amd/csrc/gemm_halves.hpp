@@ -71,9 +71,8 @@ struct HalvesRows {
     int zeros;
 };
 void launch_rows(const float *x, const float *weights, int rows, int terms, const HalvesRows &t, hipStream_t s);
-// x (rows x terms without gaps) as a first operand, all rows by the shift of its largest magnitude, whose bits *largest
-// receives (0 before).
-void launch_halves_table(const float *x, const Halves &h, uint32_t *largest, hipStream_t s);
+// x (rows x terms without gaps) as a first operand, 64 rows each by the shift of their largest magnitude (up to 126).
+void launch_halves_table(const float *x, const Halves &h, hipStream_t s);
 // x (terms x rows, rows of ld floats; with weights, times weights[k] / divisor by term k, and zeros where it is 0),
 // as a second operand, or as the one that is negated.  largest: the bits of each column's largest magnitude, which the
 // first call raises from what it holds and which may count further terms too; null with up to
@@ -94,8 +93,8 @@ struct HalvesProduct {
 };
 void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
 // C (A.terms x B.rows) = A^T B^T for A as in another product, where it was the first operand, with one shift; B is
-// negated.  C (A.rows x B.terms) = A B for such a B (of one shift, shift[0]).  What is read across is readable up to
-// 8 KB past its end.
+// negated.  C (A.rows x B.terms) = A B for such a B, with a shift for 64 rows each.  What is read across is readable up
+// to 8 KB past its end.
 void launch_product_across_a(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
 void launch_product_across_b(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s);
 // C from the sums of `slices` parts of the reduction, (M, N) each, in their order.

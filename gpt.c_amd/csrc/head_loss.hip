@@ -292,15 +292,14 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     const int padded = (piece + 127) / 128 * 128;
     Scratch scratch;
     Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
-    // The largest magnitudes of the columns of x, and of W.
-    uint32_t *largest_x = scratch.take<uint32_t>(h.C + 1), *largest = largest_x + h.C;
-    launch_halves_rows(h.x, h.weights, x, false, largest_x, h.C + 1, s);
-    // W is held by one shift, as its rows are the terms of dx: to 2^-40 of its largest value where it is below the 2^-17th
-    // of that, which counts for features of dx that small.  Laid out by rows and, for dx, a second time by columns it would
-    // be held to 2^-40 of each row's and column's largest, and cost 171 us instead of 88 (50257 x 768) and 371 instead of
-    // 164 (50257 x 1600).
+    uint32_t *largest_x = scratch.take<uint32_t>(h.C);  // magnitudes of x's columns
+    launch_halves_rows(h.x, h.weights, x, false, largest_x, h.C, s);
+    // W is held by a shift for 64 rows each, as its rows are the terms of dx, whose product takes 64 of them at a time: to
+    // 2^-40 of their largest value where it is below the 2^-17th of that, which counts for features of dx that small.  Laid
+    // out by rows and, for dx, a second time by columns it would be held to 2^-40 of each row's and column's largest, and
+    // cost 171 us instead of 69 (50257 x 768) and 371 instead of 166 (50257 x 1600).
     const Halves W = scratch.halves(h.V, h.C);
-    launch_halves_table(h.W, W, largest, s);
+    launch_halves_table(h.W, W, s);
     if (h.dW != nullptr) {
         xt = scratch.halves(h.C, piece);
         launch_column_largest(h.x, h.C, h.weights, static_cast<float>(h.rows), h.rows, h.C, largest_x, s);

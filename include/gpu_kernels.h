@@ -260,7 +260,7 @@ void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tenso
  *   outside [0, V) gives a NaN loss and the softmax part of the gradients, as
  *   cross_entropy_*_cuda_kernel.  Values of x and W are held to 24 bits where
  *   they are not far smaller than the largest of their row or column of x or
- *   of all of W, else to 2^-40 of that largest one; softmax's shares below
+ *   of 64 rows of W, else to 2^-40 of that largest one; softmax's shares below
  *   2^-16 to 2^-40.  W is taken to be finite: a value that is not
  *   makes the loss NaN.  A row of x that is not finite spoils its own loss and
  *   dx, output and dW.  V < 2^22.  Results may not overlap another tensor of

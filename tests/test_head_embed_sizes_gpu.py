@@ -260,3 +260,24 @@ def test_many_slices(rt, R, V, C):
     head.agree(one, ref)
     two = head.Call(rt, *a)
     assert np.array_equal(one.dx, two.dx)
+
+
+@pytest.mark.parametrize("R,V,C", [(4100, 200, 767), (4100, 130, 768), (4097, 129, 769), (4200, 70, 1664), (4100, 100, 1665),
+                                   (4099, 65, 2049)])
+def test_many_rows_of_many_features(rt, R, V, C):
+    """Rows of W that stay in a workgroup's registers, and longer ones."""
+    a = head.inputs(R, V, C, seed=9, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+def test_many_rows_where_w_changes_size(rt):
+    """64 tokens after the other whose largest values are far apart: each has a scale of its own, past 64 of them too."""
+    x, W, t, w = head.inputs(MANY, 5000, 40, weights=True)
+    rng = np.random.default_rng(13)
+    W = (W * np.ldexp(1.0, rng.integers(-30, 1, (79, 1))).repeat(64, 0)[:5000]).astype(np.float32)
+    W[128:192] = 0
+    W[192:256] = 1e-38
+    a = x, W, t, w
+    head.agree(head.Call(rt, *a), head.Exact(*a))
