@@ -390,21 +390,21 @@ void run_few(const HeadLoss &h, hipStream_t s) {
 // Whether W is read as it comes, again for every 128 rows and with a split of each float, instead of laid out first.
 // Rows, vocabulary x features: us as it comes / laid out.
 // With both gradients:
-//   256, 50257 x 768: 330 / 367       384, 50257 x 768: 475 / 452
-//   384, 50257 x 256: 215 / 246       512, 50257 x 256: 286 / 280
-//   384, 50257 x 64: 144 / 155        768, 50257 x 64: 254 / 222
-//   512, 5003 x 1600: 171 / 191       768, 5003 x 1600: 236 / 228
-//   1024, 1000 x 768: 97 / 101        1536, 1000 x 768: 112 / 102
-//   1024, 5003 x 100: 82 / 81         4095, 5003 x 100: 173 / 154
+//   100, 50257 x 768: 178 / 225       256, 50257 x 768: 328 / 316       384, 50257 x 768: 472 / 399
+//   256, 50257 x 256: 160 / 167       384, 50257 x 256: 208 / 200
+//   384, 50257 x 64: 138 / 142        512, 50257 x 64: 183 / 168
+//   384, 5003 x 1600: 152 / 152       768, 5003 x 1600: 233 / 199
+//   1024, 1000 x 768: 82 / 97         1536, 1000 x 768: 100 / 98
+//   512, 5003 x 100: 59 / 60          1024, 5003 x 100: 80 / 76         4095, 300 x 200: 65 / 68
 // The loss alone:
-//   100, 50257 x 768: 62 / 140        768, 50257 x 768: 270 / 279       1024, 50257 x 768: 349 / 335
-//   512, 50257 x 64: 41 / 44          1024, 50257 x 64: 63 / 61
-//   768, 5003 x 1600: 74 / 89         1536, 5003 x 1600: 121 / 121
-//   2048, 5003 x 100: 32 / 34         4095, 5003 x 100: 45 / 46
+//   100, 50257 x 768: 59 / 116        512, 50257 x 768: 183 / 194       768, 50257 x 768: 255 / 243
+//   768, 50257 x 64: 53 / 56          1536, 50257 x 64: 89 / 84
+//   768, 5003 x 1600: 71 / 80         1536, 5003 x 1600: 114 / 111
+//   2048, 5003 x 100: 31 / 33         4095, 5003 x 100: 45 / 46
 bool few_rows(int rows, int V, int C, bool grad) {
-    const int64_t read = (rows + 127) / 128 * 128, room = 2400000000 / (V * (C + 100ll));
-    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 &&
-           read <= (grad ? 256 + std::min<int64_t>(900, room) : 768 + room);
+    const int64_t read = (rows + 127) / 128 * 128, room = 1400000000 / (V * (C + 100ll));
+    const int64_t some = room >= 8192 ? 4096 : std::min<int64_t>(900, room);
+    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 && read <= (grad ? 256 + some : 600 + room);
 }
 
 }  // namespace

@@ -1,8 +1,8 @@
 """The cross entropy without logits and the sorted gradient at sizes on either side of where their kernels change, with
 the references, inputs and tolerances of test_head_loss_gpu.py and test_embed_sorted_gpu.py.
 
-W is read as it comes for few rows, up to 4096: as a multiple of 128, up to 256 + min(900, 2.4e9 / (V (C + 100))), or
-768 + 2.4e9 / (V (C + 100)) for the loss alone; else it is laid out first; there are kernels for 32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
+W is read as it comes for few rows, up to 4096: as a multiple of 128, up to 256 + min(900, room), room = 1.4e9 /
+(V (C + 100)), or for the loss alone 600 + room; for small tables, of a room past 8192, always; else it is laid out first; there are kernels for 32, 64 and 128 rows at once, and the gradient of W has its own up to 128 rows.  Up to 1024 ids are compared with each
 other; the sort ranks up to 12288 rows, then goes by digits, with more rows a workgroup from 131073 on; rows that are to be overwritten are not cleared where
 min(n, V) C >= 2^23.
 """
@@ -281,3 +281,12 @@ def test_many_rows_where_w_changes_size(rt):
     W[192:256] = 1e-38
     a = x, W, t, w
     head.agree(head.Call(rt, *a), head.Exact(*a))
+
+
+@pytest.mark.parametrize("R,V,C", [(384, 50257, 20), (385, 50257, 20), (768, 50257, 20), (769, 50257, 20),
+                                   (1152, 700, 400), (1153, 700, 400), (4096, 300, 50), (3000, 2000, 30)])
+def test_where_w_is_laid_out_by_room(rt, R, V, C):
+    a = head.inputs(R, V, C, seed=10, weights=True)
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
