@@ -64,12 +64,13 @@ __device__ __forceinline__ float2 put_logits(const LogitsArgs &l, hf32x16 (&x)[N
         }
     if (target >= 0 && target < 32 * NI && (target & 4) == 0) l.target_logits[row] = t;
     m = fmaxf(m, __shfl_xor(m, 32, 64));
-    const float ref = m == -INFINITY ? 0.0f : m * kLog2e;
+    const float ref = m == -INFINITY ? 0.0f : m;
     float s = 0.0f;
+    // The distance first, which is as exact as the logits: m times log2(e), rounded, would be off by 2^-24 of m itself.
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(x[i][r], kLog2e, -ref));
+        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((x[i][r] - ref) * kLog2e);
     s += __shfl_xor(s, 32, 64);
     return make_float2(m, s);
 }

@@ -1,0 +1,90 @@
+"""The softmax of gptc_linear_cross_entropy_cuda apart from its products: logits that are exact in fp32.
+
+x = (1, K) and W = (a_j, 1) with a_j a multiple of 1/16 and K whole: the logits a_j + K, their largest one m, and l - m are
+exact, in the two fp16 parts and in every sum.  So a row's loss and gradients may not depend on K at all, and what is
+left are the roundings of the softmax.  With u = 2^-24, V tokens:
+  e = exp(l - m) comes as exp2 of (l - m) times log2(e) in fp32: off by 1.3 u of its argument, 2 u for exp2; where a part's
+    sum moves to another largest value, that splits into distances which add up to l - m, each with 3 u more.
+  s, the sum: at most V - 1 additions of positive values that are not 0, of which no chain has more than 75 + V / 2048, in
+    at most ceil(V / 32), 12, moves:  S = (min(V - 1, 75 + V / 2048) + 3 min(ceil(V / 32), 12)) u + 2 u sum p |l - m|.
+  loss = log s - (l_t - m): S, 4 u of log s and 2 u of the loss and its larger term.
+  p = e / s: 2 u |l - m| + 6 u + S of p;  d = p - [j = t]: 2 u |d| more, and 2^-39 where its parts end.
+  dx, dW: those times the other operand, and of the products' |terms| (4 + min(n, 64) + n / 32) u for n terms.
+"""
+import numpy as np
+import pytest
+
+import test_head_loss_gpu as head
+
+pytestmark = pytest.mark.gpu
+
+U, END = head.U, head.END
+MANY = 4225  # rows past 4096: W is laid out
+
+
+def tokens(kind, V):
+    rng = np.random.default_rng([7, V])
+    if kind == "confident":  # one token 11 above the others: their shares are 1e-5 and less
+        a = rng.integers(0, 33, V) / 16
+        a[V // 2] = 13
+    elif kind == "equal":
+        a = np.full(V, 3.0)
+    else:
+        a = rng.integers(-128, 129, V) / 16
+    return a
+
+
+def problem(kind, R, V, far):
+    """Rows in pairs of one target, the second of each by K away."""
+    rng = np.random.default_rng([8, R, V])
+    a = tokens(kind, V)
+    t = np.where(rng.random(R) < 0.5, int(a.argmax()), rng.integers(0, V, R))
+    t[1::2] = t[0:2 * (R // 2):2]
+    K = rng.integers(far // 2, far + 1, R) * rng.choice([-1, 1], R)
+    K[0::2] = 0
+    x = np.stack([np.ones(R), K], 1).astype(np.float32)
+    W = np.stack([a, np.ones(V)], 1).astype(np.float32)
+    return x, W, t.astype(np.float32), a
+
+
+def bounds(x, W, t, a):
+    """(losses, bound), (dx, bound), (dW, bound) in 64 bits; the logits of all rows differ by K alone."""
+    R, V = len(x), len(a)
+    t = t.astype(int)
+    far = a - a.max()
+    e = np.exp(far)
+    s = e.sum()
+    p = e / s
+    S = (min(V - 1, 75 + V / 2048) + 3 * min(-(-V // 32), 12)) * U + 2 * U * (p * -far).sum()
+    losses = np.log(s) - far[t]
+    losses_tol = S + 4 * U * np.log(s) + 2 * U * (losses + np.abs(far[t]))
+    d = np.repeat(p[None], R, 0)
+    d[np.arange(R), t] -= 1
+    Ed = (p * (2 * U * -far + 6 * U + S))[None] + 2 * U * np.abs(d) + END
+    aW, ax = np.abs(W).astype(np.float64), np.abs(x).astype(np.float64)
+    dx = d @ W.astype(np.float64) / R
+    dx_tol = (Ed @ aW + (4 + min(V, 64) + V / 32) * U * (np.abs(d) @ aW)) / R
+    dW = d.T @ x.astype(np.float64) / R
+    dW_tol = (Ed.T @ ax + (4 + min(R, 64) + R / 32) * U * (np.abs(d).T @ ax) + END * R * ax.max(0)) / R
+    return (losses, losses_tol), (dx, dx_tol), (dW, dW_tol)
+
+
+def close(name, got, want, tol):
+    err = np.abs(got.astype(np.float64) - want)
+    print(f"  {name}: error at most {(err / tol).max():.3f} of its bound, largest {err.max():.2e}", flush=True)
+    assert (err <= tol).all(), name
+
+
+CASES = [(kind, R, V) for R in (2, 5, 31, 100, 300, MANY) for kind, V in
+         (("confident", 5), ("confident", 40), ("confident", 600), ("spread", 40), ("spread", 600), ("equal", 4),
+          ("equal", 333))]
+
+
+@pytest.mark.parametrize("far", [128, 4000])
+@pytest.mark.parametrize("kind,R,V", CASES)
+def test_losses_of_exact_logits(rt, kind, R, V, far):
+    x, W, t, a = problem(kind, R, V, far)
+    got = head.Call(rt, x, W, t, dx=False, dW=False)
+    close("losses", got.losses, *bounds(x, W, t, a)[0])
+    pairs = R // 2 * 2
+    assert np.array_equal(got.losses[0:pairs:2], got.losses[1:pairs:2])  # the same distances from the largest
