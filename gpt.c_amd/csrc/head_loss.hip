@@ -67,16 +67,17 @@ struct JoinArgs {
     const float2 *stats;
     int parts;
     const float *targets, *target_logits, *weights;
-    float *lse;
-    int *whole;  // the targets, -1 for none
+    float2 *shares;  // what a row's shares are taken by: the largest logit and 1 / sum
+    int *whole;      // the targets, -1 for none
     float *losses;
     int rows, padded, V;
     float *mean;  // MEAN: of all rows, which are the first workgroup's
 };
 
-// A row's loss, lse and target from the parts of its tokens: ROWS rows a workgroup, whose slices of
-// the parts are joined in a fixed order.  Rows that take no part, those past the last one among them:
-// lse is infinite, which makes their shares 0, and the target -1.  Latency bound (100 rows: 5.6 us).
+// A row's loss, largest logit m, 1 / sum and target from the parts of its tokens: ROWS rows a workgroup, whose slices of
+// the parts are joined in a fixed order.  m and the sum stay apart: their join, lse = m + log(sum), would be rounded to
+// 2^-24 of itself, and every share of the row with it.  Rows that take no part, those past the last one among them: 1 / sum
+// is 0 and the target -1.  Latency bound (100 rows: 5.6 us).
 constexpr int kJoinThreads = 1024;
 
 // What sums are taken relative to: without a logit but minus infinity they are 0, or NaN where there is one.
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_stats_kernel(const JoinArgs
     const int target = live ? token_of(a.targets[row], a.V) : -1;
     const float logsum = logf(s);
     const float loss = !live ? 0.0f : target >= 0 ? logsum - (a.target_logits[row] - m) : NAN;
-    a.lse[row] = live ? m + logsum : INFINITY;
+    a.shares[row] = live ? make_float2(m, 1.0f / s) : make_float2(0.0f, 0.0f);
     a.whole[row] = target;
     if (row < a.rows) a.losses[row] = loss;
     if (!MEAN || blockIdx.x > 0) return;
@@ -157,7 +158,8 @@ void launch_join_stats(const JoinArgs &a, hipStream_t s) {
 }
 
 struct ShareArgs {
-    const float *logits, *lse;
+    const float *logits;
+    const float2 *shares;  // of the rows
     const int *targets;
     hu32x4 *d, *dt;  // as first operands of d W and d^T x; either may be null
     int row_blocks, token_blocks;  // of the logits
@@ -169,7 +171,7 @@ struct ShareArgs {
 constexpr int kShareShift = 15;  // shares are held times 2^15
 constexpr int kShareStride = 36;  // words of LDS a token: 16-byte rows, no two in the same banks
 
-// d' = exp(l - lse) - [target] of a block of 32 rows x 32 tokens, in two fp16 parts, as the
+// d' = exp(l - m) / sum - [target] of a block of 32 rows x 32 tokens, in two fp16 parts, as the
 // operand of either product.  The logits come in the order of the accumulators: a lane holds row
 // l % 32 and tokens 8 q + 4 (l / 32) + {0 .. 3}, which is also its share of d's block; d^T's goes
 // through LDS.  Memory bound: 4 bytes in, 4 out for each operand (8192 rows, 50257 tokens, d alone: 575 us, 5.7 TB/s).
@@ -184,9 +186,9 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
     const int rb = blockIdx.y;
     const int first = (blockIdx.x * 4 + w) * a.per_wave;
     const int row = rb * 32 + l32;
-    const float lse = a.lse[row];
+    const float m = a.shares[row].x, by_sum = a.shares[row].y;
     const int target = a.targets[row];
-    const bool live = lse != INFINITY;  // else there may be no logits
+    const bool live = by_sum != 0.0f;  // else there may be no logits
     uint32_t *mine = lds[w];
     for (int jb = first; jb < min(first + a.per_wave, a.token_blocks); ++jb) {
         const f32x4_t *x = reinterpret_cast<const f32x4_t *>(a.logits) +
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void shares_kernel(const ShareArgs a) {
         for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = live ? __builtin_amdgcn_exp2f((v[q][e] - lse) * kLog2eF) : 0.0f;
+                const float p = live ? __builtin_amdgcn_exp2f((v[q][e] - m) * kLog2eF) * by_sum : 0.0f;
                 v[q][e] = p - (jb * 32 + 8 * q + 4 * hf + e == target ? 1.0f : 0.0f);
             }
         uint32_t high[4][2], low[4][2];
@@ -308,7 +310,8 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
     float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 64));
     int *targets = scratch.take<int>(padded);
-    float *target_logits = scratch.take<float>(padded), *lse = scratch.take<float>(padded);
+    float *target_logits = scratch.take<float>(padded);
+    float2 *shares = scratch.take<float2>(padded);
     for (int r = 0; r < h.rows; r += piece) {
         const int n = std::min(piece, h.rows - r), n_padded = (n + 127) / 128 * 128;
         const float *xr = h.x + static_cast<int64_t>(r) * h.C;
@@ -317,11 +320,11 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         if (r > 0) launch_halves_rows(xr, weights, x, false, nullptr, 0, s);
         const int part = launch_logits(
             W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
-        launch_join_stats({stats, tokens / part, h.targets + r, target_logits, weights, lse, targets, h.losses + r, n,
-                           n_padded, h.V, nullptr},
+        launch_join_stats({stats, tokens / part, h.targets + r, target_logits, weights, shares, targets, h.losses + r,
+                           n, n_padded, h.V, nullptr},
                           s);
         if (!grad) continue;
-        const ShareArgs a{logits, lse, targets, d.data, nullptr, n_padded / 32, tokens / 32, 0,
+        const ShareArgs a{logits, shares, targets, d.data, nullptr, n_padded / 32, tokens / 32, 0,
                           (h.V + 63) / 64 * 2, 0, {h.losses, h.weights, r + piece >= h.rows ? h.mean : nullptr, h.rows}};
         launch_shares(a, s);
         if (h.dx != nullptr)
@@ -352,19 +355,20 @@ void run_few(const HeadLoss &h, hipStream_t s) {
     float *logits = grad ? scratch.take<float>(static_cast<int64_t>(padded) * tokens) : nullptr;
     float2 *stats = scratch.take<float2>(static_cast<int64_t>(padded) * (tokens / 32));
     int *targets = scratch.take<int>(padded);
-    float *target_logits = scratch.take<float>(padded), *lse = scratch.take<float>(padded);
+    float *target_logits = scratch.take<float>(padded);
+    float2 *shares = scratch.take<float2>(padded);
     const int part = launch_few_logits(
         h.W, h.V, h.C, x, {logits, stats, h.targets, target_logits, h.V, h.rows, tokens / 32, padded}, s);
     const bool mean = h.rows <= kMeanRows;
-    launch_join_stats({stats, tokens / part, h.targets, target_logits, h.weights, lse, targets, h.losses, h.rows, padded,
-                       h.V, mean ? h.mean : nullptr},
+    launch_join_stats({stats, tokens / part, h.targets, target_logits, h.weights, shares, targets, h.losses, h.rows,
+                       padded, h.V, mean ? h.mean : nullptr},
                       s);
     if (!grad && !mean) launch_mean(h, s);
     if (grad) {
         Halves dt{nullptr, nullptr, kShareShift, h.V, h.rows}, xt{};
         if (h.dx != nullptr) d.data = scratch.take<hu32x4>(d.bytes() / own * blocks / 16);
         if (h.dW != nullptr) dt.data = scratch.take<hu32x4>(dt.bytes() / 16);
-        launch_shares({logits, lse, targets, d.data, dt.data, blocks, tokens / 32, dt.term_blocks() / 2,
+        launch_shares({logits, shares, targets, d.data, dt.data, blocks, tokens / 32, dt.term_blocks() / 2,
                        tokens / 32, 0, {h.losses, h.weights, mean ? nullptr : h.mean, h.rows}},
                       s);
         if (h.dx != nullptr)

@@ -88,3 +88,18 @@ def test_losses_of_exact_logits(rt, kind, R, V, far):
     close("losses", got.losses, *bounds(x, W, t, a)[0])
     pairs = R // 2 * 2
     assert np.array_equal(got.losses[0:pairs:2], got.losses[1:pairs:2])  # the same distances from the largest
+
+
+@pytest.mark.parametrize("far", [128, 4000])
+@pytest.mark.parametrize("kind,R,V", CASES)
+def test_gradients_of_exact_logits(rt, kind, R, V, far):
+    """dx of the constant feature is the sum of a row of d: 0 but for what the shares are off by together."""
+    x, W, t, a = problem(kind, R, V, far)
+    got = head.Call(rt, x, W, t)
+    losses, dx, dW = bounds(x, W, t, a)
+    close("losses", got.losses, *losses)
+    close("dx", got.dx, *dx)
+    close("dW", got.dW, *dW)
+    pairs = R // 2 * 2
+    assert np.array_equal(got.losses[0:pairs:2], got.losses[1:pairs:2])
+    assert np.array_equal(got.dx[0:pairs:2], got.dx[1:pairs:2])
