@@ -173,6 +173,14 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves)
                 }
             }
         }
+        // Past a row's last feature lie the next row's, which its scale may not see.
+        if (!DX && 32 * (step + 1) > a.C) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (32 * step + 16 * hf + 8 * k + e >= a.C) v[k][e] = 0.0f;
+        }
         float top = 0.0f;
 #pragma unroll
         for (int k = 0; k < 2; ++k)

@@ -103,3 +103,20 @@ def test_gradients_of_exact_logits(rt, kind, R, V, far):
     pairs = R // 2 * 2
     assert np.array_equal(got.losses[0:pairs:2], got.losses[1:pairs:2])
     assert np.array_equal(got.dx[0:pairs:2], got.dx[1:pairs:2])
+
+
+@pytest.mark.parametrize("R", [1, 40, 100, MANY])
+@pytest.mark.parametrize("C", [33, 63, 70])
+def test_a_loud_row_of_w_behind_a_quiet_one(rt, R, C):
+    """Row 64 begins with values of 2^60, where x is 0.  They lie behind row 63's last features in memory, and belong to
+    another 64 rows: row 63's logits, and all gradients but dx of those features, are as if they were 0."""
+    x, W, t, w = head.inputs(R, 200, C, seed=12, weights=True)
+    x[:, :31] = 0
+    W[64:128] = 0
+    t[0], w[0] = 63, 1
+    ref = head.Exact(x, W, t, w)
+    W[64, :31] = 2.0 ** 60
+    got = head.Call(rt, x, W, t, w)
+    ref.dx, ref.dx_tol, got.dx = ref.dx[:, 31:], ref.dx_tol[:, 31:], got.dx[:, 31:]
+    head.agree(got, ref)
+    head.agree(head.Call(rt, x, W, t, w, dx=False, dW=False), ref)
