@@ -50,7 +50,8 @@ __device__ __forceinline__ f32x4_t fma_of(float a, f32x4_t b, f32x4_t c) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(const T *__restrict__ W, const T *__restrict__ P,
                                                          const float *__restrict__ ids, float scale,
-                                                         T *__restrict__ out, int rows, int seq, int cols, int V) {
+                                                         T *__restrict__ out, int rows, int before, int seq, int cols,
+                                                         int V) {
     const int lane = threadIdx.x & (kWave - 1);
     const int row = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (row >= rows) return;
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(const T *__restrict__ 
     }
     const T *w = W + static_cast<int64_t>(id) * cols;
     if (P != nullptr) {
-        const T *p = P + static_cast<int64_t>(row % seq) * cols;
+        const T *p = P + static_cast<int64_t>((static_cast<uint32_t>(before) + row) % seq) * cols;
         for (int j = lane; j < cols; j += kWave) o[j] = fma_of(scale, w[j], p[j]);
     } else {
         for (int j = lane; j < cols; j += kWave) o[j] = scale * w[j];
@@ -785,16 +786,23 @@ extern "C" void gptc_embedding_forward_scaled_cuda(const tensor_t *W, const tens
                 "output may not overlap another tensor of the call.");
     if (n == 0) return;
     const int V = W->shape[0], C = W->shape[1], seq = pos != NULL ? last_dim(ids) : 1;
-    const dim3 grid((n + kWaves - 1) / kWaves);
+    const float *P = pos != NULL ? pos->t : nullptr;
     hipStream_t s = gptc_stream_checked();
-    if (C % 4 == 0 && aligned16(W->t) && aligned16(output->t) && (pos == NULL || aligned16(pos->t)))
-        lookup_kernel<f32x4_t><<<grid, dim3(kThreads), 0, s>>>(
-            reinterpret_cast<const f32x4_t *>(W->t), reinterpret_cast<const f32x4_t *>(pos != NULL ? pos->t : nullptr),
-            ids->t, scale, reinterpret_cast<f32x4_t *>(output->t), n, seq, C / 4, V);
-    else
-        lookup_kernel<float><<<grid, dim3(kThreads), 0, s>>>(W->t, pos != NULL ? pos->t : nullptr, ids->t, scale,
-                                                             output->t, n, seq, C, V);
-    hipCheck(hipGetLastError());
+    const bool vec = C % 4 == 0 && aligned16(W->t) && aligned16(output->t) && aligned16(P);
+    // A wave a row, and as many launches as that takes (of more than 2^26 rows).
+    constexpr int kMost = (kMaxGroups - 1) * kWaves;
+    for (int64_t r = 0; r < n; r += kMost) {
+        const int rows = static_cast<int>(std::min<int64_t>(n - r, kMost)), before = static_cast<int>(r % seq);
+        const dim3 grid((rows + kWaves - 1) / kWaves);
+        float *out = output->t + r * C;
+        if (vec)
+            lookup_kernel<f32x4_t><<<grid, dim3(kThreads), 0, s>>>(
+                reinterpret_cast<const f32x4_t *>(W->t), reinterpret_cast<const f32x4_t *>(P), ids->t + r, scale,
+                reinterpret_cast<f32x4_t *>(out), rows, before, seq, C / 4, V);
+        else
+            lookup_kernel<float><<<grid, dim3(kThreads), 0, s>>>(W->t, P, ids->t + r, scale, out, rows, before, seq, C, V);
+        hipCheck(hipGetLastError());
+    }
 }
 
 extern "C" void gptc_embedding_backward_sorted_cuda(const tensor_t *global_grad, const tensor_t *ids,

@@ -1,0 +1,33 @@
+"""The lookup and the sorted gradient at sizes whose launches or whole numbers end.  Values are whole numbers, whose sums
+and products are exact in fp32."""
+import numpy as np
+import pytest
+
+import test_embed_sorted_gpu as sorted_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("positions", [False, True])
+def test_lookup_of_more_ids_than_a_launch_has_waves(rt, positions):
+    """2^26 rows, a wave each, are 2^32 threads."""
+    shape = (4097, 16384)
+    ids = (np.arange(shape[0] * shape[1], dtype=np.int64) * 7 % 41).astype(np.float32).reshape(shape)
+    W = np.arange(37, dtype=np.float32)[:, None] - 11
+    P = np.arange(16384, dtype=np.float32)[:, None] if positions else None
+    got = sorted_gpu.lookup(rt, W, P, ids, 3.0)[..., 0]
+    table = np.append(3 * W[:, 0], np.full(4, np.nan, np.float32))
+    for b in (0, 1, 2048, 4094, 4095, 4096):
+        want = table[ids[b].astype(int)]
+        assert np.array_equal(got[b], want + P[:, 0] if positions else want, equal_nan=True), b
+    assert np.array_equal(np.isnan(got), ids >= 37)
+
+
+def test_gradient_of_as_many(rt):
+    shape = (4097, 16384)
+    ids = (np.arange(shape[0] * shape[1], dtype=np.int64) * 7 % 41).astype(np.float32).reshape(shape)
+    g = np.ones((*shape, 1), np.float32)
+    dW, dP = sorted_gpu.gather(rt, g, ids, 1.0, np.full((37, 1), np.nan, np.float32),
+                               np.full((16384, 1), np.nan, np.float32))
+    assert np.array_equal(dW[:, 0], np.bincount(ids.ravel().astype(np.int64), minlength=41)[:37].astype(np.float32))
+    assert (dP == 4097).all()
