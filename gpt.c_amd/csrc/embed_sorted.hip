@@ -724,7 +724,7 @@ void launch_gather(const float *ids, GatherArgs a, hipStream_t s) {
     // A wave each for 32 places, fewer where that leaves less than eight waves a CU.
     a.chunk = 32;
     while (a.chunk > 8 && static_cast<int64_t>(a.n) * a.blocks < 2048ll * a.chunk) a.chunk /= 2;
-    const int chunks = (a.n + a.chunk - 1) / a.chunk;
+    const int chunks = static_cast<int>((static_cast<int64_t>(a.n) + a.chunk - 1) / a.chunk);
     const int position_blocks = a.dP != nullptr ? (a.positions + kWaves - 1) / kWaves : 0;
     const int per = position_blocks + (chunks + kWaves - 1) / kWaves;
     CHECK_ERROR(static_cast<int64_t>(std::max(per, chunks)) * a.blocks >= kMaxGroups,

@@ -1,11 +1,18 @@
 """The lookup and the sorted gradient at sizes whose launches or whole numbers end.  Values are whole numbers, whose sums
 and products are exact in fp32."""
+import os
+import subprocess
+import sys
+import textwrap
+
 import numpy as np
 import pytest
 
 import test_embed_sorted_gpu as sorted_gpu
 
 pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.mark.parametrize("positions", [False, True])
@@ -31,3 +38,21 @@ def test_gradient_of_as_many(rt):
                                np.full((16384, 1), np.nan, np.float32))
     assert np.array_equal(dW[:, 0], np.bincount(ids.ravel().astype(np.int64), minlength=41)[:37].astype(np.float32))
     assert (dP == 4097).all()
+
+
+def test_gradient_of_too_many_is_refused():
+    """2^31 - 1 ids, whose parts' count may not wrap."""
+    code = textwrap.dedent(f"""
+        import sys
+        sys.path.insert(0, {os.path.join(ROOT, 'gpt.c_amd')!r})
+        import gptc
+        rt = gptc.Runtime(gptc.load())
+        rt.init()
+        n = (1 << 31) - 1
+        g, ids, dW = rt.empty((n, 1)), rt.empty((n,)), rt.empty((5, 1))
+        print("made", flush=True)
+        rt.lib.gptc_embedding_backward_sorted_cuda(g, ids, 1.0, dW, None, 0)
+        print("returned")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 1 and "made" in r.stdout and "Too many rows" in r.stderr and "returned" not in r.stdout, r.stderr
