@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kLog2eF = 1.4426950408889634f;
-constexpr int kMaxVocabulary = 1 << 22;      // a product's tile offsets fit 32 bits
+constexpr int kMaxVocabulary = 1 << 22;  // a product's tile offsets fit 32 bits
+constexpr int kMaxRows = 1000000000;     // 2^24 workgroups of column_largest_kernel; a piece more still fits an int
 
 __device__ __forceinline__ float weight_of(const float *weights, int row) {
     return weights != nullptr ? weights[row] : 1.0f;
@@ -431,6 +432,7 @@ extern "C" void gptc_linear_cross_entropy_cuda(const tensor_t *x, const tensor_t
     CHECK_ERROR(last_dim(x) != C, "Expected x's last dimension to be %d, but got %d.", C, last_dim(x));
     const int rows = x->length / C;
     CHECK_ERROR(rows < 1, "Expected at least one row of x.");
+    CHECK_ERROR(rows > kMaxRows, "Expected up to %d rows of x, but got %d.", kMaxRows, rows);
     CHECK_ERROR(targets->length != rows, "Expected %d targets, but got %d.", rows, targets->length);
     CHECK_ERROR(output->length < 1, "Expected output to hold the loss.");
     const tensor_t *in[4] = {x, W, targets, weights};

@@ -263,9 +263,10 @@ void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tenso
  *   of 64 rows of W, else to 2^-40 of that largest one; softmax's shares below
  *   2^-16 to 2^-40.  W is taken to be finite: a value that is not
  *   makes the loss NaN.  A row of x that is not finite spoils its own loss and
- *   dx, output and dW.  V < 2^22.  Results may not overlap another tensor of
- *   the call.  Deterministic.  Takes scratch (the logits of up to 3328 rows of
- *   50257 at a time, and W's copy): not under graph capture.
+ *   dx, output and dW.  V and C < 2^22, up to 10^9 rows.  Results may not
+ *   overlap another tensor of the call.  Deterministic.  Takes scratch (the
+ *   logits of up to 3328 rows of 50257 at a time, and W's copy): not under
+ *   graph capture.
  *
  * gptc_embedding_forward_scaled_cuda(W, pos, ids, scale, output)
  *   output (ids..., C) = scale W[ids] (+ pos[i], i the id's place in ids' last

@@ -1,4 +1,4 @@
-"""The lookup and the sorted gradient at sizes whose launches or whole numbers end.  Values are whole numbers, whose sums
+"""The two ends of a GPT at sizes whose launches or whole numbers end.  Of the tables, values are whole numbers, whose sums
 and products are exact in fp32."""
 import os
 import subprocess
@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 
 import test_embed_sorted_gpu as sorted_gpu
+import test_head_loss_gpu as head
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +57,21 @@ def test_gradient_of_too_many_is_refused():
     """)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert r.returncode == 1 and "made" in r.stdout and "Too many rows" in r.stderr and "returned" not in r.stdout, r.stderr
+
+
+@pytest.mark.parametrize("R", [5, 70])
+def test_as_many_features_as_there_may_be(rt, R):
+    """All but 200 of 2^22 - 1 features are zero in x and W: the reference has those alone."""
+    C, rng = (1 << 22) - 1, np.random.default_rng(R)
+    at = np.sort(rng.choice(C - 2, 198, replace=False))
+    at = np.concatenate([at, [C - 2, C - 1]])
+    x, W, t, w = head.inputs(R, 3, 200, weights=True)
+    ref = head.Exact(x, W, t, w)
+    wide = [np.zeros((len(a), C), np.float32) for a in (x, W)]
+    for a, b in zip(wide, (x, W)):
+        a[:, at] = b
+    got = head.Call(rt, *wide, t, w)
+    got.dx, dx, got.dW, dW = got.dx[:, at], got.dx, got.dW[:, at], got.dW
+    head.agree(got, ref)
+    assert np.count_nonzero(dx) == np.count_nonzero(got.dx) and np.count_nonzero(dW) == np.count_nonzero(got.dW)
+    head.agree(head.Call(rt, *wide, t, w, dx=False, dW=False), ref)
