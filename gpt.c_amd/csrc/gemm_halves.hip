@@ -409,6 +409,8 @@ __device__ __forceinline__ void tile_product(const Tile &t, int tm, int tn, int 
     const bool minus = ACROSS == Across::kA ? ((w / S::WN) & 1) != 0 : ACROSS == Across::kB ? ((w % S::WN) & 1) != 0 : false;
     float sign = ((s0 & 2) != 0) != minus ? -1.0f : 1.0f;
     int shifts = 0;  // of B read across: lane l holds that of the 64 terms after 64 l others
+    // There A's scale goes too: sums that kept it would pass the largest float with values of B 2^15 below it.
+    if (ACROSS == Across::kB) sign = __builtin_amdgcn_ldexpf(sign, -t.all_a);
     for (int s = s0; s < s1; s += 2) {
         float times = sign;
         if constexpr (ACROSS == Across::kB) {
@@ -530,7 +532,8 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
         const int up = ACROSS == Across::kB ? 0 : shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            int4 back = make_int4(t.all_a, t.all_a, t.all_a, t.all_a);
+            const int all_a = ACROSS == Across::kB ? 0 : t.all_a;
+            int4 back = make_int4(all_a, all_a, all_a, all_a);
             if (t.shift_a != nullptr) back = *reinterpret_cast<const int4 *>(t.shift_a + m + 8 * q);
             v[4 * q] = __builtin_amdgcn_ldexpf(v[4 * q], -up - back.x);
             v[4 * q + 1] = __builtin_amdgcn_ldexpf(v[4 * q + 1], -up - back.y);

@@ -78,6 +78,7 @@ struct FewArgs {
 // whole lines (a lane a row, as the fragments want them, costs a cycle of the address path for every lane: the
 // logits of 16 rows of 768 on 50257 tokens took 39 us so and take 28).  Up to four waves a SIMD, which hide
 // each other's chain of loads, largest value, split and products.
+constexpr int kSmallShift = kHalvesTop + 1;  // the small operand is held below 2^15: d by this shift, x by its rows'
 template <int NB>
 struct FewShape {
     static constexpr int kBlocks = NB < 2 ? NB : 2;                      // of 32 rows a wave
@@ -214,7 +215,9 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves)
 #pragma unroll
                 for (int i = 0; i < S::kBlocks; ++i) t[i] = mfma_f16(g[i][kParts[q][0]], f[kParts[q][1]], t[i]);
         }
-        const float down = __builtin_amdgcn_ldexpf(step & 2 ? -1.0f : 1.0f, -up);  // 64 terms of a sign
+        // 64 terms of a sign.  Both scales go: with the small operand's, values of W 2^15 below the largest float would take
+        // the sums past it.
+        const float down = __builtin_amdgcn_ldexpf(step & 2 ? -1.0f : 1.0f, -up - kSmallShift);
 #pragma unroll
         for (int i = 0; i < S::kBlocks; ++i)
 #pragma unroll
@@ -241,7 +244,8 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves)
                 const int shift[4] = {back.x, back.y, back.z, back.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    across[(8 * q + 4 * hf + e) * kStride + l32] = __builtin_amdgcn_ldexpf(v[0][4 * q + e], -shift[e]);
+                    across[(8 * q + 4 * hf + e) * kStride + l32] =
+                        __builtin_amdgcn_ldexpf(v[0][4 * q + e], kSmallShift - shift[e]);
             }
             wave_lds_order();
 #pragma unroll
@@ -262,9 +266,8 @@ __global__ __launch_bounds__(64 * FewShape<NB>::kWaves)
         const uint32_t lane_out = c < a.C ? 4 * (static_cast<uint32_t>((block + i) * 32 + 4 * hf) * a.C + c) : 0x80000000u;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            __builtin_amdgcn_raw_buffer_store_b32(
-                __float_as_uint(__builtin_amdgcn_ldexpf(v[0][r], -a.small.shift_all)), out, lane_out,
-                min(4 * (8 * (r >> 2) + (r & 3)) * a.C, bytes), 0);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0][r]), out, lane_out,
+                                                  min(4 * (8 * (r >> 2) + (r & 3)) * a.C, bytes), 0);
     }
     if (DX) return;
     __syncthreads();
@@ -406,6 +409,7 @@ void launch_few_dx(const FewRows &d, const float *W, int V, int C, int rows, con
     const int slice = ((kbs + slices - 1) / slices + 7) / 8 * 8;  // whole steps, whose signs alternate
     slices = (kbs + slice - 1) / slice;
     float *part = static_cast<float *>(alloc_cuda(sizeof(float) * static_cast<size_t>(rows) * C * slices));
+    CHECK_ERROR(d.shift != nullptr || d.shift_all != kSmallShift, "few_dx: shares times 2^%d.", d.shift_all);
     run_few<true>({W, V, C, d, {}, rows, slice, columns, part}, std::min(d.row_blocks, 4),
                   columns * ((slices + 7) / 8 * 8), s);
     launch_join_slices(part, rows, C, slices, p, s);

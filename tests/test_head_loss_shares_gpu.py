@@ -120,3 +120,14 @@ def test_a_loud_row_of_w_behind_a_quiet_one(rt, R, C):
     ref.dx, ref.dx_tol, got.dx = ref.dx[:, 31:], ref.dx_tol[:, 31:], got.dx[:, 31:]
     head.agree(got, ref)
     head.agree(head.Call(rt, x, W, t, w, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R", [5, 90, 300, MANY])
+@pytest.mark.parametrize("shift", [-118, -110, 110, 118])
+def test_values_near_the_ends_of_fp32(rt, R, shift):
+    """x times 2^shift and W times 2^-shift: ordinary logits, and a dx or dW of up to 2^119.  (The other one is subnormal.)"""
+    x, W, t, w = head.inputs(R, 500, 70, seed=13, weights=True)
+    a = np.ldexp(x, shift), np.ldexp(W, -shift), t, w
+    ref = head.Exact(*a)
+    head.agree(head.Call(rt, *a, dx=shift < 0, dW=shift > 0), ref)
+    head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
