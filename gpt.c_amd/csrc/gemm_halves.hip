@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void halves_rows_kernel(const floa
     uint2 *out = reinterpret_cast<uint2 *>(t.data + static_cast<int64_t>(row >> 5) * t.term_blocks * 128 + (row & 31));
     auto put = [&](int k, f32x4_t v) {
         if (k >= 16 * t.term_blocks) return;
-        const uint32_t flip = t.negate && halves_negated(k) ? 0x80008000u : 0;
+        const uint32_t flip = t.in_lines && halves_negated(k) ? 0x80008000u : 0;
         uint2 high, low;
         halves_split(__builtin_amdgcn_ldexpf(v[0], up), __builtin_amdgcn_ldexpf(v[1], up), high.x, low.x);
         halves_split(__builtin_amdgcn_ldexpf(v[2], up), __builtin_amdgcn_ldexpf(v[3], up), high.y, low.y);
@@ -273,13 +273,11 @@ __global__ __launch_bounds__(kThreads) void halves_columns_kernel(const float *_
 
 struct Tile {
     const hu32x4 *A, *B;
-    const int *shift_a, *shift_b;
-    int all_a, all_b;  // where shift_a or shift_b is null
+    const int *shift_a, *shift_b;  // of the rows; shift_a for logits alone
+    int all_a;                     // where shift_a is null
     int tiles_m, tiles_n, kbs, stages, slice;  // stages of 32 terms in all, and of a slice
     int kbs_across;  // blocks of 16 of what are rows here of the operand that is read across
 };
-
-__device__ __forceinline__ int shift_of(const int *shift, int all, int row) { return shift != nullptr ? shift[row] : all; }
 
 // The tile and slice of this workgroup (grid: tiles by slices, or slices of few tiles one after the other).  Workgroup i
 // runs on XCD i % 8: 8 contiguous ranges of a slice's tiles, or of all slices' where those are few (so that a slice's
@@ -476,7 +474,7 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
     // In a loop, as its code is fetched by every workgroup.
 #pragma unroll 1
     for (int j = 0; j < 2; ++j) {
-        const int up = shift_of(t.shift_b, t.all_b, row0 + 32 * j + l32);
+        const int up = t.shift_b[row0 + 32 * j + l32];
         hf32x16 x[S::NI];
 #pragma unroll
         for (int i = 0; i < S::NI; ++i) {
@@ -529,17 +527,9 @@ __global__ __launch_bounds__(S::kThreads) __attribute__((amdgpu_waves_per_eu(2, 
         }
         const int n = n0 + 32 * (block & 1) + l32, first = m0 + 32 * (block >> 1), m = first + 4 * hf;
         if (first >= a.M) break;
-        const int up = ACROSS == Across::kB ? 0 : shift_of(t.shift_b, t.all_b, min(n, a.N - 1));
+        const int up = ACROSS == Across::kB ? 0 : -t.all_a - t.shift_b[min(n, a.N - 1)];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int all_a = ACROSS == Across::kB ? 0 : t.all_a;
-            int4 back = make_int4(all_a, all_a, all_a, all_a);
-            if (t.shift_a != nullptr) back = *reinterpret_cast<const int4 *>(t.shift_a + m + 8 * q);
-            v[4 * q] = __builtin_amdgcn_ldexpf(v[4 * q], -up - back.x);
-            v[4 * q + 1] = __builtin_amdgcn_ldexpf(v[4 * q + 1], -up - back.y);
-            v[4 * q + 2] = __builtin_amdgcn_ldexpf(v[4 * q + 2], -up - back.z);
-            v[4 * q + 3] = __builtin_amdgcn_ldexpf(v[4 * q + 3], -up - back.w);
-        }
+        for (int r = 0; r < 16; ++r) v[r] = __builtin_amdgcn_ldexpf(v[r], up);
         // The block's rows of C or of the slice's part; what lies past the last row or column is neither read nor written.
         const int ld = a.part != nullptr ? a.N : a.p.ldc;
         float *C = a.part != nullptr ? a.part + static_cast<int64_t>(slice) * a.M * a.N : a.p.C;
@@ -606,10 +596,10 @@ __global__ __launch_bounds__(kThreads) void join_slices_kernel(const float *__re
 
 template <class S>
 Tile tile_args(const Halves &A, const Halves &B) {
-    CHECK_ERROR(A.terms != B.terms || B.rows >= 1 << 22, "Operands of %d and %d terms, %d columns.", A.terms, B.terms,
-                B.rows);
+    CHECK_ERROR(A.terms != B.terms || B.rows >= 1 << 22 || B.shift == nullptr,
+                "Operands of %d and %d terms, %d columns, or one shift for all of them.", A.terms, B.terms, B.rows);
     const int stages = A.term_blocks() / 2;
-    return {A.data, B.data, A.shift, B.shift, A.shift_all, B.shift_all, (A.rows + S::BM - 1) / S::BM,
+    return {A.data, B.data, A.shift, B.shift, A.shift_all, (A.rows + S::BM - 1) / S::BM,
             (B.rows + S::BN - 1) / S::BN, A.term_blocks(), stages, stages, 0};
 }
 
@@ -629,6 +619,7 @@ void run_logits(const Halves &A, const Halves &B, LogitsArgs l, hipStream_t s) {
 template <class S, Across ACROSS>
 void run_product(const Halves &A, const Halves &B, int kbs_across, const HalvesProduct &p, hipStream_t s) {
     constexpr int kSlots = 256 * (8 / S::kWaves);
+    CHECK_ERROR(A.shift != nullptr, "A first operand with a shift a row.");
     Tile t = tile_args<S>(A, B);
     t.kbs_across = kbs_across;
     const int tiles = t.tiles_m * t.tiles_n;
@@ -675,10 +666,9 @@ void launch_rows(const float *x, const float *weights, int rows, int terms, cons
     hipCheck(hipGetLastError());
 }
 
-void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, uint32_t *zero, int zeros,
+void launch_halves_rows(const float *x, const float *weights, const Halves &h, uint32_t *zero, int zeros,
                         hipStream_t s) {
-    launch_rows(x, weights, h.rows, h.terms,
-                {h.data, h.shift, h.row_blocks(), h.term_blocks(), negate, false, zero, zeros}, s);
+    launch_rows(x, weights, h.rows, h.terms, {h.data, h.shift, h.row_blocks(), h.term_blocks(), false, zero, zeros}, s);
 }
 
 void launch_halves_table(const float *x, const Halves &h, hipStream_t s) {
@@ -719,8 +709,8 @@ void launch_halves_product(const Halves &A, const Halves &B, const HalvesProduct
 
 // Of the operand that is read across only its size counts from here on, as it is in this product.
 void launch_product_across_a(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {
-    CHECK_ERROR(A.rows != B.terms || A.shift != nullptr, "Operands of %d and %d terms, or shifts by term.", A.rows, B.terms);
-    run_product<Small, Across::kA>({A.data, nullptr, A.shift_all, A.terms, A.rows}, B, A.term_blocks(), p, s);
+    CHECK_ERROR(A.rows != B.terms, "Operands of %d and %d terms.", A.rows, B.terms);
+    run_product<Small, Across::kA>({A.data, A.shift, A.shift_all, A.terms, A.rows}, B, A.term_blocks(), p, s);
 }
 
 void launch_product_across_b(const Halves &A, const Halves &B, const HalvesProduct &p, hipStream_t s) {

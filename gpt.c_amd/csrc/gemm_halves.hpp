@@ -56,17 +56,17 @@ __device__ __forceinline__ void halves_split(float x, float y, uint32_t &high, u
 // from adding up: the kernels subtract those sums.
 __device__ __forceinline__ bool halves_negated(int term) { return ((term >> 6) & 1) != 0; }
 
-// x (rows x terms without gaps; with weights, rows of weight 0 as zeros) into h.data and h.shift; negate: as a product's
-// first operand; `zeros` words at `zero` to 0.
-void launch_halves_rows(const float *x, const float *weights, const Halves &h, bool negate, uint32_t *zero, int zeros,
-                        hipStream_t s);
-// The same for other paddings, and (in_lines) another order of a block's terms: lane l of blocks 2 j and 2 j + 1 holds
-// 32 j + 16 (l / 32) + {0 .. 7} and {8 .. 15}, a step's 64 consecutive bytes for either half of the lanes.
+// x (rows x terms without gaps; with weights, rows of weight 0 as zeros) into h.data and h.shift, as a second operand;
+// `zeros` words at `zero` to 0.
+void launch_halves_rows(const float *x, const float *weights, const Halves &h, uint32_t *zero, int zeros, hipStream_t s);
+// The same for other paddings, or (in_lines) as the operand whose terms are negated, with another order of a block's terms:
+// lane l of blocks 2 j and 2 j + 1 holds 32 j + 16 (l / 32) + {0 .. 7} and {8 .. 15}, a step's 64 consecutive bytes for
+// either half of the lanes.
 struct HalvesRows {
     hu32x4 *data;
     int *shift;
     int row_blocks, term_blocks;  // of 32 and of 16
-    bool negate, in_lines;
+    bool in_lines;
     uint32_t *zero;  // the same launch sets `zeros` words here to 0
     int zeros;
 };
@@ -83,6 +83,7 @@ void launch_column_largest(const float *x, int ld, const float *weights, float d
 void launch_halves_columns(const float *x, int ld, const float *weights, float divisor, const Halves &h,
                            bool negate, const uint32_t *largest, hipStream_t s);
 
+// In products A has one shift, B one a row.
 // C (A.rows x B.rows, rows of ldc) = A B^T times row_factor[m] / divisor (+ C); rows of factor 0 are 0.
 struct HalvesProduct {
     float *C;

@@ -386,7 +386,7 @@ int few_row_blocks(int rows) {
 
 void launch_few_rows(const float *x, const float *weights, int rows, const FewRows &t, uint32_t *zero, int zeros,
                      hipStream_t s) {
-    launch_rows(x, weights, rows, t.terms, {t.data, t.shift, t.row_blocks, t.term_blocks(), true, true, zero, zeros}, s);
+    launch_rows(x, weights, rows, t.terms, {t.data, t.shift, t.row_blocks, t.term_blocks(), true, zero, zeros}, s);
 }
 
 int launch_few_logits(const float *W, int V, int C, const FewRows &x, const LogitsArgs &l, hipStream_t s) {

@@ -296,7 +296,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
     Scratch scratch;
     Halves x = scratch.halves(piece, h.C), xt{}, d{nullptr, nullptr, kShareShift, piece, h.V};
     uint32_t *largest_x = scratch.take<uint32_t>(h.C);  // magnitudes of x's columns
-    launch_halves_rows(h.x, h.weights, x, false, largest_x, h.C, s);
+    launch_halves_rows(h.x, h.weights, x, largest_x, h.C, s);
     // W is held by a shift for 64 rows each, as its rows are the terms of dx, whose product takes 64 of them at a time: to
     // 2^-40 of their largest value where it is below the 2^-17th of that, which counts for features of dx that small.  Laid
     // out by rows and, for dx, a second time by columns it would be held to 2^-40 of each row's and column's largest, and
@@ -318,7 +318,7 @@ void run_halves(const HeadLoss &h, hipStream_t s) {
         const float *xr = h.x + static_cast<int64_t>(r) * h.C;
         const float *weights = h.weights != nullptr ? h.weights + r : nullptr;
         x.rows = d.rows = xt.terms = n;
-        if (r > 0) launch_halves_rows(xr, weights, x, false, nullptr, 0, s);
+        if (r > 0) launch_halves_rows(xr, weights, x, nullptr, 0, s);
         const int part = launch_logits(
             W, x, {logits, stats, h.targets + r, target_logits, h.V, n, tokens / 32, n_padded}, s);
         launch_join_stats({stats, tokens / part, h.targets + r, target_logits, weights, shares, targets, h.losses + r,
