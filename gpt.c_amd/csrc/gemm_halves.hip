@@ -313,8 +313,8 @@ struct Shape {
 };
 
 // Loads of 4 KB from `base` on to LDS at `to` and behind, lane l's 16 bytes of a kilobyte from `first` there, of the last
-// two from `last`.  They write no register; the compiler does not count them, so its own waits wait for more than they
-// need.
+// two from `last`.  They write no register but m0, which nothing else of these kernels uses (it cannot be named as written:
+// the compiler keeps it to itself); the compiler does not count them, so its own waits wait for more than they need.
 __device__ __forceinline__ void load_block(const hu32x4 *base, uint32_t to, uint32_t first, uint32_t last) {
     asm volatile(
         "s_mov_b32 m0, %3\n\t"

@@ -31,8 +31,8 @@ __device__ __forceinline__ float across_halves(float x) {
     return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
 }
 
-// A kilobyte to LDS at `to` by loads that write no register (the compiler does not count them, so that its own
-// waits wait for more than they need).
+// A kilobyte to LDS at `to` by loads that write no register but m0, which nothing else of these kernels uses (the compiler
+// does not count them, so that its own waits wait for more than they need).
 __device__ __forceinline__ void load_kilobyte(const hu32x4 *from, uint32_t lane_at, uint32_t to) {
     asm volatile(
         "s_mov_b32 m0, %2\n\t"
