@@ -393,23 +393,33 @@ void run_few(const HeadLoss &h, hipStream_t s) {
 }
 
 // Whether W is read as it comes, again for every 128 rows and with a split of each float, instead of laid out first.
-// Rows, vocabulary x features: us as it comes / laid out.
-// With both gradients:
-//   100, 50257 x 768: 178 / 225       256, 50257 x 768: 328 / 316       384, 50257 x 768: 472 / 399
-//   256, 50257 x 256: 160 / 167       384, 50257 x 256: 208 / 200
-//   384, 50257 x 64: 138 / 142        512, 50257 x 64: 183 / 168
-//   384, 5003 x 1600: 152 / 152       768, 5003 x 1600: 233 / 199
-//   1024, 1000 x 768: 82 / 97         1536, 1000 x 768: 100 / 98
-//   512, 5003 x 100: 59 / 60          1024, 5003 x 100: 80 / 76         4095, 300 x 200: 65 / 68
-// The loss alone:
-//   100, 50257 x 768: 59 / 116        512, 50257 x 768: 183 / 194       768, 50257 x 768: 255 / 243
-//   768, 50257 x 64: 53 / 56          1536, 50257 x 64: 89 / 84
-//   768, 5003 x 1600: 71 / 80         1536, 5003 x 1600: 114 / 111
-//   2048, 5003 x 100: 31 / 33         4095, 5003 x 100: 45 / 46
+// A row of products costs more there (the split, W again), the call less (W's layout, wider launches).  us as it comes / laid
+// out, features x vocabulary: rows (taken from 900 sizes of 16 to 1600 x 128 to 130000, 96 to 4096 rows, all with both ways:
+// the rule's side is the quicker one or within 3 % of it for 871 of them, within 12 % for all, at a mean of 0.2 %).
+// With gradients, up to 240 rows and 1.6e9 / (V (C + 500)) more:
+//   768 x 50257   96: 179 / 227    200: 320 / 312    384: 476 / 405
+//   200 x 50257  200: 152 / 166    384: 206 / 202    512: 267 / 239
+//   16 x 50257   200: 104 / 122    384: 129 / 142    512: 168 / 168    640: 218 / 192
+//   768 x 5003   384: 84 / 89      512: 107 / 98     768: 128 / 114
+//   200 x 5003   384: 60 / 63      640: 74 / 76      768: 83 / 81      1024: 92 / 88
+//   768 x 1000   1024: 83 / 96     1280: 87 / 91     1536: 102 / 98
+//   200 x 1000   2048: 62 / 67     2944: 73 / 76     4096: 86 / 82
+// and 2^21 values of x, past which dx takes W again too often:
+//   768 x 300    1536: 75 / 79     2048: 80 / 82     2944: 105 / 91    4096: 134 / 99
+//   768 x 128    1536: 75 / 77     2048: 78 / 78     2944: 91 / 84
+// The loss alone, up to 512 rows and 5e9 / (V (C + 4)) more:
+//   768 x 50257  512: 184 / 195    640: 215 / 217    768: 269 / 248
+//   200 x 50257  512: 74 / 79      768: 100 / 98     1024: 127 / 119
+//   64 x 50257   1024: 64 / 68     1280: 74 / 73     2048: 112 / 107   2944: 156 / 138
+//   16 x 50257   2944: 112 / 126   4096: 149 / 164
+//   768 x 5003   1024: 55 / 55     1536: 66 / 66     2048: 90 / 82
+//   200 x 5003   2048: 40 / 40     2944: 49 / 48     4096: 60 / 62
+//   1600 x 1000  2048: 60 / 79     2944: 78 / 85     4096: 86 / 92
 bool few_rows(int rows, int V, int C, bool grad) {
-    const int64_t read = (rows + 127) / 128 * 128, room = 1400000000 / (V * (C + 100ll));
-    const int64_t some = room >= 8192 ? 4096 : std::min<int64_t>(900, room);
-    return rows <= 4096 && static_cast<int64_t>(rows) * C < 1 << 28 && read <= (grad ? 256 + some : 600 + room);
+    const int64_t read = (rows + 127) / 128 * 128, values = static_cast<int64_t>(rows) * C;
+    if (rows > 4096 || values >= 1 << 28) return false;  // offsets of 32 bits, and no size past 4096 that was measured
+    if (!grad) return read <= 512 + 5000000000 / (V * (C + 4ll));
+    return rows <= 128 || (read <= 240 + 1600000000 / (V * (C + 500ll)) && values <= 1 << 21);
 }
 
 }  // namespace
