@@ -121,8 +121,11 @@ constexpr int kRankRows = 12288;
 constexpr int kRankThreads = 512;
 constexpr int kRankPer = 32;  // rows a workgroup
 constexpr int kRankSlices = kRankThreads / kRankPer;
-// Enough to clear while the others rank; more only fill the queues that the ids have to pass (8192 rows of 768 on 50257:
-// the call 40 us with 512 waves, 47 with 384, 42 with 640, 51 with 2048).
+// Enough to clear while the others rank; more only fill the queues that the ids have to pass.  The call in us with 384, 448,
+// 512, 576, 1024 and 2048 waves:
+//   1100 rows of 768 on 50257: 37 33 32 35 33 34;  8192: 47 44 41 43 44 53;  12288: 56 56 57 58 61 72
+//   1100 rows of 1600 on 50257: 66 59 61 69 63 63;  12288: 97 91 88 95 95 95
+//   8192 rows of 512 on 130000: 63 58 56 61 60 60;  of 100 on 50257: 30 30 30 30 30 31;  of 768 on 5003: 38 in all
 constexpr int kRankClearWaves = 512;
 
 __global__ __launch_bounds__(kRankThreads) void rank_kernel(const float *__restrict__ ids, int n, int V,
