@@ -69,7 +69,9 @@ gpt2_t *GPT2(GPT2Config_t *config);
  * gptc_gpt2_loss_backward(gpt, x, targets, weights)
  *   The same, and every parameter's gradient is added to: forward, loss, and the
  *   two backwards of gpt.c's loop for an upstream gradient of ones.
- * Both read x, targets and weights, which stay the caller's.
+ * Both read x, targets and weights, which stay the caller's.  Both run forwards
+ * of their own: a forward that still waits for its backward is dropped, and that
+ * backward is refused.
  */
 tensor_t *gptc_gpt2_loss(gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights);
 tensor_t *gptc_gpt2_loss_backward(gpt2_t *gpt, const tensor_t *x, const tensor_t *targets, const tensor_t *weights);
