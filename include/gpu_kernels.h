@@ -261,12 +261,14 @@ void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tenso
  *   cross_entropy_*_cuda_kernel.  Values of x and W are held to 24 bits where
  *   they are not far smaller than the largest of their row or column of x or
  *   of 64 rows of W, else to 2^-40 of that largest one; softmax's shares below
- *   2^-16 to 2^-40.  W is taken to be finite: a value that is not
- *   makes the loss NaN.  A row of x that is not finite spoils its own loss and
- *   dx, output and dW.  V and C < 2^22, up to 10^9 rows.  Results may not
- *   overlap another tensor of the call.  Deterministic.  Takes scratch (the
- *   logits of up to 3328 rows of 50257 at a time, and W's copy): not under
- *   graph capture.
+ *   2^-16 to 2^-40 (of 1): a token that is nobody's target and whose shares are
+ *   all below 2^-28 has a row of dW of less than 16 bits.  Where such rows
+ *   count, Linear and cross_entropy_*_cuda_kernel keep them.  W is taken to be
+ *   finite: a value that is not makes the loss NaN.  A row of x that is not
+ *   finite spoils its own loss and dx, output and dW.  V and C < 2^22, up to
+ *   10^9 rows.  Results may not overlap another tensor of the call.
+ *   Deterministic.  Takes scratch (the logits of up to 3328 rows of 50257 at a
+ *   time, and W's copy): not under graph capture.
  *
  * gptc_embedding_forward_scaled_cuda(W, pos, ids, scale, output)
  *   output (ids..., C) = scale W[ids] (+ pos[i], i the id's place in ids' last

@@ -131,3 +131,23 @@ def test_values_near_the_ends_of_fp32(rt, R, shift):
     ref = head.Exact(*a)
     head.agree(head.Call(rt, *a, dx=shift < 0, dW=shift > 0), ref)
     head.agree(head.Call(rt, *a, dx=False, dW=False), ref)
+
+
+@pytest.mark.parametrize("R", [3, 100, MANY])
+def test_unlikely_tokens(rt, R):
+    """Shares are held to 2^-40: what a token's row of dW may be off by where all of them are far below 1, target or not."""
+    V = 40
+    a = -np.arange(V, dtype=np.float64)  # shares down to e^-39
+    rng = np.random.default_rng([14, R])
+    x = np.stack([np.ones(R), rng.integers(-2000, 2001, R)], 1).astype(np.float32)
+    W = np.stack([a, np.ones(V)], 1).astype(np.float32)
+    t = rng.integers(0, 3, R).astype(np.float32)
+    got = head.Call(rt, x, W, t)
+    _, dx, (dW, tol) = bounds(x, W, t, a)
+    close("dx", got.dx, *dx)
+    # The bound with 2^-40 of the share itself, and of x its own end 2^-40 below the column's largest.
+    p = np.exp(a) / np.exp(a).sum()
+    ax = np.abs(x).astype(np.float64)
+    rel = (2 * -a + 6 + 3 * V + 2 * (p * -a).sum() + 4 + min(R, 64) + R / 32) * U
+    tight = (2.0 ** -40 + rel * p)[3:, None] * ax.mean(0) + 2.0 ** -40 * p[3:, None] * ax.max(0)
+    close("dW of unlikely tokens", got.dW[3:], dW[3:], np.minimum(tight, tol[3:]))
