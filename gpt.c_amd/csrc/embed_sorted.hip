@@ -350,7 +350,7 @@ struct GatherArgs {
     int seqs, seq, positions;
 };
 
-// dP[t] (+)= the sequences' rows t, in their order; rows past the sequences' length: 0.
+// dP[t] (+)= the sequences' rows t, in a fixed order; rows past the sequences' length: 0.
 template <typename T>
 __device__ __forceinline__ void position_sum(const GatherArgs &a, int t, int col) {
     const int cols = a.C / (sizeof(T) / sizeof(float));
@@ -365,8 +365,8 @@ __device__ __forceinline__ void position_sum(const GatherArgs &a, int t, int col
             T v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = g[(b + k) * n];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum += v[k];
+            // Eight by themselves, in pairs: one chain of 64 sequences was off by twice as much.
+            sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
         for (; b < a.seqs; ++b) sum += g[b * n];
     }
