@@ -8,7 +8,7 @@
 // operand is small; its parts are formed once, in the order of the fragments.
 //
 // 768 features, 50257 tokens: 16 rows' logits 28 us (5.5 TB/s), where W comes from HBM 35
-// to 37; 100 rows' 53 to 58, d W 45 to 47.  With three bf16 parts, which need no scale but
+// to 37; 100 rows' 53 to 58, d W 44 to 47.  With three bf16 parts, which need no scale but
 // six products instead of three, those took 70 and 60.
 #include <algorithm>
 #include "gpu_kernels.h"

@@ -272,8 +272,8 @@ void cross_entropy_backward_cuda_kernel(const tensor_t *global_grad, const tenso
  *
  * gptc_embedding_forward_scaled_cuda(W, pos, ids, scale, output)
  *   output (ids..., C) = scale W[ids] (+ pos[i], i the id's place in ids' last
- *   dimension; pos (positions, C) or NULL).  Ids are floats truncated to int;
- *   those outside [0, V) give NaN rows.
+ *   dimension, so that every sequence begins at pos[0]; pos (positions, C) or
+ *   NULL).  Ids are floats truncated to int; those outside [0, V) give NaN rows.
  * gptc_embedding_backward_sorted_cuda(global_grad, ids, scale, dW, dpos, accumulate)
  *   Its gradients: dW (V, C) = scale sum of global_grad over the places of each
  *   id, dpos (positions, C), or NULL, = sum of global_grad over each place of
