@@ -151,3 +151,12 @@ def test_unlikely_tokens(rt, R):
     rel = (2 * -a + 6 + 3 * V + 2 * (p * -a).sum() + 4 + min(R, 64) + R / 32) * U
     tight = (2.0 ** -40 + rel * p)[3:, None] * ax.mean(0) + 2.0 ** -40 * p[3:, None] * ax.max(0)
     close("dW of unlikely tokens", got.dW[3:], dW[3:], np.minimum(tight, tol[3:]))
+
+
+@pytest.mark.parametrize("R", [5, 90, 300, MANY])
+@pytest.mark.parametrize("shift", [90, 100, 105])
+def test_scales_that_are_subnormal(rt, R, shift):
+    """Values of W of 2^-100 are held times 2^114, and come back by a factor below 2^-126; the results are ordinary."""
+    x, W, t, w = head.inputs(R, 500, 70, seed=15, weights=True)
+    a = np.ldexp(x, shift), np.ldexp(W, -shift), t, w
+    head.agree(head.Call(rt, *a), head.Exact(*a))
